@@ -98,6 +98,29 @@ SIGNATURES = {
                                            C.POINTER(View)]),
     "hpt_hip_add_layernorm": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.c_int32,
                                           C.POINTER(View), C.POINTER(View), C.c_double, C.POINTER(View)]),
+    "hpt_hip_rms_norm": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.c_int32, C.POINTER(View),
+                              C.c_double, C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_rms_norm_quant": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.c_int32,
+                              C.POINTER(View), C.c_double, C.c_int32, C.c_int64, C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View)]),
+    "hpt_hip_rms_norm_backward": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.POINTER(View),
+                              C.c_int32, C.POINTER(View), C.c_double, C.POINTER(View), C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_rms_norm_backward_workspace": (C.c_int32, [C.POINTER(View), C.c_int32, C.POINTER(C.c_size_t)]),
+    "hpt_hip_softmax_bias": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.c_double, C.POINTER(View), C.c_int32,
+                              C.c_int64, C.c_int64, C.c_int32, C.POINTER(View), C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_softmax_bias_workspace": (C.c_int32, [C.POINTER(View), C.POINTER(C.c_size_t)]),
+    "hpt_hip_softmax_bias_backward": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.c_double,
+                              C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_softmax_bias_backward_workspace": (C.c_int32, [C.POINTER(View), C.c_int64, C.POINTER(C.c_size_t)]),
+    "hpt_hip_token_logp": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_policy_loss": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View), C.POINTER(View), C.c_double, C.c_double, C.c_double,
+                              C.POINTER(View), C.POINTER(View), C.POINTER(View), C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_policy_loss_workspace": (C.c_int32, [C.POINTER(View), C.POINTER(C.c_size_t)]),
+    "hpt_hip_policy_loss_backward": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View), C.c_double, C.POINTER(View)]),
     "hpt_hip_contiguous": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View)]),
     "hpt_hip_contiguous_plan": (C.c_int32, [C.POINTER(View), C.POINTER(View), C.c_char_p, C.c_size_t]),
     "hpt_hip_binary_plan": (C.c_int32, [C.POINTER(View), C.POINTER(View), C.POINTER(View), C.c_char_p, C.c_size_t]),
@@ -130,6 +153,8 @@ def lib() -> C.CDLL:
 class _ThroughCtypes:
     """In the place of the native module where there is none: takes no call, so that every caller goes the long way, and frees through ctypes."""
     reduce = argreduce = softmax = layernorm = softmax_causal = staticmethod(lambda *_: None)
+    rms_norm = rms_norm_quant = rms_norm_backward = softmax_bias = softmax_bias_backward = staticmethod(lambda *_: None)
+    token_logp = policy_loss = policy_loss_backward = staticmethod(lambda *_: None)
 
     @staticmethod
     def free(device, ptr, nbytes, ordered):

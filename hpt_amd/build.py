@@ -48,6 +48,7 @@ def units():
             u.append((f"norm_interleaved_{k}.o", CSRC / "norm_interleaved.hip", [f"-DHPT_NORM_KIND={k}"]))
     for e in range(N_REDUCE_ENTRIES):
         u.append((f"reduce_op_{e}.o", CSRC / "reduce_op.hip", [f"-DHPT_REDUCE_ENTRY={e}"]))
+    u += [("rms_norm.o", CSRC / "rms_norm.hip", []), ("softmax_bias.o", CSRC / "softmax_bias.hip", []), ("policy_loss.o", CSRC / "policy_loss.hip", [])]
     u += [("layout.o", CSRC / "layout.cpp", ["-x", "hip"]), ("api.o", CSRC / "api.hip", []),
           ("elementwise.o", CSRC / "elementwise.hip", [])]
     if (CSRC / "transpose_norm.hip").exists():

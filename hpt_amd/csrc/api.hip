@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <list>
@@ -12,6 +13,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "block_entry.hpp"
 #include "common.hpp"
 #include "elementwise_entry.hpp"
 #include "norm_entry.hpp"
@@ -604,6 +606,236 @@ static void launch_norm(int dev, hipStream_t st, NormLaunchFn fn, NormCall& c, c
     }
 }
 
+// ---- operators around a transformer's blocks ---------------------------------------
+
+constexpr int64_t kMostCols = (int64_t)1 << 29;  // elements of a row that its kernels index with 32 bits
+
+static void check_block_dtype(const hpt_view* v, const char* name) {
+    if (v->dtype != HPT_F16 && v->dtype != HPT_BF16 && v->dtype != HPT_F32)
+        fail(HPT_ERR_DTYPE, "%s: dtype is %s, expected f16, bf16 or f32", name, dtype_name(v->dtype));
+}
+
+// An operand that is contiguous, of one dtype and one size. `shape_of`: of that shape, too.
+static void check_operand(const hpt_view* v, int dtype, int64_t count, const hpt_view* shape_of, const char* name) {
+    check_view(v, name, true);
+    if (v->dtype != dtype) fail(HPT_ERR_DTYPE, "%s: dtype is %s, expected %s", name, dtype_name(v->dtype), dtype_name(dtype));
+    if (!view_contiguous(v)) fail(HPT_ERR_SHAPE, "%s: must be contiguous", name);
+    bool same = !shape_of || v->ndim == shape_of->ndim;
+    for (int i = 0; same && shape_of && i < v->ndim; ++i) same = v->shape[i] == shape_of->shape[i];
+    if (!same) fail(HPT_ERR_SHAPE, "%s: shape differs from the input's", name);
+    if (view_size(v) != count)
+        fail(HPT_ERR_SHAPE, "%s: Size mismatch: expected %lld, got %lld", name, (long long)count, (long long)view_size(v));
+}
+
+// The rows of a view whose last `tail` dims are one run of neighbouring elements: their number and length, and where they start.
+struct RowsOf {
+    int64_t rows = 1, cols = 1;
+    Dims kept;
+};
+static RowsOf rows_of(const hpt_view* v, int tail, const char* name) {
+    RowsOf r;
+    const int lead = v->ndim - tail;
+    for (int i = 0; i < lead; ++i) r.rows *= v->shape[i];
+    for (int i = lead; i < v->ndim; ++i) r.cols *= v->shape[i];
+    if (r.rows == 0 || r.cols == 0) return r;
+    int64_t expect = 1;
+    for (int i = v->ndim - 1; i >= lead; --i) {
+        if (v->shape[i] == 1) continue;
+        if (v->strides[i] != expect) fail(HPT_ERR_SHAPE, "%s: the elements of a row must be neighbours in memory (contiguous() makes them so)", name);
+        expect *= v->shape[i];
+    }
+    if (r.cols >= kMostCols) fail(HPT_ERR_SHAPE, "%s: rows of %lld elements, fewer than %lld expected", name, (long long)r.cols, (long long)kMostCols);
+    Dims& d = r.kept;
+    for (int i = 0; i < lead; ++i) {
+        if (v->shape[i] == 1) continue;
+        if (d.n && d.stride[d.n - 1] == v->strides[i] * v->shape[i]) {
+            d.size[d.n - 1] *= v->shape[i];
+            d.stride[d.n - 1] = v->strides[i];
+            continue;
+        }
+        if (d.n == kMaxDims) fail(HPT_ERR_SHAPE, "%s: more than %d separate dims of rows", name, kMaxDims);
+        d.size[d.n] = v->shape[i];
+        d.stride[d.n++] = v->strides[i];
+    }
+    return r;
+}
+
+// What a call writes shares no memory with anything else of the call, but for operands that a result may take the very place of.
+struct Overlaps {
+    struct Of {
+        const hpt_view* v;
+        const char* name;
+    };
+    const char* what;
+    Of in[12];
+    int n_in = 0;
+    void reads(const hpt_view* v, const char* name) {
+        if (v) in[n_in++] = {v, name};
+    }
+    // `may`: operands (two at most) whose place `out` may take
+    void writes(const hpt_view* out, const hpt_view* may1 = nullptr, const hpt_view* may2 = nullptr, const hpt_view* may3 = nullptr) {
+        if (!out) return;
+        for (int i = 0; i < n_in; ++i) check_alias(in[i].v, out, in[i].v == may1 || in[i].v == may2 || in[i].v == may3, what, in[i].name);
+        in[n_in++] = {out, "another result"};
+    }
+};
+
+// Scratch of `bytes` for the launches of `go`: the caller's workspace, or the stream's own buffer, held from lookup to launch. A captured call
+// outlives that buffer: it takes the form without scratch (`go(nullptr)`) where there is one, and is refused otherwise.
+template <class F> static void with_workspace(int dev, hipStream_t st, const hpt_view* ws, size_t bytes, bool without, const char* what, F&& go) {
+    if (!bytes) return go(nullptr);
+    if (ws) {
+        const size_t have = (size_t)view_size(ws) * dtype_size(ws->dtype);
+        if (have < bytes) fail(HPT_ERR_MEMORY, "%s: the workspace holds %zu bytes, %zu are needed", what, have, bytes);
+        if ((uintptr_t)ws->data % 16) fail(HPT_ERR_PARAM, "%s: the workspace must be aligned to 16 bytes", what);
+        return go(ws->data);
+    }
+    if (capturing(st)) {
+        if (without) return go(nullptr);
+        fail(HPT_ERR_MEMORY, "%s: under capture a workspace of %zu bytes must be given", what, bytes);
+    }
+    StreamScratch& s = scratch_entry(dev, st);
+    std::lock_guard<std::mutex> g(s.mu);
+    void* p = nullptr;
+    try {
+        p = scratch_reserve(dev, s, bytes);
+    } catch (const Error&) {
+        if (!without) throw;
+    }
+    go(p);
+}
+static void check_workspace(const hpt_view* ws, const char* name) {
+    if (!ws) return;
+    check_view(ws, name, true);
+    if (!view_contiguous(ws)) fail(HPT_ERR_SHAPE, "%s: must be contiguous", name);
+}
+
+static float check_eps(double eps) {
+    const float e = (float)eps;
+    if (!(e > 0.0f) || e > 3.4e38f) fail(HPT_ERR_PARAM, "rms_norm: eps must be a positive number");
+    return e;
+}
+
+static void run_rms_norm(int dev, void* stream, const hpt_view* in, const hpt_view* residual, int n_norm_dims, const hpt_view* gamma, double eps,
+                         int quant, int64_t group, hpt_view* sum, hpt_view* out, hpt_view* scale) {
+    check_view(in, "rms_norm input", true);
+    check_block_dtype(in, "rms_norm input");
+    if (n_norm_dims <= 0 || n_norm_dims > in->ndim) fail(HPT_ERR_SHAPE, "rms_norm: %d normalized dims but input has %d", n_norm_dims, in->ndim);
+    const RowsOf r = rows_of(in, n_norm_dims, "rms_norm input");
+    const int64_t count = view_size(in);
+    RmsArgs a{};
+    a.eps = check_eps(eps);
+    if (residual) check_operand(residual, in->dtype, count, in, "rms_norm residual");
+    if (gamma) check_operand(gamma, in->dtype, r.cols, nullptr, "rms_norm gamma");
+    if (sum && !residual) fail(HPT_ERR_PARAM, "rms_norm: a sum is asked for, but there is no residual");
+    if (sum) check_out(sum, in->dtype, count, "rms_norm sum");
+    a.group = (int)r.cols;
+    if (quant == QUANT_NONE) {
+        check_out(out, in->dtype, count, "rms_norm output");
+    } else {
+        if (quant != QUANT_I8 && quant != QUANT_E4M3) fail(HPT_ERR_PARAM, "rms_norm_quant: invalid format %d", quant);
+        check_out(out, quant == QUANT_I8 ? HPT_I8 : HPT_U8, count, "rms_norm_quant output");
+        if (group < 0 || group > r.cols || (group > 0 && r.cols % group)) fail(HPT_ERR_SHAPE, "rms_norm_quant: groups of %lld do not divide rows of %lld", (long long)group, (long long)r.cols);
+        if (group > 0) a.group = (int)group;
+        check_out(scale, HPT_F32, r.cols ? r.rows * (r.cols / a.group) : view_size(scale), "rms_norm_quant scale");
+    }
+    Overlaps o{quant == QUANT_NONE ? "rms_norm" : "rms_norm_quant"};
+    o.reads(in, "the input");
+    o.reads(residual, "the residual");
+    o.reads(gamma, "gamma");
+    o.writes(sum, in, residual);
+    o.writes(out, in, residual);
+    o.writes(scale);
+    if (count == 0) return;
+    a.x = in->data;
+    a.kept = r.kept;
+    a.res = residual ? residual->data : nullptr;
+    a.gamma = gamma ? gamma->data : nullptr;
+    a.sum = sum ? sum->data : nullptr;
+    a.out = out->data;
+    a.scale = scale ? (float*)scale->data : nullptr;
+    a.rows = r.rows;
+    a.cols = (int)r.cols;
+    use_device(dev);
+    launch_rms_norm(in->dtype, quant, a, (hipStream_t)stream);
+    check_launch("rms_norm");
+}
+
+static RowsOf check_rms_backward(const hpt_view* in, int n_norm_dims) {
+    check_view(in, "rms_norm_backward input", true);
+    check_block_dtype(in, "rms_norm_backward input");
+    if (n_norm_dims <= 0 || n_norm_dims > in->ndim) fail(HPT_ERR_SHAPE, "rms_norm_backward: %d normalized dims but input has %d", n_norm_dims, in->ndim);
+    return rows_of(in, n_norm_dims, "rms_norm_backward input");
+}
+static size_t rms_backward_bytes(const hpt_view* in, const RowsOf& r) {
+    return r.rows && r.cols ? (size_t)(rms_grad_partials(in->dtype, r.rows, r.cols) * r.cols) * sizeof(float) : 0;
+}
+
+// The scores or probabilities of attention: [..., heads, queries, keys].
+struct Scores {
+    int64_t batch = 1, heads, queries, keys, rows;
+};
+static Scores scores_of(const hpt_view* v, const char* name) {
+    check_view(v, name, true);
+    check_block_dtype(v, name);
+    if (v->ndim < 3) fail(HPT_ERR_SHAPE, "%s: needs at least 3 dims (heads x queries x keys)", name);
+    Scores s;
+    for (int i = 0; i + 3 < v->ndim; ++i) s.batch *= v->shape[i];
+    s.heads = v->shape[v->ndim - 3];
+    s.queries = v->shape[v->ndim - 2];
+    s.keys = v->shape[v->ndim - 1];
+    s.rows = s.batch * s.heads * s.queries;
+    return s;
+}
+static float check_bias_scale(double scale, int64_t query_offset, const char* what) {
+    if (!(std::abs((float)scale) <= 3.4028234e38f)) fail(HPT_ERR_PARAM, "%s: scale must be a finite number", what);
+    if (query_offset < -((int64_t)1 << 40) || query_offset > ((int64_t)1 << 40)) fail(HPT_ERR_PARAM, "%s: query_offset %lld beyond 2^40", what, (long long)query_offset);
+    return (float)scale;
+}
+static void check_lengths(const hpt_view* lengths, const Scores& s, const char* name) {
+    if (!lengths) return;
+    check_view(lengths, name, true);
+    if (lengths->dtype != HPT_I32 && lengths->dtype != HPT_I64) fail(HPT_ERR_DTYPE, "%s: dtype is %s, expected i32 or i64", name, dtype_name(lengths->dtype));
+    check_operand(lengths, lengths->dtype, s.batch, nullptr, name);
+}
+
+// Logits [..., vocabulary] and a token for each row.
+static RowsOf logits_of(const hpt_view* logits, const char* name) {
+    check_view(logits, name, true);
+    check_block_dtype(logits, name);
+    if (logits->ndim < 1) fail(HPT_ERR_SHAPE, "%s: input has no dimensions", name);
+    const RowsOf r = rows_of(logits, 1, name);
+    if (r.cols == 0) fail(HPT_ERR_SHAPE, "%s: a vocabulary of no tokens", name);
+    return r;
+}
+static void check_tokens(const hpt_view* token, int64_t rows, const char* name) {
+    check_view(token, name, true);
+    if (token->dtype != HPT_I32 && token->dtype != HPT_I64) fail(HPT_ERR_DTYPE, "%s: dtype is %s, expected i32 or i64", name, dtype_name(token->dtype));
+    check_operand(token, token->dtype, rows, nullptr, name);
+}
+// Each token's loss (policy loss only), then the parts of split rows.
+static size_t policy_bytes(const hpt_view* logits, const RowsOf& r, bool losses) {
+    const int split = policy_split(logits->dtype, r.rows, r.cols);
+    return sizeof(double) * (size_t)((losses ? r.rows + (r.rows & 1) : 0) + (split > 1 ? 2 * r.rows * split : 0));
+}
+static void run_policy(int dev, void* stream, const hpt_view* logits, const RowsOf& r, PolicyArgs& a, const hpt_view* token, const hpt_view* workspace, bool losses, const char* what) {
+    a.x = logits->data;
+    a.kept = r.kept;
+    a.token = token->data;
+    a.token64 = token->dtype == HPT_I64;
+    a.rows = r.rows;
+    a.cols = (int)r.cols;
+    use_device(dev);
+    hipStream_t st = (hipStream_t)stream;
+    with_workspace(dev, st, workspace, policy_bytes(logits, r, losses), !losses, what, [&](void* p) {
+        a.split = p ? policy_split(logits->dtype, r.rows, r.cols) : 1;
+        a.each = losses ? (double*)p : nullptr;
+        a.partial = (double*)p + (losses ? r.rows + (r.rows & 1) : 0);
+        launch_policy_loss(logits->dtype, a, st);
+        check_launch(what);
+    });
+}
+
 }  // namespace hpt
 
 using namespace hpt;
@@ -1061,6 +1293,324 @@ int32_t hpt_hip_binary_plan(const hpt_view* lhs, const hpt_view* rhs, const hpt_
     return guarded([&] {
         if (!buf || !buflen) fail(HPT_ERR_PARAM, "binary_plan: no buffer");
         snprintf(buf, buflen, "%s", describe(prepare_binary(lhs, rhs, out)).c_str());
+    });
+}
+
+// ---- operators around a transformer's blocks ------------------------------------------
+
+int32_t hpt_hip_rms_norm(int32_t dev, void* stream, const hpt_view* in, const hpt_view* residual, int32_t n_norm_dims,
+                         const hpt_view* gamma, double eps, hpt_view* sum, hpt_view* out) {
+    return guarded([&] { run_rms_norm(dev, stream, in, residual, n_norm_dims, gamma, eps, QUANT_NONE, 0, sum, out, nullptr); });
+}
+
+int32_t hpt_hip_rms_norm_quant(int32_t dev, void* stream, const hpt_view* in, const hpt_view* residual, int32_t n_norm_dims,
+                               const hpt_view* gamma, double eps, int32_t format, int64_t group, hpt_view* sum, hpt_view* out,
+                               hpt_view* scale) {
+    return guarded([&] {
+        if (format != HPT_QUANT_I8 && format != HPT_QUANT_E4M3) fail(HPT_ERR_PARAM, "rms_norm_quant: invalid format %d", format);
+        if (!scale) fail(HPT_ERR_PARAM, "rms_norm_quant scale: view is null");
+        run_rms_norm(dev, stream, in, residual, n_norm_dims, gamma, eps, format == HPT_QUANT_I8 ? QUANT_I8 : QUANT_E4M3, group, sum, out, scale);
+    });
+}
+
+int32_t hpt_hip_rms_norm_backward_workspace(const hpt_view* in, int32_t n_norm_dims, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "rms_norm_backward_workspace: null output");
+        *bytes = rms_backward_bytes(in, check_rms_backward(in, n_norm_dims));
+    });
+}
+
+int32_t hpt_hip_rms_norm_backward(int32_t dev, void* stream, const hpt_view* in, const hpt_view* grad, const hpt_view* grad_sum,
+                                  int32_t n_norm_dims, const hpt_view* gamma, double eps, const hpt_view* workspace, hpt_view* grad_in,
+                                  hpt_view* grad_gamma) {
+    return guarded([&] {
+        const RowsOf r = check_rms_backward(in, n_norm_dims);
+        const int64_t count = view_size(in);
+        RmsGradArgs a{};
+        a.eps = check_eps(eps);
+        check_operand(grad, in->dtype, count, in, "rms_norm_backward grad");
+        if (grad_sum) check_operand(grad_sum, in->dtype, count, in, "rms_norm_backward grad_sum");
+        if (gamma) check_operand(gamma, in->dtype, r.cols, nullptr, "rms_norm_backward gamma");
+        check_workspace(workspace, "rms_norm_backward workspace");
+        check_out(grad_in, in->dtype, count, "rms_norm_backward grad_in");
+        if (grad_gamma) check_out(grad_gamma, HPT_F32, r.cols, "rms_norm_backward grad_gamma");
+        Overlaps o{"rms_norm_backward"};
+        o.reads(in, "the input");
+        o.reads(grad, "grad");
+        o.reads(grad_sum, "grad_sum");
+        o.reads(gamma, "gamma");
+        o.writes(grad_in, in, grad, grad_sum);
+        o.writes(grad_gamma);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        if (r.cols == 0 || (count == 0 && !grad_gamma)) return;
+        a.x = in->data;
+        a.kept = r.kept;
+        a.gy = grad->data;
+        a.gsum = grad_sum ? grad_sum->data : nullptr;
+        a.gamma = gamma ? gamma->data : nullptr;
+        a.gx = grad_in->data;
+        a.ggamma = grad_gamma ? (float*)grad_gamma->data : nullptr;
+        a.rows = r.rows;
+        a.cols = (int)r.cols;
+        use_device(dev);
+        hipStream_t st = (hipStream_t)stream;
+        with_workspace(dev, st, workspace, grad_gamma ? rms_backward_bytes(in, r) : 0, false, "rms_norm_backward", [&](void* p) {
+            a.partial = (float*)p;
+            launch_rms_norm_backward(in->dtype, a, st);
+            check_launch("rms_norm_backward");
+        });
+    });
+}
+
+int32_t hpt_hip_softmax_bias_workspace(const hpt_view* in, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "softmax_bias_workspace: null output");
+        const Scores s = scores_of(in, "softmax_bias input");
+        const int split = bias_split(in->dtype, s.rows, s.keys);
+        *bytes = split > 1 ? (size_t)(s.rows * split) * 2 * sizeof(float) : 0;
+    });
+}
+
+int32_t hpt_hip_softmax_bias(int32_t dev, void* stream, const hpt_view* in, double scale, const hpt_view* table, int32_t bidirectional,
+                             int64_t max_distance, int64_t query_offset, int32_t causal, const hpt_view* lengths,
+                             const hpt_view* workspace, hpt_view* out) {
+    return guarded([&] {
+        const Scores s = scores_of(in, "softmax_bias input");
+        const RowsOf r = rows_of(in, 1, "softmax_bias input");
+        BiasArgs a{};
+        a.scale = check_bias_scale(scale, query_offset, "softmax_bias");
+        check_view(table, "softmax_bias table", true);
+        if (table->dtype != in->dtype) fail(HPT_ERR_DTYPE, "softmax_bias table: dtype is %s, expected %s", dtype_name(table->dtype), dtype_name(in->dtype));
+        if (table->ndim != 2 || table->shape[1] != s.heads) fail(HPT_ERR_SHAPE, "softmax_bias table: must be buckets x %lld heads", (long long)s.heads);
+        a.buckets = make_buckets(table->shape[0], bidirectional != 0, max_distance);
+        check_lengths(lengths, s, "softmax_bias lengths");
+        check_workspace(workspace, "softmax_bias workspace");
+        check_out(out, in->dtype, view_size(in), "softmax_bias output");
+        Overlaps o{"softmax_bias"};
+        o.reads(in, "the input");
+        o.reads(table, "the table");
+        o.reads(lengths, "the lengths");
+        o.writes(out, in);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        if (view_size(in) == 0) return;
+        a.x = in->data;
+        a.kept = r.kept;
+        a.table = table->data;
+        a.table_bucket = table->strides[0];
+        a.table_head = table->strides[1];
+        a.out = out->data;
+        a.lengths = lengths ? lengths->data : nullptr;
+        a.lengths64 = lengths && lengths->dtype == HPT_I64;
+        a.causal = causal != 0;
+        a.heads = s.heads;
+        a.queries = s.queries;
+        a.rows = s.rows;
+        a.keys = (int)s.keys;
+        a.offset = query_offset;
+        use_device(dev);
+        hipStream_t st = (hipStream_t)stream;
+        const int split = bias_split(in->dtype, s.rows, s.keys);
+        with_workspace(dev, st, workspace, split > 1 ? (size_t)(s.rows * split) * 2 * sizeof(float) : 0, true, "softmax_bias", [&](void* p) {
+            a.partial = (float*)p;
+            a.split = p ? split : 1;
+            launch_softmax_bias(in->dtype, a, st);
+            check_launch("softmax_bias");
+        });
+    });
+}
+
+int32_t hpt_hip_softmax_bias_backward_workspace(const hpt_view* probs, int64_t buckets, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "softmax_bias_backward_workspace: null output");
+        const Scores s = scores_of(probs, "softmax_bias_backward probs");
+        if (buckets < 2 || buckets > kMostBuckets) fail(HPT_ERR_PARAM, "position bias: %lld buckets, outside 2..%d", (long long)buckets, kMostBuckets);
+        int per_item = 0;
+        *bytes = s.rows * s.keys ? (size_t)(bias_grad_items(probs->dtype, s.batch * s.heads, s.queries, s.keys, &per_item) * buckets) * sizeof(float) : 0;
+    });
+}
+
+int32_t hpt_hip_softmax_bias_backward(int32_t dev, void* stream, const hpt_view* probs, const hpt_view* grad, double scale,
+                                      int32_t bidirectional, int64_t max_distance, int64_t query_offset, int32_t causal,
+                                      const hpt_view* lengths, const hpt_view* workspace, hpt_view* grad_in, hpt_view* grad_table) {
+    return guarded([&] {
+        const Scores s = scores_of(probs, "softmax_bias_backward probs");
+        const int64_t count = view_size(probs);
+        if (s.keys >= kMostCols) fail(HPT_ERR_SHAPE, "softmax_bias_backward probs: rows of %lld elements, fewer than %lld expected", (long long)s.keys, (long long)kMostCols);
+        BiasGradArgs a{};
+        a.scale = check_bias_scale(scale, query_offset, "softmax_bias_backward");
+        check_operand(probs, probs->dtype, count, nullptr, "softmax_bias_backward probs");
+        check_operand(grad, probs->dtype, count, probs, "softmax_bias_backward grad");
+        check_lengths(lengths, s, "softmax_bias_backward lengths");
+        check_workspace(workspace, "softmax_bias_backward workspace");
+        check_out(grad_in, probs->dtype, count, "softmax_bias_backward grad_in");
+        int64_t buckets = 2;
+        if (grad_table) {
+            check_view(grad_table, "softmax_bias_backward grad_table", true);
+            if (grad_table->ndim != 2 || grad_table->shape[1] != s.heads)
+                fail(HPT_ERR_SHAPE, "softmax_bias_backward grad_table: must be buckets x %lld heads", (long long)s.heads);
+            buckets = grad_table->shape[0];
+            check_out(grad_table, HPT_F32, buckets * s.heads, "softmax_bias_backward grad_table");
+        }
+        // (without a table's gradient any buckets do: none of the results depends on them)
+        a.buckets = grad_table ? make_buckets(buckets, bidirectional != 0, max_distance) : make_buckets(2, false, 2);
+        Overlaps o{"softmax_bias_backward"};
+        o.reads(probs, "the probabilities");
+        o.reads(grad, "grad");
+        o.reads(lengths, "the lengths");
+        o.writes(grad_in, probs, grad);
+        o.writes(grad_table);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        if (s.heads == 0 || (count == 0 && !grad_table)) return;
+        a.p = probs->data;
+        a.g = grad->data;
+        a.out = grad_in->data;
+        a.table_grad = grad_table ? (float*)grad_table->data : nullptr;
+        a.lengths = lengths ? lengths->data : nullptr;
+        a.lengths64 = lengths && lengths->dtype == HPT_I64;
+        a.causal = causal != 0;
+        a.heads = s.heads;
+        a.queries = s.queries;
+        a.rows = count ? s.rows : 0;
+        a.keys = (int)s.keys;
+        a.offset = query_offset;
+        size_t bytes = 0;
+        int per_item = 0;
+        if (count && grad_table) bytes = (size_t)(bias_grad_items(probs->dtype, s.batch * s.heads, s.queries, s.keys, &per_item) * buckets) * sizeof(float);
+        use_device(dev);
+        hipStream_t st = (hipStream_t)stream;
+        with_workspace(dev, st, workspace, bytes, false, "softmax_bias_backward", [&](void* p) {
+            a.partial = (float*)p;
+            launch_softmax_bias_backward(probs->dtype, a, st);
+            check_launch("softmax_bias_backward");
+        });
+    });
+}
+
+int32_t hpt_hip_policy_loss_workspace(const hpt_view* logits, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "policy_loss_workspace: null output");
+        *bytes = policy_bytes(logits, logits_of(logits, "policy_loss logits"), true);
+    });
+}
+
+int32_t hpt_hip_token_logp(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* workspace,
+                           hpt_view* logp, hpt_view* lse) {
+    return guarded([&] {
+        const RowsOf r = logits_of(logits, "token_logp logits");
+        check_tokens(token, r.rows, "token_logp token");
+        check_workspace(workspace, "token_logp workspace");
+        check_out(logp, HPT_F32, r.rows, "token_logp logp");
+        check_out(lse, HPT_F32, r.rows, "token_logp lse");
+        Overlaps o{"token_logp"};
+        o.reads(logits, "the logits");
+        o.reads(token, "the tokens");
+        o.writes(logp);
+        o.writes(lse);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        if (r.rows == 0) return;
+        PolicyArgs a{};
+        a.logp = (float*)logp->data;
+        a.lse = (float*)lse->data;
+        run_policy(dev, stream, logits, r, a, token, workspace, false, "token_logp");
+    });
+}
+
+int32_t hpt_hip_policy_loss(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* old_logp,
+                            const hpt_view* advantage, const hpt_view* reference, const hpt_view* mask, double clip_low,
+                            double clip_high, double kl_weight, const hpt_view* workspace, hpt_view* loss, hpt_view* logp,
+                            hpt_view* lse, hpt_view* weight) {
+    return guarded([&] {
+        const RowsOf r = logits_of(logits, "policy_loss logits");
+        check_tokens(token, r.rows, "policy_loss token");
+        check_operand(old_logp, HPT_F32, r.rows, nullptr, "policy_loss old_logp");
+        check_operand(advantage, HPT_F32, r.rows, nullptr, "policy_loss advantage");
+        if (reference) check_operand(reference, HPT_F32, r.rows, nullptr, "policy_loss reference");
+        if (mask) {
+            check_view(mask, "policy_loss mask", true);
+            if (mask->dtype != HPT_F32 && mask->dtype != HPT_BOOL) fail(HPT_ERR_DTYPE, "policy_loss mask: dtype is %s, expected f32 or bool", dtype_name(mask->dtype));
+            check_operand(mask, mask->dtype, r.rows, nullptr, "policy_loss mask");
+        }
+        if (!(clip_low >= 0 && clip_low <= 1) || !(clip_high >= 0 && clip_high <= 1e30)) fail(HPT_ERR_PARAM, "policy_loss: clip_low must be in 0..1 and clip_high not negative");
+        if (!(std::abs(kl_weight) <= 1e30)) fail(HPT_ERR_PARAM, "policy_loss: kl_weight must be a finite number");
+        if (kl_weight != 0 && !reference) fail(HPT_ERR_PARAM, "policy_loss: a KL term needs the reference's log-probabilities");
+        check_workspace(workspace, "policy_loss workspace");
+        check_out(loss, HPT_F32, 1, "policy_loss loss");
+        check_out(logp, HPT_F32, r.rows, "policy_loss logp");
+        check_out(lse, HPT_F32, r.rows, "policy_loss lse");
+        check_out(weight, HPT_F32, r.rows, "policy_loss weight");
+        Overlaps o{"policy_loss"};
+        o.reads(logits, "the logits");
+        o.reads(token, "the tokens");
+        o.reads(old_logp, "old_logp");
+        o.reads(advantage, "the advantages");
+        o.reads(reference, "the reference");
+        o.reads(mask, "the mask");
+        o.writes(loss);
+        o.writes(logp);
+        o.writes(lse);
+        o.writes(weight);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        PolicyArgs a{};
+        a.old_logp = (const float*)old_logp->data;
+        a.advantage = (const float*)advantage->data;
+        a.reference = reference && kl_weight != 0 ? (const float*)reference->data : nullptr;
+        a.mask = mask ? mask->data : nullptr;
+        a.mask_bool = mask && mask->dtype == HPT_BOOL;
+        a.clip_low = clip_low;
+        a.clip_high = clip_high;
+        a.kl_weight = kl_weight;
+        a.loss = (float*)loss->data;
+        a.logp = (float*)logp->data;
+        a.lse = (float*)lse->data;
+        a.weight = (float*)weight->data;
+        run_policy(dev, stream, logits, r, a, token, workspace, true, "policy_loss");
+    });
+}
+
+int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* lse,
+                                     const hpt_view* weight, double grad, hpt_view* grad_logits) {
+    return guarded([&] {
+        const RowsOf r = logits_of(logits, "policy_loss_backward logits");
+        check_tokens(token, r.rows, "policy_loss_backward token");
+        check_operand(lse, HPT_F32, r.rows, nullptr, "policy_loss_backward lse");
+        check_operand(weight, HPT_F32, r.rows, nullptr, "policy_loss_backward weight");
+        check_out(grad_logits, logits->dtype, view_size(logits), "policy_loss_backward grad_logits");
+        Overlaps o{"policy_loss_backward"};
+        o.reads(logits, "the logits");
+        o.reads(token, "the tokens");
+        o.reads(lse, "lse");
+        o.reads(weight, "the weights");
+        o.writes(grad_logits, logits);
+        if (r.rows == 0) return;
+        PolicyGradArgs a{};
+        a.x = logits->data;
+        a.kept = r.kept;
+        a.token = token->data;
+        a.token64 = token->dtype == HPT_I64;
+        a.lse = (const float*)lse->data;
+        a.weight = (const float*)weight->data;
+        a.upstream = (float)grad;
+        a.out = grad_logits->data;
+        a.rows = r.rows;
+        a.cols = (int)r.cols;
+        use_device(dev);
+        launch_policy_loss_backward(logits->dtype, a, (hipStream_t)stream);
+        check_launch("policy_loss_backward");
     });
 }
 

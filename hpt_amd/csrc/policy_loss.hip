@@ -1,0 +1,246 @@
+// The clipped policy loss with a KL term over rows of logits x, and the gradient of the logits.
+//
+// For a row with token t:   logp = x[t] - lse,  lse = log sum exp x,  ratio = exp(logp - old),
+//   loss  = -min(ratio A, clip(ratio, 1 - low, 1 + high) A) + kl (exp(ref - logp) - (ref - logp) - 1),
+// averaged over the rows with the mask as weights; rows whose mask is 0 are not read. d loss / d logp is the row's `weight` (the free side of
+// the minimum where the two are equal), and the logits' gradient weight * (1[v = t] - exp(x - lse)).
+//
+// Bound by memory: the forward pass reads the logits once, keeping a running maximum and the sum of exponentials below it; the
+// backward pass reads them once and writes the gradient once. A token's own few values are computed in f64: next to the borders
+// of the clipping the gradient jumps, and the logits are all that is large.
+#include <algorithm>
+
+#include "block_rows.hpp"
+
+namespace hpt {
+
+namespace {
+
+template <class T> __device__ __forceinline__ void meet(float& m, double& s, float m2, double s2) {
+    const float n = fmaxf(m, m2);
+    // (nothing seen is (-inf, 0); a NaN is in its sum)
+    s = s * (double)(m == n ? 1.0f : exp_row<T>(m - n)) + s2 * (double)(m2 == n ? 1.0f : exp_row<T>(m2 - n));
+    m = n;
+}
+
+__device__ __forceinline__ int64_t token_of(const void* token, int is64, int64_t row) {
+    return is64 ? ((const int64_t*)token)[row] : (int64_t)((const int32_t*)token)[row];
+}
+__device__ __forceinline__ float mask_of(const PolicyArgs& a, int64_t row) {
+    if (!a.mask) return 1.0f;
+    return a.mask_bool ? (((const uint8_t*)a.mask)[row] ? 1.0f : 0.0f) : ((const float*)a.mask)[row];
+}
+
+// A row's results from its maximum, sum and token. A token outside the row has no probability: everything of it is NaN.
+template <class T> __device__ __forceinline__ void finish_row(const PolicyArgs& a, int64_t row, float mask, float m, double s) {
+    const int64_t t = token_of(a.token, a.token64, row);
+    float xt = __builtin_nanf("");
+    if (t >= 0 && t < a.cols) xt = Elem<T>::widen(((const T*)a.x + offset_of(a.kept, row))[t]);
+    const double lse = (double)m + log(s);
+    const double logp = (double)xt - lse;
+    a.logp[row] = (float)logp;
+    a.lse[row] = (float)lse;
+    if (!a.old_logp) return;
+    const double adv = a.advantage[row], ratio = exp(logp - (double)a.old_logp[row]);
+    const double low = 1.0 - a.clip_low, high = 1.0 + a.clip_high;
+    const double free = ratio * adv, held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
+    double loss = free <= held ? -free : -held, slope = free <= held ? -free : 0.0;
+    if (free != free || held != held) loss = slope = free + held;  // (a NaN is no side of the minimum)
+    if (a.reference) {
+        const double k = (double)a.reference[row] - logp;
+        loss += a.kl_weight * (exp(k) - k - 1.0);
+        slope += a.kl_weight * (1.0 - exp(k));
+    }
+    a.each[row] = loss * mask;
+    a.weight[row] = (float)(slope * mask);  // (over the sum of the mask: in the last launch)
+}
+// A row that the mask leaves out.
+__device__ __forceinline__ void skip_row(const PolicyArgs& a, int64_t row) {
+    a.logp[row] = a.lse[row] = 0.0f;
+    if (a.old_logp) {
+        a.each[row] = 0.0;
+        a.weight[row] = 0.0f;
+    }
+}
+
+// Maximum and sum of a part of a row. Vectors are aligned from the part's first aligned element on; the elements before it and behind the
+// last whole vector are taken one by one. Four vectors of a thread are in flight together.
+template <class T>
+__global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
+    constexpr int VEC = 16 / sizeof(T), B = 4;
+    __shared__ float most[4];
+    __shared__ double sums[4];
+    for (int64_t at = blockIdx.x; at < a.rows * a.split; at += gridDim.x) {
+        const int64_t row = at / a.split;
+        const int part = (int)(at % a.split);
+        const float mask = mask_of(a, row);
+        if (mask == 0.0f) {
+            if (part == 0 && threadIdx.x == 0 && a.split == 1) skip_row(a, row);
+            continue;  // (the same for the whole workgroup)
+        }
+        const int each = ((a.cols + a.split - 1) / a.split + VEC - 1) / VEC * VEC;
+        const int e0 = min(part * each, a.cols), n = min(each, a.cols - e0);
+        const T* x = (const T*)a.x + offset_of(a.kept, row) + e0;
+        const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+        const int vecs = (n - head) / VEC, tail = head + vecs * VEC;
+        const T* body = x + head;
+        float m = -__builtin_huge_valf(), s = 0.0f;
+        auto take = [&](const float* v, int count) {
+            float t = m;
+            for (int i = 0; i < count; ++i) t = fmaxf(t, v[i]);
+            float add = 0.0f;
+            for (int i = 0; i < count; ++i) add += v[i] == t ? 1.0f : exp_row<T>(v[i] - t);
+            s = (m == t ? s : s * exp_row<T>(m - t)) + add;
+            m = t;
+        };
+        // (fewer than two vectors of single elements: a lane each)
+        if ((int)threadIdx.x < head) {
+            const float v = Elem<T>::widen(x[threadIdx.x]);
+            take(&v, 1);
+        }
+        if ((int)threadIdx.x < n - tail) {
+            const float v = Elem<T>::widen(x[tail + threadIdx.x]);
+            take(&v, 1);
+        }
+        int v = threadIdx.x;
+        for (; v + (B - 1) * 256 < vecs; v += B * 256) {
+            Pack<T, VEC> p[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) p[b] = load_pack<T, VEC>(body + (int64_t)(v + b * 256) * VEC);
+            float f[B * VEC];
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[b * VEC + i] = Elem<T>::widen(p[b].v[i]);
+            take(f, B * VEC);
+        }
+        for (; v < vecs; v += 256) {
+            const Pack<T, VEC> p = load_pack<T, VEC>(body + (int64_t)v * VEC);
+            float f[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = Elem<T>::widen(p.v[i]);
+            take(f, VEC);
+        }
+        double sd = s;
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) meet<T>(m, sd, __shfl_xor(m, w, 64), shfl_xor_any(sd, w));
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            most[threadIdx.x >> 6] = m;
+            sums[threadIdx.x >> 6] = sd;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 4; ++w) meet<T>(m, sd, most[w], sums[w]);
+            if (a.split == 1) {
+                finish_row<T>(a, row, mask, m, sd);
+            } else {
+                a.partial[2 * at] = m;
+                a.partial[2 * at + 1] = sd;
+            }
+        }
+    }
+}
+
+// The parts of split rows, a thread per row.
+template <class T>
+__global__ __launch_bounds__(64) void policy_rows_kernel(const PolicyArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (row >= a.rows) return;
+    const float mask = mask_of(a, row);
+    if (mask == 0.0f) {
+        skip_row(a, row);
+        return;
+    }
+    const double* p = a.partial + 2 * row * a.split;
+    float m = (float)p[0];
+    double s = p[1];
+    for (int k = 1; k < a.split; ++k) meet<T>(m, s, (float)p[2 * k], p[2 * k + 1]);
+    finish_row<T>(a, row, mask, m, s);
+}
+
+// The sums over the rows, in one workgroup and a fixed order: loss = sum of the losses / sum of the mask, and the weights over
+// the same. Without a row that counts both are 0.
+__global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
+    __shared__ double place[2 * 16];
+    double v[2] = {0.0, 0.0};
+    for (int64_t row = threadIdx.x; row < a.rows; row += 1024) {
+        const float m = mask_of(a, row);
+        v[0] += a.each[row];
+        v[1] += m;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) v[k] += shfl_xor_any(v[k], w);
+        if ((threadIdx.x & 63) == 0) place[2 * (threadIdx.x >> 6) + k] = v[k];
+    }
+    __syncthreads();
+    double loss = 0.0, count = 0.0;
+    for (int w = 0; w < 16; ++w) {
+        loss += place[2 * w];
+        count += place[2 * w + 1];
+    }
+    const double inv = count == 0.0 ? 0.0 : 1.0 / count;
+    if (threadIdx.x == 0) a.loss[0] = (float)(loss * inv);
+    for (int64_t row = threadIdx.x; row < a.rows; row += 1024) a.weight[row] = (float)((double)a.weight[row] * inv);
+}
+
+// The logits' gradient, piece by piece: no sums are left. A row of weight 0 is not read. Results leave as aligned vectors, logits come as
+// they lie (aligned too where both start alike).
+template <class T>
+__global__ __launch_bounds__(256) void policy_grad_kernel(const PolicyGradArgs a, int pieces, int each) {
+    constexpr int VEC = 16 / sizeof(T);
+    for (int64_t at = blockIdx.x; at < a.rows * pieces; at += gridDim.x) {
+        const int64_t row = at / pieces;
+        const int e0 = (int)(at % pieces) * each, n = min(each, a.cols - e0);
+        T* out = (T*)a.out + row * a.cols + e0;
+        const T* x = (const T*)a.x + offset_of(a.kept, row) + e0;
+        const float w = a.weight[row] * a.upstream, lse = a.lse[row];
+        const int64_t t = token_of(a.token, a.token64, row) - e0;
+        const int token = t >= 0 && t < n ? (int)t : -1;
+        const int head = min(n, (int)((16 - ((uintptr_t)out & 15)) & 15) / (int)sizeof(T));
+        const int vecs = (n - head) / VEC, tail = head + vecs * VEC;
+        auto grad = [&](T v, int e) { return Elem<T>::narrow(w == 0.0f ? 0.0f : w * ((e == token ? 1.0f : 0.0f) - exp_row<T>(Elem<T>::widen(v) - lse))); };
+        if ((int)threadIdx.x < head) out[threadIdx.x] = grad(w == 0.0f ? T{} : x[threadIdx.x], threadIdx.x);
+        if ((int)threadIdx.x < n - tail) out[tail + threadIdx.x] = grad(w == 0.0f ? T{} : x[tail + threadIdx.x], tail + threadIdx.x);
+        for (int v = threadIdx.x; v < vecs; v += 256) {
+            const int e = head + v * VEC;
+            Pack<T, VEC> p;
+            __builtin_memset(&p, 0, sizeof p);
+            if (w != 0.0f) p = load_pack_unaligned<T, VEC>(x + e);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) p.v[i] = grad(p.v[i], e + i);
+            store_pack<T, VEC>(out + e, p);
+        }
+    }
+}
+
+}  // namespace
+
+int policy_split(int dtype, int64_t rows, int64_t cols) {
+    if (rows == 0 || rows >= 2048) return 1;
+    const int64_t bytes = cols * (int64_t)dtype_size(dtype);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({64, 2048 / rows, bytes / (16 << 10)}));
+}
+
+void launch_policy_loss(int dtype, const PolicyArgs& a, hipStream_t st) {
+    if (a.rows > 0) HPT_WITH_TYPE(dtype, {
+        policy_stats_kernel<T><<<(unsigned)std::min<int64_t>(a.rows * a.split, 1 << 20), 256, 0, st>>>(a);
+        if (a.split > 1) policy_rows_kernel<T><<<(unsigned)((a.rows + 63) / 64), 64, 0, st>>>(a);
+    });
+    if (a.old_logp) policy_sum_kernel<<<1, 1024, 0, st>>>(a);
+}
+
+void launch_policy_loss_backward(int dtype, const PolicyGradArgs& a, hipStream_t st) {
+    HPT_WITH_TYPE(dtype, {
+        constexpr int VEC = 16 / sizeof(T);
+        // pieces of four vectors per thread, or nearly
+        const int most = 256 * 4 * VEC;
+        const int pieces = (a.cols + most - 1) / most;
+        const int each = ((a.cols + pieces - 1) / pieces + VEC - 1) / VEC * VEC;
+        policy_grad_kernel<T><<<(unsigned)std::min<int64_t>(a.rows * pieces, 1 << 20), 256, 0, st>>>(a, pieces, each);
+    });
+}
+
+}  // namespace hpt

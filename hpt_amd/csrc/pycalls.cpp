@@ -311,6 +311,137 @@ PyObject* py_softmax_causal(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return st != HPT_OK ? status(st) : answer(r, r.w.shape, in.v.ndim);
 }
 
+// ---- operators around a transformer's blocks: the caller brings the results -----------------------
+
+// Reads the arguments of a call one after the other. `ok` turns false where the caller has to go the long way; an exception of the
+// interpreter is left behind where a number is no number.
+struct Reader {
+    PyObject* const* a;
+    Py_ssize_t n, at = 0;
+    bool ok = true;
+    int32_t dev = 0;
+    void* stream = nullptr;
+    View views[12];
+    int used = 0;
+
+    Reader(PyObject* const* args, Py_ssize_t count) : a(args), n(count) {}
+    PyObject* next() { return at < n ? a[at++] : (ok = false, Py_None); }
+    // the tensor that the call is made on, and its stream
+    hpt_view* first() {
+        uint64_t st = 0;
+        View* w = &views[used++];
+        if (n < 2 || !opening(a, w, &dev, &st)) ok = false;
+        stream = (void*)(uintptr_t)st;
+        at = 2;
+        return &w->v;
+    }
+    hpt_view* view() {
+        PyObject* o = next();
+        if (!ok || o == Py_None) return nullptr;
+        View* w = &views[used++];
+        if (!view_of(o, w)) ok = false;
+        return &w->v;
+    }
+    double number() {
+        PyObject* o = next();
+        return ok ? PyFloat_AsDouble(o) : 0.0;
+    }
+    int64_t whole() {
+        PyObject* o = next();
+        if (!ok) return 0;
+        int overflow = 0;
+        const long long v = PyLong_AsLongLongAndOverflow(o, &overflow);
+        if (overflow) ok = false;
+        return v;
+    }
+    int32_t small() {
+        const int64_t v = whole();
+        if (v != (int32_t)v) ok = false;
+        return (int32_t)v;
+    }
+};
+
+// The status of a call through `CALL`, None where it is not taken.
+#define HPT_TAKE(COUNT, READ, CALL)                    \
+    if (wrong_count(n, COUNT)) return nullptr;         \
+    Reader r(a, n);                                    \
+    READ;                                              \
+    if (PyErr_Occurred()) return nullptr;              \
+    if (!r.ok) Py_RETURN_NONE;                         \
+    int32_t st;                                        \
+    Py_BEGIN_ALLOW_THREADS                             \
+    st = CALL;                                         \
+    Py_END_ALLOW_THREADS                               \
+    return status(st)
+
+// rms_norm(tensor, stream, residual, normalized dims, gamma, eps, sum, out)
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(8,
+             hpt_view* in = r.first(); hpt_view* res = r.view(); const int32_t nn = r.small(); hpt_view* g = r.view(); const double eps = r.number();
+             hpt_view* sum = r.view(); hpt_view* out = r.view(),
+             hpt_hip_rms_norm(r.dev, r.stream, in, res, nn, g, eps, sum, out));
+}
+
+// rms_norm_quant(tensor, stream, residual, normalized dims, gamma, eps, format, group, sum, out, scale)
+PyObject* py_rms_norm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(11,
+             hpt_view* in = r.first(); hpt_view* res = r.view(); const int32_t nn = r.small(); hpt_view* g = r.view(); const double eps = r.number();
+             const int32_t format = r.small(); const int64_t group = r.whole(); hpt_view* sum = r.view(); hpt_view* out = r.view();
+             hpt_view* scale = r.view(),
+             hpt_hip_rms_norm_quant(r.dev, r.stream, in, res, nn, g, eps, format, group, sum, out, scale));
+}
+
+// rms_norm_backward(tensor, stream, grad, grad_sum, normalized dims, gamma, eps, workspace, grad_in, grad_gamma)
+PyObject* py_rms_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(10,
+             hpt_view* in = r.first(); hpt_view* grad = r.view(); hpt_view* more = r.view(); const int32_t nn = r.small(); hpt_view* g = r.view();
+             const double eps = r.number(); hpt_view* ws = r.view(); hpt_view* gi = r.view(); hpt_view* gg = r.view(),
+             hpt_hip_rms_norm_backward(r.dev, r.stream, in, grad, more, nn, g, eps, ws, gi, gg));
+}
+
+// softmax_bias(tensor, stream, scale, table, bidirectional, max_distance, query_offset, causal, lengths, workspace, out)
+PyObject* py_softmax_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(11,
+             hpt_view* in = r.first(); const double scale = r.number(); hpt_view* table = r.view(); const int32_t both = r.small();
+             const int64_t most = r.whole(); const int64_t offset = r.whole(); const int32_t causal = r.small(); hpt_view* lengths = r.view();
+             hpt_view* ws = r.view(); hpt_view* out = r.view(),
+             hpt_hip_softmax_bias(r.dev, r.stream, in, scale, table, both, most, offset, causal, lengths, ws, out));
+}
+
+// softmax_bias_backward(tensor, stream, grad, scale, bidirectional, max_distance, query_offset, causal, lengths, workspace, grad_in, grad_table)
+PyObject* py_softmax_bias_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(12,
+             hpt_view* in = r.first(); hpt_view* grad = r.view(); const double scale = r.number(); const int32_t both = r.small();
+             const int64_t most = r.whole(); const int64_t offset = r.whole(); const int32_t causal = r.small(); hpt_view* lengths = r.view();
+             hpt_view* ws = r.view(); hpt_view* gi = r.view(); hpt_view* gt = r.view(),
+             hpt_hip_softmax_bias_backward(r.dev, r.stream, in, grad, scale, both, most, offset, causal, lengths, ws, gi, gt));
+}
+
+// token_logp(tensor, stream, token, workspace, logp, lse)
+PyObject* py_token_logp(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(6,
+             hpt_view* in = r.first(); hpt_view* token = r.view(); hpt_view* ws = r.view(); hpt_view* logp = r.view(); hpt_view* lse = r.view(),
+             hpt_hip_token_logp(r.dev, r.stream, in, token, ws, logp, lse));
+}
+
+// policy_loss(tensor, stream, token, old_logp, advantage, reference, mask, clip_low, clip_high, kl_weight, workspace, loss, logp, lse, weight)
+PyObject* py_policy_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(15,
+             hpt_view* in = r.first(); hpt_view* token = r.view(); hpt_view* old = r.view(); hpt_view* adv = r.view(); hpt_view* ref = r.view();
+             hpt_view* mask = r.view(); const double low = r.number(); const double high = r.number(); const double kl = r.number();
+             hpt_view* ws = r.view(); hpt_view* loss = r.view(); hpt_view* logp = r.view(); hpt_view* lse = r.view(); hpt_view* weight = r.view(),
+             hpt_hip_policy_loss(r.dev, r.stream, in, token, old, adv, ref, mask, low, high, kl, ws, loss, logp, lse, weight));
+}
+
+// policy_loss_backward(tensor, stream, token, lse, weight, grad, grad_logits)
+PyObject* py_policy_loss_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(7,
+             hpt_view* in = r.first(); hpt_view* token = r.view(); hpt_view* lse = r.view(); hpt_view* weight = r.view(); const double grad = r.number();
+             hpt_view* gl = r.view(),
+             hpt_hip_policy_loss_backward(r.dev, r.stream, in, token, lse, weight, grad, gl));
+}
+#undef HPT_TAKE
+
 // free(device, address, bytes, ordered) -> status
 PyObject* py_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (wrong_count(n, 4)) return nullptr;
@@ -333,6 +464,14 @@ PyMethodDef methods[] = {HPT_CALL("reduce", py_reduce),
                          HPT_CALL("softmax", py_softmax),
                          HPT_CALL("layernorm", py_layernorm),
                          HPT_CALL("softmax_causal", py_softmax_causal),
+                         HPT_CALL("rms_norm", py_rms_norm),
+                         HPT_CALL("rms_norm_quant", py_rms_norm_quant),
+                         HPT_CALL("rms_norm_backward", py_rms_norm_backward),
+                         HPT_CALL("softmax_bias", py_softmax_bias),
+                         HPT_CALL("softmax_bias_backward", py_softmax_bias_backward),
+                         HPT_CALL("token_logp", py_token_logp),
+                         HPT_CALL("policy_loss", py_policy_loss),
+                         HPT_CALL("policy_loss_backward", py_policy_loss_backward),
                          HPT_CALL("free", py_free),
                          {nullptr, nullptr, 0, nullptr}};
 #undef HPT_CALL

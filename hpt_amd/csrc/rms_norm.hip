@@ -1,0 +1,476 @@
+// RMS norm over rows: h = x (+ residual), y = h / sqrt(mean(h^2) + eps) * gamma, y in the inputs' type or in 8 bits with scales; and
+// its backward pass.
+//
+// Backward, with r = 1 / sqrt(mean(x^2) + eps) and c = sum over the row of gy * gamma * x:
+//   gx = r * gy * gamma - x * r^3 * c / cols (+ what else arrives at x),   ggamma = sum over the rows of gy * x * r.
+// r and c come from the one read of x and gy that the result needs anyway.
+//
+// Everything here is bound by memory: a row is read once into the registers of the threads that share it and written once. Sums
+// are f32 (x of two bytes widened exactly, squares and products in f32); h is rounded to the inputs' type first, as a
+// separate addition would have stored it, and y is computed from the rounded h; y is rounded once.
+#include <algorithm>
+
+#include "block_rows.hpp"
+
+namespace hpt {
+
+namespace {
+
+// 8-bit outputs: value = y / scale, scale = the group's largest |y| over the type's largest value. 2^-120 at least, so that its
+// reciprocal exists (a row of zeros); a group with a NaN gets a NaN for scale.
+constexpr float kLeastScale = 0x1p-120f;
+
+template <int Q> __device__ __forceinline__ float group_scale(uint32_t most_bits) {
+    const float most = __uint_as_float(most_bits);
+    const float s = most / (Q == QUANT_I8 ? 127.0f : 448.0f);
+    return s < kLeastScale ? kLeastScale : s;
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// VEC values times the reciprocal of their scale, in 8 bits each: nearest, ties to even. |v| <= most * (1 + 2^-23), which rounds to the
+// largest value in both types; NaN becomes 0 in i8 and NaN in e4m3.
+template <int Q, int VEC> __device__ __forceinline__ Pack<uint8_t, VEC> quantized(const float (&y)[VEC], float inv) {
+    static_assert(VEC % 4 == 0, "four values to a word");
+    union { uint32_t w[VEC / 4]; Pack<uint8_t, VEC> p; } u;
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+        if constexpr (Q == QUANT_E4M3) {
+            int w = 0;
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, w, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, w, true);
+            u.w[i] = (uint32_t)w;
+        } else {
+            uint32_t w = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float v = y[4 * i + k] * inv;
+                const int q = v == v ? (int)__builtin_rintf(v) : 0;
+                w |= ((uint32_t)q & 0xffu) << (8 * k);
+            }
+            u.w[i] = w;
+        }
+    }
+    return u.p;
+}
+template <int Q> __device__ __forceinline__ uint8_t quantized_one(float y, float inv) {
+    const float v[4] = {y, 0.0f, 0.0f, 0.0f};
+    return quantized<Q, 4>(v, inv).v[0];
+}
+
+// Rows held in registers. Workgroups walk the rows; gamma is fetched once. Q: groups of `group` elements are `group` / VEC neighbouring lanes
+// (a power of two of them, within a wavefront), or the whole row.
+template <class T, int NC, bool AL, bool RES, int Q>
+__global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    using At = Slot<VEC, AL>;
+    __shared__ float sums[2 * 16];
+    __shared__ uint32_t mosts[2 * 16];
+    int turn = 0, turn_most = 0;
+    const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
+    Pack<T, VEC> g[NC];
+    if (a.gamma) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) g[k] = load_slot<T, AL>((const T*)a.gamma, At(lane + k * tpr, a.cols));
+    }
+    for (int64_t first = (int64_t)blockIdx.x * rpb; first < a.rows; first += (int64_t)gridDim.x * rpb) {
+        const int64_t row = first + ty;
+        const int cols = row < a.rows ? a.cols : 0;  // (threads behind the last row go along to the barriers)
+        const T* x = (const T*)a.x + (cols ? offset_of(a.kept, row) : 0);
+        Pack<T, VEC> p[NC];
+#pragma unroll
+        for (int k = 0; k < NC; ++k) p[k] = load_slot<T, AL>(x, At(lane + k * tpr, cols));
+        if constexpr (RES) {
+            Pack<T, VEC> q[NC];
+            const T* res = (const T*)a.res + row * a.cols;
+#pragma unroll
+            for (int k = 0; k < NC; ++k) q[k] = load_slot<T, AL>(res, At(lane + k * tpr, cols));
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) p[k].v[i] = Elem<T>::narrow(Elem<T>::widen(p[k].v[i]) + Elem<T>::widen(q[k].v[i]));
+                if (a.sum) store_slot<T, VEC, AL>((T*)a.sum + row * a.cols, At(lane + k * tpr, cols), p[k]);
+            }
+        }
+        float ss[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ss[0] = fmaf(Elem<T>::widen(p[k].v[i]), Elem<T>::widen(p[k].v[i]), ss[0]);
+        }
+        fold_row<SumF>(ss, tpr, sums, turn);
+        const float r = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
+        auto value = [&](int k, float (&y)[VEC]) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) y[i] = a.gamma ? Elem<T>::widen(p[k].v[i]) * r * Elem<T>::widen(g[k].v[i]) : Elem<T>::widen(p[k].v[i]) * r;
+        };
+        if constexpr (Q == QUANT_NONE) {
+            T* out = (T*)a.out + row * a.cols;
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                float y[VEC];
+                value(k, y);
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(y[i]);
+                store_slot<T, VEC, AL>(out, At(lane + k * tpr, cols), o);
+            }
+        } else {
+            uint8_t* out = (uint8_t*)a.out + row * a.cols;
+            // (places that hold no element are zeros: 0 * r is NaN where r is infinite or NaN, and then every element of the row is NaN too)
+            uint32_t m[NC];
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                float y[VEC];
+                value(k, y);
+                m[k] = 0;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) m[k] = MaxBits::comb(m[k], magnitude(y[i]));
+            }
+            if (a.group == a.cols) {
+                uint32_t all[1] = {0};
+#pragma unroll
+                for (int k = 0; k < NC; ++k) all[0] = MaxBits::comb(all[0], m[k]);
+                fold_row<MaxBits>(all, tpr, mosts, turn_most);
+                const float s = group_scale<Q>(all[0]);
+                if (lane == 0 && cols) a.scale[row] = s;
+#pragma unroll
+                for (int k = 0; k < NC; ++k) m[k] = __float_as_uint(s);
+            } else {
+                const int lanes = a.group / VEC;
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const float s = group_scale<Q>(group_reduce<MaxBits>(m[k], lanes));
+                    const int v = lane + k * tpr;
+                    if ((lane & (lanes - 1)) == 0 && v * VEC < cols) a.scale[row * (a.cols / a.group) + v / lanes] = s;
+                    m[k] = __float_as_uint(s);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                float y[VEC];
+                value(k, y);
+                store_slot<uint8_t, VEC, AL>(out, At(lane + k * tpr, cols), quantized<Q, VEC>(y, 1.0f / __uint_as_float(m[k])));
+            }
+        }
+    }
+}
+
+// Any row length and any group: a workgroup of 1024 sweeps a row twice (8-bit output with one scale per row: three times). With a
+// residual the first sweep stores the sum where the caller wants it, and later sweeps read it there: x or the residual may be that very
+// memory. A thread meets the same vectors in every sweep, but for the groups, which wavefronts take by elements behind a barrier.
+template <class T, bool RES, int Q>
+__global__ __launch_bounds__(1024) void rms_stream_kernel(const RmsArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    __shared__ float sums[2 * 16];
+    __shared__ uint32_t mosts[2 * 16];
+    int turn = 0, turn_most = 0;
+    const int vecs = (a.cols + VEC - 1) / VEC;
+    const T* gamma = (const T*)a.gamma;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = (const T*)a.x + offset_of(a.kept, row);
+        const T* res = RES ? (const T*)a.res + row * a.cols : nullptr;
+        T* sum = RES && a.sum ? (T*)a.sum + row * a.cols : nullptr;
+        float ss[1] = {0.0f};
+        for (int v = threadIdx.x; v < vecs; v += 1024) {
+            Pack<T, VEC> p = sweep_vec<T>(x, v, a.cols);
+            if constexpr (RES) {
+                const Pack<T, VEC> q = sweep_vec<T>(res, v, a.cols);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) p.v[i] = Elem<T>::narrow(Elem<T>::widen(p.v[i]) + Elem<T>::widen(q.v[i]));
+                if (sum) store_sweep_vec<T, VEC>(sum, v, a.cols, p);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ss[0] = fmaf(Elem<T>::widen(p.v[i]), Elem<T>::widen(p.v[i]), ss[0]);
+        }
+        fold_row<SumF>(ss, 1024, sums, turn);
+        const float r = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
+        const T* h = sum ? sum : x;
+        const bool add = RES && !sum;
+        auto value = [&](int e) {
+            float v = Elem<T>::widen(h[e]);
+            if (add) v = Elem<T>::widen(Elem<T>::narrow(v + Elem<T>::widen(res[e])));
+            v *= r;
+            return gamma ? v * Elem<T>::widen(gamma[e]) : v;
+        };
+        auto values = [&](int v, float (&y)[VEC]) {
+            Pack<T, VEC> p = sweep_vec<T>(h, v, a.cols);
+            if (add) {
+                const Pack<T, VEC> q = sweep_vec<T>(res, v, a.cols);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) p.v[i] = Elem<T>::narrow(Elem<T>::widen(p.v[i]) + Elem<T>::widen(q.v[i]));
+            }
+            Pack<T, VEC> g;
+            if (gamma) g = sweep_vec<T>(gamma, v, a.cols);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) y[i] = gamma ? Elem<T>::widen(p.v[i]) * r * Elem<T>::widen(g.v[i]) : Elem<T>::widen(p.v[i]) * r;
+        };
+        if constexpr (Q == QUANT_NONE) {
+            for (int v = threadIdx.x; v < vecs; v += 1024) {
+                float y[VEC];
+                values(v, y);
+                Pack<T, VEC> p;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) p.v[i] = Elem<T>::narrow(y[i]);
+                store_sweep_vec<T, VEC>((T*)a.out + row * a.cols, v, a.cols, p);
+            }
+        } else {
+            uint8_t* out = (uint8_t*)a.out + row * a.cols;
+            if (a.group == a.cols) {
+                uint32_t m[1] = {0};
+                for (int v = threadIdx.x; v < vecs; v += 1024) {
+                    float y[VEC];
+                    values(v, y);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) m[0] = MaxBits::comb(m[0], magnitude(y[i]));
+                }
+                fold_row<MaxBits>(m, 1024, mosts, turn_most);
+                const float s = group_scale<Q>(m[0]), inv = 1.0f / s;
+                if (threadIdx.x == 0) a.scale[row] = s;
+                for (int v = threadIdx.x; v < vecs; v += 1024) {
+                    float y[VEC];
+                    values(v, y);
+                    store_sweep_vec<uint8_t, VEC>(out, v, a.cols, quantized<Q, VEC>(y, inv));
+                }
+            } else {
+                __syncthreads();  // the sums that other threads have stored
+                const int groups = a.cols / a.group, l = threadIdx.x & 63;
+                for (int n = threadIdx.x >> 6; n < groups; n += 16) {
+                    uint32_t m = 0;
+                    for (int e = l; e < a.group; e += 64) m = MaxBits::comb(m, magnitude(value(n * a.group + e)));
+                    const float s = group_scale<Q>(group_reduce<MaxBits>(m, 64)), inv = 1.0f / s;
+                    if (l == 0) a.scale[row * groups + n] = s;
+                    for (int e = l; e < a.group; e += 64) out[n * a.group + e] = quantized_one<Q>(value(n * a.group + e), inv);
+                }
+            }
+        }
+    }
+}
+
+bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// Rows of whole vectors that all start on the vector grid.
+bool rows_on_grid(const void* p, const Dims& kept, int vec) {
+    bool ok = on_grid(p);
+    for (int i = 0; i < kept.n; ++i) ok = ok && (kept.size[i] == 1 || kept.stride[i] % vec == 0);
+    return ok;
+}
+
+template <class T, bool RES, int Q> void launch_of(const RmsArgs& given, hipStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);
+    RmsArgs a = given;
+    constexpr int dtype_most = sizeof(T) == 4 ? 8 : 4;
+    const bool al = a.cols % VEC == 0 && rows_on_grid(a.x, a.kept, VEC) && on_grid(a.res) && on_grid(a.gamma) && on_grid(a.sum) && on_grid(a.out);
+    const bool grouped = Q != QUANT_NONE && a.group != a.cols;
+    // lanes of a group: a power of two of them within a wavefront
+    const int lanes = grouped && a.group % VEC == 0 ? a.group / VEC : 0;
+    const bool by_lanes = !grouped || (al && lanes >= 1 && lanes <= 64 && (lanes & (lanes - 1)) == 0);
+    const RowDeal d = deal_row(a.cols, sizeof(T), 2, dtype_most, grouped && by_lanes ? lanes : 1);
+    if (!d.held() || !by_lanes || a.cols < VEC) {
+        rms_stream_kernel<T, RES, Q><<<(unsigned)std::min<int64_t>(a.rows, 1 << 16), 1024, 0, st>>>(a);
+        return;
+    }
+    a.tpr = d.tpr;
+    const int64_t blocks = (a.rows + d.rows_per_block() - 1) / d.rows_per_block();
+    const unsigned grid = (unsigned)std::min<int64_t>(blocks, 1 << 16);
+    HPT_WITH_NC(d.nc, {
+        if (al) rms_row_kernel<T, NC, true, RES, Q><<<grid, d.threads, 0, st>>>(a);
+        else rms_row_kernel<T, NC, false, RES, Q><<<grid, d.threads, 0, st>>>(a);
+    });
+}
+
+// ---- backward -------------------------------------------------------------------------------------
+
+// Rows held in registers; each workgroup walks rows and keeps its sums for gamma in registers, which leave as one row of partial sums.
+template <class T, int NC, bool AL>
+__global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    using At = Slot<VEC, AL>;
+    __shared__ float sums[2 * 16 * 2];
+    extern __shared__ float fold[];  // several rows per workgroup: [cols]
+    int turn = 0;
+    const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
+    Pack<T, VEC> g[NC];
+    if (a.gamma) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) g[k] = load_slot<T, AL>((const T*)a.gamma, At(lane + k * tpr, a.cols));
+    }
+    float acc[NC][VEC] = {};
+    for (int64_t first = (int64_t)blockIdx.x * rpb; first < a.rows; first += (int64_t)gridDim.x * rpb) {
+        const int64_t row = first + ty;
+        const int cols = row < a.rows ? a.cols : 0;
+        const T* xr = (const T*)a.x + (cols ? offset_of(a.kept, row) : 0);
+        Pack<T, VEC> x[NC], gy[NC];
+#pragma unroll
+        for (int k = 0; k < NC; ++k) x[k] = load_slot<T, AL>(xr, At(lane + k * tpr, cols));
+#pragma unroll
+        for (int k = 0; k < NC; ++k) gy[k] = load_slot<T, AL>((const T*)a.gy + row * a.cols, At(lane + k * tpr, cols));
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float xv = Elem<T>::widen(x[k].v[i]);
+                float gv = Elem<T>::widen(gy[k].v[i]);
+                if (a.gamma) gv *= Elem<T>::widen(g[k].v[i]);
+                s[0] = fmaf(xv, xv, s[0]);
+                s[1] = fmaf(gv, xv, s[1]);
+            }
+        }
+        fold_row<SumF>(s, tpr, sums, turn);
+        const float r = 1.0f / sqrtf(s[0] / (float)a.cols + a.eps);
+        const float c = r * r * (s[1] / (float)a.cols);
+        T* gx = (T*)a.gx + row * a.cols;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            const At at(lane + k * tpr, cols);
+            Pack<T, VEC> more, p;
+            if (a.gsum) more = load_slot<T, AL>((const T*)a.gsum + row * a.cols, at);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float xv = Elem<T>::widen(x[k].v[i]), gv = Elem<T>::widen(gy[k].v[i]);
+                const float gg = a.gamma ? gv * Elem<T>::widen(g[k].v[i]) : gv;
+                float d = r * (gg - xv * c);
+                if (a.gsum) d += Elem<T>::widen(more.v[i]);
+                p.v[i] = Elem<T>::narrow(d);
+                acc[k][i] = fmaf(gv, xv * r, acc[k][i]);  // (without a row x and gy are zeros and r finite: eps > 0)
+            }
+            store_slot<T, VEC, AL>(gx, at, p);
+        }
+    }
+    if (!a.ggamma) return;
+    float* part = a.partial + (int64_t)blockIdx.x * a.cols;
+    if (rpb == 1) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            const At at(lane + k * tpr, a.cols);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (i >= at.lo) part[at.s + i] = acc[k][i];
+        }
+        return;
+    }
+    for (int t = 0; t < rpb; ++t) {  // the workgroup's rows one after the other: the same order always
+        if (t == ty) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                const At at(lane + k * tpr, a.cols);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (i >= at.lo) fold[at.s + i] = t == 0 ? acc[k][i] : fold[at.s + i] + acc[k][i];
+            }
+        }
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < a.cols; e += blockDim.x) part[e] = fold[e];
+}
+
+// Rows of any length, swept twice; the sums for gamma grow in the workgroup's own row of partial sums (a thread meets its own elements).
+template <class T>
+__global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    __shared__ float sums[2 * 16 * 2];
+    int turn = 0;
+    const int vecs = (a.cols + VEC - 1) / VEC;
+    const T* gamma = (const T*)a.gamma;
+    float* part = a.ggamma ? a.partial + (int64_t)blockIdx.x * a.cols : nullptr;
+    bool fresh = true;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, fresh = false) {
+        const T* x = (const T*)a.x + offset_of(a.kept, row);
+        const T* gy = (const T*)a.gy + row * a.cols;
+        const T* gsum = a.gsum ? (const T*)a.gsum + row * a.cols : nullptr;
+        float s[2] = {0.0f, 0.0f};
+        for (int v = threadIdx.x; v < vecs; v += 1024) {
+            const Pack<T, VEC> xp = sweep_vec<T>(x, v, a.cols), gp = sweep_vec<T>(gy, v, a.cols);
+            Pack<T, VEC> g;
+            if (gamma) g = sweep_vec<T>(gamma, v, a.cols);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float xv = Elem<T>::widen(xp.v[i]);
+                float gv = Elem<T>::widen(gp.v[i]);
+                if (gamma) gv *= Elem<T>::widen(g.v[i]);
+                s[0] = fmaf(xv, xv, s[0]);
+                s[1] = fmaf(gv, xv, s[1]);
+            }
+        }
+        fold_row<SumF>(s, 1024, sums, turn);
+        const float r = 1.0f / sqrtf(s[0] / (float)a.cols + a.eps);
+        const float c = r * r * (s[1] / (float)a.cols);
+        for (int v = threadIdx.x; v < vecs; v += 1024) {
+            const Pack<T, VEC> xp = sweep_vec<T>(x, v, a.cols), gp = sweep_vec<T>(gy, v, a.cols);
+            Pack<T, VEC> g, more, p;
+            if (gamma) g = sweep_vec<T>(gamma, v, a.cols);
+            if (gsum) more = sweep_vec<T>(gsum, v, a.cols);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float xv = Elem<T>::widen(xp.v[i]), gv = Elem<T>::widen(gp.v[i]);
+                const float gg = gamma ? gv * Elem<T>::widen(g.v[i]) : gv;
+                float d = r * (gg - xv * c);
+                if (gsum) d += Elem<T>::widen(more.v[i]);
+                p.v[i] = Elem<T>::narrow(d);
+                const int e = v * VEC + i;
+                if (part && e < a.cols) part[e] = fresh ? gv * (xv * r) : part[e] + gv * (xv * r);
+            }
+            store_sweep_vec<T, VEC>((T*)a.gx + row * a.cols, v, a.cols, p);
+        }
+    }
+}
+
+// The partial sums of gamma's gradient, column by column: 32 columns and 32 rows at a time, in a fixed order, summed in f64.
+__global__ __launch_bounds__(1024) void rms_grad_columns_kernel(const float* partial, int64_t parts, int cols, float* out) {
+    __shared__ double meet[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + tx;
+    double s = 0;
+    if (col < cols) {
+#pragma unroll 8
+        for (int64_t p = ty; p < parts; p += 32) s += partial[p * cols + col];
+    }
+    meet[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && col < cols) {
+        for (int k = 1; k < 32; ++k) s += meet[k][tx];
+        out[col] = (float)s;
+    }
+}
+
+// (two vectors per thread, four of f32: with more the accumulators spill)
+RowDeal grad_deal(int dtype, int64_t cols) { return deal_row(cols, dtype_size(dtype), 2, dtype == HPT_F32 ? 4 : 2); }
+
+}  // namespace
+
+void launch_rms_norm(int dtype, int quant, const RmsArgs& a, hipStream_t st) {
+    HPT_WITH_TYPE(dtype, {
+        if (quant == QUANT_I8) a.res ? launch_of<T, true, QUANT_I8>(a, st) : launch_of<T, false, QUANT_I8>(a, st);
+        else if (quant == QUANT_E4M3) a.res ? launch_of<T, true, QUANT_E4M3>(a, st) : launch_of<T, false, QUANT_E4M3>(a, st);
+        else a.res ? launch_of<T, true, QUANT_NONE>(a, st) : launch_of<T, false, QUANT_NONE>(a, st);
+    });
+}
+
+int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) {
+    const RowDeal d = grad_deal(dtype, cols);
+    const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
+    return std::min<int64_t>(blocks, 512);
+}
+
+void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
+    RmsGradArgs a = given;
+    const RowDeal d = grad_deal(dtype, a.cols);
+    const int64_t parts = rms_grad_partials(dtype, a.rows, a.cols);  // (no rows: none, and gamma's gradient is zeros)
+    a.tpr = d.tpr;
+    const size_t lds = d.rows_per_block() > 1 ? (size_t)a.cols * 4 : 0;
+    if (parts) HPT_WITH_TYPE(dtype, {
+        constexpr int VEC = 16 / sizeof(T);
+        const bool al = a.cols % VEC == 0 && rows_on_grid(a.x, a.kept, VEC) && on_grid(a.gy) && on_grid(a.gsum) && on_grid(a.gamma) && on_grid(a.gx);
+        if (!d.held() || a.cols < VEC) {
+            rms_grad_stream_kernel<T><<<(unsigned)parts, 1024, 0, st>>>(a);
+        } else {
+            HPT_WITH_NC(d.nc, {
+                constexpr int M = sizeof(T) == 4 ? (NC > 4 ? 4 : NC) : (NC > 2 ? 2 : NC);
+                if (al) rms_grad_kernel<T, M, true><<<(unsigned)parts, d.threads, lds, st>>>(a);
+                else rms_grad_kernel<T, M, false><<<(unsigned)parts, d.threads, lds, st>>>(a);
+            });
+        }
+    });
+    if (a.ggamma) rms_grad_columns_kernel<<<(a.cols + 31) / 32, 1024, 0, st>>>(a.partial, parts, a.cols, a.ggamma);
+}
+
+}  // namespace hpt

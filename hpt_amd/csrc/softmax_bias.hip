@@ -1,0 +1,562 @@
+// Attention's softmax(scale * scores + table[bucket(key - query), head]) over the keys, and its backward pass.
+//
+// The bias depends on key - query alone, and from the distance on at which the last bucket begins (`far`) on nothing: a workgroup
+// that works on one head keeps it in LDS by distance, -far ... far, and takes the two ends for all that lies beyond. Masks are
+// parameters (causal, and the lengths of a padded batch): a row keeps the keys up to a last one, what lies behind is neither read
+// nor computed, its results are zeros, and so is a row that keeps no key.
+//
+// Backward, from the probabilities p and the gradient g that arrives at them: d = p (g - sum over the keys of p g); the scores' gradient
+// is scale * d, the table's the sum of d over all places of a bucket. Those sums are taken by distance first: within a row every
+// distance below `far` occurs once, so a row adds to its slots of LDS without a conflict, and the threads keep the sums of the
+// two ends in registers. No atomics: rows follow one another, workgroups leave a row of partial sums each, which a second kernel folds.
+//
+// Bound by memory: one read of every live score, one write of every result. Sums and maxima f32, results rounded once.
+#include <algorithm>
+#include <cmath>
+
+#include "block_rows.hpp"
+
+namespace hpt {
+
+Buckets make_buckets(int64_t total, bool both, int64_t max_distance) {
+    if (total < 2 || total > kMostBuckets) fail(HPT_ERR_PARAM, "position bias: %lld buckets, outside 2..%d", (long long)total, kMostBuckets);
+    if (both && total % 2) fail(HPT_ERR_PARAM, "position bias: an odd number of buckets (%lld) for two directions", (long long)total);
+    Buckets b;
+    b.both = both;
+    b.n = (int)(both ? total / 2 : total);
+    if (b.n < 2) fail(HPT_ERR_PARAM, "position bias: each direction needs two buckets at least");
+    const int half = b.n / 2;  // of one distance each
+    if (max_distance <= half || max_distance > kMostDistance)
+        fail(HPT_ERR_PARAM, "position bias: max_distance %lld outside %d..%d for %d buckets a direction", (long long)max_distance, half + 1, kMostDistance, b.n);
+    for (int k = 0; k <= half; ++k) b.begin[k] = (uint16_t)k;
+    // bucket half + j begins at the first whole distance not below half * (max_distance / half)^(j / (n - half)); a power that comes
+    // within 1e-9 of a whole number is taken for it (both are exact in most cases, doubles are off by 1e-15 or so)
+    for (int j = 1; half + j < b.n; ++j) {
+        const double at = half * std::pow((double)max_distance / half, (double)j / (b.n - half));
+        b.begin[half + j] = (uint16_t)std::ceil(at * (1 - 1e-9));
+    }
+    b.far = b.begin[b.n - 1];
+    return b;
+}
+
+namespace {
+
+__device__ __forceinline__ int bucket_of(const Buckets& b, int d) {
+    const int far = d < 0 ? -d : b.both ? d : 0;
+    int lo = 0, hi = b.n - 1;  // the last bucket that begins at `far` or before
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int)b.begin[mid] <= far) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo + (d > 0 && b.both ? b.n : 0);
+}
+// Slots by distance: -far ... right. Where keys behind the query share bucket 0, one slot is enough for them and for distance 0.
+__device__ __forceinline__ int right_of(const Buckets& b) { return b.both ? b.far : 0; }
+__device__ __forceinline__ int slots_of(const Buckets& b) { return b.far + right_of(b) + 1; }
+
+// A row's last key, exclusive.
+template <class A> __device__ __forceinline__ int live_keys(const A& a, int64_t matrix, int64_t q) {
+    int64_t n = a.keys;
+    if (a.lengths) {
+        const int64_t b = matrix / a.heads;
+        const int64_t len = a.lengths64 ? ((const int64_t*)a.lengths)[b] : (int64_t)((const int32_t*)a.lengths)[b];
+        n = len < n ? len : n;
+    }
+    if (a.causal) {
+        const int64_t seen = q + a.offset + 1;
+        n = seen < n ? seen : n;
+    }
+    return n < 0 ? 0 : (int)n;
+}
+// A row's position as an int: beyond +-2^30 every key is far (there are fewer than 2^29 of them).
+__device__ __forceinline__ int position(int64_t offset, int64_t q) {
+    const int64_t p = q + offset, most = (1 << 30) - 1;
+    return (int)(p > most ? most : p < -most ? -most : p);
+}
+
+template <class T> __device__ __forceinline__ void fill_bias(const BiasArgs& a, int64_t head, float* bias) {
+    const int n = slots_of(a.buckets);
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+        bias[i] = Elem<T>::widen(((const T*)a.table)[bucket_of(a.buckets, i - a.buckets.far) * a.table_bucket + head * a.table_head]);
+}
+
+// VEC scores from key e on -> scale * x + bias, -inf from key `live` on and before place lo.
+template <class T, int VEC>
+__device__ __forceinline__ void biased(const Pack<T, VEC>& p, int e, int lo, int live, int pos, float scale, int far, int right, const float* bias, float (&s)[VEC]) {
+    const int d = e - pos;
+    if (d + VEC - 1 <= -far || d >= right) {
+        const float b = bias[d >= right ? far + right : 0];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = fmaf(scale, Elem<T>::widen(p.v[i]), b);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = fmaf(scale, Elem<T>::widen(p.v[i]), bias[min(max(d + i, -far), right) + far]);
+    }
+    if (lo > 0 || e + VEC > live) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < lo || e + i >= live) s[i] = -__builtin_huge_valf();
+    }
+}
+
+// Rows held in registers. An item is `per_item` rows of one matrix; the first row is on its way while the bias comes together.
+template <class T, int NC, bool AL>
+__global__ __launch_bounds__(1024) void bias_row_kernel(const BiasArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    using At = Slot<VEC, AL>;
+    extern __shared__ float bias[];
+    __shared__ float most[2 * 16], sums[2 * 16];
+    int turn_m = 0, turn_s = 0;
+    const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
+    const int far = a.buckets.far, right = right_of(a.buckets);
+    const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+            const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+            const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
+            Pack<T, VEC> p[NC];
+            int live = 0;
+            auto fetch = [&](int64_t q) {
+                const bool there = q < q1;
+                live = there ? live_keys(a, matrix, q) : 0;
+                const int64_t row = matrix * a.queries + q;
+                const T* x = (const T*)a.x + (there ? offset_of(a.kept, row) : 0);
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    At at(lane + k * tpr, a.keys);
+                    if (at.s + at.lo >= live) at.lo = VEC;  // (nothing of it is live: not read)
+                    p[k] = load_slot<T, AL>(x, at);
+                }
+            };
+            fetch(q0 + ty);
+            __syncthreads();  // (the bias of the item before is no longer read)
+            fill_bias<T>(a, matrix % a.heads, bias);
+            __syncthreads();
+            for (int64_t first = q0; first < q1; first += rpb) {
+                const int64_t q = first + ty;
+                if (first != q0) fetch(q);
+                const int pos = position(a.offset, q);
+                float s[NC][VEC];
+                float m[1] = {-__builtin_huge_valf()};
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const At at(lane + k * tpr, a.keys);
+                    biased<T, VEC>(p[k], at.s, at.lo, live, pos, a.scale, far, right, bias, s[k]);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) m[0] = fmaxf(m[0], s[k][i]);
+                }
+                fold_row<MaxF>(m, tpr, most, turn_m);
+                float t[1] = {0.0f};
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const At at(lane + k * tpr, a.keys);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        // (a masked place is -inf: its exponential is 0, except in a row of -inf, which would be -inf - -inf)
+                        s[k][i] = i < at.lo || at.s + i >= live ? 0.0f : exp_row<T>(s[k][i] - m[0]);
+                        t[0] += s[k][i];
+                    }
+                }
+                fold_row<SumF>(t, tpr, sums, turn_s);
+                const float inv = live ? 1.0f / t[0] : 0.0f;
+                if (q < q1) {
+                    T* out = (T*)a.out + (matrix * a.queries + q) * a.keys;
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        const At at(lane + k * tpr, a.keys);
+                        Pack<T, VEC> o;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(at.s + i < live ? s[k][i] * inv : 0.0f);
+                        store_slot<T, VEC, AL>(out, at, o);
+                    }
+                }
+            }
+    }
+}
+
+// (maximum, sum of exponentials below it) of what has been seen, and of two such.
+template <class T> __device__ __forceinline__ void meet(float& m, float& s, float m2, float s2) {
+    const float n = fmaxf(m, m2);
+    // (nothing seen is (-inf, 0); equal infinities are no distance apart; a NaN is in its sum)
+    s = s * (m == n ? 1.0f : exp_row<T>(m - n)) + s2 * (m2 == n ? 1.0f : exp_row<T>(m2 - n));
+    m = n;
+}
+
+// Statistics of the live keys of `row` from vector v0 to v1, over the whole workgroup (a multiple of 64 threads).
+template <class T> __device__ __forceinline__ void sweep_stats(const BiasArgs& a, const T* x, int v0, int v1, int live, int pos, const float* bias, float* place, float& m, float& s) {
+    constexpr int VEC = 16 / sizeof(T);
+    m = -__builtin_huge_valf();
+    s = 0.0f;
+    for (int v = v0 + threadIdx.x; v < v1 && v * VEC < live; v += blockDim.x) {
+        float t[VEC];
+        biased<T, VEC>(sweep_vec<T>(x, v, a.keys), v * VEC, 0, live, pos, a.scale, a.buckets.far, right_of(a.buckets), bias, t);
+        float n = m;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) n = fmaxf(n, t[i]);
+        float add = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) add += v * VEC + i >= live ? 0.0f : t[i] == n ? 1.0f : exp_row<T>(t[i] - n);
+        s = (m == n ? s : s * exp_row<T>(m - n)) + add;
+        m = n;
+    }
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) meet<T>(m, s, __shfl_xor(m, w, 64), __shfl_xor(s, w, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        place[2 * (threadIdx.x >> 6)] = m;
+        place[2 * (threadIdx.x >> 6) + 1] = s;
+    }
+    __syncthreads();
+    m = place[0];
+    s = place[1];
+    for (int w = 1; w < (int)blockDim.x >> 6; ++w) meet<T>(m, s, place[2 * w], place[2 * w + 1]);
+}
+
+template <class T> __device__ __forceinline__ void sweep_apply(const BiasArgs& a, const T* x, T* out, int v0, int v1, int live, int pos, const float* bias, float m, float s) {
+    constexpr int VEC = 16 / sizeof(T);
+    // (a row that keeps keys of -inf alone, or one of +inf, is NaN, as any softmax's)
+    const bool none = m == -__builtin_huge_valf() || m == __builtin_huge_valf();
+    const float inv = none ? __builtin_nanf("") : 1.0f / s;
+    for (int v = v0 + threadIdx.x; v < v1; v += blockDim.x) {
+        Pack<T, VEC> o;
+        if (v * VEC < live) {
+            float t[VEC];
+            biased<T, VEC>(sweep_vec<T>(x, v, a.keys), v * VEC, 0, live, pos, a.scale, a.buckets.far, right_of(a.buckets), bias, t);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(v * VEC + i >= live ? 0.0f : exp_row<T>(t[i] - m) * inv);
+        } else {
+            __builtin_memset(&o, 0, sizeof o);
+        }
+        store_sweep_vec<T, VEC>(out, v, a.keys, o);
+    }
+}
+
+// Rows of any length, a workgroup each: statistics, then a second read.
+template <class T>
+__global__ __launch_bounds__(1024) void bias_stream_kernel(const BiasArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    extern __shared__ float bias[];
+    __shared__ float place[32];
+    const int vecs = (a.keys + VEC - 1) / VEC;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t matrix = row / a.queries, q = row % a.queries;
+        __syncthreads();
+        fill_bias<T>(a, matrix % a.heads, bias);
+        __syncthreads();
+        const int live = live_keys(a, matrix, q), pos = position(a.offset, q);
+        const T* x = (const T*)a.x + offset_of(a.kept, row);
+        float m, s;
+        sweep_stats<T>(a, x, 0, vecs, live, pos, bias, place, m, s);
+        sweep_apply<T>(a, x, (T*)a.out + row * a.keys, 0, vecs, live, pos, bias, m, s);
+    }
+}
+
+// Few, long rows: a.split workgroups share one. APPLY: the second launch, in which each folds all parts' statistics.
+template <class T, bool APPLY>
+__global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    extern __shared__ float bias[];
+    __shared__ float place[8];
+    const int64_t row = blockIdx.x / a.split, matrix = row / a.queries, q = row % a.queries;
+    const int part = blockIdx.x % a.split;
+    const int vecs = (a.keys + VEC - 1) / VEC, each = (vecs + a.split - 1) / a.split;
+    const int v0 = min(part * each, vecs), v1 = min(v0 + each, vecs);
+    fill_bias<T>(a, matrix % a.heads, bias);
+    __syncthreads();
+    const int live = live_keys(a, matrix, q), pos = position(a.offset, q);
+    const T* x = (const T*)a.x + offset_of(a.kept, row);
+    float m, s;
+    if constexpr (!APPLY) {
+        sweep_stats<T>(a, x, v0, v1, live, pos, bias, place, m, s);
+        if (threadIdx.x == 0) {
+            a.partial[2 * (row * a.split + part)] = m;
+            a.partial[2 * (row * a.split + part) + 1] = s;
+        }
+    } else {
+        const float* p = a.partial + 2 * row * a.split;
+        m = p[0];
+        s = p[1];
+        for (int k = 1; k < a.split; ++k) meet<T>(m, s, p[2 * k], p[2 * k + 1]);
+        sweep_apply<T>(a, x, (T*)a.out + row * a.keys, v0, v1, live, pos, bias, m, s);
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------------------
+
+// What a row's element at distance d adds: to its slot, or to the thread's own sum of an end.
+template <int VEC>
+__device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, int lo, int live, int pos, int far, int right, float* slots, float& left_end, float& right_end) {
+    const int r = e - pos;
+    if (r + VEC - 1 <= -far) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) left_end += d[i];  // (places that hold no live element are zeros)
+    } else if (r >= right) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) right_end += d[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int at = r + i;
+            if (i < lo || e + i >= live) continue;
+            if (at <= -far) left_end += d[i];
+            else if (at >= right) right_end += d[i];
+            else slots[at + far] += d[i];
+        }
+    }
+}
+
+// The workgroup's sums by distance -> by bucket, into its row of partial sums. `slots`: one array of them for each of `groups` rows that
+// run side by side. Every thread of the workgroup comes here.
+__device__ __forceinline__ void leave_buckets(const Buckets& b, float* slots, int groups, float left_end, float right_end, float* out) {
+    __shared__ float ends[2 * 16 * 2];
+    const int n = slots_of(b), total = b.both ? 2 * b.n : b.n;
+    float e[2] = {left_end, right_end};
+    int turn = 0;
+    fold_row<SumF>(e, blockDim.x, ends, turn);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        float s = slots[i];
+        for (int g = 1; g < groups; ++g) s += slots[g * n + i];
+        slots[i] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) slots[0] = e[0];          // distance -far and beyond
+    if (threadIdx.x == 0) slots[n - 1] = e[1];      // `right` and beyond
+    __syncthreads();
+    for (int k = threadIdx.x; k < total; k += blockDim.x) {
+        const bool behind = b.both && k >= b.n;
+        const int j = behind ? k - b.n : k;
+        const int from = b.begin[j], to = j + 1 < b.n ? b.begin[j + 1] : b.far + 1;  // distances of bucket k
+        float s = 0.0f;
+        for (int d = from; d < to; ++d) {
+            if (behind && d == 0) continue;  // (distance 0 is the other direction's)
+            s += slots[(behind ? d : -d) + b.far];
+        }
+        out[k] = s;
+    }
+}
+
+// Rows held in registers, one after the other into the same slots. Rows above a wavefront meet in a barrier between two rows' additions
+// (the fold); rows within one are kept in order by the fence.
+template <class T, int NC, bool AL>
+__global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    using At = Slot<VEC, AL>;
+    extern __shared__ float slots[];  // [rows side by side, distances]
+    __shared__ float sums[2 * 16];
+    int turn = 0;
+    const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
+    const int far = a.buckets.far, right = right_of(a.buckets), n = slots_of(a.buckets);
+    const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+        const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
+        float left_end = 0.0f, right_end = 0.0f;
+        __syncthreads();  // (the item before has left its sums)
+        for (int i = threadIdx.x; i < n * rpb; i += blockDim.x) slots[i] = 0.0f;
+        __syncthreads();
+        for (int64_t first = q0; first < q1; first += rpb) {
+            const int64_t q = first + ty, row = matrix * a.queries + q;
+            const int live = q < q1 ? live_keys(a, matrix, q) : 0, pos = position(a.offset, q);
+            const T *p = (const T*)a.p + row * a.keys, *g = (const T*)a.g + row * a.keys;
+            float pv[NC][VEC], gv[NC][VEC];
+            float s[1] = {0.0f};
+            {
+                Pack<T, VEC> pp[NC], gp[NC];
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    At at(lane + k * tpr, a.keys);
+                    if (at.s + at.lo >= live) at.lo = VEC;
+                    pp[k] = load_slot<T, AL>(p, at);
+                    gp[k] = load_slot<T, AL>(g, at);
+                }
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const At at(lane + k * tpr, a.keys);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const bool on = at.s + i < live;
+                        pv[k][i] = on ? Elem<T>::widen(pp[k].v[i]) : 0.0f;
+                        gv[k][i] = on ? Elem<T>::widen(gp[k].v[i]) : 0.0f;
+                        s[0] = fmaf(pv[k][i], gv[k][i], s[0]);
+                    }
+                }
+            }
+            fold_row<SumF>(s, tpr, sums, turn);
+            T* out = (T*)a.out + row * a.keys;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                const At at(lane + k * tpr, a.keys);
+                float d[VEC];
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    d[i] = i >= at.lo && at.s + i < live ? pv[k][i] * (gv[k][i] - s[0]) : 0.0f;
+                    o.v[i] = Elem<T>::narrow(a.scale * d[i]);
+                }
+                if (q < q1) store_slot<T, VEC, AL>(out, at, o);
+                if (a.table_grad && at.s + at.lo < live) add_by_distance<VEC>(d, at.s, at.lo, live, pos, far, right, slots + ty * n, left_end, right_end);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (a.table_grad) leave_buckets(a.buckets, slots, rpb, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+    }
+}
+
+// Rows of any length: two sweeps.
+template <class T>
+__global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    extern __shared__ float slots[];
+    __shared__ float sums[2 * 16];
+    int turn = 0;
+    const int far = a.buckets.far, right = right_of(a.buckets), n = slots_of(a.buckets), vecs = (a.keys + VEC - 1) / VEC;
+    const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+        const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
+        float left_end = 0.0f, right_end = 0.0f;
+        __syncthreads();  // (the item before has left its sums)
+        for (int i = threadIdx.x; i < n; i += 1024) slots[i] = 0.0f;
+        __syncthreads();
+        for (int64_t q = q0; q < q1; ++q) {
+            const int64_t row = matrix * a.queries + q;
+            const int live = live_keys(a, matrix, q), pos = position(a.offset, q);
+            const T *p = (const T*)a.p + row * a.keys, *g = (const T*)a.g + row * a.keys;
+            float s[1] = {0.0f};
+            for (int v = threadIdx.x; v * VEC < live; v += 1024) {
+                const Pack<T, VEC> pp = sweep_vec<T>(p, v, a.keys), gp = sweep_vec<T>(g, v, a.keys);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (v * VEC + i < live) s[0] = fmaf(Elem<T>::widen(pp.v[i]), Elem<T>::widen(gp.v[i]), s[0]);
+            }
+            fold_row<SumF>(s, 1024, sums, turn);  // (its barrier also keeps two rows' additions apart)
+            for (int v = threadIdx.x; v < vecs; v += 1024) {
+                float d[VEC];
+                Pack<T, VEC> o;
+                __builtin_memset(&o, 0, sizeof o);
+                if (v * VEC < live) {
+                    const Pack<T, VEC> pp = sweep_vec<T>(p, v, a.keys), gp = sweep_vec<T>(g, v, a.keys);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        d[i] = v * VEC + i < live ? Elem<T>::widen(pp.v[i]) * (Elem<T>::widen(gp.v[i]) - s[0]) : 0.0f;
+                        o.v[i] = Elem<T>::narrow(a.scale * d[i]);
+                    }
+                    if (a.table_grad) add_by_distance<VEC>(d, v * VEC, 0, live, pos, far, right, slots, left_end, right_end);
+                }
+                store_sweep_vec<T, VEC>((T*)a.out + row * a.keys, v, a.keys, o);
+            }
+    }
+    if (a.table_grad) leave_buckets(a.buckets, slots, 1, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+    }
+}
+
+// The table's gradient [buckets, heads]: a wavefront for each entry folds the items of its head in a fixed order, in f64.
+__global__ __launch_bounds__(256) void bias_grad_table_kernel(const float* partial, int64_t matrices, int64_t chunks, int64_t heads, int buckets, float* out) {
+    const int64_t entry = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (entry >= heads * buckets) return;
+    const int64_t bucket = entry / heads, head = entry % heads, items = matrices / heads * chunks;
+    double s = 0;
+    for (int64_t i = threadIdx.x & 63; i < items; i += 64) s += partial[((i / chunks * heads + head) * chunks + i % chunks) * buckets + bucket];
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) s += shfl_xor_any(s, w);
+    if ((threadIdx.x & 63) == 0) out[entry] = (float)s;
+}
+
+bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+size_t bias_lds(const Buckets& b) { return (size_t)(b.far + (b.both ? b.far : 0) + 1) * 4; }
+
+// A workgroup holds rows of one matrix: where that has few (a step of decoding has one), down to a wavefront.
+RowDeal deal_keys(int dtype, int64_t queries, int64_t keys, int most) {
+    RowDeal d = deal_row(keys, dtype_size(dtype), 2, most);
+    while (d.tpr <= 64 && d.threads > 64 && d.threads / 2 >= queries * d.tpr) d.threads /= 2;
+    return d;
+}
+RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) { return deal_keys(dtype, queries, keys, most_vecs(dtype)); }
+// (backward: two vectors per thread, four of f32, of two operands)
+RowDeal bias_grad_deal(int dtype, int64_t queries, int64_t keys) { return deal_keys(dtype, queries, keys, dtype == HPT_F32 ? 4 : 2); }
+
+}  // namespace
+
+// Rows that registers do not hold, and few of them, are split: parts of 64 KiB at least.
+int bias_split(int dtype, int64_t rows, int64_t keys) {
+    const RowDeal d = deal_row(keys, dtype_size(dtype), 2, most_vecs(dtype));
+    if (rows >= 512 || rows == 0 || (d.held() && keys * (int64_t)dtype_size(dtype) < (64 << 10))) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({64, 1024 / rows, keys * (int64_t)dtype_size(dtype) / (16 << 10)}));
+}
+
+void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
+    BiasArgs a = given;
+    const size_t lds = bias_lds(a.buckets);
+    const int64_t matrices = a.rows / a.queries;
+    HPT_WITH_TYPE(dtype, {
+        constexpr int VEC = 16 / sizeof(T);
+        const RowDeal d = bias_deal(dtype, a.queries, a.keys);
+        if (a.split > 1) {
+            const unsigned grid = (unsigned)(a.rows * a.split);
+            bias_split_kernel<T, false><<<grid, 256, lds, st>>>(a);
+            bias_split_kernel<T, true><<<grid, 256, lds, st>>>(a);
+        } else if (!d.held() || a.keys < VEC) {
+            bias_stream_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 16), 1024, lds, st>>>(a);
+        } else {
+            a.tpr = d.tpr;
+            const int rpb = d.rows_per_block();
+            // items enough for eight workgroups per compute unit, of up to 64 rows
+            const int64_t rounds = std::max<int64_t>(1, std::min<int64_t>(a.rows / 2048 / rpb, 64 / rpb));
+            a.per_item = (int)(rounds * rpb);
+            const int64_t items = matrices * ((a.queries + a.per_item - 1) / a.per_item);
+            bool al = a.keys % VEC == 0 && on_grid(a.x) && on_grid(a.out);
+            for (int i = 0; i < a.kept.n; ++i) al = al && (a.kept.size[i] == 1 || a.kept.stride[i] % VEC == 0);
+            const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 20);
+            HPT_WITH_NC(d.nc, {
+                if (al) bias_row_kernel<T, NC, true><<<grid, d.threads, lds, st>>>(a);
+                else bias_row_kernel<T, NC, false><<<grid, d.threads, lds, st>>>(a);
+            });
+        }
+    });
+}
+
+int64_t bias_grad_items(int dtype, int64_t matrices, int64_t queries, int64_t keys, int* per_item) {
+    const RowDeal d = bias_grad_deal(dtype, queries, keys);
+    const int64_t rpb = d.rows_per_block();
+    const int64_t rounds = std::max<int64_t>({1, std::min<int64_t>(matrices * queries / 2048 / rpb, 64 / rpb)});
+    *per_item = (int)(rounds * rpb);
+    return matrices * ((queries + *per_item - 1) / *per_item);
+}
+
+void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStream_t st) {
+    BiasGradArgs a = given;
+    if (a.rows == 0) {  // a table's gradient of zeros
+        const int buckets = a.buckets.both ? 2 * a.buckets.n : a.buckets.n;
+        bias_grad_table_kernel<<<(unsigned)((a.heads * buckets + 3) / 4), 256, 0, st>>>(nullptr, 0, 1, a.heads, buckets, a.table_grad);
+        return;
+    }
+    const int64_t matrices = a.rows / a.queries;
+    const int64_t items = bias_grad_items(dtype, matrices, a.queries, a.keys, &a.per_item);
+    const RowDeal d = bias_grad_deal(dtype, a.queries, a.keys);
+    a.tpr = d.tpr;
+    const size_t one = bias_lds(a.buckets);
+    const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 20);
+    HPT_WITH_TYPE(dtype, {
+        constexpr int VEC = 16 / sizeof(T);
+        const bool al = a.keys % VEC == 0 && on_grid(a.p) && on_grid(a.g) && on_grid(a.out);
+        if (!d.held() || a.keys < VEC || one * d.rows_per_block() > (48 << 10)) {
+            bias_grad_stream_kernel<T><<<grid, 1024, one, st>>>(a);
+        } else {
+            HPT_WITH_NC(d.nc, {
+                constexpr int M = sizeof(T) == 4 ? (NC > 4 ? 4 : NC) : (NC > 2 ? 2 : NC);
+                if (al) bias_grad_kernel<T, M, true><<<grid, d.threads, one * d.rows_per_block(), st>>>(a);
+                else bias_grad_kernel<T, M, false><<<grid, d.threads, one * d.rows_per_block(), st>>>(a);
+            });
+        }
+    });
+    if (a.table_grad) {
+        const int buckets = a.buckets.both ? 2 * a.buckets.n : a.buckets.n;
+        const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item;
+        bias_grad_table_kernel<<<(unsigned)((a.heads * buckets + 3) / 4), 256, 0, st>>>(a.partial, matrices, chunks, a.heads, buckets, a.table_grad);
+    }
+}
+
+}  // namespace hpt

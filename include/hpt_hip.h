@@ -274,6 +274,96 @@ int32_t hpt_hip_add_layernorm(int32_t dev, void* stream, const hpt_view* in, con
                               int32_t n_norm_dims, const hpt_view* gamma, const hpt_view* beta, double eps,
                               hpt_view* out);
 
+/* ---- operators around a transformer's blocks ---------------------------------
+ * No trait of the reference has these; they stand beside layernorm, softmax_causal and log_softmax for models that
+ * norm by the root mean square, bias attention by relative positions, or are trained on a policy loss, and give
+ * their gradients. Dtypes f16, bf16 and f32; statistics, sums and the results called f32 below are f32 for all
+ * of them, and every result is rounded once. A row's elements must be neighbours in memory, its rows may lie
+ * anywhere; every other operand and every result is contiguous. Results share no memory with each other or with
+ * operands, except that one may take the very place of an operand where its entry says so.
+ *
+ * `workspace` (may be NULL) is contiguous device memory of any dtype, aligned to 16 bytes, of at least as many
+ * bytes as the entry's *_workspace function says; nothing in it has to start from a known value. Without one
+ * the library uses its own scratch of the stream. A call under graph capture is recorded with the workspace it is
+ * given, and without one refused with HPT_ERR_MEMORY where it needs any (softmax_bias and token_logp then take a
+ * form without scratch). Calls that may run at the same time, replays of captured ones among them, must not share one. */
+
+/* y = h / sqrt(mean(h^2) + eps) * gamma over the trailing `n_norm_dims` dims, with h = in, or, with `residual` (in's
+ * shape and dtype), h = in + residual rounded to in's dtype, as a separate addition would store it; `sum` (may be
+ * NULL) receives that h. `gamma` (may be NULL): as many elements as the normalised dims have, in's dtype. eps > 0.
+ * `out` and `sum` may take the place of `in` or `residual`, not the same one. */
+int32_t hpt_hip_rms_norm(int32_t dev, void* stream, const hpt_view* in, const hpt_view* residual, int32_t n_norm_dims,
+                         const hpt_view* gamma, double eps, hpt_view* sum, hpt_view* out);
+
+typedef enum hpt_quant_format {
+    HPT_QUANT_I8 = 1,   /* `out` is i8: -127 ... 127 */
+    HPT_QUANT_E4M3 = 2  /* `out` is u8: the bits of 8-bit floats with 4 bits of exponent and 3 of fraction (448 at most, no infinities) */
+} hpt_quant_format;
+
+/* The same with y in 8 bits: out = y / scale, rounded to nearest (ties to even), one scale for each run of `group` elements of a
+ * row (0: the whole row; `group` divides the row). scale = largest |y| of the group / largest value of the format, at least
+ * 2^-120 (which is what a group of zeros has); a group with a NaN has a NaN for scale, and 0 (i8) or NaN (e4m3) for values.
+ * `scale`: f32, rows x groups. */
+int32_t hpt_hip_rms_norm_quant(int32_t dev, void* stream, const hpt_view* in, const hpt_view* residual, int32_t n_norm_dims,
+                               const hpt_view* gamma, double eps, int32_t format, int64_t group, hpt_view* sum, hpt_view* out,
+                               hpt_view* scale);
+
+/* The gradients of hpt_hip_rms_norm at h = `in` (with a residual: the stored sum), for `grad`, that of its output.
+ * `grad_sum` (may be NULL): what else arrives at h, the residual stream's gradient; it is added. `grad_in`: in's dtype, the
+ * gradient of h, and so that of both summands; may take the place of `in`, `grad` or `grad_sum`. `grad_gamma` (may be
+ * NULL): f32, summed over all rows. */
+int32_t hpt_hip_rms_norm_backward(int32_t dev, void* stream, const hpt_view* in, const hpt_view* grad, const hpt_view* grad_sum,
+                                  int32_t n_norm_dims, const hpt_view* gamma, double eps, const hpt_view* workspace, hpt_view* grad_in,
+                                  hpt_view* grad_gamma);
+int32_t hpt_hip_rms_norm_backward_workspace(const hpt_view* in, int32_t n_norm_dims, size_t* bytes);
+
+/* softmax over the last dim of scale * in + table[bucket(key - query), head], `in` [..., heads, queries, keys], `table` [buckets,
+ * heads] of in's dtype (any strides). Query i stands at position i + query_offset, key j at position j. With n buckets a
+ * direction (bidirectional: half of the table's, keys ahead of the query take its second half; otherwise all of them, and
+ * keys ahead take bucket 0) distances below n / 2 have a bucket each, distance d above has bucket
+ *   n/2 + floor(log(d / (n/2)) / log(max_distance / (n/2)) * (n - n/2)), n - 1 at most.
+ * 2 to 256 buckets, two a direction at least; n / 2 < max_distance <= 4096.
+ * Masks: `causal` hides the keys behind a query's own position (j > i + query_offset); `lengths` (may be NULL; i32 or i64, one
+ * per leading index) the keys from a sequence's length on. Hidden keys are not read and their results are 0, as are all
+ * of a row without a key. A row whose keys are -inf, or one of which is NaN or +inf, is NaN where it is not hidden.
+ * `out` may take the place of `in`. */
+int32_t hpt_hip_softmax_bias(int32_t dev, void* stream, const hpt_view* in, double scale, const hpt_view* table, int32_t bidirectional,
+                             int64_t max_distance, int64_t query_offset, int32_t causal, const hpt_view* lengths,
+                             const hpt_view* workspace, hpt_view* out);
+int32_t hpt_hip_softmax_bias_workspace(const hpt_view* in, size_t* bytes);
+
+/* The gradients of hpt_hip_softmax_bias from its results `probs` and their gradient `grad` (both contiguous): with
+ * d = probs * (grad - sum over the keys of probs * grad), grad_in = scale * d (probs' dtype; may take the place of `probs` or
+ * `grad`) and grad_table (f32, [buckets, heads]; may be NULL) the sum of d over all places of a bucket. Hidden keys are not
+ * read and their gradients are 0. */
+int32_t hpt_hip_softmax_bias_backward(int32_t dev, void* stream, const hpt_view* probs, const hpt_view* grad, double scale,
+                                      int32_t bidirectional, int64_t max_distance, int64_t query_offset, int32_t causal,
+                                      const hpt_view* lengths, const hpt_view* workspace, hpt_view* grad_in, hpt_view* grad_table);
+int32_t hpt_hip_softmax_bias_backward_workspace(const hpt_view* probs, int64_t buckets, size_t* bytes);
+
+/* The log-probability of one token (i32 or i64) for each row of `logits` [..., vocabulary], and the row's log of the sum of
+ * exponentials, both f32. A token outside the vocabulary has a NaN for logp. */
+int32_t hpt_hip_token_logp(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* workspace,
+                           hpt_view* logp, hpt_view* lse);
+
+/* The clipped policy loss: with ratio = exp(logp - old_logp) and A = advantage, each row's loss is
+ *   -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(reference - logp) - (reference - logp) - 1),
+ * and `loss` (f32, one element) their mean with `mask` (f32 weights or bool; NULL: all ones) as weights: 0 where the mask sums to 0.
+ * logp, lse: as hpt_hip_token_logp, `weight` the derivative of `loss` by each row's logp (all f32, one for each row); where both
+ * sides of the minimum are equal it is the unclipped one's. Rows whose mask is 0 are not read, whatever their token, and
+ * their logp, lse and weight are 0. `reference` may be NULL if kl_weight is 0. 0 <= clip_low <= 1, clip_high >= 0.
+ * The workspace also serves hpt_hip_token_logp. */
+int32_t hpt_hip_policy_loss(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* old_logp,
+                            const hpt_view* advantage, const hpt_view* reference, const hpt_view* mask, double clip_low,
+                            double clip_high, double kl_weight, const hpt_view* workspace, hpt_view* loss, hpt_view* logp,
+                            hpt_view* lse, hpt_view* weight);
+int32_t hpt_hip_policy_loss_workspace(const hpt_view* logits, size_t* bytes);
+
+/* The gradient of the logits of anything that depends on them through the rows' logp: grad * weight * (1[v = token] - exp(logits -
+ * lse)), in logits' dtype. A row of weight 0 is not read. `grad_logits` may take the place of `logits`. */
+int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* lse,
+                                     const hpt_view* weight, double grad, hpt_view* grad_logits);
+
 /* ---- the steps either side of the path ------------------------------------
  * What the callers of reductions and normalisations do to their operands just
  * before and after, kept on the device. */
