@@ -16,10 +16,22 @@ namespace hpt {
 
 namespace {
 
-template <class T> __device__ __forceinline__ void meet(float& m, double& s, float m2, double s2) {
+// Exponentials are powers of two of x * kLog2e (the float, whose distance from log2 e moves a row's lse by 1e-8 of its entropy once the
+// result is divided by the same float), so that one multiply-add makes the hardware's argument; a row's running maximum is kept in those
+// units. The sum's error is that of its terms weighted with their shares: rounding the argument costs a term |x - max| / 2^24.
+constexpr float kLog2e = 1.44269504f;
+
+// (maximum in those units, sum of the powers below it) of two lanes or wavefronts.
+__device__ __forceinline__ void meet(float& m, double& s, float m2, double s2) {
     const float n = fmaxf(m, m2);
-    // (nothing seen is (-inf, 0); a NaN is in its sum)
-    s = s * (double)(m == n ? 1.0f : exp_row<T>(m - n)) + s2 * (double)(m2 == n ? 1.0f : exp_row<T>(m2 - n));
+    // (nothing seen is (-inf, 0); equal infinities are no distance apart; a NaN is in its sum)
+    s = s * (double)(m == n ? 1.0f : __builtin_amdgcn_exp2f(m - n)) + s2 * (double)(m2 == n ? 1.0f : __builtin_amdgcn_exp2f(m2 - n));
+    m = n;
+}
+// (maximum, sum of exponentials below it) of two parts of a row.
+__device__ __forceinline__ void join(double& m, double& s, double m2, double s2) {
+    const double n = fmax(m, m2);
+    s = s * (m == n ? 1.0 : exp(m - n)) + s2 * (m2 == n ? 1.0 : exp(m2 - n));
     m = n;
 }
 
@@ -32,12 +44,12 @@ __device__ __forceinline__ float mask_of(const PolicyArgs& a, int64_t row) {
 }
 
 // A row's results from its maximum, sum and token. A token outside the row has no probability: everything of it is NaN.
-template <class T> __device__ __forceinline__ void finish_row(const PolicyArgs& a, int64_t row, float mask, float m, double s) {
+template <class T> __device__ __forceinline__ void finish_row(const PolicyArgs& a, int64_t row, float mask, double m, double s) {
     const int64_t t = token_of(a.token, a.token64, row);
     float xt = __builtin_nanf("");
     if (t >= 0 && t < a.cols) xt = Elem<T>::widen(((const T*)a.x + offset_of(a.kept, row))[t]);
-    const double lse = (double)m + log(s);
-    const double logp = (double)xt - lse;
+    const double rest = log(s), lse = m + rest;
+    const double logp = ((double)xt - m) - rest;  // (exact differences first: m may be a type's lowest value)
     a.logp[row] = (float)logp;
     a.lse[row] = (float)lse;
     if (!a.old_logp) return;
@@ -70,12 +82,13 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
     constexpr int VEC = 16 / sizeof(T), B = 4;
     __shared__ float most[4];
     __shared__ double sums[4];
+    const float inf = __builtin_huge_valf();
     for (int64_t at = blockIdx.x; at < a.rows * a.split; at += gridDim.x) {
         const int64_t row = at / a.split;
         const int part = (int)(at % a.split);
         const float mask = mask_of(a, row);
         if (mask == 0.0f) {
-            if (part == 0 && threadIdx.x == 0 && a.split == 1) skip_row(a, row);
+            if (threadIdx.x == 0 && a.split == 1) skip_row(a, row);
             continue;  // (the same for the whole workgroup)
         }
         const int each = ((a.cols + a.split - 1) / a.split + VEC - 1) / VEC * VEC;
@@ -84,88 +97,114 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
         const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
         const int vecs = (n - head) / VEC, tail = head + vecs * VEC;
         const T* body = x + head;
-        float m = -__builtin_huge_valf(), s = 0.0f;
-        auto take = [&](const float* v, int count) {
-            float t = m;
-            for (int i = 0; i < count; ++i) t = fmaxf(t, v[i]);
+        float m = -inf, s = 0.0f;
+        auto take = [&](auto& v) {
+            constexpr int N = sizeof(v) / sizeof(float);
+            float t = v[0];
+#pragma unroll
+            for (int i = 1; i < N; ++i) t = fmaxf(t, v[i]);
+            const float top = fmaxf(m, t * kLog2e);
             float add = 0.0f;
-            for (int i = 0; i < count; ++i) add += v[i] == t ? 1.0f : exp_row<T>(v[i] - t);
-            s = (m == t ? s : s * exp_row<T>(m - t)) + add;
-            m = t;
+            if (fabsf(top) < inf) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) add += __builtin_amdgcn_exp2f(fmaf(v[i], kLog2e, -top));
+                s = s * __builtin_amdgcn_exp2f(m - top) + add;
+                m = top;
+            } else {  // nothing but -inf yet, a +inf, or an overflow: if that stays, the row is swept again below; what counts now is a NaN
+#pragma unroll
+                for (int i = 0; i < N; ++i) add += v[i] == v[i] ? 0.0f : v[i];
+                s += add;
+                m = top;
+            }
         };
         // (fewer than two vectors of single elements: a lane each)
         if ((int)threadIdx.x < head) {
-            const float v = Elem<T>::widen(x[threadIdx.x]);
-            take(&v, 1);
+            float v[1] = {Elem<T>::widen(x[threadIdx.x])};
+            take(v);
         }
         if ((int)threadIdx.x < n - tail) {
-            const float v = Elem<T>::widen(x[tail + threadIdx.x]);
-            take(&v, 1);
+            float v[1] = {Elem<T>::widen(x[tail + threadIdx.x])};
+            take(v);
         }
-        int v = threadIdx.x;
-        for (; v + (B - 1) * 256 < vecs; v += B * 256) {
+        for (int v = threadIdx.x; v < vecs; v += B * 256) {
             Pack<T, VEC> p[B];
 #pragma unroll
-            for (int b = 0; b < B; ++b) p[b] = load_pack<T, VEC>(body + (int64_t)(v + b * 256) * VEC);
+            for (int b = 0; b < B; ++b) {
+                if (v + b * 256 < vecs) p[b] = load_pack_stream<T, VEC>(body + (int64_t)(v + b * 256) * VEC);
+                else
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) p[b].v[i] = Elem<T>::narrow(-inf);
+            }
             float f[B * VEC];
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) f[b * VEC + i] = Elem<T>::widen(p[b].v[i]);
-            take(f, B * VEC);
-        }
-        for (; v < vecs; v += 256) {
-            const Pack<T, VEC> p = load_pack<T, VEC>(body + (int64_t)v * VEC);
-            float f[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = Elem<T>::widen(p.v[i]);
-            take(f, VEC);
+            take(f);
         }
         double sd = s;
 #pragma unroll
-        for (int w = 1; w < 64; w <<= 1) meet<T>(m, sd, __shfl_xor(m, w, 64), shfl_xor_any(sd, w));
+        for (int w = 1; w < 64; w <<= 1) meet(m, sd, __shfl_xor(m, w, 64), shfl_xor_any(sd, w));
         __syncthreads();
         if ((threadIdx.x & 63) == 0) {
             most[threadIdx.x >> 6] = m;
             sums[threadIdx.x >> 6] = sd;
         }
         __syncthreads();
+        m = most[0];
+        sd = sums[0];
+        for (int w = 1; w < 4; ++w) meet(m, sd, most[w], sums[w]);
+        double top = (double)m / (double)kLog2e;
+        if (fabsf(m) == inf && n > 0) {
+            // infinities, or values so near to a type's end that they have none in those units (a row masked as a whole): element by element
+            float t = -inf;
+            for (int i = threadIdx.x; i < n; i += 256) t = fmaxf(t, Elem<T>::widen(x[i]));
+            t = block_reduce<MaxF>(t, most);
+            float add = 0.0f;
+            for (int i = threadIdx.x; i < n; i += 256) {
+                const float v = Elem<T>::widen(x[i]);
+                add += v == t ? 1.0f : __expf(v - t);
+            }
+            top = t;
+            sd = block_reduce<SumF>(add, most);
+        }
         if (threadIdx.x == 0) {
-            for (int w = 1; w < 4; ++w) meet<T>(m, sd, most[w], sums[w]);
             if (a.split == 1) {
-                finish_row<T>(a, row, mask, m, sd);
+                finish_row<T>(a, row, mask, top, sd);
             } else {
-                a.partial[2 * at] = m;
+                a.partial[2 * at] = top;
                 a.partial[2 * at + 1] = sd;
             }
         }
     }
 }
 
-// The parts of split rows, a thread per row.
-template <class T>
-__global__ __launch_bounds__(64) void policy_rows_kernel(const PolicyArgs a) {
-    const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (row >= a.rows) return;
-    const float mask = mask_of(a, row);
+// A split row from its parts.
+template <class T> __device__ __forceinline__ void join_row(const PolicyArgs& a, int64_t row, float mask) {
     if (mask == 0.0f) {
         skip_row(a, row);
         return;
     }
     const double* p = a.partial + 2 * row * a.split;
-    float m = (float)p[0];
-    double s = p[1];
-    for (int k = 1; k < a.split; ++k) meet<T>(m, s, (float)p[2 * k], p[2 * k + 1]);
+    double m = p[0], s = p[1];
+    for (int k = 1; k < a.split; ++k) join(m, s, p[2 * k], p[2 * k + 1]);
     finish_row<T>(a, row, mask, m, s);
+}
+template <class T>
+__global__ __launch_bounds__(64) void policy_rows_kernel(const PolicyArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (row < a.rows) join_row<T>(a, row, mask_of(a, row));
 }
 
 // The sums over the rows, in one workgroup and a fixed order: loss = sum of the losses / sum of the mask, and the weights over
-// the same. Without a row that counts both are 0.
+// the same. Without a row that counts both are 0. Split rows (there are few then) are joined on the way.
+template <class T>
 __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
     __shared__ double place[2 * 16];
     double v[2] = {0.0, 0.0};
     for (int64_t row = threadIdx.x; row < a.rows; row += 1024) {
         const float m = mask_of(a, row);
+        if (a.split > 1) join_row<T>(a, row, m);
         v[0] += a.each[row];
         v[1] += m;
     }
@@ -221,15 +260,15 @@ __global__ __launch_bounds__(256) void policy_grad_kernel(const PolicyGradArgs a
 int policy_split(int dtype, int64_t rows, int64_t cols) {
     if (rows == 0 || rows >= 2048) return 1;
     const int64_t bytes = cols * (int64_t)dtype_size(dtype);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({64, 2048 / rows, bytes / (16 << 10)}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({64, 4096 / rows, bytes / (16 << 10)}));
 }
 
 void launch_policy_loss(int dtype, const PolicyArgs& a, hipStream_t st) {
-    if (a.rows > 0) HPT_WITH_TYPE(dtype, {
-        policy_stats_kernel<T><<<(unsigned)std::min<int64_t>(a.rows * a.split, 1 << 20), 256, 0, st>>>(a);
-        if (a.split > 1) policy_rows_kernel<T><<<(unsigned)((a.rows + 63) / 64), 64, 0, st>>>(a);
+    HPT_WITH_TYPE(dtype, {
+        if (a.rows > 0) policy_stats_kernel<T><<<(unsigned)std::min<int64_t>(a.rows * a.split, 1 << 20), 256, 0, st>>>(a);
+        if (a.old_logp) policy_sum_kernel<T><<<1, 1024, 0, st>>>(a);
+        else if (a.split > 1) policy_rows_kernel<T><<<(unsigned)((a.rows + 63) / 64), 64, 0, st>>>(a);
     });
-    if (a.old_logp) policy_sum_kernel<<<1, 1024, 0, st>>>(a);
 }
 
 void launch_policy_loss_backward(int dtype, const PolicyGradArgs& a, hipStream_t st) {

@@ -280,7 +280,7 @@ template <class T, bool RES, int Q> void launch_of(const RmsArgs& given, hipStre
 // ---- backward -------------------------------------------------------------------------------------
 
 // Rows held in registers; each workgroup walks rows and keeps its sums for gamma in registers, which leave as one row of partial sums.
-template <class T, int NC, bool AL>
+template <class T, int NC, bool AL, bool MORE>
 __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
@@ -298,11 +298,15 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
         const int64_t row = first + ty;
         const int cols = row < a.rows ? a.cols : 0;
         const T* xr = (const T*)a.x + (cols ? offset_of(a.kept, row) : 0);
-        Pack<T, VEC> x[NC], gy[NC];
+        Pack<T, VEC> x[NC], gy[NC], more[MORE ? NC : 1];
 #pragma unroll
         for (int k = 0; k < NC; ++k) x[k] = load_slot<T, AL>(xr, At(lane + k * tpr, cols));
 #pragma unroll
         for (int k = 0; k < NC; ++k) gy[k] = load_slot<T, AL>((const T*)a.gy + row * a.cols, At(lane + k * tpr, cols));
+        if constexpr (MORE) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) more[k] = load_slot<T, AL>((const T*)a.gsum + row * a.cols, At(lane + k * tpr, cols));
+        }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -322,14 +326,13 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
             const At at(lane + k * tpr, cols);
-            Pack<T, VEC> more, p;
-            if (a.gsum) more = load_slot<T, AL>((const T*)a.gsum + row * a.cols, at);
+            Pack<T, VEC> p;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float xv = Elem<T>::widen(x[k].v[i]), gv = Elem<T>::widen(gy[k].v[i]);
                 const float gg = a.gamma ? gv * Elem<T>::widen(g[k].v[i]) : gv;
                 float d = r * (gg - xv * c);
-                if (a.gsum) d += Elem<T>::widen(more.v[i]);
+                if constexpr (MORE) d += Elem<T>::widen(more[k].v[i]);
                 p.v[i] = Elem<T>::narrow(d);
                 acc[k][i] = fmaf(gv, xv * r, acc[k][i]);  // (without a row x and gy are zeros and r finite: eps > 0)
             }
@@ -448,7 +451,7 @@ void launch_rms_norm(int dtype, int quant, const RmsArgs& a, hipStream_t st) {
 int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) {
     const RowDeal d = grad_deal(dtype, cols);
     const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
-    return std::min<int64_t>(blocks, 512);
+    return std::min<int64_t>(blocks, 1024);
 }
 
 void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
@@ -465,8 +468,10 @@ void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t s
         } else {
             HPT_WITH_NC(d.nc, {
                 constexpr int M = sizeof(T) == 4 ? (NC > 4 ? 4 : NC) : (NC > 2 ? 2 : NC);
-                if (al) rms_grad_kernel<T, M, true><<<(unsigned)parts, d.threads, lds, st>>>(a);
-                else rms_grad_kernel<T, M, false><<<(unsigned)parts, d.threads, lds, st>>>(a);
+                if (al && a.gsum) rms_grad_kernel<T, M, true, true><<<(unsigned)parts, d.threads, lds, st>>>(a);
+                else if (al) rms_grad_kernel<T, M, true, false><<<(unsigned)parts, d.threads, lds, st>>>(a);
+                else if (a.gsum) rms_grad_kernel<T, M, false, true><<<(unsigned)parts, d.threads, lds, st>>>(a);
+                else rms_grad_kernel<T, M, false, false><<<(unsigned)parts, d.threads, lds, st>>>(a);
             });
         }
     });

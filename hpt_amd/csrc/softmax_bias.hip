@@ -7,8 +7,9 @@
 //
 // Backward, from the probabilities p and the gradient g that arrives at them: d = p (g - sum over the keys of p g); the scores' gradient
 // is scale * d, the table's the sum of d over all places of a bucket. Those sums are taken by distance first: within a row every
-// distance below `far` occurs once, so a row adds to its slots of LDS without a conflict, and the threads keep the sums of the
-// two ends in registers. No atomics: rows follow one another, workgroups leave a row of partial sums each, which a second kernel folds.
+// distance below `far` occurs once, so a row adds to its places in LDS without a conflict, and the threads keep the sums of the
+// two ends in registers. Rows follow one another, workgroups leave a row of partial sums each, which a second kernel folds: the
+// order is the same always.
 //
 // Bound by memory: one read of every live score, one write of every result. Sums and maxima f32, results rounded once.
 #include <algorithm>
@@ -51,9 +52,11 @@ __device__ __forceinline__ int bucket_of(const Buckets& b, int d) {
     }
     return lo + (d > 0 && b.both ? b.n : 0);
 }
-// Slots by distance: -far ... right. Where keys behind the query share bucket 0, one slot is enough for them and for distance 0.
+// Places by distance in LDS: -far ... right, and a vector's length more on both sides, so that a vector that reaches into the range, from
+// either side, has all its places there. Where keys ahead of the query share bucket 0, one place is enough for them and for distance 0.
+constexpr int kPad = 8;
 __device__ __forceinline__ int right_of(const Buckets& b) { return b.both ? b.far : 0; }
-__device__ __forceinline__ int slots_of(const Buckets& b) { return b.far + right_of(b) + 1; }
+__host__ __device__ inline int places_of(const Buckets& b) { return b.far + (b.both ? b.far : 0) + 1 + 2 * kPad; }
 
 // A row's last key, exclusive.
 template <class A> __device__ __forceinline__ int live_keys(const A& a, int64_t matrix, int64_t q) {
@@ -76,22 +79,27 @@ __device__ __forceinline__ int position(int64_t offset, int64_t q) {
 }
 
 template <class T> __device__ __forceinline__ void fill_bias(const BiasArgs& a, int64_t head, float* bias) {
-    const int n = slots_of(a.buckets);
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-        bias[i] = Elem<T>::widen(((const T*)a.table)[bucket_of(a.buckets, i - a.buckets.far) * a.table_bucket + head * a.table_head]);
+    const int n = places_of(a.buckets), right = right_of(a.buckets);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int d = min(max(i - kPad - a.buckets.far, -a.buckets.far), right);
+        bias[i] = Elem<T>::widen(((const T*)a.table)[bucket_of(a.buckets, d) * a.table_bucket + head * a.table_head]);
+    }
 }
 
-// VEC scores from key e on -> scale * x + bias, -inf from key `live` on and before place lo.
+// VEC scores from key e on -> scale * x + bias, -inf from key `live` on and before place lo. Where no lane of
+// the wavefront is near the query the two ends of the bias are all that is needed, otherwise all take them from LDS, the
+// far ones from its padding.
 template <class T, int VEC>
 __device__ __forceinline__ void biased(const Pack<T, VEC>& p, int e, int lo, int live, int pos, float scale, int far, int right, const float* bias, float (&s)[VEC]) {
     const int d = e - pos;
-    if (d + VEC - 1 <= -far || d >= right) {
-        const float b = bias[d >= right ? far + right : 0];
+    if (__any(d > -far - VEC && d < right)) {
+        const float* b = bias + (min(max(d, -far - kPad), right) + far + kPad);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = fmaf(scale, Elem<T>::widen(p.v[i]), b[i]);
+    } else {
+        const float b = bias[d >= right ? far + right + kPad : 0];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s[i] = fmaf(scale, Elem<T>::widen(p.v[i]), b);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) s[i] = fmaf(scale, Elem<T>::widen(p.v[i]), bias[min(max(d + i, -far), right) + far]);
     }
     if (lo > 0 || e + VEC > live) {
 #pragma unroll
@@ -112,65 +120,75 @@ __global__ __launch_bounds__(1024) void bias_row_kernel(const BiasArgs a) {
     const int far = a.buckets.far, right = right_of(a.buckets);
     const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-            const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
-            const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
-            Pack<T, VEC> p[NC];
-            int live = 0;
-            auto fetch = [&](int64_t q) {
-                const bool there = q < q1;
-                live = there ? live_keys(a, matrix, q) : 0;
-                const int64_t row = matrix * a.queries + q;
-                const T* x = (const T*)a.x + (there ? offset_of(a.kept, row) : 0);
+        const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+        const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
+        Pack<T, VEC> p[NC];
+        int live = 0;
+        auto fetch = [&](int64_t q) {
+            const bool there = q < q1;
+            live = there ? live_keys(a, matrix, q) : 0;
+            const int64_t row = matrix * a.queries + q;
+            const T* x = (const T*)a.x + (there ? offset_of(a.kept, row) : 0);
 #pragma unroll
-                for (int k = 0; k < NC; ++k) {
-                    At at(lane + k * tpr, a.keys);
-                    if (at.s + at.lo >= live) at.lo = VEC;  // (nothing of it is live: not read)
-                    p[k] = load_slot<T, AL>(x, at);
-                }
-            };
-            fetch(q0 + ty);
-            __syncthreads();  // (the bias of the item before is no longer read)
-            fill_bias<T>(a, matrix % a.heads, bias);
-            __syncthreads();
-            for (int64_t first = q0; first < q1; first += rpb) {
-                const int64_t q = first + ty;
-                if (first != q0) fetch(q);
-                const int pos = position(a.offset, q);
-                float s[NC][VEC];
-                float m[1] = {-__builtin_huge_valf()};
+            for (int k = 0; k < NC; ++k) {
+                At at(lane + k * tpr, a.keys);
+                if (at.s + at.lo >= live) at.lo = VEC;  // (nothing of it is live: not read)
+                p[k] = load_slot<T, AL>(x, at);
+            }
+        };
+        fetch(q0 + ty);
+        __syncthreads();  // (the bias of the item before is no longer read)
+        fill_bias<T>(a, matrix % a.heads, bias);
+        __syncthreads();
+        for (int64_t first = q0; first < q1; first += rpb) {
+            const int64_t q = first + ty;
+            if (first != q0) fetch(q);
+            const int pos = position(a.offset, q);
+            float s[NC][VEC];
+            float m[1] = {-__builtin_huge_valf()};
 #pragma unroll
-                for (int k = 0; k < NC; ++k) {
-                    const At at(lane + k * tpr, a.keys);
-                    biased<T, VEC>(p[k], at.s, at.lo, live, pos, a.scale, far, right, bias, s[k]);
+            for (int k = 0; k < NC; ++k) {
+                const At at(lane + k * tpr, a.keys);
+                biased<T, VEC>(p[k], at.s, at.lo, live, pos, a.scale, far, right, bias, s[k]);
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) m[0] = fmaxf(m[0], s[k][i]);
-                }
-                fold_row<MaxF>(m, tpr, most, turn_m);
-                float t[1] = {0.0f};
+                for (int i = 0; i < VEC; ++i) m[0] = fmaxf(m[0], s[k][i]);
+            }
+            fold_row<MaxF>(m, tpr, most, turn_m);
+            // (a hidden place is -inf and its exponential 0: in a row of nothing else, too)
+            const float base = m[0] == -__builtin_huge_valf() ? 0.0f : m[0];
+            float t[1] = {0.0f};
+            // (two-byte types: one multiply-add makes the hardware's argument; what rounding base * log2 e costs is in every term and in their
+            // sum alike. It would overflow next to the type's lowest value, with which callers mask.)
+            constexpr float kLog2e = 1.44269504f;
+            const bool direct = sizeof(T) == 2 && fabsf(base) < 1e38f;
+            const float shift = -base * kLog2e;
 #pragma unroll
-                for (int k = 0; k < NC; ++k) {
-                    const At at(lane + k * tpr, a.keys);
+            for (int k = 0; k < NC; ++k) {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        // (a masked place is -inf: its exponential is 0, except in a row of -inf, which would be -inf - -inf)
-                        s[k][i] = i < at.lo || at.s + i >= live ? 0.0f : exp_row<T>(s[k][i] - m[0]);
-                        t[0] += s[k][i];
-                    }
-                }
-                fold_row<SumF>(t, tpr, sums, turn_s);
-                const float inv = live ? 1.0f / t[0] : 0.0f;
-                if (q < q1) {
-                    T* out = (T*)a.out + (matrix * a.queries + q) * a.keys;
-#pragma unroll
-                    for (int k = 0; k < NC; ++k) {
-                        const At at(lane + k * tpr, a.keys);
-                        Pack<T, VEC> o;
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(at.s + i < live ? s[k][i] * inv : 0.0f);
-                        store_slot<T, VEC, AL>(out, at, o);
-                    }
+                for (int i = 0; i < VEC; ++i) {
+                    s[k][i] = direct ? __builtin_amdgcn_exp2f(fmaf(s[k][i], kLog2e, shift)) : exp_row<T>(s[k][i] - base);
+                    t[0] += s[k][i];
                 }
             }
+            fold_row<SumF>(t, tpr, sums, turn_s);
+            const float inv = live ? 1.0f / t[0] : 0.0f;
+            const bool number = t[0] > 0.0f || !live;
+            if (q < q1) {
+                T* out = (T*)a.out + (matrix * a.queries + q) * a.keys;
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const At at(lane + k * tpr, a.keys);
+                    Pack<T, VEC> o;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(s[k][i] * inv);
+                    if (!number) {  // keys of -inf alone, or a NaN or +inf among them: the hidden ones are zeros all the same
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(at.s + i < live ? __builtin_nanf("") : 0.0f);
+                    }
+                    store_slot<T, VEC, AL>(out, at, o);
+                }
+            }
+        }
     }
 }
 
@@ -283,106 +301,106 @@ __global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
 
 // ---- backward -------------------------------------------------------------------------------------
 
-// What a row's element at distance d adds: to its slot, or to the thread's own sum of an end.
+// What a row's VEC elements from key e on add: to the places of their distances, or, beyond `far` and `right`, to the thread's own sums of
+// the ends. Hidden elements are zeros. Rows add to a place one after the other, each once, so that the sums do not depend on any order
+// though the LDS adds by itself (one instruction instead of a read, its latency and a write).
 template <int VEC>
-__device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, int lo, int live, int pos, int far, int right, float* slots, float& left_end, float& right_end) {
+__device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, int pos, int far, int right, float* places, float& left_end, float& right_end) {
     const int r = e - pos;
-    if (r + VEC - 1 <= -far) {
+    if (r > -far - VEC && r < right) {
+        float* at = places + (r + far + kPad);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) left_end += d[i];  // (places that hold no live element are zeros)
-    } else if (r >= right) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) right_end += d[i];
+        for (int i = 0; i < VEC; ++i) __hip_atomic_fetch_add(at + i, d[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     } else {
+        float s = d[0];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int at = r + i;
-            if (i < lo || e + i >= live) continue;
-            if (at <= -far) left_end += d[i];
-            else if (at >= right) right_end += d[i];
-            else slots[at + far] += d[i];
-        }
+        for (int i = 1; i < VEC; ++i) s += d[i];
+        if (r < 0) left_end += s;
+        else right_end += s;
     }
 }
 
-// The workgroup's sums by distance -> by bucket, into its row of partial sums. `slots`: one array of them for each of `groups` rows that
+// The workgroup's sums by distance -> by bucket, into its row of partial sums. `places`: one array of them for each of `groups` rows that
 // run side by side. Every thread of the workgroup comes here.
-__device__ __forceinline__ void leave_buckets(const Buckets& b, float* slots, int groups, float left_end, float right_end, float* out) {
+__device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, int groups, float left_end, float right_end, float* out) {
     __shared__ float ends[2 * 16 * 2];
-    const int n = slots_of(b), total = b.both ? 2 * b.n : b.n;
+    const int n = places_of(b), total = b.both ? 2 * b.n : b.n;
     float e[2] = {left_end, right_end};
     int turn = 0;
     fold_row<SumF>(e, blockDim.x, ends, turn);
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        float s = slots[i];
-        for (int g = 1; g < groups; ++g) s += slots[g * n + i];
-        slots[i] = s;
+        float s = places[i];
+        for (int g = 1; g < groups; ++g) s += places[g * n + i];
+        places[i] = s;
     }
     __syncthreads();
-    if (threadIdx.x == 0) slots[0] = e[0];          // distance -far and beyond
-    if (threadIdx.x == 0) slots[n - 1] = e[1];      // `right` and beyond
+    if (threadIdx.x == 0) {  // distance -far and beyond, `right` and beyond
+        for (int i = 0; i <= kPad; ++i) e[0] += places[i];
+        for (int i = 0; i <= kPad; ++i) e[1] += places[n - 1 - i];
+        places[kPad] = e[0];
+        places[n - 1 - kPad] = e[1];
+    }
     __syncthreads();
     for (int k = threadIdx.x; k < total; k += blockDim.x) {
-        const bool behind = b.both && k >= b.n;
-        const int j = behind ? k - b.n : k;
+        const bool ahead = b.both && k >= b.n;
+        const int j = ahead ? k - b.n : k;
         const int from = b.begin[j], to = j + 1 < b.n ? b.begin[j + 1] : b.far + 1;  // distances of bucket k
         float s = 0.0f;
         for (int d = from; d < to; ++d) {
-            if (behind && d == 0) continue;  // (distance 0 is the other direction's)
-            s += slots[(behind ? d : -d) + b.far];
+            if (ahead && d == 0) continue;  // (distance 0 is the other direction's)
+            s += places[(ahead ? d : -d) + b.far + kPad];
         }
         out[k] = s;
     }
 }
 
-// Rows held in registers, one after the other into the same slots. Rows above a wavefront meet in a barrier between two rows' additions
+// Rows held in registers, one after the other into the same places. Rows above a wavefront meet in a barrier between two rows' additions
 // (the fold); rows within one are kept in order by the fence.
 template <class T, int NC, bool AL>
 __global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
-    extern __shared__ float slots[];  // [rows side by side, distances]
+    extern __shared__ float places[];  // [rows side by side, distances]
     __shared__ float sums[2 * 16];
     int turn = 0;
     const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
-    const int far = a.buckets.far, right = right_of(a.buckets), n = slots_of(a.buckets);
+    const int far = a.buckets.far, right = right_of(a.buckets), n = places_of(a.buckets);
     const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
         const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
         float left_end = 0.0f, right_end = 0.0f;
         __syncthreads();  // (the item before has left its sums)
-        for (int i = threadIdx.x; i < n * rpb; i += blockDim.x) slots[i] = 0.0f;
+        for (int i = threadIdx.x; i < n * rpb; i += blockDim.x) places[i] = 0.0f;
         __syncthreads();
         for (int64_t first = q0; first < q1; first += rpb) {
             const int64_t q = first + ty, row = matrix * a.queries + q;
             const int live = q < q1 ? live_keys(a, matrix, q) : 0, pos = position(a.offset, q);
             const T *p = (const T*)a.p + row * a.keys, *g = (const T*)a.g + row * a.keys;
-            float pv[NC][VEC], gv[NC][VEC];
+            Pack<T, VEC> pp[NC], gp[NC];
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                At at(lane + k * tpr, a.keys);
+                if (at.s + at.lo >= live) at.lo = VEC;  // (nothing of it is live: not read)
+                pp[k] = load_slot<T, AL>(p, at);
+                gp[k] = load_slot<T, AL>(g, at);
+            }
             float s[1] = {0.0f};
-            {
-                Pack<T, VEC> pp[NC], gp[NC];
 #pragma unroll
-                for (int k = 0; k < NC; ++k) {
-                    At at(lane + k * tpr, a.keys);
-                    if (at.s + at.lo >= live) at.lo = VEC;
-                    pp[k] = load_slot<T, AL>(p, at);
-                    gp[k] = load_slot<T, AL>(g, at);
-                }
-#pragma unroll
-                for (int k = 0; k < NC; ++k) {
-                    const At at(lane + k * tpr, a.keys);
+            for (int k = 0; k < NC; ++k) {
+                const At at(lane + k * tpr, a.keys);
+                if (at.s + VEC > live) {  // the last live vector: hidden elements become zeros
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const bool on = at.s + i < live;
-                        pv[k][i] = on ? Elem<T>::widen(pp[k].v[i]) : 0.0f;
-                        gv[k][i] = on ? Elem<T>::widen(gp[k].v[i]) : 0.0f;
-                        s[0] = fmaf(pv[k][i], gv[k][i], s[0]);
+                        if (at.s + i >= live) pp[k].v[i] = gp[k].v[i] = Elem<T>::narrow(0.0f);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[0] = fmaf(Elem<T>::widen(pp[k].v[i]), Elem<T>::widen(gp[k].v[i]), s[0]);
             }
             fold_row<SumF>(s, tpr, sums, turn);
+            const bool finite = fabsf(s[0]) < __builtin_huge_valf();
             T* out = (T*)a.out + row * a.keys;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -391,16 +409,19 @@ __global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
                 float d[VEC];
                 Pack<T, VEC> o;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    d[i] = i >= at.lo && at.s + i < live ? pv[k][i] * (gv[k][i] - s[0]) : 0.0f;
-                    o.v[i] = Elem<T>::narrow(a.scale * d[i]);
+                for (int i = 0; i < VEC; ++i) d[i] = Elem<T>::widen(pp[k].v[i]) * (Elem<T>::widen(gp[k].v[i]) - s[0]);
+                if (!finite) {  // (0 * (0 - s) would be NaN in hidden places)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) d[i] = i >= at.lo && at.s + i < live ? d[i] : 0.0f;
                 }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(a.scale * d[i]);
                 if (q < q1) store_slot<T, VEC, AL>(out, at, o);
-                if (a.table_grad && at.s + at.lo < live) add_by_distance<VEC>(d, at.s, at.lo, live, pos, far, right, slots + ty * n, left_end, right_end);
+                if (a.table_grad && at.s + at.lo < live) add_by_distance<VEC>(d, at.s, pos, far, right, places + ty * n, left_end, right_end);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    if (a.table_grad) leave_buckets(a.buckets, slots, rpb, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+        }
+        if (a.table_grad) leave_buckets(a.buckets, places, rpb, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
     }
 }
 
@@ -408,17 +429,17 @@ __global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
 template <class T>
 __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
-    extern __shared__ float slots[];
+    extern __shared__ float places[];
     __shared__ float sums[2 * 16];
     int turn = 0;
-    const int far = a.buckets.far, right = right_of(a.buckets), n = slots_of(a.buckets), vecs = (a.keys + VEC - 1) / VEC;
+    const int far = a.buckets.far, right = right_of(a.buckets), n = places_of(a.buckets), vecs = (a.keys + VEC - 1) / VEC;
     const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
         const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
         float left_end = 0.0f, right_end = 0.0f;
         __syncthreads();  // (the item before has left its sums)
-        for (int i = threadIdx.x; i < n; i += 1024) slots[i] = 0.0f;
+        for (int i = threadIdx.x; i < n; i += 1024) places[i] = 0.0f;
         __syncthreads();
         for (int64_t q = q0; q < q1; ++q) {
             const int64_t row = matrix * a.queries + q;
@@ -443,12 +464,12 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
                         d[i] = v * VEC + i < live ? Elem<T>::widen(pp.v[i]) * (Elem<T>::widen(gp.v[i]) - s[0]) : 0.0f;
                         o.v[i] = Elem<T>::narrow(a.scale * d[i]);
                     }
-                    if (a.table_grad) add_by_distance<VEC>(d, v * VEC, 0, live, pos, far, right, slots, left_end, right_end);
+                    if (a.table_grad) add_by_distance<VEC>(d, v * VEC, pos, far, right, places, left_end, right_end);
                 }
                 store_sweep_vec<T, VEC>((T*)a.out + row * a.keys, v, a.keys, o);
             }
-    }
-    if (a.table_grad) leave_buckets(a.buckets, slots, 1, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+        }
+        if (a.table_grad) leave_buckets(a.buckets, places, 1, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
     }
 }
 
@@ -466,7 +487,7 @@ __global__ __launch_bounds__(256) void bias_grad_table_kernel(const float* parti
 
 bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-size_t bias_lds(const Buckets& b) { return (size_t)(b.far + (b.both ? b.far : 0) + 1) * 4; }
+size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
 
 // A workgroup holds rows of one matrix: where that has few (a step of decoding has one), down to a wavefront.
 RowDeal deal_keys(int dtype, int64_t queries, int64_t keys, int most) {

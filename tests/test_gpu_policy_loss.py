@@ -174,6 +174,26 @@ def test_nothing_counts(hpt, dev):
 
 
 @pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("cols", [3, 50, 40000])
+def test_the_lowest_value_as_a_mask(hpt, dev, name, cols):
+    """Logits that a caller has masked with the type's lowest value, all of a row among them, and their mirror."""
+    k, rng = Kind(hpt, name), np.random.default_rng(3)
+    low = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": -3.3895313892515355e38}[name]
+    x = rng.standard_normal((5, cols))
+    x[0] = low
+    x[1, 1:] = low
+    x[2] = -low
+    x[3, 1] = low / 1.3
+    x[3, 2:] = low
+    x[3, 0] = low
+    t, x = k.up(x)
+    token = np.array([1, 0, 2, 1, 2])
+    logp, lse = (v.numpy().astype(np.float64) for v in t.token_logp(up(hpt, token)))
+    near(logp, [-np.log(cols), 0, -np.log(cols), 0, x[4, 2] - logsumexp(x[4])], LSE + F32_STEP * 12)
+    near(lse, logsumexp(x), LSE + F32_STEP * np.abs(logsumexp(x)))
+
+
+@pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("cols", [50, 40000])
 def test_infinities_and_nan(hpt, dev, name, cols):
     k, rng = Kind(hpt, name), np.random.default_rng(3)
