@@ -1379,7 +1379,10 @@ int32_t hpt_hip_softmax_bias(int32_t dev, void* stream, const hpt_view* in, doub
                              const hpt_view* workspace, hpt_view* out) {
     return guarded([&] {
         const Scores s = scores_of(in, "softmax_bias input");
-        const RowsOf r = rows_of(in, 1, "softmax_bias input");
+        (void)rows_of(in, 1, "softmax_bias input");  // (keys side by side, fewer than 2^29)
+        hpt_view heads = *in;
+        heads.ndim = in->ndim - 2;
+        const RowsOf r = rows_of(&heads, 0, "softmax_bias input");
         BiasArgs a{};
         a.scale = check_bias_scale(scale, query_offset, "softmax_bias");
         check_view(table, "softmax_bias table", true);
@@ -1400,7 +1403,8 @@ int32_t hpt_hip_softmax_bias(int32_t dev, void* stream, const hpt_view* in, doub
         }
         if (view_size(in) == 0) return;
         a.x = in->data;
-        a.kept = r.kept;
+        a.matrices = r.kept;
+        a.query_stride = in->strides[in->ndim - 2];
         a.table = table->data;
         a.table_bucket = table->strides[0];
         a.table_head = table->strides[1];

@@ -99,7 +99,8 @@ Buckets make_buckets(int64_t total, bool both, int64_t max_distance);
 
 struct BiasArgs {
     const void* x;        // [batch, heads, queries, keys], keys side by side
-    Dims kept;
+    Dims matrices;        // where each head's rows start
+    int64_t query_stride;
     const void* table;    // [buckets, heads]
     int64_t table_bucket, table_head;  // its strides
     void* out;

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
             Pack<T, VEC> p[B];
 #pragma unroll
             for (int b = 0; b < B; ++b) {
-                if (v + b * 256 < vecs) p[b] = load_pack_stream<T, VEC>(body + (int64_t)(v + b * 256) * VEC);
+                if (v + b * 256 < vecs) p[b] = load_pack<T, VEC>(body + (int64_t)(v + b * 256) * VEC);
                 else
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) p[b].v[i] = Elem<T>::narrow(-inf);
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256) void policy_grad_kernel(const PolicyGradArgs a
             if (w != 0.0f) p = load_pack_unaligned<T, VEC>(x + e);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) p.v[i] = grad(p.v[i], e + i);
-            store_pack<T, VEC>(out + e, p);
+            store_pack_stream<T, VEC>(out + e, p);
         }
     }
 }

@@ -58,25 +58,24 @@ constexpr int kPad = 8;
 __device__ __forceinline__ int right_of(const Buckets& b) { return b.both ? b.far : 0; }
 __host__ __device__ inline int places_of(const Buckets& b) { return b.far + (b.both ? b.far : 0) + 1 + 2 * kPad; }
 
-// A row's last key, exclusive.
-template <class A> __device__ __forceinline__ int live_keys(const A& a, int64_t matrix, int64_t q) {
-    int64_t n = a.keys;
-    if (a.lengths) {
-        const int64_t b = matrix / a.heads;
-        const int64_t len = a.lengths64 ? ((const int64_t*)a.lengths)[b] : (int64_t)((const int32_t*)a.lengths)[b];
-        n = len < n ? len : n;
+// What the rows of a matrix have in common: how many keys its sequence has, and the position of its query q0. Beyond +-2^29 every key is
+// far or hidden, as there are fewer than 2^29 of them.
+struct Place {
+    int length, pos;
+    template <class A> __device__ __forceinline__ Place(const A& a, int64_t matrix, int64_t q0) {
+        int64_t n = a.keys;
+        if (a.lengths) {
+            const int64_t b = matrix / a.heads;
+            const int64_t len = a.lengths64 ? ((const int64_t*)a.lengths)[b] : (int64_t)((const int32_t*)a.lengths)[b];
+            n = len < 0 ? 0 : len < n ? len : n;
+        }
+        length = (int)n;
+        const int64_t p = q0 + a.offset, most = 1 << 29;
+        pos = (int)(p > most ? most : p < -most ? -most : p);
     }
-    if (a.causal) {
-        const int64_t seen = q + a.offset + 1;
-        n = seen < n ? seen : n;
-    }
-    return n < 0 ? 0 : (int)n;
-}
-// A row's position as an int: beyond +-2^30 every key is far (there are fewer than 2^29 of them).
-__device__ __forceinline__ int position(int64_t offset, int64_t q) {
-    const int64_t p = q + offset, most = (1 << 30) - 1;
-    return (int)(p > most ? most : p < -most ? -most : p);
-}
+    // The end of the keys that query q0 + i sees.
+    __device__ __forceinline__ int live(int i, int causal) const { return causal ? max(min(length, pos + i + 1), 0) : length; }
+};
 
 template <class T> __device__ __forceinline__ void fill_bias(const BiasArgs& a, int64_t head, float* bias) {
     const int n = places_of(a.buckets), right = right_of(a.buckets);
@@ -108,9 +107,10 @@ __device__ __forceinline__ void biased(const Pack<T, VEC>& p, int e, int lo, int
     }
 }
 
-// Rows held in registers. An item is `per_item` rows of one matrix; the first row is on its way while the bias comes together.
+// Rows held in registers. An item is `per_item` rows of one matrix; the first row is on its way while the bias comes together, every other
+// one while the row before it is summed and written.
 template <class T, int NC, bool AL>
-__global__ __launch_bounds__(1024) void bias_row_kernel(const BiasArgs a) {
+__global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_row_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
     extern __shared__ float bias[];
@@ -121,14 +121,14 @@ __global__ __launch_bounds__(1024) void bias_row_kernel(const BiasArgs a) {
     const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
-        const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
+        const int n = (int)min((int64_t)a.per_item, a.queries - q0);  // rows
+        const Place place(a, matrix, q0);
+        const T* x0 = (const T*)a.x + offset_of(a.matrices, matrix) + q0 * a.query_stride;
+        T* out0 = (T*)a.out + (matrix * a.queries + q0) * a.keys;
         Pack<T, VEC> p[NC];
-        int live = 0;
-        auto fetch = [&](int64_t q) {
-            const bool there = q < q1;
-            live = there ? live_keys(a, matrix, q) : 0;
-            const int64_t row = matrix * a.queries + q;
-            const T* x = (const T*)a.x + (there ? offset_of(a.kept, row) : 0);
+        auto fetch = [&](int i) {
+            const int live = i < n ? place.live(i, a.causal) : 0;
+            const T* x = x0 + i * a.query_stride;
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
                 At at(lane + k * tpr, a.keys);
@@ -136,14 +136,13 @@ __global__ __launch_bounds__(1024) void bias_row_kernel(const BiasArgs a) {
                 p[k] = load_slot<T, AL>(x, at);
             }
         };
-        fetch(q0 + ty);
+        fetch(ty);
         __syncthreads();  // (the bias of the item before is no longer read)
         fill_bias<T>(a, matrix % a.heads, bias);
         __syncthreads();
-        for (int64_t first = q0; first < q1; first += rpb) {
-            const int64_t q = first + ty;
-            if (first != q0) fetch(q);
-            const int pos = position(a.offset, q);
+        for (int first = 0; first < n; first += rpb) {
+            const int i = first + ty;
+            const int live = i < n ? place.live(i, a.causal) : 0, pos = place.pos + i;
             float s[NC][VEC];
             float m[1] = {-__builtin_huge_valf()};
 #pragma unroll
@@ -151,39 +150,50 @@ __global__ __launch_bounds__(1024) void bias_row_kernel(const BiasArgs a) {
                 const At at(lane + k * tpr, a.keys);
                 biased<T, VEC>(p[k], at.s, at.lo, live, pos, a.scale, far, right, bias, s[k]);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) m[0] = fmaxf(m[0], s[k][i]);
+                for (int j = 0; j < VEC; ++j) m[0] = fmaxf(m[0], s[k][j]);
             }
+            if (first + rpb < n) fetch(i + rpb);
             fold_row<MaxF>(m, tpr, most, turn_m);
             // (a hidden place is -inf and its exponential 0: in a row of nothing else, too)
             const float base = m[0] == -__builtin_huge_valf() ? 0.0f : m[0];
             float t[1] = {0.0f};
             // (two-byte types: one multiply-add makes the hardware's argument; what rounding base * log2 e costs is in every term and in their
             // sum alike. It would overflow next to the type's lowest value, with which callers mask.)
-            constexpr float kLog2e = 1.44269504f;
-            const bool direct = sizeof(T) == 2 && fabsf(base) < 1e38f;
-            const float shift = -base * kLog2e;
+            if (sizeof(T) == 2 && fabsf(base) < 1e38f) {
+                constexpr float kLog2e = 1.44269504f;
+                const float shift = -base * kLog2e;
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
+                for (int k = 0; k < NC; ++k) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    s[k][i] = direct ? __builtin_amdgcn_exp2f(fmaf(s[k][i], kLog2e, shift)) : exp_row<T>(s[k][i] - base);
-                    t[0] += s[k][i];
+                    for (int j = 0; j < VEC; ++j) {
+                        s[k][j] = __builtin_amdgcn_exp2f(fmaf(s[k][j], kLog2e, shift));
+                        t[0] += s[k][j];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        s[k][j] = exp_row<T>(s[k][j] - base);
+                        t[0] += s[k][j];
+                    }
                 }
             }
             fold_row<SumF>(t, tpr, sums, turn_s);
             const float inv = live ? 1.0f / t[0] : 0.0f;
             const bool number = t[0] > 0.0f || !live;
-            if (q < q1) {
-                T* out = (T*)a.out + (matrix * a.queries + q) * a.keys;
+            if (i < n) {
+                T* out = out0 + (int64_t)i * a.keys;
 #pragma unroll
                 for (int k = 0; k < NC; ++k) {
                     const At at(lane + k * tpr, a.keys);
                     Pack<T, VEC> o;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(s[k][i] * inv);
-                    if (!number) {  // keys of -inf alone, or a NaN or +inf among them: the hidden ones are zeros all the same
+                    for (int j = 0; j < VEC; ++j) o.v[j] = Elem<T>::narrow(s[k][j] * inv);
+                    if (__any(!number)) {  // keys of -inf alone, or a NaN or +inf among them: the hidden ones are zeros all the same
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(at.s + i < live ? __builtin_nanf("") : 0.0f);
+                        for (int j = 0; j < VEC; ++j) o.v[j] = number ? o.v[j] : Elem<T>::narrow(at.s + j < live ? __builtin_nanf("") : 0.0f);
                     }
                     store_slot<T, VEC, AL>(out, at, o);
                 }
@@ -254,17 +264,18 @@ template <class T>
 __global__ __launch_bounds__(1024) void bias_stream_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     extern __shared__ float bias[];
-    __shared__ float place[32];
+    __shared__ float fold[32];
     const int vecs = (a.keys + VEC - 1) / VEC;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t matrix = row / a.queries, q = row % a.queries;
         __syncthreads();
         fill_bias<T>(a, matrix % a.heads, bias);
         __syncthreads();
-        const int live = live_keys(a, matrix, q), pos = position(a.offset, q);
-        const T* x = (const T*)a.x + offset_of(a.kept, row);
+        const Place place(a, matrix, q);
+        const int live = place.live(0, a.causal), pos = place.pos;
+        const T* x = (const T*)a.x + offset_of(a.matrices, matrix) + q * a.query_stride;
         float m, s;
-        sweep_stats<T>(a, x, 0, vecs, live, pos, bias, place, m, s);
+        sweep_stats<T>(a, x, 0, vecs, live, pos, bias, fold, m, s);
         sweep_apply<T>(a, x, (T*)a.out + row * a.keys, 0, vecs, live, pos, bias, m, s);
     }
 }
@@ -274,18 +285,19 @@ template <class T, bool APPLY>
 __global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     extern __shared__ float bias[];
-    __shared__ float place[8];
+    __shared__ float fold[8];
     const int64_t row = blockIdx.x / a.split, matrix = row / a.queries, q = row % a.queries;
     const int part = blockIdx.x % a.split;
     const int vecs = (a.keys + VEC - 1) / VEC, each = (vecs + a.split - 1) / a.split;
     const int v0 = min(part * each, vecs), v1 = min(v0 + each, vecs);
     fill_bias<T>(a, matrix % a.heads, bias);
     __syncthreads();
-    const int live = live_keys(a, matrix, q), pos = position(a.offset, q);
-    const T* x = (const T*)a.x + offset_of(a.kept, row);
+    const Place place(a, matrix, q);
+    const int live = place.live(0, a.causal), pos = place.pos;
+    const T* x = (const T*)a.x + offset_of(a.matrices, matrix) + q * a.query_stride;
     float m, s;
     if constexpr (!APPLY) {
-        sweep_stats<T>(a, x, v0, v1, live, pos, bias, place, m, s);
+        sweep_stats<T>(a, x, v0, v1, live, pos, bias, fold, m, s);
         if (threadIdx.x == 0) {
             a.partial[2 * (row * a.split + part)] = m;
             a.partial[2 * (row * a.split + part) + 1] = s;
@@ -358,27 +370,25 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, i
 // Rows held in registers, one after the other into the same places. Rows above a wavefront meet in a barrier between two rows' additions
 // (the fold); rows within one are kept in order by the fence.
 template <class T, int NC, bool AL>
-__global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
+__global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_grad_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
     extern __shared__ float places[];  // [rows side by side, distances]
     __shared__ float sums[2 * 16];
     int turn = 0;
     const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
-    const int far = a.buckets.far, right = right_of(a.buckets), n = places_of(a.buckets);
+    const int far = a.buckets.far, right = right_of(a.buckets), each = places_of(a.buckets);
     const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
-        const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
+        const int n = (int)min((int64_t)a.per_item, a.queries - q0);  // rows
+        const Place place(a, matrix, q0);
+        const int64_t at0 = (matrix * a.queries + q0) * a.keys;
         float left_end = 0.0f, right_end = 0.0f;
-        __syncthreads();  // (the item before has left its sums)
-        for (int i = threadIdx.x; i < n * rpb; i += blockDim.x) places[i] = 0.0f;
-        __syncthreads();
-        for (int64_t first = q0; first < q1; first += rpb) {
-            const int64_t q = first + ty, row = matrix * a.queries + q;
-            const int live = q < q1 ? live_keys(a, matrix, q) : 0, pos = position(a.offset, q);
-            const T *p = (const T*)a.p + row * a.keys, *g = (const T*)a.g + row * a.keys;
-            Pack<T, VEC> pp[NC], gp[NC];
+        Pack<T, VEC> pp[NC], gp[NC];
+        auto fetch = [&](int i) {
+            const int live = i < n ? place.live(i, a.causal) : 0;
+            const T *p = (const T*)a.p + at0 + (int64_t)i * a.keys, *g = (const T*)a.g + at0 + (int64_t)i * a.keys;
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
                 At at(lane + k * tpr, a.keys);
@@ -386,22 +396,30 @@ __global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
                 pp[k] = load_slot<T, AL>(p, at);
                 gp[k] = load_slot<T, AL>(g, at);
             }
+        };
+        __syncthreads();  // (the item before has left its sums)
+        for (int i = threadIdx.x; i < each * rpb; i += blockDim.x) places[i] = 0.0f;
+        __syncthreads();
+        for (int first = 0; first < n; first += rpb) {
+            const int i = first + ty;
+            const int live = i < n ? place.live(i, a.causal) : 0, pos = place.pos + i;
+            fetch(i);
             float s[1] = {0.0f};
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
                 const At at(lane + k * tpr, a.keys);
                 if (at.s + VEC > live) {  // the last live vector: hidden elements become zeros
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        if (at.s + i >= live) pp[k].v[i] = gp[k].v[i] = Elem<T>::narrow(0.0f);
+                    for (int j = 0; j < VEC; ++j) {
+                        if (at.s + j >= live) pp[k].v[j] = gp[k].v[j] = Elem<T>::narrow(0.0f);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) s[0] = fmaf(Elem<T>::widen(pp[k].v[i]), Elem<T>::widen(gp[k].v[i]), s[0]);
+                for (int j = 0; j < VEC; ++j) s[0] = fmaf(Elem<T>::widen(pp[k].v[j]), Elem<T>::widen(gp[k].v[j]), s[0]);
             }
             fold_row<SumF>(s, tpr, sums, turn);
             const bool finite = fabsf(s[0]) < __builtin_huge_valf();
-            T* out = (T*)a.out + row * a.keys;
+            T* out = (T*)a.out + at0 + (int64_t)i * a.keys;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
@@ -409,15 +427,15 @@ __global__ __launch_bounds__(1024) void bias_grad_kernel(const BiasGradArgs a) {
                 float d[VEC];
                 Pack<T, VEC> o;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) d[i] = Elem<T>::widen(pp[k].v[i]) * (Elem<T>::widen(gp[k].v[i]) - s[0]);
-                if (!finite) {  // (0 * (0 - s) would be NaN in hidden places)
+                for (int j = 0; j < VEC; ++j) d[j] = Elem<T>::widen(pp[k].v[j]) * (Elem<T>::widen(gp[k].v[j]) - s[0]);
+                if (__any(!finite)) {  // (0 * (0 - s) would be NaN in hidden places)
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) d[i] = i >= at.lo && at.s + i < live ? d[i] : 0.0f;
+                    for (int j = 0; j < VEC; ++j) d[j] = finite || (j >= at.lo && at.s + j < live) ? d[j] : 0.0f;
                 }
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) o.v[i] = Elem<T>::narrow(a.scale * d[i]);
-                if (q < q1) store_slot<T, VEC, AL>(out, at, o);
-                if (a.table_grad && at.s + at.lo < live) add_by_distance<VEC>(d, at.s, pos, far, right, places + ty * n, left_end, right_end);
+                for (int j = 0; j < VEC; ++j) o.v[j] = Elem<T>::narrow(a.scale * d[j]);
+                if (i < n) store_slot<T, VEC, AL>(out, at, o);
+                if (a.table_grad && at.s + at.lo < live) add_by_distance<VEC>(d, at.s, pos, far, right, places + ty * each, left_end, right_end);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
@@ -443,7 +461,8 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
         __syncthreads();
         for (int64_t q = q0; q < q1; ++q) {
             const int64_t row = matrix * a.queries + q;
-            const int live = live_keys(a, matrix, q), pos = position(a.offset, q);
+            const Place place(a, matrix, q);
+            const int live = place.live(0, a.causal), pos = place.pos;
             const T *p = (const T*)a.p + row * a.keys, *g = (const T*)a.g + row * a.keys;
             float s[1] = {0.0f};
             for (int v = threadIdx.x; v * VEC < live; v += 1024) {
@@ -528,8 +547,8 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
             const int64_t rounds = std::max<int64_t>(1, std::min<int64_t>(a.rows / 2048 / rpb, 64 / rpb));
             a.per_item = (int)(rounds * rpb);
             const int64_t items = matrices * ((a.queries + a.per_item - 1) / a.per_item);
-            bool al = a.keys % VEC == 0 && on_grid(a.x) && on_grid(a.out);
-            for (int i = 0; i < a.kept.n; ++i) al = al && (a.kept.size[i] == 1 || a.kept.stride[i] % VEC == 0);
+            bool al = a.keys % VEC == 0 && on_grid(a.x) && on_grid(a.out) && (a.queries == 1 || a.query_stride % VEC == 0);
+            for (int i = 0; i < a.matrices.n; ++i) al = al && (a.matrices.size[i] == 1 || a.matrices.stride[i] % VEC == 0);
             const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 20);
             HPT_WITH_NC(d.nc, {
                 if (al) bias_row_kernel<T, NC, true><<<grid, d.threads, lds, st>>>(a);
