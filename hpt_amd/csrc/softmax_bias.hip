@@ -42,15 +42,13 @@ Buckets make_buckets(int64_t total, bool both, int64_t max_distance) {
 
 namespace {
 
+// (Counted along `begin`, which every lane reads at the same place: a search would wait for one load after the other.)
 __device__ __forceinline__ int bucket_of(const Buckets& b, int d) {
-    const int far = d < 0 ? -d : b.both ? d : 0;
-    int lo = 0, hi = b.n - 1;  // the last bucket that begins at `far` or before
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((int)b.begin[mid] <= far) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo + (d > 0 && b.both ? b.n : 0);
+    const int far = d < 0 ? -d : b.both ? d : 0, half = b.n / 2;
+    int k = min(far, half);
+#pragma unroll 4
+    for (int j = half + 1; j < b.n; ++j) k += (int)b.begin[j] <= far;
+    return k + (d > 0 && b.both ? b.n : 0);
 }
 // Places by distance in LDS: -far ... right, and a vector's length more on both sides, so that a vector that reaches into the range, from
 // either side, has all its places there. Where keys ahead of the query share bucket 0, one place is enough for them and for distance 0.
@@ -332,38 +330,29 @@ __device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, in
     }
 }
 
-// The workgroup's sums by distance -> by bucket, into its row of partial sums. `places`: one array of them for each of `groups` rows that
-// run side by side. Every thread of the workgroup comes here.
-__device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, int groups, float left_end, float right_end, float* out) {
+// The workgroup's sums by distance -> by bucket, into its row of partial sums; eight lanes share a bucket. `places`: one array of them for each
+// of `groups` rows that run side by side. Every thread of the workgroup comes here.
+__device__ __forceinline__ void leave_buckets(const Buckets& b, const float* places, int groups, float left_end, float right_end, float* out) {
     __shared__ float ends[2 * 16 * 2];
-    const int n = places_of(b), total = b.both ? 2 * b.n : b.n;
+    const int n = places_of(b), total = b.both ? 2 * b.n : b.n, zero = b.far + kPad;
     float e[2] = {left_end, right_end};
     int turn = 0;
     fold_row<SumF>(e, blockDim.x, ends, turn);
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        float s = places[i];
-        for (int g = 1; g < groups; ++g) s += places[g * n + i];
-        places[i] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {  // distance -far and beyond, `right` and beyond
-        for (int i = 0; i <= kPad; ++i) e[0] += places[i];
-        for (int i = 0; i <= kPad; ++i) e[1] += places[n - 1 - i];
-        places[kPad] = e[0];
-        places[n - 1 - kPad] = e[1];
-    }
-    __syncthreads();
-    for (int k = threadIdx.x; k < total; k += blockDim.x) {
+    __syncthreads();  // (a single wavefront has passed none in the fold)
+    const int part = threadIdx.x & 7;
+    for (int k = threadIdx.x >> 3; k < total; k += blockDim.x >> 3) {
         const bool ahead = b.both && k >= b.n;
         const int j = ahead ? k - b.n : k;
-        const int from = b.begin[j], to = j + 1 < b.n ? b.begin[j + 1] : b.far + 1;  // distances of bucket k
-        float s = 0.0f;
-        for (int d = from; d < to; ++d) {
-            if (ahead && d == 0) continue;  // (distance 0 is the other direction's)
-            s += places[(ahead ? d : -d) + b.far + kPad];
+        // distances of bucket k: of its direction's last one also those of the margin; bucket 0 of a single direction has the other's margin
+        const int from = ahead && j == 0 ? 1 : !b.both && j == 0 ? -kPad : b.begin[j], to = j + 1 < b.n ? b.begin[j + 1] : b.far + kPad + 1;
+        float s = part == 0 && j == b.n - 1 ? e[ahead] : 0.0f;
+        if (part == 0 && !b.both && j == 0) s += e[1];
+        for (int d = from + part; d < to; d += 8) {
+            const float* at = places + (ahead ? zero + d : zero - d);
+            for (int g = 0; g < groups; ++g) s += at[g * n];
         }
-        out[k] = s;
+        s = group_reduce<SumF>(s, 8);
+        if (part == 0) out[k] = s;
     }
 }
 
@@ -543,8 +532,9 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
         } else {
             a.tpr = d.tpr;
             const int rpb = d.rows_per_block();
-            // items enough for eight workgroups per compute unit, of up to 64 rows
-            const int64_t rounds = std::max<int64_t>(1, std::min<int64_t>(a.rows / 2048 / rpb, 64 / rpb));
+            // items for sixteen workgroups per compute unit, of up to 64 rows each: bf16 [8, 16, 1024, 1024] 110 us with half as many (their last round
+            // is a third full), 102 with this many and with twice as many, 112 with four times (each needs the bias in LDS first)
+            const int64_t rounds = std::max<int64_t>(1, std::min<int64_t>(a.rows / 4096 / rpb, 64 / rpb));
             a.per_item = (int)(rounds * rpb);
             const int64_t items = matrices * ((a.queries + a.per_item - 1) / a.per_item);
             bool al = a.keys % VEC == 0 && on_grid(a.x) && on_grid(a.out) && (a.queries == 1 || a.query_stride % VEC == 0);
@@ -561,7 +551,9 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
 int64_t bias_grad_items(int dtype, int64_t matrices, int64_t queries, int64_t keys, int* per_item) {
     const RowDeal d = bias_grad_deal(dtype, queries, keys);
     const int64_t rpb = d.rows_per_block();
-    const int64_t rounds = std::max<int64_t>({1, std::min<int64_t>(matrices * queries / 2048 / rpb, 64 / rpb)});
+    // sixteen workgroups per compute unit, of up to 64 rows each: bf16 [4, 16, 1024, 1024], causal, 87 us with half as many, 75 with this many, 84
+    // with twice as many (each clears its places and leaves its sums)
+    const int64_t rounds = std::max<int64_t>({1, std::min<int64_t>(matrices * queries / 4096 / rpb, 64 / rpb)});
     *per_item = (int)(rounds * rpb);
     return matrices * ((queries + *per_item - 1) / *per_item);
 }
