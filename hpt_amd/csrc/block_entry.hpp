@@ -116,6 +116,7 @@ struct BiasArgs {
     Buckets buckets;
     int tpr;
     int per_item;         // rows of one matrix that a workgroup takes
+    int64_t chunks, items;  // such items: of a matrix, of all
     int split;            // > 1: workgroups that share a row
 };
 
@@ -139,6 +140,7 @@ struct BiasGradArgs {
     Buckets buckets;
     int tpr;
     int per_item;
+    int64_t chunks, items;
 };
 
 // Rows of one matrix that a workgroup takes, and the number of such items.

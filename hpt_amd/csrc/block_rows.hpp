@@ -7,6 +7,13 @@
 
 namespace hpt {
 
+// a / b of numbers that are not negative: in 32 bits where both fit (a 64-bit division is some hundred instructions, and small launches wait
+// for several of them before their first load).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((uint64_t)(a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
+}
+
 struct SumF {
     __device__ static __forceinline__ float comb(float a, float b) { return a + b; }
 };

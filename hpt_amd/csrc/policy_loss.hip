@@ -28,13 +28,6 @@ __device__ __forceinline__ void meet(float& m, double& s, float m2, double s2) {
     s = s * (double)(m == n ? 1.0f : __builtin_amdgcn_exp2f(m - n)) + s2 * (double)(m2 == n ? 1.0f : __builtin_amdgcn_exp2f(m2 - n));
     m = n;
 }
-// (maximum, sum of exponentials below it) of two parts of a row.
-__device__ __forceinline__ void join(double& m, double& s, double m2, double s2) {
-    const double n = fmax(m, m2);
-    s = s * (m == n ? 1.0 : exp(m - n)) + s2 * (m2 == n ? 1.0 : exp(m2 - n));
-    m = n;
-}
-
 __device__ __forceinline__ int64_t token_of(const void* token, int is64, int64_t row) {
     return is64 ? ((const int64_t*)token)[row] : (int64_t)((const int32_t*)token)[row];
 }
@@ -43,25 +36,38 @@ __device__ __forceinline__ float mask_of(const PolicyArgs& a, int64_t row) {
     return a.mask_bool ? (((const uint8_t*)a.mask)[row] ? 1.0f : 0.0f) : ((const float*)a.mask)[row];
 }
 
-// A row's results from its maximum, sum and token. A token outside the row has no probability: everything of it is NaN.
-template <class T> __device__ __forceinline__ void finish_row(const PolicyArgs& a, int64_t row, float mask, double m, double s) {
-    const int64_t t = token_of(a.token, a.token64, row);
-    float xt = __builtin_nanf("");
-    if (t >= 0 && t < a.cols) xt = Elem<T>::widen(((const T*)a.x + offset_of(a.kept, row))[t]);
+// What a token brings along: read together, so that one latency covers all but the logit itself.
+struct Token {
+    int64_t id;
+    float old, advantage, reference;
+    __device__ __forceinline__ Token(const PolicyArgs& a, int64_t row) {
+        id = token_of(a.token, a.token64, row);
+        old = a.old_logp ? a.old_logp[row] : 0.0f;
+        advantage = a.old_logp ? a.advantage[row] : 0.0f;
+        reference = a.reference ? a.reference[row] : 0.0f;
+    }
+};
+// The token's logit; NaN for a token outside the row.
+template <class T> __device__ __forceinline__ float logit_of(const PolicyArgs& a, int64_t row, int64_t token) {
+    return token >= 0 && token < a.cols ? Elem<T>::widen(((const T*)a.x + offset_of(a.kept, row))[token]) : __builtin_nanf("");
+}
+
+// A row's results from its maximum, sum and token.
+__device__ __forceinline__ void finish_row(const PolicyArgs& a, int64_t row, float mask, const Token& t, float xt, double m, double s) {
     const double rest = log(s), lse = m + rest;
     const double logp = ((double)xt - m) - rest;  // (exact differences first: m may be a type's lowest value)
     a.logp[row] = (float)logp;
     a.lse[row] = (float)lse;
     if (!a.old_logp) return;
-    const double adv = a.advantage[row], ratio = exp(logp - (double)a.old_logp[row]);
+    const double adv = t.advantage, ratio = exp(logp - (double)t.old);
     const double low = 1.0 - a.clip_low, high = 1.0 + a.clip_high;
     const double free = ratio * adv, held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
     double loss = free <= held ? -free : -held, slope = free <= held ? -free : 0.0;
     if (free != free || held != held) loss = slope = free + held;  // (a NaN is no side of the minimum)
     if (a.reference) {
-        const double k = (double)a.reference[row] - logp;
-        loss += a.kl_weight * (exp(k) - k - 1.0);
-        slope += a.kl_weight * (1.0 - exp(k));
+        const double k = (double)t.reference - logp, e = exp(k);
+        loss += a.kl_weight * (e - k - 1.0);
+        slope += a.kl_weight * (1.0 - e);
     }
     a.each[row] = loss * mask;
     a.weight[row] = (float)(slope * mask);  // (over the sum of the mask: in the last launch)
@@ -84,8 +90,8 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
     __shared__ double sums[4];
     const float inf = __builtin_huge_valf();
     for (int64_t at = blockIdx.x; at < a.rows * a.split; at += gridDim.x) {
-        const int64_t row = at / a.split;
-        const int part = (int)(at % a.split);
+        const int64_t row = quotient(at, a.split);
+        const int part = (int)(at - row * a.split);
         const float mask = mask_of(a, row);
         if (mask == 0.0f) {
             if (threadIdx.x == 0 && a.split == 1) skip_row(a, row);
@@ -170,7 +176,8 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
         }
         if (threadIdx.x == 0) {
             if (a.split == 1) {
-                finish_row<T>(a, row, mask, top, sd);
+                const Token t(a, row);
+                finish_row(a, row, mask, t, logit_of<T>(a, row, t.id), top, sd);
             } else {
                 a.partial[2 * at] = top;
                 a.partial[2 * at + 1] = sd;
@@ -179,16 +186,22 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
     }
 }
 
-// A split row from its parts.
+// A split row from its parts. The mask and what its token brings along are on their way together; a hidden row's logits are not read.
 template <class T> __device__ __forceinline__ void join_row(const PolicyArgs& a, int64_t row, float mask) {
+    const Token t(a, row);
     if (mask == 0.0f) {
         skip_row(a, row);
         return;
     }
+    const float xt = logit_of<T>(a, row, t.id);
     const double* p = a.partial + 2 * row * a.split;
-    double m = p[0], s = p[1];
-    for (int k = 1; k < a.split; ++k) join(m, s, p[2 * k], p[2 * k + 1]);
-    finish_row<T>(a, row, mask, m, s);
+    double m = p[0], s = 0.0;
+#pragma unroll 4
+    for (int k = 1; k < a.split; ++k) m = fmax(m, p[2 * k]);
+    // (equal infinities are no distance apart; a part of nothing is (-inf, 0))
+#pragma unroll 4
+    for (int k = 0; k < a.split; ++k) s += p[2 * k + 1] * (double)(p[2 * k] == m ? 1.0f : __expf((float)(p[2 * k] - m)));
+    finish_row(a, row, mask, t, xt, m, s);
 }
 template <class T>
 __global__ __launch_bounds__(64) void policy_rows_kernel(const PolicyArgs a) {
@@ -202,11 +215,13 @@ template <class T>
 __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
     __shared__ double place[2 * 16];
     double v[2] = {0.0, 0.0};
+    if (a.split > 1) {
+        for (int64_t row = threadIdx.x; row < a.rows; row += 1024) join_row<T>(a, row, mask_of(a, row));
+    }
+#pragma unroll 4
     for (int64_t row = threadIdx.x; row < a.rows; row += 1024) {
-        const float m = mask_of(a, row);
-        if (a.split > 1) join_row<T>(a, row, m);
         v[0] += a.each[row];
-        v[1] += m;
+        v[1] += mask_of(a, row);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -222,6 +237,7 @@ __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
     }
     const double inv = count == 0.0 ? 0.0 : 1.0 / count;
     if (threadIdx.x == 0) a.loss[0] = (float)(loss * inv);
+#pragma unroll 4
     for (int64_t row = threadIdx.x; row < a.rows; row += 1024) a.weight[row] = (float)((double)a.weight[row] * inv);
 }
 
@@ -231,8 +247,8 @@ template <class T>
 __global__ __launch_bounds__(256) void policy_grad_kernel(const PolicyGradArgs a, int pieces, int each) {
     constexpr int VEC = 16 / sizeof(T);
     for (int64_t at = blockIdx.x; at < a.rows * pieces; at += gridDim.x) {
-        const int64_t row = at / pieces;
-        const int e0 = (int)(at % pieces) * each, n = min(each, a.cols - e0);
+        const int64_t row = quotient(at, pieces);
+        const int e0 = (int)(at - row * pieces) * each, n = min(each, a.cols - e0);
         T* out = (T*)a.out + row * a.cols + e0;
         const T* x = (const T*)a.x + offset_of(a.kept, row) + e0;
         const float w = a.weight[row] * a.upstream, lse = a.lse[row];

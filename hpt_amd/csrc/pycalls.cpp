@@ -15,7 +15,7 @@ namespace {
 constexpr int kRank = 32;
 constexpr size_t kAlign = 64;  // of every tensor's memory
 
-PyObject *s_ptr, *s_shape, *s_strides, *s_dtype, *s_code, *s_device;
+PyObject *s_ptr, *s_shape, *s_strides, *s_dtype, *s_code, *s_device, *s_backend, *s_hip, *s_storage, *s_pending;
 
 struct View {
     hpt_view v;
@@ -313,8 +313,33 @@ PyObject* py_softmax_causal(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- operators around a transformer's blocks: the caller brings the results -----------------------
 
-// Reads the arguments of a call one after the other. `ok` turns false where the caller has to go the long way; an exception of the
-// interpreter is left behind where a number is no number.
+// Whether a tensor is one of the device `dev`.
+bool lives_on(PyObject* t, int32_t dev) {
+    int64_t d;
+    PyObject* b = PyObject_GetAttr(t, s_backend);
+    if (!b) {
+        PyErr_Clear();
+        return false;
+    }
+    const bool hip = b == s_hip || (PyUnicode_Check(b) && PyUnicode_Compare(b, s_hip) == 0);
+    Py_DECREF(b);
+    return hip && integer(t, s_device, &d) && d == dev;
+}
+
+// Records in a tensor's storage that work on the stream uses it (what _touch does). False with an exception where that fails.
+bool touch(PyObject* t, PyObject* stream) {
+    PyObject* st = PyObject_GetAttr(t, s_storage);
+    if (!st) return false;
+    PyObject* pending = PyObject_GetAttr(st, s_pending);
+    Py_DECREF(st);
+    if (!pending) return false;
+    const bool ok = PySet_Add(pending, stream) == 0;
+    Py_DECREF(pending);
+    return ok;
+}
+
+// Reads the arguments of a call one after the other. `ok` turns false where the caller has to go the long way (which says what is wrong, if
+// anything is); an exception of the interpreter is left behind where a number is no number.
 struct Reader {
     PyObject* const* a;
     Py_ssize_t n, at = 0;
@@ -322,25 +347,28 @@ struct Reader {
     int32_t dev = 0;
     void* stream = nullptr;
     View views[12];
+    PyObject* tensors[12];
     int used = 0;
 
     Reader(PyObject* const* args, Py_ssize_t count) : a(args), n(count) {}
     PyObject* next() { return at < n ? a[at++] : (ok = false, Py_None); }
+    hpt_view* keep(PyObject* o, bool read) {
+        tensors[used] = o;
+        if (!read || !lives_on(o, dev)) ok = false;
+        return &views[used++].v;
+    }
     // the tensor that the call is made on, and its stream
     hpt_view* first() {
         uint64_t st = 0;
-        View* w = &views[used++];
-        if (n < 2 || !opening(a, w, &dev, &st)) ok = false;
+        const bool read = n >= 2 && opening(a, &views[0], &dev, &st);
         stream = (void*)(uintptr_t)st;
         at = 2;
-        return &w->v;
+        return keep(a[0], read);
     }
     hpt_view* view() {
         PyObject* o = next();
         if (!ok || o == Py_None) return nullptr;
-        View* w = &views[used++];
-        if (!view_of(o, w)) ok = false;
-        return &w->v;
+        return keep(o, view_of(o, &views[used]));
     }
     double number() {
         PyObject* o = next();
@@ -359,6 +387,13 @@ struct Reader {
         if (v != (int32_t)v) ok = false;
         return (int32_t)v;
     }
+    // The answer of a call that has been made: its status, the tensors' storage knowing of its work.
+    PyObject* answer(int32_t st) {
+        if (st == HPT_OK)
+            for (int i = 0; i < used; ++i)
+                if (!touch(tensors[i], a[1])) return nullptr;
+        return status(st);
+    }
 };
 
 // The status of a call through `CALL`, None where it is not taken.
@@ -372,7 +407,7 @@ struct Reader {
     Py_BEGIN_ALLOW_THREADS                             \
     st = CALL;                                         \
     Py_END_ALLOW_THREADS                               \
-    return status(st)
+    return r.answer(st)
 
 // rms_norm(tensor, stream, residual, normalized dims, gamma, eps, sum, out)
 PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -487,6 +522,10 @@ PyMODINIT_FUNC PyInit__calls(void) {
     s_dtype = PyUnicode_InternFromString("dtype");
     s_code = PyUnicode_InternFromString("code");
     s_device = PyUnicode_InternFromString("device");
-    if (!s_ptr || !s_shape || !s_strides || !s_dtype || !s_code || !s_device) return nullptr;
+    s_backend = PyUnicode_InternFromString("backend");
+    s_hip = PyUnicode_InternFromString("hip");
+    s_storage = PyUnicode_InternFromString("_storage");
+    s_pending = PyUnicode_InternFromString("pending");
+    if (!s_ptr || !s_shape || !s_strides || !s_dtype || !s_code || !s_device || !s_backend || !s_hip || !s_storage || !s_pending) return nullptr;
     return PyModule_Create(&module);
 }

@@ -31,9 +31,11 @@ Buckets make_buckets(int64_t total, bool both, int64_t max_distance) {
         fail(HPT_ERR_PARAM, "position bias: max_distance %lld outside %d..%d for %d buckets a direction", (long long)max_distance, half + 1, kMostDistance, b.n);
     for (int k = 0; k <= half; ++k) b.begin[k] = (uint16_t)k;
     // bucket half + j begins at the first whole distance not below half * (max_distance / half)^(j / (n - half)); a power that comes
-    // within 1e-9 of a whole number is taken for it (both are exact in most cases, doubles are off by 1e-15 or so)
+    // within 1e-9 of a whole number is taken for it (doubles are off by 1e-14 or so after up to 127 products)
+    const double step = std::pow((double)max_distance / half, 1.0 / (b.n - half));
+    double at = half;
     for (int j = 1; half + j < b.n; ++j) {
-        const double at = half * std::pow((double)max_distance / half, (double)j / (b.n - half));
+        at *= step;
         b.begin[half + j] = (uint16_t)std::ceil(at * (1 - 1e-9));
     }
     b.far = b.begin[b.n - 1];
@@ -63,7 +65,7 @@ struct Place {
     template <class A> __device__ __forceinline__ Place(const A& a, int64_t matrix, int64_t q0) {
         int64_t n = a.keys;
         if (a.lengths) {
-            const int64_t b = matrix / a.heads;
+            const int64_t b = quotient(matrix, a.heads);
             const int64_t len = a.lengths64 ? ((const int64_t*)a.lengths)[b] : (int64_t)((const int32_t*)a.lengths)[b];
             n = len < 0 ? 0 : len < n ? len : n;
         }
@@ -108,7 +110,7 @@ __device__ __forceinline__ void biased(const Pack<T, VEC>& p, int e, int lo, int
 // Rows held in registers. An item is `per_item` rows of one matrix; the first row is on its way while the bias comes together, every other
 // one while the row before it is summed and written.
 template <class T, int NC, bool AL>
-__global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_row_kernel(const BiasArgs a) {
+__global__ __launch_bounds__(1024, NC <= 2 ? 5 : 4) void bias_row_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
     extern __shared__ float bias[];
@@ -116,9 +118,8 @@ __global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_row_kernel(const B
     int turn_m = 0, turn_s = 0;
     const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
     const int far = a.buckets.far, right = right_of(a.buckets);
-    const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+    for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
+        const int64_t matrix = quotient(item, a.chunks), q0 = (item - matrix * a.chunks) * a.per_item;
         const int n = (int)min((int64_t)a.per_item, a.queries - q0);  // rows
         const Place place(a, matrix, q0);
         const T* x0 = (const T*)a.x + offset_of(a.matrices, matrix) + q0 * a.query_stride;
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_row_kernel(const B
         };
         fetch(ty);
         __syncthreads();  // (the bias of the item before is no longer read)
-        fill_bias<T>(a, matrix % a.heads, bias);
+        fill_bias<T>(a, matrix - quotient(matrix, a.heads) * a.heads, bias);
         __syncthreads();
         for (int first = 0; first < n; first += rpb) {
             const int i = first + ty;
@@ -265,9 +266,9 @@ __global__ __launch_bounds__(1024) void bias_stream_kernel(const BiasArgs a) {
     __shared__ float fold[32];
     const int vecs = (a.keys + VEC - 1) / VEC;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int64_t matrix = row / a.queries, q = row % a.queries;
+        const int64_t matrix = quotient(row, a.queries), q = row - matrix * a.queries;
         __syncthreads();
-        fill_bias<T>(a, matrix % a.heads, bias);
+        fill_bias<T>(a, matrix - quotient(matrix, a.heads) * a.heads, bias);
         __syncthreads();
         const Place place(a, matrix, q);
         const int live = place.live(0, a.causal), pos = place.pos;
@@ -284,11 +285,11 @@ __global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     extern __shared__ float bias[];
     __shared__ float fold[8];
-    const int64_t row = blockIdx.x / a.split, matrix = row / a.queries, q = row % a.queries;
+    const int64_t row = blockIdx.x / (unsigned)a.split, matrix = quotient(row, a.queries), q = row - matrix * a.queries;
     const int part = blockIdx.x % a.split;
     const int vecs = (a.keys + VEC - 1) / VEC, each = (vecs + a.split - 1) / a.split;
     const int v0 = min(part * each, vecs), v1 = min(v0 + each, vecs);
-    fill_bias<T>(a, matrix % a.heads, bias);
+    fill_bias<T>(a, matrix - quotient(matrix, a.heads) * a.heads, bias);
     __syncthreads();
     const Place place(a, matrix, q);
     const int live = place.live(0, a.causal), pos = place.pos;
@@ -359,7 +360,7 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, const float* pla
 // Rows held in registers, one after the other into the same places. Rows above a wavefront meet in a barrier between two rows' additions
 // (the fold); rows within one are kept in order by the fence.
 template <class T, int NC, bool AL>
-__global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_grad_kernel(const BiasGradArgs a) {
+__global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
     extern __shared__ float places[];  // [rows side by side, distances]
@@ -367,9 +368,8 @@ __global__ __launch_bounds__(1024, NC <= 2 ? 6 : 4) void bias_grad_kernel(const 
     int turn = 0;
     const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
     const int far = a.buckets.far, right = right_of(a.buckets), each = places_of(a.buckets);
-    const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+    for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
+        const int64_t matrix = quotient(item, a.chunks), q0 = (item - matrix * a.chunks) * a.per_item;
         const int n = (int)min((int64_t)a.per_item, a.queries - q0);  // rows
         const Place place(a, matrix, q0);
         const int64_t at0 = (matrix * a.queries + q0) * a.keys;
@@ -440,9 +440,8 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
     __shared__ float sums[2 * 16];
     int turn = 0;
     const int far = a.buckets.far, right = right_of(a.buckets), n = places_of(a.buckets), vecs = (a.keys + VEC - 1) / VEC;
-    const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item, items = a.rows / a.queries * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t matrix = item / chunks, q0 = item % chunks * a.per_item;
+    for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
+        const int64_t matrix = quotient(item, a.chunks), q0 = (item - matrix * a.chunks) * a.per_item;
         const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
         float left_end = 0.0f, right_end = 0.0f;
         __syncthreads();  // (the item before has left its sums)
@@ -485,9 +484,12 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
 __global__ __launch_bounds__(256) void bias_grad_table_kernel(const float* partial, int64_t matrices, int64_t chunks, int64_t heads, int buckets, float* out) {
     const int64_t entry = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (entry >= heads * buckets) return;
-    const int64_t bucket = entry / heads, head = entry % heads, items = matrices / heads * chunks;
+    const int64_t bucket = quotient(entry, heads), head = entry - bucket * heads, items = quotient(matrices, heads) * chunks;
     double s = 0;
-    for (int64_t i = threadIdx.x & 63; i < items; i += 64) s += partial[((i / chunks * heads + head) * chunks + i % chunks) * buckets + bucket];
+    for (int64_t i = threadIdx.x & 63; i < items; i += 64) {
+        const int64_t batch = quotient(i, chunks);  // (item i of this head is item batch * heads * chunks + head * chunks + i % chunks of all)
+        s += partial[((batch * (heads - 1) + head) * chunks + i) * buckets + bucket];
+    }
 #pragma unroll
     for (int w = 1; w < 64; w <<= 1) s += shfl_xor_any(s, w);
     if ((threadIdx.x & 63) == 0) out[entry] = (float)s;
@@ -536,10 +538,11 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
             // is a third full), 102 with this many and with twice as many, 112 with four times (each needs the bias in LDS first)
             const int64_t rounds = std::max<int64_t>(1, std::min<int64_t>(a.rows / 4096 / rpb, 64 / rpb));
             a.per_item = (int)(rounds * rpb);
-            const int64_t items = matrices * ((a.queries + a.per_item - 1) / a.per_item);
+            a.chunks = (a.queries + a.per_item - 1) / a.per_item;
+            a.items = matrices * a.chunks;
             bool al = a.keys % VEC == 0 && on_grid(a.x) && on_grid(a.out) && (a.queries == 1 || a.query_stride % VEC == 0);
             for (int i = 0; i < a.matrices.n; ++i) al = al && (a.matrices.size[i] == 1 || a.matrices.stride[i] % VEC == 0);
-            const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 20);
+            const unsigned grid = (unsigned)std::min<int64_t>(a.items, 1 << 20);
             HPT_WITH_NC(d.nc, {
                 if (al) bias_row_kernel<T, NC, true><<<grid, d.threads, lds, st>>>(a);
                 else bias_row_kernel<T, NC, false><<<grid, d.threads, lds, st>>>(a);
@@ -566,11 +569,12 @@ void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStrea
         return;
     }
     const int64_t matrices = a.rows / a.queries;
-    const int64_t items = bias_grad_items(dtype, matrices, a.queries, a.keys, &a.per_item);
+    a.items = bias_grad_items(dtype, matrices, a.queries, a.keys, &a.per_item);
+    a.chunks = (a.queries + a.per_item - 1) / a.per_item;
     const RowDeal d = bias_grad_deal(dtype, a.queries, a.keys);
     a.tpr = d.tpr;
     const size_t one = bias_lds(a.buckets);
-    const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 20);
+    const unsigned grid = (unsigned)std::min<int64_t>(a.items, 1 << 20);
     HPT_WITH_TYPE(dtype, {
         constexpr int VEC = 16 / sizeof(T);
         const bool al = a.keys % VEC == 0 && on_grid(a.p) && on_grid(a.g) && on_grid(a.out);
@@ -586,8 +590,7 @@ void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStrea
     });
     if (a.table_grad) {
         const int buckets = a.buckets.both ? 2 * a.buckets.n : a.buckets.n;
-        const int64_t chunks = (a.queries + a.per_item - 1) / a.per_item;
-        bias_grad_table_kernel<<<(unsigned)((a.heads * buckets + 3) / 4), 256, 0, st>>>(a.partial, matrices, chunks, a.heads, buckets, a.table_grad);
+        bias_grad_table_kernel<<<(unsigned)((a.heads * buckets + 3) / 4), 256, 0, st>>>(a.partial, matrices, a.chunks, a.heads, buckets, a.table_grad);
     }
 }
 

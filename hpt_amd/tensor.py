@@ -735,31 +735,36 @@ class Tensor:
     # ---- operators around a transformer's blocks ----------------------------------------
     # No trait of the reference has these (include/hpt_hip.h says what each computes, of which dtypes). Results go to the
     # `*out` tensors where the caller gives them, otherwise to fresh ones; `workspace` is described in the header.
-    def _block_call(self, name: str, stream, tensors, args) -> None:
-        """One call of the entry `hpt_hip_<name>` on this tensor. `args`: the entry's arguments after the input, tensors (or
-        None) among them; `tensors`: which of them there are, for the checks and for what the call uses."""
-        self._require_hip(name)
-        for t in tensors:
-            if t is not None:
+    def _block_call(self, name: str, stream, *args) -> None:
+        """One call of the entry `hpt_hip_<name>` on this tensor with the entry's arguments after the input, tensors (or None) among
+        them. The native module checks that the tensors are of this device and records what the call uses."""
+        k = 0 if stream is None else _native_stream(stream)
+        status = getattr(_ffi.calls(), name)(self, k, *args) if k >= 0 else None
+        if status is None:
+            self._require_hip(name)
+            tensors = [a for a in args if isinstance(a, Tensor)]
+            for t in tensors:
                 t._require_hip(name)
                 if t.device != self.device:
                     raise ParamError(_ffi.ERR_PARAM, f"{name}: operands on device {self.device} and on device {t.device}")
-        k = _native_stream(stream)
-        status = getattr(_ffi.calls(), name)(self, k, *args) if k >= 0 else None
-        if status is None:
-            entry = getattr(_ffi.lib(), "hpt_hip_" + name)
-            views = [t._c_view() for t in (self, *(a for a in args if isinstance(a, Tensor)))]
+            views = [t._c_view() for t in (self, *tensors)]
             left = iter(views)
             given = [C.byref(next(left)[0])] + [C.byref(next(left)[0]) if isinstance(a, Tensor) else a for a in args]
-            status = entry(self.device, stream, *given)
+            check(getattr(_ffi.lib(), "hpt_hip_" + name)(self.device, stream, *given))
             del views
-        check(status)
-        _touch(stream, self, *tensors)
+            _touch(stream, self, *tensors)
+        elif status:
+            check(status)
 
     def _fresh(self, out: Optional["Tensor"], shape, dtype: DType, stream) -> "Tensor":
-        return Tensor._result(shape, dtype, self.device, stream) if out is None else out
+        if out is not None:
+            return out
+        self._require_hip("a new result")
+        return Tensor._result(shape, dtype, self.device, stream)
 
     def _norm_dims(self, normalized_shape) -> int:
+        if type(normalized_shape) is list and normalized_shape and self.shape[-len(normalized_shape):] == normalized_shape:
+            return len(normalized_shape)
         ns = [int(s) for s in (normalized_shape if isinstance(normalized_shape, Iterable) else [normalized_shape])]
         if len(ns) > self.ndim or (ns and self.shape[self.ndim - len(ns):] != ns) or not ns:
             raise ShapeError(_ffi.ERR_SHAPE, "normalized dims must match last dims of input tensor, "
@@ -769,21 +774,19 @@ class Tensor:
     def rms_norm(self, normalized_shape, gamma: Optional["Tensor"] = None, eps: float = 1e-6, stream=None,
                  out: Optional["Tensor"] = None) -> "Tensor":
         """self / sqrt(mean(self^2) + eps) * gamma over the trailing dims `normalized_shape`."""
-        self._require_hip("rms_norm")
         nn = self._norm_dims(normalized_shape)
         out = self._fresh(out, self.shape, self.dtype, stream)
-        self._block_call("rms_norm", stream, (gamma, out), (None, nn, gamma, float(eps), None, out))
+        self._block_call("rms_norm", stream, None, nn, gamma, float(eps), None, out)
         return out
 
     def add_rms_norm(self, residual: "Tensor", normalized_shape, gamma: Optional["Tensor"] = None, eps: float = 1e-6, stream=None,
                      out: Optional["Tensor"] = None, sum_out: Optional["Tensor"] = None):
         """(rms_norm(self + residual), self + residual) in one pass; the sum is rounded to the tensors' dtype first. The sum may
         take the residual's place: `sum_out=residual`."""
-        self._require_hip("add_rms_norm")
         nn = self._norm_dims(normalized_shape)
         out = self._fresh(out, self.shape, self.dtype, stream)
         total = self._fresh(sum_out, self.shape, self.dtype, stream)
-        self._block_call("rms_norm", stream, (residual, gamma, total, out), (residual, nn, gamma, float(eps), total, out))
+        self._block_call("rms_norm", stream, residual, nn, gamma, float(eps), total, out)
         return out, total
 
     def rms_norm_quant(self, normalized_shape, gamma: Optional["Tensor"] = None, eps: float = 1e-6, residual: Optional["Tensor"] = None,
@@ -792,21 +795,22 @@ class Tensor:
         """rms_norm of self (+ residual) in 8 bits with a scale for each row or each `group` elements of one: (values, scales), and the
         sum where there is a residual. The norm is values * scales; values are i8 for format "i8", and u8 for "e4m3", the bits
         of 8-bit floats."""
-        self._require_hip("rms_norm_quant")
         nn = self._norm_dims(normalized_shape)
         if format not in _QUANT_FORMATS:
             raise ParamError(_ffi.ERR_PARAM, f"rms_norm_quant: unknown format {format!r}, expected one of {sorted(_QUANT_FORMATS)}")
         code, dtype = _QUANT_FORMATS[format]
-        cols, lead = math.prod(self.shape[self.ndim - nn:]), self.shape[:self.ndim - nn]
-        if group < 0 or (group > 0 and cols % group):
-            raise ShapeError(_ffi.ERR_SHAPE, f"rms_norm_quant: groups of {group} do not divide rows of {cols}")
-        out = self._fresh(out, self.shape, dtype, stream)
-        scales = self._fresh(scale_out, lead + [cols // group] if group else lead or [1], f32, stream)
-        total = None if residual is None else self._fresh(sum_out, self.shape, self.dtype, stream)
         if residual is None and sum_out is not None:
             raise ParamError(_ffi.ERR_PARAM, "rms_norm_quant: a sum is asked for, but there is no residual")
-        self._block_call("rms_norm_quant", stream, (residual, gamma, total, out, scales),
-                         (residual, nn, gamma, float(eps), code, int(group), total, out, scales))
+        out = self._fresh(out, self.shape, dtype, stream)
+        scales, total = scale_out, sum_out
+        if scales is None:
+            cols, lead = math.prod(self.shape[self.ndim - nn:]), self.shape[:self.ndim - nn]
+            if group < 0 or (group > 0 and cols % group):
+                raise ShapeError(_ffi.ERR_SHAPE, f"rms_norm_quant: groups of {group} do not divide rows of {cols}")
+            scales = self._fresh(None, lead + [cols // group] if group else lead or [1], f32, stream)
+        if residual is not None and total is None:
+            total = self._fresh(None, self.shape, self.dtype, stream)
+        self._block_call("rms_norm_quant", stream, residual, nn, gamma, float(eps), code, int(group), total, out, scales)
         return (out, scales) if total is None else (out, scales, total)
 
     def rms_norm_backward(self, grad: "Tensor", normalized_shape, gamma: Optional["Tensor"] = None, eps: float = 1e-6,
@@ -814,12 +818,10 @@ class Tensor:
                           gamma_out: Optional["Tensor"] = None, workspace: Optional["Tensor"] = None):
         """(gradient of self, gradient of gamma) for `grad`, the gradient of rms_norm(self); after add_rms_norm self is the sum, and
         `grad_sum` the gradient that the sum gets elsewhere. The gradient of gamma is f32."""
-        self._require_hip("rms_norm_backward")
         nn = self._norm_dims(normalized_shape)
         out = self._fresh(out, self.shape, self.dtype, stream)
         ggamma = self._fresh(gamma_out, self.shape[self.ndim - nn:], f32, stream)
-        self._block_call("rms_norm_backward", stream, (grad, grad_sum, gamma, workspace, out, ggamma),
-                         (grad, grad_sum, nn, gamma, float(eps), workspace, out, ggamma))
+        self._block_call("rms_norm_backward", stream, grad, grad_sum, nn, gamma, float(eps), workspace, out, ggamma)
         return out, ggamma
 
     def softmax_bias(self, table: "Tensor", scale: float = 1.0, bidirectional: bool = True, max_distance: int = 128, query_offset: int = 0,
@@ -828,10 +830,9 @@ class Tensor:
         """softmax(-1) of scale * self + table[bucket(key - query), head] for scores [..., heads, queries, keys] and a table [buckets,
         heads]: attention with a learned relative position bias. Query i stands at position i + query_offset; `causal` hides the
         keys behind it, `lengths` those from each sequence's end on, and a row without a key is zeros."""
-        self._require_hip("softmax_bias")
         out = self._fresh(out, self.shape, self.dtype, stream)
-        self._block_call("softmax_bias", stream, (table, lengths, workspace, out),
-                         (float(scale), table, int(bidirectional), int(max_distance), int(query_offset), int(causal), lengths, workspace, out))
+        self._block_call("softmax_bias", stream, float(scale), table, int(bidirectional), int(max_distance), int(query_offset), int(causal),
+                         lengths, workspace, out)
         return out
 
     def softmax_bias_backward(self, grad: "Tensor", buckets: int, scale: float = 1.0, bidirectional: bool = True, max_distance: int = 128,
@@ -839,25 +840,22 @@ class Tensor:
                               out: Optional["Tensor"] = None, table_out: Optional["Tensor"] = None, workspace: Optional["Tensor"] = None):
         """(gradient of the scores, gradient of the table) from softmax_bias's result `self` and its gradient `grad`, with the same
         arguments; the table's is f32 [buckets, heads]."""
-        self._require_hip("softmax_bias_backward")
         if self.ndim < 3:
             raise ShapeError(_ffi.ERR_SHAPE, "softmax_bias_backward probs: needs at least 3 dims (heads x queries x keys)")
         out = self._fresh(out, self.shape, self.dtype, stream)
         gtable = self._fresh(table_out, [int(buckets), self.shape[-3]], f32, stream)
         if gtable.shape != [int(buckets), self.shape[-3]]:
             raise ShapeError(_ffi.ERR_SHAPE, f"softmax_bias_backward grad_table: must be {buckets} buckets x {self.shape[-3]} heads")
-        self._block_call("softmax_bias_backward", stream, (grad, lengths, workspace, out, gtable),
-                         (grad, float(scale), int(bidirectional), int(max_distance), int(query_offset), int(causal), lengths, workspace, out,
-                          gtable))
+        self._block_call("softmax_bias_backward", stream, grad, float(scale), int(bidirectional), int(max_distance), int(query_offset),
+                         int(causal), lengths, workspace, out, gtable)
         return out, gtable
 
     def token_logp(self, token: "Tensor", stream=None, logp_out: Optional["Tensor"] = None, lse_out: Optional["Tensor"] = None,
                    workspace: Optional["Tensor"] = None):
         """(log-probability of one token, log of the sum of exponentials) of each row of logits [..., vocabulary], both f32."""
-        self._require_hip("token_logp")
         lead = self.shape[:-1] or [1]
         logp, lse = self._fresh(logp_out, lead, f32, stream), self._fresh(lse_out, lead, f32, stream)
-        self._block_call("token_logp", stream, (token, workspace, logp, lse), (token, workspace, logp, lse))
+        self._block_call("token_logp", stream, token, workspace, logp, lse)
         return logp, lse
 
     def policy_loss(self, token: "Tensor", old_logp: "Tensor", advantage: "Tensor", reference: Optional["Tensor"] = None,
@@ -866,21 +864,18 @@ class Tensor:
                     weight_out: Optional["Tensor"] = None, workspace: Optional["Tensor"] = None) -> PolicyLoss:
         """The clipped policy loss with a KL term over logits [..., vocabulary], averaged with `mask` as weights: a PolicyLoss, whose
         parts policy_loss_backward takes. All f32."""
-        self._require_hip("policy_loss")
         lead = self.shape[:-1] or [1]
         loss = self._fresh(loss_out, [1], f32, stream)
         logp, lse, weight = (self._fresh(t, lead, f32, stream) for t in (logp_out, lse_out, weight_out))
-        self._block_call("policy_loss", stream, (token, old_logp, advantage, reference, mask, workspace, loss, logp, lse, weight),
-                         (token, old_logp, advantage, reference, mask, float(clip_low), float(clip_high), float(kl_weight), workspace, loss,
-                          logp, lse, weight))
+        self._block_call("policy_loss", stream, token, old_logp, advantage, reference, mask, float(clip_low), float(clip_high),
+                         float(kl_weight), workspace, loss, logp, lse, weight)
         return PolicyLoss(loss, logp, lse, weight)
 
     def policy_loss_backward(self, token: "Tensor", lse: "Tensor", weight: "Tensor", grad: float = 1.0, stream=None,
                              out: Optional["Tensor"] = None) -> "Tensor":
         """The gradient of the logits `self` from a PolicyLoss's lse and weight, times `grad`; `out` may be the logits."""
-        self._require_hip("policy_loss_backward")
         out = self._fresh(out, self.shape, self.dtype, stream)
-        self._block_call("policy_loss_backward", stream, (token, lse, weight, out), (token, lse, weight, float(grad), out))
+        self._block_call("policy_loss_backward", stream, token, lse, weight, float(grad), out)
         return out
 
     # ---- the steps either side of the path ------------------------------------------
