@@ -451,7 +451,11 @@ void launch_rms_norm(int dtype, int quant, const RmsArgs& a, hipStream_t st) {
 int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) {
     const RowDeal d = grad_deal(dtype, cols);
     const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
-    return std::min<int64_t>(blocks, 1024);
+    // As many workgroups as run at once, four wavefronts on each SIMD: in more, the last round is mostly empty, in fewer, memory waits. us, bf16
+    // [16384, 4096] 512 workgroups 129, 768 98, 1024 85, 2048 93; f16 [8000, 8192] 512 88, 1024 94, 2048 108; bf16 [6000, 5120] 768 48, 1024 61.
+    // Few rows: two to a workgroup, as each leaves a row of partial sums ([1000, 4096] 16.3 in 1000 workgroups, 13.6 in 512).
+    const int64_t resident = 256 * std::max(1, 16 / (d.threads / 64));
+    return std::min({blocks, resident, std::max<int64_t>(512, blocks / 2)});
 }
 
 void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
