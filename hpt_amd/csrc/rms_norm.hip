@@ -57,7 +57,14 @@ template <int Q> __device__ __forceinline__ uint8_t quantized_one(float y, float
     return quantized<Q, 4>(v, inv).v[0];
 }
 
-// Rows held in registers. Workgroups walk the rows; gamma is fetched once. Q: groups of `group` elements are `group` / VEC neighbouring lanes
+// Whether workgroups walk the rows with the next one on its way while a row is summed and written, or take a row each and leave it to their
+// number that memory is busy. us, a row each -> walked: one operand f16 [13107, 5120] 64 -> 50, bf16 [4096, 16384] 65 -> 50, [8190, 4097]
+// 32 -> 27, [16384, 4096] 50.4 -> 49.7; in 8 bits [13107, 5120] 87 -> 50, [16384, 4096] 61 -> 44; x + residual in 8 bits [8192, 8192] 93 -> 84,
+// [8192, 4096] 46.8 -> 45.6, [16384, 4096] 88 -> 92. x + residual in its own type is ahead without ([16384, 4096] 89 against 97, [13107, 5120]
+// 89 against 99), and beyond 16 elements per thread a second row does not fit the registers.
+template <class T, int NC, bool RES, int Q> constexpr bool kAhead = (!RES || Q != QUANT_NONE) && NC * 16 / (int)sizeof(T) <= 16;
+
+// Rows held in registers; gamma is fetched once. Q: groups of `group` elements are `group` / VEC neighbouring lanes
 // (a power of two of them, within a wavefront), or the whole row.
 template <class T, int NC, bool AL, bool RES, int Q>
 __global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {
@@ -72,36 +79,52 @@ __global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) g[k] = load_slot<T, AL>((const T*)a.gamma, At(lane + k * tpr, a.cols));
     }
-    for (int64_t first = (int64_t)blockIdx.x * rpb; first < a.rows; first += (int64_t)gridDim.x * rpb) {
-        const int64_t row = first + ty;
+    const int64_t step = (int64_t)gridDim.x * rpb;
+    Pack<T, VEC> p[NC], q[RES ? NC : 1];
+    auto fetch = [&](int64_t row) {
         const int cols = row < a.rows ? a.cols : 0;  // (threads behind the last row go along to the barriers)
         const T* x = (const T*)a.x + (cols ? offset_of(a.kept, row) : 0);
-        Pack<T, VEC> p[NC];
 #pragma unroll
         for (int k = 0; k < NC; ++k) p[k] = load_slot<T, AL>(x, At(lane + k * tpr, cols));
         if constexpr (RES) {
-            Pack<T, VEC> q[NC];
-            const T* res = (const T*)a.res + row * a.cols;
 #pragma unroll
-            for (int k = 0; k < NC; ++k) q[k] = load_slot<T, AL>(res, At(lane + k * tpr, cols));
+            for (int k = 0; k < NC; ++k) q[k] = load_slot<T, AL>((const T*)a.res + row * a.cols, At(lane + k * tpr, cols));
+        }
+    };
+    if constexpr (kAhead<T, NC, RES, Q>) fetch((int64_t)blockIdx.x * rpb + ty);
+    for (int64_t first = (int64_t)blockIdx.x * rpb; first < a.rows; first += step) {
+        const int64_t row = first + ty;
+        const int cols = row < a.rows ? a.cols : 0;
+        if constexpr (!kAhead<T, NC, RES, Q>) fetch(row);
+        Pack<T, VEC> h[NC];
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
+        for (int k = 0; k < NC; ++k) {
+            h[k] = p[k];
+            if constexpr (RES) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) p[k].v[i] = Elem<T>::narrow(Elem<T>::widen(p[k].v[i]) + Elem<T>::widen(q[k].v[i]));
-                if (a.sum) store_slot<T, VEC, AL>((T*)a.sum + row * a.cols, At(lane + k * tpr, cols), p[k]);
+                for (int i = 0; i < VEC; ++i) h[k].v[i] = Elem<T>::narrow(Elem<T>::widen(p[k].v[i]) + Elem<T>::widen(q[k].v[i]));
+            }
+        }
+        if constexpr (kAhead<T, NC, RES, Q>) {
+            if (first + step < a.rows) fetch(row + step);
+        }
+        if constexpr (RES) {
+            if (a.sum) {
+#pragma unroll
+                for (int k = 0; k < NC; ++k) store_slot<T, VEC, AL>((T*)a.sum + row * a.cols, At(lane + k * tpr, cols), h[k]);
             }
         }
         float ss[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) ss[0] = fmaf(Elem<T>::widen(p[k].v[i]), Elem<T>::widen(p[k].v[i]), ss[0]);
+            for (int i = 0; i < VEC; ++i) ss[0] = fmaf(Elem<T>::widen(h[k].v[i]), Elem<T>::widen(h[k].v[i]), ss[0]);
         }
         fold_row<SumF>(ss, tpr, sums, turn);
         const float r = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
         auto value = [&](int k, float (&y)[VEC]) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) y[i] = a.gamma ? Elem<T>::widen(p[k].v[i]) * r * Elem<T>::widen(g[k].v[i]) : Elem<T>::widen(p[k].v[i]) * r;
+            for (int i = 0; i < VEC; ++i) y[i] = a.gamma ? Elem<T>::widen(h[k].v[i]) * r * Elem<T>::widen(g[k].v[i]) : Elem<T>::widen(h[k].v[i]) * r;
         };
         if constexpr (Q == QUANT_NONE) {
             T* out = (T*)a.out + row * a.cols;
@@ -270,8 +293,11 @@ template <class T, bool RES, int Q> void launch_of(const RmsArgs& given, hipStre
     }
     a.tpr = d.tpr;
     const int64_t blocks = (a.rows + d.rows_per_block() - 1) / d.rows_per_block();
-    const unsigned grid = (unsigned)std::min<int64_t>(blocks, 1 << 16);
+    // walked: as many workgroups as run at once, of six wavefronts on each SIMD, with a residual four (24 -> 16 wavefronts per compute unit: bf16
+    // [8192, 8192] in 8 bits 96 -> 84 us, without a residual 46 -> 51)
+    const int64_t resident = 256 * std::max(1, (RES ? 16 : 24) / (d.threads / 64));
     HPT_WITH_NC(d.nc, {
+        const unsigned grid = (unsigned)std::min<int64_t>(blocks, kAhead<T, NC, RES, Q> ? resident : 1 << 16);
         if (al) rms_row_kernel<T, NC, true, RES, Q><<<grid, d.threads, 0, st>>>(a);
         else rms_row_kernel<T, NC, false, RES, Q><<<grid, d.threads, 0, st>>>(a);
     });
