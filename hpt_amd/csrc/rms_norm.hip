@@ -280,13 +280,14 @@ bool rows_on_grid(const void* p, const Dims& kept, int vec) {
 template <class T, bool RES, int Q> void launch_of(const RmsArgs& given, hipStream_t st) {
     constexpr int VEC = 16 / sizeof(T);
     RmsArgs a = given;
-    constexpr int dtype_most = sizeof(T) == 4 ? 8 : 4;
+    // (eight vectors of f32 and of a residual spill: [1024, 30001] 128 us, streamed 114)
+    constexpr int most = sizeof(T) == 4 ? (RES ? 6 : 8) : 4;
     const bool al = a.cols % VEC == 0 && rows_on_grid(a.x, a.kept, VEC) && on_grid(a.res) && on_grid(a.gamma) && on_grid(a.sum) && on_grid(a.out);
     const bool grouped = Q != QUANT_NONE && a.group != a.cols;
     // lanes of a group: a power of two of them within a wavefront
     const int lanes = grouped && a.group % VEC == 0 ? a.group / VEC : 0;
     const bool by_lanes = !grouped || (al && lanes >= 1 && lanes <= 64 && (lanes & (lanes - 1)) == 0);
-    const RowDeal d = deal_row(a.cols, sizeof(T), 2, dtype_most, grouped && by_lanes ? lanes : 1);
+    const RowDeal d = deal_row(a.cols, sizeof(T), 2, most, grouped && by_lanes ? lanes : 1);
     if (!d.held() || !by_lanes || a.cols < VEC) {
         rms_stream_kernel<T, RES, Q><<<(unsigned)std::min<int64_t>(a.rows, 1 << 16), 1024, 0, st>>>(a);
         return;
@@ -297,9 +298,10 @@ template <class T, bool RES, int Q> void launch_of(const RmsArgs& given, hipStre
     // [8192, 8192] in 8 bits 96 -> 84 us, without a residual 46 -> 51)
     const int64_t resident = 256 * std::max(1, (RES ? 16 : 24) / (d.threads / 64));
     HPT_WITH_NC(d.nc, {
-        const unsigned grid = (unsigned)std::min<int64_t>(blocks, kAhead<T, NC, RES, Q> ? resident : 1 << 16);
-        if (al) rms_row_kernel<T, NC, true, RES, Q><<<grid, d.threads, 0, st>>>(a);
-        else rms_row_kernel<T, NC, false, RES, Q><<<grid, d.threads, 0, st>>>(a);
+        constexpr int N = NC > most ? most : NC;
+        const unsigned grid = (unsigned)std::min<int64_t>(blocks, kAhead<T, N, RES, Q> ? resident : 1 << 16);
+        if (al) rms_row_kernel<T, N, true, RES, Q><<<grid, d.threads, 0, st>>>(a);
+        else rms_row_kernel<T, N, false, RES, Q><<<grid, d.threads, 0, st>>>(a);
     });
 }
 
