@@ -312,9 +312,15 @@ __global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
 
 // ---- backward -------------------------------------------------------------------------------------
 
-// What a row's VEC elements from key e on add: to the places of their distances, or, beyond `far` and `right`, to the thread's own sums of
+// By how much the places of rows at position `pos` are shifted, and the quadruples of an array with room for any shift.
+__device__ __forceinline__ int shift_of(const Buckets& b, int pos) { return (pos - b.far - kPad) & 3; }
+__host__ __device__ inline int quads_of(const Buckets& b) { return (places_of(b) + 3 + 3) / 4; }
+
+typedef float Quad __attribute__((ext_vector_type(4), may_alias));
+
+// (Rows that are swept.) What a row's VEC elements from key e on add: to the places of their distances, or, beyond `far` and `right`, to the thread's own sums of
 // the ends. Hidden elements are zeros. Rows add to a place one after the other, each once, so that the sums do not depend on any order
-// though the LDS adds by itself (one instruction instead of a read, its latency and a write).
+// though the LDS adds by itself.
 template <int VEC>
 __device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, int pos, int far, int right, float* places, float& left_end, float& right_end) {
     const int r = e - pos;
@@ -331,11 +337,11 @@ __device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, in
     }
 }
 
-// The workgroup's sums by distance -> by bucket, into its row of partial sums; eight lanes share a bucket. `places`: one array of them for each
-// of `groups` rows that run side by side. Every thread of the workgroup comes here.
-__device__ __forceinline__ void leave_buckets(const Buckets& b, const float* places, int groups, float left_end, float right_end, float* out) {
+// The workgroup's sums by distance -> by bucket, into its row of partial sums; eight lanes share a bucket. `places`: arrays of `length`, number g for
+// rows at positions pos + g modulo 4. Every thread of the workgroup comes here.
+__device__ __forceinline__ void leave_buckets(const Buckets& b, const float* places, int arrays, int length, int pos, float left_end, float right_end, float* out) {
     __shared__ float ends[2 * 16 * 2];
-    const int n = places_of(b), total = b.both ? 2 * b.n : b.n, zero = b.far + kPad;
+    const int total = b.both ? 2 * b.n : b.n, zero = b.far + kPad;
     float e[2] = {left_end, right_end};
     int turn = 0;
     fold_row<SumF>(e, blockDim.x, ends, turn);
@@ -350,24 +356,27 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, const float* pla
         if (part == 0 && !b.both && j == 0) s += e[1];
         for (int d = from + part; d < to; d += 8) {
             const float* at = places + (ahead ? zero + d : zero - d);
-            for (int g = 0; g < groups; ++g) s += at[g * n];
+            for (int g = 0; g < arrays; ++g) s += at[g * length + shift_of(b, pos + g)];
         }
         s = group_reduce<SumF>(s, 8);
         if (part == 0) out[k] = s;
     }
 }
 
-// Rows held in registers, one after the other into the same places. Rows above a wavefront meet in a barrier between two rows' additions
-// (the fold); rows within one are kept in order by the fence.
+// Rows held in registers, one after the other into the same places. The rows that meet in one array of places all stand at the same position
+// modulo 4 (four rows side by side or more have an array each, longer ones are dealt to four in turn), and the array is shifted by what that
+// is, so that a vector's places are whole aligned quadruples: read, added to and written with 128-bit accesses that meet no bank
+// twice. (By single words, eight to a vector, every instruction met each bank eight times: 73 us of bf16 [16, 16, 256, 256] were theirs.)
+// Rows above a wavefront pass a barrier between two rows' additions (the fold); rows within one are kept in order by the fence.
 template <class T, int NC, bool AL>
 __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     using At = Slot<VEC, AL>;
-    extern __shared__ float places[];  // [rows side by side, distances]
+    extern __shared__ __attribute__((aligned(16))) float places[];  // [arrays, quads]
     __shared__ float sums[2 * 16];
     int turn = 0;
     const int tpr = a.tpr, lane = threadIdx.x % tpr, ty = threadIdx.x / tpr, rpb = blockDim.x / tpr;
-    const int far = a.buckets.far, right = right_of(a.buckets), each = places_of(a.buckets);
+    const int far = a.buckets.far, right = right_of(a.buckets), quads = quads_of(a.buckets), arrays = max(rpb, 4);
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
         const int64_t matrix = quotient(item, a.chunks), q0 = (item - matrix * a.chunks) * a.per_item;
         const int n = (int)min((int64_t)a.per_item, a.queries - q0);  // rows
@@ -375,8 +384,12 @@ __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_ke
         const int64_t at0 = (matrix * a.queries + q0) * a.keys;
         float left_end = 0.0f, right_end = 0.0f;
         Pack<T, VEC> pp[NC], gp[NC];
-        auto fetch = [&](int i) {
-            const int live = i < n ? place.live(i, a.causal) : 0;
+        __syncthreads();  // (the item before has left its sums)
+        for (int i = threadIdx.x; i < quads * arrays; i += blockDim.x) ((Quad*)places)[i] = Quad{0.0f, 0.0f, 0.0f, 0.0f};
+        __syncthreads();
+        for (int first = 0; first < n; first += rpb) {
+            const int i = first + ty;
+            const int live = i < n ? place.live(i, a.causal) : 0, pos = place.pos + i;
             const T *p = (const T*)a.p + at0 + (int64_t)i * a.keys, *g = (const T*)a.g + at0 + (int64_t)i * a.keys;
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
@@ -385,14 +398,6 @@ __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_ke
                 pp[k] = load_slot<T, AL>(p, at);
                 gp[k] = load_slot<T, AL>(g, at);
             }
-        };
-        __syncthreads();  // (the item before has left its sums)
-        for (int i = threadIdx.x; i < each * rpb; i += blockDim.x) places[i] = 0.0f;
-        __syncthreads();
-        for (int first = 0; first < n; first += rpb) {
-            const int i = first + ty;
-            const int live = i < n ? place.live(i, a.causal) : 0, pos = place.pos + i;
-            fetch(i);
             float s[1] = {0.0f};
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
@@ -409,6 +414,8 @@ __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_ke
             fold_row<SumF>(s, tpr, sums, turn);
             const bool finite = fabsf(s[0]) < __builtin_huge_valf();
             T* out = (T*)a.out + at0 + (int64_t)i * a.keys;
+            float* mine = places + (rpb >= 4 ? ty : i & 3) * 4 * quads;
+            const int shift = far + kPad - pos + shift_of(a.buckets, pos);  // of a key's place: a multiple of 4 for keys that are
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
@@ -424,11 +431,28 @@ __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_ke
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) o.v[j] = Elem<T>::narrow(a.scale * d[j]);
                 if (i < n) store_slot<T, VEC, AL>(out, at, o);
-                if (a.table_grad && at.s + at.lo < live) add_by_distance<VEC>(d, at.s, pos, far, right, places + ty * each, left_end, right_end);
+                if (!a.table_grad || at.s + at.lo >= live) continue;
+                const int r = at.s - pos;
+                if (r <= -far - VEC || r >= right) {
+                    float t = d[0];
+#pragma unroll
+                    for (int j = 1; j < VEC; ++j) t += d[j];
+                    if (r < 0) left_end += t;
+                    else right_end += t;
+                } else if (AL || at.lo == 0) {
+                    Quad* to = (Quad*)(mine + at.s + shift);
+#pragma unroll
+                    for (int j = 0; j < VEC / 4; ++j) to[j] += Quad{d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]};
+                } else {  // the row's last vector, taken from its end backwards: its own elements by words
+#pragma unroll
+                    for (int j = 1; j < VEC; ++j) {
+                        if (j >= at.lo) mine[at.s + shift + j] += d[j];
+                    }
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        if (a.table_grad) leave_buckets(a.buckets, places, rpb, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+        if (a.table_grad) leave_buckets(a.buckets, places, arrays, 4 * quads, place.pos, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
     }
 }
 
@@ -476,7 +500,7 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
                 store_sweep_vec<T, VEC>((T*)a.out + row * a.keys, v, a.keys, o);
             }
         }
-        if (a.table_grad) leave_buckets(a.buckets, places, 1, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+        if (a.table_grad) leave_buckets(a.buckets, places, 1, 0, far + kPad, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
     }
 }
 
@@ -500,21 +524,30 @@ bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
 
 // A workgroup holds rows of one matrix: where that has few (a step of decoding has one), down to a wavefront.
-RowDeal deal_keys(int dtype, int64_t queries, int64_t keys, int most) {
-    RowDeal d = deal_row(keys, dtype_size(dtype), 2, most);
+RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) {
+    RowDeal d = deal_row(keys, dtype_size(dtype), dtype == HPT_F32 ? 4 : 2, most_vecs(dtype));  // (16 elements a thread: f32 of two vectors 94 us, of four 86, [4, 16, 1024, 1024])
     while (d.tpr <= 64 && d.threads > 64 && d.threads / 2 >= queries * d.tpr) d.threads /= 2;
     return d;
 }
-RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) { return deal_keys(dtype, queries, keys, most_vecs(dtype)); }
-// (backward: two vectors per thread, four of f32, of two operands)
-RowDeal bias_grad_deal(int dtype, int64_t queries, int64_t keys) { return deal_keys(dtype, queries, keys, dtype == HPT_F32 ? 4 : 2); }
+// Backward: two vectors per thread, four of f32, of two operands; 32 rows side by side at most, because each of them has places of its own.
+RowDeal bias_grad_deal(int dtype, int64_t keys) {
+    return deal_row(keys, dtype_size(dtype), dtype == HPT_F32 ? 4 : 2, dtype == HPT_F32 ? 4 : 2, 8);
+}
+// Rows of a matrix that a workgroup takes one after the other, in rounds of those side by side: 96 KiB of operands and results for 256 threads (a
+// workgroup is started every 5 ns at best, and each fetches its bias or clears its places first), 64 rows at most, but so that there are
+// 512 of them. us, forward / backward, for 64, 96 and 128 KiB: bf16 [4, 16, 1024, 1024], causal, 52 / 69, 49 / 65, 58 / 67, [2, 16, 2048, 2048], causal,
+// 112 / 147, 105 / 124, 103 / 126, [8, 16, 1024, 1024] 93 / 151, 96 / 141, 98 / 144. [16, 16, 256, 256] with 1024 workgroups 14.1 / 24.6, with 4096
+// 18.9 / 30.8.
+int64_t rounds_of(int64_t rows, const RowDeal& d, int64_t row_bytes) {
+    return std::max<int64_t>(1, std::min<int64_t>({(int64_t)384 * d.threads / row_bytes, 64, rows / 512}) / d.rows_per_block());
+}
 
 }  // namespace
 
-// Rows that registers do not hold, and few of them, are split: parts of 64 KiB at least.
+// Rows that registers do not hold, and few of them, are split into parts of 16 KiB at least: two launches, but on more compute units. (Rows that
+// registers hold stay whole: bf16 [32, 32768] 9.9 us against 13.9 split, [256, 32768] 12.6 against 19.)
 int bias_split(int dtype, int64_t rows, int64_t keys) {
-    const RowDeal d = deal_row(keys, dtype_size(dtype), 2, most_vecs(dtype));
-    if (rows >= 512 || rows == 0 || (d.held() && keys * (int64_t)dtype_size(dtype) < (64 << 10))) return 1;
+    if (rows == 0 || rows >= 512 || deal_row(keys, dtype_size(dtype), 1, most_vecs(dtype)).held()) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({64, 1024 / rows, keys * (int64_t)dtype_size(dtype) / (16 << 10)}));
 }
 
@@ -533,11 +566,7 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
             bias_stream_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 16), 1024, lds, st>>>(a);
         } else {
             a.tpr = d.tpr;
-            const int rpb = d.rows_per_block();
-            // items for sixteen workgroups per compute unit, of up to 64 rows each: bf16 [8, 16, 1024, 1024] 110 us with half as many (their last round
-            // is a third full), 102 with this many and with twice as many, 112 with four times (each needs the bias in LDS first)
-            const int64_t rounds = std::max<int64_t>(1, std::min<int64_t>(a.rows / 4096 / rpb, 64 / rpb));
-            a.per_item = (int)(rounds * rpb);
+            a.per_item = (int)(rounds_of(a.rows, d, 2 * a.keys * (int64_t)sizeof(T)) * d.rows_per_block());
             a.chunks = (a.queries + a.per_item - 1) / a.per_item;
             a.items = matrices * a.chunks;
             bool al = a.keys % VEC == 0 && on_grid(a.x) && on_grid(a.out) && (a.queries == 1 || a.query_stride % VEC == 0);
@@ -552,12 +581,8 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
 }
 
 int64_t bias_grad_items(int dtype, int64_t matrices, int64_t queries, int64_t keys, int* per_item) {
-    const RowDeal d = bias_grad_deal(dtype, queries, keys);
-    const int64_t rpb = d.rows_per_block();
-    // sixteen workgroups per compute unit, of up to 64 rows each: bf16 [4, 16, 1024, 1024], causal, 87 us with half as many, 75 with this many, 84
-    // with twice as many (each clears its places and leaves its sums)
-    const int64_t rounds = std::max<int64_t>({1, std::min<int64_t>(matrices * queries / 4096 / rpb, 64 / rpb)});
-    *per_item = (int)(rounds * rpb);
+    const RowDeal d = bias_grad_deal(dtype, keys);
+    *per_item = (int)(rounds_of(matrices * queries, d, 3 * keys * (int64_t)dtype_size(dtype)) * d.rows_per_block());
     return matrices * ((queries + *per_item - 1) / *per_item);
 }
 
@@ -571,20 +596,26 @@ void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStrea
     const int64_t matrices = a.rows / a.queries;
     a.items = bias_grad_items(dtype, matrices, a.queries, a.keys, &a.per_item);
     a.chunks = (a.queries + a.per_item - 1) / a.per_item;
-    const RowDeal d = bias_grad_deal(dtype, a.queries, a.keys);
-    a.tpr = d.tpr;
+    RowDeal d = bias_grad_deal(dtype, a.keys);
+    const bool held = d.held();
     const size_t one = bias_lds(a.buckets);
+    // (far buckets take more LDS: fewer rows side by side, the same items)
+    const size_t array = (size_t)quads_of(a.buckets) * 16;
+    while (d.tpr < 64 && array * d.rows_per_block() > (20 << 10)) d.tpr *= 2;
+    const size_t lds = array * std::max(4, d.rows_per_block());
+    d.nc = (int)(((int64_t)a.keys * (int64_t)dtype_size(dtype) + 16 * d.tpr - 1) / (16 * d.tpr));
+    a.tpr = d.tpr;
     const unsigned grid = (unsigned)std::min<int64_t>(a.items, 1 << 20);
     HPT_WITH_TYPE(dtype, {
         constexpr int VEC = 16 / sizeof(T);
         const bool al = a.keys % VEC == 0 && on_grid(a.p) && on_grid(a.g) && on_grid(a.out);
-        if (!d.held() || a.keys < VEC || one * d.rows_per_block() > (48 << 10)) {
+        if (!held || a.keys < VEC || lds > (48 << 10)) {
             bias_grad_stream_kernel<T><<<grid, 1024, one, st>>>(a);
         } else {
             HPT_WITH_NC(d.nc, {
                 constexpr int M = sizeof(T) == 4 ? (NC > 4 ? 4 : NC) : (NC > 2 ? 2 : NC);
-                if (al) bias_grad_kernel<T, M, true><<<grid, d.threads, one * d.rows_per_block(), st>>>(a);
-                else bias_grad_kernel<T, M, false><<<grid, d.threads, one * d.rows_per_block(), st>>>(a);
+                if (al) bias_grad_kernel<T, M, true><<<grid, d.threads, lds, st>>>(a);
+                else bias_grad_kernel<T, M, false><<<grid, d.threads, lds, st>>>(a);
             });
         }
     });
