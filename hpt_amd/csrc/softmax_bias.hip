@@ -533,9 +533,8 @@ RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) {
 RowDeal bias_grad_deal(int dtype, int64_t keys) {
     return deal_row(keys, dtype_size(dtype), dtype == HPT_F32 ? 4 : 2, dtype == HPT_F32 ? 4 : 2, 8);
 }
-// Rows of a matrix that a workgroup takes one after the other, in rounds of those side by side: 96 KiB of operands and results for 256 threads (a
-// workgroup is started every 5 ns at best, and each fetches its bias or clears its places first), 64 rows at most, but so that there are
-// 512 of them. us, forward / backward, for 64, 96 and 128 KiB: bf16 [4, 16, 1024, 1024], causal, 52 / 69, 49 / 65, 58 / 67, [2, 16, 2048, 2048], causal,
+// Rows of a matrix that a workgroup takes one after the other, in rounds of those side by side: 96 KiB of operands and results for 256 threads
+// (each workgroup fetches its bias or clears its places first), 64 rows at most, but so that there are 512 workgroups. us, forward / backward, for 64, 96 and 128 KiB: bf16 [4, 16, 1024, 1024], causal, 52 / 69, 49 / 65, 58 / 67, [2, 16, 2048, 2048], causal,
 // 112 / 147, 105 / 124, 103 / 126, [8, 16, 1024, 1024] 93 / 151, 96 / 141, 98 / 144. [16, 16, 256, 256] with 1024 workgroups 14.1 / 24.6, with 4096
 // 18.9 / 30.8.
 int64_t rounds_of(int64_t rows, const RowDeal& d, int64_t row_bytes) {
