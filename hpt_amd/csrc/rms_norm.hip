@@ -449,17 +449,20 @@ __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs
 __global__ __launch_bounds__(1024) void rms_grad_columns_kernel(const float* partial, int64_t parts, int cols, float* out) {
     __shared__ double meet[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + tx;
-    double s = 0;
-    if (col < cols) {
+    for (int first = blockIdx.x * 32; first < cols; first += gridDim.x * 32) {
+        const int col = first + tx;
+        double s = 0;
+        if (col < cols) {
 #pragma unroll 8
-        for (int64_t p = ty; p < parts; p += 32) s += partial[p * cols + col];
-    }
-    meet[ty][tx] = s;
-    __syncthreads();
-    if (ty == 0 && col < cols) {
-        for (int k = 1; k < 32; ++k) s += meet[k][tx];
-        out[col] = (float)s;
+            for (int64_t p = ty; p < parts; p += 32) s += partial[p * cols + col];
+        }
+        __syncthreads();  // (the columns before have been read)
+        meet[ty][tx] = s;
+        __syncthreads();
+        if (ty == 0 && col < cols) {
+            for (int k = 1; k < 32; ++k) s += meet[k][tx];
+            out[col] = (float)s;
+        }
     }
 }
 
@@ -483,7 +486,8 @@ int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) {
     // [16384, 4096] 512 workgroups 129, 768 98, 1024 85, 2048 93; f16 [8000, 8192] 512 88, 1024 94, 2048 108; bf16 [6000, 5120] 768 48, 1024 61.
     // Few rows: two to a workgroup, as each leaves a row of partial sums ([1000, 4096] 16.3 in 1000 workgroups, 13.6 in 512).
     const int64_t resident = 256 * std::max(1, 16 / (d.threads / 64));
-    return std::min({blocks, resident, std::max<int64_t>(512, blocks / 2)});
+    // (256 MiB of them at most)
+    return std::min({blocks, resident, std::max<int64_t>(512, blocks / 2), std::max<int64_t>(1, (64 << 20) / std::max<int64_t>(1, cols))});
 }
 
 void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
@@ -507,7 +511,7 @@ void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t s
             });
         }
     });
-    if (a.ggamma) rms_grad_columns_kernel<<<(a.cols + 31) / 32, 1024, 0, st>>>(a.partial, parts, a.cols, a.ggamma);
+    if (a.ggamma) rms_grad_columns_kernel<<<std::min((a.cols + 31) / 32, 1 << 16), 1024, 0, st>>>(a.partial, parts, a.cols, a.ggamma);
 }
 
 }  // namespace hpt

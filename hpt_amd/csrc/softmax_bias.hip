@@ -506,17 +506,23 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
 
 // The table's gradient [buckets, heads]: a wavefront for each entry folds the items of its head in a fixed order, in f64.
 __global__ __launch_bounds__(256) void bias_grad_table_kernel(const float* partial, int64_t matrices, int64_t chunks, int64_t heads, int buckets, float* out) {
-    const int64_t entry = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (entry >= heads * buckets) return;
-    const int64_t bucket = quotient(entry, heads), head = entry - bucket * heads, items = quotient(matrices, heads) * chunks;
-    double s = 0;
-    for (int64_t i = threadIdx.x & 63; i < items; i += 64) {
-        const int64_t batch = quotient(i, chunks);  // (item i of this head is item batch * heads * chunks + head * chunks + i % chunks of all)
-        s += partial[((batch * (heads - 1) + head) * chunks + i) * buckets + bucket];
-    }
+    const int64_t items = quotient(matrices, heads) * chunks;
+    for (int64_t entry = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); entry < heads * buckets; entry += (int64_t)gridDim.x * 4) {
+        const int64_t bucket = quotient(entry, heads), head = entry - bucket * heads;
+        double s = 0;
+        for (int64_t i = threadIdx.x & 63; i < items; i += 64) {
+            const int64_t batch = quotient(i, chunks);  // (item i of this head is item batch * heads * chunks + head * chunks + i % chunks of all)
+            s += partial[((batch * (heads - 1) + head) * chunks + i) * buckets + bucket];
+        }
 #pragma unroll
-    for (int w = 1; w < 64; w <<= 1) s += shfl_xor_any(s, w);
-    if ((threadIdx.x & 63) == 0) out[entry] = (float)s;
+        for (int w = 1; w < 64; w <<= 1) s += shfl_xor_any(s, w);
+        if ((threadIdx.x & 63) == 0) out[entry] = (float)s;
+    }
+}
+void launch_table(const BiasGradArgs& a, int64_t matrices, hipStream_t st) {
+    const int buckets = a.buckets.both ? 2 * a.buckets.n : a.buckets.n;
+    const unsigned grid = (unsigned)std::min<int64_t>((a.heads * buckets + 3) / 4, 1 << 20);
+    bias_grad_table_kernel<<<grid, 256, 0, st>>>(a.partial, matrices, a.chunks, a.heads, buckets, a.table_grad);
 }
 
 bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -588,8 +594,8 @@ int64_t bias_grad_items(int dtype, int64_t matrices, int64_t queries, int64_t ke
 void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStream_t st) {
     BiasGradArgs a = given;
     if (a.rows == 0) {  // a table's gradient of zeros
-        const int buckets = a.buckets.both ? 2 * a.buckets.n : a.buckets.n;
-        bias_grad_table_kernel<<<(unsigned)((a.heads * buckets + 3) / 4), 256, 0, st>>>(nullptr, 0, 1, a.heads, buckets, a.table_grad);
+        a.chunks = 1;
+        launch_table(a, 0, st);
         return;
     }
     const int64_t matrices = a.rows / a.queries;
@@ -618,10 +624,7 @@ void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStrea
             });
         }
     });
-    if (a.table_grad) {
-        const int buckets = a.buckets.both ? 2 * a.buckets.n : a.buckets.n;
-        bias_grad_table_kernel<<<(unsigned)((a.heads * buckets + 3) / 4), 256, 0, st>>>(a.partial, matrices, a.chunks, a.heads, buckets, a.table_grad);
-    }
+    if (a.table_grad) launch_table(a, matrices, st);
 }
 
 }  // namespace hpt

@@ -280,7 +280,8 @@ int32_t hpt_hip_add_layernorm(int32_t dev, void* stream, const hpt_view* in, con
  * their gradients. Dtypes f16, bf16 and f32; statistics, sums and the results called f32 below are f32 for all
  * of them, and every result is rounded once. A row's elements must be neighbours in memory, its rows may lie
  * anywhere; every other operand and every result is contiguous. Results share no memory with each other or with
- * operands, except that one may take the very place of an operand where its entry says so.
+ * operands, except that one may take the very place of an operand where its entry says so. An operand that is read
+ * several times (rows of stride 0, a table that heads share) has its gradients at every place: whoever broadcast it sums them.
  *
  * `workspace` (may be NULL) is contiguous device memory of any dtype, aligned to 16 bytes, of at least as many
  * bytes as the entry's *_workspace function says; nothing in it has to start from a known value. Without one
