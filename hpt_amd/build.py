@@ -126,20 +126,23 @@ def build_calls(force: bool = False) -> Path | None:
 
 HOST_TEST_SRC = ROOT.parent / "tests" / "cpp" / "host_api_test.cpp"
 HOST_TEST_BIN = ROOT / "lib" / "host_api_test"
+BLOCK_TEST_SRC = ROOT.parent / "tests" / "cpp" / "block_api_test.cpp"
+BLOCK_TEST_BIN = ROOT / "lib" / "block_api_test"
 
 
 def build_host_test(force: bool = False) -> Path:
-    """The C++ host side (include/hpt_hip.hpp) and its device test program, compiled with the host
+    """The C++ host side (include/hpt_hip.hpp) and its device test programs, compiled with the host
     compiler alone: the ABI is plain C, no HIP header is needed above it."""
-    deps = [HOST_TEST_SRC, INCLUDE / "hpt_hip.hpp", INCLUDE / "hpt_hip.h", LIB]
-    if not force and HOST_TEST_BIN.exists() and HOST_TEST_BIN.stat().st_mtime > max(d.stat().st_mtime for d in deps):
-        return HOST_TEST_BIN
-    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", f"-I{INCLUDE}", str(HOST_TEST_SRC),
-           "-o", str(HOST_TEST_BIN), f"-L{LIB.parent}", "-lhpt_hip", "-Wl,-rpath,$ORIGIN",
-           "-Wl,-rpath-link,/opt/rocm/lib"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("host test build failed:\n" + r.stderr)
+    for src, out in ((BLOCK_TEST_SRC, BLOCK_TEST_BIN), (HOST_TEST_SRC, HOST_TEST_BIN)):
+        deps = [src, INCLUDE / "hpt_hip.hpp", INCLUDE / "hpt_hip.h", LIB]
+        if not force and out.exists() and out.stat().st_mtime > max(d.stat().st_mtime for d in deps):
+            continue
+        cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", f"-I{INCLUDE}", str(src),
+               "-o", str(out), f"-L{LIB.parent}", "-lhpt_hip", "-Wl,-rpath,$ORIGIN",
+               "-Wl,-rpath-link,/opt/rocm/lib"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("host test build failed:\n" + r.stderr)
     return HOST_TEST_BIN
 
 

@@ -19,6 +19,8 @@
 //   argmax argmin                                 IndexReduce   (:6-42)
 //   softmax log_softmax layernorm                 NormalizationOps (hpt-traits/src/ops/normalization.rs:6-64)
 //   contiguous astype add_ sub_ mul_ div_         Contiguous, astype, NormalBinOps
+//   rms_norm add_rms_norm rms_norm_quant softmax_bias token_logp policy_loss and their *_backward
+//                                                 no trait: the operators around a transformer's blocks (hpt_hip.h)
 //
 // Errors are thrown as hpt::TensorError, whose `kind` is the TensorError variant the Rust shim
 // would return (hpt-common/src/error/base.rs:8-45) and whose text is the library's.
@@ -33,6 +35,7 @@
 #include <stdexcept>
 #include <string>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "hpt_hip.h"
@@ -143,6 +146,24 @@ inline Shape contiguous_strides(const Shape& shape) {
     }
     return st;
 }
+
+// How softmax_bias places queries and keys and what it hides (hpt_hip.h).
+template <class T> class Tensor;
+struct PositionBias {
+    double scale = 1.0;
+    bool bidirectional = true;
+    int64_t max_distance = 128;
+    int64_t query_offset = 0;
+    bool causal = false;
+    const Tensor<int64_t>* lengths = nullptr;
+};
+// What policy_loss weighs and clips, and what it returns.
+struct PolicyTerms {
+    const Tensor<float>* reference = nullptr;
+    const Tensor<float>* mask = nullptr;
+    double clip_low = 0.2, clip_high = 0.2, kl_weight = 0.0;
+};
+struct PolicyLoss;
 
 template <class T> class Tensor {
   public:
@@ -367,6 +388,80 @@ template <class T> class Tensor {
         return res;
     }
 
+    // ---- operators around a transformer's blocks (T: f16, bf16 or float) -----------------------------
+    Tensor rms_norm(const Shape& normalized_shape, const Tensor* gamma, double eps = 1e-6) const {
+        Tensor res = empty(shape_, device_);
+        hpt_view vin = view(), vout = res.view(), vg{};
+        check(hpt_hip_rms_norm(device_, nullptr, &vin, nullptr, norm_dims(normalized_shape), optional(gamma, vg), eps, nullptr, &vout));
+        return res;
+    }
+    // (the norm of the sum, the sum)
+    std::pair<Tensor, Tensor> add_rms_norm(const Tensor& residual, const Shape& normalized_shape, const Tensor* gamma, double eps = 1e-6) const {
+        Tensor res = empty(shape_, device_), sum = empty(shape_, device_);
+        hpt_view vin = view(), vr = residual.view(), vout = res.view(), vs = sum.view(), vg{};
+        check(hpt_hip_rms_norm(device_, nullptr, &vin, &vr, norm_dims(normalized_shape), optional(gamma, vg), eps, &vs, &vout));
+        return {res, sum};
+    }
+    // (values, scales): Q is int8_t, or uint8_t for the bits of e4m3
+    template <class Q>
+    std::pair<Tensor<Q>, Tensor<float>> rms_norm_quant(const Shape& normalized_shape, const Tensor* gamma, double eps = 1e-6, int64_t group = 0) const {
+        static_assert(std::is_same<Q, int8_t>::value || std::is_same<Q, uint8_t>::value, "8-bit results");
+        const int32_t nn = norm_dims(normalized_shape);
+        int64_t cols = 1;
+        for (int64_t d : normalized_shape) cols *= d;
+        if (group < 0 || (group > 0 && cols % group)) throw TensorError(ErrorKind::Shape, "rms_norm_quant: groups do not divide the rows");
+        Shape lead(shape_.begin(), shape_.end() - nn);
+        if (group > 0) lead.push_back(cols / group);
+        if (lead.empty()) lead.push_back(1);
+        Tensor<Q> res = Tensor<Q>::empty(shape_, device_);
+        Tensor<float> scale = Tensor<float>::empty(lead, device_);
+        hpt_view vin = view(), vout = res.view(), vs = scale.view(), vg{};
+        check(hpt_hip_rms_norm_quant(device_, nullptr, &vin, nullptr, nn, optional(gamma, vg), eps,
+                                     std::is_same<Q, int8_t>::value ? HPT_QUANT_I8 : HPT_QUANT_E4M3, group, nullptr, &vout, &vs));
+        return {res, scale};
+    }
+    // (gradient of this tensor, gradient of gamma)
+    std::pair<Tensor, Tensor<float>> rms_norm_backward(const Tensor& grad, const Shape& normalized_shape, const Tensor* gamma, double eps = 1e-6,
+                                                       const Tensor* grad_sum = nullptr) const {
+        Tensor res = empty(shape_, device_);
+        Tensor<float> gg = Tensor<float>::empty(normalized_shape, device_);
+        hpt_view vin = view(), vgrad = grad.view(), vout = res.view(), vgg = gg.view(), vg{}, vm{};
+        check(hpt_hip_rms_norm_backward(device_, nullptr, &vin, &vgrad, optional(grad_sum, vm), norm_dims(normalized_shape), optional(gamma, vg), eps,
+                                        nullptr, &vout, &vgg));
+        return {res, gg};
+    }
+    Tensor softmax_bias(const Tensor& table, const PositionBias& b) const {
+        Tensor res = empty(shape_, device_);
+        hpt_view vin = view(), vt = table.view(), vout = res.view(), vl{};
+        check(hpt_hip_softmax_bias(device_, nullptr, &vin, b.scale, &vt, b.bidirectional, b.max_distance, b.query_offset, b.causal,
+                                   optional(b.lengths, vl), nullptr, &vout));
+        return res;
+    }
+    // of softmax_bias's result: (gradient of the scores, gradient of the table)
+    std::pair<Tensor, Tensor<float>> softmax_bias_backward(const Tensor& grad, int64_t buckets, const PositionBias& b) const {
+        if (ndim() < 3) throw TensorError(ErrorKind::Shape, "softmax_bias_backward: needs at least 3 dims (heads x queries x keys)");
+        Tensor res = empty(shape_, device_);
+        Tensor<float> gt = Tensor<float>::empty({buckets, shape_[ndim() - 3]}, device_);
+        hpt_view vin = view(), vg = grad.view(), vout = res.view(), vt = gt.view(), vl{};
+        check(hpt_hip_softmax_bias_backward(device_, nullptr, &vin, &vg, b.scale, b.bidirectional, b.max_distance, b.query_offset, b.causal,
+                                            optional(b.lengths, vl), nullptr, &vout, &vt));
+        return {res, gt};
+    }
+    // (log-probability of each row's token, log of the sum of exponentials)
+    std::pair<Tensor<float>, Tensor<float>> token_logp(const Tensor<int64_t>& token) const {
+        Tensor<float> logp = Tensor<float>::empty(rows_shape(), device_), lse = Tensor<float>::empty(rows_shape(), device_);
+        hpt_view vin = view(), vt = token.view(), vp = logp.view(), vl = lse.view();
+        check(hpt_hip_token_logp(device_, nullptr, &vin, &vt, nullptr, &vp, &vl));
+        return {logp, lse};
+    }
+    PolicyLoss policy_loss(const Tensor<int64_t>& token, const Tensor<float>& old_logp, const Tensor<float>& advantage, const PolicyTerms& terms) const;
+    Tensor policy_loss_backward(const Tensor<int64_t>& token, const Tensor<float>& lse, const Tensor<float>& weight, double grad = 1.0) const {
+        Tensor res = empty(shape_, device_);
+        hpt_view vin = view(), vt = token.view(), vl = lse.view(), vw = weight.view(), vout = res.view();
+        check(hpt_hip_policy_loss_backward(device_, nullptr, &vin, &vt, &vl, &vw, grad, &vout));
+        return res;
+    }
+
     // ---- the steps either side ---------------------------------------------------------------------
     Tensor contiguous() const {
         Tensor res = empty(shape_, device_);
@@ -408,6 +503,18 @@ template <class T> class Tensor {
     int device_ = 0;
     bool is_view_ = false;  // Hpt's `parent.is_some()`
 
+    template <class U> static const hpt_view* optional(const Tensor<U>* t, hpt_view& v) {
+        if (!t) return nullptr;
+        v = t->view();
+        return &v;
+    }
+    int32_t norm_dims(const Shape& normalized_shape) const {
+        bool ok = !normalized_shape.empty() && (int)normalized_shape.size() <= ndim();
+        for (size_t i = 0; ok && i < normalized_shape.size(); ++i) ok = shape_[ndim() - normalized_shape.size() + i] == normalized_shape[i];
+        if (!ok) throw TensorError(ErrorKind::Shape, "normalized dims must match last dims of input tensor");
+        return (int32_t)normalized_shape.size();
+    }
+    Shape rows_shape() const { return ndim() > 1 ? Shape(shape_.begin(), shape_.end() - 1) : Shape{1}; }
     Tensor alias() const {
         Tensor t = *this;
         t.is_view_ = true;
@@ -463,6 +570,21 @@ template <class T> class Tensor {
         return res;
     }
 };
+
+struct PolicyLoss {
+    Tensor<float> loss, logp, lse, weight;  // loss: one element; the others: one for each row
+};
+template <class T>
+PolicyLoss Tensor<T>::policy_loss(const Tensor<int64_t>& token, const Tensor<float>& old_logp, const Tensor<float>& advantage,
+                                  const PolicyTerms& terms) const {
+    auto rows = [&] { return Tensor<float>::empty(rows_shape(), device_); };
+    PolicyLoss r{Tensor<float>::empty({1}, device_), rows(), rows(), rows()};
+    hpt_view vin = view(), vt = token.view(), vo = old_logp.view(), va = advantage.view(), vr{}, vm{};
+    hpt_view v0 = r.loss.view(), v1 = r.logp.view(), v2 = r.lse.view(), v3 = r.weight.view();
+    check(hpt_hip_policy_loss(device_, nullptr, &vin, &vt, &vo, &va, optional(terms.reference, vr), optional(terms.mask, vm), terms.clip_low,
+                              terms.clip_high, terms.kl_weight, nullptr, &v0, &v1, &v2, &v3));
+    return r;
+}
 
 inline int device_count() {
     int32_t n = 0;

@@ -216,6 +216,16 @@ def test_threads(hpt, dev, hip):
     assert not errors, errors
 
 
+def test_the_cpp_host_side():
+    """The prebuilt program hpt_amd/lib/block_api_test (source tests/cpp/block_api_test.cpp)."""
+    import subprocess
+
+    from hpt_amd import build
+    assert build.BLOCK_TEST_BIN.exists(), f"{build.BLOCK_TEST_BIN} is missing: run `python -m hpt_amd.build`"
+    r = subprocess.run([str(build.BLOCK_TEST_BIN)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and " 0 failures" in r.stdout, f"{r.stdout}\n{r.stderr}"
+
+
 # ---- more than 2^31 elements ---------------------------------------------------------------------------
 
 def test_rows_beyond_two_to_the_31(hpt, dev):
