@@ -91,7 +91,7 @@ struct Buckets {
     int n = 0;
     int both = 0;
     int far = 0;  // begin[n - 1]
-    uint16_t begin[kMostBuckets] = {};
+    alignas(16) uint16_t begin[kMostBuckets] = {};  // from n on larger than any distance
 };
 
 // Throws where no such buckets exist.

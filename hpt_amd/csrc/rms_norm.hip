@@ -466,8 +466,28 @@ __global__ __launch_bounds__(1024) void rms_grad_columns_kernel(const float* par
     }
 }
 
-// (two vectors per thread, four of f32: with more the accumulators spill)
-RowDeal grad_deal(int dtype, int64_t cols) { return deal_row(cols, dtype_size(dtype), 2, dtype == HPT_F32 ? 4 : 2); }
+// Two vectors per thread, four of f32: with more the accumulators spill. `more`: a third operand. With it a row of two-byte elements goes to four or
+// to eight wavefronts: of five (a second one on one of the four SIMDs) fewer workgroups run at once: us, bf16 [13107, 5120] 184 with 320 threads, 141 with 512,
+// but 90 against 112 without a third operand, where three workgroups of five wavefronts have room.
+RowDeal grad_deal(int dtype, int64_t cols, bool more) {
+    RowDeal d = deal_row(cols, dtype_size(dtype), 2, dtype == HPT_F32 ? 4 : 2);
+    if (dtype != HPT_F32 && more && d.threads > 256 && d.threads < 512) d.tpr = d.threads = 512;
+    return d;
+}
+// As many workgroups as run at once; in more, the last round is mostly empty, in fewer, memory waits. That is four wavefronts on each SIMD of two-byte
+// elements, five without a third operand where a row has four at most: us, bf16 [16384, 4096] and a third operand 512 workgroups 170, 768 125, 1024 108,
+// 1280 145; [16384, 4096] without 86 in 1024, 82 in 1280. Of f32 three and two are enough, and more meet in memory: [32768, 1024] and a third operand 99 in 1024, 105
+// in 2048, [16384, 2048] 98 in 512, 105 in 1024.
+// Few rows: near two to a workgroup, each of which leaves a row of partial sums, and the same on every compute unit: f32 [1237, 1001] 12.0 in 512, 12.6 in 618,
+// 11.5 in 768, 13.7 in 1237.
+int64_t grad_parts(int dtype, int64_t rows, int64_t cols, bool more) {
+    const RowDeal d = grad_deal(dtype, cols, more);
+    const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
+    const int waves = d.threads / 64;
+    const int64_t resident = 256 * (dtype == HPT_F32 ? std::max(2, (more ? 8 : 12) / waves) : std::max(1, (more || waves > 4 ? 16 : 20) / waves));
+    // (256 MiB of partial sums at most)
+    return std::min({blocks, resident, std::max<int64_t>(512, blocks * 5 / 8 / 256 * 256), std::max<int64_t>(1, (64 << 20) / std::max<int64_t>(1, cols))});
+}
 
 }  // namespace
 
@@ -479,21 +499,13 @@ void launch_rms_norm(int dtype, int quant, const RmsArgs& a, hipStream_t st) {
     });
 }
 
-int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) {
-    const RowDeal d = grad_deal(dtype, cols);
-    const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
-    // As many workgroups as run at once, four wavefronts on each SIMD: in more, the last round is mostly empty, in fewer, memory waits. us, bf16
-    // [16384, 4096] 512 workgroups 129, 768 98, 1024 85, 2048 93; f16 [8000, 8192] 512 88, 1024 94, 2048 108; bf16 [6000, 5120] 768 48, 1024 61.
-    // Few rows: two to a workgroup, as each leaves a row of partial sums ([1000, 4096] 16.3 in 1000 workgroups, 13.6 in 512).
-    const int64_t resident = 256 * std::max(1, 16 / (d.threads / 64));
-    // (256 MiB of them at most)
-    return std::min({blocks, resident, std::max<int64_t>(512, blocks / 2), std::max<int64_t>(1, (64 << 20) / std::max<int64_t>(1, cols))});
-}
+// (The caller of a workspace's size does not say whether there is a third operand.)
+int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) { return std::max(grad_parts(dtype, rows, cols, false), grad_parts(dtype, rows, cols, true)); }
 
 void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
     RmsGradArgs a = given;
-    const RowDeal d = grad_deal(dtype, a.cols);
-    const int64_t parts = rms_grad_partials(dtype, a.rows, a.cols);  // (no rows: none, and gamma's gradient is zeros)
+    const RowDeal d = grad_deal(dtype, a.cols, a.gsum);
+    const int64_t parts = grad_parts(dtype, a.rows, a.cols, a.gsum);  // (no rows: none, and gamma's gradient is zeros)
     a.tpr = d.tpr;
     const size_t lds = d.rows_per_block() > 1 ? (size_t)a.cols * 4 : 0;
     if (parts) HPT_WITH_TYPE(dtype, {

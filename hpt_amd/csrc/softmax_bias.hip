@@ -39,17 +39,23 @@ Buckets make_buckets(int64_t total, bool both, int64_t max_distance) {
         b.begin[half + j] = (uint16_t)std::ceil(at * (1 - 1e-9));
     }
     b.far = b.begin[b.n - 1];
+    std::fill(b.begin + b.n, b.begin + kMostBuckets, (uint16_t)0xffff);
     return b;
 }
 
 namespace {
 
-// (Counted along `begin`, which every lane reads at the same place: a search would wait for one load after the other.)
+// (Counted along `begin`, eight at a time, which every lane reads at the same place: a search would wait for one load after the other.)
 __device__ __forceinline__ int bucket_of(const Buckets& b, int d) {
-    const int far = d < 0 ? -d : b.both ? d : 0, half = b.n / 2;
-    int k = min(far, half);
-#pragma unroll 4
-    for (int j = half + 1; j < b.n; ++j) k += (int)b.begin[j] <= far;
+    typedef uint32_t Eight __attribute__((ext_vector_type(4), may_alias));
+    const int far = d < 0 ? -d : b.both ? d : 0, first = b.n / 2 & ~7;  // below it a bucket is its distance
+    int k = min(far, first - 1);
+#pragma unroll 2
+    for (int j = first; j < b.n; j += 8) {
+        const Eight e = *(const Eight*)(b.begin + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k += ((int)(e[i] & 0xffff) <= far) + ((int)(e[i] >> 16) <= far);
+    }
     return k + (d > 0 && b.both ? b.n : 0);
 }
 // Places by distance in LDS: -far ... right, and a vector's length more on both sides, so that a vector that reaches into the range, from
@@ -529,15 +535,44 @@ bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
 
-// A workgroup holds rows of one matrix: where that has few (a step of decoding has one), down to a wavefront.
+// Four vectors per thread: a row's maximum and sum cost the same for two. us, f16 [8, 16, 256 queries or so, keys] of 65 vectors 78 with two, 61.5 with up to
+// four, of 129 84 and 58, of 128 56.3 and 54.7.
+// Rows above a wavefront go to workgroups of 128, 256, 512 or 768 threads with three or four vectors each (f32 four to six): a fifth wavefront shares a
+// SIMD with the first, and then fewer workgroups run at once. us, f16 [1, 16, 256, 8208 keys and more], 320 threads of two vectors 69, 256 of three 50;
+// [.., 6144] 384 of two 58, 256 of three 39; one query, [64, 32, 1, 4104] 320 of two 20.3, 256 of three 14.3; f32 [.., 4400] 320 of four 35.9, 256 of five 27.2.
+// (385 ... 512 two-byte vectors: of whole matrices 256 threads of two 49, 128 of four 55; of one query 12.3 and 10.4.)
+// A workgroup holds rows of one matrix: where that has few (a step of decoding has one), they get the lanes of a wavefront (f32 [128, 16, 1, 256] 6.0 with 64, 7.2 with 16),
+// and the workgroup is no larger than they need.
 RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) {
-    RowDeal d = deal_row(keys, dtype_size(dtype), dtype == HPT_F32 ? 4 : 2, most_vecs(dtype));  // (16 elements a thread: f32 of two vectors 94 us, of four 86, [4, 16, 1024, 1024])
+    const bool wide = dtype == HPT_F32;
+    const int64_t vecs = (keys * (int64_t)dtype_size(dtype) + 15) / 16;
+    RowDeal d = deal_row(keys, dtype_size(dtype), 4, most_vecs(dtype));
+    if (!d.held()) return d;
+    if (d.tpr > 64) {
+        const int64_t fit[] = {wide ? 512 : queries == 1 ? 512 : 384, wide ? 1536 : 1024, wide ? 4096 : 2048, wide ? 0 : 2304};
+        const int threads[] = {128, 256, 512, 768};
+        d.tpr = 1024;
+        for (int i = 3; i >= 0; --i)
+            if (vecs <= fit[i]) d.tpr = threads[i];
+        d.threads = d.tpr;
+    }
+    while (d.tpr < 64 && queries * d.tpr < 64) d.tpr *= 2;
+    d.nc = (int)((vecs + d.tpr - 1) / d.tpr);
     while (d.tpr <= 64 && d.threads > 64 && d.threads / 2 >= queries * d.tpr) d.threads /= 2;
     return d;
 }
-// Backward: two vectors per thread, four of f32, of two operands; 32 rows side by side at most, because each of them has places of its own.
+// Backward: two vectors per thread of two operands, four of f32 (two-byte elements with three and four: us, bf16 [.., 256 queries, keys] of 65 vectors 121 and 121, of 384 84
+// and 98, of 512 83 and 106), but one where two would leave a third of the lanes idle or so, 129 ... 256 vectors (of 150 101 and 93, of 192 90 and 83, of 256 87 and 82). 32 rows side
+// by side at most, because each of them has places of its own. 768 threads are three wavefronts on each SIMD: [1, 16, 256, 9600] with 640 threads 69, with 768 63; f32 [.., 8196] 95 and 83.
 RowDeal bias_grad_deal(int dtype, int64_t keys) {
-    return deal_row(keys, dtype_size(dtype), dtype == HPT_F32 ? 4 : 2, dtype == HPT_F32 ? 4 : 2, 8);
+    const bool wide = dtype == HPT_F32;
+    const int64_t vecs = (keys * (int64_t)dtype_size(dtype) + 15) / 16;
+    RowDeal d = deal_row(keys, dtype_size(dtype), wide ? 4 : vecs > 128 && vecs <= 256 ? 1 : 2, wide ? 4 : 2, 8);
+    if (d.held() && d.threads > 512 && d.threads < 768) {
+        d.tpr = d.threads = 768;
+        d.nc = (int)((vecs + 767) / 768);
+    }
+    return d;
 }
 // Rows of a matrix that a workgroup takes one after the other, in rounds of those side by side: 96 KiB of operands and results for 256 threads
 // (each workgroup fetches its bias or clears its places first), 64 rows at most, but so that there are 512 workgroups. us, forward / backward, for 64, 96 and 128 KiB: bf16 [4, 16, 1024, 1024], causal, 52 / 69, 49 / 65, 58 / 67, [2, 16, 2048, 2048], causal,
