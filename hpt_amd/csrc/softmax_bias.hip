@@ -542,8 +542,9 @@ size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
 // [.., 6144] 384 of two 58, 256 of three 39; one query, [64, 32, 1, 4104] 320 of two 20.3, 256 of three 14.3; f32 [.., 4400] 320 of four 35.9, 256 of five 27.2.
 // (385 ... 512 two-byte vectors: of whole matrices 256 threads of two 49, 128 of four 55; of one query 12.3 and 10.4.)
 // A workgroup holds rows of one matrix: where that has few (a step of decoding has one), they get the lanes of a wavefront (f32 [128, 16, 1, 256] 6.0 with 64, 7.2 with 16),
-// and the workgroup is no larger than they need.
-RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) {
+// and the workgroup is no larger than they need. Up to four rows of one query for each compute unit get up to four wavefronts, as the latency of a row is
+// all there is: f16 [16, 32, 1, 2048] 6.0 with 256 threads, 7.1 with 64, f32 [16, 32, 1, 1000] 5.9 and 7.0; f16 [128, 16, 1, 1536] 7.3 with 64, 8.2 with 128.
+RowDeal bias_deal(int dtype, int64_t rows, int64_t queries, int64_t keys) {
     const bool wide = dtype == HPT_F32;
     const int64_t vecs = (keys * (int64_t)dtype_size(dtype) + 15) / 16;
     RowDeal d = deal_row(keys, dtype_size(dtype), 4, most_vecs(dtype));
@@ -557,6 +558,7 @@ RowDeal bias_deal(int dtype, int64_t queries, int64_t keys) {
         d.threads = d.tpr;
     }
     while (d.tpr < 64 && queries * d.tpr < 64) d.tpr *= 2;
+    if (queries == 1 && rows <= 1024 && d.tpr < 256 && vecs > 64) d.tpr = d.threads = (int)std::min<int64_t>(256, (vecs + 63) / 64 * 64);
     d.nc = (int)((vecs + d.tpr - 1) / d.tpr);
     while (d.tpr <= 64 && d.threads > 64 && d.threads / 2 >= queries * d.tpr) d.threads /= 2;
     return d;
@@ -597,7 +599,7 @@ void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
     const int64_t matrices = a.rows / a.queries;
     HPT_WITH_TYPE(dtype, {
         constexpr int VEC = 16 / sizeof(T);
-        const RowDeal d = bias_deal(dtype, a.queries, a.keys);
+        const RowDeal d = bias_deal(dtype, a.rows, a.queries, a.keys);
         if (a.split > 1) {
             const unsigned grid = (unsigned)(a.rows * a.split);
             bias_split_kernel<T, false><<<grid, 256, lds, st>>>(a);

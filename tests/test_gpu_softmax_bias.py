@@ -108,6 +108,17 @@ def test_forward(hpt, dev, name, c):
     assert np.array_equal(again.numpy(), out.numpy())
 
 
+# Where the deal of a row to threads changes: one row of few, one of many, and whole matrices, one vector to both sides.
+EDGES = [(1, 2, q, n, 32, True, 64, q // 2 + n // 2, False, None) for n in (1016, 1025, 1031, 2047, 2049, 3079, 4105, 6145, 8200, 9217, 16391, 18440) for q in (1, 5)] + [
+    (8, 130, 1, n, 16, False, 32, n - 1, True, None) for n in (130, 513, 1030, 2056, 3085)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("c", EDGES, ids=ids)
+def test_edges_of_the_deal(hpt, dev, name, c):
+    test_forward(hpt, dev, name, c)
+
+
 @pytest.mark.parametrize("total,both,most", [(32, True, 128), (32, False, 128), (16, True, 64), (2, False, 2), (4, True, 2), (256, True, 4096), (256, False, 4096), (6, True, 1000),
                                              (7, False, 33), (64, True, 17)])
 def test_every_distance_is_in_its_bucket(hpt, dev, total, both, most):
@@ -258,6 +269,12 @@ def test_backward(hpt, dev, name, c):
     gr, _ = k.up(np.where(live, g, 0))
     a, b = t.softmax_bias_backward(gr, total, 0.3, lengths=ln, out=t, **args_of(c))
     assert np.array_equal(a.numpy(), out.numpy()) and np.array_equal(b.numpy(), tg.numpy())
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n", [510, 520, 1033, 2047, 2056, 4104, 6160, 9000])
+def test_edges_of_the_backward_deal(hpt, dev, name, n):
+    test_backward(hpt, dev, name, (1, 2, 37, n, 32, True, 64, n // 2, False, None))
 
 
 def test_backward_without_rows_or_table(hpt, dev):
