@@ -37,26 +37,30 @@ template <int VEC, bool AL> struct Slot {
     }
 };
 
-// The slot's own elements, zeros in the other places.
+// The slot's vector, with what it holds of the one before; zeros where it has no element.
 template <class T, bool AL> __device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_slot(const T* row, const Slot<16 / sizeof(T), AL>& at) {
     constexpr int VEC = 16 / sizeof(T);
     Pack<T, VEC> p;
     if (at.lo < VEC) {
         if constexpr (AL) p = load_pack<T, VEC>(row + at.s);
         else p = load_pack_unaligned<T, VEC>(row + at.s);
-        if constexpr (!AL) {
-            if (at.lo) {
-                T zero;
-                __builtin_memset(&zero, 0, sizeof zero);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    if (i < at.lo) p.v[i] = zero;
-            }
-        }
     } else {
         __builtin_memset(&p, 0, sizeof p);
     }
     return p;
+}
+// Zeros in the places that are the vector's before. (Apart from the load, behind all of a row's: next to it, each load would be waited for before the next one
+// is made: softmax with a bias f16 [1, 32, 1, 4097] 7.5 -> 7.0 us, norm f32 [3000, 7001] 33 -> 28.)
+template <class T, bool AL> __device__ __forceinline__ void clean_slot(Pack<T, 16 / sizeof(T)>& p, const Slot<16 / sizeof(T), AL>& at) {
+    constexpr int VEC = 16 / sizeof(T);
+    if constexpr (!AL) {
+        if (__any(at.lo & (VEC - 1))) {
+            T zero;
+            __builtin_memset(&zero, 0, sizeof zero);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) p.v[i] = i < at.lo ? zero : p.v[i];
+        }
+    }
 }
 
 // Only the slot's own elements are written: those before belong to another thread, which may not have read them yet where the result

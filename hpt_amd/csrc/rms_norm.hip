@@ -78,6 +78,8 @@ __global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {
     if (a.gamma) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) g[k] = load_slot<T, AL>((const T*)a.gamma, At(lane + k * tpr, a.cols));
+#pragma unroll
+        for (int k = 0; k < NC; ++k) clean_slot<T, AL>(g[k], At(lane + k * tpr, a.cols));
     }
     const int64_t step = (int64_t)gridDim.x * rpb;
     Pack<T, VEC> p[NC], q[RES ? NC : 1];
@@ -104,6 +106,7 @@ __global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) h[k].v[i] = Elem<T>::narrow(Elem<T>::widen(p[k].v[i]) + Elem<T>::widen(q[k].v[i]));
             }
+            clean_slot<T, AL>(h[k], At(lane + k * tpr, cols));
         }
         if constexpr (kAhead<T, NC, RES, Q>) {
             if (first + step < a.rows) fetch(row + step);
@@ -320,6 +323,8 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
     if (a.gamma) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) g[k] = load_slot<T, AL>((const T*)a.gamma, At(lane + k * tpr, a.cols));
+#pragma unroll
+        for (int k = 0; k < NC; ++k) clean_slot<T, AL>(g[k], At(lane + k * tpr, a.cols));
     }
     float acc[NC][VEC] = {};
     for (int64_t first = (int64_t)blockIdx.x * rpb; first < a.rows; first += (int64_t)gridDim.x * rpb) {
@@ -338,6 +343,8 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
+            clean_slot<T, AL>(x[k], At(lane + k * tpr, cols));
+            clean_slot<T, AL>(gy[k], At(lane + k * tpr, cols));
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float xv = Elem<T>::widen(x[k].v[i]);
@@ -475,16 +482,16 @@ RowDeal grad_deal(int dtype, int64_t cols, bool more) {
     return d;
 }
 // As many workgroups as run at once; in more, the last round is mostly empty, in fewer, memory waits. That is four wavefronts on each SIMD of two-byte
-// elements, five without a third operand where a row has four at most: us, bf16 [16384, 4096] and a third operand 512 workgroups 170, 768 125, 1024 108,
+// elements, five (`five`) without a third operand in whole, aligned vectors where a row has four at most ([20000, 513] off the grid 26 in 1024, 33 in 1280): us, bf16 [16384, 4096] and a third operand 512 workgroups 170, 768 125, 1024 108,
 // 1280 145; [16384, 4096] without 86 in 1024, 82 in 1280. Of f32 three and two are enough, and more meet in memory: [32768, 1024] and a third operand 99 in 1024, 105
 // in 2048, [16384, 2048] 98 in 512, 105 in 1024.
 // Few rows: near two to a workgroup, each of which leaves a row of partial sums, and the same on every compute unit: f32 [1237, 1001] 12.0 in 512, 12.6 in 618,
 // 11.5 in 768, 13.7 in 1237.
-int64_t grad_parts(int dtype, int64_t rows, int64_t cols, bool more) {
+int64_t grad_parts(int dtype, int64_t rows, int64_t cols, bool more, bool five) {
     const RowDeal d = grad_deal(dtype, cols, more);
     const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
     const int waves = d.threads / 64;
-    const int64_t resident = 256 * (dtype == HPT_F32 ? std::max(2, (more ? 8 : 12) / waves) : std::max(1, (more || waves > 4 ? 16 : 20) / waves));
+    const int64_t resident = 256 * (dtype == HPT_F32 ? std::max(2, (more ? 8 : 12) / waves) : std::max(1, (five && waves <= 4 ? 20 : 16) / waves));
     // (256 MiB of partial sums at most)
     return std::min({blocks, resident, std::max<int64_t>(512, blocks * 5 / 8 / 256 * 256), std::max<int64_t>(1, (64 << 20) / std::max<int64_t>(1, cols))});
 }
@@ -500,17 +507,18 @@ void launch_rms_norm(int dtype, int quant, const RmsArgs& a, hipStream_t st) {
 }
 
 // (The caller of a workspace's size does not say whether there is a third operand.)
-int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) { return std::max(grad_parts(dtype, rows, cols, false), grad_parts(dtype, rows, cols, true)); }
+int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) { return std::max(grad_parts(dtype, rows, cols, false, true), grad_parts(dtype, rows, cols, true, false)); }
 
 void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
     RmsGradArgs a = given;
     const RowDeal d = grad_deal(dtype, a.cols, a.gsum);
-    const int64_t parts = grad_parts(dtype, a.rows, a.cols, a.gsum);  // (no rows: none, and gamma's gradient is zeros)
+    const int vec = 16 / (int)dtype_size(dtype);
+    const bool al = a.cols % vec == 0 && rows_on_grid(a.x, a.kept, vec) && on_grid(a.gy) && on_grid(a.gsum) && on_grid(a.gamma) && on_grid(a.gx);
+    const int64_t parts = grad_parts(dtype, a.rows, a.cols, a.gsum, al && !a.gsum);  // (no rows: none, and gamma's gradient is zeros)
     a.tpr = d.tpr;
     const size_t lds = d.rows_per_block() > 1 ? (size_t)a.cols * 4 : 0;
     if (parts) HPT_WITH_TYPE(dtype, {
         constexpr int VEC = 16 / sizeof(T);
-        const bool al = a.cols % VEC == 0 && rows_on_grid(a.x, a.kept, VEC) && on_grid(a.gy) && on_grid(a.gsum) && on_grid(a.gamma) && on_grid(a.gx);
         if (!d.held() || a.cols < VEC) {
             rms_grad_stream_kernel<T><<<(unsigned)parts, 1024, 0, st>>>(a);
         } else {

@@ -408,6 +408,8 @@ __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_ke
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
                 const At at(lane + k * tpr, a.keys);
+                clean_slot<T, AL>(pp[k], at);
+                clean_slot<T, AL>(gp[k], at);
                 if (at.s + VEC > live) {  // the last live vector: hidden elements become zeros
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
