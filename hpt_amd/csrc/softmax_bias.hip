@@ -114,7 +114,8 @@ __device__ __forceinline__ void biased(const Pack<T, VEC>& p, int e, int lo, int
 }
 
 // Rows held in registers. An item is `per_item` rows of one matrix; the first row is on its way while the bias comes together, every other
-// one while the row before it is summed and written.
+// one while the row before it is summed and written. bf16 [8, 16, 1024, 1024] with lengths 92 us, 4.9 TB/s: next to memory, the bias by distance and an
+// exponential for every element. One query, f16 [16, 32, 1, 4097], 7.8 us: bias, loads, two folds and the store follow one another.
 template <class T, int NC, bool AL>
 __global__ __launch_bounds__(1024, NC <= 2 ? 5 : 4) void bias_row_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
@@ -374,6 +375,7 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, const float* pla
 // is, so that a vector's places are whole aligned quadruples: read, added to and written with 128-bit accesses that meet no bank
 // twice. (By single words, eight to a vector, every instruction met each bank eight times: 73 us of bf16 [16, 16, 256, 256] were theirs.)
 // Rows above a wavefront pass a barrier between two rows' additions (the fold); rows within one are kept in order by the fence.
+// bf16 [4, 16, 1024, 1024], causal, 61 us, 4.4 TB/s, and 4 us for the table; next to memory, the additions in LDS.
 template <class T, int NC, bool AL>
 __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);

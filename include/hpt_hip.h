@@ -343,7 +343,8 @@ int32_t hpt_hip_softmax_bias_backward(int32_t dev, void* stream, const hpt_view*
 int32_t hpt_hip_softmax_bias_backward_workspace(const hpt_view* probs, int64_t buckets, size_t* bytes);
 
 /* The log-probability of one token (i32 or i64) for each row of `logits` [..., vocabulary], and the row's log of the sum of
- * exponentials, both f32. A token outside the vocabulary has a NaN for logp. */
+ * exponentials, both f32. (A row whose LARGEST logit is beyond 2^24 in magnitude has an lse as coarse as f32 is there, and so has
+ * the gradient that is made from it; logp does not go through lse.) A token outside the vocabulary has a NaN for logp. */
 int32_t hpt_hip_token_logp(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* workspace,
                            hpt_view* logp, hpt_view* lse);
 
