@@ -345,14 +345,25 @@ __device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, in
 }
 
 // The workgroup's sums by distance -> by bucket, into its row of partial sums; eight lanes share a bucket. `places`: arrays of `length`, number g for
-// rows at positions pos + g modulo 4. Every thread of the workgroup comes here.
-__device__ __forceinline__ void leave_buckets(const Buckets& b, const float* places, int arrays, int length, int pos, float left_end, float right_end, float* out) {
+// rows at positions pos + g modulo 4. They become one first, each place by a thread that alone reads it in all of them (without that step, f16 [32, 12, 64, 64] 11.1 us, with it
+// 10.1; unrolled further it costs the rows' loop registers). Every thread of the workgroup comes here.
+__device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, int arrays, int length, int pos, float left_end, float right_end, float* out) {
     __shared__ float ends[2 * 16 * 2];
     const int total = b.both ? 2 * b.n : b.n, zero = b.far + kPad;
     float e[2] = {left_end, right_end};
     int turn = 0;
     fold_row<SumF>(e, blockDim.x, ends, turn);
     __syncthreads();  // (a single wavefront has passed none in the fold)
+    const int shift = shift_of(b, pos);
+    if (arrays > 1) {
+        for (int q = threadIdx.x; q < places_of(b); q += blockDim.x) {
+            float s = places[q + shift];
+#pragma unroll 2
+            for (int g = 1; g < arrays; ++g) s += places[g * length + q + shift_of(b, pos + g)];
+            places[q + shift] = s;
+        }
+        __syncthreads();
+    }
     const int part = threadIdx.x & 7;
     for (int k = threadIdx.x >> 3; k < total; k += blockDim.x >> 3) {
         const bool ahead = b.both && k >= b.n;
@@ -361,10 +372,8 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, const float* pla
         const int from = ahead && j == 0 ? 1 : !b.both && j == 0 ? -kPad : b.begin[j], to = j + 1 < b.n ? b.begin[j + 1] : b.far + kPad + 1;
         float s = part == 0 && j == b.n - 1 ? e[ahead] : 0.0f;
         if (part == 0 && !b.both && j == 0) s += e[1];
-        for (int d = from + part; d < to; d += 8) {
-            const float* at = places + (ahead ? zero + d : zero - d);
-            for (int g = 0; g < arrays; ++g) s += at[g * length + shift_of(b, pos + g)];
-        }
+        for (int d = from + part; d < to; d += 8)
+            s += places[(ahead ? zero + d : zero - d) + shift];
         s = group_reduce<SumF>(s, 8);
         if (part == 0) out[k] = s;
     }
