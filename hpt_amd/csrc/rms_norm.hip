@@ -388,8 +388,17 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
         }
         return;
     }
-    for (int t = 0; t < rpb; ++t) {  // the workgroup's rows one after the other: the same order always
-        if (t == ty) {
+    // The rows that share a wavefront by their lanes, then the wavefronts one after the other: the same order always. (All rows one after the other, 32 of them:
+    // bf16 [577, 90] 27 us, so 9.6, [131072, 64] 29.5 and 17.3.)
+    for (int w = tpr; w < 64; w <<= 1) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[k][i] += __shfl_xor(acc[k][i], w, 64);
+        }
+    }
+    for (int t = 0; t < (int)blockDim.x >> 6; ++t) {
+        if (t == (int)threadIdx.x >> 6 && (threadIdx.x & 63) < (unsigned)tpr) {
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
                 const At at(lane + k * tpr, a.cols);
