@@ -487,19 +487,25 @@ __global__ __launch_bounds__(1024) void rms_grad_columns_kernel(const float* par
 // Two vectors per thread, four of f32: with more the accumulators spill. `more`: a third operand. With it a row of two-byte elements goes to four or
 // to eight wavefronts: of five (a second one on one of the four SIMDs) fewer workgroups run at once: us, bf16 [13107, 5120] 184 with 320 threads, 141 with 512,
 // but 90 against 112 without a third operand, where three workgroups of five wavefronts have room.
-RowDeal grad_deal(int dtype, int64_t cols, bool more) {
-    RowDeal d = deal_row(cols, dtype_size(dtype), 2, dtype == HPT_F32 ? 4 : 2);
-    if (dtype != HPT_F32 && more && d.threads > 256 && d.threads < 512) d.tpr = d.threads = 512;
+// Two-byte rows above a wavefront have one vector per thread while each workgroup has few rows to walk, up to 48 MiB, of longer ones 16 MiB: us, bf16 [6000, 1608] 29 with two, 25
+// with one, [1500, 2353] 19 and 17, [500, 5120] 13.3 and 11.1, but [12000, 4096] 65 and 77.
+RowDeal grad_deal(int dtype, int64_t rows, int64_t cols, bool more) {
+    const bool wide = dtype == HPT_F32;
+    const int64_t vecs = (cols * (int64_t)dtype_size(dtype) + 15) / 16;
+    const bool one = !wide && vecs > 128 && vecs <= 1024 && rows * vecs <= (int64_t)(vecs <= 256 ? 3 : 1) << 20;
+    RowDeal d = deal_row(cols, dtype_size(dtype), one ? 1 : 2, wide ? 4 : 2);
+    if (!wide && more && d.nc > 1 && d.threads > 256 && d.threads < 512) d.tpr = d.threads = 512;
     return d;
 }
 // As many workgroups as run at once; in more, the last round is mostly empty, in fewer, memory waits. That is four wavefronts on each SIMD of two-byte
-// elements, five (`five`) without a third operand in whole, aligned vectors where a row has four at most ([20000, 513] off the grid 26 in 1024, 33 in 1280): us, bf16 [16384, 4096] and a third operand 512 workgroups 170, 768 125, 1024 108,
+// elements, five (`five`) of bf16 without a third operand in whole, aligned vectors where a row has four at most (f16 takes more registers: [51392, 640] 55 in 1024, 77
+// in 1280; bf16 [20000, 513] off the grid 26 and 33): us, bf16 [16384, 4096] and a third operand 512 workgroups 170, 768 125, 1024 108,
 // 1280 145; [16384, 4096] without 86 in 1024, 82 in 1280. Of f32 three and two are enough, and more meet in memory: [32768, 1024] and a third operand 99 in 1024, 105
 // in 2048, [16384, 2048] 98 in 512, 105 in 1024.
 // Few rows: near two to a workgroup, each of which leaves a row of partial sums, and the same on every compute unit: f32 [1237, 1001] 12.0 in 512, 12.6 in 618,
 // 11.5 in 768, 13.7 in 1237.
 int64_t grad_parts(int dtype, int64_t rows, int64_t cols, bool more, bool five) {
-    const RowDeal d = grad_deal(dtype, cols, more);
+    const RowDeal d = grad_deal(dtype, rows, cols, more);
     const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
     const int waves = d.threads / 64;
     const int64_t resident = 256 * (dtype == HPT_F32 ? std::max(2, (more ? 8 : 12) / waves) : std::max(1, (five && waves <= 4 ? 20 : 16) / waves));
@@ -522,10 +528,10 @@ int64_t rms_grad_partials(int dtype, int64_t rows, int64_t cols) { return std::m
 
 void launch_rms_norm_backward(int dtype, const RmsGradArgs& given, hipStream_t st) {
     RmsGradArgs a = given;
-    const RowDeal d = grad_deal(dtype, a.cols, a.gsum);
+    const RowDeal d = grad_deal(dtype, a.rows, a.cols, a.gsum);
     const int vec = 16 / (int)dtype_size(dtype);
     const bool al = a.cols % vec == 0 && rows_on_grid(a.x, a.kept, vec) && on_grid(a.gy) && on_grid(a.gsum) && on_grid(a.gamma) && on_grid(a.gx);
-    const int64_t parts = grad_parts(dtype, a.rows, a.cols, a.gsum, al && !a.gsum);  // (no rows: none, and gamma's gradient is zeros)
+    const int64_t parts = grad_parts(dtype, a.rows, a.cols, a.gsum, al && !a.gsum && dtype == HPT_BF16);  // (no rows: none, and gamma's gradient is zeros)
     a.tpr = d.tpr;
     const size_t lds = d.rows_per_block() > 1 ? (size_t)a.cols * 4 : 0;
     if (parts) HPT_WITH_TYPE(dtype, {
