@@ -382,9 +382,13 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
             const At at(lane + k * tpr, a.cols);
+            if (at.lo == 0) {
+                __builtin_memcpy(part + at.s, acc[k], sizeof acc[k]);
+            } else if constexpr (!AL) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (i >= at.lo) part[at.s + i] = acc[k][i];
+                for (int i = 1; i < VEC; ++i)
+                    if (i >= at.lo) part[at.s + i] = acc[k][i];
+            }
         }
         return;
     }

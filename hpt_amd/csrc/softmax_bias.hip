@@ -369,7 +369,7 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, i
         const bool ahead = b.both && k >= b.n;
         const int j = ahead ? k - b.n : k;
         // distances of bucket k: of its direction's last one also those of the margin; bucket 0 of a single direction has the other's margin
-        const int from = ahead && j == 0 ? 1 : !b.both && j == 0 ? -kPad : b.begin[j], to = j + 1 < b.n ? b.begin[j + 1] : b.far + kPad + 1;
+        const int from = ahead && j == 0 ? 1 : !b.both && j == 0 ? -kPad : b.begin[j], to = j + 1 < b.n ? min((int)b.begin[j + 1], b.far + kPad + 1) : b.far + kPad + 1;
         float s = part == 0 && j == b.n - 1 ? e[ahead] : 0.0f;
         if (part == 0 && !b.both && j == 0) s += e[1];
         for (int d = from + part; d < to; d += 8)
@@ -544,6 +544,14 @@ void launch_table(const BiasGradArgs& a, int64_t matrices, hipStream_t st) {
     bias_grad_table_kernel<<<grid, 256, 0, st>>>(a.partial, matrices, a.chunks, a.heads, buckets, a.table_grad);
 }
 
+// Distances that no query and key have need no place: `far` as if the last bucket began right behind the largest there is. (256 distances both ways, backward, bf16
+// [40, 32, 45, 45] 23.3 us, so 15.6.)
+Buckets within_reach(Buckets b, int64_t queries, int64_t keys, int64_t offset) {
+    const int64_t behind = queries - 1 + offset, ahead = b.both ? keys - 1 - offset : 0;
+    b.far = (int)std::min<int64_t>(b.far, std::max<int64_t>({behind, ahead, 0}) + 1);
+    return b;
+}
+
 bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
@@ -608,6 +616,7 @@ int bias_split(int dtype, int64_t rows, int64_t keys) {
 
 void launch_softmax_bias(int dtype, const BiasArgs& given, hipStream_t st) {
     BiasArgs a = given;
+    a.buckets = within_reach(a.buckets, a.queries, a.keys, a.offset);
     const size_t lds = bias_lds(a.buckets);
     const int64_t matrices = a.rows / a.queries;
     HPT_WITH_TYPE(dtype, {
@@ -648,6 +657,7 @@ void launch_softmax_bias_backward(int dtype, const BiasGradArgs& given, hipStrea
         launch_table(a, 0, st);
         return;
     }
+    a.buckets = within_reach(a.buckets, a.queries, a.keys, a.offset);
     const int64_t matrices = a.rows / a.queries;
     a.items = bias_grad_items(dtype, matrices, a.queries, a.keys, &a.per_item);
     a.chunks = (a.queries + a.per_item - 1) / a.per_item;

@@ -113,6 +113,17 @@ EDGES = [(1, 2, q, n, 32, True, 64, q // 2 + n // 2, False, None) for n in (1016
     (8, 130, 1, n, 16, False, 32, n - 1, True, None) for n in (130, 513, 1030, 2056, 3085)]
 
 
+# Fewer queries and keys than distances, in front of one another, apart by less and by more than the last bucket begins at.
+NEAR = [(2, 2, 6, 10, 32, both, 256, offset, causal, None) for both, causal in ((True, False), (False, True), (False, False)) for offset in (0, -5, 9, -50, 300, -300, 1 << 40, -(1 << 40))]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("c", NEAR, ids=lambda c: f"{'both' if c[5] else ''}{c[7]}{'-causal' if c[8] else ''}")
+def test_distances_out_of_reach(hpt, dev, name, c):
+    test_forward(hpt, dev, name, c)
+    test_backward(hpt, dev, name, c)
+
+
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("c", EDGES, ids=ids)
 def test_edges_of_the_deal(hpt, dev, name, c):
