@@ -16,10 +16,12 @@ namespace hpt {
 
 namespace {
 
-// Exponentials are powers of two of x * kLog2e (the float, whose distance from log2 e moves a row's lse by 1e-8 of its entropy once the
-// result is divided by the same float), so that one multiply-add makes the hardware's argument; a row's running maximum is kept in those
-// units. The sum's error is that of its terms weighted with their shares: rounding the argument costs a term |x - max| / 2^24.
-constexpr float kLog2e = 1.44269504f;
+// Exponentials are powers of two of x log2 e below a row's running maximum, which is kept in those units (any float near it serves). log2 e comes in two
+// pieces: the float alone is 1e-8 of itself off, which would move every row's lse by 1e-8 of its distance below the maximum, all in one direction, and a loss that is the mean of
+// terms of both signs shows that. The second piece is large against the first product's roundings (one next to the float's own last place would be rounded away every time).
+// The sum's error is that of its terms weighted with their shares: each rounding of the argument costs a term |x - max| / 2^24, to either side.
+constexpr double kLog2eExact = 1.4426950408889634;
+constexpr float kLog2e = 1.4423828125f, kLog2eRest = (float)(kLog2eExact - 1.4423828125);  // (1477 / 1024, and what is left)
 
 // (maximum in those units, sum of the powers below it) of two lanes or wavefronts.
 __device__ __forceinline__ void meet(float& m, double& s, float m2, double s2) {
@@ -54,12 +56,11 @@ template <class T> __device__ __forceinline__ float logit_of(const PolicyArgs& a
 
 // What a row adds to the loss, and the loss's slope by its logp, both times the mask.
 struct RowLoss {
-    double loss;
-    float slope;
+    double loss, slope;
     __device__ __forceinline__ void store(const PolicyArgs& a, int64_t row) const {
         if (!a.old_logp) return;
         a.each[row] = loss;
-        a.weight[row] = slope;  // (over the sum of the mask: in the last launch)
+        a.weight[row] = (float)slope;  // (over the sum of the mask: in the last launch)
     }
 };
 // A row's results from its maximum, sum and token.
@@ -68,7 +69,7 @@ __device__ __forceinline__ RowLoss finish_row(const PolicyArgs& a, int64_t row, 
     const double logp = ((double)xt - m) - rest;  // (exact differences first: m may be a type's lowest value)
     a.logp[row] = (float)logp;
     a.lse[row] = (float)lse;
-    if (!a.old_logp) return {0.0, 0.0f};
+    if (!a.old_logp) return {0.0, 0.0};
     const double adv = t.advantage, ratio = exp(logp - (double)t.old);
     const double low = 1.0 - a.clip_low, high = 1.0 + a.clip_high;
     const double free = ratio * adv, held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
@@ -79,12 +80,12 @@ __device__ __forceinline__ RowLoss finish_row(const PolicyArgs& a, int64_t row, 
         loss += a.kl_weight * (e - k - 1.0);
         slope += a.kl_weight * (1.0 - e);
     }
-    return {loss * mask, (float)(slope * mask)};
+    return {loss * mask, slope * mask};
 }
 // A row that the mask leaves out.
 __device__ __forceinline__ RowLoss skip_row(const PolicyArgs& a, int64_t row) {
     a.logp[row] = a.lse[row] = 0.0f;
-    return {0.0, 0.0f};
+    return {0.0, 0.0};
 }
 
 // Maximum and sum of a part of a row. Vectors are aligned from the part's first aligned element on; the elements before it and behind the
@@ -115,11 +116,11 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
             float t = v[0];
 #pragma unroll
             for (int i = 1; i < N; ++i) t = fmaxf(t, v[i]);
-            const float top = fmaxf(m, t * kLog2e);
+            const float top = fmaxf(m, t * (float)kLog2eExact);
             float add = 0.0f;
             if (fabsf(top) < inf) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) add += __builtin_amdgcn_exp2f(fmaf(v[i], kLog2e, -top));
+                for (int i = 0; i < N; ++i) add += __builtin_amdgcn_exp2f(fmaf(v[i], kLog2eRest, fmaf(v[i], kLog2e, -top)));
                 s = s * __builtin_amdgcn_exp2f(m - top) + add;
                 m = top;
             } else {  // nothing but -inf yet, a +inf, or an overflow: if that stays, the row is swept again below; what counts now is a NaN
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(256) void policy_stats_kernel(const PolicyArgs a) {
         m = most[0];
         sd = sums[0];
         for (int w = 1; w < 4; ++w) meet(m, sd, most[w], sums[w]);
-        double top = (double)m / (double)kLog2e;
+        double top = (double)m / kLog2eExact;
         if (fabsf(m) == inf && n > 0) {
             // infinities, or values so near to a type's end that they have none in those units (a row masked as a whole): element by element
             float t = -inf;
@@ -233,7 +234,7 @@ template <class T>
 __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
     __shared__ double place[2 * 16];
     double v[2] = {0.0, 0.0};
-    float slope[2] = {0.0f, 0.0f};
+    double slope[2] = {0.0, 0.0};
     if (a.split > 1) {
         static_assert(kMostSplit <= 2 * 1024, "two rows a thread");
 #pragma unroll
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int64_t row = threadIdx.x + k * 1024;
-            if (row < a.rows) a.weight[row] = (float)((double)slope[k] * inv);
+            if (row < a.rows) a.weight[row] = (float)(slope[k] * inv);
         }
     } else {
 #pragma unroll 4
