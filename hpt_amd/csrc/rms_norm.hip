@@ -312,7 +312,7 @@ template <class T, bool RES, int Q> void launch_of(const RmsArgs& given, hipStre
 // ---- backward -------------------------------------------------------------------------------------
 
 // Rows held in registers; each workgroup walks rows and keeps its sums for gamma in registers, which leave as one row of partial sums. Bound by memory:
-// bf16 [16384, 4096] with a third operand 103 us, 5.2 TB/s, and 5 us for the columns; f32 [1237, 1001] 8 and 4 us, two launches and their latency.
+// bf16 [16384, 4096] with a third operand 103 us, 5.2 TB/s, and 5 us for the columns; f32 [1237, 1001] 7 and 4 us, two launches and their latency.
 template <class T, int NC, bool AL, bool MORE>
 __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);

@@ -114,7 +114,7 @@ __device__ __forceinline__ void biased(const Pack<T, VEC>& p, int e, int lo, int
 }
 
 // Rows held in registers. An item is `per_item` rows of one matrix; the first row is on its way while the bias comes together, every other
-// one while the row before it is summed and written. bf16 [8, 16, 1024, 1024] with lengths 92 us, 4.9 TB/s: next to memory, the bias by distance and an
+// one while the row before it is summed and written. bf16 [8, 16, 1024, 1024] with lengths 90 us, 5.0 TB/s: next to memory, the bias by distance and an
 // exponential for every element. One query, f16 [16, 32, 1, 4097], 7.8 us: bias, loads, two folds and the store follow one another.
 template <class T, int NC, bool AL>
 __global__ __launch_bounds__(1024, NC <= 2 ? 5 : 4) void bias_row_kernel(const BiasArgs a) {
@@ -558,7 +558,7 @@ size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
 
 // Four vectors per thread: a row's maximum and sum cost the same for two. us, f16 [8, 16, 256 queries or so, keys] of 65 vectors 78 with two, 61.5 with up to
 // four, of 129 84 and 58, of 128 56.3 and 54.7.
-// Rows above a wavefront go to workgroups of 128, 256, 512 or 768 threads with three or four vectors each (f32 four to six): a fifth wavefront shares a
+// Rows above a wavefront go to workgroups of 128, 256, 512 or 768 threads with three or four vectors each (f32 four to eight): a fifth wavefront shares a
 // SIMD with the first, and then fewer workgroups run at once. us, f16 [1, 16, 256, 8208 keys and more], 320 threads of two vectors 69, 256 of three 50;
 // [.., 6144] 384 of two 58, 256 of three 39; one query, [64, 32, 1, 4104] 320 of two 20.3, 256 of three 14.3; f32 [.., 4400] 320 of four 35.9, 256 of five 27.2.
 // (385 ... 512 two-byte vectors: of whole matrices 256 threads of two 49, 128 of four 55; of one query 12.3 and 10.4.)
