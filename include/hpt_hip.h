@@ -301,8 +301,8 @@ typedef enum hpt_quant_format {
     HPT_QUANT_E4M3 = 2  /* `out` is u8: the bits of 8-bit floats with 4 bits of exponent and 3 of fraction (448 at most, no infinities) */
 } hpt_quant_format;
 
-/* The same with y in 8 bits: out = y / scale, rounded to nearest (ties to even), one scale for each run of `group` elements of a
- * row (0: the whole row; `group` divides the row). scale = largest |y| of the group / largest value of the format, at least
+/* The same with y in 8 bits: out = y / scale, the f32 quotient rounded to nearest (ties to even), one scale for each run of `group`
+ * elements of a row (0: the whole row; `group` divides the row). scale = largest |y| of the group / largest value of the format, at least
  * 2^-120 (which is what a group of zeros has); a group with a NaN has a NaN for scale, and 0 (i8) or NaN (e4m3) for values.
  * `scale`: f32, rows x groups. */
 int32_t hpt_hip_rms_norm_quant(int32_t dev, void* stream, const hpt_view* in, const hpt_view* residual, int32_t n_norm_dims,
