@@ -77,3 +77,86 @@ def test_8_bit_values_of_tiny_and_huge_norms(hpt, dev, fmt, power):
     q, s = x.rms_norm_quant([cols], up(hpt, gamma), 1e-30, format=fmt)
     assert (s.numpy() == scale).all()
     assert np.array_equal(q.numpy(), np.broadcast_to(codes(fmt, gamma / scale), (2, cols)))
+
+
+# ---- logits of any finite size --------------------------------------------------------------------------------
+
+LSE = 128 * F32_STEP  # absolute, of the log of the sum
+MASKS = [-1e4, -65504.0, -9e4, -1.2e5, -2e5, -1e6, -1e9, -1e10, -1e12, -1e20, -1e30, -1e37, -1.6e38, -3e38]
+
+
+def logsumexp(x):
+    m = x.max(-1, keepdims=True)
+    return (m + np.log(np.exp(x - m).sum(-1, keepdims=True)))[..., 0]
+
+
+def masked_rows(x, v):
+    """Rows of which all, a stretch, or all but a few logits are v."""
+    n = x.shape[-1]
+    stretches = [slice(0, n), slice(0, n // 2), slice(n // 2, n), slice(n // 3, 2 * n // 3), slice(1, n), slice(0, n - 1), slice(0, n, 2), slice(0, 0)]
+    for i in range(len(x)):
+        x[i, stretches[i % len(stretches)]] = v
+    x[-1] = v
+    x[-1, n // 2] = 0.5
+    return x
+
+
+def check_rows(hpt, k, x, what):
+    """Log-probabilities of both ends of each row's range, and the loss with its gradient, against 64 bits."""
+    t, x = k.up(x)
+    rows = len(x)
+    lse = logsumexp(x)
+    for token in (x.argmax(-1), x.argmin(-1)):
+        logp = (x[np.arange(rows), token] - x.max(-1)) - (lse - x.max(-1) if np.abs(x).max() < 1e3 else logsumexp(x - x.max(-1, keepdims=True)))
+        a, b = t.token_logp(up(hpt, token))
+        near(a.numpy(), logp, LSE + F32_STEP * np.abs(logp), f"logp {what}")
+        near(b.numpy(), lse, LSE + F32_STEP * np.abs(lse), f"lse {what}")
+    token = x.argmax(-1)
+    logp = -logsumexp(x - x.max(-1, keepdims=True))
+    old = (logp + 0.05).astype(np.float32)
+    adv = np.where(np.arange(rows) % 2, 1, -1).astype(np.float32)
+    r = t.policy_loss(up(hpt, token), up(hpt, old), up(hpt, adv))
+    ratio = np.exp(logp - old.astype(np.float64))
+    near(r.weight.numpy(), -ratio * adv / rows, (LSE * ratio + 4 * F32_STEP) / rows, f"weight {what}")
+    near(r.loss.numpy()[0], (-ratio * adv).mean(), (LSE * ratio + 4 * F32_STEP).mean(), f"loss {what}")
+    d = k.down(t.policy_loss_backward(up(hpt, token), r.lse, r.weight, 64.0))
+    assert np.isfinite(d).all(), what
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,cols", [(9, 50), (9, 5000), (9, 40000), (2100, 70)])
+def test_finite_masks_of_any_size(hpt, dev, name, rows, cols):
+    """Whole rows, stretches that whole threads, wavefronts and parts of a split row meet nothing else of, and all but one."""
+    k, rng = Kind(hpt, name), np.random.default_rng(cols)
+    for v in MASKS:
+        if name != "f16" or v >= -65504:
+            check_rows(hpt, k, masked_rows(rng.standard_normal((rows, cols)) * 3, v), f"mask {v}")
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("cols", [50, 5000, 40000])
+def test_maxima_of_any_size(hpt, dev, name, cols):
+    """One logit far above the others, and rows that lie far from zero as a whole."""
+    k, rng = Kind(hpt, name), np.random.default_rng(cols)
+    for v in [-m for m in MASKS]:
+        if name == "f16" and v > 65504:
+            continue
+        x = rng.standard_normal((9, cols)) * 3
+        x[np.arange(9), rng.integers(0, cols, 9)] = v
+        x[0] = v
+        x[1, ::2] = v
+        check_rows(hpt, k, x, f"maximum {v}")
+    for c in (1e3, 3e4, 6e4, 8.9e4, 9.2e4, 1e5, 1.7e5, 1.9e5, 1e6, 1e7):
+        for sign in (1, -1):
+            if name == "f16" and c > 6e4:
+                continue
+            # of both sides of a stretch, a few apart, in either order
+            x = sign * c + rng.standard_normal((6, cols)) * 3
+            x[1, : cols // 2] += 4
+            x[2, cols // 2:] += 4
+            x[3, cols // 3: cols // 2] -= 5000
+            x[4, : cols // 2] -= 90000 if name != "f16" else 5000
+            x[5, cols // 2:] -= 90000 if name != "f16" else 5000
+            if name == "f16":
+                x = np.clip(x, -65504, 65504)
+            check_rows(hpt, k, x, f"around {sign * c}")
