@@ -164,8 +164,9 @@ __global__ __launch_bounds__(1024, NC <= 2 ? 5 : 4) void bias_row_kernel(const B
             const float base = m[0] == -__builtin_huge_valf() ? 0.0f : m[0];
             float t[1] = {0.0f};
             // (two-byte types: one multiply-add makes the hardware's argument; what rounding base * log2 e costs is in every term and in their
-            // sum alike. It would overflow next to the type's lowest value, with which callers mask.)
-            if (sizeof(T) == 2 && fabsf(base) < 1e38f) {
+            // sum alike. It is 2^-4 at most while the row's largest score is within 2^20, but beyond some 1e9 it leaves the exponential's range: rows that a caller has
+            // masked as a whole with a large finite number take the differences, which are exact where they matter.)
+            if (sizeof(T) == 2 && fabsf(base) < 0x1p20f) {
                 constexpr float kLog2e = 1.44269504f;
                 const float shift = -base * kLog2e;
 #pragma unroll

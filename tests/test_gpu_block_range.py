@@ -160,3 +160,44 @@ def test_maxima_of_any_size(hpt, dev, name, cols):
             if name == "f16":
                 x = np.clip(x, -65504, 65504)
             check_rows(hpt, k, x, f"around {sign * c}")
+
+
+# ---- scores of any finite size --------------------------------------------------------------------------------
+
+def softmax(s):
+    e = np.exp(s - s.max(-1, keepdims=True))
+    return e / e.sum(-1, keepdims=True)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n,queries", [(40, 24), (1000, 24), (2056, 24), (9000, 24), (70000, 24), (1500, 1)])
+def test_masks_and_maxima_of_any_size(hpt, dev, name, n, queries):
+    """Queries all of whose keys a caller has masked with one finite number, part of them, or one key far above the others. The scores that the
+    probabilities are taken of are scale * x + bias in f32: what they say is computed from those."""
+    k, rng = Kind(hpt, name), np.random.default_rng(n)
+    low = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": -3.3895313892515355e38}[name]
+    values = [v for v in (-1e4, -6e4, -9e5, -1.3e6, -1e9, -1e10, -1e12, -1e15, -1e20, -1e30, -1e37, low) if name != "f16" or v >= -65504]
+    values += [-v for v in values]
+    tab, table = k.up(np.array([0, 1, -1, 2, 0.5, -0.5, 1.5, 3])[:, None])
+    q, j = np.arange(queries)[:, None], np.arange(n)
+    d = q + (n - queries) - j
+    bias = table[:, 0][np.where(d < 4, np.maximum(d, 0), np.minimum(7, 4 + np.floor(np.log2(np.maximum(d, 1) / 4) / 2 * 4 + 1e-9).astype(int)))]
+    for scale in (1.0, 0.125, 0.0884):
+        sc = np.float64(np.float32(scale))
+        for first in range(0, len(values), queries):
+            some = values[first:first + queries]
+            for pattern in ("all", "part", "one"):
+                x = rng.standard_normal((queries, n)) * 4
+                for i, v in enumerate(some):
+                    if pattern == "all":
+                        x[i] = v
+                    elif pattern == "part":
+                        x[i, n // 3: n - 5] = v
+                    else:
+                        x[i, rng.integers(0, n)] = v
+                t, x = k.up(x[None, None])
+                s = (sc * x[0, 0] + bias).astype(np.float32).astype(np.float64)
+                want = softmax(s)
+                got = k.down(t.softmax_bias(tab, scale, bidirectional=False, max_distance=16, query_offset=n - queries))[0, 0]
+                # a difference of two scores is rounded once, and twice on its way to a power of two: it is weighted with e^-difference <= 1 / difference
+                near(got, want, want * (k.step + (100 + 3 * np.minimum(s.max(-1, keepdims=True) - s, 200)) * F32_STEP) + k.least, f"{pattern} {some[:2]} scale {scale}")
