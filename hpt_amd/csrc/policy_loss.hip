@@ -114,7 +114,8 @@ __global__ __launch_bounds__(256, 5) void policy_stats_kernel(const PolicyArgs a
         const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
         const int vecs = (n - head) / VEC, tail = head + vecs * VEC;
         const T* body = x + head;
-        float m = -inf, s = 0.0f;
+        float m = -inf;
+        double s = 0.0;  // (as few as a thousand sums of 32 terms, one after the other in f32, would show in lse)
         auto take = [&](auto& v) {
             constexpr int N = sizeof(v) / sizeof(float);
             float t = v[0];
@@ -125,12 +126,12 @@ __global__ __launch_bounds__(256, 5) void policy_stats_kernel(const PolicyArgs a
             if (fabsf(top) < 2 * kNear) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) add += __builtin_amdgcn_exp2f(fmaf(v[i], kLog2eRest, fmaf(v[i], kLog2e, -top)));
-                s = s * __builtin_amdgcn_exp2f(m - top) + add;
+                s = s * (double)__builtin_amdgcn_exp2f(m - top) + (double)add;
                 m = top;
             } else {  // nothing but masked logits yet, or logits far from zero: if that stays, the row is swept again below; what counts now is a NaN
 #pragma unroll
                 for (int i = 0; i < N; ++i) add += v[i] == v[i] ? 0.0f : v[i];
-                s += add;
+                s += (double)add;
                 m = top;
             }
         };
@@ -159,18 +160,17 @@ __global__ __launch_bounds__(256, 5) void policy_stats_kernel(const PolicyArgs a
                 for (int i = 0; i < VEC; ++i) f[b * VEC + i] = Elem<T>::widen(p[b].v[i]);
             take(f);
         }
-        double sd = s;
 #pragma unroll
-        for (int w = 1; w < 64; w <<= 1) meet(m, sd, __shfl_xor(m, w, 64), shfl_xor_any(sd, w));
+        for (int w = 1; w < 64; w <<= 1) meet(m, s, __shfl_xor(m, w, 64), shfl_xor_any(s, w));
         __syncthreads();
         if ((threadIdx.x & 63) == 0) {
             most[threadIdx.x >> 6] = m;
-            sums[threadIdx.x >> 6] = sd;
+            sums[threadIdx.x >> 6] = s;
         }
         __syncthreads();
         m = most[0];
-        sd = sums[0];
-        for (int w = 1; w < 4; ++w) meet(m, sd, most[w], sums[w]);
+        s = sums[0];
+        for (int w = 1; w < 4; ++w) meet(m, s, most[w], sums[w]);
         double top = (double)m / kLog2eExact;
         if (!(fabsf(m) < kNear) && n > 0) {
             // infinities, or finite logits far from zero (a row masked as a whole, or a part of one): element by element, by their differences from the largest
@@ -180,22 +180,22 @@ __global__ __launch_bounds__(256, 5) void policy_stats_kernel(const PolicyArgs a
 #pragma unroll 8
             for (int i = threadIdx.x; i < n; i += 256) t = fmaxf(t, Elem<T>::widen(x[i]));
             t = block_reduce<MaxF>(t, most);
-            float add = 0.0f;
+            double add = 0.0;
 #pragma unroll 8
             for (int i = threadIdx.x; i < n; i += 256) {
                 const float v = Elem<T>::widen(x[i]);
-                add += v == t ? 1.0f : __expf(v - t);
+                add += (double)(v == t ? 1.0f : __expf(v - t));
             }
             top = t;
-            sd = block_reduce<SumF>(add, most);
+            s = block_reduce<SumD>(add, sums);
         }
         if (threadIdx.x == 0) {
             if (a.split == 1) {
                 const Token t(a, row);
-                finish_row(a, row, mask, t, logit_of<T>(a, row, t.id), top, sd).store(a, row);
+                finish_row(a, row, mask, t, logit_of<T>(a, row, t.id), top, s).store(a, row);
             } else {
                 a.partial[2 * at] = top;
-                a.partial[2 * at + 1] = sd;
+                a.partial[2 * at + 1] = s;
             }
         }
     }

@@ -5,8 +5,8 @@
 //   gx = r * gy * gamma - x * r^3 * c / cols (+ what else arrives at x),   ggamma = sum over the rows of gy * x * r.
 // r and c come from the one read of x and gy that the result needs anyway.
 //
-// Everything here is bound by memory: a row is read once into the registers of the threads that share it and written once. Sums
-// are f32 (x of two bytes widened exactly, squares and products in f32); h is rounded to the inputs' type first, as a
+// Everything here is bound by memory: a row is read once into the registers of the threads that share it and written once (longer rows are swept). Sums
+// are f32 (x of two bytes widened exactly, squares and products in f32), of rows that are swept f64 from vector to vector; h is rounded to the inputs' type first, as a
 // separate addition would have stored it, and y is computed from the rounded h; y is rounded once.
 #include <algorithm>
 
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {
 template <class T, bool RES, int Q>
 __global__ __launch_bounds__(1024) void rms_stream_kernel(const RmsArgs a) {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ float sums[2 * 16];
+    __shared__ double sums[2 * 16];
     __shared__ uint32_t mosts[2 * 16];
     int turn = 0, turn_most = 0;
     const int vecs = (a.cols + VEC - 1) / VEC;
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(1024) void rms_stream_kernel(const RmsArgs a) {
         const T* x = (const T*)a.x + offset_of(a.kept, row);
         const T* res = RES ? (const T*)a.res + row * a.cols : nullptr;
         T* sum = RES && a.sum ? (T*)a.sum + row * a.cols : nullptr;
-        float ss[1] = {0.0f};
+        double ss[1] = {0.0};
         for (int v = threadIdx.x; v < vecs; v += 1024) {
             Pack<T, VEC> p = sweep_vec<T>(x, v, a.cols);
             if constexpr (RES) {
@@ -222,11 +222,13 @@ __global__ __launch_bounds__(1024) void rms_stream_kernel(const RmsArgs a) {
                 for (int i = 0; i < VEC; ++i) p.v[i] = Elem<T>::narrow(Elem<T>::widen(p.v[i]) + Elem<T>::widen(q.v[i]));
                 if (sum) store_sweep_vec<T, VEC>(sum, v, a.cols, p);
             }
+            float add = 0.0f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) ss[0] = fmaf(Elem<T>::widen(p.v[i]), Elem<T>::widen(p.v[i]), ss[0]);
+            for (int i = 0; i < VEC; ++i) add = fmaf(Elem<T>::widen(p.v[i]), Elem<T>::widen(p.v[i]), add);
+            ss[0] += add;
         }
-        fold_row<SumF>(ss, 1024, sums, turn);
-        const float r = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
+        fold_row<SumD>(ss, 1024, sums, turn);
+        const float r = 1.0f / sqrtf((float)(ss[0] / a.cols) + a.eps);
         const T* h = sum ? sum : x;
         const bool add = RES && !sum;
         auto value = [&](int e) {
@@ -436,7 +438,7 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
 template <class T>
 __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ float sums[2 * 16 * 2];
+    __shared__ double sums[2 * 16 * 2];
     int turn = 0;
     const int vecs = (a.cols + VEC - 1) / VEC;
     const T* gamma = (const T*)a.gamma;
@@ -446,23 +448,26 @@ __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs
         const T* x = (const T*)a.x + offset_of(a.kept, row);
         const T* gy = (const T*)a.gy + row * a.cols;
         const T* gsum = a.gsum ? (const T*)a.gsum + row * a.cols : nullptr;
-        float s[2] = {0.0f, 0.0f};
+        double s[2] = {0.0, 0.0};
         for (int v = threadIdx.x; v < vecs; v += 1024) {
             const Pack<T, VEC> xp = sweep_vec<T>(x, v, a.cols), gp = sweep_vec<T>(gy, v, a.cols);
             Pack<T, VEC> g;
             if (gamma) g = sweep_vec<T>(gamma, v, a.cols);
+            float add[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float xv = Elem<T>::widen(xp.v[i]);
                 float gv = Elem<T>::widen(gp.v[i]);
                 if (gamma) gv *= Elem<T>::widen(g.v[i]);
-                s[0] = fmaf(xv, xv, s[0]);
-                s[1] = fmaf(gv, xv, s[1]);
+                add[0] = fmaf(xv, xv, add[0]);
+                add[1] = fmaf(gv, xv, add[1]);
             }
+            s[0] += add[0];
+            s[1] += add[1];
         }
-        fold_row<SumF>(s, 1024, sums, turn);
-        const float r = 1.0f / sqrtf(s[0] / (float)a.cols + a.eps);
-        const float c = r * r * (s[1] / (float)a.cols);
+        fold_row<SumD>(s, 1024, sums, turn);
+        const float r = 1.0f / sqrtf((float)(s[0] / a.cols) + a.eps);
+        const float c = r * r * (float)(s[1] / a.cols);
         for (int v = threadIdx.x; v < vecs; v += 1024) {
             const Pack<T, VEC> xp = sweep_vec<T>(x, v, a.cols), gp = sweep_vec<T>(gy, v, a.cols);
             Pack<T, VEC> g, more, p;

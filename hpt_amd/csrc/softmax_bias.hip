@@ -11,7 +11,8 @@
 // two ends in registers. Rows follow one another, workgroups leave a row of partial sums each, which a second kernel folds: the
 // order is the same always.
 //
-// Bound by memory: one read of every live score, one write of every result. Sums and maxima f32, results rounded once.
+// Bound by memory: one read of every live score, one write of every result (longer rows are swept twice). Sums and maxima f32, sums of rows that are swept f64 from
+// vector to vector; results rounded once.
 #include <algorithm>
 #include <cmath>
 
@@ -210,18 +211,18 @@ __global__ __launch_bounds__(1024, NC <= 2 ? 5 : 4) void bias_row_kernel(const B
 }
 
 // (maximum, sum of exponentials below it) of what has been seen, and of two such.
-template <class T> __device__ __forceinline__ void meet(float& m, float& s, float m2, float s2) {
+template <class T, class S> __device__ __forceinline__ void meet(float& m, S& s, float m2, S s2) {
     const float n = fmaxf(m, m2);
     // (nothing seen is (-inf, 0); equal infinities are no distance apart; a NaN is in its sum)
-    s = s * (m == n ? 1.0f : exp_row<T>(m - n)) + s2 * (m2 == n ? 1.0f : exp_row<T>(m2 - n));
+    s = s * (S)(m == n ? 1.0f : exp_row<T>(m - n)) + s2 * (S)(m2 == n ? 1.0f : exp_row<T>(m2 - n));
     m = n;
 }
 
 // Statistics of the live keys of `row` from vector v0 to v1, over the whole workgroup (a multiple of 64 threads).
-template <class T> __device__ __forceinline__ void sweep_stats(const BiasArgs& a, const T* x, int v0, int v1, int live, int pos, const float* bias, float* place, float& m, float& s) {
+template <class T> __device__ __forceinline__ void sweep_stats(const BiasArgs& a, const T* x, int v0, int v1, int live, int pos, const float* bias, float* most, double* sums, float& m, float& total) {
     constexpr int VEC = 16 / sizeof(T);
     m = -__builtin_huge_valf();
-    s = 0.0f;
+    double s = 0.0;
     for (int v = v0 + threadIdx.x; v < v1 && v * VEC < live; v += blockDim.x) {
         float t[VEC];
         biased<T, VEC>(sweep_vec<T>(x, v, a.keys), v * VEC, 0, live, pos, a.scale, a.buckets.far, right_of(a.buckets), bias, t);
@@ -231,20 +232,21 @@ template <class T> __device__ __forceinline__ void sweep_stats(const BiasArgs& a
         float add = 0.0f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) add += v * VEC + i >= live ? 0.0f : t[i] == n ? 1.0f : exp_row<T>(t[i] - n);
-        s = (m == n ? s : s * exp_row<T>(m - n)) + add;
+        s = (m == n ? s : s * (double)exp_row<T>(m - n)) + (double)add;
         m = n;
     }
 #pragma unroll
-    for (int w = 1; w < 64; w <<= 1) meet<T>(m, s, __shfl_xor(m, w, 64), __shfl_xor(s, w, 64));
+    for (int w = 1; w < 64; w <<= 1) meet<T>(m, s, __shfl_xor(m, w, 64), shfl_xor_any(s, w));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
-        place[2 * (threadIdx.x >> 6)] = m;
-        place[2 * (threadIdx.x >> 6) + 1] = s;
+        most[threadIdx.x >> 6] = m;
+        sums[threadIdx.x >> 6] = s;
     }
     __syncthreads();
-    m = place[0];
-    s = place[1];
-    for (int w = 1; w < (int)blockDim.x >> 6; ++w) meet<T>(m, s, place[2 * w], place[2 * w + 1]);
+    m = most[0];
+    s = sums[0];
+    for (int w = 1; w < (int)blockDim.x >> 6; ++w) meet<T>(m, s, most[w], sums[w]);
+    total = (float)s;
 }
 
 template <class T> __device__ __forceinline__ void sweep_apply(const BiasArgs& a, const T* x, T* out, int v0, int v1, int live, int pos, const float* bias, float m, float s) {
@@ -271,7 +273,8 @@ template <class T>
 __global__ __launch_bounds__(1024) void bias_stream_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     extern __shared__ float bias[];
-    __shared__ float fold[32];
+    __shared__ float most[16];
+    __shared__ double sums[16];
     const int vecs = (a.keys + VEC - 1) / VEC;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t matrix = quotient(row, a.queries), q = row - matrix * a.queries;
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(1024) void bias_stream_kernel(const BiasArgs a) {
         const int live = place.live(0, a.causal), pos = place.pos;
         const T* x = (const T*)a.x + offset_of(a.matrices, matrix) + q * a.query_stride;
         float m, s;
-        sweep_stats<T>(a, x, 0, vecs, live, pos, bias, fold, m, s);
+        sweep_stats<T>(a, x, 0, vecs, live, pos, bias, most, sums, m, s);
         sweep_apply<T>(a, x, (T*)a.out + row * a.keys, 0, vecs, live, pos, bias, m, s);
     }
 }
@@ -292,7 +295,8 @@ template <class T, bool APPLY>
 __global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     extern __shared__ float bias[];
-    __shared__ float fold[8];
+    __shared__ float most[4];
+    __shared__ double sums[4];
     const int64_t row = blockIdx.x / (unsigned)a.split, matrix = quotient(row, a.queries), q = row - matrix * a.queries;
     const int part = blockIdx.x % a.split;
     const int vecs = (a.keys + VEC - 1) / VEC, each = (vecs + a.split - 1) / a.split;
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(256) void bias_split_kernel(const BiasArgs a) {
     const T* x = (const T*)a.x + offset_of(a.matrices, matrix) + q * a.query_stride;
     float m, s;
     if constexpr (!APPLY) {
-        sweep_stats<T>(a, x, v0, v1, live, pos, bias, fold, m, s);
+        sweep_stats<T>(a, x, v0, v1, live, pos, bias, most, sums, m, s);
         if (threadIdx.x == 0) {
             a.partial[2 * (row * a.split + part)] = m;
             a.partial[2 * (row * a.split + part) + 1] = s;
@@ -330,7 +334,7 @@ typedef float Quad __attribute__((ext_vector_type(4), may_alias));
 // the ends. Hidden elements are zeros. Rows add to a place one after the other, each once, so that the sums do not depend on any order
 // though the LDS adds by itself.
 template <int VEC>
-__device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, int pos, int far, int right, float* places, float& left_end, float& right_end) {
+__device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, int pos, int far, int right, float* places, double& left_end, double& right_end) {
     const int r = e - pos;
     if (r > -far - VEC && r < right) {
         float* at = places + (r + far + kPad);
@@ -348,12 +352,12 @@ __device__ __forceinline__ void add_by_distance(const float (&d)[VEC], int e, in
 // The workgroup's sums by distance -> by bucket, into its row of partial sums; eight lanes share a bucket. `places`: arrays of `length`, number g for
 // rows at positions pos + g modulo 4. They become one first, each place by a thread that alone reads it in all of them (without that step, f16 [32, 12, 64, 64] 11.1 us, with it
 // 10.1; unrolled further it costs the rows' loop registers). Every thread of the workgroup comes here.
-__device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, int arrays, int length, int pos, float left_end, float right_end, float* out) {
-    __shared__ float ends[2 * 16 * 2];
+template <class Op, class A> __device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, int arrays, int length, int pos, A left_end, A right_end, float* out) {
+    __shared__ A ends[2 * 16 * 2];
     const int total = b.both ? 2 * b.n : b.n, zero = b.far + kPad;
-    float e[2] = {left_end, right_end};
+    A e[2] = {left_end, right_end};
     int turn = 0;
-    fold_row<SumF>(e, blockDim.x, ends, turn);
+    fold_row<Op>(e, blockDim.x, ends, turn);
     __syncthreads();  // (a single wavefront has passed none in the fold)
     const int shift = shift_of(b, pos);
     if (arrays > 1) {
@@ -371,8 +375,8 @@ __device__ __forceinline__ void leave_buckets(const Buckets& b, float* places, i
         const int j = ahead ? k - b.n : k;
         // distances of bucket k: of its direction's last one also those of the margin; bucket 0 of a single direction has the other's margin
         const int from = ahead && j == 0 ? 1 : !b.both && j == 0 ? -kPad : b.begin[j], to = j + 1 < b.n ? min((int)b.begin[j + 1], b.far + kPad + 1) : b.far + kPad + 1;
-        float s = part == 0 && j == b.n - 1 ? e[ahead] : 0.0f;
-        if (part == 0 && !b.both && j == 0) s += e[1];
+        float s = part == 0 && j == b.n - 1 ? (float)e[ahead] : 0.0f;
+        if (part == 0 && !b.both && j == 0) s += (float)e[1];
         for (int d = from + part; d < to; d += 8)
             s += places[(ahead ? zero + d : zero - d) + shift];
         s = group_reduce<SumF>(s, 8);
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(1024, NC <= 2 ? (AL ? 6 : 5) : 4) void bias_grad_ke
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        if (a.table_grad) leave_buckets(a.buckets, places, arrays, 4 * quads, place.pos, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+        if (a.table_grad) leave_buckets<SumF>(a.buckets, places, arrays, 4 * quads, place.pos, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
     }
 }
 
@@ -481,13 +485,13 @@ template <class T>
 __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     extern __shared__ float places[];
-    __shared__ float sums[2 * 16];
+    __shared__ double sums[2 * 16];
     int turn = 0;
     const int far = a.buckets.far, right = right_of(a.buckets), n = places_of(a.buckets), vecs = (a.keys + VEC - 1) / VEC;
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
         const int64_t matrix = quotient(item, a.chunks), q0 = (item - matrix * a.chunks) * a.per_item;
         const int64_t q1 = q0 + a.per_item < a.queries ? q0 + a.per_item : a.queries;
-        float left_end = 0.0f, right_end = 0.0f;
+        double left_end = 0.0, right_end = 0.0;
         __syncthreads();  // (the item before has left its sums)
         for (int i = threadIdx.x; i < n; i += 1024) places[i] = 0.0f;
         __syncthreads();
@@ -496,14 +500,17 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
             const Place place(a, matrix, q);
             const int live = place.live(0, a.causal), pos = place.pos;
             const T *p = (const T*)a.p + row * a.keys, *g = (const T*)a.g + row * a.keys;
-            float s[1] = {0.0f};
+            double fold[1] = {0.0};
             for (int v = threadIdx.x; v * VEC < live; v += 1024) {
                 const Pack<T, VEC> pp = sweep_vec<T>(p, v, a.keys), gp = sweep_vec<T>(g, v, a.keys);
+                float add = 0.0f;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i)
-                    if (v * VEC + i < live) s[0] = fmaf(Elem<T>::widen(pp.v[i]), Elem<T>::widen(gp.v[i]), s[0]);
+                    if (v * VEC + i < live) add = fmaf(Elem<T>::widen(pp.v[i]), Elem<T>::widen(gp.v[i]), add);
+                fold[0] += add;
             }
-            fold_row<SumF>(s, 1024, sums, turn);  // (its barrier also keeps two rows' additions apart)
+            fold_row<SumD>(fold, 1024, sums, turn);  // (its barrier also keeps two rows' additions apart)
+            const float s = (float)fold[0];
             for (int v = threadIdx.x; v < vecs; v += 1024) {
                 float d[VEC];
                 Pack<T, VEC> o;
@@ -512,7 +519,7 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
                     const Pack<T, VEC> pp = sweep_vec<T>(p, v, a.keys), gp = sweep_vec<T>(g, v, a.keys);
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        d[i] = v * VEC + i < live ? Elem<T>::widen(pp.v[i]) * (Elem<T>::widen(gp.v[i]) - s[0]) : 0.0f;
+                        d[i] = v * VEC + i < live ? Elem<T>::widen(pp.v[i]) * (Elem<T>::widen(gp.v[i]) - s) : 0.0f;
                         o.v[i] = Elem<T>::narrow(a.scale * d[i]);
                     }
                     if (a.table_grad) add_by_distance<VEC>(d, v * VEC, pos, far, right, places, left_end, right_end);
@@ -520,7 +527,7 @@ __global__ __launch_bounds__(1024) void bias_grad_stream_kernel(const BiasGradAr
                 store_sweep_vec<T, VEC>((T*)a.out + row * a.keys, v, a.keys, o);
             }
         }
-        if (a.table_grad) leave_buckets(a.buckets, places, 1, 0, far + kPad, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
+        if (a.table_grad) leave_buckets<SumD>(a.buckets, places, 1, 0, far + kPad, left_end, right_end, a.partial + item * (a.buckets.both ? 2 * a.buckets.n : a.buckets.n));
     }
 }
 

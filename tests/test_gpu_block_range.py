@@ -201,3 +201,126 @@ def test_masks_and_maxima_of_any_size(hpt, dev, name, n, queries):
                 got = k.down(t.softmax_bias(tab, scale, bidirectional=False, max_distance=16, query_offset=n - queries))[0, 0]
                 # a difference of two scores is rounded once, and twice on its way to a power of two: it is weighted with e^-difference <= 1 / difference
                 near(got, want, want * (k.step + (100 + 3 * np.minimum(s.max(-1, keepdims=True) - s, 200)) * F32_STEP) + k.least, f"{pattern} {some[:2]} scale {scale}")
+
+
+# ---- rows of many millions of elements --------------------------------------------------------------------------
+
+@pytest.fixture()
+def hip():
+    h = C.CDLL("libamdhip64.so")
+    h.hipStreamCreateWithFlags.argtypes = [C.POINTER(P), C.c_uint]
+    h.hipStreamBeginCapture.argtypes = [P, C.c_int]
+    h.hipStreamEndCapture.argtypes = [P, C.POINTER(P)]
+    h.hipGraphInstantiate.argtypes = [C.POINTER(P), P, P, P, C.c_size_t]
+    h.hipGraphLaunch.argtypes = [P, P]
+    for f in (h.hipStreamSynchronize, h.hipGraphExecDestroy, h.hipGraphDestroy, h.hipStreamDestroy):
+        f.argtypes = [P]
+    return h
+
+
+def captured(hip, call):
+    """The call recorded without a workspace, so in the form without scratch, and replayed once."""
+    s, g, e = P(), P(), P()
+    assert hip.hipStreamCreateWithFlags(C.byref(s), 1) == 0
+    try:
+        assert hip.hipStreamBeginCapture(s, 0) == 0
+        try:
+            call(s)
+        finally:
+            rc = hip.hipStreamEndCapture(s, C.byref(g))
+        assert rc == 0 and g.value and hip.hipGraphInstantiate(C.byref(e), g, None, None, 0) == 0
+        assert hip.hipGraphLaunch(e, s) == 0 and hip.hipStreamSynchronize(s) == 0
+        hip.hipGraphExecDestroy(e)
+        hip.hipGraphDestroy(g)
+    finally:
+        hip.hipStreamDestroy(s)
+
+
+def part(hpt, t, first, n):
+    """n elements of a tensor's memory."""
+    return hpt.Tensor.from_raw(t.ptr + first * t.dtype.size, [n], t.dtype)
+
+
+LONG = 1 << 26  # elements of a row: 65536 of a thread, whose sum in f32, term by term, would be off by 1e-4 and more
+SUM = 64 * F32_STEP
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_of_a_long_row(hpt, dev, residual):
+    x = hpt.Tensor.full(1.1, [1, LONG], hpt.f32)
+    v = np.float64(np.float32(1.1))
+    if residual:
+        r = hpt.Tensor.full(0.2, [1, LONG], hpt.f32)
+        v = np.float64(np.float32(1.1) + np.float32(0.2))
+        y, _ = x.add_rms_norm(r, [LONG], None, 0.25, sum_out=r)
+    else:
+        y = x.rms_norm([LONG], None, 0.25)
+    want = v / np.sqrt(v * v + 0.25)
+    for first in (0, LONG - 100):
+        near(part(hpt, y, first, 100).numpy(), np.full(100, want), (SUM + F32_STEP) * want)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_8_bit_norm_of_a_long_row(hpt, dev, name):
+    k = Kind(hpt, name)
+    v = float(k.round(1.1))
+    _, s = hpt.Tensor.full(1.1, [1, LONG], k.dtype).rms_norm_quant([LONG], None, 0.25)
+    want = v / np.sqrt(v * v + 0.25) / 127
+    near(s.numpy(), [want], (SUM + 2 * F32_STEP) * want)
+
+
+def test_norm_gradient_of_a_long_row(hpt, dev):
+    x, gy = hpt.Tensor.full(1.1, [1, LONG], hpt.f32), hpt.Tensor.full(0.7, [1, LONG], hpt.f32)
+    a, b = np.float64(np.float32(1.1)), np.float64(np.float32(0.7))
+    r = 1 / np.sqrt(a * a + 0.25)
+    gx, gg = x.rms_norm_backward(gy, [LONG], None, 0.25)
+    size = r * (b + a * r * r * a * b)
+    for first in (0, LONG - 100):
+        near(part(hpt, gx, first, 100).numpy(), np.full(100, r * (b - a * r * r * a * b)), (2 * SUM + F32_STEP) * size)
+        near(part(hpt, gg, first, 100).numpy(), np.full(100, a * b * r), (SUM + F32_STEP) * a * b * r)
+
+
+def test_softmax_of_a_long_row(hpt, dev, hip):
+    """One score of 0, all others -0.1: split, and as a whole."""
+    x = hpt.Tensor.full(-0.1, [1, 1, LONG], hpt.f32)
+    assert hpt.lib().hpt_hip_memcpy_h2d_sync(0, P(x.ptr + 4 * 5), np.zeros(1, np.float32).ctypes.data_as(P), 4) == 0
+    tab = hpt.Tensor.zeros([8, 1], hpt.f32)
+    e = np.exp(np.float64(np.float32(-0.1)))
+    total = 1 + (LONG - 1) * e
+    out = hpt.Tensor.zeros([1, 1, LONG], hpt.f32)
+
+    def check(y):
+        for first in (6, LONG - 100):
+            near(part(hpt, y, first, 100).numpy(), np.full(100, e / total), (F32_STEP + SUM) * e / total)
+        near(part(hpt, y, 5, 1).numpy(), [1 / total], (F32_STEP + SUM) / total)
+
+    check(x.softmax_bias(tab, max_distance=16))
+    captured(hip, lambda s: x.softmax_bias(tab, max_distance=16, out=out, stream=s))
+    check(out)
+
+
+def test_softmax_gradient_of_a_long_row(hpt, dev):
+    """All gradients alike: those of the scores are zeros, but for roundings of what cancels."""
+    p, g = hpt.Tensor.full(2.0 ** -26, [1, 1, LONG], hpt.f32), hpt.Tensor.full(1.1, [1, 1, LONG], hpt.f32)
+    gx, gt = p.softmax_bias_backward(g, 8, max_distance=16)
+    for first in (0, LONG - 100):
+        near(part(hpt, gx, first, 100).numpy(), np.zeros(100), (SUM + 4 * F32_STEP) * 1.1 * 2.0 ** -26)
+    near(gt.numpy(), np.zeros((8, 1)), (SUM + 64 * F32_STEP) * 1.1)
+
+
+@pytest.mark.parametrize("top", [0.0, 2.0 ** 18, 2.0 ** 20])
+def test_log_probability_of_a_long_row(hpt, dev, hip, top):
+    """One logit of `top`, all others an eighth below: split, and as a whole."""
+    x = hpt.Tensor.full(top - 0.125, [1, LONG], hpt.f32)
+    assert hpt.lib().hpt_hip_memcpy_h2d_sync(0, P(x.ptr + 4 * 7), np.full(1, top, np.float32).ctypes.data_as(P), 4) == 0
+    token = up(hpt, np.array([7]))
+    rest = np.log(1 + (LONG - 1) * np.exp(-0.125))
+    logp, lse = hpt.Tensor.zeros([1], hpt.f32), hpt.Tensor.zeros([1], hpt.f32)
+
+    def check(logp, lse):
+        near(logp.numpy(), [-rest], (SUM + 32 * F32_STEP))
+        near(lse.numpy(), [top + rest], SUM + 32 * F32_STEP + F32_STEP * top)
+
+    check(*x.token_logp(token))
+    captured(hip, lambda s: x.token_logp(token, logp_out=logp, lse_out=lse, stream=s))
+    check(logp, lse)
