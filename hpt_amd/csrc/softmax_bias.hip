@@ -65,8 +65,8 @@ constexpr int kPad = 8;
 __device__ __forceinline__ int right_of(const Buckets& b) { return b.both ? b.far : 0; }
 __host__ __device__ inline int places_of(const Buckets& b) { return b.far + (b.both ? b.far : 0) + 1 + 2 * kPad; }
 
-// What the rows of a matrix have in common: how many keys its sequence has, and the position of its query q0. Beyond +-2^29 every key is
-// far or hidden, as there are fewer than 2^29 of them.
+// What the rows of a matrix have in common: how many keys its sequence has, and the position of its query q0. Beyond +-2^30 every key is
+// far or hidden, as there are fewer than 2^29 of them (and distances stay within 32 bits).
 struct Place {
     int length, pos;
     template <class A> __device__ __forceinline__ Place(const A& a, int64_t matrix, int64_t q0) {
@@ -77,7 +77,7 @@ struct Place {
             n = len < 0 ? 0 : len < n ? len : n;
         }
         length = (int)n;
-        const int64_t p = q0 + a.offset, most = 1 << 29;
+        const int64_t p = q0 + a.offset, most = 1 << 30;
         pos = (int)(p > most ? most : p < -most ? -most : p);
     }
     // The end of the keys that query q0 + i sees.

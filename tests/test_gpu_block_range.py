@@ -263,7 +263,7 @@ def test_norm_of_a_long_row(hpt, dev, residual):
 @pytest.mark.parametrize("name", TYPES)
 def test_8_bit_norm_of_a_long_row(hpt, dev, name):
     k = Kind(hpt, name)
-    v = float(k.round(1.1))
+    v = float(k.round([1.1])[0])
     _, s = hpt.Tensor.full(1.1, [1, LONG], k.dtype).rms_norm_quant([LONG], None, 0.25)
     want = v / np.sqrt(v * v + 0.25) / 127
     near(s.numpy(), [want], (SUM + 2 * F32_STEP) * want)
@@ -324,3 +324,31 @@ def test_log_probability_of_a_long_row(hpt, dev, hip, top):
     check(*x.token_logp(token))
     captured(hip, lambda s: x.token_logp(token, logp_out=logp, lse_out=lse, stream=s))
     check(logp, lse)
+
+
+# ---- positions beyond 2^29 ---------------------------------------------------------------------------------------
+
+def test_a_query_beyond_two_to_the_29(hpt, dev):
+    """A query some places behind the last of nearly 2^29 keys: the buckets of their distances, forward and backward."""
+    k = Kind(hpt, "bf16")
+    n, tail = (1 << 29) - 2, 256
+    offset = (1 << 29) + 5
+    begin = [0, 1, 2, 3, 4, 8, 16, 32]  # 8 buckets, distances up to 64
+    d = offset - np.arange(n - tail, n)
+    which = np.array([max(b for b in range(8) if begin[b] <= v) for v in d])
+    x = hpt.Tensor.zeros([1, 1, n], hpt.bf16)
+    tab, table = k.up(np.array([0, 1, 2, 3, 4, 5, 6, 0.5])[:, None])
+    p = x.softmax_bias(tab, bidirectional=False, max_distance=64, query_offset=offset, out=x)
+    near_ones = np.exp(table[which, 0])
+    total = (n - tail) * np.exp(0.5) + near_ones.sum()
+    assert sorted(set(which)) == [5, 6, 7], "the last keys are in the buckets before the last one"
+    near(k.down(part(hpt, p, n - tail, tail)), near_ones / total, near_ones / total * (k.step + 400 * F32_STEP))
+    g = hpt.Tensor.zeros([1, 1, n], hpt.bf16)
+    ones, last = k.up(np.ones(tail))
+    assert hpt.lib().hpt_hip_memcpy_d2d_sync(0, P(g.ptr + 2 * (n - tail)), P(ones.ptr), 2 * tail) == 0
+    p_tail = k.down(part(hpt, p, n - tail, tail))
+    gt = p.softmax_bias_backward(g, 8, bidirectional=False, max_distance=64, query_offset=offset, out=p)[1].numpy()[:, 0]
+    s = p_tail.sum()
+    want = np.array([(p_tail * (1 - s))[which == b].sum() for b in range(8)])
+    assert not gt[:5].any()
+    near(gt[5:7], want[5:7], 400 * F32_STEP * want[5:7])
