@@ -434,7 +434,8 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
     for (int e = threadIdx.x; e < a.cols; e += blockDim.x) part[e] = fold[e];
 }
 
-// Rows of any length, swept twice; the sums for gamma grow in the workgroup's own row of partial sums (a thread meets its own elements).
+// Rows of any length, swept twice; the sums for gamma grow in the workgroup's own row of partial sums (a thread meets its own elements). Rows shorter than a vector can be
+// many thousands for each workgroup: the first thread keeps their sums in f64 (in f32, 4096 rows of the same sign were 5e-5 off).
 template <class T>
 __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs a) {
     constexpr int VEC = 16 / sizeof(T);
@@ -444,6 +445,7 @@ __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs
     const T* gamma = (const T*)a.gamma;
     float* part = a.ggamma ? a.partial + (int64_t)blockIdx.x * a.cols : nullptr;
     bool fresh = true;
+    double few[VEC] = {};
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, fresh = false) {
         const T* x = (const T*)a.x + offset_of(a.kept, row);
         const T* gy = (const T*)a.gy + row * a.cols;
@@ -481,10 +483,16 @@ __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs
                 if (gsum) d += Elem<T>::widen(more.v[i]);
                 p.v[i] = Elem<T>::narrow(d);
                 const int e = v * VEC + i;
-                if (part && e < a.cols) part[e] = fresh ? gv * (xv * r) : part[e] + gv * (xv * r);
+                if (vecs == 1) few[i] += gv * (xv * r);
+                else if (part && e < a.cols) part[e] = fresh ? gv * (xv * r) : part[e] + gv * (xv * r);
             }
             store_sweep_vec<T, VEC>((T*)a.gx + row * a.cols, v, a.cols, p);
         }
+    }
+    if (part && vecs == 1 && threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < a.cols) part[i] = (float)few[i];
     }
 }
 

@@ -352,3 +352,13 @@ def test_a_query_beyond_two_to_the_29(hpt, dev):
     want = np.array([(p_tail * (1 - s))[which == b].sum() for b in range(8)])
     assert not gt[:5].any()
     near(gt[5:7], want[5:7], 400 * F32_STEP * want[5:7])
+
+
+@pytest.mark.parametrize("cols", [1, 3])
+def test_norm_gradient_of_millions_of_rows_shorter_than_a_vector(hpt, dev, cols):
+    """The gradient of gamma, thousands of rows for each workgroup."""
+    rows = 1 << 22
+    x, gy = hpt.Tensor.full(1.1, [rows, cols], hpt.f32), hpt.Tensor.full(0.7, [rows, cols], hpt.f32)
+    a, b = np.float64(np.float32(1.1)), np.float64(np.float32(0.7))
+    want = rows * a * b / np.sqrt(a * a + 0.25)
+    near(x.rms_norm_backward(gy, [cols], None, 0.25)[1].numpy(), np.full(cols, want), SUM * want)
