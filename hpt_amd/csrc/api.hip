@@ -813,10 +813,10 @@ static void check_tokens(const hpt_view* token, int64_t rows, const char* name) 
     if (token->dtype != HPT_I32 && token->dtype != HPT_I64) fail(HPT_ERR_DTYPE, "%s: dtype is %s, expected i32 or i64", name, dtype_name(token->dtype));
     check_operand(token, token->dtype, rows, nullptr, name);
 }
-// Each token's loss (policy loss only), then the parts of split rows.
+// The parts of split rows, or each token's loss and slope (policy loss only).
 static size_t policy_bytes(const hpt_view* logits, const RowsOf& r, bool losses) {
     const int split = policy_split(logits->dtype, r.rows, r.cols);
-    return sizeof(double) * (size_t)((losses ? r.rows + (r.rows & 1) : 0) + (split > 1 ? 2 * r.rows * split : 0));
+    return sizeof(double) * (size_t)(split > 1 ? 2 * r.rows * split : losses ? 2 * r.rows : 0);
 }
 static void run_policy(int dev, void* stream, const hpt_view* logits, const RowsOf& r, PolicyArgs& a, const hpt_view* token, const hpt_view* workspace, bool losses, const char* what) {
     a.x = logits->data;
@@ -829,8 +829,7 @@ static void run_policy(int dev, void* stream, const hpt_view* logits, const Rows
     hipStream_t st = (hipStream_t)stream;
     with_workspace(dev, st, workspace, policy_bytes(logits, r, losses), !losses, what, [&](void* p) {
         a.split = p ? policy_split(logits->dtype, r.rows, r.cols) : 1;
-        a.each = losses ? (double*)p : nullptr;
-        a.partial = (double*)p + (losses ? r.rows + (r.rows & 1) : 0);
+        a.each = a.partial = (double*)p;
         launch_policy_loss(logits->dtype, a, st);
         check_launch(what);
     });

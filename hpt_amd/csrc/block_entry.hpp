@@ -161,8 +161,8 @@ struct PolicyArgs {
     int mask_bool;
     double clip_low, clip_high, kl_weight;
     float *loss, *logp, *lse, *weight;
-    double* each;         // [rows] scratch: the tokens' losses
-    double* partial;      // [rows, split, 2] scratch
+    double* each;         // [rows, 2] scratch of rows that are not split: the tokens' losses and slopes, times the mask
+    double* partial;      // [rows, split, 2] scratch of rows that are
     int64_t rows;
     int cols;
     int split;

@@ -63,8 +63,8 @@ struct RowLoss {
     double loss, slope;
     __device__ __forceinline__ void store(const PolicyArgs& a, int64_t row) const {
         if (!a.old_logp) return;
-        a.each[row] = loss;
-        a.weight[row] = (float)slope;  // (over the sum of the mask: in the last launch)
+        a.each[2 * row] = loss;
+        a.each[2 * row + 1] = slope;  // (becomes the weight over the sum of the mask, in the last launch)
     }
 };
 // A row's results from its maximum, sum and token.
@@ -92,10 +92,13 @@ __device__ __forceinline__ RowLoss skip_row(const PolicyArgs& a, int64_t row) {
     return {0.0, 0.0};
 }
 
+// Wavefronts on a SIMD: five as long as that needs no more than 96 registers (bf16 [8192, 50257] 167 us, with four of them, or with five and two registers spilled, 185); f16 needs a few more.
+template <class T> constexpr int kStatsWaves = std::is_same<T, f16_t>::value ? 4 : 5;
+
 // Maximum and sum of a part of a row. Vectors are aligned from the part's first aligned element on; the elements before it and behind the
 // last whole vector are taken one by one. Four vectors of a thread are in flight together. Bound by memory: bf16 [8192, 50257] 153 us, 5.4 TB/s.
 template <class T>
-__global__ __launch_bounds__(256, 5) void policy_stats_kernel(const PolicyArgs a) {
+__global__ __launch_bounds__(256, kStatsWaves<T>) void policy_stats_kernel(const PolicyArgs a) {
     constexpr int VEC = 16 / sizeof(T), B = 4;
     __shared__ float most[4];
     __shared__ double sums[4];
@@ -174,14 +177,11 @@ __global__ __launch_bounds__(256, 5) void policy_stats_kernel(const PolicyArgs a
         double top = (double)m / kLog2eExact;
         if (!(fabsf(m) < kNear) && n > 0) {
             // infinities, or finite logits far from zero (a row masked as a whole, or a part of one): element by element, by their differences from the largest
-            // (loss alone, bf16 [8, 152000] with three quarters masked by -1e9, whole parts of the split rows among them, 15.1 us, without a mask 11.3). Five wavefronts per SIMD hold
-            // as long as this needs no more than 96 registers: bf16 [8192, 50257] 167 us, with four 184.
+            // (loss alone, bf16 [8, 152000] with three quarters masked by -1e9, whole parts of the split rows among them, 15.8 us, without a mask 11.2).
             float t = -inf;
-#pragma unroll 8
             for (int i = threadIdx.x; i < n; i += 256) t = fmaxf(t, Elem<T>::widen(x[i]));
             t = block_reduce<MaxF>(t, most);
             double add = 0.0;
-#pragma unroll 8
             for (int i = threadIdx.x; i < n; i += 256) {
                 const float v = Elem<T>::widen(x[i]);
                 add += (double)(v == t ? 1.0f : __expf(v - t));
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
     } else {
 #pragma unroll 4
         for (int64_t row = threadIdx.x; row < a.rows; row += 1024) {
-            v[0] += a.each[row];
+            v[0] += a.each[2 * row];
             v[1] += mask_of(a, row);
         }
     }
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(1024) void policy_sum_kernel(const PolicyArgs a) {
         }
     } else {
 #pragma unroll 4
-        for (int64_t row = threadIdx.x; row < a.rows; row += 1024) a.weight[row] = (float)((double)a.weight[row] * inv);
+        for (int64_t row = threadIdx.x; row < a.rows; row += 1024) a.weight[row] = (float)(a.each[2 * row + 1] * inv);
     }
 }
 

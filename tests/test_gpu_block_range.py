@@ -354,6 +354,24 @@ def test_a_query_beyond_two_to_the_29(hpt, dev):
     near(gt[5:7], want[5:7], 400 * F32_STEP * want[5:7])
 
 
+# ---- weights of the mask next to the ends of f32 -----------------------------------------------------------------
+
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1.0, 1e30, 1e37])
+@pytest.mark.parametrize("rows,cols", [(2100, 40), (9, 40)])
+def test_a_mask_of_any_size(hpt, dev, rows, cols, size):
+    """The mask's weights are relative: all of them 1e-38 or 1e37 are the same as all of them 1."""
+    k, rng = Kind(hpt, "f32"), np.random.default_rng(rows)
+    t, x = k.up(rng.standard_normal((rows, cols)) * 3)
+    token = rng.integers(0, cols, rows)
+    logp = x[np.arange(rows), token] - logsumexp(x)
+    old, adv = (logp + 0.05).astype(np.float32), (rng.standard_normal(rows) * 30).astype(np.float32)
+    mask = np.full(rows, size, np.float32)
+    r = t.policy_loss(up(hpt, token), up(hpt, old), up(hpt, adv), mask=up(hpt, mask))
+    each = -np.exp(logp - old.astype(np.float64)) * adv
+    near(r.weight.numpy(), each / rows, (LSE + 4 * F32_STEP) * np.abs(each) / rows)
+    near(r.loss.numpy()[0], each.mean(), (LSE + 4 * F32_STEP) * np.abs(each).mean())
+
+
 @pytest.mark.parametrize("cols", [1, 3])
 def test_norm_gradient_of_millions_of_rows_shorter_than_a_vector(hpt, dev, cols):
     """The gradient of gamma, thousands of rows for each workgroup."""
