@@ -362,7 +362,8 @@ int32_t hpt_hip_policy_loss(int32_t dev, void* stream, const hpt_view* logits, c
 int32_t hpt_hip_policy_loss_workspace(const hpt_view* logits, size_t* bytes);
 
 /* The gradient of the logits of anything that depends on them through the rows' logp: grad * weight * (1[v = token] - exp(logits -
- * lse)), in logits' dtype. A row of weight 0 is not read. `grad_logits` may take the place of `logits`. */
+ * lse)), in logits' dtype. A row of weight 0 is not read and has zeros, whatever `grad` is. `grad_logits` may take the place
+ * of `logits`. `grad` is a number of the host: a captured call keeps it. */
 int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* lse,
                                      const hpt_view* weight, double grad, hpt_view* grad_logits);
 

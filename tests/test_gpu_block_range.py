@@ -380,3 +380,19 @@ def test_norm_gradient_of_millions_of_rows_shorter_than_a_vector(hpt, dev, cols)
     a, b = np.float64(np.float32(1.1)), np.float64(np.float32(0.7))
     want = rows * a * b / np.sqrt(a * a + 0.25)
     near(x.rms_norm_backward(gy, [cols], None, 0.25)[1].numpy(), np.full(cols, want), SUM * want)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("grad", [float("inf"), float("-inf"), float("nan"), 1e300, 2.0])
+def test_a_row_of_weight_0_has_no_gradient(hpt, dev, name, grad):
+    """Whatever the logits and the loss's gradient are (a loss scale that has overflowed)."""
+    k, rng = Kind(hpt, name), np.random.default_rng(1)
+    x = rng.standard_normal((3, 5003))
+    x[1] = np.nan
+    t, x = k.up(x)
+    zero = hpt.Tensor.zeros([3], hpt.f32)
+    weight = up(hpt, np.array([1, 0, -0.0], np.float32))
+    got = k.down(t.policy_loss_backward(up(hpt, np.array([3, -100, 4])), zero, weight, grad))
+    assert not got[1:].any()
+    if grad == 2.0:
+        assert np.isfinite(got[0]).all() and got[0].any()
