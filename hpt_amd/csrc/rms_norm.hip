@@ -376,7 +376,7 @@ __global__ __launch_bounds__(1024) void rms_grad_kernel(const RmsGradArgs a) {
         }
         fold_row<SumF>(s, tpr, sums, turn);
         const float r = 1.0f / sqrtf(s[0] / (float)a.cols + a.eps);
-        const float c = r * r * (s[1] / (float)a.cols);
+        const float c = r * (r * (s[1] / (float)a.cols));  // (r^2 alone may be beyond f32)
         T* gx = (T*)a.gx + row * a.cols;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(1024) void rms_grad_stream_kernel(const RmsGradArgs
         }
         fold_row<SumD>(s, 1024, sums, turn);
         const float r = 1.0f / sqrtf((float)(s[0] / a.cols) + a.eps);
-        const float c = r * r * (float)(s[1] / a.cols);
+        const float c = r * (r * (float)(s[1] / a.cols));
         for (int v = threadIdx.x; v < vecs; v += 1024) {
             const Pack<T, VEC> xp = sweep_vec<T>(x, v, a.cols), gp = sweep_vec<T>(gy, v, a.cols);
             Pack<T, VEC> g, more, p;

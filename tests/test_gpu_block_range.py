@@ -396,3 +396,20 @@ def test_a_row_of_weight_0_has_no_gradient(hpt, dev, name, grad):
     assert not got[1:].any()
     if grad == 2.0:
         assert np.isfinite(got[0]).all() and got[0].any()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [5, 64, 1001, 4096, 40000])
+@pytest.mark.parametrize("eps", [1e-12, 1e-38, 1e-40])
+def test_gradient_of_rows_of_zeros(hpt, dev, name, cols, eps):
+    """1 / sqrt(eps) times the gradient, also where 1 / eps is beyond f32."""
+    k, rng = Kind(hpt, name), np.random.default_rng(cols)
+    x = rng.standard_normal((5, cols))
+    x[::2] = 0
+    t, x = k.up(x)
+    gy, grad = k.up(rng.standard_normal((5, cols)))
+    gx, gg = t.rms_norm_backward(gy, [cols], None, eps)
+    e = np.float64(np.float32(eps))
+    want = grad[::2] / np.sqrt(e)
+    near(k.down(gx)[::2], want, (k.step + 64 * F32_STEP) * np.abs(want))
+    assert np.isfinite(k.down(gx)).all() and np.isfinite(gg.numpy()).all()
