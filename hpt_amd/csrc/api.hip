@@ -765,7 +765,10 @@ static RowsOf check_rms_backward(const hpt_view* in, int n_norm_dims) {
     check_view(in, "rms_norm_backward input", true);
     check_block_dtype(in, "rms_norm_backward input");
     if (n_norm_dims <= 0 || n_norm_dims > in->ndim) fail(HPT_ERR_SHAPE, "rms_norm_backward: %d normalized dims but input has %d", n_norm_dims, in->ndim);
-    return rows_of(in, n_norm_dims, "rms_norm_backward input");
+    const RowsOf r = rows_of(in, n_norm_dims, "rms_norm_backward input");
+    // (no rows are of any length, but gamma has a gradient of zeros)
+    if (r.cols >= kMostCols) fail(HPT_ERR_SHAPE, "rms_norm_backward input: rows of %lld elements, fewer than %lld expected", (long long)r.cols, (long long)kMostCols);
+    return r;
 }
 static size_t rms_backward_bytes(const hpt_view* in, const RowsOf& r) {
     return r.rows && r.cols ? (size_t)(rms_grad_partials(in->dtype, r.rows, r.cols) * r.cols) * sizeof(float) : 0;

@@ -542,7 +542,7 @@ int64_t grad_parts(int dtype, int64_t rows, int64_t cols, bool more, bool five) 
     const int64_t blocks = (rows + d.rows_per_block() - 1) / d.rows_per_block();
     const int waves = d.threads / 64;
     const int64_t resident = 256 * (dtype == HPT_F32 ? std::max(2, (more ? 8 : 12) / waves) : std::max(1, (five && waves <= 4 ? 20 : 16) / waves));
-    // (256 MiB of partial sums at most)
+    // (256 MiB of partial sums at most, or one row of them where that is longer: from 32 Mi columns on a single workgroup walks the rows)
     return std::min({blocks, resident, std::max<int64_t>(512, blocks * 5 / 8 / 256 * 256), std::max<int64_t>(1, (64 << 20) / std::max<int64_t>(1, cols))});
 }
 
