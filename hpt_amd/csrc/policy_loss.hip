@@ -201,7 +201,8 @@ __global__ __launch_bounds__(256, kStatsWaves<T>) void policy_stats_kernel(const
     }
 }
 
-// A split row from its parts. The mask and what its token brings along are on their way together; a hidden row's logits are not read.
+// A split row from its parts. They are weighted by the hardware's exponential, of f32 logits too: one of -D is off by D / 2^24 of itself or so, which is D e^-D / 2^24 of the row's sum at
+// most, less than a rounding. The mask and what its token brings along are on their way together; a hidden row's logits are not read.
 template <class T> __device__ __forceinline__ RowLoss join_row(const PolicyArgs& a, int64_t row, float mask) {
     const Token t(a, row);
     if (mask == 0.0f) return skip_row(a, row);

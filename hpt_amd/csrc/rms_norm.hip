@@ -75,13 +75,13 @@ template <int Q> __device__ __forceinline__ uint8_t quantized_one(float y, float
 
 // Whether workgroups walk the rows with the next one on its way while a row is summed and written, or take a row each and leave it to their
 // number that memory is busy. us, a row each -> walked: one operand f16 [13107, 5120] 64 -> 50, bf16 [4096, 16384] 65 -> 50, [8190, 4097]
-// 32 -> 27, [16384, 4096] 50.4 -> 49.7; in 8 bits [13107, 5120] 87 -> 50, [16384, 4096] 61 -> 44; x + residual in 8 bits [8192, 8192] 93 -> 84,
-// [8192, 4096] 46.8 -> 45.6, [16384, 4096] 88 -> 92. x + residual in its own type is ahead without ([16384, 4096] 89 against 97, [13107, 5120]
+// 32 -> 27, [16384, 4096] 50.4 -> 49.7; in 8 bits bf16 [13107, 5120] 73.2 -> 49.3, [16384, 4096] 51.7 -> 42.6, f32 [8192, 2048] 22.4 -> 20.1; x + residual in 8 bits f16 [13107, 5120] 80.7 -> 77.7, bf16 [8192, 8192]
+// 77.5 -> 75.0, but [8192, 4096] 38.7 -> 41.1 and [16384, 4096] 73.0 -> 78.0. x + residual in its own type is ahead without ([16384, 4096] 89 against 97, [13107, 5120]
 // 89 against 99), and beyond 16 elements per thread a second row does not fit the registers.
 template <class T, int NC, bool RES, int Q> constexpr bool kAhead = (!RES || Q != QUANT_NONE) && NC * 16 / (int)sizeof(T) <= 16;
 
 // Rows held in registers; gamma is fetched once. x + residual f16 [13107, 5120] 90 us, 6.0 TB/s of two reads and two writes; in 8 bits by 128 bf16 [8192, 4096]
-// 45 us, 5.2 TB/s; a step of decoding, bf16 [8, 4096], 4.5 us, a launch and the latency of one row. Q: groups of `group` elements are `group` / VEC neighbouring lanes
+// 46 us, 5.1 TB/s; a step of decoding, bf16 [8, 4096], 4.5 us, a launch and the latency of one row. Q: groups of `group` elements are `group` / VEC neighbouring lanes
 // (a power of two of them, within a wavefront), or the whole row.
 template <class T, int NC, bool AL, bool RES, int Q>
 __global__ __launch_bounds__(1024) void rms_row_kernel(const RmsArgs a) {

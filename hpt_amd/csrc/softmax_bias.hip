@@ -564,15 +564,15 @@ bool on_grid(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 size_t bias_lds(const Buckets& b) { return (size_t)places_of(b) * 4; }
 
-// Four vectors per thread: a row's maximum and sum cost the same for two. us, f16 [8, 16, 256 queries or so, keys] of 65 vectors 78 with two, 61.5 with up to
-// four, of 129 84 and 58, of 128 56.3 and 54.7.
+// Four vectors per thread: a row's maximum and sum cost the same for two. us of two vectors per thread and of up to four, f16 [8, 16, 512, 520] (65 vectors) 42.4 and 31.5, [.., 1032]
+// 77.3 and 53.3, and alike for 1024 keys, 45.2.
 // Rows above a wavefront go to workgroups of 128, 256, 512 or 768 threads with three or four vectors each (f32 four to eight): a fifth wavefront shares a
-// SIMD with the first, and then fewer workgroups run at once. us, f16 [1, 16, 256, 8208 keys and more], 320 threads of two vectors 69, 256 of three 50;
-// [.., 6144] 384 of two 58, 256 of three 39; one query, [64, 32, 1, 4104] 320 of two 20.3, 256 of three 14.3; f32 [.., 4400] 320 of four 35.9, 256 of five 27.2.
-// (385 ... 512 two-byte vectors: of whole matrices 256 threads of two 49, 128 of four 55; of one query 12.3 and 10.4.)
-// A workgroup holds rows of one matrix: where that has few (a step of decoding has one), they get the lanes of a wavefront (f32 [128, 16, 1, 256] 6.0 with 64, 7.2 with 16),
+// SIMD with the first, and then fewer workgroups run at once. us, f16 [8, 16, 256, 4104] 320 threads of two vectors 148, 256 of three 109; [1, 16, 256, 8208] 576 of two 55, 512
+// of three 41; [4, 16, 256, 6144] 384 of two 98, 256 of three 63; one query, [64, 32, 1, 4104] 320 of two 20.1, 256 of three 14.1; f32 [4, 16, 256, 4400] 320 of four 117, 256 of five 96.
+// (385 ... 512 two-byte vectors: of whole matrices, [8, 16, 256, 4096], 256 threads of two 83, 128 of four 109; of one query, [64, 32, 1, 4096], 12.2 and 9.7.)
+// A workgroup holds rows of one matrix: where that has few (a step of decoding has one), they get the lanes of a wavefront (f32 [128, 16, 1, 256] 6.1 with 64, 7.4 with 16),
 // and the workgroup is no larger than they need. Up to four rows of one query for each compute unit get up to four wavefronts, as the latency of a row is
-// all there is: f16 [16, 32, 1, 2048] 6.0 with 256 threads, 7.1 with 64, f32 [16, 32, 1, 1000] 5.9 and 7.0; f16 [128, 16, 1, 1536] 7.3 with 64, 8.2 with 128.
+// all there is: f16 [16, 32, 1, 2048] 6.0 with 256 threads, 7.0 with 64, f32 [16, 32, 1, 1000] 5.9 and 6.9; f16 [128, 16, 1, 1536] 7.5 with 64, 8.6 with 128.
 RowDeal bias_deal(int dtype, int64_t rows, int64_t queries, int64_t keys) {
     const bool wide = dtype == HPT_F32;
     const int64_t vecs = (keys * (int64_t)dtype_size(dtype) + 15) / 16;
@@ -592,9 +592,9 @@ RowDeal bias_deal(int dtype, int64_t rows, int64_t queries, int64_t keys) {
     while (d.tpr <= 64 && d.threads > 64 && d.threads / 2 >= queries * d.tpr) d.threads /= 2;
     return d;
 }
-// Backward: two vectors per thread of two operands, four of f32 (two-byte elements with three and four: us, bf16 [.., 256 queries, keys] of 65 vectors 121 and 121, of 384 84
-// and 98, of 512 83 and 106), but one where two would leave a third of the lanes idle or so, 129 ... 256 vectors (of 150 101 and 93, of 192 90 and 83, of 256 87 and 82). 32 rows side
-// by side at most, because each of them has places of its own. 768 threads are three wavefronts on each SIMD: [1, 16, 256, 9600] with 640 threads 69, with 768 63; f32 [.., 8196] 95 and 83.
+// Backward: two vectors per thread of two operands, four of f32 (two-byte elements with four: us, bf16 [8, 16, 256, 520] 27.3 with two and 34.0, [.., 4096] 158 and 207), but one for 129 ...
+// 256 vectors, where two would leave a third of the lanes idle or so (us of one and of two, [.., 1200] 49.5 and 55.4, [.., 1536] 59.6 and 65.7, [.., 2048] 70.9 and 77.1). 32 rows side
+// by side at most, because each of them has places of its own. 768 threads are three wavefronts on each SIMD: [1, 16, 256, 9600] with 640 threads 57.8, with 768 51.8; f32 [1, 16, 256, 8196] with 576 87, with 768 71.
 RowDeal bias_grad_deal(int dtype, int64_t keys) {
     const bool wide = dtype == HPT_F32;
     const int64_t vecs = (keys * (int64_t)dtype_size(dtype) + 15) / 16;
