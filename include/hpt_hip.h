@@ -278,10 +278,10 @@ int32_t hpt_hip_add_layernorm(int32_t dev, void* stream, const hpt_view* in, con
  * No trait of the reference has these; they stand beside layernorm, softmax_causal and log_softmax for models that
  * norm by the root mean square, bias attention by relative positions, or are trained on a policy loss, and give
  * their gradients. Dtypes f16, bf16 and f32; statistics, sums and the results called f32 below are f32 for all
- * of them (a score or a mean square beyond its range is an infinity), and every result is rounded once. A row's elements must be neighbours in memory, its rows may lie
- * anywhere; every other operand and every result is contiguous. Results share no memory with each other or with
- * operands, except that one may take the very place of an operand where its entry says so. An operand that is read
- * several times (rows of stride 0, a table that heads share) has its gradients at every place: whoever broadcast it sums them.
+ * of them (a scaled score, or a row's sum of squares, beyond its range is an infinity), and every result is rounded
+ * once. A row's elements must be neighbours in memory, its rows may lie anywhere; every other operand and every
+ * result is contiguous. Results share no memory with each other or with operands, except that one may take the very
+ * place of an operand where its entry says so. An operand that is read several times (rows of stride 0, a table that heads share) has its gradients at every place: whoever broadcast it sums them.
  *
  * `workspace` (may be NULL) is contiguous device memory of any dtype, aligned to 16 bytes, of at least as many
  * bytes as the entry's *_workspace function says; nothing in it has to start from a known value. Without one

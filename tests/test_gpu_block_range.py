@@ -242,6 +242,7 @@ def part(hpt, t, first, n):
 
 
 LONG = 1 << 26  # elements of a row: 65536 of a thread, whose sum in f32, term by term, would be off by 1e-4 and more
+# A vector's sum in f32 (up to 16 terms, or 32 logits with their exponentials), the rest in 64 bits, a rounding, a root, a reciprocal and products: below 64 half steps.
 SUM = 64 * F32_STEP
 
 
@@ -342,6 +343,7 @@ def test_a_query_beyond_two_to_the_29(hpt, dev):
     near_ones = np.exp(table[which, 0])
     total = (n - tail) * np.exp(0.5) + near_ones.sum()
     assert sorted(set(which)) == [5, 6, 7], "the last keys are in the buckets before the last one"
+    # (scores up to 6: 4 * 6 + 72 half steps as for any probabilities, and as much again for each of the steps between the parts of a row; 400 covers them)
     near(k.down(part(hpt, p, n - tail, tail)), near_ones / total, near_ones / total * (k.step + 400 * F32_STEP))
     g = hpt.Tensor.zeros([1, 1, n], hpt.bf16)
     ones, last = k.up(np.ones(tail))
