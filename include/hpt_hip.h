@@ -281,7 +281,8 @@ int32_t hpt_hip_add_layernorm(int32_t dev, void* stream, const hpt_view* in, con
  * of them (a scaled score, or a row's sum of squares, beyond its range is an infinity), and every result is rounded
  * once. A row's elements must be neighbours in memory, its rows may lie anywhere; every other operand and every
  * result is contiguous. Results share no memory with each other or with operands, except that one may take the very
- * place of an operand where its entry says so. An operand that is read several times (rows of stride 0, a table that heads share) has its gradients at every place: whoever broadcast it sums them.
+ * place of an operand where its entry says so. An operand that is read several times (rows of stride 0, a table that
+ * heads share) has its gradients at every place: whoever broadcast it sums them.
  *
  * `workspace` (may be NULL) is contiguous device memory of any dtype, aligned to 16 bytes, of at least as many
  * bytes as the entry's *_workspace function says; nothing in it has to start from a known value. Without one
@@ -343,8 +344,9 @@ int32_t hpt_hip_softmax_bias_backward(int32_t dev, void* stream, const hpt_view*
 int32_t hpt_hip_softmax_bias_backward_workspace(const hpt_view* probs, int64_t buckets, size_t* bytes);
 
 /* The log-probability of one token (i32 or i64) for each row of `logits` [..., vocabulary], and the row's log of the sum of
- * exponentials, both f32. (A row whose LARGEST logit is beyond 2^24 in magnitude has an lse as coarse as f32 is there, and so has
- * the gradient that is made from it; logp does not go through lse.) A token outside the vocabulary has a NaN for logp. */
+ * exponentials, both f32; logp does not go through lse. (Rounding costs lse up to |lse| / 2^24, and the gradient that is made from
+ * it as much of itself: with logits around 2^24 and beyond it is no gradient any more.) A token outside the vocabulary has a NaN
+ * for logp. */
 int32_t hpt_hip_token_logp(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* workspace,
                            hpt_view* logp, hpt_view* lse);
 
