@@ -121,6 +121,19 @@ SIGNATURES = {
     "hpt_hip_policy_loss_workspace": (C.c_int32, [C.POINTER(View), C.POINTER(C.c_size_t)]),
     "hpt_hip_policy_loss_backward": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View),
                               C.POINTER(View), C.POINTER(View), C.c_double, C.POINTER(View)]),
+    "hpt_hip_topk": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.c_int64, C.c_double, C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_topk_workspace": (C.c_int32, [C.POINTER(View), C.c_int64, C.POINTER(C.c_size_t)]),
+    "hpt_hip_sample": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.c_double, C.POINTER(View), C.c_int64,
+                              C.POINTER(View), C.c_double, C.POINTER(View), C.c_double, C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_sample_workspace": (C.c_int32, [C.POINTER(View), C.POINTER(C.c_size_t)]),
+    "hpt_hip_distill_loss": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View), C.c_double, C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.POINTER(View)]),
+    "hpt_hip_distill_loss_workspace": (C.c_int32, [C.POINTER(View), C.POINTER(C.c_size_t)]),
+    "hpt_hip_distill_loss_backward": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View), C.POINTER(View),
+                              C.POINTER(View), C.c_double, C.c_double, C.POINTER(View)]),
     "hpt_hip_contiguous": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.POINTER(View)]),
     "hpt_hip_contiguous_plan": (C.c_int32, [C.POINTER(View), C.POINTER(View), C.c_char_p, C.c_size_t]),
     "hpt_hip_binary_plan": (C.c_int32, [C.POINTER(View), C.POINTER(View), C.POINTER(View), C.c_char_p, C.c_size_t]),
@@ -155,6 +168,7 @@ class _ThroughCtypes:
     reduce = argreduce = softmax = layernorm = softmax_causal = staticmethod(lambda *_: None)
     rms_norm = rms_norm_quant = rms_norm_backward = softmax_bias = softmax_bias_backward = staticmethod(lambda *_: None)
     token_logp = policy_loss = policy_loss_backward = staticmethod(lambda *_: None)
+    topk = sample = distill_loss = distill_loss_backward = staticmethod(lambda *_: None)
 
     @staticmethod
     def free(device, ptr, nbytes, ordered):

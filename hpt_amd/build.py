@@ -49,6 +49,7 @@ def units():
     for e in range(N_REDUCE_ENTRIES):
         u.append((f"reduce_op_{e}.o", CSRC / "reduce_op.hip", [f"-DHPT_REDUCE_ENTRY={e}"]))
     u += [("rms_norm.o", CSRC / "rms_norm.hip", []), ("softmax_bias.o", CSRC / "softmax_bias.hip", []), ("policy_loss.o", CSRC / "policy_loss.hip", [])]
+    u += [(f"{n}.o", CSRC / f"{n}.hip", []) for n in ("topk", "sample", "distill_loss")]
     u += [("layout.o", CSRC / "layout.cpp", ["-x", "hip"]), ("api.o", CSRC / "api.hip", []),
           ("elementwise.o", CSRC / "elementwise.hip", [])]
     if (CSRC / "transpose_norm.hip").exists():
@@ -128,12 +129,14 @@ HOST_TEST_SRC = ROOT.parent / "tests" / "cpp" / "host_api_test.cpp"
 HOST_TEST_BIN = ROOT / "lib" / "host_api_test"
 BLOCK_TEST_SRC = ROOT.parent / "tests" / "cpp" / "block_api_test.cpp"
 BLOCK_TEST_BIN = ROOT / "lib" / "block_api_test"
+VOCAB_TEST_SRC = ROOT.parent / "tests" / "cpp" / "vocab_api_test.cpp"
+VOCAB_TEST_BIN = ROOT / "lib" / "vocab_api_test"
 
 
 def build_host_test(force: bool = False) -> Path:
     """The C++ host side (include/hpt_hip.hpp) and its device test programs, compiled with the host
     compiler alone: the ABI is plain C, no HIP header is needed above it."""
-    for src, out in ((BLOCK_TEST_SRC, BLOCK_TEST_BIN), (HOST_TEST_SRC, HOST_TEST_BIN)):
+    for src, out in ((VOCAB_TEST_SRC, VOCAB_TEST_BIN), (BLOCK_TEST_SRC, BLOCK_TEST_BIN), (HOST_TEST_SRC, HOST_TEST_BIN)):
         deps = [src, INCLUDE / "hpt_hip.hpp", INCLUDE / "hpt_hip.h", LIB]
         if not force and out.exists() and out.stat().st_mtime > max(d.stat().st_mtime for d in deps):
             continue

@@ -838,6 +838,71 @@ static void run_policy(int dev, void* stream, const hpt_view* logits, const Rows
     });
 }
 
+static void check_integers(const hpt_view* v, int64_t count, const char* name) {
+    check_view(v, name, true);
+    if (v->dtype != HPT_I32 && v->dtype != HPT_I64) fail(HPT_ERR_DTYPE, "%s: dtype is %s, expected i32 or i64", name, dtype_name(v->dtype));
+    check_operand(v, v->dtype, count, nullptr, name);
+}
+static double check_temperature(double t, bool zero, const char* what) {
+    if (!(t >= 1e-30 && t <= 1e30) && !(zero && t == 0)) fail(HPT_ERR_PARAM, "%s: temperature must be a positive number (1e-30 ... 1e30)%s", what, zero ? " or 0" : "");
+    return t;
+}
+
+static RowsOf top_rows_of(const hpt_view* in, int64_t k) {
+    const RowsOf r = logits_of(in, "topk input");
+    if (r.cols >= kMostCols) fail(HPT_ERR_SHAPE, "topk input: rows of %lld elements, fewer than %lld expected", (long long)r.cols, (long long)kMostCols);
+    if (k < 1 || k > r.cols || k > kMostTop) fail(HPT_ERR_PARAM, "topk: k is %lld, expected 1 to %lld", (long long)k, (long long)std::min<int64_t>(r.cols, kMostTop));
+    return r;
+}
+static size_t topk_bytes(const hpt_view* in, const RowsOf& r, bool lse) {
+    if (r.rows == 0) return 0;
+    const size_t row = topk_row_bytes(in->dtype, r.cols, lse);
+    return (size_t)rows_of_run(r.rows, row) * row;
+}
+
+static RowsOf sampled_rows_of(const hpt_view* logits) {
+    const RowsOf r = logits_of(logits, "sample logits");
+    if (r.cols > kMostSampled) fail(HPT_ERR_SHAPE, "sample logits: a vocabulary of %lld tokens, at most %lld expected", (long long)r.cols, (long long)kMostSampled);
+    return r;
+}
+static size_t sample_bytes(const RowsOf& r) {
+    if (r.rows == 0) return 0;
+    const size_t row = sample_row_bytes(r.cols);
+    return (size_t)rows_of_run(r.rows, row) * row;
+}
+// A setting for all rows or for each.
+static Setting setting_of(double all, const hpt_view* each, int64_t rows, bool whole, const char* name) {
+    if (!each) {
+        if (all != all) fail(HPT_ERR_PARAM, "%s: must be a number", name);
+        return {all, nullptr, 0};
+    }
+    if (whole) check_integers(each, rows, name);
+    else check_operand(each, HPT_F32, rows, nullptr, name);
+    return {0.0, each->data, each->dtype};
+}
+
+static RowsOf distill_rows_of(const hpt_view* logits, const char* name) {
+    const RowsOf r = logits_of(logits, name);
+    if (r.cols >= kMostCols) fail(HPT_ERR_SHAPE, "%s: rows of %lld elements, fewer than %lld expected", name, (long long)r.cols, (long long)kMostCols);
+    return r;
+}
+// The teacher's entries: [rows, k] logits and tokens.
+static int entries_of(const hpt_view* teacher, const hpt_view* index, int64_t rows, const char* what) {
+    const std::string t = std::string(what) + " teacher", i = std::string(what) + " index";
+    check_view(teacher, t.c_str(), true);
+    check_block_dtype(teacher, t.c_str());
+    if (teacher->ndim < 1) fail(HPT_ERR_SHAPE, "%s: input has no dimensions", t.c_str());
+    const int64_t k = teacher->shape[teacher->ndim - 1];
+    if (k < 1 || k > kMostEntries) fail(HPT_ERR_SHAPE, "%s: %lld entries a row, 1 to %d expected", t.c_str(), (long long)k, kMostEntries);
+    check_operand(teacher, teacher->dtype, rows * k, nullptr, t.c_str());
+    check_integers(index, rows * k, i.c_str());
+    if (index->ndim < 1 || index->shape[index->ndim - 1] != k) fail(HPT_ERR_SHAPE, "%s: must have as many entries a row as the teacher's logits", i.c_str());
+    return (int)k;
+}
+static size_t distill_bytes(const hpt_view* logits, const RowsOf& r) {
+    return (size_t)r.rows * (r.rows ? distill_split(logits->dtype, r.rows, r.cols) : 0) * kDistillPart * sizeof(double);
+}
+
 }  // namespace hpt
 
 using namespace hpt;
@@ -1617,6 +1682,219 @@ int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* 
         use_device(dev);
         launch_policy_loss_backward(logits->dtype, a, (hipStream_t)stream);
         check_launch("policy_loss_backward");
+    });
+}
+
+int32_t hpt_hip_topk_workspace(const hpt_view* in, int64_t k, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "topk_workspace: null output");
+        *bytes = topk_bytes(in, top_rows_of(in, k), true);
+    });
+}
+
+int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, double temperature, const hpt_view* workspace,
+                     hpt_view* values, hpt_view* index, hpt_view* lse) {
+    return guarded([&] {
+        const RowsOf r = top_rows_of(in, k);
+        if (lse) check_temperature(temperature, false, "topk");
+        check_workspace(workspace, "topk workspace");
+        check_out(values, in->dtype, r.rows * k, "topk values");
+        if (!index) fail(HPT_ERR_PARAM, "topk index: null view");
+        check_out(index, index->dtype == HPT_I32 ? HPT_I32 : HPT_I64, r.rows * k, "topk index");
+        if (lse) check_out(lse, HPT_F32, r.rows, "topk lse");
+        Overlaps o{"topk"};
+        o.reads(in, "the input");
+        o.writes(values);
+        o.writes(index);
+        o.writes(lse);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        if (r.rows == 0) return;
+        TopkArgs a{};
+        a.x = in->data;
+        a.kept = r.kept;
+        a.values = values->data;
+        a.index = index->data;
+        a.index64 = index->dtype == HPT_I64;
+        a.lse = lse ? (float*)lse->data : nullptr;
+        if (lse) {
+            a.inv_temperature = 1.0 / temperature;
+            a.steps = steps_of(temperature);
+        }
+        a.rows = r.rows;
+        a.cols = (int)r.cols;
+        a.k = (int)k;
+        a.tiles = (int)((r.cols + kTile - 1) / kTile);
+        const size_t row = topk_row_bytes(in->dtype, r.cols, lse != nullptr);
+        a.run = rows_of_run(r.rows, row);
+        use_device(dev);
+        hipStream_t st = (hipStream_t)stream;
+        with_workspace(dev, st, workspace, (size_t)a.run * row, false, "topk", [&](void* p) {
+            a.keys = p;
+            a.sums = (double*)((char*)p + (size_t)a.run * a.tiles * kTileGroups * dtype_size(in->dtype));
+            launch_topk(in->dtype, a, st);
+            check_launch("topk");
+        });
+    });
+}
+
+int32_t hpt_hip_sample_workspace(const hpt_view* logits, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "sample_workspace: null output");
+        *bytes = sample_bytes(sampled_rows_of(logits));
+    });
+}
+
+int32_t hpt_hip_sample(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* u, double temperature, const hpt_view* temperatures,
+                       int64_t top_k, const hpt_view* top_ks, double top_p, const hpt_view* top_ps, double min_p, const hpt_view* min_ps,
+                       const hpt_view* workspace, hpt_view* token, hpt_view* logp) {
+    return guarded([&] {
+        const RowsOf r = sampled_rows_of(logits);
+        check_operand(u, HPT_F32, r.rows, nullptr, "sample u");
+        SampleArgs a{};
+        if (!temperatures) check_temperature(temperature, true, "sample");
+        a.temperature = setting_of(temperature, temperatures, r.rows, false, "sample temperature");
+        a.top_k = setting_of((double)std::min<int64_t>(top_k, r.cols), top_ks, r.rows, true, "sample top_k");
+        a.top_p = setting_of(top_p, top_ps, r.rows, false, "sample top_p");
+        a.min_p = setting_of(min_p, min_ps, r.rows, false, "sample min_p");
+        check_workspace(workspace, "sample workspace");
+        if (!token) fail(HPT_ERR_PARAM, "sample token: null view");
+        check_out(token, token->dtype == HPT_I32 ? HPT_I32 : HPT_I64, r.rows, "sample token");
+        check_out(logp, HPT_F32, r.rows, "sample logp");
+        Overlaps o{"sample"};
+        o.reads(logits, "the logits");
+        o.reads(u, "u");
+        o.reads(temperatures, "the temperatures");
+        o.reads(top_ks, "top_k");
+        o.reads(top_ps, "top_p");
+        o.reads(min_ps, "min_p");
+        o.writes(token);
+        o.writes(logp);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        if (r.rows == 0) return;
+        a.x = logits->data;
+        a.kept = r.kept;
+        a.u = (const float*)u->data;
+        a.token = token->data;
+        a.token64 = token->dtype == HPT_I64;
+        a.logp = (float*)logp->data;
+        a.rows = r.rows;
+        a.cols = (int)r.cols;
+        a.tiles = (int)((r.cols + kTile - 1) / kTile);
+        const size_t row = sample_row_bytes(r.cols);
+        a.run = rows_of_run(r.rows, row);
+        use_device(dev);
+        hipStream_t st = (hipStream_t)stream;
+        with_workspace(dev, st, workspace, (size_t)a.run * row, false, "sample", [&](void* p) {
+            a.heads = p;
+            launch_sample(logits->dtype, a, st);
+            check_launch("sample");
+        });
+    });
+}
+
+int32_t hpt_hip_distill_loss_workspace(const hpt_view* logits, size_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(HPT_ERR_PARAM, "distill_loss_workspace: null output");
+        *bytes = distill_bytes(logits, distill_rows_of(logits, "distill_loss logits"));
+    });
+}
+
+int32_t hpt_hip_distill_loss(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* teacher, const hpt_view* index,
+                             const hpt_view* teacher_lse, const hpt_view* mask, double temperature, const hpt_view* workspace,
+                             hpt_view* loss, hpt_view* kl, hpt_view* terms) {
+    return guarded([&] {
+        const RowsOf r = distill_rows_of(logits, "distill_loss logits");
+        DistillArgs a{};
+        a.k = entries_of(teacher, index, r.rows, "distill_loss");
+        if (teacher_lse) check_operand(teacher_lse, HPT_F32, r.rows, nullptr, "distill_loss teacher_lse");
+        if (mask) {
+            check_view(mask, "distill_loss mask", true);
+            if (mask->dtype != HPT_F32 && mask->dtype != HPT_BOOL) fail(HPT_ERR_DTYPE, "distill_loss mask: dtype is %s, expected f32 or bool", dtype_name(mask->dtype));
+            check_operand(mask, mask->dtype, r.rows, nullptr, "distill_loss mask");
+        }
+        check_temperature(temperature, false, "distill_loss");
+        check_workspace(workspace, "distill_loss workspace");
+        check_out(loss, HPT_F32, 1, "distill_loss loss");
+        check_out(kl, HPT_F32, r.rows, "distill_loss kl");
+        check_out(terms, HPT_F32, r.rows * kTerms, "distill_loss terms");
+        Overlaps o{"distill_loss"};
+        o.reads(logits, "the logits");
+        o.reads(teacher, "the teacher's logits");
+        o.reads(index, "the index");
+        o.reads(teacher_lse, "teacher_lse");
+        o.reads(mask, "the mask");
+        o.writes(loss);
+        o.writes(kl);
+        o.writes(terms);
+        if (workspace) {
+            hpt_view w = *workspace;
+            o.writes(&w);
+        }
+        a.x = logits->data;
+        a.kept = r.kept;
+        a.teacher = teacher->data;
+        a.teacher_dtype = teacher->dtype;
+        a.index = index->data;
+        a.index64 = index->dtype == HPT_I64;
+        a.teacher_lse = teacher_lse ? (const float*)teacher_lse->data : nullptr;
+        a.mask = mask ? mask->data : nullptr;
+        a.mask_bool = mask && mask->dtype == HPT_BOOL;
+        a.temperature = temperature;
+        a.steps = steps_of(temperature);
+        a.loss = (float*)loss->data;
+        a.kl = (float*)kl->data;
+        a.terms = (float*)terms->data;
+        a.rows = r.rows;
+        a.cols = (int)r.cols;
+        a.split = distill_split(logits->dtype, r.rows, r.cols);
+        use_device(dev);
+        hipStream_t st = (hipStream_t)stream;
+        with_workspace(dev, st, workspace, distill_bytes(logits, r), false, "distill_loss", [&](void* p) {
+            a.partial = (double*)p;
+            launch_distill_loss(logits->dtype, a, st);
+            check_launch("distill_loss");
+        });
+    });
+}
+
+int32_t hpt_hip_distill_loss_backward(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* teacher, const hpt_view* index,
+                                      const hpt_view* terms, double temperature, double grad, hpt_view* grad_logits) {
+    return guarded([&] {
+        const RowsOf r = distill_rows_of(logits, "distill_loss_backward logits");
+        DistillGradArgs a{};
+        a.k = entries_of(teacher, index, r.rows, "distill_loss_backward");
+        check_operand(terms, HPT_F32, r.rows * kTerms, nullptr, "distill_loss_backward terms");
+        check_temperature(temperature, false, "distill_loss_backward");
+        check_out(grad_logits, logits->dtype, view_size(logits), "distill_loss_backward grad_logits");
+        Overlaps o{"distill_loss_backward"};
+        o.reads(logits, "the logits");
+        o.reads(teacher, "the teacher's logits");
+        o.reads(index, "the index");
+        o.reads(terms, "the terms");
+        o.writes(grad_logits, logits);
+        if (r.rows == 0) return;
+        a.x = logits->data;
+        a.kept = r.kept;
+        a.teacher = teacher->data;
+        a.teacher_dtype = teacher->dtype;
+        a.index = index->data;
+        a.index64 = index->dtype == HPT_I64;
+        a.terms = (const float*)terms->data;
+        a.temperature = temperature;
+        a.steps = steps_of(temperature);
+        a.upstream = (float)grad;
+        a.out = grad_logits->data;
+        a.rows = r.rows;
+        a.cols = (int)r.cols;
+        use_device(dev);
+        launch_distill_loss_backward(logits->dtype, a, (hipStream_t)stream);
+        check_launch("distill_loss_backward");
     });
 }
 

@@ -1,5 +1,5 @@
 // Operators around a transformer's blocks: what the C ABI hands to their launchers (rms_norm.hip, softmax_bias.hip,
-// policy_loss.hip). The host has checked shapes, dtypes and overlaps; every tensor but `x` is contiguous.
+// policy_loss.hip, topk.hip, sample.hip, distill_loss.hip). The host has checked shapes, dtypes and overlaps; every tensor but `x` is contiguous.
 #pragma once
 
 #include <hip/hip_runtime_api.h>
@@ -185,5 +185,112 @@ struct PolicyGradArgs {
     int cols;
 };
 void launch_policy_loss_backward(int dtype, const PolicyGradArgs& a, hipStream_t st);
+
+// ---- the largest logits, and sampling ---------------------------------------------------------------
+
+constexpr int kTile = 8192;             // neighbouring logits that a workgroup of 256 threads takes at once, 32 a thread
+constexpr int kTileGroups = 256;        // one for each thread
+constexpr int kMostTop = 1024;          // logits that topk returns at most, and that a sampled row picks from in one piece
+constexpr int64_t kMostSampled = (int64_t)1 << 22;  // tokens of a vocabulary to sample from: kMostParts tiles
+constexpr int kMostParts = (int)(kMostSampled / kTile);
+constexpr size_t kMostRowScratch = (size_t)64 << 20;  // rows are taken in runs whose scratch stays below this
+
+// log2 e / temperature in two pieces: twelve bits, and what is left, large against the first product's roundings (a piece of the float's own last place would be rounded
+// away every time) and above 0, so that -inf times either is -inf.
+struct Steps {
+    float hi, lo;
+};
+Steps steps_of(double temperature);
+
+struct TopkArgs {
+    const void* x;        // rows of `cols` neighbouring logits
+    Dims kept;
+    void* values;         // [rows, k]
+    void* index;          // [rows, k] of i32 or i64
+    int index64;
+    float* lse;           // or null
+    double inv_temperature;  // (of lse alone)
+    Steps steps;
+    void* keys;           // [rows of a run, tiles, 256] scratch: each thread's largest, as an order key of the logits' size
+    double* sums;         // [rows of a run, tiles, 2] scratch: a tile's largest and its sum of exponentials below it
+    int64_t rows;
+    int cols, k;
+    int tiles;
+    int64_t run;          // rows of a run
+};
+
+// Scratch for each row, and rows of a run.
+size_t topk_row_bytes(int dtype, int64_t cols, bool lse);
+int64_t rows_of_run(int64_t rows, size_t row_bytes);
+void launch_topk(int dtype, const TopkArgs& a, hipStream_t st);
+
+// A setting of each row's sampling: one number for all, or a tensor of f32, i32 or i64.
+struct Setting {
+    double all;
+    const void* each;  // or null
+    int dtype;
+};
+
+struct SampleArgs {
+    const void* x;
+    Dims kept;
+    const float* u;       // [rows]
+    Setting temperature, top_k, top_p, min_p;
+    void* token;          // [rows] of i32 or i64
+    int token64;
+    float* logp;
+    void* heads;          // [rows of a run, tiles] scratch: SampleHead
+    void* bodies;         // [rows of a run, tiles] scratch: SampleBody
+    int64_t rows;
+    int cols;
+    int tiles;
+    int64_t run;
+};
+size_t sample_row_bytes(int64_t cols);
+void launch_sample(int dtype, const SampleArgs& a, hipStream_t st);
+
+// ---- distillation -----------------------------------------------------------------------------------
+
+constexpr int kTerms = 8;  // numbers that a row keeps for its gradient
+
+struct DistillArgs {
+    const void* x;            // rows of `cols` neighbouring logits
+    Dims kept;
+    const void* teacher;      // [rows, k] of f16, bf16 or f32
+    int teacher_dtype;
+    const void* index;        // [rows, k] of i32 or i64
+    int index64;
+    const float* teacher_lse; // or null: the entries are the whole of the teacher
+    const void* mask;
+    int mask_bool;
+    double temperature;
+    Steps steps;
+    float *loss, *kl, *terms;
+    double* partial;          // [rows, split, kDistillPart] scratch
+    int64_t rows;
+    int cols, k;
+    int split;
+};
+constexpr int kMostEntries = 1024;
+constexpr int kDistillPart = 8;
+int distill_split(int dtype, int64_t rows, int64_t cols);
+void launch_distill_loss(int dtype, const DistillArgs& a, hipStream_t st);
+
+struct DistillGradArgs {
+    const void* x;
+    Dims kept;
+    const void* teacher;
+    int teacher_dtype;
+    const void* index;
+    int index64;
+    const float* terms;
+    double temperature;
+    Steps steps;
+    float upstream;
+    void* out;
+    int64_t rows;
+    int cols, k;
+};
+void launch_distill_loss_backward(int dtype, const DistillGradArgs& a, hipStream_t st);
 
 }  // namespace hpt

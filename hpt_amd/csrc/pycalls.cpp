@@ -475,6 +475,39 @@ PyObject* py_policy_loss_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
              hpt_view* gl = r.view(),
              hpt_hip_policy_loss_backward(r.dev, r.stream, in, token, lse, weight, grad, gl));
 }
+
+// topk(tensor, stream, k, temperature, workspace, values, index, lse)
+PyObject* py_topk(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(8,
+             hpt_view* in = r.first(); const int64_t k = r.whole(); const double t = r.number(); hpt_view* ws = r.view(); hpt_view* v = r.view();
+             hpt_view* i = r.view(); hpt_view* lse = r.view(),
+             hpt_hip_topk(r.dev, r.stream, in, k, t, ws, v, i, lse));
+}
+
+// sample(tensor, stream, u, temperature, temperatures, top_k, top_ks, top_p, top_ps, min_p, min_ps, workspace, token, logp)
+PyObject* py_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(14,
+             hpt_view* in = r.first(); hpt_view* u = r.view(); const double t = r.number(); hpt_view* ts = r.view(); const int64_t k = r.whole();
+             hpt_view* ks = r.view(); const double p = r.number(); hpt_view* ps = r.view(); const double m = r.number(); hpt_view* ms = r.view();
+             hpt_view* ws = r.view(); hpt_view* token = r.view(); hpt_view* logp = r.view(),
+             hpt_hip_sample(r.dev, r.stream, in, u, t, ts, k, ks, p, ps, m, ms, ws, token, logp));
+}
+
+// distill_loss(tensor, stream, teacher, index, teacher_lse, mask, temperature, workspace, loss, kl, terms)
+PyObject* py_distill_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(11,
+             hpt_view* in = r.first(); hpt_view* teacher = r.view(); hpt_view* index = r.view(); hpt_view* lse = r.view(); hpt_view* mask = r.view();
+             const double t = r.number(); hpt_view* ws = r.view(); hpt_view* loss = r.view(); hpt_view* kl = r.view(); hpt_view* terms = r.view(),
+             hpt_hip_distill_loss(r.dev, r.stream, in, teacher, index, lse, mask, t, ws, loss, kl, terms));
+}
+
+// distill_loss_backward(tensor, stream, teacher, index, terms, temperature, grad, grad_logits)
+PyObject* py_distill_loss_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HPT_TAKE(8,
+             hpt_view* in = r.first(); hpt_view* teacher = r.view(); hpt_view* index = r.view(); hpt_view* terms = r.view(); const double t = r.number();
+             const double grad = r.number(); hpt_view* gl = r.view(),
+             hpt_hip_distill_loss_backward(r.dev, r.stream, in, teacher, index, terms, t, grad, gl));
+}
 #undef HPT_TAKE
 
 // free(device, address, bytes, ordered) -> status
@@ -507,6 +540,10 @@ PyMethodDef methods[] = {HPT_CALL("reduce", py_reduce),
                          HPT_CALL("token_logp", py_token_logp),
                          HPT_CALL("policy_loss", py_policy_loss),
                          HPT_CALL("policy_loss_backward", py_policy_loss_backward),
+                         HPT_CALL("topk", py_topk),
+                         HPT_CALL("sample", py_sample),
+                         HPT_CALL("distill_loss", py_distill_loss),
+                         HPT_CALL("distill_loss_backward", py_distill_loss_backward),
                          HPT_CALL("free", py_free),
                          {nullptr, nullptr, 0, nullptr}};
 #undef HPT_CALL

@@ -1,0 +1,222 @@
+// Device-side pieces that the operators over rows of logits share (topk.hip, sample.hip, distill_loss.hip): logits as order keys, a tile of
+// a row in a workgroup's registers, and the search for a place in a row's order.
+//
+// The order of a row's logits: NaN before everything, then the larger value, equal ones (and -0, +0) by their index. A key orders as the
+// value does, 0 is below all keys; a place is a key with the index behind it, counted down, so that places of a row differ.
+#pragma once
+
+#include "block_rows.hpp"
+
+namespace hpt {
+
+template <class T> struct Bits {
+    using type = uint16_t;
+    static constexpr uint32_t sign = 0x8000u, all = 0xFFFFu, inf = std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
+};
+template <> struct Bits<float> {
+    using type = uint32_t;
+    static constexpr uint32_t sign = 0x80000000u, all = 0xFFFFFFFFu, inf = 0x7F800000u;
+};
+template <class T> using KeyOf = typename Bits<T>::type;
+template <class T> constexpr uint32_t kNanKey = Bits<T>::all;
+template <class T> constexpr uint32_t kInfKey = Bits<T>::sign | Bits<T>::inf;
+template <class T> constexpr uint32_t kNegInfKey = ~(Bits<T>::sign | Bits<T>::inf) & Bits<T>::all;
+template <class T> constexpr int kKeyBits = 8 * sizeof(T);
+
+template <class T> __device__ __forceinline__ uint32_t bits_of(T x) { return __builtin_bit_cast(KeyOf<T>, x); }
+template <class T> __device__ __forceinline__ uint32_t key_of_bits(uint32_t b) {
+    using B = Bits<T>;
+    if ((b & ~B::sign) > B::inf) return kNanKey<T>;
+    if (b == B::sign) b = 0;
+    return b & B::sign ? ~b & B::all : b | B::sign;
+}
+template <class T> __device__ __forceinline__ uint32_t key_of(T x) { return key_of_bits<T>(bits_of(x)); }
+// The value of a key that is no NaN's.
+template <class T> __device__ __forceinline__ float value_of(uint32_t key) {
+    using B = Bits<T>;
+    const uint32_t b = key & B::sign ? key & ~B::sign : ~key & B::all;
+    return Elem<T>::widen(__builtin_bit_cast(T, (KeyOf<T>)b));
+}
+
+// The largest key of some vectors: two-byte logits two at a time, as signed numbers whose order is the values'. Negative NaNs, which that order puts below
+// everything, show as the largest plain bits.
+template <class T, int N> __device__ __forceinline__ uint32_t most_key(const Pack<T, 16 / sizeof(T)> (&p)[N]) {
+    using B = Bits<T>;
+    typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (sizeof(T) == 2) {
+        s16x2 top = {-32768, -32768};
+        u16x2 raw = {0, 0};
+#pragma unroll
+        for (int b = 0; b < N; ++b) {
+            struct Words {
+                uint32_t w[4];
+            };
+            const Words words = __builtin_bit_cast(Words, p[b]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const s16x2 s = __builtin_bit_cast(s16x2, words.w[i]);
+                const s16x2 o = s ^ ((s >> 15) & (int16_t)0x7FFF);
+                top = __builtin_elementwise_max(top, o);
+                raw = __builtin_elementwise_max(raw, __builtin_bit_cast(u16x2, words.w[i]));
+            }
+        }
+        const int16_t t = top.x > top.y ? top.x : top.y;
+        const uint16_t r = raw.x > raw.y ? raw.x : raw.y;
+        if (r > (B::sign | B::inf)) return kNanKey<T>;
+        return key_of_bits<T>((uint16_t)(t ^ ((t >> 15) & 0x7FFF)));
+    } else {
+        int32_t top = INT32_MIN;
+        uint32_t raw = 0;
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = bits_of(p[b].v[i]);
+                const int32_t s = (int32_t)u, o = s ^ ((s >> 31) & 0x7FFFFFFF);
+                top = top > o ? top : o;
+                raw = raw > u ? raw : u;
+            }
+        if (raw > (B::sign | B::inf)) return kNanKey<T>;
+        return key_of_bits<T>((uint32_t)(top ^ ((top >> 31) & 0x7FFFFFFF)));
+    }
+}
+
+// Vector v of a row of `cols` logits, -inf behind its end.
+template <class T> __device__ __forceinline__ Pack<T, 16 / sizeof(T)> logit_vec(const T* row, int v, int cols) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int e = v * VEC;
+    if (e + VEC <= cols) return load_pack_unaligned<T, VEC>(row + e);
+    Pack<T, VEC> p;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) p.v[i] = e + i < cols ? row[e + i] : Elem<T>::narrow(-__builtin_huge_valf());
+    return p;
+}
+// Vector b of the 32 logits that a thread has of a tile: the vectors of a tile lie thread beside thread.
+template <class T> __device__ __forceinline__ int tile_vec(int tile, int b, int thread) { return tile * (kTile * (int)sizeof(T) / 16) + b * kTileGroups + thread; }
+template <class T> constexpr int kTileVecs = kTile * sizeof(T) / 16 / kTileGroups;  // of a thread
+// All of them. A tile that is whole needs no look at the row's end, and its loads are on their way together.
+template <class T> __device__ __forceinline__ void load_tile(const T* row, int tile, int cols, Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
+    constexpr int VEC = 16 / sizeof(T);
+    if ((tile + 1) * (int64_t)kTile <= cols) {
+#pragma unroll
+        for (int b = 0; b < kTileVecs<T>; ++b) p[b] = load_pack_unaligned<T, VEC>(row + (int64_t)tile_vec<T>(tile, b, threadIdx.x) * VEC);
+    } else {
+#pragma unroll
+        for (int b = 0; b < kTileVecs<T>; ++b) p[b] = logit_vec<T>(row, tile_vec<T>(tile, b, threadIdx.x), cols);
+    }
+}
+
+struct MaxU {
+    __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+struct SumU64 {
+    __device__ static __forceinline__ uint64_t comb(uint64_t a, uint64_t b) { return a + b; }
+};
+
+// The sum of v over the threads before this one; `total`: over all of them. Every order is fixed. `place`: one number for each wavefront.
+__device__ __forceinline__ double scan_before(double v, double* place, double& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    double sum = v;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        union { double d; int i[2]; } in, out;
+        in.d = sum;
+        out.i[0] = __shfl_up(in.i[0], w, 64);
+        out.i[1] = __shfl_up(in.i[1], w, 64);
+        if (lane >= w) sum += out.d;
+    }
+    __syncthreads();
+    if (lane == 63) place[wave] = sum;
+    __syncthreads();
+    double before = 0.0, all = 0.0;
+    for (int w = 0; w < waves; ++w) {
+        if (w == wave) before = all;
+        all += place[w];
+    }
+    total = all;
+    double mine;
+    {
+        union { double d; int i[2]; } in, out;
+        in.d = sum;
+        out.i[0] = __shfl_up(in.i[0], 1, 64);
+        out.i[1] = __shfl_up(in.i[1], 1, 64);
+        mine = lane ? out.d : 0.0;
+    }
+    return before + mine;
+}
+
+// Digits of eight bits: how many of what is looked at have each, in four tables that neighbouring lanes take in turn (the largest of a row's groups of logits
+// have nearly all the same first digit, and lanes that add to one address wait for each other).
+struct Digits {
+    uint32_t n[256 * 4];
+    __device__ __forceinline__ void clear() {
+        for (int i = threadIdx.x; i < 256 * 4; i += blockDim.x) n[i] = 0;
+    }
+    __device__ __forceinline__ void add(uint32_t digit) { atomicAdd(&n[digit * 4 + (threadIdx.x & 3)], 1u); }
+    // The digit of the k-th from the top (k >= 1), and how many have a larger one: called by the whole first wavefront after a barrier; 0 with all of them before it where there are fewer than k.
+    __device__ __forceinline__ void find(uint32_t k, uint32_t& digit, uint32_t& above) const {
+        const int lane = threadIdx.x & 63;
+        uint32_t c[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // (lane 0 has the four largest digits)
+            const uint32_t* p = n + (255 - (lane * 4 + i)) * 4;
+            c[i] = p[0] + p[1] + p[2] + p[3];
+            sum += c[i];
+        }
+        uint32_t upto = sum;
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) {
+            const uint32_t o = __shfl_up(upto, w, 64);
+            if (lane >= w) upto += o;
+        }
+        const uint64_t reach = __ballot(upto >= k);
+        const int at = reach ? __builtin_ctzll(reach) : 63;
+        uint32_t before = upto - sum, d = 255 - lane * 4;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (before + c[i] < k && d == (uint32_t)(255 - (lane * 4 + i))) {
+                before += c[i];
+                --d;
+            }
+        digit = __shfl(d, at, 64);
+        above = __shfl(before, at, 64);
+    }
+};
+
+// Lanes of one wavefront, in the order of their bits: this lane's place among those that `want` one. One of them reserves them all.
+__device__ __forceinline__ uint32_t reserve(bool want, uint32_t* count) {
+    const uint64_t who = __ballot(want);
+    if (!who) return 0;
+    const int lane = threadIdx.x & 63, first = __builtin_ctzll(who);
+    uint32_t base = 0;
+    if (lane == first) base = atomicAdd(count, (uint32_t)__builtin_popcountll(who));
+    base = __shfl(base, first, 64);
+    return base + (uint32_t)__builtin_popcountll(who & ((1ull << lane) - 1));
+}
+
+// A place of the order in 64 bits.
+__device__ __forceinline__ uint64_t place_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (0xFFFFFFFFu - index); }
+__device__ __forceinline__ uint32_t index_of(uint64_t place) { return 0xFFFFFFFFu - (uint32_t)place; }
+__device__ __forceinline__ uint32_t key_of_place(uint64_t place) { return (uint32_t)(place >> 32); }
+
+// Largest first; n a power of two, every thread of the workgroup. Steps within 128 neighbours stay with a wavefront, whose accesses to LDS are in order.
+__device__ __forceinline__ void sort_places(uint64_t* list, int n) {
+    __syncthreads();
+    for (int size = 2; size <= n; size <<= 1)
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            for (int p = threadIdx.x; p < n / 2; p += blockDim.x) {
+                const int i = 2 * p - (p & (stride - 1)), j = i + stride;
+                const uint64_t a = list[i], b = list[j];
+                if (((i & size) == 0) == (a < b)) {
+                    list[i] = b;
+                    list[j] = a;
+                }
+            }
+            if (stride > 64 || (stride == 1 && size >= 128)) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    __syncthreads();
+}
+
+}  // namespace hpt

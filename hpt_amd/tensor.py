@@ -233,6 +233,14 @@ class PolicyLoss(NamedTuple):
     weight: "Tensor"
 
 
+class DistillLoss(NamedTuple):
+    """What distill_loss returns: the loss (one element), each row's divergence, and the numbers that distill_loss_backward takes
+    of each row."""
+    loss: "Tensor"
+    kl: "Tensor"
+    terms: "Tensor"
+
+
 class Tensor:
     def __init__(self, storage, ptr: int, shape, strides, dtype: DType, backend: str, device: int,
                  parent: Optional[int] = None):
@@ -878,6 +886,54 @@ class Tensor:
         self._block_call("policy_loss_backward", stream, token, lse, weight, float(grad), out)
         return out
 
+    def topk(self, k: int, temperature: float = 1.0, lse: bool = False, stream=None, values_out: Optional["Tensor"] = None,
+             index_out: Optional["Tensor"] = None, lse_out: Optional["Tensor"] = None, workspace: Optional["Tensor"] = None):
+        """(values, indices) of the k largest elements of each row [..., cols], largest first (NaN before all, equal ones by their
+        index), k at most 1024. With `lse` also the rows' log of the sum of exp(self / temperature), f32: what a teacher hands to
+        distill_loss."""
+        k, lead = int(k), self.shape[:-1]
+        values = self._fresh(values_out, lead + [max(k, 0)], self.dtype, stream)
+        index = self._fresh(index_out, lead + [max(k, 0)], i64, stream)
+        total = self._fresh(lse_out, lead or [1], f32, stream) if lse or lse_out is not None else None
+        self._block_call("topk", stream, k, float(temperature), workspace, values, index, total)
+        return (values, index) if total is None else (values, index, total)
+
+    def sample(self, u: "Tensor", temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=None, token_out: Optional["Tensor"] = None,
+               logp_out: Optional["Tensor"] = None, workspace: Optional["Tensor"] = None):
+        """(token, log-probability that it was drawn with) of each row of logits [..., vocabulary], picked by `u`, an f32 number in [0, 1) a
+        row, from softmax(self / temperature) over the kept tokens in the order of their indices: the `top_k` first (by value, then by
+        index; 0: all), of these the fewest that hold `top_p` of their probability, of these the ones with at least `min_p` of the
+        likeliest one's. A temperature of 0 takes the likeliest. Each setting is a number, or a tensor with one for each row."""
+        lead = self.shape[:-1] or [1]
+        token = self._fresh(token_out, lead, i64, stream)
+        logp = self._fresh(logp_out, lead, f32, stream)
+        given = []
+        for value, number in ((temperature, float), (top_k, int), (top_p, float), (min_p, float)):
+            given += [number(0), value] if isinstance(value, Tensor) else [number(value), None]
+        self._block_call("sample", stream, u, *given, workspace, token, logp)
+        return token, logp
+
+    def distill_loss(self, teacher: "Tensor", index: "Tensor", teacher_lse: Optional["Tensor"] = None, mask: Optional["Tensor"] = None,
+                     temperature: float = 1.0, stream=None, loss_out: Optional["Tensor"] = None, kl_out: Optional["Tensor"] = None,
+                     terms_out: Optional["Tensor"] = None, workspace: Optional["Tensor"] = None) -> DistillLoss:
+        """The divergence of logits [..., vocabulary] from a teacher's, of which `teacher` [..., k] are known at the tokens `index` (negative:
+        no entry), at `temperature`, times its square, averaged with `mask` as weights: a DistillLoss, whose terms
+        distill_loss_backward takes. With `teacher_lse` (topk's, at the same temperature) all other tokens count as one;
+        otherwise the teacher's probabilities are those of its entries alone."""
+        lead = self.shape[:-1]
+        loss = self._fresh(loss_out, [1], f32, stream)
+        kl = self._fresh(kl_out, lead or [1], f32, stream)
+        terms = self._fresh(terms_out, lead + [8], f32, stream)
+        self._block_call("distill_loss", stream, teacher, index, teacher_lse, mask, float(temperature), workspace, loss, kl, terms)
+        return DistillLoss(loss, kl, terms)
+
+    def distill_loss_backward(self, teacher: "Tensor", index: "Tensor", terms: "Tensor", temperature: float = 1.0, grad: float = 1.0,
+                              stream=None, out: Optional["Tensor"] = None) -> "Tensor":
+        """The gradient of the logits `self` from a DistillLoss's terms, times `grad`; `out` may be the logits."""
+        out = self._fresh(out, self.shape, self.dtype, stream)
+        self._block_call("distill_loss_backward", stream, teacher, index, terms, float(temperature), float(grad), out)
+        return out
+
     # ---- the steps either side of the path ------------------------------------------
     def astype(self, dtype: DType, stream=None) -> "Tensor":
         """astype (hpt/src/backends/cuda/tensor_impls.rs:129-140) to a float dtype (or to the same dtype)."""
@@ -1064,6 +1120,18 @@ def softmax_bias_backward_workspace(probs: Tensor, buckets: int) -> int:
 def policy_loss_workspace(logits: Tensor) -> int:
     """Of policy_loss and of token_logp."""
     return _workspace("policy_loss", logits)
+
+
+def topk_workspace(x: Tensor, k: int) -> int:
+    return _workspace("topk", x, int(k))
+
+
+def sample_workspace(logits: Tensor) -> int:
+    return _workspace("sample", logits)
+
+
+def distill_loss_workspace(logits: Tensor) -> int:
+    return _workspace("distill_loss", logits)
 
 
 def synchronize(device: int = 0, stream=None) -> None:

@@ -369,6 +369,43 @@ int32_t hpt_hip_policy_loss_workspace(const hpt_view* logits, size_t* bytes);
 int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* token, const hpt_view* lse,
                                      const hpt_view* weight, double grad, hpt_view* grad_logits);
 
+/* The k largest elements of each row of `in` [..., cols], 1 <= k <= 1024 (and cols), in order: a NaN before everything, then the larger value, equal
+ * values (and -0 and +0) by their index. `values` [..., k] of in's dtype, `index` [..., k] i32 or i64. `lse` (may be NULL; f32, one for each
+ * row): log sum exp(in / temperature), NaN where the row has one, otherwise +inf where it has one. The workspace is that of a call with lse. */
+int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, double temperature, const hpt_view* workspace,
+                     hpt_view* values, hpt_view* index, hpt_view* lse);
+int32_t hpt_hip_topk_workspace(const hpt_view* in, int64_t k, size_t* bytes);
+
+/* One token for each row of `logits` [..., vocabulary] (2^22 tokens at most), picked by the row's number `u` (f32; in [0, 1): what lies outside is taken as
+ * the nearer end, a NaN as 0). With weights w = exp((logit - largest) / temperature), what is kept of the row are the `top_k` first of the order of hpt_hip_topk (k <= 0: all),
+ * of these the fewest first ones whose weights reach top_p of theirs together (top_p >= 1: all; the first in any case), and of these the ones with w >= min_p
+ * (<= 0: all; above 1 counts as 1). `token` (i32 or i64) is the first, by index, at which the sum of the kept weights exceeds u times the sum of all
+ * kept ones, and `logp` (f32) the logarithm of its weight over that sum. Sums and weights have 64 bits. A temperature of 0 takes the first of the
+ * order. Settings are for all rows, or for each (a view that is not NULL: temperatures, top_ps and min_ps f32, top_ks i32 or i64; the number beside it
+ * is then not looked at). A row without a distribution (largest logit NaN or infinite, a temperature that is neither 0 nor 1e-30 ... 1e30, another setting that
+ * is NaN; as a number for all rows such settings are refused) has token -1 and logp NaN. */
+int32_t hpt_hip_sample(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* u, double temperature, const hpt_view* temperatures,
+                       int64_t top_k, const hpt_view* top_ks, double top_p, const hpt_view* top_ps, double min_p, const hpt_view* min_ps,
+                       const hpt_view* workspace, hpt_view* token, hpt_view* logp);
+int32_t hpt_hip_sample_workspace(const hpt_view* logits, size_t* bytes);
+
+/* The divergence of a student from a teacher of which 1 <= k <= 1024 logits a row are known: `teacher` [..., k] (f16, bf16 or f32, whatever the
+ * student's are) at the tokens `index` [..., k] (i32 or i64; negative: no entry). With p = softmax(logits / temperature) and q = softmax(teacher /
+ * temperature) over the row's entries, kl = sum q (log q - log p). With `teacher_lse` (f32, one for each row, of all of the teacher's logits over the
+ * temperature: hpt_hip_topk's) q = exp(teacher / temperature - teacher_lse), and all tokens without an entry count as one: kl gets r (log r -
+ * log s) with r = max(0, 1 - sum q) and s what p gives them (r is 0 where nothing is left to s). `loss` (one element) is temperature^2 times the mean of `kl` (one for each row) with `mask` (f32 weights
+ * or bool; NULL: all ones) as weights, 0 where the mask sums to 0. Rows whose mask is 0 are not read, and their kl is 0, as is that of a row whose entries
+ * are missing or -inf altogether. An entry outside the vocabulary makes the row's kl NaN; entries that name one token twice both count. `terms`: 8 numbers for each row, for the gradient. All f32. */
+int32_t hpt_hip_distill_loss(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* teacher, const hpt_view* index,
+                             const hpt_view* teacher_lse, const hpt_view* mask, double temperature, const hpt_view* workspace,
+                             hpt_view* loss, hpt_view* kl, hpt_view* terms);
+int32_t hpt_hip_distill_loss_workspace(const hpt_view* logits, size_t* bytes);
+
+/* The gradient of the logits from the terms of hpt_hip_distill_loss, called with the same operands and temperature, times `grad` (a number of the host: a captured
+ * call keeps it), in logits' dtype. Rows that do not count are not read and have zeros. `grad_logits` may take the place of `logits`. */
+int32_t hpt_hip_distill_loss_backward(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* teacher, const hpt_view* index,
+                                      const hpt_view* terms, double temperature, double grad, hpt_view* grad_logits);
+
 /* ---- the steps either side of the path ------------------------------------
  * What the callers of reductions and normalisations do to their operands just
  * before and after, kept on the device. */

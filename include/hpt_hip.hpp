@@ -19,7 +19,7 @@
 //   argmax argmin                                 IndexReduce   (:6-42)
 //   softmax log_softmax layernorm                 NormalizationOps (hpt-traits/src/ops/normalization.rs:6-64)
 //   contiguous astype add_ sub_ mul_ div_         Contiguous, astype, NormalBinOps
-//   rms_norm add_rms_norm rms_norm_quant softmax_bias token_logp policy_loss and their *_backward
+//   rms_norm add_rms_norm rms_norm_quant softmax_bias token_logp policy_loss topk sample distill_loss and their *_backward
 //                                                 no trait: the operators around a transformer's blocks (hpt_hip.h)
 //
 // Errors are thrown as hpt::TensorError, whose `kind` is the TensorError variant the Rust shim
@@ -34,6 +34,7 @@
 #include <numeric>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -164,6 +165,21 @@ struct PolicyTerms {
     double clip_low = 0.2, clip_high = 0.2, kl_weight = 0.0;
 };
 struct PolicyLoss;
+// How sample filters: numbers for all rows, or one for each where a tensor is given.
+struct SampleSettings {
+    double temperature = 1.0;
+    int64_t top_k = 0;
+    double top_p = 1.0, min_p = 0.0;
+    const Tensor<float>*temperatures = nullptr, *top_ps = nullptr, *min_ps = nullptr;
+    const Tensor<int64_t>* top_ks = nullptr;
+};
+// What distill_loss is told beside the teacher's entries, and what it returns.
+struct DistillTerms {
+    const Tensor<float>* teacher_lse = nullptr;  // (topk_lse's, at the same temperature) all other tokens count as one
+    const Tensor<float>* mask = nullptr;
+    double temperature = 1.0;
+};
+struct DistillLoss;
 
 template <class T> class Tensor {
   public:
@@ -461,6 +477,38 @@ template <class T> class Tensor {
         check(hpt_hip_policy_loss_backward(device_, nullptr, &vin, &vt, &vl, &vw, grad, &vout));
         return res;
     }
+    // (values, indices) of the k largest of each row, in order
+    std::pair<Tensor, Tensor<int64_t>> topk(int64_t k) const {
+        auto [values, index] = top_of(k);
+        hpt_view vin = view(), vv = values.view(), vi = index.view();
+        check(hpt_hip_topk(device_, nullptr, &vin, k, 1.0, nullptr, &vv, &vi, nullptr));
+        return {values, index};
+    }
+    // the same, and the rows' log of the sum of exp(x / temperature)
+    std::tuple<Tensor, Tensor<int64_t>, Tensor<float>> topk_lse(int64_t k, double temperature = 1.0) const {
+        auto [values, index] = top_of(k);
+        Tensor<float> lse = Tensor<float>::empty(rows_shape(), device_);
+        hpt_view vin = view(), vv = values.view(), vi = index.view(), vl = lse.view();
+        check(hpt_hip_topk(device_, nullptr, &vin, k, temperature, nullptr, &vv, &vi, &vl));
+        return {values, index, lse};
+    }
+    // (token, the log-probability that it was drawn with) of each row, by its number in [0, 1)
+    std::pair<Tensor<int64_t>, Tensor<float>> sample(const Tensor<float>& u, const SampleSettings& s = {}) const {
+        Tensor<int64_t> token = Tensor<int64_t>::empty(rows_shape(), device_);
+        Tensor<float> logp = Tensor<float>::empty(rows_shape(), device_);
+        hpt_view vin = view(), vu = u.view(), vt = token.view(), vl = logp.view(), v1{}, v2{}, v3{}, v4{};
+        check(hpt_hip_sample(device_, nullptr, &vin, &vu, s.temperature, optional(s.temperatures, v1), s.top_k, optional(s.top_ks, v2), s.top_p,
+                             optional(s.top_ps, v3), s.min_p, optional(s.min_ps, v4), nullptr, &vt, &vl));
+        return {token, logp};
+    }
+    template <class U> DistillLoss distill_loss(const Tensor<U>& teacher, const Tensor<int64_t>& index, const DistillTerms& terms = {}) const;
+    template <class U>
+    Tensor distill_loss_backward(const Tensor<U>& teacher, const Tensor<int64_t>& index, const Tensor<float>& terms, double temperature = 1.0, double grad = 1.0) const {
+        Tensor res = empty(shape_, device_);
+        hpt_view vin = view(), vt = teacher.view(), vi = index.view(), vs = terms.view(), vout = res.view();
+        check(hpt_hip_distill_loss_backward(device_, nullptr, &vin, &vt, &vi, &vs, temperature, grad, &vout));
+        return res;
+    }
 
     // ---- the steps either side ---------------------------------------------------------------------
     Tensor contiguous() const {
@@ -513,6 +561,13 @@ template <class T> class Tensor {
         for (size_t i = 0; ok && i < normalized_shape.size(); ++i) ok = shape_[ndim() - normalized_shape.size() + i] == normalized_shape[i];
         if (!ok) throw TensorError(ErrorKind::Shape, "normalized dims must match last dims of input tensor");
         return (int32_t)normalized_shape.size();
+    }
+    // (results of topk)
+    std::pair<Tensor, Tensor<int64_t>> top_of(int64_t k) const {
+        Shape each = shape_;
+        if (each.empty()) each = {1};
+        each.back() = k > 0 ? k : 0;
+        return {empty(each, device_), Tensor<int64_t>::empty(each, device_)};
     }
     Shape rows_shape() const { return ndim() > 1 ? Shape(shape_.begin(), shape_.end() - 1) : Shape{1}; }
     Tensor alias() const {
@@ -583,6 +638,21 @@ PolicyLoss Tensor<T>::policy_loss(const Tensor<int64_t>& token, const Tensor<flo
     hpt_view v0 = r.loss.view(), v1 = r.logp.view(), v2 = r.lse.view(), v3 = r.weight.view();
     check(hpt_hip_policy_loss(device_, nullptr, &vin, &vt, &vo, &va, optional(terms.reference, vr), optional(terms.mask, vm), terms.clip_low,
                               terms.clip_high, terms.kl_weight, nullptr, &v0, &v1, &v2, &v3));
+    return r;
+}
+
+struct DistillLoss {
+    Tensor<float> loss, kl, terms;  // loss: one element; kl: one for each row; terms: what the gradient takes
+};
+template <class T>
+template <class U>
+DistillLoss Tensor<T>::distill_loss(const Tensor<U>& teacher, const Tensor<int64_t>& index, const DistillTerms& terms) const {
+    Shape each = shape_;
+    if (!each.empty()) each.back() = 8;
+    DistillLoss r{Tensor<float>::empty({1}, device_), Tensor<float>::empty(rows_shape(), device_), Tensor<float>::empty(each, device_)};
+    hpt_view vin = view(), vt = teacher.view(), vi = index.view(), vl{}, vm{}, v0 = r.loss.view(), v1 = r.kl.view(), v2 = r.terms.view();
+    check(hpt_hip_distill_loss(device_, nullptr, &vin, &vt, &vi, optional(terms.teacher_lse, vl), optional(terms.mask, vm), terms.temperature,
+                               nullptr, &v0, &v1, &v2));
     return r;
 }
 
