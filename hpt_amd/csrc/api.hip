@@ -900,7 +900,7 @@ static int entries_of(const hpt_view* teacher, const hpt_view* index, int64_t ro
     return (int)k;
 }
 static size_t distill_bytes(const hpt_view* logits, const RowsOf& r) {
-    return (size_t)r.rows * (r.rows ? distill_split(logits->dtype, r.rows, r.cols) : 0) * kDistillPart * sizeof(double);
+    return (size_t)r.rows * (1 + kDistillPart * (r.rows ? distill_split(logits->dtype, r.rows, r.cols) : 0)) * sizeof(double);
 }
 
 }  // namespace hpt
@@ -1856,7 +1856,8 @@ int32_t hpt_hip_distill_loss(int32_t dev, void* stream, const hpt_view* logits, 
         use_device(dev);
         hipStream_t st = (hipStream_t)stream;
         with_workspace(dev, st, workspace, distill_bytes(logits, r), false, "distill_loss", [&](void* p) {
-            a.partial = (double*)p;
+            a.each = (double*)p;
+            a.partial = a.each + r.rows;
             launch_distill_loss(logits->dtype, a, st);
             check_launch("distill_loss");
         });

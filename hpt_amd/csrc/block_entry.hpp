@@ -266,13 +266,14 @@ struct DistillArgs {
     double temperature;
     Steps steps;
     float *loss, *kl, *terms;
-    double* partial;          // [rows, split, kDistillPart] scratch
+    double* each;             // [rows] scratch: their divergences
+    double* partial;          // [rows, split, kDistillPart] scratch: each part's largest logit, its sum of exponentials, and whether a token is named twice
     int64_t rows;
     int cols, k;
     int split;
 };
 constexpr int kMostEntries = 1024;
-constexpr int kDistillPart = 8;
+constexpr int kDistillPart = 3;
 int distill_split(int dtype, int64_t rows, int64_t cols);
 void launch_distill_loss(int dtype, const DistillArgs& a, hipStream_t st);
 

@@ -18,7 +18,6 @@ namespace {
 
 constexpr double kLog2eD = 1.4426950408889634;
 constexpr int kThreads = 256;
-constexpr int kOwn = kMostEntries / kThreads;  // entries of a thread
 constexpr int kBlock = 1 << 16;                // tokens that have a bit at a time
 
 __device__ __forceinline__ float mask_of(const void* mask, int is_bool, int64_t row) {
@@ -42,6 +41,10 @@ __device__ __forceinline__ void meet(float& m, double& s, float m2, double s2, f
     s = s * (double)(m == n ? 1.0f : __builtin_amdgcn_exp2f((m - n) * steps)) + s2 * (double)(m2 == n ? 1.0f : __builtin_amdgcn_exp2f((m2 - n) * steps));
     m = n;
 }
+
+// Wavefronts on a SIMD.
+template <class T> constexpr int kStatsWaves = 5;
+constexpr int kGradVecs = 4;  // vectors of a lane
 
 // What a row's parts have of it together.
 struct RowSums {
@@ -95,49 +98,24 @@ __device__ __forceinline__ void skip_row(const DistillArgs& a, int64_t row) {
     for (int i = 0; i < kTerms; ++i) a.terms[row * kTerms + i] = 0.0f;
 }
 
-// A row, or a part of one.
+// Largest logit and sum of exponentials of a row, or of a part of one; where the rest counts, of the tokens that no entry names (a bit each tells).
 template <class T, bool REST>
-__global__ __launch_bounds__(kThreads) void distill_stats_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(kThreads, kStatsWaves<T>) void distill_stats_kernel(const DistillArgs a) {
     constexpr int VEC = 16 / sizeof(T), B = 4;
     const float inf = __builtin_huge_valf();
-    __shared__ uint32_t bits[REST ? kBlock / 32 : 1];
+    __shared__ uint32_t bits[REST ? kBlock / 32 + 1 : 1];
     __shared__ float most[4];
-    __shared__ double sums[4], sums2[4];
-    __shared__ int again;
+    __shared__ double sums[4];
+    __shared__ int again;  // a token is named twice
     const float steps = a.steps.hi + a.steps.lo;
-    const double inv = 1.0 / a.temperature;
     for (int64_t at = blockIdx.x; at < a.rows * a.split; at += gridDim.x) {
         const int64_t row = quotient(at, a.split);
         const int part = (int)(at - row * a.split);
-        if (mask_of(a.mask, a.mask_bool, row) == 0.0f) {
-            if (threadIdx.x == 0 && a.split == 1) {
-                skip_row(a, row);
-                a.partial[at * kDistillPart] = 0.0;
-            }
-            continue;  // (the same for the whole workgroup)
-        }
+        if (mask_of(a.mask, a.mask_bool, row) == 0.0f) continue;  // (the same for the whole workgroup)
         const int each = ((a.cols + a.split - 1) / a.split + VEC - 1) / VEC * VEC;
         const int e0 = min(part * each, a.cols), e1 = min(e0 + each, a.cols);
         const T* x = (const T*)a.x + offset_of(a.kept, row);
-        // the entries, and the student's logits of those in this part
-        int token[kOwn];
-        float t[kOwn], xt[kOwn];
-        bool fresh[kOwn];  // (the first that names its token)
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const int j = threadIdx.x + i * kThreads;
-            token[i] = -1;
-            t[i] = -inf;
-            if (j < a.k) {
-                token[i] = token_of(a.index, a.index64, row * a.k + j, a.cols);
-                if (token[i] >= 0) t[i] = logit_of(a.teacher, a.teacher_dtype, row * a.k + j);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            xt[i] = token[i] >= e0 && token[i] < e1 ? Elem<T>::widen(x[token[i]]) : 0.0f;
-            fresh[i] = false;
-        }
+        if (threadIdx.x == 0) again = 0;  // (the thread that reads it)
         float m = -inf;
         double s = 0.0;
         auto take = [&](auto& v) {
@@ -158,65 +136,65 @@ __global__ __launch_bounds__(kThreads) void distill_stats_kernel(const DistillAr
         };
         for (int b0 = e0; b0 < e1; b0 += REST ? kBlock : e1 - e0) {
             const int b1 = REST ? min(b0 + kBlock, e1) : e1;
+            // vectors are aligned from the block's first aligned logit on; a token's bit stands so that those of a vector stand together
+            const int head = min(b1 - b0, (int)((16 - ((uintptr_t)(x + b0) & 15)) & 15) / (int)sizeof(T));
+            const int vecs = (b1 - b0 - head) / VEC, tail = b0 + head + vecs * VEC, first = b0 + head - VEC;
+            const T* body = x + b0 + head;
+            auto named = [&](int e) { return bits[(e - first) >> 5] >> ((e - first) & 31); };
             if constexpr (REST) {
                 __syncthreads();
-                if (threadIdx.x == 0) again = 0;
-                for (int i = threadIdx.x; i < (b1 - b0 + 31) / 32; i += kThreads) bits[i] = 0;
+                for (int i = threadIdx.x; i <= (b1 - first) / 32; i += kThreads) bits[i] = 0;
                 __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i)
-                    if (token[i] >= b0 && token[i] < b1) {
-                        const uint32_t bit = 1u << ((token[i] - b0) & 31);
-                        fresh[i] = !(atomicOr(&bits[(token[i] - b0) >> 5], bit) & bit);
-                        if (!fresh[i]) again = 1;
+                for (int j = threadIdx.x; j < a.k; j += kThreads) {
+                    const int e = token_of(a.index, a.index64, row * a.k + j, a.cols);
+                    if (e >= b0 && e < b1) {
+                        const uint32_t bit = 1u << ((e - first) & 31);
+                        if (atomicOr(&bits[(e - first) >> 5], bit) & bit) again = 1;
                     }
-                __syncthreads();
-                if (again) {  // an index twice: the entry that comes first
-#pragma unroll
-                    for (int i = 0; i < kOwn; ++i)
-                        if (token[i] >= b0 && token[i] < b1) {
-                            const int j = threadIdx.x + i * kThreads;
-                            fresh[i] = true;
-                            for (int l = 0; l < j && fresh[i]; ++l) fresh[i] = token_of(a.index, a.index64, row * a.k + l, a.cols) != token[i];
-                        }
                 }
+                __syncthreads();
             }
-            const int vecs = (b1 - b0) / VEC, tail = b0 + vecs * VEC;
-            if ((int)threadIdx.x < b1 - tail) {
-                const int e = tail + threadIdx.x;
+            // (fewer than two vectors of single logits: a lane each)
+            auto single = [&](int e) {
                 float v[1] = {Elem<T>::widen(x[e])};
                 if constexpr (REST)
-                    if (bits[(e - b0) >> 5] >> ((e - b0) & 31) & 1) v[0] = -inf;
+                    if (named(e) & 1) v[0] = -inf;
                 take(v);
-            }
-            for (int v = threadIdx.x; v < vecs; v += B * kThreads) {
+            };
+            if ((int)threadIdx.x < head) single(b0 + threadIdx.x);
+            if ((int)threadIdx.x < b1 - tail) single(tail + threadIdx.x);
+            // (no load hangs on a condition: the compiler would wait for each before the next)
+            for (int v0 = 0; v0 < vecs; v0 += B * kThreads) {
                 Pack<T, VEC> p[B];
 #pragma unroll
-                for (int b = 0; b < B; ++b) {
-                    if (v + b * kThreads < vecs) p[b] = load_pack_unaligned<T, VEC>(x + b0 + (int64_t)(v + b * kThreads) * VEC);
-                    else
+                for (int b = 0; b < B; ++b) p[b] = load_pack_stream<T, VEC>(body + (int64_t)min(v0 + (int)threadIdx.x + b * kThreads, vecs - 1) * VEC);
+                if constexpr (REST) {
+                    uint32_t some[B], any = 0;
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) p[b].v[i] = Elem<T>::narrow(-inf);
+                    for (int b = 0; b < B; ++b) {
+                        some[b] = named(b0 + head + min(v0 + (int)threadIdx.x + b * kThreads, vecs - 1) * VEC) & ((1u << VEC) - 1);
+                        any |= some[b];
+                    }
+                    if (any != 0) {
+#pragma unroll
+                        for (int b = 0; b < B; ++b)
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i)
+                                if (some[b] >> i & 1) p[b].v[i] = Elem<T>::narrow(-inf);
+                    }
+                }
+                if (v0 + B * kThreads > vecs) {
+#pragma unroll
+                    for (int b = 0; b < B; ++b)
+                        if (v0 + (int)threadIdx.x + b * kThreads >= vecs)
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) p[b].v[i] = Elem<T>::narrow(-inf);
                 }
                 float f[B * VEC];
 #pragma unroll
                 for (int b = 0; b < B; ++b)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) f[b * VEC + i] = Elem<T>::widen(p[b].v[i]);
-                if constexpr (REST) {
-                    uint32_t named[B], any = 0;
-#pragma unroll
-                    for (int b = 0; b < B; ++b) {
-                        const int e = min(v + b * kThreads, vecs - 1) * VEC;
-                        named[b] = bits[e >> 5] >> (e & 31) & ((1u << VEC) - 1);
-                        any |= named[b];
-                    }
-                    if (__any(any != 0))
-#pragma unroll
-                        for (int b = 0; b < B; ++b)
-#pragma unroll
-                            for (int i = 0; i < VEC; ++i) f[b * VEC + i] = named[b] >> i & 1 ? -inf : f[b * VEC + i];
-                }
                 take(f);
             }
         }
@@ -228,82 +206,126 @@ __global__ __launch_bounds__(kThreads) void distill_stats_kernel(const DistillAr
             sums[threadIdx.x >> 6] = s;
         }
         __syncthreads();
-        m = most[0];
-        s = sums[0];
-        for (int w = 1; w < 4; ++w) meet(m, s, most[w], sums[w], steps);
-        // the teacher's entries
-        float teacher_most = -inf, named_most = -inf;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            teacher_most = fmaxf(teacher_most, t[i]);
-            if (REST && fresh[i]) named_most = fmaxf(named_most, xt[i]);
-            bad |= token[i] == a.cols;
-        }
-        teacher_most = block_reduce<MaxF>(teacher_most, most);
-        if constexpr (REST) named_most = block_reduce<MaxF>(named_most, most);
-        double ea = 0.0, eb = 0.0, named = 0.0;
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-            if (token[i] >= e0 && token[i] < e1) {
-                const double e = t[i] == -inf ? 0.0 : exp(((double)t[i] - (double)teacher_most) * inv);
-                ea += e;
-                if (e != 0.0) eb += e * (((double)t[i] - (double)xt[i]) * inv);
-                if (REST && fresh[i]) named += xt[i] == -inf ? 0.0 : exp(((double)xt[i] - (double)named_most) * inv);
-            }
-        if (bad && part == 0) ea = __builtin_nan("");
-        ea = block_reduce<SumD>(ea, sums2);
-        eb = block_reduce<SumD>(eb, sums);
-        if constexpr (REST) named = block_reduce<SumD>(named, sums2);
         if (threadIdx.x == 0) {
+            m = most[0];
+            s = sums[0];
+            for (int w = 1; w < 4; ++w) meet(m, s, most[w], sums[w], steps);
             double* p = a.partial + at * kDistillPart;
-            const RowSums r{m, s, named_most, named, teacher_most, ea, eb};
-            if (a.split == 1) {
-                p[0] = finish_row(a, row, r);
-            } else {
-                p[0] = r.most;
-                p[1] = r.sum;
-                p[2] = r.named_most;
-                p[3] = r.named;
-                p[4] = r.teacher_most;
-                p[5] = r.a;
-                p[6] = r.b;
-            }
+            p[0] = m;
+            p[1] = s;
+            p[2] = again ? 1.0 : 0.0;
         }
     }
 }
 
-// A split row from its parts, a lane each.
-__global__ __launch_bounds__(64) void distill_rows_kernel(const DistillArgs a) {
-    const int64_t row = blockIdx.x;
-    double* p = a.partial + row * a.split * kDistillPart;
-    if (mask_of(a.mask, a.mask_bool, row) == 0.0f) {
-        if (threadIdx.x == 0) {
-            skip_row(a, row);
-            p[0] = 0.0;
-        }
-        return;
-    }
+// A row's sums from its parts (at most 64, a lane each) and its entries, for a wavefront.
+template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillArgs& a, int64_t row) {
+    const int lane = threadIdx.x & 63;
     const double inf = __builtin_huge_val(), inv = 1.0 / a.temperature;
+    const T* x = (const T*)a.x + offset_of(a.kept, row);
     RowSums r{-inf, 0.0, -inf, 0.0, -inf, 0.0, 0.0};
-    if ((int)threadIdx.x < a.split) {
-        const double* q = p + threadIdx.x * kDistillPart;
-        r = {q[0], q[1], q[2], q[3], q[4], q[5], q[6]};
+    double twice = 0.0;
+    if (lane < a.split) {
+        const double* p = a.partial + (row * a.split + lane) * kDistillPart;
+        r.most = p[0];
+        r.sum = p[1];
+        twice = p[2];
     }
-    auto meet = [&](double& m, double& s) {
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-            const double m2 = shfl_xor_any(m, w), s2 = shfl_xor_any(s, w), n = fmax(m, m2);
-            const double f1 = m == n ? 1.0 : exp((m - n) * inv), f2 = m2 == n ? 1.0 : exp((m2 - n) * inv);
-            s = s * f1 + s2 * f2;
-            m = n;
-        }
+    // the entries: four of a lane at a time on their way together
+    struct Entry {
+        int token;
+        float t, x;
     };
-    meet(r.most, r.sum);
-    if (a.teacher_lse) meet(r.named_most, r.named);
+    auto entry = [&](int j) {
+        Entry e{-1, -(float)inf, 0.0f};
+        if (j < a.k) {
+            e.token = token_of(a.index, a.index64, row * a.k + j, a.cols);
+            if (e.token >= 0) e.t = logit_of(a.teacher, a.teacher_dtype, row * a.k + j);
+            if (e.token >= 0 && e.token < a.cols) e.x = Elem<T>::widen(x[e.token]);
+        }
+        return e;
+    };
+    float teacher_most = -(float)inf, named_most = -(float)inf;
+    bool bad = false;
+    const bool rest = a.teacher_lse != nullptr;
+    Entry few[4];
+    for (int j0 = 0; j0 < a.k; j0 += 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) few[i] = entry(j0 + i * 64 + lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            teacher_most = fmaxf(teacher_most, few[i].t);
+            if (few[i].token >= 0) named_most = fmaxf(named_most, few[i].x);
+            bad |= few[i].token == a.cols;
+        }
+    }
+    teacher_most = group_reduce<MaxF>(teacher_most, 64);
+    named_most = group_reduce<MaxF>(named_most, 64);
+    for (int j0 = 0; j0 < a.k; j0 += 256) {
+        if (a.k > 256)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) few[i] = entry(j0 + i * 64 + lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Entry& e = few[i];
+            if (e.token < 0 || e.token == a.cols) continue;
+            const double p = e.t == -(float)inf ? 0.0 : exp(((double)e.t - (double)teacher_most) * inv);
+            r.a += p;
+            if (p != 0.0) r.b += p * (((double)e.t - (double)e.x) * inv);
+        }
+        if (rest) {
+            // the student's, each token once: where one is named twice, an entry whose token one before it names is passed over
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const Entry& e = few[i];
+                bool first = e.token >= 0 && e.token < a.cols && e.x != -(float)inf;
+                if (__any(twice != 0.0)) {
+                    const int j = j0 + i * 64 + lane;
+                    for (int l = 0; l < j && first; ++l) first = token_of(a.index, a.index64, row * a.k + l, a.cols) != e.token;
+                }
+                if (first) r.named += exp(((double)e.x - (double)named_most) * inv);
+            }
+        }
+    }
+    if (__any(bad)) r.a = __builtin_nan("");
     r.a = group_reduce<SumD>(r.a, 64);
     r.b = group_reduce<SumD>(r.b, 64);
-    if (threadIdx.x == 0) p[0] = finish_row(a, row, r);
+    r.named = group_reduce<SumD>(r.named, 64);
+    r.teacher_most = teacher_most;
+    r.named_most = named_most;
+    // (lane 0 has them all)
+    if (a.split > 1) {
+        for (int w = 1; w < a.split; w <<= 1) {
+            const double m2 = shfl_xor_any(r.most, w), s2 = shfl_xor_any(r.sum, w), n = fmax(r.most, m2);
+            const double f1 = r.most == n ? 1.0 : exp((r.most - n) * inv), f2 = m2 == n ? 1.0 : exp((m2 - n) * inv);
+            r.sum = r.sum * f1 + s2 * f2;
+            r.most = n;
+        }
+    }
+    return r;
+}
+
+// Rows from their sums: a wavefront takes one, and those of a workgroup are finished together, a lane each (the logarithms and exponentials of 64 bits are some thousand
+// instructions, for one lane as for all).
+constexpr int kRowsAtOnce = 16;
+template <class T>
+__global__ __launch_bounds__(64 * kRowsAtOnce, 8) void distill_rows_kernel(const DistillArgs a) {
+    __shared__ RowSums sums[kRowsAtOnce];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row0 = (int64_t)blockIdx.x * kRowsAtOnce;
+    if (row0 + wave < a.rows && mask_of(a.mask, a.mask_bool, row0 + wave) != 0.0f) {
+        const RowSums r = sums_of_row<T>(a, row0 + wave);
+        if ((threadIdx.x & 63) == 0) sums[wave] = r;
+    }
+    __syncthreads();
+    const int64_t row = row0 + threadIdx.x;
+    if (threadIdx.x >= kRowsAtOnce || row >= a.rows) return;
+    if (mask_of(a.mask, a.mask_bool, row) == 0.0f) {
+        skip_row(a, row);
+        a.each[row] = 0.0;
+    } else {
+        a.each[row] = finish_row(a, row, sums[threadIdx.x]);
+    }
 }
 
 // The sums over the rows, in one workgroup and a fixed order, and each row's weight. Without a row that counts all are 0.
@@ -314,7 +336,7 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const DistillArgs a) 
     for (int64_t row = threadIdx.x; row < a.rows; row += 1024) {
         const float mask = mask_of(a.mask, a.mask_bool, row);
         if (mask != 0.0f) {
-            loss += a.partial[row * a.split * kDistillPart] * mask;
+            loss += a.each[row] * mask;
             count += mask;
         }
     }
@@ -327,13 +349,16 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const DistillArgs a) 
         a.terms[row * kTerms + 7] *= (float)(mask_of(a.mask, a.mask_bool, row) * inv * a.temperature);
 }
 
-// The logits' gradient, piece by piece. A row of weight 0 is not read and has zeros.
+// The logits' gradient, a piece for each wavefront, which waits for nobody. A row of weight 0 is not read and has zeros. Every lane has what its tokens' vectors get if no
+// entry names them; a named token (a bit tells) is left out there and written by the lane of the first entry that names it.
 template <class T>
 __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGradArgs a, int pieces, int each) {
-    constexpr int VEC = 16 / sizeof(T), N = 2;
-    __shared__ float probs[kThreads * N * VEC];  // the teacher's of the piece's tokens, -1 where no entry names one
-    __shared__ int again;
-    for (int64_t at = blockIdx.x; at < a.rows * pieces; at += gridDim.x) {
+    constexpr int VEC = 16 / sizeof(T), N = kGradVecs, WORDS = (64 * N * VEC + VEC + 31) / 32;
+    __shared__ uint32_t shared_bits[kThreads / 64][WORDS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t* bits = shared_bits[wave];
+    auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };  // (a wavefront's accesses to LDS are in order)
+    for (int64_t at = (int64_t)blockIdx.x * (kThreads / 64) + wave; at < a.rows * pieces; at += (int64_t)gridDim.x * (kThreads / 64)) {
         const int64_t row = quotient(at, pieces);
         const int e0 = (int)(at - row * pieces) * each, n = min(each, a.cols - e0);
         T* out = (T*)a.out + row * a.cols + e0;
@@ -341,6 +366,8 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
         const float* terms = a.terms + row * kTerms;
         const float weight = terms[7], w = weight == 0.0f ? 0.0f : weight * a.upstream;
         const bool on = weight != 0.0f;
+        auto token = [&](int j) { return token_of(a.index, a.index64, row * a.k + j, a.cols); };
+        int named = lane < a.k ? token(lane) : -1;
         // results leave as aligned vectors, logits come as they lie
         const int head = min(n, (int)((16 - ((uintptr_t)out & 15)) & 15) / (int)sizeof(T));
         const int vecs = (n - head) / VEC, tail = head + vecs * VEC;
@@ -351,63 +378,83 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
         __builtin_memset(&last, 0, sizeof last);
         if (on) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int v = threadIdx.x + i * kThreads;
-                if (v < vecs) p[i] = load_pack_unaligned<T, VEC>(x + head + v * VEC);
-            }
-            if ((int)threadIdx.x < head) first = x[threadIdx.x];
-            if ((int)threadIdx.x < n - tail) last = x[tail + threadIdx.x];
+            for (int i = 0; i < N; ++i)
+                if (lane + i * 64 < vecs) p[i] = load_pack_unaligned<T, VEC>(x + head + (lane + i * 64) * VEC);
+            if (lane < head) first = x[lane];
+            if (lane < n - tail) last = x[tail + lane];
         }
-        const float base_hi = terms[0], base_lo = terms[1], rest_hi = terms[2], rest_lo = terms[3], coef = terms[6];
-        const double teacher = (double)terms[4] + (double)terms[5];
-        auto prob = [&](int j) { return (float)exp2((double)logit_of(a.teacher, a.teacher_dtype, row * a.k + j) * (kLog2eD / a.temperature) - teacher); };
+        const float rest_hi = terms[2], rest_lo = terms[3], coef = w * terms[6];
+        // a token's bit stands so that those of a vector stand together
+        const int shift = VEC - head;
         if (on) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n; i += kThreads) probs[i] = -1.0f;
-            if (threadIdx.x == 0) again = 0;
-            __syncthreads();
-            for (int j = threadIdx.x; j < a.k; j += kThreads) {
-                const int e = token_of(a.index, a.index64, row * a.k + j, a.cols) - e0;
-                if (e >= 0 && e < n && e + e0 < a.cols) {
-                    const uint32_t old = atomicExch((uint32_t*)&probs[e], __float_as_uint(prob(j)));
-                    if (old != __float_as_uint(-1.0f)) again = 1;
+            for (int i = lane; i < WORDS; i += 64) bits[i] = 0;
+            fence();
+            uint32_t mine = 0;  // entries of this lane that name a token of the piece
+            bool twice = false;
+            for (int i = 0; i * 64 < a.k; ++i) {
+                if (i) named = i * 64 + lane < a.k ? token(i * 64 + lane) : -1;
+                const int e = named - e0;
+                if (e >= 0 && e < n) {
+                    const int b = e + shift;
+                    twice |= atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1;
+                    mine |= 1u << i;
                 }
             }
-            __syncthreads();
-            if (again) {  // an index twice: the sum, in the entries' order
-                for (int i = threadIdx.x; i < n; i += kThreads) probs[i] = -1.0f;
-                __syncthreads();
-                if (threadIdx.x == 0)
-                    for (int j = 0; j < a.k; ++j) {
-                        const int e = token_of(a.index, a.index64, row * a.k + j, a.cols) - e0;
-                        if (e >= 0 && e < n && e + e0 < a.cols) probs[e] = (probs[e] == -1.0f ? 0.0f : probs[e]) + prob(j);
-                    }
-                __syncthreads();
+            static_assert(kMostEntries <= 64 * 32, "a bit for each entry of a lane");
+            twice = __any(twice);
+            fence();
+            while (mine) {
+                const int j = __builtin_ctz(mine) * 64 + lane, e = token(j);
+                mine &= mine - 1;
+                const double teacher = (double)terms[4] + (double)terms[5], per = kLog2eD / a.temperature;
+                // (the exponent in 64 bits, its fraction's power by the hardware: the library's 64-bit routine costs a wavefront a SIMD in registers)
+                auto prob = [&](int j) {
+                    const double d = (double)logit_of(a.teacher, a.teacher_dtype, row * a.k + j) * per - teacher, whole = rint(d);
+                    return d < -160.0 ? 0.0f : ldexpf(__builtin_amdgcn_exp2f((float)(d - whole)), (int)fmin(whole, 1000.0));
+                };
+                const float f = Elem<T>::widen(x[e - e0]);
+                float q = prob(j);
+                bool is_first = true;
+                if (twice) {  // an index twice: the first adds up the others
+                    for (int l = 0; l < j && is_first; ++l) is_first = token(l) != e;
+                    for (int l = j + 1; l < a.k && is_first; ++l)
+                        if (token(l) == e) q += prob(l);
+                }
+                const float y = __builtin_amdgcn_exp2f(fmaf(f, a.steps.hi, -terms[0]) + fmaf(f, a.steps.lo, -terms[1]));
+                if (is_first) out[e - e0] = Elem<T>::narrow(w * (y - q));
             }
         }
-        auto grad = [&](T v, int e) {
-            if (!on) return Elem<T>::narrow(0.0f);
-            const float q = probs[e], f = Elem<T>::widen(v);
-            const bool named = !(q == -1.0f);
-            const float y = __builtin_amdgcn_exp2f(fmaf(f, a.steps.hi, named ? -base_hi : -rest_hi) + fmaf(f, a.steps.lo, named ? -base_lo : -rest_lo));
-            return Elem<T>::narrow(w * (named ? y - q : coef * y));
+        auto grad = [&](T v) {
+            const float f = Elem<T>::widen(v);
+            return Elem<T>::narrow(coef * __builtin_amdgcn_exp2f(fmaf(f, a.steps.hi, -rest_hi) + fmaf(f, a.steps.lo, -rest_lo)));
         };
-        if ((int)threadIdx.x < head) out[threadIdx.x] = grad(first, threadIdx.x);
-        if ((int)threadIdx.x < n - tail) out[tail + threadIdx.x] = grad(last, tail + threadIdx.x);
+        auto is_named = [&](int e) { return on && bits[(e + shift) >> 5] >> ((e + shift) & 31) & 1; };
+        if (lane < head && !is_named(lane)) out[lane] = on ? grad(first) : first;
+        if (lane < n - tail && !is_named(tail + lane)) out[tail + lane] = on ? grad(last) : last;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int v = threadIdx.x + i * kThreads;
+            const int v = lane + i * 64;
             if (v >= vecs) continue;
             const int e = head + v * VEC;
+            uint32_t some = 0;
+            if (on) {
 #pragma unroll
-            for (int l = 0; l < VEC; ++l) p[i].v[l] = grad(p[i].v[l], e + l);
-            store_pack_stream<T, VEC>(out + e, p[i]);
+                for (int l = 0; l < VEC; ++l) p[i].v[l] = grad(p[i].v[l]);
+                some = bits[(e + shift) >> 5] >> ((e + shift) & 31) & ((1u << VEC) - 1);
+            }
+            if (some == 0) store_pack_stream<T, VEC>(out + e, p[i]);
+            else
+#pragma unroll
+                for (int l = 0; l < VEC; ++l)
+                    if (!(some >> l & 1)) out[e + l] = p[i].v[l];
         }
+        fence();
     }
 }
 
 }  // namespace
 
+// (us of loss alone, bf16 [8192, 50257] with the rest, rows whole, in two, four and eight parts: 186, 213, 245, 313)
 int distill_split(int dtype, int64_t rows, int64_t cols) {
     if (rows == 0 || rows > 2047) return 1;
     const int64_t bytes = cols * (int64_t)dtype_size(dtype);
@@ -415,24 +462,24 @@ int distill_split(int dtype, int64_t rows, int64_t cols) {
 }
 
 void launch_distill_loss(int dtype, const DistillArgs& a, hipStream_t st) {
-    if (a.rows > 0) {
+    if (a.rows > 0)
         HPT_WITH_TYPE(dtype, {
             const unsigned blocks = (unsigned)std::min<int64_t>(a.rows * a.split, 1 << 20);
             if (a.teacher_lse) distill_stats_kernel<T, true><<<blocks, kThreads, 0, st>>>(a);
             else distill_stats_kernel<T, false><<<blocks, kThreads, 0, st>>>(a);
+            distill_rows_kernel<T><<<(unsigned)((a.rows + kRowsAtOnce - 1) / kRowsAtOnce), 64 * kRowsAtOnce, 0, st>>>(a);
         });
-        if (a.split > 1) distill_rows_kernel<<<(unsigned)a.rows, 64, 0, st>>>(a);
-    }
     distill_sum_kernel<<<1, 1024, 0, st>>>(a);
 }
 
 void launch_distill_loss_backward(int dtype, const DistillGradArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
         constexpr int VEC = 16 / sizeof(T);
-        const int most = kThreads * 2 * VEC;
+        const int most = 64 * kGradVecs * VEC;
         const int pieces = (a.cols + most - 1) / most;
         const int each = ((a.cols + pieces - 1) / pieces + VEC - 1) / VEC * VEC;
-        distill_grad_kernel<T><<<(unsigned)std::min<int64_t>(a.rows * pieces, 1 << 20), kThreads, 0, st>>>(a, pieces, each);
+        const int64_t blocks = (a.rows * pieces + kThreads / 64 - 1) / (kThreads / 64);
+        distill_grad_kernel<T><<<(unsigned)std::min<int64_t>(blocks, 1 << 20), kThreads, 0, st>>>(a, pieces, each);
     });
 }
 
