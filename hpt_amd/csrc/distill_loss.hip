@@ -56,28 +56,34 @@ struct RowSums {
 // A row's divergence, and what its gradient needs: log2 of the sums that probabilities are over, in two pieces each (f32 alone would cost a gradient |lse| / 2^24 of itself).
 __device__ __forceinline__ double finish_row(const DistillArgs& a, int64_t row, const RowSums& s) {
     const double inv = 1.0 / a.temperature, inf = __builtin_huge_val();
-    auto scaled = [&](double x, double most) { return x == most ? 1.0 : exp((x - most) * inv); };
-    double lse, rest = 0.0, kl, mass = 1.0, coef = 1.0, teacher;
+    double lse, rest, kl, base, coef = 1.0, teacher;
     bool counts = true;
     if (!a.teacher_lse) {
         lse = rest = s.most * inv + log(s.sum);
+        base = lse * kLog2eD;
         teacher = s.teacher_most * inv + log(s.a);
         kl = s.b / s.a - teacher + lse;
         counts = s.a != 0.0;
         if (!counts) kl = 0.0;
     } else {
-        const double top = fmax(s.most, s.named_most);
-        lse = top * inv + log(s.sum * scaled(s.most, top) + s.named * scaled(s.named_most, top));
+        // (one exponential for both sums' distance; equal infinities are no distance apart)
+        const bool below = s.most < s.named_most;
+        const double far = s.most == s.named_most ? 1.0 : exp(-fabs(s.most - s.named_most) * inv);
+        const double left = s.sum * (below ? far : 1.0), all = left + s.named * (below ? 1.0 : far);
+        lse = fmax(s.most, s.named_most) * inv + log(all);
         teacher = a.teacher_lse[row];
         const double part = s.a == 0.0 ? 0.0 : exp(s.teacher_most * inv - teacher), q = s.a * part;
         const bool others = s.sum != 0.0;
-        double r = 1.0 - q;
-        r = !others || r < 0.0 ? 0.0 : r;
+        double r = 1.0 - q, mass = 1.0;
+        if (!others || r < 0.0) {
+            r = 0.0;
+            mass = q;
+        }
         rest = others ? s.most * inv + log(s.sum) : lse;
-        kl = (part == 0.0 ? 0.0 : part * s.b) + q * (lse - teacher) + (r == 0.0 ? 0.0 : r * (log(r) - (rest - lse)));
-        if (q == 0.0) kl = r == 0.0 ? 0.0 : r * (log(r) - (rest - lse));
-        mass = q + r;
-        coef = others ? mass * exp(rest - lse) - r : 0.0;
+        kl = r == 0.0 ? 0.0 : r * (log(r) - (rest - lse));
+        if (q != 0.0) kl += part * s.b + q * (lse - teacher);
+        base = lse * kLog2eD - (mass == 1.0 ? 0.0 : log2(mass));
+        coef = others ? mass * (left / all) - r : 0.0;
     }
     a.kl[row] = (float)kl;
     float* t = a.terms + row * kTerms;
@@ -86,7 +92,7 @@ __device__ __forceinline__ double finish_row(const DistillArgs& a, int64_t row, 
         to[0] = hi;
         to[1] = fabsf(hi) < (float)inf ? (float)(v - (double)hi) : 0.0f;
     };
-    pieces(t, lse * kLog2eD - log2(mass));
+    pieces(t, base);
     pieces(t + 2, rest * kLog2eD);
     pieces(t + 4, teacher * kLog2eD);
     t[6] = (float)coef;
@@ -224,6 +230,7 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
     const double inf = __builtin_huge_val(), inv = 1.0 / a.temperature;
     const T* x = (const T*)a.x + offset_of(a.kept, row);
     RowSums r{-inf, 0.0, -inf, 0.0, -inf, 0.0, 0.0};
+    const float steps = a.steps.hi + a.steps.lo;
     double twice = 0.0;
     if (lane < a.split) {
         const double* p = a.partial + (row * a.split + lane) * kDistillPart;
@@ -297,8 +304,9 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
     if (a.split > 1) {
         for (int w = 1; w < a.split; w <<= 1) {
             const double m2 = shfl_xor_any(r.most, w), s2 = shfl_xor_any(r.sum, w), n = fmax(r.most, m2);
-            const double f1 = r.most == n ? 1.0 : exp((r.most - n) * inv), f2 = m2 == n ? 1.0 : exp((m2 - n) * inv);
-            r.sum = r.sum * f1 + s2 * f2;
+            // (the hardware's exponential: one of -D is off by D / 2^24 of itself or so, which is D e^-D / 2^24 of the row's sum at most, less than a rounding)
+            const float f1 = r.most == n ? 1.0f : __builtin_amdgcn_exp2f((float)(r.most - n) * steps), f2 = m2 == n ? 1.0f : __builtin_amdgcn_exp2f((float)(m2 - n) * steps);
+            r.sum = r.sum * (double)f1 + s2 * (double)f2;
             r.most = n;
         }
     }
