@@ -865,9 +865,9 @@ static RowsOf sampled_rows_of(const hpt_view* logits) {
     if (r.cols > kMostSampled) fail(HPT_ERR_SHAPE, "sample logits: a vocabulary of %lld tokens, at most %lld expected", (long long)r.cols, (long long)kMostSampled);
     return r;
 }
-static size_t sample_bytes(const RowsOf& r) {
+static size_t sample_bytes(const hpt_view* logits, const RowsOf& r) {
     if (r.rows == 0) return 0;
-    const size_t row = sample_row_bytes(r.cols);
+    const size_t row = sample_row_bytes(logits->dtype, r.cols);
     return (size_t)rows_of_run(r.rows, row) * row;
 }
 // A setting for all rows or for each.
@@ -1726,7 +1726,7 @@ int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, d
         a.rows = r.rows;
         a.cols = (int)r.cols;
         a.k = (int)k;
-        a.tiles = (int)((r.cols + kTile - 1) / kTile);
+        a.tiles = (int)tiles_of(in->dtype, r.cols, rows_shifted(in->dtype, in->data, r.kept));
         const size_t row = topk_row_bytes(in->dtype, r.cols, lse != nullptr);
         a.run = rows_of_run(r.rows, row);
         use_device(dev);
@@ -1743,7 +1743,7 @@ int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, d
 int32_t hpt_hip_sample_workspace(const hpt_view* logits, size_t* bytes) {
     return guarded([&] {
         if (!bytes) fail(HPT_ERR_PARAM, "sample_workspace: null output");
-        *bytes = sample_bytes(sampled_rows_of(logits));
+        *bytes = sample_bytes(logits, sampled_rows_of(logits));
     });
 }
 
@@ -1785,8 +1785,8 @@ int32_t hpt_hip_sample(int32_t dev, void* stream, const hpt_view* logits, const 
         a.logp = (float*)logp->data;
         a.rows = r.rows;
         a.cols = (int)r.cols;
-        a.tiles = (int)((r.cols + kTile - 1) / kTile);
-        const size_t row = sample_row_bytes(r.cols);
+        a.tiles = (int)tiles_of(logits->dtype, r.cols, rows_shifted(logits->dtype, logits->data, r.kept));
+        const size_t row = sample_row_bytes(logits->dtype, r.cols);
         a.run = rows_of_run(r.rows, row);
         use_device(dev);
         hipStream_t st = (hipStream_t)stream;

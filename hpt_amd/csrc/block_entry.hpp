@@ -189,10 +189,11 @@ void launch_policy_loss_backward(int dtype, const PolicyGradArgs& a, hipStream_t
 // ---- the largest logits, and sampling ---------------------------------------------------------------
 
 constexpr int kTile = 8192;             // neighbouring logits that a workgroup of 256 threads takes at once, 32 a thread
-constexpr int kTileGroups = 256;        // one for each thread
+constexpr int kTileGroups = 256;        // of 32 logits, one for each thread
+constexpr int kTileWaves = kTileGroups / 64;
 constexpr int kMostTop = 1024;          // logits that topk returns at most, and that a sampled row picks from in one piece
 constexpr int64_t kMostSampled = (int64_t)1 << 22;  // tokens of a vocabulary to sample from: kMostParts tiles
-constexpr int kMostParts = (int)(kMostSampled / kTile);
+constexpr int kMostParts = (int)(kMostSampled / kTile) + 1;
 constexpr size_t kMostRowScratch = (size_t)64 << 20;  // rows are taken in runs whose scratch stays below this
 
 // log2 e / temperature in two pieces: twelve bits, and what is left, large against the first product's roundings (a piece of the float's own last place would be rounded
@@ -211,15 +212,17 @@ struct TopkArgs {
     float* lse;           // or null
     double inv_temperature;  // (of lse alone)
     Steps steps;
-    void* keys;           // [rows of a run, tiles, 256] scratch: each thread's largest, as an order key of the logits' size
-    double* sums;         // [rows of a run, tiles, 2] scratch: a tile's largest and its sum of exponentials below it
+    void* keys;           // [rows of a run, tiles, 256] scratch: each group's largest, as an order key of the logits' size
+    double* sums;         // [rows of a run, tiles, 4, 2] scratch: a wavefront's largest and its sum of exponentials below it
     int64_t rows;
     int cols, k;
     int tiles;
     int64_t run;          // rows of a run
 };
 
-// Scratch for each row, and rows of a run.
+// Tiles of a row, taken as the aligned vectors that contain it (`shifted`: rows may start off a vector); scratch for each row wherever it starts, and rows of a run.
+int64_t tiles_of(int dtype, int64_t cols, bool shifted);
+bool rows_shifted(int dtype, const void* x, const Dims& kept);
 size_t topk_row_bytes(int dtype, int64_t cols, bool lse);
 int64_t rows_of_run(int64_t rows, size_t row_bytes);
 void launch_topk(int dtype, const TopkArgs& a, hipStream_t st);
@@ -246,7 +249,7 @@ struct SampleArgs {
     int tiles;
     int64_t run;
 };
-size_t sample_row_bytes(int64_t cols);
+size_t sample_row_bytes(int dtype, int64_t cols);
 void launch_sample(int dtype, const SampleArgs& a, hipStream_t st);
 
 // ---- distillation -----------------------------------------------------------------------------------

@@ -5,13 +5,13 @@
 // a place of the order (key and index), and the token is the first, by index, at which the kept weights' sum is above u of their whole.
 //
 // Which token that is hangs on sums over the row: an error of 1e-7 of the sum, f32's, moves one of 10^5 borders across u in a row out of fifty. Weights and sums have 52
-// bits here: with t = x log2 e 32 / temperature, w is 2^(floor(t) / 32) from a table of 32 times a polynomial in t - floor(t) (degree 5, 2e-15). f64 multiply-adds run
-// at the rate of f32 ones, so the first launch still reads at some TB/s.
+// bits here: with t = x log2 e 64 / temperature and n the whole number next to it, w is 2^(n / 64), from a table of 64, times a polynomial in t - n (degree 4, 4e-14). f64
+// multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s.
 //
-// Two launches. The first takes tiles of 8192 logits and leaves, by what the row's filters need: its threads' largest keys (top_k of at most 1024: only the first places
+// Two launches. The first takes tiles of 8192 logits and leaves, by what the row's filters need: the largest keys of its groups (top_k of at most 1024: only the first places
 // matter); the sum of the weights (no filter); or the weights' sums by size, in buckets of an eighth of a power of two, as integers, whose sum has no order (with their
 // numbers where top_k is larger). The second has a workgroup for each row: it finds the bucket in which a border lies, collects that bucket's logits, narrows the border to one
-// place, and then looks through the one tile in which u's token lies.
+// place, and then looks through the one tile in which u's token lies. (Rows of which at most 128 places matter take a wavefront each.)
 #include <algorithm>
 
 #include "top_rows.hpp"
@@ -20,14 +20,15 @@ namespace hpt {
 
 namespace {
 
-constexpr int kBuckets = 256, kCopies = 4;
-constexpr int kFar = 32 * 128;             // weights below 2^-128 of the largest are 0
+constexpr int kSteps = 64;                   // of a power of two
+constexpr int kBuckets = 256, kCopies = 4;   // of eight steps
+constexpr int kFar = kSteps * 128;           // weights below 2^-128 of the largest are 0
+constexpr int kMostList = 2048;
 
 struct SampleHead {
-    double top;     // 31 + 32 floor(t / 32) of the tile's largest: the octave that its weights are counted from
-    double sum;     // of its weights, in that octave's units
+    double sum;     // of the tile's weights, in units of the octave of its largest
     uint32_t most;  // the largest key
-    uint32_t unused[3];
+    uint32_t unused;
 };
 struct SampleBody {
     union {
@@ -41,7 +42,7 @@ struct SampleBody {
 
 // ---- a row's settings -----------------------------------------------------------------------------
 
-enum { BAD, FEW, PLAIN, SORTED };
+enum Mode { BAD, FEW, PLAIN, SORTED, ANY };
 __device__ __forceinline__ double number_of(const Setting& s, int64_t row) {
     if (!s.each) return s.all;
     if (s.dtype == HPT_F32) return ((const float*)s.each)[row];
@@ -49,83 +50,91 @@ __device__ __forceinline__ double number_of(const Setting& s, int64_t row) {
 }
 struct Settings {
     int mode, k;
-    double steps, p, least;  // steps: of 1/32 octave for each unit of a logit
-    __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row) {
-        double t = number_of(a.temperature, row);
-        const double kk = number_of(a.top_k, row);
-        p = number_of(a.top_p, row);
-        least = number_of(a.min_p, row);
-        k = kk >= 1.0 && kk < (double)a.cols ? (int)kk : a.cols;
+    double steps, p, least;  // steps: of each unit of a logit
+    // (the host, too: settings for all rows have kernels of their own)
+    __host__ __device__ __forceinline__ Settings(double t, double kk, double p, double least, int cols) : p(p), least(least) {
+        k = kk >= 1.0 && kk < (double)cols ? (int)kk : cols;
         const bool bad = !(t == 0.0 || (t >= 1e-30 && t <= 1e30)) || p != p || least != least;
         if (t == 0.0) {  // the first of the order
             t = 1.0;
             k = 1;
         }
         if (p <= 0.0) k = 1;
-        steps = 32.0 * 1.4426950408889634 / t;
-        const bool few = k <= kMostTop && k < a.cols;
-        mode = bad ? BAD : few || a.cols == 1 ? FEW : p >= 1.0 && least <= 0.0 && k == a.cols ? PLAIN : SORTED;
+        steps = kSteps * 1.4426950408889634 / t;
+        const bool few = k <= kMostTop && k < cols;
+        mode = bad ? BAD : few || cols == 1 ? FEW : p >= 1.0 && least <= 0.0 && k == cols ? PLAIN : SORTED;
     }
+    __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row)
+        : Settings(number_of(a.temperature, row), number_of(a.top_k, row), number_of(a.top_p, row), number_of(a.min_p, row), a.cols) {}
 };
 
 // ---- weights --------------------------------------------------------------------------------------
 
-// 2^(f / 32) for f in [0, 1): Taylor's polynomial at 1/2, written in powers of f.
-struct Poly {
-    double c[6];
+// 2^(f / 64) for |f| <= 1/2, and 2^(j / 64).
+struct Powers {
+    double c[5], table[kSteps];
 };
-constexpr Poly make_poly() {
-    const double l = 0.6931471805599453 / 32.0;
-    double a[6] = {};
-    // e^(l / 2)
-    double middle = 0.0, term = 1.0;
-    for (int i = 0; i < 20; ++i) {
-        middle += term;
-        term *= (l / 2) / (i + 1);
-    }
-    a[0] = middle;
-    for (int i = 1; i < 6; ++i) a[i] = a[i - 1] * l / i;
-    Poly p{};
-    for (int i = 0; i < 6; ++i) {
-        double binomial = 1.0;
-        for (int k = i; k >= 0; --k) {  // C(i, k) (-1/2)^(i - k)
-            p.c[k] += a[i] * binomial;
-            binomial = binomial * k / (i - k + 1) * -0.5;
+constexpr Powers make_powers() {
+    const double l = 0.6931471805599453 / kSteps;
+    Powers p{};
+    p.c[0] = 1.0;
+    for (int i = 1; i < 5; ++i) p.c[i] = p.c[i - 1] * l / i;
+    for (int j = 0; j < kSteps; ++j) {
+        double sum = 0.0, term = 1.0;
+        for (int i = 1; i < 30; ++i) {
+            sum += term;
+            term *= l * j / i;
         }
+        p.table[j] = sum;
     }
     return p;
 }
-constexpr Poly kPoly = make_poly();
+__device__ constexpr Powers kPowers = make_powers();
 
+// Whole numbers next to t, in the low bits of a sum (|t| < 2^51).
+constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
 struct Weights {
-    const double* table;  // 2^(j / 32) in LDS
-    double steps, top;
-    // How many steps below the top octave's end a logit lies (1000000: far, or -inf), and its weight's mantissa, in [1, 2).
-    __device__ __forceinline__ int below(float x, double& f) const {
-        const double t = (double)x * steps, n = floor(t);
-        f = t - n;
-        return (int)fmax(fmin(top - n, 1e6), 0.0);
+    const double* table;  // 2^(j / 64) in LDS
+    double steps;
+    int top;  // the low bits of the whole number that the largest's octave ends with: a multiple of 64, and 63
+    // `most`: the largest logit, a number. Where t would leave the whole numbers' range the steps are shortened: there, logits that differ do so by octaves beyond counting.
+    __device__ __forceinline__ Weights(const double* table, float most, double steps) : table(table), steps(steps) {
+        if (fabs((double)most * steps) > 0x1p49) this->steps = 0x1p49 / fabs((double)most);
+        top = whole(most) | (kSteps - 1);
     }
-    __device__ __forceinline__ int below(float x) const {
-        double f;
-        return below(x, f);
+    __device__ __forceinline__ int whole(float x) const { return (int)(uint32_t)__builtin_bit_cast(uint64_t, fma((double)x, steps, kRound)); }
+    // How many steps below the top octave's end a logit lies that is not below `lowest`; f: what the whole number leaves.
+    __device__ __forceinline__ int below(double x, double& f) const {
+        const double sum = fma(x, steps, kRound);
+        f = fma(x, steps, kRound - sum);  // (exact but for one rounding, whatever t's size)
+        return top - (int)(uint32_t)__builtin_bit_cast(uint64_t, sum);
     }
+    // in [1, 2), or next to it
     __device__ __forceinline__ double mantissa(int r, double f) const {
-        double v = kPoly.c[5];
+        double v = kPowers.c[4];
 #pragma unroll
-        for (int i = 4; i >= 0; --i) v = fma(v, f, kPoly.c[i]);
-        return v * table[31 - (r & 31)];
+        for (int i = 3; i >= 0; --i) v = fma(v, f, kPowers.c[i]);
+        return v * table[(kSteps - 1) - (r & (kSteps - 1))];
     }
-    // In units of the top octave: in [1, 2) within it.
-    __device__ __forceinline__ double of(float x) const {
+    // The lowest logit that `below` may be asked for: 96 octaves down weigh nothing. (64 bits tell it from the largest, whose t is below 2^50.)
+    __device__ __forceinline__ double lowest(float most) const { return (double)most - 96.0 * kSteps / steps; }
+
+    // Of any logit: steps below (kFar: at least so many), and its weight in units of the top octave.
+    __device__ __forceinline__ int below_any(float x, float most, double& f) const {
+        const bool far = ((double)most - (double)x) * steps >= 100.0 * kSteps;
+        const int r = below(far ? most : x, f);
+        return far ? kFar : r;
+    }
+    __device__ __forceinline__ double of(float x, float most) const {
         double f;
-        const int r = below(x, f);
-        return r < kFar ? ldexp(mantissa(r, f), -(r >> 5)) : 0.0;
+        const int r = below_any(x, most, f);
+        return r < kFar ? shifted(mantissa(r, f), r / kSteps) : 0.0;
     }
+    // v 2^-n of a number v that is not small, by its exponent
+    static __device__ __forceinline__ double shifted(double v, int n) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v) - ((uint64_t)(uint32_t)(n << 20) << 32)); }
 };
-__device__ __forceinline__ double top_of(float most, double steps) { return 32.0 * floor((double)most * steps * (1.0 / 32.0)) + 31.0; }
 __device__ __forceinline__ void make_table(double* table) {
-    if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
+    if (threadIdx.x < kSteps) table[threadIdx.x] = kPowers.table[threadIdx.x];
 }
 // Mantissas as integers, for sums without an order: of 2^-44 (in a larger vocabulary 2^-40), so that a row's are below 2^63. The same everywhere: equal weights
 // reach a half of their sum at the half of their number.
@@ -135,91 +144,91 @@ struct Fixed {
     // 0 <= v < 2, rounded, from where it lies in the sum's mantissa
     __device__ __forceinline__ uint64_t operator()(double v) const { return __builtin_bit_cast(uint64_t, v + base) - __builtin_bit_cast(uint64_t, base); }
 };
-__device__ __forceinline__ double pow2(int n) { return ldexp(1.0, n); }
-__device__ __forceinline__ bool no_number(uint32_t key, uint32_t inf, uint32_t neg) { return key >= inf || key <= neg; }
+__device__ __forceinline__ double pow2(int n) { return __builtin_bit_cast(double, (uint64_t)(1023 + n) << 52); }  // |n| < 1000
+template <class T> __device__ __forceinline__ bool no_number(uint32_t key) { return key >= kInfKey<T> || key <= kNegInfKey<T>; }
 
 // ---- first launch ---------------------------------------------------------------------------------
 
-template <class T>
+template <class T, int MODE>
 __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleArgs a, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
+    constexpr bool BUCKETS = MODE == SORTED || MODE == ANY;
     __shared__ uint32_t tops[4];
-    __shared__ double sums[4], table[32];
-    __shared__ uint64_t mass[kBuckets * kCopies];
-    __shared__ uint32_t count[kBuckets * kCopies];
+    __shared__ double sums[4], table[kSteps];
+    __shared__ uint64_t mass[BUCKETS ? kBuckets * kCopies : 1];
+    __shared__ uint32_t count[BUCKETS ? kBuckets * kCopies : 1];
+    if (MODE != FEW) make_table(table);  // (a barrier of the largest's search comes before its use)
     const Fixed fixed(a.cols);
-    make_table(table);
-    __syncthreads();
     for (int64_t at = blockIdx.x; at < rows * a.tiles; at += gridDim.x) {
         const int64_t row = quotient(at, a.tiles);
         const int tile = (int)(at - row * a.tiles);
         Pack<T, VEC> p[V];
-        load_tile<T>((const T*)a.x + offset_of(a.kept, row0 + row), tile, a.cols, p);
+        load_tile<T>(LogitRow<T>((const T*)a.x + offset_of(a.kept, row0 + row), a.cols), tile, p);
         const Settings set(a, row0 + row);
-        if (set.mode == BAD) continue;
+        const int mode = MODE == ANY ? set.mode : MODE;
+        if (mode == BAD) continue;
         SampleBody& body = ((SampleBody*)a.bodies)[at];
-        const uint32_t key = most_key<T>(p);
-        if (set.mode == FEW) {
-            ((KeyOf<T>*)body.keys)[threadIdx.x] = (KeyOf<T>)key;
+        uint32_t key = 0;
+        if (mode == FEW) {
+            ((KeyOf<T>*)body.keys)[threadIdx.x] = (KeyOf<T>)group_key<T>(p);
             continue;
         }
         SampleHead& head = ((SampleHead*)a.heads)[at];
-        const uint32_t most = block_reduce<MaxU>(key, tops);
-        if (no_number(most, kInfKey<T>, kNegInfKey<T>)) {
-            if (threadIdx.x == 0) {
-                head.top = -__builtin_huge_val();
-                head.sum = 0.0;
-                head.most = most;
-            }
-            continue;
-        }
-        const Weights w{table, set.steps, top_of(value_of<T>(most), set.steps)};
+#pragma unroll
+        for (int b = 0; b < V; ++b) key = max(key, most_key<T>(p[b]));
+        key = block_reduce<MaxU>(key, tops);
         double sum = 0.0;
-        if (set.mode == PLAIN) {
+        if (!no_number<T>(key)) {
+            const float most = value_of<T>(key);
+            const Weights w(table, most, set.steps);
+            const double lowest = w.lowest(most);
+            if (!BUCKETS || mode == PLAIN) {
 #pragma unroll
-            for (int b = 0; b < V; ++b)
+                for (int b = 0; b < V; ++b)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) sum += w.of(Elem<T>::widen(p[b].v[i]));
-        } else {
-            const bool counted = set.k < a.cols;
-            for (int i = threadIdx.x; i < kBuckets * kCopies; i += kTileGroups) {
-                mass[i] = 0;
-                count[i] = 0;
-            }
-            __syncthreads();
-            const int copy = threadIdx.x & (kCopies - 1);
+                    for (int i = 0; i < VEC; ++i) {
+                        double f;
+                        const int r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), f);
+                        sum += Weights::shifted(w.mantissa(r, f), r / kSteps);
+                    }
+            } else {
+                const bool counted = set.k < a.cols;
+                for (int i = threadIdx.x; i < kBuckets * kCopies; i += kTileGroups) {
+                    mass[i] = 0;
+                    count[i] = 0;
+                }
+                __syncthreads();
+                const int copy = threadIdx.x & (kCopies - 1);
 #pragma unroll
-            for (int b = 0; b < V; ++b)
+                for (int b = 0; b < V; ++b)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    double f;
-                    const int r = w.below(Elem<T>::widen(p[b].v[i]), f);
-                    const int bucket = min(r >> 2, kBuckets - 1);
-                    // (the last bucket holds all that is below: in units of its own octave)
-                    if (r < kFar) {
-                        const double v = ldexp(w.mantissa(r, f), -max((r >> 5) - (kBuckets / 8 - 1), 0));
+                    for (int i = 0; i < VEC; ++i) {
+                        double f;
+                        const int r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), f);
+                        const int bucket = min(r >> 3, kBuckets - 1);
+                        // (the last bucket holds all that is below: in units of its own octave)
+                        const double v = Weights::shifted(w.mantissa(r, f), max(r / kSteps - (kBuckets / 8 - 1), 0));
                         __hip_atomic_fetch_add(&mass[bucket * kCopies + copy], fixed(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                         if (counted) __hip_atomic_fetch_add(&count[bucket * kCopies + copy], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
-                }
-            __syncthreads();
-            static_assert(kBuckets == kTileGroups, "a bucket a thread");
-            uint64_t m = 0;
-            uint32_t c = 0;
+                __syncthreads();
+                static_assert(kBuckets == kTileGroups, "a bucket a thread");
+                uint64_t m = 0;
+                uint32_t c = 0;
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) {
-                m += mass[threadIdx.x * kCopies + i];
-                c += count[threadIdx.x * kCopies + i];
+                for (int i = 0; i < kCopies; ++i) {
+                    m += mass[threadIdx.x * kCopies + i];
+                    c += count[threadIdx.x * kCopies + i];
+                }
+                body.mass[threadIdx.x] = m;
+                if (counted) body.count[threadIdx.x] = c;
+                sum = (double)m * fixed.unit * pow2(-(int)(threadIdx.x >> 3));
             }
-            body.mass[threadIdx.x] = m;
-            if (counted) body.count[threadIdx.x] = c;
-            sum = (double)m * fixed.unit * pow2(-(int)(threadIdx.x >> 3));
+            sum = block_reduce<SumD>(sum, sums);
         }
-        sum = block_reduce<SumD>(sum, sums);
         if (threadIdx.x == 0) {
-            head.top = w.top;
             head.sum = sum;
-            head.most = most;
+            head.most = key;
         }
     }
 }
@@ -230,54 +239,66 @@ struct SortedShared {
     uint64_t list[kMostList];
     uint64_t mass[kBuckets];  // of a digit
     uint32_t count[kBuckets];
-    double row_mass[kBuckets];  // of a bucket of the row, in the top octave's units
-    uint32_t row_count[kBuckets];
+    double row_mass[4 * kBuckets];  // of a bucket of the row, in the top octave's units (in four parts at first)
+    uint32_t row_count[4 * kBuckets];
     uint64_t within[kMostParts];  // kept weights of a tile within the border's bucket
     uint16_t active[kMostParts];
     uint64_t few[64];
     uint32_t n, n_active;
     // what a search hands on
     int bucket;
-    double before;          // weights, and number, of what is before the range
-    uint32_t count_before;
+    double before;  // weights, and number, of what is before the range
+    uint32_t count_before, left;
     uint64_t lo, hi;
     uint64_t border;
-    double reach;           // weights up to the border
+    double reach;  // weights up to the border
 };
-struct PickShared {
+struct Nothing {};
+template <int MODE> struct PickShared {
     union {
-        TopShared top;
-        SortedShared sorted;
+        std::conditional_t<MODE == FEW || MODE == ANY, TopShared<kMostList>, Nothing> top;
+        std::conditional_t<MODE == SORTED || MODE == ANY, SortedShared, Nothing> sorted;
     };
-    double part[kMostParts];  // kept weights of a tile
+    double part[kMostParts];  // kept weights of a tile, in units of the row's top octave
     int shift[kMostParts];    // by how many buckets its top octave is below the row's
-    double table[32], place[16];
-    uint32_t tops[16];
-    double pick_before;
-    int pick, pick_last;
+    double table[kSteps], place[16];
+    int pick;
     uint32_t token;
+    double pick_before;
 };
 
-// A row as the second launch sees it.
+// Writes a row's answer.
+__device__ __forceinline__ void answer(const SampleArgs& a, int64_t row, int64_t token, double logp) {
+    if (a.token64) ((int64_t*)a.token)[row] = token;
+    else ((int32_t*)a.token)[row] = (int32_t)token;
+    a.logp[row] = (float)logp;
+}
+
+// A row that is cut by its size or by its weights, as the second launch sees it.
 template <class T> struct Row {
+    static constexpr int VEC = 16 / sizeof(T);
     const SampleArgs& a;
-    const T* x;
-    const SampleHead* heads;
+    LogitRow<T> x;
     const SampleBody* bodies;
-    Settings set;
     Weights w;
     Fixed fixed;
     uint32_t most;
+    float most_value;
     int index_bits;
 
     __device__ __forceinline__ uint64_t place(uint32_t key, uint32_t index) const { return ((uint64_t)key << index_bits) | ((1u << index_bits) - 1 - index); }
     __device__ __forceinline__ uint32_t key_at(uint64_t place) const { return (uint32_t)(place >> index_bits); }
     __device__ __forceinline__ uint32_t index_at(uint64_t place) const { return ((1u << index_bits) - 1) - ((uint32_t)place & ((1u << index_bits) - 1)); }
-    __device__ __forceinline__ int bucket(uint32_t key) const { return min(w.below(value_of<T>(key)) >> 2, kBuckets - 1); }
+    __device__ __forceinline__ double weight(uint32_t key) const { return w.of(value_of<T>(key), most_value); }
+    __device__ __forceinline__ int bucket(uint32_t key) const {
+        double f;
+        return min(w.below_any(value_of<T>(key), most_value, f) >> 3, kBuckets - 1);
+    }
 
-    // The smallest key from `lo` to `most` of which `is` holds; it holds for `most`, and above any key of which it holds. Every wavefront for itself, 64 keys at a time.
+    // The smallest key up to `most` of which `is` holds; it holds for `most`, and above any key of which it holds. Every wavefront for itself, 64 keys at a time.
     template <class Is> __device__ __forceinline__ uint32_t first_key(Is&& is) const {
         uint32_t lo = kNegInfKey<T> - 1, hi = most;  // not of lo, of hi
+#pragma clang loop unroll(disable)
         while (hi - lo > 1) {
             const uint32_t step = (hi - lo + 63) / 64;
             const uint64_t at = (uint64_t)lo + (uint64_t)step * ((threadIdx.x & 63) + 1);
@@ -290,40 +311,53 @@ template <class T> struct Row {
         }
         return hi;
     }
-    // The largest key of a bucket that the row has something in.
-    __device__ __forceinline__ uint32_t last_key(int b) const {
-        return bucket(most) == b ? most : first_key([&](uint32_t key) { return bucket(key) < b; }) - 1;
+    // The smallest key of a bucket and those above it.
+    __device__ __forceinline__ uint32_t first_key_of(int b) const {
+        if (b == kBuckets - 1) return kNegInfKey<T>;
+        return first_key([&](uint32_t key) { return bucket(key) <= b; });
     }
-    // Calls f(on, place, value) of every logit of the tiles of s.active for whole wavefronts, in no order; `on`: there is one, and its place is in lo ... hi.
+    // The largest key of a bucket that the row has something in.
+    __device__ __forceinline__ uint32_t last_key_of(int b) const { return bucket(most) == b ? most : first_key_of(b - 1) - 1; }
+
+    // Calls f(place, value) of every logit of the tiles of s.active whose place is in lo ... hi, in no order: a wavefront takes 2048 logits at a time.
     template <class F> __device__ __forceinline__ void sweep(const SortedShared& s, uint64_t lo, uint64_t hi, F&& f) const {
-        constexpr int VEC = 16 / sizeof(T), per = kTile / VEC;
-        const uint32_t klo = key_at(lo), khi = key_at(hi);
-        const int all = (int)s.n_active * per;
-        for (int i0 = 0; i0 < all; i0 += blockDim.x) {
-            const int i = i0 + threadIdx.x;
-            Pack<T, VEC> p;
-            int e = a.cols;
-            if (i < all) {
-                const int v = s.active[i / per] * per + i % per;
-                if (v * VEC < a.cols) {
-                    e = v * VEC;
-                    p = logit_vec<T>(x, v, a.cols);
-                }
-            }
+        constexpr int N = 32 / VEC, per = 4;  // vectors of a lane, such pieces of a tile
+        const float vlo = value_of<T>(key_at(lo)), vhi = value_of<T>(key_at(hi));
+        const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, all = (int)s.n_active * per, last = x.vecs() - 1;
+        auto first_vec = [&](int i) { return s.active[min(i, all - 1) / per] * (kTile / VEC) + min(i, all - 1) % per * (64 * N) + lane; };
+        if (all == 0) return;
+        Pack<T, VEC> next[N];
+        int i = threadIdx.x >> 6, v = first_vec(i);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const uint32_t key = e + j < a.cols ? key_of(p.v[j]) : 0;
-                bool on = key >= klo && key <= khi && e + j < a.cols;
-                const uint64_t at = place(key, on ? e + j : 0);
-                on = on && at >= lo && at <= hi;
-                f(on, at, p.v[j]);
+        for (int n = 0; n < N; ++n) next[n] = x.raw(min(v + n * 64, last));
+#pragma clang loop unroll(disable)
+        for (; i < all; i += waves) {
+            uint32_t hits = 0;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float e = Elem<T>::widen(next[n].v[j]);
+                    hits |= e >= vlo && e <= vhi ? 1u << (n * VEC + j) : 0;
+                }
+            const int here = v;
+            v = first_vec(i + waves);
+#pragma unroll
+            for (int n = 0; n < N; ++n) next[n] = x.raw(min(v + n * 64, last));
+            while (hits) {
+                const int b = __builtin_ctz(hits), e = (here + b / VEC * 64) * VEC + b % VEC;
+                hits &= hits - 1;
+                if (!x.holds(e)) continue;
+                const T value = x.base[e];
+                const uint64_t at = place(key_of(value), e - x.lead);
+                if (at >= lo && at <= hi) f(at, Elem<T>::widen(value));
             }
         }
     }
 };
 
 // The tiles that have logits in a bucket of the row.
-template <class T> __device__ __forceinline__ void find_active(const Row<T>& r, PickShared& s, int bucket) {
+template <class T, class Shared> __device__ __forceinline__ void find_active(const Row<T>& r, Shared& s, int bucket) {
     SortedShared& q = s.sorted;
     __syncthreads();
     if (threadIdx.x == 0) q.n_active = 0;
@@ -337,100 +371,107 @@ template <class T> __device__ __forceinline__ void find_active(const Row<T>& r, 
     __syncthreads();
 }
 
-// The border: the first place of the order at which the number of tokens reaches `k` (BY_COUNT) or their weights reach `target`. Returns the place (0: all of the row
+// Of 256 sums in order, four a lane (lane 0 has the first): the first at which `reached(sum, number up to it)` holds, or the last that is not empty; with what is before it.
+// For a wavefront.
+template <class M, class Reached> __device__ __forceinline__ int crossing(const M (&m)[4], const uint32_t (&c)[4], bool by_count, M& before, uint32_t& count_before, Reached&& reached) {
+    const int lane = threadIdx.x & 63;
+    M upto = m[0] + m[1] + m[2] + m[3];
+    uint32_t number = c[0] + c[1] + c[2] + c[3];
+    const bool some = by_count ? number > 0 : upto > (M)0;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        union {
+            M m;
+            int i[2];
+        } in, out;
+        in.m = upto;
+        out.i[0] = __shfl_up(in.i[0], w, 64);
+        out.i[1] = __shfl_up(in.i[1], w, 64);
+        const uint32_t o = __shfl_up(number, w, 64);
+        if (lane >= w) {
+            upto += out.m;
+            number += o;
+        }
+    }
+    const uint64_t reach = __ballot(some && reached(upto, number)), any = __ballot(some);
+    const int at = reach ? __builtin_ctzll(reach) : any ? 63 - __builtin_clzll(any) : 63;
+    union {
+        M m;
+        int i[2];
+    } in, out;
+    in.m = upto;
+    out.i[0] = __shfl_up(in.i[0], 1, 64);
+    out.i[1] = __shfl_up(in.i[1], 1, 64);
+    M b = lane ? out.m : (M)0;
+    uint32_t n = __shfl_up(number, 1, 64);
+    n = lane ? n : 0;
+    int last = 0, d = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (by_count ? c[i] > 0 : m[i] > (M)0) last = i;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool full = by_count ? c[i] > 0 : m[i] > (M)0;
+        if (!found && (i == last || (full && reached(b + m[i], n + c[i])))) {
+            found = true;
+            d = i;
+        }
+        if (!found) {
+            b += m[i];
+            n += c[i];
+        }
+    }
+    union {
+        M m;
+        int i[2];
+    } from, to;
+    from.m = b;
+    to.i[0] = __shfl(from.i[0], at, 64);
+    to.i[1] = __shfl(from.i[1], at, 64);
+    before = to.m;
+    count_before = __shfl(n, at, 64);
+    return at * 4 + __shfl(d, at, 64);
+}
+
+// The border: the first place of the order at which the number of tokens reaches `k` (by_count) or their weights reach `target`. Returns the place (0: all of the row
 // is before it), in s.sorted.reach the weights up to it. `listed`: the bucket whose logits s.sorted.list holds, all of them, q.n in number.
-template <bool BY_COUNT, class T> __device__ __forceinline__ uint64_t find_border(const Row<T>& r, PickShared& s, uint32_t k, double target, int& listed) {
+template <class T, class Shared> __device__ __forceinline__ uint64_t find_border(const Row<T>& r, Shared& s, bool by_count, uint32_t k, double target, int& listed) {
     SortedShared& q = s.sorted;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        double m[4], sum = 0.0;
-        uint32_t c[4], number = 0;
+    int bucket;
+    double before;
+    uint32_t count_before;
+    {
+        // (every wavefront for itself)
+        const int lane = threadIdx.x & 63;
+        double m[4];
+        uint32_t c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             m[i] = q.row_mass[lane * 4 + i];
-            c[i] = BY_COUNT ? q.row_count[lane * 4 + i] : 0;
-            sum += m[i];
-            number += c[i];
+            c[i] = by_count ? q.row_count[lane * 4 + i] : 0;
         }
-        double upto = sum;
-        uint32_t number_upto = number;
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-            union { double d; int i[2]; } in, out;
-            in.d = upto;
-            out.i[0] = __shfl_up(in.i[0], w, 64);
-            out.i[1] = __shfl_up(in.i[1], w, 64);
-            const uint32_t o = __shfl_up(number_upto, w, 64);
-            if (lane >= w) {
-                upto += out.d;
-                number_upto += o;
-            }
-        }
-        double before = upto - sum;
-        uint32_t number_before = number_upto - number;
-        // (the difference may be a rounding off the sum before: the lane before's own)
-        {
-            union { double d; int i[2]; } in, out;
-            in.d = upto;
-            out.i[0] = __shfl_up(in.i[0], 1, 64);
-            out.i[1] = __shfl_up(in.i[1], 1, 64);
-            before = lane ? out.d : 0.0;
-        }
-        const uint64_t reach = __ballot(BY_COUNT ? number_upto >= k : upto >= target);
-        const uint64_t some = __ballot(BY_COUNT ? number > 0 : sum > 0.0);
-        const int at = reach ? __builtin_ctzll(reach) : 63 - __builtin_clzll(some | 1);
-        if (lane == at) {
-            int b = 0;
-            // (where rounding keeps the sum below the target, the last bucket with anything)
-            int last = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (BY_COUNT ? c[i] > 0 : m[i] > 0.0) last = i;
-            bool found = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (!found && i <= last) {
-                    const bool here = i == last || (BY_COUNT ? number_before + c[i] >= k : before + m[i] >= target);
-                    if (here) {
-                        found = true;
-                        b = i;
-                    } else {
-                        before += m[i];
-                        number_before += c[i];
-                    }
-                }
-            q.bucket = lane * 4 + b;
-            q.before = before;
-            q.count_before = number_before;
-        }
+        bucket = crossing(m, c, by_count, before, count_before, [&](double m, uint32_t n) { return by_count ? n >= k : m >= target; });
     }
-    __syncthreads();
-    const int bucket = q.bucket;
-    double before = q.before;
-    uint32_t count_before = q.count_before;
-    const uint32_t klo = bucket == kBuckets - 1 ? kNegInfKey<T> : r.first_key([&](uint32_t key) { return r.bucket(key) <= bucket; });
-    const uint32_t khi = r.last_key(bucket);
-    uint64_t lo = r.place(klo, (1u << r.index_bits) - 1), hi = r.place(khi, 0);
-    const double unit = pow2(-(bucket >> 3)) * r.fixed.unit;  // of the bucket's octave
-    auto weight = [&](float x) { return r.fixed(r.w.of(x) * pow2(bucket >> 3)); };
-    bool have = listed == bucket;
+    uint64_t lo = r.place(r.first_key_of(bucket), (1u << r.index_bits) - 1), hi = r.place(r.last_key_of(bucket), 0);
+    const double up = pow2(bucket >> 3), unit = pow2(-(bucket >> 3)) * r.fixed.unit;  // of the bucket's octave
+    auto weight = [&](float x) { return r.fixed(r.w.of(x, r.most_value) * up); };
+    bool have = listed == bucket, first = true;
     uint32_t n = have ? q.n : 0xFFFFFFFFu;
     if (!have) {
         find_active(r, s, bucket);
         listed = -1;
     }
-    bool first = true;
+#pragma clang loop unroll(disable)
     while (true) {
         if (!have && (first || n <= kMostList)) {
             __syncthreads();
             if (threadIdx.x == 0) q.n = 0;
             __syncthreads();
-            r.sweep(q, lo, hi, [&](bool on, uint64_t at, T) {
-                if (__any(on)) {
-                    const uint32_t i = reserve(on, &q.n);
-                    if (on && i < kMostList) q.list[i] = at;
-                }
+            r.sweep(q, lo, hi, [&](uint64_t at, float) {
+                const uint32_t i = atomicAdd(&q.n, 1u);
+                if (i < kMostList) q.list[i] = at;
             });
             __syncthreads();
             n = q.n;
@@ -461,382 +502,516 @@ template <bool BY_COUNT, class T> __device__ __forceinline__ uint64_t find_borde
                 if (at >= lo && at <= hi) count(at, value_of<T>(r.key_at(at)));
             }
         } else {
-            r.sweep(q, lo, hi, [&](bool on, uint64_t at, T v) {
-                if (on) count(at, Elem<T>::widen(v));
-            });
+            r.sweep(q, lo, hi, count);
         }
         __syncthreads();
-        if (threadIdx.x < 64) {
-            const int lane = threadIdx.x;
-            uint64_t m[4], sum = 0;
-            uint32_t c[4], number = 0;
+        const int lane = threadIdx.x & 63;
+        uint64_t m[4], above;
+        uint32_t c[4], number;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                m[i] = q.mass[255 - (lane * 4 + i)];
-                c[i] = q.count[255 - (lane * 4 + i)];
-                sum += m[i];
-                number += c[i];
-            }
-            uint64_t upto = sum;
-            uint32_t number_upto = number;
-#pragma unroll
-            for (int w = 1; w < 64; w <<= 1) {
-                const uint32_t o0 = __shfl_up((uint32_t)upto, w, 64), o1 = __shfl_up((uint32_t)(upto >> 32), w, 64), o = __shfl_up(number_upto, w, 64);
-                if (lane >= w) {
-                    upto += (uint64_t)o1 << 32 | o0;
-                    number_upto += o;
-                }
-            }
-            auto reached = [&](uint64_t m, uint32_t c) { return BY_COUNT ? count_before + c >= k : before + (double)m * unit >= target; };
-            const uint64_t reach = __ballot(number > 0 && reached(upto, number_upto));
-            const uint64_t some = __ballot(number > 0);
-            const int at = reach ? __builtin_ctzll(reach) : 63 - __builtin_clzll(some | 1);
-            if (lane == at) {
-                uint64_t above = upto - sum;
-                uint32_t number_above = number_upto - number;
-                int last = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (c[i] > 0) last = i;
-                int d = 0;
-                bool found = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!found && i <= last) {
-                        if (i == last || (c[i] > 0 && reached(above + m[i], number_above + c[i]))) {
-                            found = true;
-                            d = i;
-                        } else {
-                            above += m[i];
-                            number_above += c[i];
-                        }
-                    }
-                const uint64_t digit = 255 - (lane * 4 + d);
-                q.lo = lo + (digit << shift);
-                q.hi = min(hi, q.lo + ((1ull << shift) - 1));
-                q.before = before + (double)above * unit;
-                q.count_before = count_before + number_above;
-                q.few[0] = q.count[digit];
-            }
+        for (int i = 0; i < 4; ++i) {
+            m[i] = q.mass[255 - (lane * 4 + i)];
+            c[i] = q.count[255 - (lane * 4 + i)];
         }
-        __syncthreads();
-        lo = q.lo;
-        hi = q.hi;
-        before = q.before;
-        count_before = q.count_before;
-        n = (uint32_t)q.few[0];
-        __syncthreads();
+        // (empty digits have no logits: by number, also where weights are looked at)
+        const int d = crossing(m, c, true, above, number, [&](uint64_t m, uint32_t c) { return by_count ? count_before + c >= k : before + (double)m * unit >= target; });
+        const uint64_t digit = 255 - d;
+        lo += digit << shift;
+        hi = min(hi, lo + ((1ull << shift) - 1));
+        before += (double)above * unit;
+        count_before += number;
+        n = q.count[digit];
     }
     // at most 64 are left: a lane each
     __syncthreads();
-    if (threadIdx.x == 0) q.n_active = 0;  // (their number; the tiles are not needed any more)
+    if (threadIdx.x == 0) q.left = 0;
     __syncthreads();
-    {
-        const uint32_t all = q.n;
-        for (uint32_t i0 = 0; i0 < all; i0 += blockDim.x) {
-            const uint32_t i = i0 + threadIdx.x;
-            const uint64_t at = i < all ? q.list[i] : 0;
-            const bool on = i < all && at >= lo && at <= hi;
-            if (__any(on)) {
-                const uint32_t to = reserve(on, &q.n_active);
-                if (on && to < 64) q.few[to] = at;
-            }
-        }
+    for (uint32_t i = threadIdx.x; i < min(q.n, (uint32_t)kMostList); i += blockDim.x) {
+        const uint64_t at = q.list[i];
+        if (at >= lo && at <= hi) q.few[atomicAdd(&q.left, 1u) & 63] = at;
     }
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        const int left = (int)q.n_active;
-        const uint64_t mine = lane < left ? q.few[lane] : 0;
-        const uint64_t m = lane < left ? weight(value_of<T>(r.key_at(mine))) : 0;
-        uint64_t upto = 0;
-        uint32_t number = 0;
-        for (int j = 0; j < left; ++j) {
-            const uint64_t other = q.few[j];
-            const uint64_t om = (uint64_t)(uint32_t)__shfl((uint32_t)(m >> 32), j, 64) << 32 | (uint32_t)__shfl((uint32_t)m, j, 64);
-            if (other >= mine) {
-                upto += om;
-                ++number;
-            }
+    const int lane = threadIdx.x & 63, left = min((int)q.left, 64);
+    const uint64_t mine = lane < left ? q.few[lane] : 0;
+    const uint64_t m = lane < left ? weight(value_of<T>(r.key_at(mine))) : 0;
+    uint64_t upto = 0;
+    uint32_t number = 0;
+#pragma unroll 4
+    for (int j = 0; j < left; ++j) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+        const uint64_t om = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)m, j);
+        if (other >= mine) {
+            upto += om;
+            ++number;
         }
-        const bool reached = lane < left && (BY_COUNT ? count_before + number >= k : before + (double)upto * unit >= target);
-        // the first that reaches it, or the last there is
-        const uint32_t score = reached ? 1024 - number : lane < left ? number : 0;
-        if (score == group_reduce<MaxU>(score, 64)) {
-            q.border = mine;
-            q.reach = before + (double)upto * unit;
-        }
+    }
+    const bool reached = lane < left && (by_count ? count_before + number >= k : before + (double)upto * unit >= target);
+    // the first that reaches it, or the last there is
+    const uint32_t score = reached ? 1024 - number : lane < left ? number : 0;
+    const uint64_t best = __ballot(score == group_reduce<MaxU>(score, 64));
+    if (threadIdx.x < 64 && lane == __builtin_ctzll(best)) {
+        q.border = mine;
+        q.reach = before + (double)upto * unit;
     }
     __syncthreads();
     return q.border;
 }
 
-// Writes a row's answer.
-template <class T> __device__ __forceinline__ void answer(const SampleArgs& a, int64_t row, int64_t token, double logp) {
-    if (a.token64) ((int64_t*)a.token)[row] = token;
-    else ((int32_t*)a.token)[row] = (int32_t)token;
-    a.logp[row] = (float)logp;
+// u's token among the first k <= 2 * 64 of an order in LDS (key and index as place_of has them), for a wavefront; `weight`: as many numbers in LDS.
+template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs& a, int64_t row, const Settings& set, const double* table, const uint64_t* order, double* weight, int k, double u) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t most = key_of_place(order[0]);
+    if (no_number<T>(most)) {
+        if (lane == 0) answer(a, row, -1, __builtin_nan(""));
+        return;
+    }
+    const Weights w(table, value_of<T>(most), set.steps);
+    double v[2], sum = 0.0;
+    uint32_t index[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t at = lane * 2 + i < k ? order[lane * 2 + i] : 0;
+        index[i] = index_of(at);
+        v[i] = lane * 2 + i < k ? w.of(value_of<T>(key_of_place(at)), value_of<T>(most)) : 0.0;
+        if (lane * 2 + i < k) weight[lane * 2 + i] = v[i];
+        sum += v[i];
+    }
+    wave_fence();
+    auto up = [](double v, int w) {
+        union {
+            double d;
+            int i[2];
+        } in, out;
+        in.d = v;
+        out.i[0] = __shfl_up(in.i[0], w, 64);
+        out.i[1] = __shfl_up(in.i[1], w, 64);
+        return out.d;
+    };
+    auto of_lane = [](double v, int l) {
+        union {
+            double d;
+            int i[2];
+        } in, out;
+        in.d = v;
+        out.i[0] = __shfl(in.i[0], l, 64);
+        out.i[1] = __shfl(in.i[1], l, 64);
+        return out.d;
+    };
+    double upto = sum;
+#pragma unroll
+    for (int n = 1; n < 64; n <<= 1) {
+        const double o = up(upto, n);
+        if (lane >= n) upto += o;
+    }
+    const double shifted = up(upto, 1), before = lane ? shifted : 0.0;
+    const double target = set.p * of_lane(upto, 63), least = fmin(set.least, 1.0) * of_lane(v[0], 0);
+    // how many are kept
+    int cut = k;
+#pragma unroll
+    for (int i = 1; i >= 0; --i) {
+        const int at = lane * 2 + i;
+        const double here = i ? before + sum : before + v[0];
+        if (at >= k) continue;
+        if (set.p < 1.0 && here >= target) cut = at + 1;
+        if (v[i] < least && at > 0) cut = at;
+    }
+    struct MinI {
+        __device__ static __forceinline__ int comb(int a, int b) { return min(a, b); }
+    };
+    const int kept = group_reduce<MinI>(cut, 64);
+    const double whole = of_lane(((kept - 1) & 1) ? before + sum : before + v[0], (kept - 1) >> 1);
+    // u's token: the last by index whose weights before it do not exceed u's part
+    const double part = u * whole;
+    double s0 = 0.0, s1 = 0.0;
+#pragma unroll 4
+    for (int j = 0; j < kept; ++j) {
+        const uint32_t other = index_of(order[j]);
+        const double o = weight[j];
+        s0 += other < index[0] ? o : 0.0;
+        s1 += other < index[1] ? o : 0.0;
+    }
+    uint32_t token = 0;
+    if (lane * 2 < kept && v[0] > 0.0 && s0 <= part) token = index[0] + 1;
+    if (lane * 2 + 1 < kept && v[1] > 0.0 && s1 <= part) token = max(token, index[1] + 1);
+    const uint32_t best = group_reduce<MaxU>(token, 64);
+    if (token == best && best) answer(a, row, best - 1, log((index[0] + 1 == best ? v[0] : v[1]) / whole));
 }
 
-template <class T>
+template <class T, int MODE>
 __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ PickShared s;
+    __shared__ PickShared<MODE> s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     make_table(s.table);
     for (int64_t at = blockIdx.x; at < rows; at += gridDim.x) {
         const int64_t row = row0 + at;
         __syncthreads();
-        Row<T> r{a, (const T*)a.x + offset_of(a.kept, row), (const SampleHead*)a.heads + at * a.tiles, (const SampleBody*)a.bodies + at * a.tiles,
-                 Settings(a, row), Weights{s.table, 0.0, 0.0}, Fixed(a.cols), 0, a.cols > 1 ? 32 - __builtin_clz((unsigned)a.cols - 1) : 0};
-        const Settings& set = r.set;
-        r.w.steps = set.steps;
+        const LogitRow<T> x((const T*)a.x + offset_of(a.kept, row), a.cols);
+        const SampleHead* heads = (const SampleHead*)a.heads + at * a.tiles;
+        const SampleBody* bodies = (const SampleBody*)a.bodies + at * a.tiles;
+        const Settings set(a, row);
+        const int mode = MODE == ANY ? set.mode : MODE;
         double u = a.u[row];
         u = u > 0.0 ? u : 0.0;
-        if (set.mode == BAD) {
-            if (threadIdx.x == 0) answer<T>(a, row, -1, __builtin_nan(""));
+        if (mode == BAD) {
+            if (threadIdx.x == 0) answer(a, row, -1, __builtin_nan(""));
             continue;
         }
-        if (set.mode == FEW) {
-            // (the tiles' keys lie a body apart, one tile's side by side)
-            const int k = set.k;
-            const int n = collect_top<T>(s.top, r.x, a.cols, (const KeyOf<T>*)r.bodies, a.tiles, k, sizeof(SampleBody));
-            uint64_t* order = (uint64_t*)s.top.groups;
-            static_assert(sizeof s.top.groups >= kMostTop * sizeof(uint64_t), "");
-            rank_top(s.top, n, k, [&](int rank, uint64_t p) { order[rank] = p; });
-            __syncthreads();
-            const uint32_t most = key_of_place(order[0]);
-            if (no_number(most, kInfKey<T>, kNegInfKey<T>)) {
-                if (threadIdx.x == 0) answer<T>(a, row, -1, __builtin_nan(""));
+        if constexpr (MODE == FEW || MODE == ANY) {
+            if (mode == FEW) {
+                // (the tiles' keys lie a body apart, one tile's side by side)
+                const int k = set.k;
+                const int n = collect_top(s.top, x, bodies, a.tiles, k, sizeof(SampleBody));
+                uint64_t* order = (uint64_t*)s.top.groups;
+                static_assert(sizeof s.top.groups >= kMostTop * sizeof(uint64_t), "");
+                rank_top(s.top, n, k, [&](int rank, uint64_t p) { order[rank] = p; });
+                __syncthreads();
+                double* weight = (double*)s.top.list;
+                static_assert(sizeof s.top.list >= kMostTop * sizeof(double), "");
+                if (k <= 128) {
+                    if (wave == 0) pick_of_few<T>(a, row, set, s.table, order, weight, k, u);
+                    continue;
+                }
+                const uint32_t most = key_of_place(order[0]);
+                if (no_number<T>(most)) {
+                    if (threadIdx.x == 0) answer(a, row, -1, __builtin_nan(""));
+                    continue;
+                }
+                const Weights w(s.table, value_of<T>(most), set.steps);
+                const int each = (k + (int)blockDim.x - 1) / (int)blockDim.x, i0 = min((int)threadIdx.x * each, k), i1 = min(i0 + each, k);
+                double mine = 0.0;
+                for (int i = i0; i < i1; ++i) mine += weight[i] = w.of(value_of<T>(key_of_place(order[i])), value_of<T>(most));
+                double all;
+                const double before = scan_before(mine, s.place, all);
+                // how many are kept
+                if (threadIdx.x == 0) s.pick = k;
+                __syncthreads();
+                const double target = set.p * all, least = fmin(set.least, 1.0) * weight[0];
+                double upto = before;
+                int cut = k;
+                for (int i = i0; i < i1 && cut == k; ++i) {
+                    if (weight[i] < least && i > 0) cut = i;
+                    upto += weight[i];
+                    if (set.p < 1.0 && upto >= target) cut = min(cut, i + 1);
+                }
+                if (cut < k) atomicMin(&s.pick, cut);
+                __syncthreads();
+                const int kept = s.pick;
+                upto = before;
+                for (int i = i0; i < i1; ++i) {
+                    upto += weight[i];
+                    if (i == kept - 1) s.pick_before = upto;
+                }
+                if (threadIdx.x == 0) s.token = 0;
+                __syncthreads();
+                // u's token: the last by index whose weights before it do not exceed u's part
+                const double part = u * s.pick_before;
+                for (int i = threadIdx.x; i < kept; i += blockDim.x) {
+                    const uint32_t index = index_of(order[i]);
+                    double sum = 0.0;
+#pragma unroll 4
+                    for (int j = 0; j < kept; ++j) sum += index_of(order[j]) < index ? weight[j] : 0.0;
+                    if (weight[i] > 0.0 && sum <= part) atomicMax(&s.token, index + 1);
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < kept; i += blockDim.x)
+                    if (index_of(order[i]) + 1 == s.token) answer(a, row, s.token - 1, log(weight[i] / s.pick_before));
                 continue;
             }
-            r.w.top = top_of(value_of<T>(most), set.steps);
-            double* weight = (double*)s.top.list;
-            static_assert(sizeof s.top.list >= kMostTop * sizeof(double), "");
-            const int each = (k + (int)blockDim.x - 1) / (int)blockDim.x, i0 = min((int)threadIdx.x * each, k), i1 = min(i0 + each, k);
-            double mine = 0.0;
-            for (int i = i0; i < i1; ++i) mine += weight[i] = r.w.of(value_of<T>(key_of_place(order[i])));
-            double all;
-            const double before = scan_before(mine, s.place, all);
-            // how many are kept
-            if (threadIdx.x == 0) s.pick = k;
-            __syncthreads();
-            const double target = set.p * all, least = fmin(set.least, 1.0) * weight[0];
-            double upto = before;
-            int cut = k;
-            for (int i = i0; i < i1 && cut == k; ++i) {
-                if (weight[i] < least && i > 0) cut = i;
-                upto += weight[i];
-                if (set.p < 1.0 && upto >= target) cut = min(cut, i + 1);
+        }
+        if constexpr (MODE != FEW) {
+            // the tiles together (every wavefront for itself)
+            uint32_t most = 0;
+            for (int t = lane; t < a.tiles; t += 64) most = max(most, heads[t].most);
+            most = group_reduce<MaxU>(most, 64);
+            if (no_number<T>(most)) {
+                if (threadIdx.x == 0) answer(a, row, -1, __builtin_nan(""));
+                continue;
             }
-            if (cut < k) atomicMin(&s.pick, cut);
-            __syncthreads();
-            const int kept = s.pick;
-            upto = before;
-            for (int i = i0; i < i1; ++i) {
-                upto += weight[i];
-                if (i == kept - 1) s.pick_before = upto;
+            const float most_value = value_of<T>(most);
+            Row<T> r{a, x, bodies, Weights(s.table, most_value, set.steps), Fixed(a.cols), most, most_value, a.cols > 1 ? 32 - __builtin_clz((unsigned)a.cols - 1) : 0};
+            uint64_t border = 0;
+            for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) {
+                const uint32_t key = heads[t].most;
+                int shift = 1 << 20;
+                double part = 0.0;
+                if (key > kNegInfKey<T>) {
+                    const float v = value_of<T>(key);
+                    // (what a tile's largest is 96 octaves below weighs nothing, here as for a single logit)
+                    if (((double)most_value - (double)v) * r.w.steps < 96.0 * kSteps) {
+                        shift = (r.w.top - (r.w.whole(v) | (kSteps - 1))) >> 3;
+                        part = heads[t].sum * pow2(-(shift >> 3));
+                    }
+                }
+                s.shift[t] = shift;
+                s.part[t] = part;
             }
-            if (threadIdx.x == 0) s.token = 0;
-            __syncthreads();
-            // u's token: the last by index whose weights before it do not exceed u's part
-            const double part = u * s.pick_before;
-            for (int i = threadIdx.x; i < kept; i += blockDim.x) {
-                const uint32_t index = index_of(order[i]);
-                double sum = 0.0;
+            if constexpr (MODE == SORTED || MODE == ANY) {
+                if (mode == SORTED) {
+                    SortedShared& q = s.sorted;
+                    const bool counted = set.k < a.cols;
+                    __syncthreads();
+                    // the row's buckets: those of its tiles, dealt to up to four threads a bucket
+                    const int parts = blockDim.x / kBuckets, b = threadIdx.x % kBuckets;
+                    double mine = 0.0;
+                    uint32_t number = 0;
+                    if (b < kBuckets - 1) {
 #pragma unroll 4
-                for (int j = 0; j < kept; ++j) sum += index_of(order[j]) < index ? weight[j] : 0.0;
-                if (weight[i] > 0.0 && sum <= part) atomicMax(&s.token, index + 1);
+                        for (int t = threadIdx.x / kBuckets; t < a.tiles; t += parts) {
+                            const int src = b - s.shift[t];
+                            const uint64_t m = bodies[t].mass[max(src, 0)];
+                            mine += src >= 0 ? (double)m : 0.0;
+                        }
+                        if (counted)
+#pragma unroll 4
+                            for (int t = threadIdx.x / kBuckets; t < a.tiles; t += parts) {
+                                const int src = b - s.shift[t];
+                                const uint32_t c = bodies[t].count[max(src, 0)];
+                                number += src >= 0 ? c : 0;
+                            }
+                    }
+                    q.row_mass[threadIdx.x] = mine;
+                    q.row_count[threadIdx.x] = number;
+                    double all = 0.0;  // (the same in every wavefront)
+                    for (int t = lane; t < a.tiles; t += 64) all += s.part[t];
+                    all = group_reduce<SumD>(all, 64);
+                    __syncthreads();
+                    if (threadIdx.x < kBuckets) {
+                        for (int i = 1; i < parts; ++i) {
+                            mine += q.row_mass[threadIdx.x + i * kBuckets];
+                            number += q.row_count[threadIdx.x + i * kBuckets];
+                        }
+                        q.row_mass[threadIdx.x] = mine * (pow2(-(b >> 3)) * r.fixed.unit);
+                        q.row_count[threadIdx.x] = number;
+                    }
+                    __syncthreads();
+                    if (wave == 0) {
+                        // the last bucket has the rest
+                        double upper = 0.0;
+                        uint32_t above = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            upper += q.row_mass[lane * 4 + i];
+                            above += q.row_count[lane * 4 + i];
+                        }
+                        struct SumU {
+                            __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a + b; }
+                        };
+                        upper = group_reduce<SumD>(upper, 64);
+                        above = group_reduce<SumU>(above, 64);
+                        if (lane == 63) {
+                            q.row_mass[kBuckets - 1] = fmax(all - upper, 0.0);
+                            q.row_count[kBuckets - 1] = a.cols - above;
+                        }
+                    }
+                    int listed = -1;
+                    double whole = all;
+#pragma clang loop unroll(disable)
+                    for (int by = counted ? 0 : 1; by < (set.p < 1.0 ? 2 : 1); ++by) {
+                        border = max(border, find_border(r, s, by == 0, set.k, set.p * whole, listed));
+                        if (by == 0) whole = q.reach;
+                    }
+                    if (set.least > 0.0) {
+                        const double least = fmin(set.least, 1.0) * r.weight(most);
+                        border = max(border, (uint64_t)r.first_key([&](uint32_t key) { return r.weight(key) >= least; }) << r.index_bits);
+                    }
+                    __syncthreads();
+                    if (border) {
+                        // what is kept of each tile: its buckets above the border's, and within that bucket the logits up to the border
+                        const int bucket = r.bucket(r.key_at(border));
+                        for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) q.within[t] = 0;
+                        if (listed != bucket) find_active(r, s, bucket);
+                        __syncthreads();
+                        const double up = pow2(bucket >> 3);
+                        auto add = [&](uint64_t at, float v) {
+                            __hip_atomic_fetch_add(&q.within[(r.index_at(at) + x.lead) / kTile], r.fixed(r.w.of(v, most_value) * up), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                        };
+                        if (listed == bucket) {
+                            for (uint32_t i = threadIdx.x; i < q.n; i += blockDim.x) {
+                                const uint64_t p = q.list[i];
+                                if (p >= border) add(p, value_of<T>(r.key_at(p)));
+                            }
+                        } else {
+                            r.sweep(q, border, r.place(r.last_key_of(bucket), 0), add);
+                        }
+                        __syncthreads();
+                        for (int t = wave; t < a.tiles; t += waves) {
+                            double kept = 0.0;
+#pragma unroll
+                            for (int i = 0; i < kBuckets / 64; ++i) {
+                                const int b = lane + 64 * i, src = b - s.shift[t];
+                                if (b < bucket && src >= 0) kept += (double)bodies[t].mass[src] * pow2(-(b >> 3));
+                            }
+                            kept = group_reduce<SumD>(kept, 64) * r.fixed.unit;
+                            if (lane == 0) s.part[t] = kept + (double)q.within[t] * (pow2(-(bucket >> 3)) * r.fixed.unit);
+                        }
+                    }
+                }
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < kept; i += blockDim.x)
-                if (index_of(order[i]) + 1 == s.token) answer<T>(a, row, s.token - 1, log(weight[i] / s.pick_before));
-            continue;
-        }
-        // the tiles together
-        double top = -__builtin_huge_val();
-        uint32_t most = 0;
-        for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) {
-            top = fmax(top, r.heads[t].top);
-            most = max(most, r.heads[t].most);
-        }
-        most = block_reduce<MaxU>(most, s.tops);
-        struct MaxD {
-            __device__ static __forceinline__ double comb(double a, double b) { return fmax(a, b); }
-        };
-        top = block_reduce<MaxD>(top, s.place);
-        if (no_number(most, kInfKey<T>, kNegInfKey<T>)) {
-            if (threadIdx.x == 0) answer<T>(a, row, -1, __builtin_nan(""));
-            continue;
-        }
-        r.most = most;
-        r.w.top = top;
-        double all = 0.0;
-        for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) {
-            const int shift = (int)fmin((top - r.heads[t].top) * 0.25, 1e6);
-            s.shift[t] = shift;
-            s.part[t] = shift < 8 * 1024 ? ldexp(r.heads[t].sum, -(shift >> 3)) : 0.0;
-            all += s.part[t];
-        }
-        uint64_t border = 0;
-        if (set.mode == SORTED) {
-            SortedShared& q = s.sorted;
-            const bool counted = set.k < a.cols;
-            all = block_reduce<SumD>(all, s.place);
-            __syncthreads();
-            // the row's buckets
+            // u's tile: the first at which the sum exceeds u of the whole (every wavefront for itself; a lane has the tiles from t0 on)
+            const int each = (a.tiles + 63) / 64, t0 = min(lane * each, a.tiles), t1 = min(t0 + each, a.tiles);
             double mine = 0.0;
-            uint32_t number = 0;
-            if ((int)threadIdx.x < kBuckets - 1) {
-                const int b = threadIdx.x;
-                for (int t = 0; t < a.tiles; ++t) {
-                    const int src = b - s.shift[t];
-                    if (src < 0) continue;
-                    mine += (double)r.bodies[t].mass[src];
-                    if (counted) number += r.bodies[t].count[src];
-                }
-                mine *= pow2(-(b >> 3)) * r.fixed.unit;
-                q.row_mass[b] = mine;
-                q.row_count[b] = number;
-            }
-            const double upper = block_reduce<SumD>(mine, s.place);
-            struct SumU {
-                __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a + b; }
+            for (int t = t0; t < t1; ++t) mine += s.part[t];
+            auto shuffle_up = [](double v, int w) {
+                union {
+                    double d;
+                    int i[2];
+                } in, out;
+                in.d = v;
+                out.i[0] = __shfl_up(in.i[0], w, 64);
+                out.i[1] = __shfl_up(in.i[1], w, 64);
+                return out.d;
             };
-            number = block_reduce<SumU>(number, s.tops);
-            if (threadIdx.x == 0) {
-                q.row_mass[kBuckets - 1] = fmax(all - upper, 0.0);
-                q.row_count[kBuckets - 1] = a.cols - number;
+            auto of_lane = [](double v, int l) {
+                union {
+                    double d;
+                    int i[2];
+                } in, out;
+                in.d = v;
+                out.i[0] = __shfl(in.i[0], l, 64);
+                out.i[1] = __shfl(in.i[1], l, 64);
+                return out.d;
+            };
+            double upto = mine;
+#pragma unroll
+            for (int w = 1; w < 64; w <<= 1) {
+                const double o = shuffle_up(upto, w);
+                if (lane >= w) upto += o;
             }
-            int listed = -1;
-            double whole = all;
-            if (counted) {
-                border = find_border<true>(r, s, set.k, 0.0, listed);
-                whole = q.reach;
+            const double whole = of_lane(upto, 63), target = u * whole;
+            const uint64_t above = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
+            const int owner = above ? __builtin_ctzll(above) : 63 - __builtin_clzll(some);
+            const double shifted = shuffle_up(upto, 1);
+            double before = lane ? shifted : 0.0;
+            int tile = t0;
+            for (int t = t0, last = -1; t < t1; ++t) {
+                if (s.part[t] > 0.0) {
+                    if (last >= 0) {
+                        before += s.part[last];
+                        last = -1;
+                    }
+                    tile = t;
+                    if (before + s.part[t] > target) break;
+                    last = t;
+                }
             }
-            if (set.p < 1.0) border = max(border, find_border<false>(r, s, 0, set.p * whole, listed));
-            if (set.least > 0.0) {
-                const double least = fmin(set.least, 1.0) * r.w.of(value_of<T>(most));
-                border = max(border, (uint64_t)r.first_key([&](uint32_t key) { return r.w.of(value_of<T>(key)) >= least; }) << r.index_bits);
+            tile = __shfl(tile, owner, 64);
+            double rest = fmax(target - of_lane(before, owner), 0.0);
+            // and its token there: a thread has `run` neighbours of the tile
+            const int run = kTile / (int)blockDim.x, e0 = tile * kTile + (int)threadIdx.x * run;
+            mine = 0.0;
+#pragma clang loop unroll(disable)
+            for (int v = e0 / VEC; v < (e0 + run) / VEC; ++v) {
+                if (v > x.vecs() - 1) break;
+                const Pack<T, VEC> p = x.raw(v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int e = v * VEC + i;
+                    const bool on = x.holds(e) && r.place(key_of(p.v[i]), e - x.lead) >= border;
+                    mine += on ? r.w.of(Elem<T>::widen(p.v[i]), most_value) : 0.0;
+                }
             }
+            double tile_sum;
+            const double here = scan_before(mine, s.place, tile_sum);
+            // (the sum over the tile may be a rounding off the part that it was chosen by)
+            if (rest >= tile_sum) rest = tile_sum * (1.0 - 0x1p-50);
+            // the wavefront in which the sum crosses it, the first thread there that does, or the last that has something
+            const double wave_before = of_lane(here, 0), wave_upto = wave + 1 < waves ? [&] {
+                double sum = 0.0;
+                for (int w = 0; w <= wave; ++w) sum += s.place[w];
+                return sum;
+            }() : tile_sum;
+            if ((wave == 0 || wave_before <= rest) && wave_upto > rest) {
+                const uint64_t crosses = __ballot(mine > 0.0 && here + mine > rest), some = __ballot(mine > 0.0);
+                const int l = crosses ? __builtin_ctzll(crosses) : some ? 63 - __builtin_clzll(some) : 0;
+                const int e = __shfl(e0, l, 64) + lane;
+                double w = 0.0;  // (no shuffle below hangs on a condition: a lane that is not asked has nothing to give)
+                if (lane < run && x.holds(e)) {
+                    const T v = x.base[e];
+                    if (r.place(key_of(v), e - x.lead) >= border) w = r.w.of(Elem<T>::widen(v), most_value);
+                }
+                const double from = of_lane(here, l);
+                double sum = w;
+#pragma unroll
+                for (int n = 1; n < 64; n <<= 1) {
+                    const double o = shuffle_up(sum, n);
+                    if (lane >= n) sum += o;
+                }
+                const uint64_t over = __ballot(w > 0.0 && from + sum > rest), any = __ballot(w > 0.0);
+                const int pick = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
+                if (lane == pick) answer(a, row, e - x.lead, log(fmin(w / whole, 1.0)));
+            }
+        }
+    }
+}
+
+// A wavefront for each row, of which at most 128 places matter. One of which it would collect too much is left to the workgroup.
+template <class T>
+__global__ __launch_bounds__(kTileGroups) void sample_wave_kernel(const SampleArgs a, int64_t row0, int64_t rows) {
+    constexpr int N = kTileGroups / 64;
+    __shared__ union {
+        WaveShared wave[N];
+        TopShared<512> all;
+    } s;
+    __shared__ uint64_t order[N][kWaveTop];
+    __shared__ double weight[N][kWaveTop], table[kSteps];
+    __shared__ int left[N];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    make_table(table);
+    __syncthreads();
+    for (int64_t r0 = (int64_t)blockIdx.x * N; r0 < rows; r0 += (int64_t)gridDim.x * N) {
+        const int64_t r = r0 + wave;
+        auto body_of = [&](int64_t r) { return (const SampleBody*)a.bodies + r * a.tiles; };
+        auto row_of = [&](int64_t r) { return LogitRow<T>((const T*)a.x + offset_of(a.kept, row0 + r), a.cols); };
+        int n = 0;
+        if (r < rows) {
+            const Settings set(a, row0 + r);
+            n = wave_top(s.wave[wave], row_of(r), body_of(r), a.tiles, set.k, sizeof(SampleBody));
+            if (n >= 0) wave_rank(s.wave[wave], n, set.k, [&](int rank, uint64_t p) { order[wave][rank] = p; });
+        }
+        if (lane == 0) left[wave] = n < 0;
+        __syncthreads();
+        for (int w = 0; w < N; ++w) {
+            if (!left[w]) continue;
+            const Settings set(a, row0 + r0 + w);
+            const int all = collect_top(s.all, row_of(r0 + w), body_of(r0 + w), a.tiles, set.k, sizeof(SampleBody));
+            rank_top(s.all, all, set.k, [&](int rank, uint64_t p) { order[w][rank] = p; });
             __syncthreads();
-            if (border) {
-                // what is kept of each tile: its buckets above the border's, and within that bucket the logits up to the border
-                const int bucket = r.bucket(r.key_at(border));
-                for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) q.within[t] = 0;
-                if (listed != bucket) find_active(r, s, bucket);
-                __syncthreads();
-                const double up = pow2(bucket >> 3);
-                auto add = [&](uint64_t at, float x) {
-                    __hip_atomic_fetch_add(&q.within[r.index_at(at) / kTile], r.fixed(r.w.of(x) * up), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                };
-                if (listed == bucket) {
-                    for (uint32_t i = threadIdx.x; i < q.n; i += blockDim.x) {
-                        const uint64_t p = q.list[i];
-                        if (p >= border) add(p, value_of<T>(r.key_at(p)));
-                    }
-                } else {
-                    r.sweep(q, border, r.place(r.last_key(bucket), 0), [&](bool on, uint64_t p, T v) {
-                        if (on) add(p, Elem<T>::widen(v));
-                    });
-                }
-                __syncthreads();
-                for (int t = threadIdx.x >> 6; t < a.tiles; t += blockDim.x >> 6) {
-                    double kept = 0.0;
-#pragma unroll
-                    for (int i = 0; i < kBuckets / 64; ++i) {
-                        const int b = (threadIdx.x & 63) + 64 * i, src = b - s.shift[t];
-                        if (b < bucket && src >= 0) kept += (double)r.bodies[t].mass[src] * pow2(-(b >> 3));
-                    }
-                    kept = group_reduce<SumD>(kept, 64) * r.fixed.unit;
-                    if ((threadIdx.x & 63) == 0) s.part[t] = kept + (double)q.within[t] * (pow2(-(bucket >> 3)) * r.fixed.unit);
-                }
-            }
+        }
+        if (r < rows) {
+            const Settings set(a, row0 + r);
+            const double u = a.u[row0 + r];
+            pick_of_few<T>(a, row0 + r, set, table, order[wave], weight[wave], set.k, u > 0.0 ? u : 0.0);
         }
         __syncthreads();
-        // u's tile: the first at which the sum exceeds u of the whole
-        const int each = (a.tiles + (int)blockDim.x - 1) / (int)blockDim.x, t0 = min((int)threadIdx.x * each, a.tiles), t1 = min(t0 + each, a.tiles);
-        double mine = 0.0;
-        for (int t = t0; t < t1; ++t) mine += s.part[t];
-        double whole;
-        double before = scan_before(mine, s.place, whole);
-        if (threadIdx.x == 0) {
-            s.pick = INT32_MAX;
-            s.pick_last = 0;
-        }
-        __syncthreads();
-        const double target = u * whole;
-        double upto = before;
-        for (int t = t0; t < t1; ++t) {
-            if (s.part[t] > 0.0) atomicMax(&s.pick_last, t);
-            upto += s.part[t];
-            if (s.part[t] > 0.0 && upto > target) {
-                atomicMin(&s.pick, t);
-                break;
-            }
-        }
-        __syncthreads();
-        const int tile = s.pick == INT32_MAX ? s.pick_last : s.pick;
-        if (t0 <= tile && tile < t1) {
-            for (int t = t0; t < tile; ++t) before += s.part[t];
-            s.pick_before = before;
-        }
-        __syncthreads();
-        const double rest = target - s.pick_before;
-        // and its token there
-        const int run = kTile / (int)blockDim.x, e0 = tile * kTile + (int)threadIdx.x * run;
-        auto look = [&](auto&& f) {
-            for (int v = 0; v < run / VEC; ++v) {
-                const int e = e0 + v * VEC;
-                if (e >= a.cols) break;
-                const Pack<T, VEC> p = logit_vec<T>(r.x, e / VEC, a.cols);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    if (e + i < a.cols && r.place(key_of(p.v[i]), e + i) >= border) f(e + i, r.w.of(Elem<T>::widen(p.v[i])));
-            }
-        };
-        mine = 0.0;
-        look([&](int, double w) { mine += w; });
-        double tile_sum;
-        const double here = scan_before(mine, s.place, tile_sum);
-        if (threadIdx.x == 0) {
-            s.pick = INT32_MAX;
-            s.pick_last = -1;
-        }
-        __syncthreads();
-        if (mine > 0.0) {
-            double sum = here;
-            int last = -1, first = INT32_MAX;
-            look([&](int e, double w) {
-                if (w > 0.0) {
-                    last = e;
-                    sum += w;
-                    if (sum > rest && e < first) first = e;
-                }
-            });
-            atomicMax(&s.pick_last, last);
-            if (first != INT32_MAX) atomicMin(&s.pick, first);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const int token = s.pick == INT32_MAX ? s.pick_last : s.pick;
-            answer<T>(a, row, token, token < 0 ? __builtin_nan("") : log(fmin(r.w.of(Elem<T>::widen(r.x[token])) / whole, 1.0)));
-        }
     }
 }
 
 }  // namespace
 
-size_t sample_row_bytes(int64_t cols) { return (size_t)((cols + kTile - 1) / kTile) * (sizeof(SampleHead) + sizeof(SampleBody)); }
+size_t sample_row_bytes(int dtype, int64_t cols) { return (size_t)tiles_of(dtype, cols, true) * (sizeof(SampleHead) + sizeof(SampleBody)); }
 
 void launch_sample(int dtype, const SampleArgs& args, hipStream_t st) {
     SampleArgs a = args;
     static_assert(sizeof(SampleHead) % 16 == 0 && sizeof(SampleBody) % 16 == 0, "both arrays are aligned");
     a.bodies = (char*)a.heads + (size_t)a.run * a.tiles * sizeof(SampleHead);
+    const bool each = a.temperature.each || a.top_k.each || a.top_p.each || a.min_p.each;
+    const Settings set(a.temperature.all, a.top_k.all, a.top_p.all, a.min_p.all, a.cols);
     HPT_WITH_TYPE(dtype, {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
-            sample_tiles_kernel<T><<<(unsigned)std::min<int64_t>(rows * a.tiles, 1 << 20), kTileGroups, 0, st>>>(a, row0, rows);
-            sample_pick_kernel<T><<<(unsigned)std::min<int64_t>(rows, 1 << 20), rows <= 512 ? 1024 : 256, 0, st>>>(a, row0, rows);
+            const unsigned blocks = (unsigned)std::min<int64_t>(rows, 1 << 20), threads = rows <= 512 ? 1024 : 256;
+            auto both = [&](auto mode) {
+                constexpr int MODE = decltype(mode)::value;
+                sample_tiles_kernel<T, MODE><<<(unsigned)std::min<int64_t>(rows * a.tiles, 1 << 20), kTileGroups, 0, st>>>(a, row0, rows);
+                if (MODE == FEW && rows > 512 && for_a_wave<T>(a.tiles, set.k)) sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
+                else sample_pick_kernel<T, MODE><<<blocks, MODE == SORTED || MODE == ANY ? threads : 256, 0, st>>>(a, row0, rows);
+            };
+            if (each) both(std::integral_constant<int, ANY>{});
+            else if (set.mode == FEW) both(std::integral_constant<int, FEW>{});
+            else if (set.mode == PLAIN) both(std::integral_constant<int, PLAIN>{});
+            else both(std::integral_constant<int, SORTED>{});
         }
     });
 }

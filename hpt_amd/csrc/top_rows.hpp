@@ -1,30 +1,31 @@
-// The first k places of a row's order, from the largest key of each thread's 32 logits: shared by topk.hip and the rows of sample.hip that
+// The first k places of a row's order, from the largest key of each group of 32 neighbours: shared by topk.hip and the rows of sample.hip that
 // are cut to few tokens. One workgroup for each row.
 //
-// The k-th largest of the groups' keys is at most the k-th largest logit's (each group's largest is one of the row's logits), so only groups that
-// reach it are read again: k of them and those that tie. What they hold at or above that key is collected, and its first k places are the row's.
-// Where that is too much (a row of few different values), the k-th place itself is found by sweeps over the row, eight bits of its key at a
-// time, and the row is collected in its order.
+// The k-th largest of the groups' keys is at most the k-th largest logit's (each group's largest is one of the row's logits), and so is any key below it. One is found
+// from a histogram of the distances below the row's largest, in sixteenths of a power of two; only groups that reach it are read again: k of them, and
+// some more. What they hold at or above that key is collected, and its first k places are the row's. Where that is too much (a row of few different
+// values), the k-th place itself is found by sweeps over the row, eight bits of its key at a time, and the row is collected in its order.
+//
+// Up to 128 places are a wavefront's work, which waits for nobody (wave_top): its histogram is a search by halves over the largest of each vector of keys.
 #pragma once
 
 #include "vocab_rows.hpp"
 
 namespace hpt {
 
-constexpr int kMostList = 2048;  // places collected
-static_assert(kMostTop <= kMostList, "the first k fit the list");
-
-struct TopShared {
-    uint64_t list[kMostList];
-    uint32_t groups[kMostList];  // those that are read again
+// CAP: places collected.
+template <int CAP> struct TopShared {
+    uint64_t list[CAP];
+    uint32_t groups[CAP];  // those that are read again
     Digits digits;
     uint32_t count, many, digit, above;
     uint32_t waves[2 * 16];
 };
 
-// The k-th largest of `n` keys (0 where there are fewer), eight bits at a time; `each` gives the keys to a function: sweep(f) calls f(key) or passes.
-template <int BITS, class Sweep> __device__ __forceinline__ uint32_t kth_key(TopShared& s, uint32_t k, uint32_t* left, Sweep&& sweep) {
+// The k-th largest key of a row, eight bits at a time; `left`: how many of those that equal it are among the first k. sweep(f) calls f(key) for each.
+template <int BITS, int CAP, class Sweep> __device__ __forceinline__ uint32_t kth_key(TopShared<CAP>& s, uint32_t k, uint32_t& left, Sweep&& sweep) {
     uint32_t prefix = 0;
+#pragma clang loop unroll(disable)
     for (int shift = BITS - 8; shift >= 0; shift -= 8) {
         __syncthreads();
         s.digits.clear();
@@ -45,91 +46,34 @@ template <int BITS, class Sweep> __device__ __forceinline__ uint32_t kth_key(Top
         prefix |= s.digit << shift;
         k = k > s.above ? k - s.above : 1;
     }
-    if (left) *left = k;  // so many of those that equal it
+    left = k;
     return prefix;
 }
 
-// Collects into s.list (unordered) the first k <= kMostTop places of the row and perhaps some behind them; returns how many. k <= cols.
-// Each tile's keys lie side by side, `apart` bytes from the next one's.
-template <class T> __device__ __forceinline__ int collect_top(TopShared& s, const T* x, int cols, const void* keys, int tiles, int k, size_t apart = kTileGroups * sizeof(T)) {
-    constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
-    constexpr int KV = 16 / sizeof(KeyOf<T>);  // keys of a vector
-    const int groups = tiles * kTileGroups;
-    constexpr int per = kTileGroups / KV;
-    auto keys_at = [&](int i) { return load_pack<KeyOf<T>, KV>((const KeyOf<T>*)((const char*)keys + (i / per) * apart) + (i % per) * KV); };
-    const uint32_t least = kth_key<kKeyBits<T>>(s, k, nullptr, [&](auto&& f) {
-        for (int i = threadIdx.x; i < groups / KV; i += blockDim.x) {
-            const Pack<KeyOf<T>, KV> p = keys_at(i);
-#pragma unroll
-            for (int j = 0; j < KV; ++j) f((uint32_t)p.v[j]);
-        }
-    });
-    __syncthreads();
-    if (threadIdx.x == 0) s.count = s.many = 0;
-    __syncthreads();
-    const int rounds = (groups / KV + (int)blockDim.x - 1) / (int)blockDim.x;
-    for (int r = 0; r < rounds; ++r) {
-        const int i = r * (int)blockDim.x + (int)threadIdx.x;
-        Pack<KeyOf<T>, KV> p;
-        __builtin_memset(&p, 0, sizeof p);
-        if (i < groups / KV) p = keys_at(i);
-#pragma unroll
-        for (int j = 0; j < KV; ++j) {
-            const bool want = i < groups / KV && p.v[j] >= least;
-            if (__any(want)) {
-                const uint32_t at = reserve(want, &s.many);
-                if (want && at < kMostList) s.groups[at] = i * KV + j;
-            }
-        }
-    }
-    __syncthreads();
-    const int many = (int)s.many;
-    if (many <= kMostList) {
-        for (int w0 = 0; w0 < many * V; w0 += blockDim.x) {
-            const int w = w0 + threadIdx.x;
-            const bool on = w < many * V;
-            Pack<T, VEC> p;
-            int e = cols;
-            if (on) {
-                const uint32_t g = s.groups[w / V];
-                const int v = tile_vec<T>(g / kTileGroups, w % V, g % kTileGroups);
-                e = v * VEC;
-                if (e < cols) p = logit_vec<T>(x, v, cols);
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const uint32_t key = e + i < cols ? key_of(p.v[i]) : 0;
-                const bool want = e + i < cols && key >= least;
-                if (__any(want)) {
-                    const uint32_t at = reserve(want, &s.count);
-                    if (want && at < kMostList) s.list[at] = place_of(key, e + i);
-                }
-            }
-        }
-        __syncthreads();
-        if (s.count <= kMostList) return (int)s.count;
-    }
-    // the key of the k-th place, and how many of those that equal it belong to the first k
+// The first k places by the row alone, in no order, into s.list.
+template <class T, int CAP> __device__ __forceinline__ void collect_by_sweeps(TopShared<CAP>& s, const LogitRow<T>& row, int k) {
+    constexpr int VEC = 16 / sizeof(T);
     uint32_t ties;
-    const int vecs = (cols + VEC - 1) / VEC;
-    const uint32_t key = kth_key<kKeyBits<T>>(s, k, &ties, [&](auto&& f) {
+    const int vecs = row.vecs();
+    const uint32_t key = kth_key<kKeyBits<T>>(s, k, ties, [&](auto&& f) {
         for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-            const Pack<T, VEC> p = logit_vec<T>(x, v, cols);
+            const Pack<T, VEC> p = row.raw(v);
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                if (v * VEC + i < cols) f(key_of(p.v[i]));
+                if (row.holds(v * VEC + i)) f(key_of(p.v[i]));
         }
     });
     // in the row's own order, so that of the equal ones the first are taken
     uint32_t over = 0, equal = 0;  // of both so far
+#pragma clang loop unroll(disable)
     for (int v0 = 0; v0 < vecs; v0 += blockDim.x) {
         const int v = v0 + threadIdx.x;
         Pack<T, VEC> p;
-        if (v < vecs) p = logit_vec<T>(x, v, cols);
+        if (v < vecs) p = row.raw(v);
         uint32_t more = 0, same = 0;
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-            if (v * VEC + i < cols) {
+            if (row.holds(v * VEC + i)) {
                 const uint32_t q = key_of(p.v[i]);
                 more += q > key;
                 same += q == key;
@@ -152,11 +96,11 @@ template <class T> __device__ __forceinline__ int collect_top(TopShared& s, cons
         if (v < vecs)
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                if (v * VEC + i < cols) {
+                if (row.holds(v * VEC + i)) {
                     const uint32_t q = key_of(p.v[i]);
-                    if (q > key) s.list[a++] = place_of(q, v * VEC + i);  // (fewer than k)
+                    if (q > key) s.list[a++] = place_of(q, v * VEC + i - row.lead);  // (fewer than k)
                     else if (q == key) {
-                        if (b < ties) s.list[k - ties + b] = place_of(q, v * VEC + i);
+                        if (b < ties) s.list[k - ties + b] = place_of(q, v * VEC + i - row.lead);
                         ++b;
                     }
                 }
@@ -164,13 +108,240 @@ template <class T> __device__ __forceinline__ int collect_top(TopShared& s, cons
         equal += all >> 16;
     }
     __syncthreads();
+}
+
+// Collects into s.list (unordered) the first k places of the row and perhaps some behind them; returns how many. k <= cols, k <= CAP. Each tile's keys lie
+// side by side, `apart` bytes from the next one's. `smem`: a number for each wavefront.
+template <class T, int CAP> __device__ __forceinline__ int collect_top(TopShared<CAP>& s, const LogitRow<T>& row, const void* keys, int tiles, int k, size_t apart) {
+    constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
+    constexpr int KV = 16 / sizeof(KeyOf<T>), per = kTileGroups / KV;  // keys of a vector, vectors of a tile
+    constexpr int SHIFT = (std::is_same<T, f16_t>::value ? 10 : std::is_same<T, float>::value ? 23 : 7) - 4;
+    const int threads = (int)blockDim.x, vecs = tiles * per, rounds = (vecs + threads - 1) / threads;
+    typedef Pack<KeyOf<T>, KV> Keys;
+    auto keys_at = [&](int r) {
+        const int i = r * threads + (int)threadIdx.x;
+        Keys p;
+        __builtin_memset(&p, 0, sizeof p);
+        if (i < vecs) p = load_pack<KeyOf<T>, KV>((const KeyOf<T>*)((const char*)keys + (i / per) * apart) + (i % per) * KV);
+        return p;
+    };
+    // (two vectors of a thread stay; keys of longer rows are fetched again)
+    const Keys first = keys_at(0), second = rounds > 1 ? keys_at(1) : first;
+    auto keys_of_round = [&](int r) { return r == 0 ? first : r == 1 ? second : keys_at(r); };
+    uint32_t most = 0;
+    for (int r = 0; r < rounds; ++r) {
+        const Keys p = keys_of_round(r);
+#pragma unroll
+        for (int j = 0; j < KV; ++j) most = max(most, (uint32_t)p.v[j]);
+    }
+    s.digits.clear();
+    if (threadIdx.x == 0) s.count = s.many = 0;
+    most = block_reduce<MaxU>(most, s.waves);
+    for (int r = 0; r < rounds; ++r) {
+        const Keys p = keys_of_round(r);
+#pragma unroll
+        for (int j = 0; j < KV; ++j)
+            if (p.v[j]) s.digits.add(255 - min((most - p.v[j]) >> SHIFT, 255u));
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        uint32_t d, above;
+        s.digits.find(k, d, above);
+        if (threadIdx.x == 0) s.digit = d;
+    }
+    __syncthreads();
+    // (the last of the distances holds all that is further)
+    const uint32_t far = (256 - s.digit) << SHIFT, least = s.digit == 0 || far > most ? 1 : most - far + 1;
+    for (int r = 0; r < rounds; ++r) {
+        const Keys p = keys_of_round(r);
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < KV; ++j) hits |= p.v[j] >= least ? 1u << j : 0;
+        while (hits) {
+            const int j = __builtin_ctz(hits);
+            hits &= hits - 1;
+            const uint32_t at = atomicAdd(&s.many, 1u);
+            if (at < CAP) s.groups[at] = (r * threads + threadIdx.x) * KV + j;
+        }
+    }
+    __syncthreads();
+    const int many = (int)s.many;
+    if (many <= CAP) {
+#pragma clang loop unroll(disable)
+        for (int w = threadIdx.x; w < many * V; w += threads) {
+            const int v = group_vec<T>(s.groups[w / V], w % V), e = v * VEC;
+            if (e >= row.end) continue;
+            const Pack<T, VEC> p = row.raw(v);
+            uint32_t key[VEC], hits = 0;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                key[i] = key_of(p.v[i]);
+                hits |= key[i] >= least && row.holds(e + i) ? 1u << i : 0;
+            }
+            if (hits) {
+                uint32_t at = atomicAdd(&s.count, (uint32_t)__builtin_popcount(hits));
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (hits >> i & 1) {
+                        if (at < CAP) s.list[at] = place_of(key[i], e + i - row.lead);
+                        ++at;
+                    }
+            }
+        }
+        __syncthreads();
+        if (s.count <= CAP) return (int)s.count;
+    }
+    collect_by_sweeps<T>(s, row, k);
     return k;
+}
+
+// ---- a wavefront's form ---------------------------------------------------------------------------
+
+constexpr int kWaveTop = 128;    // places at most
+constexpr int kWaveList = 256;   // places, groups and vectors of keys that are collected
+constexpr int kWaveRounds = 20;  // vectors of keys of a lane
+struct WaveShared {
+    union {
+        uint32_t tops[kWaveRounds * 64];  // the largest of each vector of keys
+        uint64_t list[kWaveList];
+    };
+    uint32_t vectors[kWaveList], groups[kWaveList];
+};
+// Whether a row is for it: fewer vectors of keys than places would find no bound.
+template <class T> __host__ __device__ constexpr bool for_a_wave(int tiles, int k) {
+    constexpr int per = kTileGroups * (int)sizeof(T) / 16;
+    return k <= kWaveTop && tiles * per >= 2 * k && tiles * per <= kWaveRounds * 64;
+}
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }  // (a wavefront's accesses to LDS are in order)
+__device__ __forceinline__ int lanes_before(uint64_t who) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0)); }
+
+// Collects into s.list (unordered) the first k places of the row and perhaps some behind them; returns how many, or -1 where that is too much.
+template <class T> __device__ __forceinline__ int wave_top(WaveShared& s, const LogitRow<T>& row, const void* keys, int tiles, int k, size_t apart) {
+    constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
+    constexpr int KV = 16 / sizeof(KeyOf<T>), per = kTileGroups / KV;
+    constexpr int SHIFT = (std::is_same<T, f16_t>::value ? 10 : std::is_same<T, float>::value ? 23 : 7) - 4;
+    typedef Pack<KeyOf<T>, KV> Keys;
+    const int lane = threadIdx.x & 63, vecs = tiles * per, rounds = (vecs + 63) / 64;
+    auto keys_at = [&](int i) { return load_pack<KeyOf<T>, KV>((const KeyOf<T>*)((const char*)keys + (i / per) * apart) + (i % per) * KV); };
+    // the largest of each vector of keys, four vectors on their way together
+    uint32_t most = 0;
+#pragma clang loop unroll(disable)
+    for (int c = 0; c < rounds; c += 4) {
+        Keys p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = keys_at(min((c + i) * 64 + lane, vecs - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < KV; ++j) m = max(m, (uint32_t)p[i].v[j]);
+            s.tops[(c + i) * 64 + lane] = (c + i) * 64 + lane < vecs ? m : 0;
+            most = max(most, m);
+        }
+    }
+    static_assert(kWaveRounds % 4 == 0, "the last round of four stays within");
+    most = group_reduce<MaxU>(most, 64);
+    // the smallest distance below the largest, in sixteenths of a power of two, that k of them are within
+    auto from = [&](int d) {
+        const uint32_t far = (uint32_t)(d + 1) << SHIFT;
+        return d == 255 || far > most ? 1u : most - far + 1;
+    };
+    int lo = -1, hi = 255;
+#pragma clang loop unroll(disable)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        const uint32_t least = from(mid);
+        int n = 0;
+        for (int c = 0; c < rounds; ++c) n += __builtin_popcountll(__ballot(s.tops[c * 64 + lane] >= least));
+        (n >= k ? hi : lo) = mid;
+    }
+    const uint32_t least = from(hi);
+    int na = 0, nb = 0, n = 0;
+    for (int c = 0; c < rounds; ++c) {
+        const bool want = s.tops[c * 64 + lane] >= least;
+        const uint64_t who = __ballot(want);
+        const int at = na + lanes_before(who);
+        if (want && at < kWaveList) s.vectors[at] = c * 64 + lane;
+        na += __builtin_popcountll(who);
+    }
+    if (na > kWaveList) return -1;
+    wave_fence();
+#pragma clang loop unroll(disable)
+    for (int i0 = 0; i0 < na; i0 += 64) {
+        const uint32_t v = s.vectors[min(i0 + lane, na - 1)];
+        const Keys p = keys_at(v);
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < KV; ++j) hits |= p.v[j] >= least ? 1u << j : 0;
+        if (i0 + lane >= na) hits = 0;
+        while (__any(hits)) {
+            const uint64_t who = __ballot(hits != 0);
+            const int at = nb + lanes_before(who);
+            if (hits) {
+                if (at < kWaveList) s.groups[at] = v * KV + __builtin_ctz(hits);
+                hits &= hits - 1;
+            }
+            nb += __builtin_popcountll(who);
+        }
+    }
+    if (nb > kWaveList) return -1;
+    wave_fence();
+#pragma clang loop unroll(disable)
+    for (int w0 = 0; w0 < nb * V; w0 += 64 * 4) {
+        Pack<T, VEC> p[4];
+        int e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int w = w0 + i * 64 + lane;
+            const int v = group_vec<T>(s.groups[min(w / V, nb - 1)], w % V);
+            e[i] = w < nb * V ? v * VEC : row.end;
+            p[i] = row.raw(min(v, row.vecs() - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (w0 + i * 64 >= nb * V) continue;
+            uint32_t key[VEC], hits = 0;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                key[j] = key_of(p[i].v[j]);
+                hits |= key[j] >= least && row.holds(e[i] + j) ? 1u << j : 0;
+            }
+            const int mine = __builtin_popcount(hits);
+            int upto = mine;
+#pragma unroll
+            for (int w = 1; w < 64; w <<= 1) {
+                const int o = __shfl_up(upto, w, 64);
+                if (lane >= w) upto += o;
+            }
+            int at = n + upto - mine;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (hits >> j & 1) {
+                    if (at < kWaveList) s.list[at] = place_of(key[j], e[i] + j - row.lead);
+                    ++at;
+                }
+            n += __shfl(upto, 63, 64);
+        }
+    }
+    wave_fence();
+    return n <= kWaveList ? n : -1;
+}
+
+// Gives each of the first k of `n` places that a wavefront has collected to `out(rank, place)`.
+template <class Out> __device__ __forceinline__ void wave_rank(const WaveShared& s, int n, int k, Out&& out) {
+    for (int i = threadIdx.x & 63; i < n; i += 64) {
+        const uint64_t mine = s.list[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += s.list[j] > mine;
+        if (rank < k) out(rank, mine);
+    }
 }
 
 // Gives each of the first k of `n` collected places to `out(rank, place)`, the ranks counted from 0. Up to kMostRanked of them a thread counts what is before its own; beyond they are sorted.
 constexpr int kMostRanked = 512;
-template <class Out> __device__ __forceinline__ void rank_top(TopShared& s, int n, int k, Out&& out) {
-    if (n <= kMostRanked) {
+template <int CAP, class Out> __device__ __forceinline__ void rank_top(TopShared<CAP>& s, int n, int k, Out&& out) {
+    if (CAP <= kMostRanked || n <= kMostRanked) {
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
             const uint64_t mine = s.list[i];
             int rank = 0;

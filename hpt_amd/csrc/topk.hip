@@ -1,7 +1,7 @@
 // The k largest logits of each row, in order, and the log of the sum of exponentials of the row over a temperature.
 //
-// Two launches. The first reads the logits once, in tiles of 8192: each thread keeps the largest key of its 32 logits (and, where the sum is wanted, adds
-// their exponentials below the tile's largest). The second has a workgroup for each row, which finds the first k places from those keys (top_rows.hpp).
+// Two launches. The first reads the logits once, in tiles of 8192: the largest key of each 32 neighbours stays (and, where the sum is wanted, a wavefront
+// adds the exponentials of its 2048 below their largest). The second has a workgroup for each row, which finds the first k places from those keys (top_rows.hpp).
 // The first is bound by memory, the second by the latency of its steps.
 #include <algorithm>
 #include <cmath>
@@ -20,33 +20,39 @@ Steps steps_of(double temperature) {
     return s;
 }
 
+int64_t tiles_of(int dtype, int64_t cols, bool shifted) { return (cols + (shifted ? 16 / (int64_t)dtype_size(dtype) - 1 : 0) + kTile - 1) / kTile; }
+bool rows_shifted(int dtype, const void* x, const Dims& kept) {
+    bool aligned = (uintptr_t)x % 16 == 0;
+    for (int i = 0; i < kept.n; ++i) aligned = aligned && kept.stride[i] * (int64_t)dtype_size(dtype) % 16 == 0;
+    return !aligned;
+}
 int64_t rows_of_run(int64_t rows, size_t row_bytes) { return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(kMostRowScratch / row_bytes))); }
-static int64_t tiles_of(int64_t cols) { return (cols + kTile - 1) / kTile; }
 size_t topk_row_bytes(int dtype, int64_t cols, bool lse) {
-    return (size_t)tiles_of(cols) * (kTileGroups * dtype_size(dtype) + (lse ? 2 * sizeof(double) : 0));
+    return (size_t)tiles_of(dtype, cols, true) * (kTileGroups * dtype_size(dtype) + (lse ? kTileWaves * 2 * sizeof(double) : 0));
 }
 
 namespace {
 
+constexpr int kMostList = 2048;
+
 template <class T, bool LSE>
 __global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs a, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
-    __shared__ uint32_t tops[4];
-    __shared__ double sums[4];
     for (int64_t at = blockIdx.x; at < rows * a.tiles; at += gridDim.x) {
         const int64_t row = quotient(at, a.tiles);
         const int tile = (int)(at - row * a.tiles);
         Pack<T, VEC> p[V];
-        load_tile<T>((const T*)a.x + offset_of(a.kept, row0 + row), tile, a.cols, p);
-        const uint32_t key = most_key<T>(p);
+        load_tile<T>(LogitRow<T>((const T*)a.x + offset_of(a.kept, row0 + row), a.cols), tile, p);
+        const uint32_t key = group_key<T>(p);
         ((KeyOf<T>*)a.keys)[at * kTileGroups + threadIdx.x] = (KeyOf<T>)key;
         if constexpr (LSE) {
-            const uint32_t top = block_reduce<MaxU>(key, tops);
-            double add = 0.0;
+            // a wavefront's part of the sum, below its own largest
+            const uint32_t top = group_reduce<MaxU>(key, 64);
+            float part = 0.0f;
             // (NaN, +inf and nothing but -inf are told from the largest alone)
-            if (top < kInfKey<T> && top > kNegInfKey<T>) {
-                const float most = value_of<T>(top);
-                float part = 0.0f;
+            const bool number = top < kInfKey<T> && top > kNegInfKey<T>;
+            const float most = number ? value_of<T>(top) : top == kInfKey<T> ? __builtin_huge_valf() : top <= kNegInfKey<T> ? -__builtin_huge_valf() : __builtin_nanf("");
+            if (number) {
 #pragma unroll
                 for (int b = 0; b < V; ++b)
 #pragma unroll
@@ -54,54 +60,95 @@ __global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs
                         const float d = Elem<T>::widen(p[b].v[i]) - most;
                         part += __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo));
                     }
-                add = part;
             }
-            add = block_reduce<SumD>(add, sums);
-            if (threadIdx.x == 0) {
-                a.sums[2 * at] = top >= kInfKey<T> || top <= kNegInfKey<T> ? (top == kInfKey<T> ? __builtin_huge_val() : top <= kNegInfKey<T> ? -__builtin_huge_val() : __builtin_nan("")) : (double)value_of<T>(top);
-                a.sums[2 * at + 1] = add;
+            const double sum = group_reduce<SumD>((double)part, 64);
+            if ((threadIdx.x & 63) == 0) {
+                double* to = a.sums + (at * kTileWaves + (threadIdx.x >> 6)) * 2;
+                to[0] = most;
+                to[1] = sum;
             }
         }
     }
 }
 
+// What a row's k places become.
+template <class T> struct Answer {
+    const TopkArgs& a;
+    const T* x;
+    int64_t row;
+    __device__ __forceinline__ void operator()(int rank, uint64_t at) const {
+        const uint32_t i = index_of(at), key = key_of_place(at);
+        // (a key tells the logit, but for zeros' signs and NaNs' bits)
+        ((T*)a.values)[row * a.k + rank] = key == Bits<T>::sign || key == kNanKey<T> ? x[i] : Elem<T>::narrow(value_of<T>(key));
+        if (a.index64) ((int64_t*)a.index)[row * a.k + rank] = i;
+        else ((int32_t*)a.index)[row * a.k + rank] = (int32_t)i;
+    }
+};
+// The log of the sum from its parts, by a wavefront. They are weighted by the hardware's exponential: one of -D is off by D / 2^24 of itself or so, which is D e^-D / 2^24
+// of the sum at most, less than a rounding. The sum is at least 1; its logarithm in 32 bits is off by one part of 2^24 of lse at most.
+__device__ __forceinline__ void store_lse(const TopkArgs& a, const double* p, int64_t row) {
+    const int lane = threadIdx.x & 63;
+    const float steps = a.steps.hi + a.steps.lo;
+    auto scale = [&](double from, double to) { return (double)(from == to ? 1.0f : __builtin_amdgcn_exp2f((float)(from - to) * steps)); };
+    double top = -__builtin_huge_val(), sum = 0.0;
+    bool nan = false;
+    for (int t = lane; t < a.tiles * kTileWaves; t += 64) {
+        const double most = p[2 * t], part = p[2 * t + 1], n = fmax(top, most);
+        nan |= most != most;
+        sum = sum * scale(top, n) + (part > 0.0 ? part * scale(most, n) : 0.0);
+        top = n;
+    }
+    double all = top;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) all = fmax(all, shfl_xor_any(all, w));
+    sum = group_reduce<SumD>(sum * scale(top, all), 64);
+    if (__any(nan)) all = __builtin_nan("");
+    if (lane == 0) a.lse[row] = (float)(all * a.inv_temperature + (fabs(all) < __builtin_huge_val() ? (double)__builtin_amdgcn_logf((float)sum) * 0.6931471805599453 : 0.0));
+}
+
+// A workgroup for each row.
 template <class T, bool LSE>
 __global__ __launch_bounds__(1024) void topk_pick_kernel(const TopkArgs a, int64_t row0, int64_t rows) {
-    __shared__ TopShared s;
-    __shared__ double place[16], place2[16];
+    __shared__ TopShared<kMostList> s;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int64_t row = row0 + r;
-        const T* x = (const T*)a.x + offset_of(a.kept, row);
-        if constexpr (LSE) {
-            const double* p = a.sums + 2 * r * a.tiles;
-            double top = -__builtin_huge_val(), nan = 0.0;
-            for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) {
-                top = fmax(top, p[2 * t]);
-                nan += p[2 * t] != p[2 * t] ? 1.0 : 0.0;
-            }
-            struct MaxD {
-                __device__ static __forceinline__ double comb(double a, double b) { return fmax(a, b); }
-            };
-            top = block_reduce<MaxD>(top, place);
-            double sum = 0.0;
-            for (int t = threadIdx.x; t < a.tiles; t += blockDim.x)
-                if (p[2 * t + 1] > 0.0) sum += p[2 * t + 1] * exp((p[2 * t] - top) * a.inv_temperature);
-            sum = block_reduce<SumD>(sum, place2);
-            nan = block_reduce<SumD>(nan, place);
-            if (threadIdx.x == 0) {
-                double lse = top * a.inv_temperature;
-                if (nan > 0.0) lse = __builtin_nan("");
-                else if (fabs(top) < __builtin_huge_val()) lse += log(sum);
-                a.lse[row] = (float)lse;
-            }
+        const T* x = (const T*)a.x + offset_of(a.kept, row0 + r);
+        const int n = collect_top(s, LogitRow<T>(x, a.cols), (const KeyOf<T>*)a.keys + r * a.tiles * kTileGroups, a.tiles, a.k, kTileGroups * sizeof(T));
+        rank_top(s, n, a.k, Answer<T>{a, x, row0 + r});
+        // (the last wavefront has fewest places to rank)
+        if (LSE && threadIdx.x >= blockDim.x - 64) store_lse(a, a.sums + 2 * r * a.tiles * kTileWaves, row0 + r);
+        __syncthreads();
+    }
+}
+
+// A wavefront for each row, few places. A row of which it would collect too much is left to the workgroup.
+template <class T, bool LSE>
+__global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a, int64_t row0, int64_t rows) {
+    constexpr int N = kTileGroups / 64;
+    __shared__ union {
+        WaveShared wave[N];
+        TopShared<512> all;
+    } s;
+    static_assert(kWaveTop <= 512, "the first k fit the list");
+    __shared__ int left[N];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t r0 = (int64_t)blockIdx.x * N; r0 < rows; r0 += (int64_t)gridDim.x * N) {
+        const int64_t r = r0 + wave;
+        int n = 0;
+        if (r < rows) {
+            const T* x = (const T*)a.x + offset_of(a.kept, row0 + r);
+            n = wave_top(s.wave[wave], LogitRow<T>(x, a.cols), (const KeyOf<T>*)a.keys + r * a.tiles * kTileGroups, a.tiles, a.k, kTileGroups * sizeof(T));
+            if (n >= 0) wave_rank(s.wave[wave], n, a.k, Answer<T>{a, x, row0 + r});
+            if (LSE) store_lse(a, a.sums + 2 * r * a.tiles * kTileWaves, row0 + r);
         }
-        const int n = collect_top<T>(s, x, a.cols, (const KeyOf<T>*)a.keys + r * a.tiles * kTileGroups, a.tiles, a.k);
-        rank_top(s, n, a.k, [&](int rank, uint64_t at) {
-            const uint32_t i = index_of(at);
-            ((T*)a.values)[row * a.k + rank] = x[i];
-            if (a.index64) ((int64_t*)a.index)[row * a.k + rank] = i;
-            else ((int32_t*)a.index)[row * a.k + rank] = (int32_t)i;
-        });
+        if ((threadIdx.x & 63) == 0) left[wave] = n < 0;
+        __syncthreads();
+        for (int w = 0; w < N; ++w) {
+            if (!left[w]) continue;
+            const T* x = (const T*)a.x + offset_of(a.kept, row0 + r0 + w);
+            const int all = collect_top(s.all, LogitRow<T>(x, a.cols), (const KeyOf<T>*)a.keys + (r0 + w) * a.tiles * kTileGroups, a.tiles, a.k, kTileGroups * sizeof(T));
+            rank_top(s.all, all, a.k, Answer<T>{a, x, row0 + r0 + w});
+            __syncthreads();
+        }
         __syncthreads();
     }
 }
@@ -112,16 +159,15 @@ void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
-            const unsigned tiles = (unsigned)std::min<int64_t>(rows * a.tiles, 1 << 20);
-            // few rows: more threads for each
-            const unsigned threads = rows <= 512 ? 1024 : 256;
-            if (a.lse) {
-                topk_groups_kernel<T, true><<<tiles, kTileGroups, 0, st>>>(a, row0, rows);
-                topk_pick_kernel<T, true><<<(unsigned)std::min<int64_t>(rows, 1 << 20), threads, 0, st>>>(a, row0, rows);
-            } else {
-                topk_groups_kernel<T, false><<<tiles, kTileGroups, 0, st>>>(a, row0, rows);
-                topk_pick_kernel<T, false><<<(unsigned)std::min<int64_t>(rows, 1 << 20), threads, 0, st>>>(a, row0, rows);
-            }
+            const unsigned tiles = (unsigned)std::min<int64_t>(rows * a.tiles, 1 << 20), blocks = (unsigned)std::min<int64_t>(rows, 1 << 20);
+            auto both = [&](auto lse) {
+                constexpr bool LSE = decltype(lse)::value;
+                topk_groups_kernel<T, LSE><<<tiles, kTileGroups, 0, st>>>(a, row0, rows);
+                if (for_a_wave<T>(a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
+                else topk_pick_kernel<T, LSE><<<blocks, rows <= 512 ? 1024 : 256, 0, st>>>(a, row0, rows);  // (few rows: more threads for each)
+            };
+            if (a.lse) both(std::true_type{});
+            else both(std::false_type{});
         }
     });
 }

@@ -38,28 +38,25 @@ template <class T> __device__ __forceinline__ float value_of(uint32_t key) {
     return Elem<T>::widen(__builtin_bit_cast(T, (KeyOf<T>)b));
 }
 
-// The largest key of some vectors: two-byte logits two at a time, as signed numbers whose order is the values'. Negative NaNs, which that order puts below
+// The largest key of a vector: two-byte logits two at a time, as signed numbers whose order is the values'. Negative NaNs, which that order puts below
 // everything, show as the largest plain bits.
-template <class T, int N> __device__ __forceinline__ uint32_t most_key(const Pack<T, 16 / sizeof(T)> (&p)[N]) {
+template <class T> __device__ __forceinline__ uint32_t most_key(const Pack<T, 16 / sizeof(T)>& p) {
     using B = Bits<T>;
     typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     if constexpr (sizeof(T) == 2) {
         s16x2 top = {-32768, -32768};
         u16x2 raw = {0, 0};
+        struct Words {
+            uint32_t w[4];
+        };
+        const Words words = __builtin_bit_cast(Words, p);
 #pragma unroll
-        for (int b = 0; b < N; ++b) {
-            struct Words {
-                uint32_t w[4];
-            };
-            const Words words = __builtin_bit_cast(Words, p[b]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const s16x2 s = __builtin_bit_cast(s16x2, words.w[i]);
-                const s16x2 o = s ^ ((s >> 15) & (int16_t)0x7FFF);
-                top = __builtin_elementwise_max(top, o);
-                raw = __builtin_elementwise_max(raw, __builtin_bit_cast(u16x2, words.w[i]));
-            }
+        for (int i = 0; i < 4; ++i) {
+            const s16x2 s = __builtin_bit_cast(s16x2, words.w[i]);
+            const s16x2 o = s ^ ((s >> 15) & (int16_t)0x7FFF);
+            top = __builtin_elementwise_max(top, o);
+            raw = __builtin_elementwise_max(raw, __builtin_bit_cast(u16x2, words.w[i]));
         }
         const int16_t t = top.x > top.y ? top.x : top.y;
         const uint16_t r = raw.x > raw.y ? raw.x : raw.y;
@@ -69,47 +66,94 @@ template <class T, int N> __device__ __forceinline__ uint32_t most_key(const Pac
         int32_t top = INT32_MIN;
         uint32_t raw = 0;
 #pragma unroll
-        for (int b = 0; b < N; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t u = bits_of(p[b].v[i]);
-                const int32_t s = (int32_t)u, o = s ^ ((s >> 31) & 0x7FFFFFFF);
-                top = top > o ? top : o;
-                raw = raw > u ? raw : u;
-            }
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = bits_of(p.v[i]);
+            const int32_t s = (int32_t)u, o = s ^ ((s >> 31) & 0x7FFFFFFF);
+            top = top > o ? top : o;
+            raw = raw > u ? raw : u;
+        }
         if (raw > (B::sign | B::inf)) return kNanKey<T>;
         return key_of_bits<T>((uint32_t)(top ^ ((top >> 31) & 0x7FFFFFFF)));
     }
 }
 
-// Vector v of a row of `cols` logits, -inf behind its end.
-template <class T> __device__ __forceinline__ Pack<T, 16 / sizeof(T)> logit_vec(const T* row, int v, int cols) {
-    constexpr int VEC = 16 / sizeof(T);
-    const int e = v * VEC;
-    if (e + VEC <= cols) return load_pack_unaligned<T, VEC>(row + e);
-    Pack<T, VEC> p;
+// A row of logits as the aligned vectors that contain it: `lead` elements before its first one (they may be another row's) and those behind its last are -inf. (Unaligned
+// vectors, from the row's start on: loss of distillation alone, bf16 [8192, 50257] 206 -> 179 us.)
+template <class T> struct LogitRow {
+    static constexpr int VEC = 16 / sizeof(T);
+    const T* base;
+    int lead, end;  // the row is at lead ... end - 1
+    __device__ __forceinline__ LogitRow(const T* x, int cols) : lead((int)((uintptr_t)x & 15) / (int)sizeof(T)), end(lead + cols) { base = x - lead; }
+    __device__ __forceinline__ bool holds(int e) const { return e >= lead && e < end; }
+    __device__ __forceinline__ int vecs() const { return (end + VEC - 1) / VEC; }
+    // v below vecs()
+    __device__ __forceinline__ Pack<T, VEC> raw(int v) const { return load_pack<T, VEC>(base + (int64_t)v * VEC); }
+    __device__ __forceinline__ void clean(Pack<T, VEC>& p, int v) const {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p.v[i] = e + i < cols ? row[e + i] : Elem<T>::narrow(-__builtin_huge_valf());
-    return p;
-}
+        for (int i = 0; i < VEC; ++i)
+            if (!holds(v * VEC + i)) p.v[i] = Elem<T>::narrow(-__builtin_huge_valf());
+    }
+    __device__ __forceinline__ Pack<T, VEC> vec(int v) const {
+        Pack<T, VEC> p = raw(v);
+        clean(p, v);
+        return p;
+    }
+};
 // Vector b of the 32 logits that a thread has of a tile: the vectors of a tile lie thread beside thread.
 template <class T> __device__ __forceinline__ int tile_vec(int tile, int b, int thread) { return tile * (kTile * (int)sizeof(T) / 16) + b * kTileGroups + thread; }
 template <class T> constexpr int kTileVecs = kTile * sizeof(T) / 16 / kTileGroups;  // of a thread
-// All of them. A tile that is whole needs no look at the row's end, and its loads are on their way together.
-template <class T> __device__ __forceinline__ void load_tile(const T* row, int tile, int cols, Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
+// All of them: their loads are on their way together, and only a tile with an end of the row looks for it. STREAM: past the caches.
+template <class T, bool STREAM = false> __device__ __forceinline__ void load_tile(const LogitRow<T>& row, int tile, Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
     constexpr int VEC = 16 / sizeof(T);
-    if ((tile + 1) * (int64_t)kTile <= cols) {
+    const int last = row.vecs() - 1;
 #pragma unroll
-        for (int b = 0; b < kTileVecs<T>; ++b) p[b] = load_pack_unaligned<T, VEC>(row + (int64_t)tile_vec<T>(tile, b, threadIdx.x) * VEC);
-    } else {
+    for (int b = 0; b < kTileVecs<T>; ++b) {
+        const T* at = row.base + (int64_t)min(tile_vec<T>(tile, b, threadIdx.x), last) * VEC;
+        p[b] = STREAM ? load_pack_stream<T, VEC>(at) : load_pack<T, VEC>(at);
+    }
+    if ((tile == 0 && row.lead) || (tile + 1) * (int64_t)kTile > row.end) {
 #pragma unroll
-        for (int b = 0; b < kTileVecs<T>; ++b) p[b] = logit_vec<T>(row, tile_vec<T>(tile, b, threadIdx.x), cols);
+        for (int b = 0; b < kTileVecs<T>; ++b) row.clean(p[b], tile_vec<T>(tile, b, threadIdx.x));
     }
 }
 
 struct MaxU {
     __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a > b ? a : b; }
 };
+// A tile's logits are dealt to groups of 32 neighbours, whose largest keys its threads get one each: thread l that of the kTileVecs vectors from (l % kTileVecs) * 256 +
+// l / kTileVecs * kTileVecs on (vectors that neighbouring threads have loaded together; 64 or 128 bytes side by side, so that a group that is read again is one or two lines).
+// Each of 4 (8) threads gives away half of its vectors' largest for the other half of its partner's, then half of those, until one is left.
+template <class T> __device__ __forceinline__ uint32_t group_key(const Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
+    const int lane = threadIdx.x & 63;
+    uint32_t m[kTileVecs<T>];
+#pragma unroll
+    for (int i = 0; i < kTileVecs<T>; ++i) m[i] = most_key<T>(p[i]);
+    if constexpr (kTileVecs<T> == 8) {
+        const bool upper = lane & 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t give = upper ? m[i] : m[i + 4], keep = upper ? m[i + 4] : m[i];
+            m[i] = max(keep, dpp_move<0x141>(give));  // (mirrored within eight)
+        }
+    }
+    {
+        const bool upper = lane & 2;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t give = upper ? m[i] : m[i + 2], keep = upper ? m[i + 2] : m[i];
+            m[i] = max(keep, dpp_move<0x4E>(give));
+        }
+    }
+    const bool upper = lane & 1;
+    const uint32_t give = upper ? m[0] : m[1], keep = upper ? m[1] : m[0];
+    return max(keep, dpp_move<0xB1>(give));
+}
+// Vector w of the group with number g of a row.
+template <class T> __device__ __forceinline__ int group_vec(uint32_t g, int w) {
+    constexpr int V = kTileVecs<T>;
+    const int l = g % kTileGroups;
+    return tile_vec<T>(g / kTileGroups, l % V, l / V * V + w);
+}
 struct SumU64 {
     __device__ static __forceinline__ uint64_t comb(uint64_t a, uint64_t b) { return a + b; }
 };
