@@ -1791,7 +1791,7 @@ int32_t hpt_hip_sample(int32_t dev, void* stream, const hpt_view* logits, const 
         use_device(dev);
         hipStream_t st = (hipStream_t)stream;
         with_workspace(dev, st, workspace, (size_t)a.run * row, false, "sample", [&](void* p) {
-            a.heads = p;
+            a.tiles_scratch = p;
             launch_sample(logits->dtype, a, st);
             check_launch("sample");
         });

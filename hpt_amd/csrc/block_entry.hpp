@@ -242,8 +242,7 @@ struct SampleArgs {
     void* token;          // [rows] of i32 or i64
     int token64;
     float* logp;
-    void* heads;          // [rows of a run, tiles] scratch: SampleHead
-    void* bodies;         // [rows of a run, tiles] scratch: SampleBody
+    void* tiles_scratch;  // [rows of a run, tiles] scratch: what the tiles leave
     int64_t rows;
     int cols;
     int tiles;

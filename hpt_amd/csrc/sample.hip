@@ -25,17 +25,19 @@ constexpr int kBuckets = 256, kCopies = 4;   // of eight steps
 constexpr int kFar = kSteps * 128;           // weights below 2^-128 of the largest are 0
 constexpr int kMostList = 2048;
 
+// What a tile leaves (of each of its wavefronts' 2048 logits, where there is no filter).
 struct SampleHead {
-    double sum;     // of the tile's weights, in units of the octave of its largest
+    double sum;     // of the weights, in units of the octave of the largest
     uint32_t most;  // the largest key
     uint32_t unused;
 };
-struct SampleBody {
+struct SampleTile {
+    SampleHead heads[kTileWaves];
     union {
         uint32_t keys[kTileGroups];
         struct {
-            uint64_t mass[kBuckets];
-            uint32_t count[kBuckets];
+            double mass[kBuckets];     // of a bucket and all above it, in units of the tile's top octave
+            uint32_t count[kBuckets];  // likewise
         };
     };
 };
@@ -63,6 +65,11 @@ struct Settings {
         steps = kSteps * 1.4426950408889634 / t;
         const bool few = k <= kMostTop && k < cols;
         mode = bad ? BAD : few || cols == 1 ? FEW : p >= 1.0 && least <= 0.0 && k == cols ? PLAIN : SORTED;
+    }
+    // of a row; `all`: those for all rows
+    template <int MODE> static __device__ __forceinline__ Settings of(const SampleArgs& a, const Settings& all, int64_t row) {
+        if constexpr (MODE == ANY) return Settings(a, row);
+        else return all;
     }
     __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row)
         : Settings(number_of(a.temperature, row), number_of(a.top_k, row), number_of(a.top_p, row), number_of(a.min_p, row), a.cols) {}
@@ -150,39 +157,42 @@ template <class T> __device__ __forceinline__ bool no_number(uint32_t key) { ret
 // ---- first launch ---------------------------------------------------------------------------------
 
 template <class T, int MODE>
-__global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleArgs a, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleArgs a, const Settings all, int64_t row0) {
     constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
     constexpr bool BUCKETS = MODE == SORTED || MODE == ANY;
     __shared__ uint32_t tops[4];
-    __shared__ double sums[4], table[kSteps];
+    __shared__ double sums[4], table[MODE == FEW ? 1 : kSteps];
     __shared__ uint64_t mass[BUCKETS ? kBuckets * kCopies : 1];
-    __shared__ uint32_t count[BUCKETS ? kBuckets * kCopies : 1];
-    if (MODE != FEW) make_table(table);  // (a barrier of the largest's search comes before its use)
-    const Fixed fixed(a.cols);
-    for (int64_t at = blockIdx.x; at < rows * a.tiles; at += gridDim.x) {
-        const int64_t row = quotient(at, a.tiles);
-        const int tile = (int)(at - row * a.tiles);
+    __shared__ uint32_t count[BUCKETS ? kBuckets * kCopies : 1], counts[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = blockIdx.y;
+    const Settings set = Settings::of<MODE>(a, all, row0 + row);
+    const int mode = MODE == ANY ? set.mode : MODE;
+    if (mode == BAD) return;
+    const LogitRow<T> x((const T*)a.x + offset_of(a.kept, row0 + row), a.cols);
+    if (mode != FEW) {
+        make_table(table);
+        __syncthreads();
+    }
+    for (int at = blockIdx.x; at < a.tiles; at += gridDim.x) {
+        SampleTile& tile = ((SampleTile*)a.tiles_scratch)[row * a.tiles + at];
         Pack<T, VEC> p[V];
-        load_tile<T>(LogitRow<T>((const T*)a.x + offset_of(a.kept, row0 + row), a.cols), tile, p);
-        const Settings set(a, row0 + row);
-        const int mode = MODE == ANY ? set.mode : MODE;
-        if (mode == BAD) continue;
-        SampleBody& body = ((SampleBody*)a.bodies)[at];
-        uint32_t key = 0;
+        load_tile<T>(x, at, p);
         if (mode == FEW) {
-            ((KeyOf<T>*)body.keys)[threadIdx.x] = (KeyOf<T>)group_key<T>(p);
+            ((KeyOf<T>*)tile.keys)[threadIdx.x] = (KeyOf<T>)group_key<T>(p);
             continue;
         }
-        SampleHead& head = ((SampleHead*)a.heads)[at];
+        uint32_t key = 0;
 #pragma unroll
         for (int b = 0; b < V; ++b) key = max(key, most_key<T>(p[b]));
-        key = block_reduce<MaxU>(key, tops);
+        key = group_reduce<MaxU>(key, 64);
         double sum = 0.0;
-        if (!no_number<T>(key)) {
-            const float most = value_of<T>(key);
-            const Weights w(table, most, set.steps);
-            const double lowest = w.lowest(most);
-            if (!BUCKETS || mode == PLAIN) {
+        if (!BUCKETS || mode == PLAIN) {
+            // a wavefront's part, in the octave of its own largest: nobody waits for anybody
+            if (!no_number<T>(key)) {
+                const float most = value_of<T>(key);
+                const Weights w(table, most, set.steps);
+                const double lowest = w.lowest(most);
 #pragma unroll
                 for (int b = 0; b < V; ++b)
 #pragma unroll
@@ -191,13 +201,29 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
                         const int r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), f);
                         sum += Weights::shifted(w.mantissa(r, f), r / kSteps);
                     }
-            } else {
+                sum = group_reduce<SumD>(sum, 64);
+            }
+            if (lane == 0) {
+                tile.heads[wave].sum = sum;
+                tile.heads[wave].most = key;
+            }
+            continue;
+        }
+        if constexpr (BUCKETS) {
+            __syncthreads();
+            if (lane == 0) tops[wave] = key;
+            for (int i = threadIdx.x; i < kBuckets * kCopies; i += kTileGroups) {
+                mass[i] = 0;
+                count[i] = 0;
+            }
+            __syncthreads();
+            key = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+            if (!no_number<T>(key)) {
                 const bool counted = set.k < a.cols;
-                for (int i = threadIdx.x; i < kBuckets * kCopies; i += kTileGroups) {
-                    mass[i] = 0;
-                    count[i] = 0;
-                }
-                __syncthreads();
+                const float most = value_of<T>(key);
+                const Weights w(table, most, set.steps);
+                const Fixed fixed(a.cols);
+                const double lowest = w.lowest(most);
                 const int copy = threadIdx.x & (kCopies - 1);
 #pragma unroll
                 for (int b = 0; b < V; ++b)
@@ -212,44 +238,55 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
                         if (counted) __hip_atomic_fetch_add(&count[bucket * kCopies + copy], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
                 __syncthreads();
-                static_assert(kBuckets == kTileGroups, "a bucket a thread");
-                uint64_t m = 0;
-                uint32_t c = 0;
+                static_assert(kBuckets == kTileGroups && kCopies == 4, "a bucket a thread");
+                const uint64_t m = (mass[threadIdx.x * 4] + mass[threadIdx.x * 4 + 1]) + (mass[threadIdx.x * 4 + 2] + mass[threadIdx.x * 4 + 3]);
+                uint32_t c = (count[threadIdx.x * 4] + count[threadIdx.x * 4 + 1]) + (count[threadIdx.x * 4 + 2] + count[threadIdx.x * 4 + 3]);
+                sum = wave_scan((double)m * fixed.unit * pow2(-(int)(threadIdx.x >> 3)));
+                if (counted) {
 #pragma unroll
-                for (int i = 0; i < kCopies; ++i) {
-                    m += mass[threadIdx.x * kCopies + i];
-                    c += count[threadIdx.x * kCopies + i];
+                    for (int n = 1; n < 64; n <<= 1) {
+                        const uint32_t o = __shfl_up(c, n, 64);
+                        if (lane >= n) c += o;
+                    }
                 }
-                body.mass[threadIdx.x] = m;
-                if (counted) body.count[threadIdx.x] = c;
-                sum = (double)m * fixed.unit * pow2(-(int)(threadIdx.x >> 3));
+                if (lane == 63) {
+                    sums[wave] = sum;
+                    counts[wave] = c;
+                }
+                __syncthreads();
+                for (int i = 0; i < wave; ++i) {
+                    sum += sums[i];
+                    c += counts[i];
+                }
+                tile.mass[threadIdx.x] = sum;
+                if (counted) tile.count[threadIdx.x] = c;
             }
-            sum = block_reduce<SumD>(sum, sums);
-        }
-        if (threadIdx.x == 0) {
-            head.sum = sum;
-            head.most = key;
+            if (threadIdx.x == kTileGroups - 1) {
+                tile.heads[0].sum = sum;
+                tile.heads[0].most = key;
+            }
         }
     }
 }
 
 // ---- second launch --------------------------------------------------------------------------------
 
+constexpr int kMostParts2048 = kMostParts * kTileWaves;
 struct SortedShared {
     uint64_t list[kMostList];
     uint64_t mass[kBuckets];  // of a digit
     uint32_t count[kBuckets];
-    double row_mass[4 * kBuckets];  // of a bucket of the row, in the top octave's units (in four parts at first)
+    double row_mass[4 * kBuckets];  // of a bucket of the row and all above it, in the top octave's units (in four parts at first)
     uint32_t row_count[4 * kBuckets];
     uint64_t within[kMostParts];  // kept weights of a tile within the border's bucket
     uint16_t active[kMostParts];
     uint64_t few[64];
-    uint32_t n, n_active;
-    // what a search hands on
+    uint32_t n, n_active, left;
+    // what the first wavefront finds for all
     int bucket;
-    double before;  // weights, and number, of what is before the range
-    uint32_t count_before, left;
     uint64_t lo, hi;
+    double before;  // weights, and number, of what is before the range
+    uint32_t count_before;
     uint64_t border;
     double reach;  // weights up to the border
 };
@@ -259,8 +296,8 @@ template <int MODE> struct PickShared {
         std::conditional_t<MODE == FEW || MODE == ANY, TopShared<kMostList>, Nothing> top;
         std::conditional_t<MODE == SORTED || MODE == ANY, SortedShared, Nothing> sorted;
     };
-    double part[kMostParts];  // kept weights of a tile, in units of the row's top octave
-    int shift[kMostParts];    // by how many buckets its top octave is below the row's
+    double part[MODE == FEW ? 1 : MODE == SORTED ? kMostParts : kMostParts2048];  // kept weights of a tile (or of a wavefront's part of it), in units of the row's top octave
+    int shift[MODE == SORTED || MODE == ANY ? kMostParts : 1];                    // by how many buckets a tile's top octave is below the row's
     double table[kSteps], place[16];
     int pick;
     uint32_t token;
@@ -276,10 +313,10 @@ __device__ __forceinline__ void answer(const SampleArgs& a, int64_t row, int64_t
 
 // A row that is cut by its size or by its weights, as the second launch sees it.
 template <class T> struct Row {
-    static constexpr int VEC = 16 / sizeof(T);
-    const SampleArgs& a;
+    static constexpr int VEC = 16 / sizeof(T), N = 32 / VEC;  // vectors of a lane: a wavefront takes 2048 logits at a time
     LogitRow<T> x;
-    const SampleBody* bodies;
+    const SampleTile* tiles;
+    int n_tiles;
     Weights w;
     Fixed fixed;
     uint32_t most;
@@ -295,7 +332,7 @@ template <class T> struct Row {
         return min(w.below_any(value_of<T>(key), most_value, f) >> 3, kBuckets - 1);
     }
 
-    // The smallest key up to `most` of which `is` holds; it holds for `most`, and above any key of which it holds. Every wavefront for itself, 64 keys at a time.
+    // The smallest key up to `most` of which `is` holds; it holds for `most`, and above any key of which it holds. For a wavefront, 64 keys at a time.
     template <class Is> __device__ __forceinline__ uint32_t first_key(Is&& is) const {
         uint32_t lo = kNegInfKey<T> - 1, hi = most;  // not of lo, of hi
 #pragma clang loop unroll(disable)
@@ -319,40 +356,106 @@ template <class T> struct Row {
     // The largest key of a bucket that the row has something in.
     __device__ __forceinline__ uint32_t last_key_of(int b) const { return bucket(most) == b ? most : first_key_of(b - 1) - 1; }
 
-    // Calls f(place, value) of every logit of the tiles of s.active whose place is in lo ... hi, in no order: a wavefront takes 2048 logits at a time.
-    template <class F> __device__ __forceinline__ void sweep(const SortedShared& s, uint64_t lo, uint64_t hi, F&& f) const {
-        constexpr int N = 32 / VEC, per = 4;  // vectors of a lane, such pieces of a tile
-        const float vlo = value_of<T>(key_at(lo)), vhi = value_of<T>(key_at(hi));
-        const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, all = (int)s.n_active * per, last = x.vecs() - 1;
-        auto first_vec = [&](int i) { return s.active[min(i, all - 1) / per] * (kTile / VEC) + min(i, all - 1) % per * (64 * N) + lane; };
+    // Calls f(first vector of a lane, its bits) for every 2048 logits of the tiles of s.active, a wavefront each: the bits tell which of a lane's 32 have keys in klo ... khi.
+    template <class F> __device__ __forceinline__ void each_piece(const SortedShared& s, uint32_t klo, uint32_t khi, F&& f) const {
+        const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, all = (int)s.n_active * kTileWaves, last = x.vecs() - 1;
         if (all == 0) return;
+        auto first_vec = [&](int i) { return (s.active[min(i, all - 1) / kTileWaves] * kTileWaves + min(i, all - 1) % kTileWaves) * (64 * N) + lane; };
+        // keys side by side are bits side by side, but for zeros, whose sign does not count
+        const uint32_t zero = Bits<T>::sign;
+        const bool plain = khi < zero || klo > zero;
+        const uint32_t base = klo > zero ? klo & ~zero : ~khi & Bits<T>::all, width = khi - klo;
+        const float vlo = value_of<T>(klo), vhi = value_of<T>(khi);
         Pack<T, VEC> next[N];
         int i = threadIdx.x >> 6, v = first_vec(i);
 #pragma unroll
         for (int n = 0; n < N; ++n) next[n] = x.raw(min(v + n * 64, last));
 #pragma clang loop unroll(disable)
         for (; i < all; i += waves) {
-            uint32_t hits = 0;
+            uint32_t miss = 0;  // bit 31 - m for logit m of a lane (two-byte ones: bit 15 - m / 2 for even ones, 31 - m / 2 for odd ones)
+            if (!plain) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float e = Elem<T>::widen(next[n].v[j]);
-                    hits |= e >= vlo && e <= vhi ? 1u << (n * VEC + j) : 0;
+                    for (int j = 0; j < VEC; ++j) {
+                        const float e = Elem<T>::widen(next[n].v[j]);
+                        const int m = n * VEC + j, bit = sizeof(T) == 2 ? (m & 1 ? 31 : 15) - m / 2 : 31 - m;
+                        miss |= e >= vlo && e <= vhi ? 0 : 1u << bit;
+                    }
+            } else if constexpr (sizeof(T) == 2) {
+                typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                struct Words {
+                    uint32_t w[4];
+                };
+                const u16x2 b2 = {(uint16_t)base, (uint16_t)base}, w2 = {(uint16_t)width, (uint16_t)width}, one = {1, 1};
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const Words words = __builtin_bit_cast(Words, next[n]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const u16x2 d = __builtin_bit_cast(u16x2, words.w[j]) - b2, out = __builtin_elementwise_min(d, w2) ^ d;
+                        miss = miss << 1 | __builtin_bit_cast(uint32_t, __builtin_elementwise_min(out, one));
+                    }
                 }
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) miss = miss << 1 | (bits_of(next[n].v[j]) - base > width ? 1u : 0u);
+            }
             const int here = v;
             v = first_vec(i + waves);
 #pragma unroll
             for (int n = 0; n < N; ++n) next[n] = x.raw(min(v + n * 64, last));
-            while (hits) {
-                const int b = __builtin_ctz(hits), e = (here + b / VEC * 64) * VEC + b % VEC;
-                hits &= hits - 1;
+            f(here, ~miss);
+        }
+    }
+    // Where the logit of a bit lies.
+    static __device__ __forceinline__ int element_of(int first_vec, int bit) {
+        const int m = sizeof(T) == 2 ? 2 * (15 - (bit & 15)) + (bit >> 4) : 31 - bit;
+        return (first_vec + m / VEC * 64) * VEC + m % VEC;
+    }
+    // Collects into s.list the places of a range of keys; s.n: how many, of which only the first kMostList are there.
+    __device__ __forceinline__ void collect(SortedShared& s, uint32_t klo, uint32_t khi) const {
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        each_piece(s, klo, khi, [&](int first, uint32_t hits) {
+            // (what lies outside the row)
+            if ((first & ~63) * VEC < x.lead || (first - (int)(threadIdx.x & 63) + 64 * N) * VEC > x.end)
+                for (uint32_t h = hits; h; h &= h - 1)
+                    if (!x.holds(element_of(first, __builtin_ctz(h)))) hits &= ~(h & -h);
+            const int mine = __builtin_popcount(hits), lane = threadIdx.x & 63;
+            int upto = mine;
+#pragma unroll
+            for (int w = 1; w < 64; w <<= 1) {
+                const int o = __shfl_up(upto, w, 64);
+                if (lane >= w) upto += o;
+            }
+            uint32_t from = 0;
+            if (lane == 63 && upto) from = atomicAdd(&s.n, (uint32_t)upto);
+            uint32_t at = __shfl(from, 63, 64) + upto - mine;
+            for (; hits; hits &= hits - 1, ++at)
+                if (at < kMostList) s.list[at] = (uint32_t)element_of(first, __builtin_ctz(hits));
+        });
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < min(s.n, (uint32_t)kMostList); i += blockDim.x) {
+            const int e = (int)s.list[i];
+            s.list[i] = place(key_of(x.base[e]), e - x.lead);
+        }
+        __syncthreads();
+    }
+    // Calls f(place, value) of every logit whose place is in lo ... hi.
+    template <class F> __device__ __forceinline__ void sweep(const SortedShared& s, uint64_t lo, uint64_t hi, F&& f) const {
+        each_piece(s, key_at(lo), key_at(hi), [&](int first, uint32_t hits) {
+            for (; hits; hits &= hits - 1) {
+                const int e = element_of(first, __builtin_ctz(hits));
                 if (!x.holds(e)) continue;
                 const T value = x.base[e];
                 const uint64_t at = place(key_of(value), e - x.lead);
                 if (at >= lo && at <= hi) f(at, Elem<T>::widen(value));
             }
-        }
+        });
     }
 };
 
@@ -362,136 +465,78 @@ template <class T, class Shared> __device__ __forceinline__ void find_active(con
     __syncthreads();
     if (threadIdx.x == 0) q.n_active = 0;
     __syncthreads();
-    for (int t = threadIdx.x; t < r.a.tiles; t += blockDim.x) {
+    for (int t = threadIdx.x; t < r.n_tiles; t += blockDim.x) {
         const int src = bucket - s.shift[t];
         // (of the last bucket anything may be there, also what weighs nothing)
-        const bool on = bucket == kBuckets - 1 || (src >= 0 && r.bodies[t].mass[src] != 0);
+        const bool on = bucket == kBuckets - 1 || (src >= 0 && r.tiles[t].mass[src] > (src ? r.tiles[t].mass[src - 1] : 0.0));
         if (on) q.active[atomicAdd(&q.n_active, 1u)] = (uint16_t)t;
     }
     __syncthreads();
 }
 
-// Of 256 sums in order, four a lane (lane 0 has the first): the first at which `reached(sum, number up to it)` holds, or the last that is not empty; with what is before it.
-// For a wavefront.
-template <class M, class Reached> __device__ __forceinline__ int crossing(const M (&m)[4], const uint32_t (&c)[4], bool by_count, M& before, uint32_t& count_before, Reached&& reached) {
-    const int lane = threadIdx.x & 63;
-    M upto = m[0] + m[1] + m[2] + m[3];
-    uint32_t number = c[0] + c[1] + c[2] + c[3];
-    const bool some = by_count ? number > 0 : upto > (M)0;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        union {
-            M m;
-            int i[2];
-        } in, out;
-        in.m = upto;
-        out.i[0] = __shfl_up(in.i[0], w, 64);
-        out.i[1] = __shfl_up(in.i[1], w, 64);
-        const uint32_t o = __shfl_up(number, w, 64);
-        if (lane >= w) {
-            upto += out.m;
-            number += o;
-        }
-    }
-    const uint64_t reach = __ballot(some && reached(upto, number)), any = __ballot(some);
-    const int at = reach ? __builtin_ctzll(reach) : any ? 63 - __builtin_clzll(any) : 63;
-    union {
-        M m;
-        int i[2];
-    } in, out;
-    in.m = upto;
-    out.i[0] = __shfl_up(in.i[0], 1, 64);
-    out.i[1] = __shfl_up(in.i[1], 1, 64);
-    M b = lane ? out.m : (M)0;
-    uint32_t n = __shfl_up(number, 1, 64);
-    n = lane ? n : 0;
-    int last = 0, d = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (by_count ? c[i] > 0 : m[i] > (M)0) last = i;
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool full = by_count ? c[i] > 0 : m[i] > (M)0;
-        if (!found && (i == last || (full && reached(b + m[i], n + c[i])))) {
-            found = true;
-            d = i;
-        }
-        if (!found) {
-            b += m[i];
-            n += c[i];
-        }
-    }
-    union {
-        M m;
-        int i[2];
-    } from, to;
-    from.m = b;
-    to.i[0] = __shfl(from.i[0], at, 64);
-    to.i[1] = __shfl(from.i[1], at, 64);
-    before = to.m;
-    count_before = __shfl(n, at, 64);
-    return at * 4 + __shfl(d, at, 64);
-}
-
-// The border: the first place of the order at which the number of tokens reaches `k` (by_count) or their weights reach `target`. Returns the place (0: all of the row
-// is before it), in s.sorted.reach the weights up to it. `listed`: the bucket whose logits s.sorted.list holds, all of them, q.n in number.
+// The border: the first place of the order at which the number of tokens reaches `k` (by_count) or their weights reach `target`. Returns the place, in s.sorted.reach the weights up to it. `listed`: the bucket whose logits s.sorted.list holds, all of them, q.n in number.
 template <class T, class Shared> __device__ __forceinline__ uint64_t find_border(const Row<T>& r, Shared& s, bool by_count, uint32_t k, double target, int& listed) {
     SortedShared& q = s.sorted;
+    const int lane = threadIdx.x & 63;
     __syncthreads();
-    int bucket;
-    double before;
-    uint32_t count_before;
-    {
-        // (every wavefront for itself)
-        const int lane = threadIdx.x & 63;
-        double m[4];
-        uint32_t c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            m[i] = q.row_mass[lane * 4 + i];
-            c[i] = by_count ? q.row_count[lane * 4 + i] : 0;
+    if (threadIdx.x < 64) {
+        // the first bucket at which it is reached; where rounding keeps the sum below the target, the last that adds anything
+        int b = -1, last = 0;
+        for (int c = 0; c < kBuckets / 64; ++c) {
+            const int i = c * 64 + lane;
+            const bool some = by_count ? q.row_count[i] > (i ? q.row_count[i - 1] : 0) : q.row_mass[i] > (i ? q.row_mass[i - 1] : 0.0);
+            const uint64_t any = __ballot(some), reach = __ballot(some && (by_count ? q.row_count[i] >= k : q.row_mass[i] >= target));
+            if (any) last = c * 64 + 63 - __builtin_clzll(any);
+            if (b < 0 && reach) b = c * 64 + __builtin_ctzll(reach);
         }
-        bucket = crossing(m, c, by_count, before, count_before, [&](double m, uint32_t n) { return by_count ? n >= k : m >= target; });
+        if (b < 0) b = last;
+        const uint64_t lo = r.place(r.first_key_of(b), (1u << r.index_bits) - 1), hi = r.place(r.last_key_of(b), 0);
+        if (lane == 0) {
+            q.bucket = b;
+            q.before = b ? q.row_mass[b - 1] : 0.0;
+            q.count_before = b && by_count ? q.row_count[b - 1] : 0;
+            q.lo = lo;
+            q.hi = hi;
+        }
     }
-    uint64_t lo = r.place(r.first_key_of(bucket), (1u << r.index_bits) - 1), hi = r.place(r.last_key_of(bucket), 0);
+    __syncthreads();
+    const int bucket = q.bucket;
     const double up = pow2(bucket >> 3), unit = pow2(-(bucket >> 3)) * r.fixed.unit;  // of the bucket's octave
     auto weight = [&](float x) { return r.fixed(r.w.of(x, r.most_value) * up); };
-    bool have = listed == bucket, first = true;
-    uint32_t n = have ? q.n : 0xFFFFFFFFu;
-    if (!have) {
+    if (listed != bucket) {
         find_active(r, s, bucket);
-        listed = -1;
+        r.collect(q, r.key_at(q.lo), r.key_at(q.hi));
+        listed = q.n <= kMostList ? bucket : -1;
+        // (sums that differ by a rounding may show something in an empty bucket: what is before it reaches the target then)
+        if (q.n == 0) {
+            if (threadIdx.x == 0) q.reach = q.before;
+            return q.hi + 1;
+        }
     }
+    uint32_t n = q.n;
+    bool have = n <= kMostList;
 #pragma clang loop unroll(disable)
     while (true) {
-        if (!have && (first || n <= kMostList)) {
+        if (!have && n <= kMostList) {
+            // (never reached with more than that: what is counted is what is found)
             __syncthreads();
             if (threadIdx.x == 0) q.n = 0;
             __syncthreads();
-            r.sweep(q, lo, hi, [&](uint64_t at, float) {
-                const uint32_t i = atomicAdd(&q.n, 1u);
-                if (i < kMostList) q.list[i] = at;
-            });
+            r.sweep(q, q.lo, q.hi, [&](uint64_t at, float) { q.list[atomicAdd(&q.n, 1u) % kMostList] = at; });
             __syncthreads();
-            n = q.n;
-            have = n <= kMostList;
-            if (have && first) listed = bucket;
-            if (n == 0) return 0;
+            have = true;
         }
-        first = false;
         if (have && n <= 64) break;
         // by eight bits of the place
-        __syncthreads();
         for (int i = threadIdx.x; i < kBuckets; i += blockDim.x) {
             q.mass[i] = 0;
             q.count[i] = 0;
         }
         __syncthreads();
-        const uint64_t width = hi - lo;
+        const uint64_t lo = q.lo, hi = q.hi, width = hi - lo;
         const int bits = width ? 64 - __builtin_clzll(width) : 0, shift = bits > 8 ? bits - 8 : 0;
         auto count = [&](uint64_t at, float x) {
-            const int d = (int)((at - lo) >> shift);
+            const int d = 255 - (int)((at - lo) >> shift);  // (the largest first)
             __hip_atomic_fetch_add(&q.count[d], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             __hip_atomic_fetch_add(&q.mass[d], weight(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         };
@@ -505,22 +550,52 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
             r.sweep(q, lo, hi, count);
         }
         __syncthreads();
-        const int lane = threadIdx.x & 63;
-        uint64_t m[4], above;
-        uint32_t c[4], number;
+        if (threadIdx.x < 64) {
+            // the first digit at which it is reached, or the last that there is, 64 digits at a time
+            uint64_t mass = 0;
+            uint32_t number = 0;
+            int d = -1, last = 0;
+            uint64_t mass_last = 0, mass_before = 0;
+            uint32_t number_last = 0, number_before = 0;
+            for (int c = 0; c < kBuckets / 64 && d < 0; ++c) {
+                const uint64_t m = wave_scan(q.mass[c * 64 + lane]) + mass;
+                uint32_t n = q.count[c * 64 + lane];
+                const bool some = n > 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            m[i] = q.mass[255 - (lane * 4 + i)];
-            c[i] = q.count[255 - (lane * 4 + i)];
+                for (int w = 1; w < 64; w <<= 1) {
+                    const uint32_t o = __shfl_up(n, w, 64);
+                    if (lane >= w) n += o;
+                }
+                n += number;
+                const uint64_t any = __ballot(some), reach = __ballot(some && (by_count ? q.count_before + n >= k : q.before + (double)m * unit >= target));
+                const int at = reach ? __builtin_ctzll(reach) : any ? 63 - __builtin_clzll(any) : 0;
+                // (what is before that digit)
+                const uint64_t m0 = shfl_any(m - q.mass[c * 64 + lane], at);
+                const uint32_t n0 = __shfl(n - q.count[c * 64 + lane], at, 64);
+                if (any) {
+                    last = c * 64 + at;
+                    mass_last = m0;
+                    number_last = n0;
+                }
+                if (reach) {
+                    d = last;
+                }
+                mass = shfl_any(m, 63);
+                number = __shfl(n, 63, 64);
+            }
+            mass_before = mass_last;
+            number_before = number_last;
+            wave_fence();
+            if (lane == 0) {
+                q.lo = lo + ((uint64_t)(255 - last) << shift);
+                q.hi = min(hi, q.lo + ((1ull << shift) - 1));
+                q.before += (double)mass_before * unit;
+                q.count_before += number_before;
+                q.left = q.count[last];
+            }
         }
-        // (empty digits have no logits: by number, also where weights are looked at)
-        const int d = crossing(m, c, true, above, number, [&](uint64_t m, uint32_t c) { return by_count ? count_before + c >= k : before + (double)m * unit >= target; });
-        const uint64_t digit = 255 - d;
-        lo += digit << shift;
-        hi = min(hi, lo + ((1ull << shift) - 1));
-        before += (double)above * unit;
-        count_before += number;
-        n = q.count[digit];
+        __syncthreads();
+        n = q.left;
     }
     // at most 64 are left: a lane each
     __syncthreads();
@@ -528,30 +603,33 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < min(q.n, (uint32_t)kMostList); i += blockDim.x) {
         const uint64_t at = q.list[i];
-        if (at >= lo && at <= hi) q.few[atomicAdd(&q.left, 1u) & 63] = at;
+        if (at >= q.lo && at <= q.hi) q.few[atomicAdd(&q.left, 1u) & 63] = at;
     }
     __syncthreads();
-    const int lane = threadIdx.x & 63, left = min((int)q.left, 64);
-    const uint64_t mine = lane < left ? q.few[lane] : 0;
-    const uint64_t m = lane < left ? weight(value_of<T>(r.key_at(mine))) : 0;
-    uint64_t upto = 0;
-    uint32_t number = 0;
+    if (threadIdx.x < 64) {
+        const int left = min((int)q.left, 64);
+        const uint64_t mine = lane < left ? q.few[lane] : 0;
+        const uint64_t m = lane < left ? weight(value_of<T>(r.key_at(mine))) : 0;
+        uint64_t upto = 0;
+        uint32_t number = 0;
 #pragma unroll 4
-    for (int j = 0; j < left; ++j) {
-        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
-        const uint64_t om = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)m, j);
-        if (other >= mine) {
-            upto += om;
-            ++number;
+        for (int j = 0; j < left; ++j) {
+            const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+            const uint64_t om = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)m, j);
+            if (other >= mine) {
+                upto += om;
+                ++number;
+            }
         }
-    }
-    const bool reached = lane < left && (by_count ? count_before + number >= k : before + (double)upto * unit >= target);
-    // the first that reaches it, or the last there is
-    const uint32_t score = reached ? 1024 - number : lane < left ? number : 0;
-    const uint64_t best = __ballot(score == group_reduce<MaxU>(score, 64));
-    if (threadIdx.x < 64 && lane == __builtin_ctzll(best)) {
-        q.border = mine;
-        q.reach = before + (double)upto * unit;
+        const bool reached = lane < left && (by_count ? q.count_before + number >= k : q.before + (double)upto * unit >= target);
+        // the first that reaches it, or the last there is
+        const uint32_t score = reached ? 1024 - number : lane < left ? number : 0;
+        const uint64_t best = __ballot(score == group_reduce<MaxU>(score, 64));
+        wave_fence();
+        if (lane == __builtin_ctzll(best)) {
+            q.border = mine;
+            q.reach = q.before + (double)upto * unit;
+        }
     }
     __syncthreads();
     return q.border;
@@ -577,34 +655,8 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
         sum += v[i];
     }
     wave_fence();
-    auto up = [](double v, int w) {
-        union {
-            double d;
-            int i[2];
-        } in, out;
-        in.d = v;
-        out.i[0] = __shfl_up(in.i[0], w, 64);
-        out.i[1] = __shfl_up(in.i[1], w, 64);
-        return out.d;
-    };
-    auto of_lane = [](double v, int l) {
-        union {
-            double d;
-            int i[2];
-        } in, out;
-        in.d = v;
-        out.i[0] = __shfl(in.i[0], l, 64);
-        out.i[1] = __shfl(in.i[1], l, 64);
-        return out.d;
-    };
-    double upto = sum;
-#pragma unroll
-    for (int n = 1; n < 64; n <<= 1) {
-        const double o = up(upto, n);
-        if (lane >= n) upto += o;
-    }
-    const double shifted = up(upto, 1), before = lane ? shifted : 0.0;
-    const double target = set.p * of_lane(upto, 63), least = fmin(set.least, 1.0) * of_lane(v[0], 0);
+    const double upto = wave_scan(sum), shifted = shfl_up_any(upto, 1), before = lane ? shifted : 0.0;
+    const double target = set.p * shfl_any(upto, 63), least = fmin(set.least, 1.0) * shfl_any(v[0], 0);
     // how many are kept
     int cut = k;
 #pragma unroll
@@ -619,7 +671,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
         __device__ static __forceinline__ int comb(int a, int b) { return min(a, b); }
     };
     const int kept = group_reduce<MinI>(cut, 64);
-    const double whole = of_lane(((kept - 1) & 1) ? before + sum : before + v[0], (kept - 1) >> 1);
+    const double whole = shfl_any(((kept - 1) & 1) ? before + sum : before + v[0], (kept - 1) >> 1);
     // u's token: the last by index whose weights before it do not exceed u's part
     const double part = u * whole;
     double s0 = 0.0, s1 = 0.0;
@@ -638,7 +690,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
 }
 
 template <class T, int MODE>
-__global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ PickShared<MODE> s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -647,9 +699,8 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
         const int64_t row = row0 + at;
         __syncthreads();
         const LogitRow<T> x((const T*)a.x + offset_of(a.kept, row), a.cols);
-        const SampleHead* heads = (const SampleHead*)a.heads + at * a.tiles;
-        const SampleBody* bodies = (const SampleBody*)a.bodies + at * a.tiles;
-        const Settings set(a, row);
+        const SampleTile* tiles = (const SampleTile*)a.tiles_scratch + at * a.tiles;
+        const Settings set = Settings::of<MODE>(a, all_rows, row);
         const int mode = MODE == ANY ? set.mode : MODE;
         double u = a.u[row];
         u = u > 0.0 ? u : 0.0;
@@ -659,9 +710,8 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
         }
         if constexpr (MODE == FEW || MODE == ANY) {
             if (mode == FEW) {
-                // (the tiles' keys lie a body apart, one tile's side by side)
                 const int k = set.k;
-                const int n = collect_top(s.top, x, bodies, a.tiles, k, sizeof(SampleBody));
+                const int n = collect_top(s.top, x, tiles->keys, a.tiles, k, sizeof(SampleTile));
                 uint64_t* order = (uint64_t*)s.top.groups;
                 static_assert(sizeof s.top.groups >= kMostTop * sizeof(uint64_t), "");
                 rank_top(s.top, n, k, [&](int rank, uint64_t p) { order[rank] = p; });
@@ -720,30 +770,32 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
             }
         }
         if constexpr (MODE != FEW) {
-            // the tiles together (every wavefront for itself)
+            // the parts together (every wavefront for itself): tiles, or a wavefront's 2048 logits of one
+            const int per = MODE == PLAIN || mode == PLAIN ? kTileWaves : 1, parts = a.tiles * per;
+            auto head = [&](int t) -> const SampleHead& { return tiles[t / per].heads[t % per]; };
             uint32_t most = 0;
-            for (int t = lane; t < a.tiles; t += 64) most = max(most, heads[t].most);
+            for (int t = lane; t < parts; t += 64) most = max(most, head(t).most);
             most = group_reduce<MaxU>(most, 64);
             if (no_number<T>(most)) {
                 if (threadIdx.x == 0) answer(a, row, -1, __builtin_nan(""));
                 continue;
             }
             const float most_value = value_of<T>(most);
-            Row<T> r{a, x, bodies, Weights(s.table, most_value, set.steps), Fixed(a.cols), most, most_value, a.cols > 1 ? 32 - __builtin_clz((unsigned)a.cols - 1) : 0};
+            Row<T> r{x, tiles, a.tiles, Weights(s.table, most_value, set.steps), Fixed(a.cols), most, most_value, a.cols > 1 ? 32 - __builtin_clz((unsigned)a.cols - 1) : 0};
             uint64_t border = 0;
-            for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) {
-                const uint32_t key = heads[t].most;
+            for (int t = threadIdx.x; t < parts; t += blockDim.x) {
+                const uint32_t key = head(t).most;
                 int shift = 1 << 20;
                 double part = 0.0;
                 if (key > kNegInfKey<T>) {
                     const float v = value_of<T>(key);
-                    // (what a tile's largest is 96 octaves below weighs nothing, here as for a single logit)
+                    // (what a part's largest is 96 octaves below weighs nothing, here as for a single logit)
                     if (((double)most_value - (double)v) * r.w.steps < 96.0 * kSteps) {
                         shift = (r.w.top - (r.w.whole(v) | (kSteps - 1))) >> 3;
-                        part = heads[t].sum * pow2(-(shift >> 3));
+                        part = head(t).sum * pow2(-(shift >> 3));
                     }
                 }
-                s.shift[t] = shift;
+                if (MODE != PLAIN && per == 1) s.shift[t] = shift;
                 s.part[t] = part;
             }
             if constexpr (MODE == SORTED || MODE == ANY) {
@@ -752,24 +804,22 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
                     const bool counted = set.k < a.cols;
                     __syncthreads();
                     // the row's buckets: those of its tiles, dealt to up to four threads a bucket
-                    const int parts = blockDim.x / kBuckets, b = threadIdx.x % kBuckets;
+                    const int quarters = blockDim.x / kBuckets, b = threadIdx.x % kBuckets;
                     double mine = 0.0;
                     uint32_t number = 0;
-                    if (b < kBuckets - 1) {
-#pragma unroll 4
-                        for (int t = threadIdx.x / kBuckets; t < a.tiles; t += parts) {
-                            const int src = b - s.shift[t];
-                            const uint64_t m = bodies[t].mass[max(src, 0)];
-                            mine += src >= 0 ? (double)m : 0.0;
-                        }
-                        if (counted)
-#pragma unroll 4
-                            for (int t = threadIdx.x / kBuckets; t < a.tiles; t += parts) {
-                                const int src = b - s.shift[t];
-                                const uint32_t c = bodies[t].count[max(src, 0)];
-                                number += src >= 0 ? c : 0;
-                            }
+#pragma unroll 8
+                    for (int t = threadIdx.x / kBuckets; t < a.tiles; t += quarters) {
+                        const int shift = s.shift[t], src = max(b - shift, 0);
+                        const double m = tiles[t].mass[src];
+                        mine += b >= shift ? m * pow2(-min(shift >> 3, 1000)) : 0.0;
                     }
+                    if (counted)
+#pragma unroll 8
+                        for (int t = threadIdx.x / kBuckets; t < a.tiles; t += quarters) {
+                            const int shift = s.shift[t];
+                            const uint32_t c = tiles[t].count[max(b - shift, 0)];
+                            number += b >= shift ? c : 0;
+                        }
                     q.row_mass[threadIdx.x] = mine;
                     q.row_count[threadIdx.x] = number;
                     double all = 0.0;  // (the same in every wavefront)
@@ -777,32 +827,13 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
                     all = group_reduce<SumD>(all, 64);
                     __syncthreads();
                     if (threadIdx.x < kBuckets) {
-                        for (int i = 1; i < parts; ++i) {
+                        for (int i = 1; i < quarters; ++i) {
                             mine += q.row_mass[threadIdx.x + i * kBuckets];
                             number += q.row_count[threadIdx.x + i * kBuckets];
                         }
-                        q.row_mass[threadIdx.x] = mine * (pow2(-(b >> 3)) * r.fixed.unit);
-                        q.row_count[threadIdx.x] = number;
-                    }
-                    __syncthreads();
-                    if (wave == 0) {
-                        // the last bucket has the rest
-                        double upper = 0.0;
-                        uint32_t above = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            upper += q.row_mass[lane * 4 + i];
-                            above += q.row_count[lane * 4 + i];
-                        }
-                        struct SumU {
-                            __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a + b; }
-                        };
-                        upper = group_reduce<SumD>(upper, 64);
-                        above = group_reduce<SumU>(above, 64);
-                        if (lane == 63) {
-                            q.row_mass[kBuckets - 1] = fmax(all - upper, 0.0);
-                            q.row_count[kBuckets - 1] = a.cols - above;
-                        }
+                        // (the last bucket has all the rest)
+                        q.row_mass[threadIdx.x] = b == kBuckets - 1 ? all : fmin(mine, all);
+                        q.row_count[threadIdx.x] = b == kBuckets - 1 ? (uint32_t)a.cols : number;
                     }
                     int listed = -1;
                     double whole = all;
@@ -811,17 +842,26 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
                         border = max(border, find_border(r, s, by == 0, set.k, set.p * whole, listed));
                         if (by == 0) whole = q.reach;
                     }
-                    if (set.least > 0.0) {
-                        const double least = fmin(set.least, 1.0) * r.weight(most);
-                        border = max(border, (uint64_t)r.first_key([&](uint32_t key) { return r.weight(key) >= least; }) << r.index_bits);
-                    }
                     __syncthreads();
+                    if (wave == 0) {
+                        if (set.least > 0.0) {
+                            const double least = fmin(set.least, 1.0) * r.weight(most);
+                            border = max(border, (uint64_t)r.first_key([&](uint32_t key) { return r.weight(key) >= least; }) << r.index_bits);
+                        }
+                        const int bucket = border ? r.bucket(r.key_at(border)) : 0;
+                        const uint32_t khi = r.last_key_of(bucket);
+                        if (lane == 0) {
+                            q.border = border;
+                            q.bucket = bucket;
+                            q.hi = r.place(khi, 0);
+                        }
+                    }
+                    for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) q.within[t] = 0;
+                    __syncthreads();
+                    border = q.border;
                     if (border) {
                         // what is kept of each tile: its buckets above the border's, and within that bucket the logits up to the border
-                        const int bucket = r.bucket(r.key_at(border));
-                        for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) q.within[t] = 0;
-                        if (listed != bucket) find_active(r, s, bucket);
-                        __syncthreads();
+                        const int bucket = q.bucket;
                         const double up = pow2(bucket >> 3);
                         auto add = [&](uint64_t at, float v) {
                             __hip_atomic_fetch_add(&q.within[(r.index_at(at) + x.lead) / kTile], r.fixed(r.w.of(v, most_value) * up), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -832,78 +872,44 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
                                 if (p >= border) add(p, value_of<T>(r.key_at(p)));
                             }
                         } else {
-                            r.sweep(q, border, r.place(r.last_key_of(bucket), 0), add);
+                            find_active(r, s, bucket);
+                            r.sweep(q, border, q.hi, add);
                         }
                         __syncthreads();
-                        for (int t = wave; t < a.tiles; t += waves) {
-                            double kept = 0.0;
-#pragma unroll
-                            for (int i = 0; i < kBuckets / 64; ++i) {
-                                const int b = lane + 64 * i, src = b - s.shift[t];
-                                if (b < bucket && src >= 0) kept += (double)bodies[t].mass[src] * pow2(-(b >> 3));
-                            }
-                            kept = group_reduce<SumD>(kept, 64) * r.fixed.unit;
-                            if (lane == 0) s.part[t] = kept + (double)q.within[t] * (pow2(-(bucket >> 3)) * r.fixed.unit);
+                        for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) {
+                            const int shift = s.shift[t], src = bucket - 1 - shift;
+                            const double above = src >= 0 ? tiles[t].mass[src] * pow2(-(shift >> 3)) : 0.0;
+                            s.part[t] = above + (double)q.within[t] * (pow2(-(bucket >> 3)) * r.fixed.unit);
                         }
                     }
                 }
             }
             __syncthreads();
-            // u's tile: the first at which the sum exceeds u of the whole (every wavefront for itself; a lane has the tiles from t0 on)
-            const int each = (a.tiles + 63) / 64, t0 = min(lane * each, a.tiles), t1 = min(t0 + each, a.tiles);
+            // u's part: the first at which the sum exceeds u of the whole (every wavefront for itself; a lane has the parts from t0 on)
+            const int each = (parts + 63) / 64, t0 = min(lane * each, parts), t1 = min(t0 + each, parts);
             double mine = 0.0;
             for (int t = t0; t < t1; ++t) mine += s.part[t];
-            auto shuffle_up = [](double v, int w) {
-                union {
-                    double d;
-                    int i[2];
-                } in, out;
-                in.d = v;
-                out.i[0] = __shfl_up(in.i[0], w, 64);
-                out.i[1] = __shfl_up(in.i[1], w, 64);
-                return out.d;
-            };
-            auto of_lane = [](double v, int l) {
-                union {
-                    double d;
-                    int i[2];
-                } in, out;
-                in.d = v;
-                out.i[0] = __shfl(in.i[0], l, 64);
-                out.i[1] = __shfl(in.i[1], l, 64);
-                return out.d;
-            };
-            double upto = mine;
-#pragma unroll
-            for (int w = 1; w < 64; w <<= 1) {
-                const double o = shuffle_up(upto, w);
-                if (lane >= w) upto += o;
-            }
-            const double whole = of_lane(upto, 63), target = u * whole;
+            const double upto = wave_scan(mine), whole = shfl_any(upto, 63), target = u * whole, upto_before = shfl_up_any(upto, 1);
             const uint64_t above = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
             const int owner = above ? __builtin_ctzll(above) : 63 - __builtin_clzll(some);
-            const double shifted = shuffle_up(upto, 1);
-            double before = lane ? shifted : 0.0;
-            int tile = t0;
+            double before = lane ? upto_before : 0.0;
+            int part = t0;
             for (int t = t0, last = -1; t < t1; ++t) {
                 if (s.part[t] > 0.0) {
-                    if (last >= 0) {
-                        before += s.part[last];
-                        last = -1;
-                    }
-                    tile = t;
+                    if (last >= 0) before += s.part[last];
+                    part = t;
                     if (before + s.part[t] > target) break;
                     last = t;
                 }
             }
-            tile = __shfl(tile, owner, 64);
-            double rest = fmax(target - of_lane(before, owner), 0.0);
-            // and its token there: a thread has `run` neighbours of the tile
-            const int run = kTile / (int)blockDim.x, e0 = tile * kTile + (int)threadIdx.x * run;
+            part = __shfl(part, owner, 64);
+            double rest = fmax(target - shfl_any(before, owner), 0.0);
+            // and its token there: a thread has `run` neighbours of the part
+            const int size = kTile / per, run = max(size / (int)blockDim.x, VEC), e0 = part * size + (int)threadIdx.x * run;
             mine = 0.0;
 #pragma clang loop unroll(disable)
             for (int v = e0 / VEC; v < (e0 + run) / VEC; ++v) {
-                if (v > x.vecs() - 1) break;
+                if (v > x.vecs() - 1 || e0 >= (part + 1) * size) break;
                 const Pack<T, VEC> p = x.raw(v);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
@@ -912,32 +918,22 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
                     mine += on ? r.w.of(Elem<T>::widen(p.v[i]), most_value) : 0.0;
                 }
             }
-            double tile_sum;
-            const double here = scan_before(mine, s.place, tile_sum);
-            // (the sum over the tile may be a rounding off the part that it was chosen by)
-            if (rest >= tile_sum) rest = tile_sum * (1.0 - 0x1p-50);
+            double part_sum;
+            const double here = scan_before(mine, s.place, part_sum);
+            // (the sum over the part may be a rounding off what it was chosen by)
+            if (rest >= part_sum) rest = part_sum * (1.0 - 0x1p-50);
             // the wavefront in which the sum crosses it, the first thread there that does, or the last that has something
-            const double wave_before = of_lane(here, 0), wave_upto = wave + 1 < waves ? [&] {
-                double sum = 0.0;
-                for (int w = 0; w <= wave; ++w) sum += s.place[w];
-                return sum;
-            }() : tile_sum;
+            const double wave_before = shfl_any(here, 0), wave_upto = shfl_any(wave_scan(lane < waves ? s.place[lane] : 0.0), wave);
             if ((wave == 0 || wave_before <= rest) && wave_upto > rest) {
                 const uint64_t crosses = __ballot(mine > 0.0 && here + mine > rest), some = __ballot(mine > 0.0);
                 const int l = crosses ? __builtin_ctzll(crosses) : some ? 63 - __builtin_clzll(some) : 0;
                 const int e = __shfl(e0, l, 64) + lane;
-                double w = 0.0;  // (no shuffle below hangs on a condition: a lane that is not asked has nothing to give)
+                double w = 0.0;
                 if (lane < run && x.holds(e)) {
                     const T v = x.base[e];
                     if (r.place(key_of(v), e - x.lead) >= border) w = r.w.of(Elem<T>::widen(v), most_value);
                 }
-                const double from = of_lane(here, l);
-                double sum = w;
-#pragma unroll
-                for (int n = 1; n < 64; n <<= 1) {
-                    const double o = shuffle_up(sum, n);
-                    if (lane >= n) sum += o;
-                }
+                const double from = shfl_any(here, l), sum = wave_scan(w);
                 const uint64_t over = __ballot(w > 0.0 && from + sum > rest), any = __ballot(w > 0.0);
                 const int pick = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
                 if (lane == pick) answer(a, row, e - x.lead, log(fmin(w / whole, 1.0)));
@@ -948,7 +944,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const SampleArgs a, i
 
 // A wavefront for each row, of which at most 128 places matter. One of which it would collect too much is left to the workgroup.
 template <class T>
-__global__ __launch_bounds__(kTileGroups) void sample_wave_kernel(const SampleArgs a, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(kTileGroups) void sample_wave_kernel(const SampleArgs a, const Settings set, int64_t row0, int64_t rows) {
     constexpr int N = kTileGroups / 64;
     __shared__ union {
         WaveShared wave[N];
@@ -962,25 +958,22 @@ __global__ __launch_bounds__(kTileGroups) void sample_wave_kernel(const SampleAr
     __syncthreads();
     for (int64_t r0 = (int64_t)blockIdx.x * N; r0 < rows; r0 += (int64_t)gridDim.x * N) {
         const int64_t r = r0 + wave;
-        auto body_of = [&](int64_t r) { return (const SampleBody*)a.bodies + r * a.tiles; };
+        auto keys_of = [&](int64_t r) { return ((const SampleTile*)a.tiles_scratch + r * a.tiles)->keys; };
         auto row_of = [&](int64_t r) { return LogitRow<T>((const T*)a.x + offset_of(a.kept, row0 + r), a.cols); };
         int n = 0;
         if (r < rows) {
-            const Settings set(a, row0 + r);
-            n = wave_top(s.wave[wave], row_of(r), body_of(r), a.tiles, set.k, sizeof(SampleBody));
+            n = wave_top(s.wave[wave], row_of(r), keys_of(r), a.tiles, set.k, sizeof(SampleTile));
             if (n >= 0) wave_rank(s.wave[wave], n, set.k, [&](int rank, uint64_t p) { order[wave][rank] = p; });
         }
         if (lane == 0) left[wave] = n < 0;
         __syncthreads();
         for (int w = 0; w < N; ++w) {
             if (!left[w]) continue;
-            const Settings set(a, row0 + r0 + w);
-            const int all = collect_top(s.all, row_of(r0 + w), body_of(r0 + w), a.tiles, set.k, sizeof(SampleBody));
+            const int all = collect_top(s.all, row_of(r0 + w), keys_of(r0 + w), a.tiles, set.k, sizeof(SampleTile));
             rank_top(s.all, all, set.k, [&](int rank, uint64_t p) { order[w][rank] = p; });
             __syncthreads();
         }
         if (r < rows) {
-            const Settings set(a, row0 + r);
             const double u = a.u[row0 + r];
             pick_of_few<T>(a, row0 + r, set, table, order[wave], weight[wave], set.k, u > 0.0 ? u : 0.0);
         }
@@ -990,23 +983,21 @@ __global__ __launch_bounds__(kTileGroups) void sample_wave_kernel(const SampleAr
 
 }  // namespace
 
-size_t sample_row_bytes(int dtype, int64_t cols) { return (size_t)tiles_of(dtype, cols, true) * (sizeof(SampleHead) + sizeof(SampleBody)); }
+size_t sample_row_bytes(int dtype, int64_t cols) { return (size_t)tiles_of(dtype, cols, true) * sizeof(SampleTile); }
 
-void launch_sample(int dtype, const SampleArgs& args, hipStream_t st) {
-    SampleArgs a = args;
-    static_assert(sizeof(SampleHead) % 16 == 0 && sizeof(SampleBody) % 16 == 0, "both arrays are aligned");
-    a.bodies = (char*)a.heads + (size_t)a.run * a.tiles * sizeof(SampleHead);
+void launch_sample(int dtype, const SampleArgs& a, hipStream_t st) {
+    static_assert(sizeof(SampleTile) % 16 == 0, "every tile's keys are aligned");
     const bool each = a.temperature.each || a.top_k.each || a.top_p.each || a.min_p.each;
     const Settings set(a.temperature.all, a.top_k.all, a.top_p.all, a.min_p.all, a.cols);
     HPT_WITH_TYPE(dtype, {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
-            const unsigned blocks = (unsigned)std::min<int64_t>(rows, 1 << 20), threads = rows <= 512 ? 1024 : 256;
+            const unsigned blocks = (unsigned)rows, threads = rows <= 512 ? 1024 : 256;
             auto both = [&](auto mode) {
                 constexpr int MODE = decltype(mode)::value;
-                sample_tiles_kernel<T, MODE><<<(unsigned)std::min<int64_t>(rows * a.tiles, 1 << 20), kTileGroups, 0, st>>>(a, row0, rows);
-                if (MODE == FEW && rows > 512 && for_a_wave<T>(a.tiles, set.k)) sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
-                else sample_pick_kernel<T, MODE><<<blocks, MODE == SORTED || MODE == ANY ? threads : 256, 0, st>>>(a, row0, rows);
+                sample_tiles_kernel<T, MODE><<<dim3((unsigned)a.tiles, blocks), kTileGroups, 0, st>>>(a, set, row0);
+                if (MODE == FEW && rows > 512 && for_a_wave<T>(a.tiles, set.k)) sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, set, row0, rows);
+                else sample_pick_kernel<T, MODE><<<blocks, MODE == PLAIN ? 256 : threads, 0, st>>>(a, set, row0, rows);
             };
             if (each) both(std::integral_constant<int, ANY>{});
             else if (set.mode == FEW) both(std::integral_constant<int, FEW>{});

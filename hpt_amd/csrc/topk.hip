@@ -26,7 +26,8 @@ bool rows_shifted(int dtype, const void* x, const Dims& kept) {
     for (int i = 0; i < kept.n; ++i) aligned = aligned && kept.stride[i] * (int64_t)dtype_size(dtype) % 16 == 0;
     return !aligned;
 }
-int64_t rows_of_run(int64_t rows, size_t row_bytes) { return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(kMostRowScratch / row_bytes))); }
+// (as many as a launch's second dim takes, too)
+int64_t rows_of_run(int64_t rows, size_t row_bytes) { return std::max<int64_t>(1, std::min<int64_t>({rows, 32768, (int64_t)(kMostRowScratch / row_bytes)})); }
 size_t topk_row_bytes(int dtype, int64_t cols, bool lse) {
     return (size_t)tiles_of(dtype, cols, true) * (kTileGroups * dtype_size(dtype) + (lse ? kTileWaves * 2 * sizeof(double) : 0));
 }
@@ -36,11 +37,11 @@ namespace {
 constexpr int kMostList = 2048;
 
 template <class T, bool LSE>
-__global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs a, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs a, int64_t row0) {
     constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
-    for (int64_t at = blockIdx.x; at < rows * a.tiles; at += gridDim.x) {
-        const int64_t row = quotient(at, a.tiles);
-        const int tile = (int)(at - row * a.tiles);
+    const int64_t row = blockIdx.y;
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+        const int64_t at = row * a.tiles + tile;
         Pack<T, VEC> p[V];
         load_tile<T>(LogitRow<T>((const T*)a.x + offset_of(a.kept, row0 + row), a.cols), tile, p);
         const uint32_t key = group_key<T>(p);
@@ -159,10 +160,11 @@ void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
-            const unsigned tiles = (unsigned)std::min<int64_t>(rows * a.tiles, 1 << 20), blocks = (unsigned)std::min<int64_t>(rows, 1 << 20);
+            const unsigned blocks = (unsigned)rows;
+            const dim3 tiles((unsigned)std::min(a.tiles, 4096), (unsigned)rows);
             auto both = [&](auto lse) {
                 constexpr bool LSE = decltype(lse)::value;
-                topk_groups_kernel<T, LSE><<<tiles, kTileGroups, 0, st>>>(a, row0, rows);
+                topk_groups_kernel<T, LSE><<<tiles, kTileGroups, 0, st>>>(a, row0);
                 if (for_a_wave<T>(a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
                 else topk_pick_kernel<T, LSE><<<blocks, rows <= 512 ? 1024 : 256, 0, st>>>(a, row0, rows);  // (few rows: more threads for each)
             };

@@ -99,29 +99,32 @@ template <class T> struct LogitRow {
         return p;
     }
 };
-// Vector b of the 32 logits that a thread has of a tile: the vectors of a tile lie thread beside thread.
-template <class T> __device__ __forceinline__ int tile_vec(int tile, int b, int thread) { return tile * (kTile * (int)sizeof(T) / 16) + b * kTileGroups + thread; }
+// Vector b of the 32 logits that a thread has of a tile: a wavefront has 2048 neighbours, and its vectors lie lane beside lane.
 template <class T> constexpr int kTileVecs = kTile * sizeof(T) / 16 / kTileGroups;  // of a thread
-// All of them: their loads are on their way together, and only a tile with an end of the row looks for it. STREAM: past the caches.
-template <class T, bool STREAM = false> __device__ __forceinline__ void load_tile(const LogitRow<T>& row, int tile, Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
+template <class T> __device__ __forceinline__ int tile_vec(int tile, int b, int thread) {
+    return (tile * (kTileGroups / 64) + (thread >> 6)) * (64 * kTileVecs<T>) + b * 64 + (thread & 63);
+}
+// All of them: their loads are on their way together, and only a tile with an end of the row looks for it.
+template <class T> __device__ __forceinline__ void load_tile(const LogitRow<T>& row, int tile, Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
     constexpr int VEC = 16 / sizeof(T);
-    const int last = row.vecs() - 1;
-#pragma unroll
-    for (int b = 0; b < kTileVecs<T>; ++b) {
-        const T* at = row.base + (int64_t)min(tile_vec<T>(tile, b, threadIdx.x), last) * VEC;
-        p[b] = STREAM ? load_pack_stream<T, VEC>(at) : load_pack<T, VEC>(at);
-    }
     if ((tile == 0 && row.lead) || (tile + 1) * (int64_t)kTile > row.end) {
+        const int last = row.vecs() - 1;
+#pragma unroll
+        for (int b = 0; b < kTileVecs<T>; ++b) p[b] = row.raw(min(tile_vec<T>(tile, b, threadIdx.x), last));
 #pragma unroll
         for (int b = 0; b < kTileVecs<T>; ++b) row.clean(p[b], tile_vec<T>(tile, b, threadIdx.x));
+    } else {
+        const T* at = row.base + (int64_t)tile_vec<T>(tile, 0, threadIdx.x) * VEC;
+#pragma unroll
+        for (int b = 0; b < kTileVecs<T>; ++b) p[b] = load_pack<T, VEC>(at + b * 64 * VEC);
     }
 }
 
 struct MaxU {
     __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a > b ? a : b; }
 };
-// A tile's logits are dealt to groups of 32 neighbours, whose largest keys its threads get one each: thread l that of the kTileVecs vectors from (l % kTileVecs) * 256 +
-// l / kTileVecs * kTileVecs on (vectors that neighbouring threads have loaded together; 64 or 128 bytes side by side, so that a group that is read again is one or two lines).
+// A tile's logits are dealt to groups of 32 neighbours, whose largest keys its threads get one each: lane l that of the kTileVecs vectors of its wavefront from
+// (l % kTileVecs) * 64 + l / kTileVecs * kTileVecs on (vectors that neighbouring lanes have loaded together; 64 or 128 bytes side by side, so that a group that is read again is one or two lines).
 // Each of 4 (8) threads gives away half of its vectors' largest for the other half of its partner's, then half of those, until one is left.
 template <class T> __device__ __forceinline__ uint32_t group_key(const Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
     const int lane = threadIdx.x & 63;
@@ -151,43 +154,58 @@ template <class T> __device__ __forceinline__ uint32_t group_key(const Pack<T, 1
 // Vector w of the group with number g of a row.
 template <class T> __device__ __forceinline__ int group_vec(uint32_t g, int w) {
     constexpr int V = kTileVecs<T>;
-    const int l = g % kTileGroups;
-    return tile_vec<T>(g / kTileGroups, l % V, l / V * V + w);
+    const int l = g % 64;
+    return g / 64 * (64 * V) + l % V * 64 + l / V * V + w;
 }
 struct SumU64 {
     __device__ static __forceinline__ uint64_t comb(uint64_t a, uint64_t b) { return a + b; }
 };
 
+// v of a lane before this one, and of lane l. (Both for all lanes that take part: a lane that is not asked has nothing to give.)
+template <class A> __device__ __forceinline__ A shfl_up_any(A v, int by) {
+    static_assert(sizeof(A) == 8, "two words");
+    union {
+        A a;
+        int w[2];
+    } in, out;
+    in.a = v;
+    out.w[0] = __shfl_up(in.w[0], by, 64);
+    out.w[1] = __shfl_up(in.w[1], by, 64);
+    return out.a;
+}
+template <class A> __device__ __forceinline__ A shfl_any(A v, int l) {
+    static_assert(sizeof(A) == 8, "two words");
+    union {
+        A a;
+        int w[2];
+    } in, out;
+    in.a = v;
+    out.w[0] = __shfl(in.w[0], l, 64);
+    out.w[1] = __shfl(in.w[1], l, 64);
+    return out.a;
+}
+// The sum of v over this lane and those before it.
+template <class A> __device__ __forceinline__ A wave_scan(A v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        const A o = shfl_up_any(v, w);
+        if (lane >= w) v += o;
+    }
+    return v;
+}
 // The sum of v over the threads before this one; `total`: over all of them. Every order is fixed. `place`: one number for each wavefront.
 __device__ __forceinline__ double scan_before(double v, double* place, double& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    double sum = v;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        union { double d; int i[2]; } in, out;
-        in.d = sum;
-        out.i[0] = __shfl_up(in.i[0], w, 64);
-        out.i[1] = __shfl_up(in.i[1], w, 64);
-        if (lane >= w) sum += out.d;
-    }
+    const double sum = wave_scan(v);
     __syncthreads();
     if (lane == 63) place[wave] = sum;
     __syncthreads();
-    double before = 0.0, all = 0.0;
-    for (int w = 0; w < waves; ++w) {
-        if (w == wave) before = all;
-        all += place[w];
-    }
-    total = all;
-    double mine;
-    {
-        union { double d; int i[2]; } in, out;
-        in.d = sum;
-        out.i[0] = __shfl_up(in.i[0], 1, 64);
-        out.i[1] = __shfl_up(in.i[1], 1, 64);
-        mine = lane ? out.d : 0.0;
-    }
-    return before + mine;
+    // (every wavefront adds them up for itself, a lane each)
+    const double upto = wave_scan(lane < waves ? place[lane] : 0.0), shifted = shfl_up_any(sum, 1);
+    total = shfl_any(upto, 63);
+    const double before = shfl_any(upto, max(wave - 1, 0));
+    return (wave ? before : 0.0) + (lane ? shifted : 0.0);
 }
 
 // Digits of eight bits: how many of what is looked at have each, in four tables that neighbouring lanes take in turn (the largest of a row's groups of logits
