@@ -5,8 +5,8 @@
 // a place of the order (key and index), and the token is the first, by index, at which the kept weights' sum is above u of their whole.
 //
 // Which token that is hangs on sums over the row: an error of 1e-7 of the sum, f32's, moves one of 10^5 borders across u in a row out of fifty. Weights and sums have 52
-// bits here: with t = x log2 e 64 / temperature and n the whole number next to it, w is 2^(n / 64), from a table of 64, times a polynomial in t - n (degree 4, 4e-14). f64
-// multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s.
+// bits here: with t = x log2 e 128 / temperature and n the whole number next to it, w is 2^(n / 128), from a table of 128, times a polynomial in t - n (degree 3, 3e-13). f64
+// multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s; it is bound by its instructions, some 17 for each logit.
 //
 // Two launches. The first takes tiles of 8192 logits and leaves, by what the row's filters need: the largest keys of its groups (top_k of at most 1024: only the first places
 // matter); the sum of the weights (no filter); or the weights' sums by size, in buckets of an eighth of a power of two, as integers, whose sum has no order (with their
@@ -20,8 +20,9 @@ namespace hpt {
 
 namespace {
 
-constexpr int kSteps = 64;                   // of a power of two
-constexpr int kBuckets = 256, kCopies = 4;   // of eight steps
+constexpr int kSteps = 128;                  // of a power of two
+constexpr int kBuckets = 256, kCopies = 4;   // of an eighth of a power of two
+constexpr int kBucketSteps = kSteps / 8;
 constexpr int kFar = kSteps * 128;           // weights below 2^-128 of the largest are 0
 constexpr int kMostList = 2048;
 
@@ -77,15 +78,17 @@ struct Settings {
 
 // ---- weights --------------------------------------------------------------------------------------
 
-// 2^(f / 64) for |f| <= 1/2, and 2^(j / 64).
+// 2^(f / 128) for |f| <= 1/2 (Taylor's polynomial, its next term by the quadratic next to it on that range), and 2^(j / 128).
 struct Powers {
-    double c[5], table[kSteps];
+    double c[4], table[kSteps];
 };
 constexpr Powers make_powers() {
-    const double l = 0.6931471805599453 / kSteps;
+    const double l = 0.6931471805599453 / kSteps, next = l * l * l * l / 24;
     Powers p{};
-    p.c[0] = 1.0;
-    for (int i = 1; i < 5; ++i) p.c[i] = p.c[i - 1] * l / i;
+    p.c[0] = 1.0 - next / 128;
+    p.c[1] = l;
+    p.c[2] = l * l / 2 + next / 4;
+    p.c[3] = l * l * l / 6;
     for (int j = 0; j < kSteps; ++j) {
         double sum = 0.0, term = 1.0;
         for (int i = 1; i < 30; ++i) {
@@ -101,44 +104,44 @@ __device__ constexpr Powers kPowers = make_powers();
 // Whole numbers next to t, in the low bits of a sum (|t| < 2^51).
 constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
 struct Weights {
-    const double* table;  // 2^(j / 64) in LDS
+    const double* table;  // 2^(j / 128) in LDS
     double steps;
-    int top;  // the low bits of the whole number that the largest's octave ends with: a multiple of 64, and 63
+    int top;  // the low bits of the whole number that the largest's octave ends with: a multiple of 128, and 127
     // `most`: the largest logit, a number. Where t would leave the whole numbers' range the steps are shortened: there, logits that differ do so by octaves beyond counting.
     __device__ __forceinline__ Weights(const double* table, float most, double steps) : table(table), steps(steps) {
         if (fabs((double)most * steps) > 0x1p49) this->steps = 0x1p49 / fabs((double)most);
         top = whole(most) | (kSteps - 1);
     }
     __device__ __forceinline__ int whole(float x) const { return (int)(uint32_t)__builtin_bit_cast(uint64_t, fma((double)x, steps, kRound)); }
-    // How many steps below the top octave's end a logit lies that is not below `lowest`; f: what the whole number leaves.
-    __device__ __forceinline__ int below(double x, double& f) const {
-        const double sum = fma(x, steps, kRound);
-        f = fma(x, steps, kRound - sum);  // (exact but for one rounding, whatever t's size)
-        return top - (int)(uint32_t)__builtin_bit_cast(uint64_t, sum);
-    }
-    // in [1, 2), or next to it
-    __device__ __forceinline__ double mantissa(int r, double f) const {
-        double v = kPowers.c[4];
+    // How many steps below the top octave's end a logit lies that is not below `lowest`, and its weight's mantissa, in [1, 2) or next to it.
+    __device__ __forceinline__ uint32_t below(double x, double& mantissa) const {
+        const double sum = fma(x, steps, kRound), f = fma(x, steps, kRound - sum);  // (exact but for one rounding, whatever t's size)
+        const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, sum);
+        double v = kPowers.c[3];
 #pragma unroll
-        for (int i = 3; i >= 0; --i) v = fma(v, f, kPowers.c[i]);
-        return v * table[(kSteps - 1) - (r & (kSteps - 1))];
+        for (int i = 2; i >= 0; --i) v = fma(v, f, kPowers.c[i]);
+        mantissa = v * table[n & (kSteps - 1)];
+        return (uint32_t)top - n;
     }
     // The lowest logit that `below` may be asked for: 96 octaves down weigh nothing. (64 bits tell it from the largest, whose t is below 2^50.)
     __device__ __forceinline__ double lowest(float most) const { return (double)most - 96.0 * kSteps / steps; }
 
     // Of any logit: steps below (kFar: at least so many), and its weight in units of the top octave.
-    __device__ __forceinline__ int below_any(float x, float most, double& f) const {
+    __device__ __forceinline__ int below_any(float x, float most) const {
         const bool far = ((double)most - (double)x) * steps >= 100.0 * kSteps;
-        const int r = below(far ? most : x, f);
-        return far ? kFar : r;
+        return far ? kFar : (int)((uint32_t)top - (uint32_t)whole(x));
     }
     __device__ __forceinline__ double of(float x, float most) const {
-        double f;
-        const int r = below_any(x, most, f);
-        return r < kFar ? shifted(mantissa(r, f), r / kSteps) : 0.0;
+        const bool far = ((double)most - (double)x) * steps >= 100.0 * kSteps;
+        double v;
+        const uint32_t r = below(far ? most : x, v);
+        return far ? 0.0 : lowered(v, r);
     }
-    // v 2^-n of a number v that is not small, by its exponent
-    static __device__ __forceinline__ double shifted(double v, int n) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v) - ((uint64_t)(uint32_t)(n << 20) << 32)); }
+    // v 2^-n for n whole octaves in r steps (of a number v that is not small), by its exponent
+    static __device__ __forceinline__ double lowered(double v, uint32_t r) {
+        static_assert(kSteps == 1 << 7, "an octave is 2^20 of the upper word");
+        return __hiloint2double((int)((uint32_t)__double2hiint(v) - ((r & ~(uint32_t)(kSteps - 1)) << (20 - 7))), __double2loint(v));
+    }
 };
 __device__ __forceinline__ void make_table(double* table) {
     if (threadIdx.x < kSteps) table[threadIdx.x] = kPowers.table[threadIdx.x];
@@ -147,9 +150,13 @@ __device__ __forceinline__ void make_table(double* table) {
 // reach a half of their sum at the half of their number.
 struct Fixed {
     double base, unit;
-    __device__ __forceinline__ explicit Fixed(int cols) : base(cols <= 1 << 18 ? 256.0 : 4096.0), unit(cols <= 1 << 18 ? 0x1p-44 : 0x1p-40) {}
+    uint32_t upper;  // of the base's words: the other is 0
+    __device__ __forceinline__ explicit Fixed(int cols) : base(cols <= 1 << 18 ? 256.0 : 4096.0), unit(cols <= 1 << 18 ? 0x1p-44 : 0x1p-40), upper(cols <= 1 << 18 ? 0x40700000u : 0x40B00000u) {}
     // 0 <= v < 2, rounded, from where it lies in the sum's mantissa
-    __device__ __forceinline__ uint64_t operator()(double v) const { return __builtin_bit_cast(uint64_t, v + base) - __builtin_bit_cast(uint64_t, base); }
+    __device__ __forceinline__ uint64_t operator()(double v) const {
+        const double sum = v + base;
+        return (uint64_t)((uint32_t)__double2hiint(sum) - upper) << 32 | (uint32_t)__double2loint(sum);
+    }
 };
 __device__ __forceinline__ double pow2(int n) { return __builtin_bit_cast(double, (uint64_t)(1023 + n) << 52); }  // |n| < 1000
 template <class T> __device__ __forceinline__ bool no_number(uint32_t key) { return key >= kInfKey<T> || key <= kNegInfKey<T>; }
@@ -197,9 +204,9 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
                 for (int b = 0; b < V; ++b)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        double f;
-                        const int r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), f);
-                        sum += Weights::shifted(w.mantissa(r, f), r / kSteps);
+                        double v;
+                        const uint32_t r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), v);
+                        sum += Weights::lowered(v, r);
                     }
                 sum = group_reduce<SumD>(sum, 64);
             }
@@ -229,11 +236,11 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
                 for (int b = 0; b < V; ++b)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        double f;
-                        const int r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), f);
-                        const int bucket = min(r >> 3, kBuckets - 1);
+                        double v;
+                        const uint32_t r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), v);
+                        const uint32_t bucket = min(r / kBucketSteps, (uint32_t)kBuckets - 1);
                         // (the last bucket holds all that is below: in units of its own octave)
-                        const double v = Weights::shifted(w.mantissa(r, f), max(r / kSteps - (kBuckets / 8 - 1), 0));
+                        v = Weights::lowered(v, __builtin_elementwise_sub_sat(r, (uint32_t)(kBuckets / 8 - 1) * kSteps));
                         __hip_atomic_fetch_add(&mass[bucket * kCopies + copy], fixed(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                         if (counted) __hip_atomic_fetch_add(&count[bucket * kCopies + copy], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
@@ -328,8 +335,7 @@ template <class T> struct Row {
     __device__ __forceinline__ uint32_t index_at(uint64_t place) const { return ((1u << index_bits) - 1) - ((uint32_t)place & ((1u << index_bits) - 1)); }
     __device__ __forceinline__ double weight(uint32_t key) const { return w.of(value_of<T>(key), most_value); }
     __device__ __forceinline__ int bucket(uint32_t key) const {
-        double f;
-        return min(w.below_any(value_of<T>(key), most_value, f) >> 3, kBuckets - 1);
+        return min(w.below_any(value_of<T>(key), most_value) / kBucketSteps, kBuckets - 1);
     }
 
     // The smallest key up to `most` of which `is` holds; it holds for `most`, and above any key of which it holds. For a wavefront, 64 keys at a time.
@@ -791,7 +797,7 @@ __global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel
                     const float v = value_of<T>(key);
                     // (what a part's largest is 96 octaves below weighs nothing, here as for a single logit)
                     if (((double)most_value - (double)v) * r.w.steps < 96.0 * kSteps) {
-                        shift = (r.w.top - (r.w.whole(v) | (kSteps - 1))) >> 3;
+                        shift = (r.w.top - (r.w.whole(v) | (kSteps - 1))) / kBucketSteps;
                         part = head(t).sum * pow2(-(shift >> 3));
                     }
                 }

@@ -47,7 +47,9 @@ __global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs
         const uint32_t key = group_key<T>(p);
         ((KeyOf<T>*)a.keys)[at * kTileGroups + threadIdx.x] = (KeyOf<T>)key;
         if constexpr (LSE) {
-            // a wavefront's part of the sum, below its own largest
+            // a wavefront's part of the sum, below its own largest (log2 e / temperature as one f32: 2^-25 of a distance D, which costs the log D / 2^25; two pieces are a sixth more
+            // instructions of a kernel that is bound by them)
+            const float steps = a.steps.hi + a.steps.lo;
             const uint32_t top = group_reduce<MaxU>(key, 64);
             float part = 0.0f;
             // (NaN, +inf and nothing but -inf are told from the largest alone)
@@ -58,8 +60,7 @@ __global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs
                 for (int b = 0; b < V; ++b)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const float d = Elem<T>::widen(p[b].v[i]) - most;
-                        part += __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo));
+                        part += __builtin_amdgcn_exp2f((Elem<T>::widen(p[b].v[i]) - most) * steps);
                     }
             }
             const double sum = group_reduce<SumD>((double)part, 64);

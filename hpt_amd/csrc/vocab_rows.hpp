@@ -125,31 +125,64 @@ struct MaxU {
 };
 // A tile's logits are dealt to groups of 32 neighbours, whose largest keys its threads get one each: lane l that of the kTileVecs vectors of its wavefront from
 // (l % kTileVecs) * 64 + l / kTileVecs * kTileVecs on (vectors that neighbouring lanes have loaded together; 64 or 128 bytes side by side, so that a group that is read again is one or two lines).
-// Each of 4 (8) threads gives away half of its vectors' largest for the other half of its partner's, then half of those, until one is left.
-template <class T> __device__ __forceinline__ uint32_t group_key(const Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
+// Each of 4 (8) lanes gives away half of its vectors' largest for the other half of its partner's, then half of those, until one is left.
+template <class A, int N, class Comb> __device__ __forceinline__ A trade(A (&m)[N], Comb&& comb) {
     const int lane = threadIdx.x & 63;
-    uint32_t m[kTileVecs<T>];
-#pragma unroll
-    for (int i = 0; i < kTileVecs<T>; ++i) m[i] = most_key<T>(p[i]);
-    if constexpr (kTileVecs<T> == 8) {
+    if constexpr (N == 8) {
         const bool upper = lane & 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t give = upper ? m[i] : m[i + 4], keep = upper ? m[i + 4] : m[i];
-            m[i] = max(keep, dpp_move<0x141>(give));  // (mirrored within eight)
+            const A give = upper ? m[i] : m[i + 4], keep = upper ? m[i + 4] : m[i];
+            m[i] = comb(keep, dpp_move<0x141>(give));  // (mirrored within eight)
         }
     }
     {
         const bool upper = lane & 2;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t give = upper ? m[i] : m[i + 2], keep = upper ? m[i + 2] : m[i];
-            m[i] = max(keep, dpp_move<0x4E>(give));
+            const A give = upper ? m[i] : m[i + 2], keep = upper ? m[i + 2] : m[i];
+            m[i] = comb(keep, dpp_move<0x4E>(give));
         }
     }
     const bool upper = lane & 1;
-    const uint32_t give = upper ? m[0] : m[1], keep = upper ? m[1] : m[0];
-    return max(keep, dpp_move<0xB1>(give));
+    const A give = upper ? m[0] : m[1], keep = upper ? m[1] : m[0];
+    return comb(keep, dpp_move<0xB1>(give));
+}
+template <class T> __device__ __forceinline__ uint32_t group_key(const Pack<T, 16 / sizeof(T)> (&p)[kTileVecs<T>]) {
+    using B = Bits<T>;
+    constexpr int V = kTileVecs<T>;
+    uint32_t m[V];
+    if constexpr (sizeof(T) == 2) {
+        // two by two, as signed numbers that order as the values do, and the lanes' halves met last; but negative NaNs, which show as the largest plain bits, take the way of single logits
+        typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 raw = {0, 0};
+#pragma unroll
+        for (int b = 0; b < V; ++b) {
+            struct Words {
+                uint32_t w[4];
+            };
+            const Words words = __builtin_bit_cast(Words, p[b]);
+            s16x2 top = {-32768, -32768};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const s16x2 s = __builtin_bit_cast(s16x2, words.w[i]);
+                top = __builtin_elementwise_max(top, s ^ ((s >> 15) & (int16_t)0x7FFF));
+                raw = __builtin_elementwise_max(raw, __builtin_bit_cast(u16x2, words.w[i]));
+            }
+            m[b] = __builtin_bit_cast(uint32_t, top);
+        }
+        if (!__any(max((uint32_t)raw.x, (uint32_t)raw.y) > (B::sign | B::inf))) {
+            const s16x2 top = __builtin_bit_cast(s16x2, trade(m, [](uint32_t a, uint32_t b) {
+                return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+            }));
+            const uint32_t key = (uint16_t)(top.x > top.y ? top.x : top.y) ^ B::sign;
+            return key > kInfKey<T> ? kNanKey<T> : key == B::sign - 1 ? B::sign : key;  // (-0 is 0)
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = most_key<T>(p[i]);
+    return trade(m, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 // Vector w of the group with number g of a row.
 template <class T> __device__ __forceinline__ int group_vec(uint32_t g, int w) {
