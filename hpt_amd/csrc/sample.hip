@@ -249,13 +249,7 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
                 const uint64_t m = (mass[threadIdx.x * 4] + mass[threadIdx.x * 4 + 1]) + (mass[threadIdx.x * 4 + 2] + mass[threadIdx.x * 4 + 3]);
                 uint32_t c = (count[threadIdx.x * 4] + count[threadIdx.x * 4 + 1]) + (count[threadIdx.x * 4 + 2] + count[threadIdx.x * 4 + 3]);
                 sum = wave_scan((double)m * fixed.unit * pow2(-(int)(threadIdx.x >> 3)));
-                if (counted) {
-#pragma unroll
-                    for (int n = 1; n < 64; n <<= 1) {
-                        const uint32_t o = __shfl_up(c, n, 64);
-                        if (lane >= n) c += o;
-                    }
-                }
+                if (counted) c = wave_scan(c);
                 if (lane == 63) {
                     sums[wave] = sum;
                     counts[wave] = c;
@@ -431,22 +425,17 @@ template <class T> struct Row {
             if ((first & ~63) * VEC < x.lead || (first - (int)(threadIdx.x & 63) + 64 * N) * VEC > x.end)
                 for (uint32_t h = hits; h; h &= h - 1)
                     if (!x.holds(element_of(first, __builtin_ctz(h)))) hits &= ~(h & -h);
-            const int mine = __builtin_popcount(hits), lane = threadIdx.x & 63;
-            int upto = mine;
-#pragma unroll
-            for (int w = 1; w < 64; w <<= 1) {
-                const int o = __shfl_up(upto, w, 64);
-                if (lane >= w) upto += o;
-            }
+            const int mine = __builtin_popcount(hits), upto = wave_scan(mine);
             uint32_t from = 0;
-            if (lane == 63 && upto) from = atomicAdd(&s.n, (uint32_t)upto);
-            uint32_t at = __shfl(from, 63, 64) + upto - mine;
+            if ((threadIdx.x & 63) == 63 && upto) from = atomicAdd(&s.n, (uint32_t)upto);
+            uint32_t at = lane_of(from, 63) + upto - mine;
+            const uint32_t lane_at = (uint32_t)first << 5;  // (a vector's number is below 2^22)
             for (; hits; hits &= hits - 1, ++at)
-                if (at < kMostList) s.list[at] = (uint32_t)element_of(first, __builtin_ctz(hits));
+                if (at < kMostList) s.list[at] = lane_at | __builtin_ctz(hits);
         });
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < min(s.n, (uint32_t)kMostList); i += blockDim.x) {
-            const int e = (int)s.list[i];
+            const int e = element_of((int)((uint32_t)s.list[i] >> 5), (int)s.list[i] & 31);
             s.list[i] = place(key_of(x.base[e]), e - x.lead);
         }
         __syncthreads();
@@ -565,19 +554,13 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
             uint32_t number_last = 0, number_before = 0;
             for (int c = 0; c < kBuckets / 64 && d < 0; ++c) {
                 const uint64_t m = wave_scan(q.mass[c * 64 + lane]) + mass;
-                uint32_t n = q.count[c * 64 + lane];
-                const bool some = n > 0;
-#pragma unroll
-                for (int w = 1; w < 64; w <<= 1) {
-                    const uint32_t o = __shfl_up(n, w, 64);
-                    if (lane >= w) n += o;
-                }
-                n += number;
+                const bool some = q.count[c * 64 + lane] > 0;
+                const uint32_t n = wave_scan(q.count[c * 64 + lane]) + number;
                 const uint64_t any = __ballot(some), reach = __ballot(some && (by_count ? q.count_before + n >= k : q.before + (double)m * unit >= target));
                 const int at = reach ? __builtin_ctzll(reach) : any ? 63 - __builtin_clzll(any) : 0;
                 // (what is before that digit)
-                const uint64_t m0 = shfl_any(m - q.mass[c * 64 + lane], at);
-                const uint32_t n0 = __shfl(n - q.count[c * 64 + lane], at, 64);
+                const uint64_t m0 = lane_of(m - q.mass[c * 64 + lane], at);
+                const uint32_t n0 = lane_of(n - q.count[c * 64 + lane], at);
                 if (any) {
                     last = c * 64 + at;
                     mass_last = m0;
@@ -586,8 +569,8 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
                 if (reach) {
                     d = last;
                 }
-                mass = shfl_any(m, 63);
-                number = __shfl(n, 63, 64);
+                mass = lane_of(m, 63);
+                number = lane_of(n, 63);
             }
             mass_before = mass_last;
             number_before = number_last;
@@ -661,8 +644,8 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
         sum += v[i];
     }
     wave_fence();
-    const double upto = wave_scan(sum), shifted = shfl_up_any(upto, 1), before = lane ? shifted : 0.0;
-    const double target = set.p * shfl_any(upto, 63), least = fmin(set.least, 1.0) * shfl_any(v[0], 0);
+    const double upto = wave_scan(sum), before = lane_before(upto);
+    const double target = set.p * lane_of(upto, 63), least = fmin(set.least, 1.0) * lane_of(v[0], 0);
     // how many are kept
     int cut = k;
 #pragma unroll
@@ -677,7 +660,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
         __device__ static __forceinline__ int comb(int a, int b) { return min(a, b); }
     };
     const int kept = group_reduce<MinI>(cut, 64);
-    const double whole = shfl_any(((kept - 1) & 1) ? before + sum : before + v[0], (kept - 1) >> 1);
+    const double whole = lane_of(((kept - 1) & 1) ? before + sum : before + v[0], (kept - 1) >> 1);
     // u's token: the last by index whose weights before it do not exceed u's part
     const double part = u * whole;
     double s0 = 0.0, s1 = 0.0;
@@ -895,10 +878,10 @@ __global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel
             const int each = (parts + 63) / 64, t0 = min(lane * each, parts), t1 = min(t0 + each, parts);
             double mine = 0.0;
             for (int t = t0; t < t1; ++t) mine += s.part[t];
-            const double upto = wave_scan(mine), whole = shfl_any(upto, 63), target = u * whole, upto_before = shfl_up_any(upto, 1);
+            const double upto = wave_scan(mine), whole = lane_of(upto, 63), target = u * whole;
             const uint64_t above = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
             const int owner = above ? __builtin_ctzll(above) : 63 - __builtin_clzll(some);
-            double before = lane ? upto_before : 0.0;
+            double before = lane_before(upto);
             int part = t0;
             for (int t = t0, last = -1; t < t1; ++t) {
                 if (s.part[t] > 0.0) {
@@ -908,8 +891,8 @@ __global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel
                     last = t;
                 }
             }
-            part = __shfl(part, owner, 64);
-            double rest = fmax(target - shfl_any(before, owner), 0.0);
+            part = lane_of(part, owner);
+            double rest = fmax(target - lane_of(before, owner), 0.0);
             // and its token there: a thread has `run` neighbours of the part
             const int size = kTile / per, run = max(size / (int)blockDim.x, VEC), e0 = part * size + (int)threadIdx.x * run;
             mine = 0.0;
@@ -929,17 +912,17 @@ __global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel
             // (the sum over the part may be a rounding off what it was chosen by)
             if (rest >= part_sum) rest = part_sum * (1.0 - 0x1p-50);
             // the wavefront in which the sum crosses it, the first thread there that does, or the last that has something
-            const double wave_before = shfl_any(here, 0), wave_upto = shfl_any(wave_scan(lane < waves ? s.place[lane] : 0.0), wave);
+            const double wave_before = lane_of(here, 0), wave_upto = lane_of(wave_scan(lane < waves ? s.place[lane] : 0.0), wave);
             if ((wave == 0 || wave_before <= rest) && wave_upto > rest) {
                 const uint64_t crosses = __ballot(mine > 0.0 && here + mine > rest), some = __ballot(mine > 0.0);
                 const int l = crosses ? __builtin_ctzll(crosses) : some ? 63 - __builtin_clzll(some) : 0;
-                const int e = __shfl(e0, l, 64) + lane;
+                const int e = lane_of(e0, l) + lane;
                 double w = 0.0;
                 if (lane < run && x.holds(e)) {
                     const T v = x.base[e];
                     if (r.place(key_of(v), e - x.lead) >= border) w = r.w.of(Elem<T>::widen(v), most_value);
                 }
-                const double from = shfl_any(here, l), sum = wave_scan(w);
+                const double from = lane_of(here, l), sum = wave_scan(w);
                 const uint64_t over = __ballot(w > 0.0 && from + sum > rest), any = __ballot(w > 0.0);
                 const int pick = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
                 if (lane == pick) answer(a, row, e - x.lead, log(fmin(w / whole, 1.0)));

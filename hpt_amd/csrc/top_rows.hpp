@@ -78,12 +78,7 @@ template <class T, int CAP> __device__ __forceinline__ void collect_by_sweeps(To
                 more += q > key;
                 same += q == key;
             }
-        uint32_t both = more | same << 16, sum = both;  // (at most 8 * 1024 of each)
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-            const uint32_t o = __shfl_up(sum, w, 64);
-            if ((int)(threadIdx.x & 63) >= w) sum += o;
-        }
+        const uint32_t both = more | same << 16, sum = wave_scan(both);  // (at most 8 * 1024 of each)
         __syncthreads();
         if ((threadIdx.x & 63) == 63) s.waves[threadIdx.x >> 6] = sum;
         __syncthreads();
@@ -111,7 +106,7 @@ template <class T, int CAP> __device__ __forceinline__ void collect_by_sweeps(To
 }
 
 // Collects into s.list (unordered) the first k places of the row and perhaps some behind them; returns how many. k <= cols, k <= CAP. Each tile's keys lie
-// side by side, `apart` bytes from the next one's. `smem`: a number for each wavefront.
+// side by side, `apart` bytes from the next one's.
 template <class T, int CAP> __device__ __forceinline__ int collect_top(TopShared<CAP>& s, const LogitRow<T>& row, const void* keys, int tiles, int k, size_t apart) {
     constexpr int VEC = 16 / sizeof(T), V = kTileVecs<T>;
     constexpr int KV = 16 / sizeof(KeyOf<T>), per = kTileGroups / KV;  // keys of a vector, vectors of a tile
@@ -307,12 +302,7 @@ template <class T> __device__ __forceinline__ int wave_top(WaveShared& s, const 
                 hits |= key[j] >= least && row.holds(e[i] + j) ? 1u << j : 0;
             }
             const int mine = __builtin_popcount(hits);
-            int upto = mine;
-#pragma unroll
-            for (int w = 1; w < 64; w <<= 1) {
-                const int o = __shfl_up(upto, w, 64);
-                if (lane >= w) upto += o;
-            }
+            const int upto = wave_scan(mine);
             int at = n + upto - mine;
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
@@ -320,7 +310,7 @@ template <class T> __device__ __forceinline__ int wave_top(WaveShared& s, const 
                     if (at < kWaveList) s.list[at] = place_of(key[j], e[i] + j - row.lead);
                     ++at;
                 }
-            n += __shfl(upto, 63, 64);
+            n += lane_of(upto, 63);
         }
     }
     wave_fence();

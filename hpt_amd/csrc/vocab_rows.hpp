@@ -190,41 +190,39 @@ template <class T> __device__ __forceinline__ int group_vec(uint32_t g, int w) {
     const int l = g % 64;
     return g / 64 * (64 * V) + l % V * 64 + l / V * V + w;
 }
-struct SumU64 {
-    __device__ static __forceinline__ uint64_t comb(uint64_t a, uint64_t b) { return a + b; }
-};
-
-// v of a lane before this one, and of lane l. (Both for all lanes that take part: a lane that is not asked has nothing to give.)
-template <class A> __device__ __forceinline__ A shfl_up_any(A v, int by) {
-    static_assert(sizeof(A) == 8, "two words");
+// v of lane l, the same l for all lanes, and of the lane before this one (0 for lane 0). By the vector unit alone, as the scan below is: through LDS each of their
+// steps would wait some 130 cycles, which a workgroup that has a row for itself cannot fill. Whole wavefronts only.
+template <class A> __device__ __forceinline__ A lane_of(A v, int l) {
     union {
         A a;
-        int w[2];
+        int w[sizeof(A) / 4];
     } in, out;
     in.a = v;
-    out.w[0] = __shfl_up(in.w[0], by, 64);
-    out.w[1] = __shfl_up(in.w[1], by, 64);
-    return out.a;
-}
-template <class A> __device__ __forceinline__ A shfl_any(A v, int l) {
-    static_assert(sizeof(A) == 8, "two words");
-    union {
-        A a;
-        int w[2];
-    } in, out;
-    in.a = v;
-    out.w[0] = __shfl(in.w[0], l, 64);
-    out.w[1] = __shfl(in.w[1], l, 64);
-    return out.a;
-}
-// The sum of v over this lane and those before it.
-template <class A> __device__ __forceinline__ A wave_scan(A v) {
-    const int lane = threadIdx.x & 63;
+    l = __builtin_amdgcn_readfirstlane(l);
 #pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        const A o = shfl_up_any(v, w);
-        if (lane >= w) v += o;
-    }
+    for (int i = 0; i < (int)sizeof(A) / 4; ++i) out.w[i] = __builtin_amdgcn_readlane(in.w[i], l);
+    return out.a;
+}
+// (along a DPP pattern, 0 where it has nothing to give or ROWS, a bit for each 16 lanes, leaves a lane out)
+template <int CTRL, int ROWS, class A> __device__ __forceinline__ A dpp_or_zero(A v) {
+    union {
+        A a;
+        int w[sizeof(A) / 4];
+    } in, out;
+    in.a = v;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(A) / 4; ++i) out.w[i] = __builtin_amdgcn_update_dpp(0, in.w[i], CTRL, ROWS, 0xF, true);
+    return out.a;
+}
+template <class A> __device__ __forceinline__ A lane_before(A v) { return dpp_or_zero<0x138, 0xF>(v); }  // wave_shr:1
+// The sum of v over this lane and those before it: within 16 lanes by shifts of 1, 2, 4, 8, then the last of a row added to the next one, and of the first two to the last two.
+template <class A> __device__ __forceinline__ A wave_scan(A v) {
+    v += dpp_or_zero<0x111, 0xF>(v);
+    v += dpp_or_zero<0x112, 0xF>(v);
+    v += dpp_or_zero<0x114, 0xF>(v);
+    v += dpp_or_zero<0x118, 0xF>(v);
+    v += dpp_or_zero<0x142, 0xA>(v);  // row_bcast:15
+    v += dpp_or_zero<0x143, 0xC>(v);  // row_bcast:31
     return v;
 }
 // The sum of v over the threads before this one; `total`: over all of them. Every order is fixed. `place`: one number for each wavefront.
@@ -235,10 +233,10 @@ __device__ __forceinline__ double scan_before(double v, double* place, double& t
     if (lane == 63) place[wave] = sum;
     __syncthreads();
     // (every wavefront adds them up for itself, a lane each)
-    const double upto = wave_scan(lane < waves ? place[lane] : 0.0), shifted = shfl_up_any(sum, 1);
-    total = shfl_any(upto, 63);
-    const double before = shfl_any(upto, max(wave - 1, 0));
-    return (wave ? before : 0.0) + (lane ? shifted : 0.0);
+    const double upto = wave_scan(lane < waves ? place[lane] : 0.0), shifted = lane_before(sum);
+    total = lane_of(upto, 63);
+    const double before = lane_of(upto, max(wave - 1, 0));
+    return (wave ? before : 0.0) + shifted;
 }
 
 // Digits of eight bits: how many of what is looked at have each, in four tables that neighbouring lanes take in turn (the largest of a row's groups of logits
@@ -259,12 +257,7 @@ struct Digits {
             c[i] = p[0] + p[1] + p[2] + p[3];
             sum += c[i];
         }
-        uint32_t upto = sum;
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-            const uint32_t o = __shfl_up(upto, w, 64);
-            if (lane >= w) upto += o;
-        }
+        const uint32_t upto = wave_scan(sum);
         const uint64_t reach = __ballot(upto >= k);
         const int at = reach ? __builtin_ctzll(reach) : 63;
         uint32_t before = upto - sum, d = 255 - lane * 4;
@@ -274,21 +267,10 @@ struct Digits {
                 before += c[i];
                 --d;
             }
-        digit = __shfl(d, at, 64);
-        above = __shfl(before, at, 64);
+        digit = lane_of(d, at);
+        above = lane_of(before, at);
     }
 };
-
-// Lanes of one wavefront, in the order of their bits: this lane's place among those that `want` one. One of them reserves them all.
-__device__ __forceinline__ uint32_t reserve(bool want, uint32_t* count) {
-    const uint64_t who = __ballot(want);
-    if (!who) return 0;
-    const int lane = threadIdx.x & 63, first = __builtin_ctzll(who);
-    uint32_t base = 0;
-    if (lane == first) base = atomicAdd(count, (uint32_t)__builtin_popcountll(who));
-    base = __shfl(base, first, 64);
-    return base + (uint32_t)__builtin_popcountll(who & ((1ull << lane) - 1));
-}
 
 // A place of the order in 64 bits.
 __device__ __forceinline__ uint64_t place_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (0xFFFFFFFFu - index); }
