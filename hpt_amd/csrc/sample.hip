@@ -21,10 +21,9 @@ namespace hpt {
 namespace {
 
 constexpr int kSteps = 128;                  // of a power of two
-constexpr int kBuckets = 256, kCopies = 4;   // of an eighth of a power of two
+constexpr int kBuckets = 256, kCopies = 8;   // of an eighth of a power of two
 constexpr int kBucketSteps = kSteps / 8;
 constexpr int kFar = kSteps * 128;           // weights below 2^-128 of the largest are 0
-constexpr int kMostList = 2048;
 
 // What a tile leaves (of each of its wavefronts' 2048 logits, where there is no filter).
 struct SampleHead {
@@ -245,9 +244,14 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
                         if (counted) __hip_atomic_fetch_add(&count[bucket * kCopies + copy], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
                 __syncthreads();
-                static_assert(kBuckets == kTileGroups && kCopies == 4, "a bucket a thread");
-                const uint64_t m = (mass[threadIdx.x * 4] + mass[threadIdx.x * 4 + 1]) + (mass[threadIdx.x * 4 + 2] + mass[threadIdx.x * 4 + 3]);
-                uint32_t c = (count[threadIdx.x * 4] + count[threadIdx.x * 4 + 1]) + (count[threadIdx.x * 4 + 2] + count[threadIdx.x * 4 + 3]);
+                static_assert(kBuckets == kTileGroups, "a bucket a thread");
+                uint64_t m = 0;
+                uint32_t c = 0;
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    m += mass[threadIdx.x * kCopies + i];
+                    c += count[threadIdx.x * kCopies + i];
+                }
                 sum = wave_scan((double)m * fixed.unit * pow2(-(int)(threadIdx.x >> 3)));
                 if (counted) c = wave_scan(c);
                 if (lane == 63) {
@@ -273,12 +277,13 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
 // ---- second launch --------------------------------------------------------------------------------
 
 constexpr int kMostParts2048 = kMostParts * kTileWaves;
-struct SortedShared {
-    uint64_t list[kMostList];
+// CAP: places collected.
+template <int CAP> struct SortedShared {
+    static constexpr int kMost = CAP;
     uint64_t mass[kBuckets];  // of a digit
     uint32_t count[kBuckets];
-    double row_mass[4 * kBuckets];  // of a bucket of the row and all above it, in the top octave's units (in four parts at first)
-    uint32_t row_count[4 * kBuckets];
+    double row_mass[kBuckets];  // of a bucket of the row and all above it, in the top octave's units
+    uint32_t row_count[kBuckets];
     uint64_t within[kMostParts];  // kept weights of a tile within the border's bucket
     uint16_t active[kMostParts];
     uint64_t few[64];
@@ -290,19 +295,27 @@ struct SortedShared {
     uint32_t count_before;
     uint64_t border;
     double reach;  // weights up to the border
+    // (last, as the largest: what lies behind 64 KB has no offset of its own in an instruction)
+    union {
+        uint64_t list[CAP];
+        struct {  // (before there is a list: the row's buckets in up to four parts)
+            double mass_part[4 * kBuckets];
+            uint32_t count_part[4 * kBuckets];
+        };
+    };
 };
 struct Nothing {};
-template <int MODE> struct PickShared {
-    union {
-        std::conditional_t<MODE == FEW || MODE == ANY, TopShared<kMostList>, Nothing> top;
-        std::conditional_t<MODE == SORTED || MODE == ANY, SortedShared, Nothing> sorted;
-    };
+template <int MODE, int CAP> struct PickShared {
     double part[MODE == FEW ? 1 : MODE == SORTED ? kMostParts : kMostParts2048];  // kept weights of a tile (or of a wavefront's part of it), in units of the row's top octave
     int shift[MODE == SORTED || MODE == ANY ? kMostParts : 1];                    // by how many buckets a tile's top octave is below the row's
     double table[kSteps], place[16];
     int pick;
     uint32_t token;
     double pick_before;
+    union {
+        std::conditional_t<MODE == FEW || MODE == ANY, TopShared<2048>, Nothing> top;
+        std::conditional_t<MODE == SORTED || MODE == ANY, SortedShared<CAP>, Nothing> sorted;
+    };
 };
 
 // Writes a row's answer.
@@ -357,7 +370,7 @@ template <class T> struct Row {
     __device__ __forceinline__ uint32_t last_key_of(int b) const { return bucket(most) == b ? most : first_key_of(b - 1) - 1; }
 
     // Calls f(first vector of a lane, its bits) for every 2048 logits of the tiles of s.active, a wavefront each: the bits tell which of a lane's 32 have keys in klo ... khi.
-    template <class F> __device__ __forceinline__ void each_piece(const SortedShared& s, uint32_t klo, uint32_t khi, F&& f) const {
+    template <class Q, class F> __device__ __forceinline__ void each_piece(const Q& s, uint32_t klo, uint32_t khi, F&& f) const {
         const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, all = (int)s.n_active * kTileWaves, last = x.vecs() - 1;
         if (all == 0) return;
         auto first_vec = [&](int i) { return (s.active[min(i, all - 1) / kTileWaves] * kTileWaves + min(i, all - 1) % kTileWaves) * (64 * N) + lane; };
@@ -415,8 +428,8 @@ template <class T> struct Row {
         const int m = sizeof(T) == 2 ? 2 * (15 - (bit & 15)) + (bit >> 4) : 31 - bit;
         return (first_vec + m / VEC * 64) * VEC + m % VEC;
     }
-    // Collects into s.list the places of a range of keys; s.n: how many, of which only the first kMostList are there.
-    __device__ __forceinline__ void collect(SortedShared& s, uint32_t klo, uint32_t khi) const {
+    // Collects into s.list the places of a range of keys; s.n: how many, of which only as many as it holds are there.
+    template <class Q> __device__ __forceinline__ void collect(Q& s, uint32_t klo, uint32_t khi) const {
         __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
@@ -431,17 +444,17 @@ template <class T> struct Row {
             uint32_t at = lane_of(from, 63) + upto - mine;
             const uint32_t lane_at = (uint32_t)first << 5;  // (a vector's number is below 2^22)
             for (; hits; hits &= hits - 1, ++at)
-                if (at < kMostList) s.list[at] = lane_at | __builtin_ctz(hits);
+                if (at < Q::kMost) s.list[at] = lane_at | __builtin_ctz(hits);
         });
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < min(s.n, (uint32_t)kMostList); i += blockDim.x) {
+        for (uint32_t i = threadIdx.x; i < min(s.n, (uint32_t)Q::kMost); i += blockDim.x) {
             const int e = element_of((int)((uint32_t)s.list[i] >> 5), (int)s.list[i] & 31);
             s.list[i] = place(key_of(x.base[e]), e - x.lead);
         }
         __syncthreads();
     }
     // Calls f(place, value) of every logit whose place is in lo ... hi.
-    template <class F> __device__ __forceinline__ void sweep(const SortedShared& s, uint64_t lo, uint64_t hi, F&& f) const {
+    template <class Q, class F> __device__ __forceinline__ void sweep(const Q& s, uint64_t lo, uint64_t hi, F&& f) const {
         each_piece(s, key_at(lo), key_at(hi), [&](int first, uint32_t hits) {
             for (; hits; hits &= hits - 1) {
                 const int e = element_of(first, __builtin_ctz(hits));
@@ -456,7 +469,7 @@ template <class T> struct Row {
 
 // The tiles that have logits in a bucket of the row.
 template <class T, class Shared> __device__ __forceinline__ void find_active(const Row<T>& r, Shared& s, int bucket) {
-    SortedShared& q = s.sorted;
+    auto& q = s.sorted;
     __syncthreads();
     if (threadIdx.x == 0) q.n_active = 0;
     __syncthreads();
@@ -471,7 +484,8 @@ template <class T, class Shared> __device__ __forceinline__ void find_active(con
 
 // The border: the first place of the order at which the number of tokens reaches `k` (by_count) or their weights reach `target`. Returns the place, in s.sorted.reach the weights up to it. `listed`: the bucket whose logits s.sorted.list holds, all of them, q.n in number.
 template <class T, class Shared> __device__ __forceinline__ uint64_t find_border(const Row<T>& r, Shared& s, bool by_count, uint32_t k, double target, int& listed) {
-    SortedShared& q = s.sorted;
+    auto& q = s.sorted;
+    constexpr int kMostList = std::remove_reference_t<decltype(q)>::kMost;
     const int lane = threadIdx.x & 63;
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -601,7 +615,6 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
         const uint64_t m = lane < left ? weight(value_of<T>(r.key_at(mine))) : 0;
         uint64_t upto = 0;
         uint32_t number = 0;
-#pragma unroll 4
         for (int j = 0; j < left; ++j) {
             const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
             const uint64_t om = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)m, j);
@@ -678,10 +691,11 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
     if (token == best && best) answer(a, row, best - 1, log((index[0] + 1 == best ? v[0] : v[1]) / whole));
 }
 
-template <class T, int MODE>
-__global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
+// THREADS: at most. Few rows have larger workgroups, and room for more of a bucket.
+template <class T, int MODE, int THREADS>
+__global__ __launch_bounds__(THREADS, MODE == SORTED ? 4 : 1) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ PickShared<MODE> s;
+    __shared__ PickShared<MODE, THREADS == 1024 ? 8192 : 2048> s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     make_table(s.table);
     for (int64_t at = blockIdx.x; at < rows; at += gridDim.x) {
@@ -789,7 +803,7 @@ __global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel
             }
             if constexpr (MODE == SORTED || MODE == ANY) {
                 if (mode == SORTED) {
-                    SortedShared& q = s.sorted;
+                    auto& q = s.sorted;
                     const bool counted = set.k < a.cols;
                     __syncthreads();
                     // the row's buckets: those of its tiles, dealt to up to four threads a bucket
@@ -809,16 +823,16 @@ __global__ __launch_bounds__(MODE == PLAIN ? 256 : 1024) void sample_pick_kernel
                             const uint32_t c = tiles[t].count[max(b - shift, 0)];
                             number += b >= shift ? c : 0;
                         }
-                    q.row_mass[threadIdx.x] = mine;
-                    q.row_count[threadIdx.x] = number;
+                    q.mass_part[threadIdx.x] = mine;
+                    q.count_part[threadIdx.x] = number;
                     double all = 0.0;  // (the same in every wavefront)
                     for (int t = lane; t < a.tiles; t += 64) all += s.part[t];
                     all = group_reduce<SumD>(all, 64);
                     __syncthreads();
                     if (threadIdx.x < kBuckets) {
                         for (int i = 1; i < quarters; ++i) {
-                            mine += q.row_mass[threadIdx.x + i * kBuckets];
-                            number += q.row_count[threadIdx.x + i * kBuckets];
+                            mine += q.mass_part[threadIdx.x + i * kBuckets];
+                            number += q.count_part[threadIdx.x + i * kBuckets];
                         }
                         // (the last bucket has all the rest)
                         q.row_mass[threadIdx.x] = b == kBuckets - 1 ? all : fmin(mine, all);
@@ -981,12 +995,20 @@ void launch_sample(int dtype, const SampleArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
-            const unsigned blocks = (unsigned)rows, threads = rows <= 512 ? 1024 : 256;
+            const unsigned blocks = (unsigned)rows;
+            const bool many = rows > 512;
             auto both = [&](auto mode) {
                 constexpr int MODE = decltype(mode)::value;
                 sample_tiles_kernel<T, MODE><<<dim3((unsigned)a.tiles, blocks), kTileGroups, 0, st>>>(a, set, row0);
-                if (MODE == FEW && rows > 512 && for_a_wave<T>(a.tiles, set.k)) sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, set, row0, rows);
-                else sample_pick_kernel<T, MODE><<<blocks, MODE == PLAIN ? 256 : threads, 0, st>>>(a, set, row0, rows);
+                if constexpr (MODE == PLAIN) {
+                    sample_pick_kernel<T, MODE, 256><<<blocks, 256, 0, st>>>(a, set, row0, rows);
+                } else {
+                    if constexpr (MODE == FEW)
+                        if (many && for_a_wave<T>(a.tiles, set.k)) return sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, set, row0, rows);
+                    if constexpr (MODE == SORTED)
+                        if (many) return sample_pick_kernel<T, MODE, 256><<<blocks, 256, 0, st>>>(a, set, row0, rows);
+                    sample_pick_kernel<T, MODE, 1024><<<blocks, many ? 256 : 1024, 0, st>>>(a, set, row0, rows);
+                }
             };
             if (each) both(std::integral_constant<int, ANY>{});
             else if (set.mode == FEW) both(std::integral_constant<int, FEW>{});
