@@ -17,8 +17,10 @@ namespace hpt {
 template <int CAP> struct TopShared {
     uint64_t list[CAP];
     uint32_t groups[CAP];  // those that are read again
+    uint16_t by_digit[CAP];
     Digits digits;
     uint32_t count, many, digit, above;
+    uint32_t most, least;  // no collected key is above or below
     uint32_t waves[2 * 16];
 };
 
@@ -102,6 +104,7 @@ template <class T, int CAP> __device__ __forceinline__ void collect_by_sweeps(To
         over += all & 0xFFFF;
         equal += all >> 16;
     }
+    if (threadIdx.x == 0) s.least = key;
     __syncthreads();
 }
 
@@ -161,26 +164,41 @@ template <class T, int CAP> __device__ __forceinline__ int collect_top(TopShared
     }
     __syncthreads();
     const int many = (int)s.many;
+    if (threadIdx.x == 0) {
+        s.most = most;
+        s.least = least;
+    }
     if (many <= CAP) {
+        // (four vectors of a thread on their way together)
 #pragma clang loop unroll(disable)
-        for (int w = threadIdx.x; w < many * V; w += threads) {
-            const int v = group_vec<T>(s.groups[w / V], w % V), e = v * VEC;
-            if (e >= row.end) continue;
-            const Pack<T, VEC> p = row.raw(v);
-            uint32_t key[VEC], hits = 0;
+        for (int w0 = threadIdx.x; w0 < many * V; w0 += 4 * threads) {
+            Pack<T, VEC> p[4];
+            int at[4];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                key[i] = key_of(p.v[i]);
-                hits |= key[i] >= least && row.holds(e + i) ? 1u << i : 0;
+            for (int n = 0; n < 4; ++n) {
+                const int w = w0 + n * threads, v = group_vec<T>(s.groups[min(w / V, many - 1)], w % V);
+                at[n] = w < many * V ? v * VEC : row.end;
+                p[n] = row.raw(min(v, row.vecs() - 1));
             }
-            if (hits) {
-                uint32_t at = atomicAdd(&s.count, (uint32_t)__builtin_popcount(hits));
 #pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    if (hits >> i & 1) {
-                        if (at < CAP) s.list[at] = place_of(key[i], e + i - row.lead);
-                        ++at;
-                    }
+            for (int n = 0; n < 4; ++n) {
+                const int e = at[n];
+                if (e >= row.end) continue;
+                uint32_t key[VEC], hits = 0;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    key[i] = key_of(p[n].v[i]);
+                    hits |= key[i] >= least && row.holds(e + i) ? 1u << i : 0;
+                }
+                if (hits) {
+                    uint32_t at = atomicAdd(&s.count, (uint32_t)__builtin_popcount(hits));
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        if (hits >> i & 1) {
+                            if (at < CAP) s.list[at] = place_of(key[i], e + i - row.lead);
+                            ++at;
+                        }
+                }
             }
         }
         __syncthreads();
@@ -328,10 +346,11 @@ template <class Out> __device__ __forceinline__ void wave_rank(const WaveShared&
     }
 }
 
-// Gives each of the first k of `n` collected places to `out(rank, place)`, the ranks counted from 0. Up to kMostRanked of them a thread counts what is before its own; beyond they are sorted.
-constexpr int kMostRanked = 512;
+// Gives each of the first k of `n` collected places to `out(rank, place)`, the ranks counted from 0. Up to kMostRanked of them a thread counts what is before its own. Of more it
+// counts only those of its own digit: eight bits below the largest key, which deal them out first. They are sorted where one digit has too many (keys that are equal).
+constexpr int kMostRanked = 128, kMostOfDigit = 256;
 template <int CAP, class Out> __device__ __forceinline__ void rank_top(TopShared<CAP>& s, int n, int k, Out&& out) {
-    if (CAP <= kMostRanked || n <= kMostRanked) {
+    if (n <= kMostRanked) {
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
             const uint64_t mine = s.list[i];
             int rank = 0;
@@ -341,7 +360,47 @@ template <int CAP, class Out> __device__ __forceinline__ void rank_top(TopShared
         }
         return;
     }
-    int size = 1024;
+    uint32_t *upto = s.digits.n, *from = upto + 256;  // where a digit's places end (so far) and begin
+    const uint32_t most = s.most, width = most - s.least, shift = width < 256 ? 0 : 24 - __builtin_clz(width);
+    auto digit = [&](uint64_t place) { return (most - key_of_place(place)) >> shift; };
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) upto[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) atomicAdd(&upto[digit(s.list[i])], 1u);
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        uint32_t c[4], sum = 0, largest = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            c[i] = upto[threadIdx.x * 4 + i];
+            sum += c[i];
+            largest = max(largest, c[i]);
+        }
+        largest = group_reduce<MaxU>(largest, 64);
+        uint32_t at = wave_scan(sum) - sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            upto[threadIdx.x * 4 + i] = from[threadIdx.x * 4 + i] = at;
+            at += c[i];
+        }
+        if (threadIdx.x == 0) s.many = largest;
+    }
+    __syncthreads();
+    if (s.many <= kMostOfDigit) {
+        for (int i = threadIdx.x; i < n; i += blockDim.x) s.by_digit[atomicAdd(&upto[digit(s.list[i])], 1u)] = (uint16_t)i;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
+            const uint64_t mine = s.list[i];
+            const uint32_t d = digit(mine), end = upto[d];
+            uint32_t rank = from[d];
+            if (rank >= (uint32_t)k) continue;
+#pragma unroll 4
+            for (uint32_t j = rank, all = end; j < all; ++j) rank += s.list[s.by_digit[j]] > mine;
+            if (rank < (uint32_t)k) out(rank, mine);
+        }
+        return;
+    }
+    int size = 256;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += blockDim.x) s.list[i] = 0;
     sort_places(s.list, size);
