@@ -105,41 +105,42 @@ constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
 struct Weights {
     const double* table;  // 2^(j / 128) in LDS
     double steps;
-    int top;  // the low bits of the whole number that the largest's octave ends with: a multiple of 128, and 127
+    double round;  // kRound less the whole number that the largest's octave begins with, a multiple of 128: sums with it have steps above that in their low bits
     // `most`: the largest logit, a number. Where t would leave the whole numbers' range the steps are shortened: there, logits that differ do so by octaves beyond counting.
     __device__ __forceinline__ Weights(const double* table, float most, double steps) : table(table), steps(steps) {
         if (fabs((double)most * steps) > 0x1p49) this->steps = 0x1p49 / fabs((double)most);
-        top = whole(most) | (kSteps - 1);
+        round = kRound - floor((fma((double)most, this->steps, kRound) - kRound) / kSteps) * kSteps;
     }
-    __device__ __forceinline__ int whole(float x) const { return (int)(uint32_t)__builtin_bit_cast(uint64_t, fma((double)x, steps, kRound)); }
-    // How many steps below the top octave's end a logit lies that is not below `lowest`, and its weight's mantissa, in [1, 2) or next to it.
-    __device__ __forceinline__ uint32_t below(double x, double& mantissa) const {
-        const double sum = fma(x, steps, kRound), f = fma(x, steps, kRound - sum);  // (exact but for one rounding, whatever t's size)
-        const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, sum);
+    // Steps above the beginning of the largest's octave: 0 to 127 within it, negative below.
+    __device__ __forceinline__ int above(float x) const { return (int)(uint32_t)__builtin_bit_cast(uint64_t, fma((double)x, steps, round)); }
+    // Likewise of a logit that is not below `lowest`, and its weight's mantissa, in [1, 2) or next to it.
+    __device__ __forceinline__ int above(double x, double& mantissa) const {
+        const double sum = fma(x, steps, round), f = fma(x, steps, round - sum);  // (exact but for one rounding, whatever t's size)
+        const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, sum);
         double v = kPowers.c[3];
 #pragma unroll
         for (int i = 2; i >= 0; --i) v = fma(v, f, kPowers.c[i]);
         mantissa = v * table[n & (kSteps - 1)];
-        return (uint32_t)top - n;
+        return n;
     }
-    // The lowest logit that `below` may be asked for: 96 octaves down weigh nothing. (64 bits tell it from the largest, whose t is below 2^50.)
+    // The lowest logit that `above` may be asked for: 96 octaves down weigh nothing. (64 bits tell it from the largest, whose t is below 2^50.)
     __device__ __forceinline__ double lowest(float most) const { return (double)most - 96.0 * kSteps / steps; }
 
-    // Of any logit: steps below (kFar: at least so many), and its weight in units of the top octave.
+    // Of any logit: how many steps below the top octave's end (kFar: at least so many), and its weight in units of the top octave.
     __device__ __forceinline__ int below_any(float x, float most) const {
         const bool far = ((double)most - (double)x) * steps >= 100.0 * kSteps;
-        return far ? kFar : (int)((uint32_t)top - (uint32_t)whole(x));
+        return far ? kFar : kSteps - 1 - above(x);
     }
     __device__ __forceinline__ double of(float x, float most) const {
         const bool far = ((double)most - (double)x) * steps >= 100.0 * kSteps;
         double v;
-        const uint32_t r = below(far ? most : x, v);
-        return far ? 0.0 : lowered(v, r);
+        const int n = above(far ? most : x, v);
+        return far ? 0.0 : moved(v, n);
     }
-    // v 2^-n for n whole octaves in r steps (of a number v that is not small), by its exponent
-    static __device__ __forceinline__ double lowered(double v, uint32_t r) {
+    // v 2^(n / 128), rounded down to whole octaves (of a number v that is not small), by its exponent
+    static __device__ __forceinline__ double moved(double v, int n) {
         static_assert(kSteps == 1 << 7, "an octave is 2^20 of the upper word");
-        return __hiloint2double((int)((uint32_t)__double2hiint(v) - ((r & ~(uint32_t)(kSteps - 1)) << (20 - 7))), __double2loint(v));
+        return __hiloint2double((int)((uint32_t)__double2hiint(v) + ((uint32_t)(n & ~(kSteps - 1)) << (20 - 7))), __double2loint(v));
     }
 };
 __device__ __forceinline__ void make_table(double* table) {
@@ -204,8 +205,8 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
                         double v;
-                        const uint32_t r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), v);
-                        sum += Weights::lowered(v, r);
+                        const int n = w.above(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), v);
+                        sum += Weights::moved(v, n);
                     }
                 sum = group_reduce<SumD>(sum, 64);
             }
@@ -236,10 +237,10 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
                         double v;
-                        const uint32_t r = w.below(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), v);
-                        const uint32_t bucket = min(r / kBucketSteps, (uint32_t)kBuckets - 1);
+                        const int n = w.above(fmax((double)Elem<T>::widen(p[b].v[i]), lowest), v);
+                        const uint32_t bucket = min((uint32_t)(kSteps - 1 - n) / kBucketSteps, (uint32_t)kBuckets - 1);
                         // (the last bucket holds all that is below: in units of its own octave)
-                        v = Weights::lowered(v, __builtin_elementwise_sub_sat(r, (uint32_t)(kBuckets / 8 - 1) * kSteps));
+                        v = Weights::moved(v, min(n + (kBuckets / 8 - 1) * kSteps, 0));
                         __hip_atomic_fetch_add(&mass[bucket * kCopies + copy], fixed(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                         if (counted) __hip_atomic_fetch_add(&count[bucket * kCopies + copy], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
@@ -794,7 +795,7 @@ __global__ __launch_bounds__(THREADS, MODE == SORTED ? 4 : 1) void sample_pick_k
                     const float v = value_of<T>(key);
                     // (what a part's largest is 96 octaves below weighs nothing, here as for a single logit)
                     if (((double)most_value - (double)v) * r.w.steps < 96.0 * kSteps) {
-                        shift = (r.w.top - (r.w.whole(v) | (kSteps - 1))) / kBucketSteps;
+                        shift = -(r.w.above(v) >> 7) * 8;
                         part = head(t).sum * pow2(-(shift >> 3));
                     }
                 }
