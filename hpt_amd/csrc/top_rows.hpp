@@ -362,7 +362,7 @@ template <int CAP, class Out> __device__ __forceinline__ void rank_top(TopShared
     }
     uint32_t *upto = s.digits.n, *from = upto + 256;  // where a digit's places end (so far) and begin
     const uint32_t most = s.most, width = most - s.least, shift = width < 256 ? 0 : 24 - __builtin_clz(width);
-    auto digit = [&](uint64_t place) { return (most - key_of_place(place)) >> shift; };
+    auto digit = [&](uint64_t place) { return min((most - key_of_place(place)) >> shift, 255u); };
     __syncthreads();
     for (int i = threadIdx.x; i < 256; i += blockDim.x) upto[i] = 0;
     __syncthreads();

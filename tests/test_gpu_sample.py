@@ -180,3 +180,45 @@ def test_more_rows_than_a_run(hpt, dev):
     u = rng.uniform(size=7).astype(np.float32)
     token = v.sample(up(hpt, np.tile(u, rep)), top_p=0.8)[0].numpy()
     assert np.array_equal(token, np.broadcast_to([sampled(x[r], u[r], top_p=0.8)[0] for r in range(7)], (rep, 7)))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("each", [False, True])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=20, top_p=0.8), dict(top_k=600, min_p=0.01), dict(top_p=0.9), dict(min_p=0.05), dict(top_k=3000, top_p=0.9), dict(temperature=0.0)], ids=str)
+def test_many_rows(hpt, dev, name, each, settings):
+    """More rows than the forms for few rows take: the same twenty again and again, of which some have few values or masks."""
+    kind, rng, cols, rep = Kind(hpt, name), np.random.default_rng(8), 20001, 40
+    x = rng.standard_normal((20, cols)) * 3
+    x[3] = rng.integers(-2, 3, cols)
+    x[7] = 1.5
+    x[9, cols // 9:] = -np.inf
+    x[11, :-3] = -65504.0
+    x[13, cols // 2] = np.nan
+    x[17] = -np.inf
+    t, x = kind.up(x)
+    u = rng.uniform(size=20).astype(np.float32)
+    want = [sampled(x[r], u[r], **settings) for r in range(20)]
+    clear = np.array([w[2] > NEAR for w in want])
+    assert clear.sum() >= 18
+    v = hpt.Tensor.from_raw(t.ptr, [rep, 20, cols], kind.dtype, 0, [0, cols, 1])
+    if each:
+        full = dict(dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **settings)
+        settings = {n: up(hpt, np.full(rep * 20, a, np.int64 if n == "top_k" else np.float32)) for n, a in full.items()}
+        # (a setting of f32 is not quite the number in 64 bits: what it is decides)
+        want = [sampled(x[r], u[r], **{n: int(a) if n == "top_k" else float(np.float32(a)) for n, a in full.items()}) for r in range(20)]
+        clear = np.array([w[2] > NEAR for w in want])
+    token, logp = v.sample(up(hpt, np.tile(u, rep)), **settings)
+    token, logp = token.numpy().reshape(rep, 20), logp.numpy().reshape(rep, 20).astype(np.float64)
+    assert (token == token[:1]).all() and np.array_equal(logp, np.broadcast_to(logp[:1], logp.shape), equal_nan=True)
+    tokens, logs = np.array([w[0] for w in want]), np.array([w[1] for w in want])
+    assert np.array_equal(token[0][clear], tokens[clear])
+    near(logp[0][clear], logs[clear], F32_STEP * np.abs(logs[clear]) + 1e-11)
+
+
+def test_a_bucket_of_many(hpt, dev):
+    """More logits within an eighth of a power of two of the weights than a list holds, none like another, at the border."""
+    rng, cols = np.random.default_rng(9), 120000
+    x = np.concatenate([rng.uniform(0, 0.08, (2, 40000)), rng.uniform(-9, -3, (2, cols - 40000))], 1)
+    t, x = Kind(hpt, "f32").up(np.stack([rng.permutation(r) for r in x]))
+    for settings in (dict(top_p=0.5), dict(top_k=20000), dict(top_k=20000, top_p=0.3), dict(min_p=0.97)):
+        check(hpt, t, x, np.array([0.4, 0.9], np.float32), settings)

@@ -134,3 +134,26 @@ def test_more_rows_than_a_run(hpt, dev, cols):
     assert hpt.topk_workspace(v, 5) < rep * 7 * row
     index = v.topk(5)[1].numpy()
     assert np.array_equal(index, np.broadcast_to(order(x)[:, :5], (rep, 7, 5)))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("k", [3, 64, 128, 200, 513, 1024])
+def test_many_rows(hpt, dev, name, k):
+    """More rows than the form for few rows takes: rows of few values and masks among others, again and again."""
+    kind, rng, cols, rep = Kind(hpt, name), np.random.default_rng(k), 20001, 30
+    ties = rows_that_tie(rng, cols)
+    # (places that differ by their index alone but for a few: more than the digits of a key can tell apart)
+    near_same = 1.0 + (rng.uniform(size=(2, cols)) < 0.02) * 2.0 ** -7 * np.array([[1.0], [2.0]])
+    t, x = kind.up(np.concatenate([ties, near_same, rng.standard_normal((12, cols)) * 3]))
+    n = x.shape[0]
+    v = hpt.Tensor.from_raw(t.ptr, [rep, n, cols], kind.dtype, 0, [0, cols, 1])
+    values, index, lse = v.topk(k, lse=True)
+    want = order(x)[:, :k]
+    assert np.array_equal(index.numpy(), np.broadcast_to(want, (rep, n, k)))
+    assert np.array_equal(values.numpy(), np.broadcast_to(kind.store(np.take_along_axis(x, want, -1)), (rep, n, k)), equal_nan=name != "bf16")
+    few = t.topk(k, lse=True)
+    assert np.array_equal(few[1].numpy(), want)
+    got, nan = lse.numpy().astype(np.float64), np.isnan(x).any(-1)
+    exact = np.where(nan, np.nan, logsumexp(np.where(np.isnan(x), 0, x)))
+    near(got[0], exact, LSE + F32_STEP * np.abs(np.where(np.isfinite(exact), exact, 0)))
+    assert np.array_equal(got, np.broadcast_to(got[:1], got.shape), equal_nan=True)
