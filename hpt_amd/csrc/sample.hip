@@ -311,7 +311,6 @@ template <int MODE, int CAP> struct PickShared {
     int shift[MODE == SORTED || MODE == ANY ? kMostParts : 1];                    // by how many buckets a tile's top octave is below the row's
     double table[kSteps], place[16];
     int pick;
-    uint32_t token;
     double pick_before;
     union {
         std::conditional_t<MODE == FEW || MODE == ANY, TopShared<2048>, Nothing> top;
@@ -756,20 +755,51 @@ __global__ __launch_bounds__(THREADS, MODE == SORTED ? 4 : 1) void sample_pick_k
                     upto += weight[i];
                     if (i == kept - 1) s.pick_before = upto;
                 }
-                if (threadIdx.x == 0) s.token = 0;
                 __syncthreads();
-                // u's token: the last by index whose weights before it do not exceed u's part
+                // u's token, by eight bits of the index at a time, from sums of whole numbers of 2^-50, which have no order (every wavefront looks for itself)
                 const double part = u * s.pick_before;
-                for (int i = threadIdx.x; i < kept; i += blockDim.x) {
-                    const uint32_t index = index_of(order[i]);
-                    double sum = 0.0;
-#pragma unroll 4
-                    for (int j = 0; j < kept; ++j) sum += index_of(order[j]) < index ? weight[j] : 0.0;
-                    if (weight[i] > 0.0 && sum <= part) atomicMax(&s.token, index + 1);
+                uint64_t* mass = (uint64_t*)s.top.digits.n;
+                static_assert(sizeof s.top.digits.n >= 256 * sizeof(uint64_t), "");
+                uint32_t prefix = 0;
+                uint64_t upto_prefix = 0;
+#pragma clang loop unroll(disable)
+                for (int shift = a.cols > 1 << 16 ? 16 : a.cols > 1 << 8 ? 8 : 0; shift >= 0; shift -= 8) {
+                    for (int i = threadIdx.x; i < 256; i += blockDim.x) mass[i] = 0;
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < kept; i += blockDim.x) {
+                        const uint32_t index = index_of(order[i]);
+                        if (index >> (shift + 8) == prefix)
+                            __hip_atomic_fetch_add(&mass[index >> shift & 255], __builtin_bit_cast(uint64_t, weight[i] + 4.0) - __builtin_bit_cast(uint64_t, 4.0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    }
+                    __syncthreads();
+                    // the first digit at which the sum exceeds u's part, or the last that has something
+                    uint64_t m[4], sum = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        m[i] = mass[lane * 4 + i];
+                        sum += m[i];
+                    }
+                    const uint64_t end = wave_scan(sum) + upto_prefix;
+                    const uint64_t over = __ballot(sum > 0 && (double)end * 0x1p-50 > part), some = __ballot(sum > 0);
+                    const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+                    uint64_t before = end - sum, from = before;
+                    int digit = 0;
+                    bool done = false;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (m[i] > 0 && !done) {
+                            digit = lane * 4 + i;
+                            from = before;
+                            done = (double)(before + m[i]) * 0x1p-50 > part;
+                        }
+                        before += m[i];
+                    }
+                    prefix = prefix << 8 | lane_of((uint32_t)digit, l);
+                    upto_prefix = lane_of(from, l);
+                    __syncthreads();
                 }
-                __syncthreads();
                 for (int i = threadIdx.x; i < kept; i += blockDim.x)
-                    if (index_of(order[i]) + 1 == s.token) answer(a, row, s.token - 1, log(weight[i] / s.pick_before));
+                    if (index_of(order[i]) == prefix) answer(a, row, prefix, log(weight[i] / s.pick_before));
                 continue;
             }
         }
@@ -1006,7 +1036,7 @@ void launch_sample(int dtype, const SampleArgs& a, hipStream_t st) {
                 } else {
                     if constexpr (MODE == FEW)
                         if (many && for_a_wave<T>(a.tiles, set.k)) return sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, set, row0, rows);
-                    if constexpr (MODE == SORTED)
+                    if constexpr (MODE != FEW)
                         if (many) return sample_pick_kernel<T, MODE, 256><<<blocks, 256, 0, st>>>(a, set, row0, rows);
                     sample_pick_kernel<T, MODE, 1024><<<blocks, many ? 256 : 1024, 0, st>>>(a, set, row0, rows);
                 }

@@ -242,7 +242,7 @@ __device__ __forceinline__ double scan_before(double v, double* place, double& t
 // Digits of eight bits: how many of what is looked at have each, in four tables that neighbouring lanes take in turn (the largest of a row's groups of logits
 // have nearly all the same first digit, and lanes that add to one address wait for each other).
 struct Digits {
-    uint32_t n[256 * 4];
+    alignas(16) uint32_t n[256 * 4];
     __device__ __forceinline__ void clear() {
         for (int i = threadIdx.x; i < 256 * 4; i += blockDim.x) n[i] = 0;
     }
