@@ -693,7 +693,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
 
 // THREADS: at most. Few rows have larger workgroups, and room for more of a bucket.
 template <class T, int MODE, int THREADS>
-__global__ __launch_bounds__(THREADS, MODE == SORTED ? 4 : 1) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == PLAIN ? 1 : 3) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ PickShared<MODE, THREADS == 1024 ? 8192 : 2048> s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;

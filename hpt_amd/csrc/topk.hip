@@ -2,7 +2,10 @@
 //
 // Two launches. The first reads the logits once, in tiles of 8192: the largest key of each 32 neighbours stays (and, where the sum is wanted, a wavefront
 // adds the exponentials of its 2048 below their largest). The second has a workgroup for each row, which finds the first k places from those keys (top_rows.hpp).
-// The first is bound by memory, the second by the latency of its steps.
+// The second is bound by the latency of its steps.
+//
+// The first reads bf16 [4096, 50257] in 68 us (6.0 TB/s) without the sum; with it the launch is bound by its instructions, five for each logit, 88 to 92 us (4.6 TB/s). The second takes 35 of k = 64
+// there (by wavefronts), 9.7 of one row of 152000 and of 37 of 50257, 19.5 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
 #include <algorithm>
 #include <cmath>
 
@@ -155,10 +158,94 @@ __global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a
     }
 }
 
+// Rows of at most 64 N elements, a wavefront each, one launch: the row stays in registers (element i of lane l is at 64 i + l), and the largest is taken out k times.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, dpp_or_zero<0x111, 0xF>(v));
+    v = max(v, dpp_or_zero<0x112, 0xF>(v));
+    v = max(v, dpp_or_zero<0x114, 0xF>(v));
+    v = max(v, dpp_or_zero<0x118, 0xF>(v));
+    v = max(v, dpp_or_zero<0x142, 0xA>(v));
+    v = max(v, dpp_or_zero<0x143, 0xC>(v));
+    return lane_of(v, 63);
+}
+template <class T, int N, bool LSE>
+__global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows; row += (int64_t)gridDim.x * 4) {
+        const T* x = (const T*)a.x + offset_of(a.kept, row);
+        T v[N];
+        uint32_t key[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = x[min(i * 64 + lane, a.cols - 1)];
+#pragma unroll
+        for (int i = 0; i < N; ++i) key[i] = i * 64 + lane < a.cols ? key_of(v[i]) : 0;
+        uint32_t best = 0;
+        int which = 0;
+        auto find = [&] {
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (key[i] > best) {
+                    best = key[i];
+                    which = i;
+                }
+        };
+        find();
+        if constexpr (LSE) {
+            // (as the groups' launch and store_lse have it)
+            const float steps = a.steps.hi + a.steps.lo;
+            const uint32_t top = wave_max(best);
+            const bool number = top < kInfKey<T> && top > kNegInfKey<T>;
+            const float most = number ? value_of<T>(top) : top == kInfKey<T> ? __builtin_huge_valf() : top <= kNegInfKey<T> ? -__builtin_huge_valf() : __builtin_nanf("");
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) part += i * 64 + lane < a.cols ? __builtin_amdgcn_exp2f((Elem<T>::widen(v[i]) - most) * steps) : 0.0f;
+            const double sum = group_reduce<SumD>((double)part, 64);
+            if (lane == 0) a.lse[row] = (float)((double)most * a.inv_temperature + (number ? (double)__builtin_amdgcn_logf((float)sum) * 0.6931471805599453 : 0.0));
+        }
+        uint32_t mine = 0, at = 0;
+#pragma clang loop unroll(disable)
+        for (int r = 0; r < a.k; ++r) {
+            const uint32_t most = wave_max(best);
+            const uint64_t who = __ballot(best == most);
+            int l = __builtin_ctzll(who);
+            if (who & (who - 1)) l = (int)(~wave_max(best == most ? ~(uint32_t)(which * 64 + lane) : 0u) & 63);  // (equal ones: the first)
+            const uint32_t index = (uint32_t)lane_of(which, l) * 64 + l;
+            if (lane == r) {
+                mine = most;
+                at = index;
+            }
+            const int gone = lane == l ? which : -1;
+#pragma unroll
+            for (int i = 0; i < N; ++i) key[i] = i == gone ? 0 : key[i];
+            find();
+        }
+        if (lane < a.k) Answer<T>{a, x, row}(lane, place_of(mine, at));
+    }
+}
+
+// Which rows it takes (us, f32, against the two launches). Few rows, where a wavefront's steps stand one behind the other: [1, 2000] of k 8 10.0 / 10.4, of 20 18.6 / 11.1, [1, 256] of 64 12.9 / 14.2.
+// Many: [500, 2000] of 20 19.9 / 20.2, of 64 52 / 70; a router's [16384, 64] of 8 7.2 / 132, [16384, 1000] of 64 161 / 717.
+bool for_registers(const TopkArgs& a) { return a.cols <= 64 * 32 && a.k <= 64 && (a.rows > 256 || a.k * ((a.cols + 63) / 64) <= 256); }
+
 }  // namespace
 
 void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
+        if (for_registers(a)) {
+            auto small = [&](auto n, auto lse) {
+                topk_small_kernel<T, decltype(n)::value, decltype(lse)::value><<<(unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20), 256, 0, st>>>(a);
+            };
+            auto sized = [&](auto lse) {
+                if (a.cols <= 64) small(std::integral_constant<int, 1>{}, lse);
+                else if (a.cols <= 256) small(std::integral_constant<int, 4>{}, lse);
+                else if (a.cols <= 1024) small(std::integral_constant<int, 16>{}, lse);
+                else small(std::integral_constant<int, 32>{}, lse);
+            };
+            if (a.lse) sized(std::true_type{});
+            else sized(std::false_type{});
+            return;
+        }
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
             const unsigned blocks = (unsigned)rows;

@@ -157,3 +157,25 @@ def test_many_rows(hpt, dev, name, k):
     exact = np.where(nan, np.nan, logsumexp(np.where(np.isnan(x), 0, x)))
     near(got[0], exact, LSE + F32_STEP * np.abs(np.where(np.isfinite(exact), exact, 0)))
     assert np.array_equal(got, np.broadcast_to(got[:1], got.shape), equal_nan=True)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("cols,k", [(9, 9), (40, 8), (64, 64), (65, 33), (256, 64), (257, 1), (1000, 20), (1024, 64), (2048, 64), (2048, 3), (2049, 64)])
+def test_small_rows(hpt, dev, name, cols, k):
+    """A router's rows and others that a wavefront holds: few and many of them, of few values, off the vectors' grid, every k-th of a wider buffer."""
+    kind, rng = Kind(hpt, name), np.random.default_rng(cols * 3 + k)
+    x = np.concatenate([rows_that_tie(rng, cols), rng.standard_normal((13, cols))])
+    t, x, _ = shifted(hpt, kind, x, 1)
+    values, at, lse = check(hpt, t, x, k, kind.dtype, True, 0.8)
+    assert np.array_equal(kind.load(values), np.take_along_axis(x, at, -1), equal_nan=True)
+    nan = np.isnan(x).any(-1)
+    exact = np.where(nan, np.nan, logsumexp(np.where(np.isnan(x), 0, x) / 0.8))
+    near(lse, exact, LSE + F32_STEP * np.abs(np.where(np.isfinite(exact), exact, 0)))
+    n = len(x)
+    v = hpt.Tensor.from_raw(t.ptr, [50, n, cols], kind.dtype, 0, [0, cols, 1])
+    i32 = hpt.Tensor.empty([50, n, k], hpt.i32)
+    many = v.topk(k, index_out=i32)
+    assert np.array_equal(i32.numpy(), np.broadcast_to(at, (50, n, k)))
+    assert np.array_equal(kind.load(many[0].numpy()), np.broadcast_to(np.take_along_axis(x, at, -1), (50, n, k)), equal_nan=True)
+    apart = v[:, ::2]
+    assert np.array_equal(apart.topk(k)[1].numpy(), np.broadcast_to(at[::2], (50, len(at[::2]), k)))
