@@ -169,38 +169,43 @@ template <class T, int CAP> __device__ __forceinline__ int collect_top(TopShared
         s.least = least;
     }
     if (many <= CAP) {
-        // (four vectors of a thread on their way together)
+        // N vectors of a thread on their way together
+        auto look = [&](auto vectors) {
+            constexpr int N = decltype(vectors)::value;
 #pragma clang loop unroll(disable)
-        for (int w0 = threadIdx.x; w0 < many * V; w0 += 4 * threads) {
-            Pack<T, VEC> p[4];
-            int at[4];
+            for (int w0 = threadIdx.x; w0 < many * V; w0 += N * threads) {
+                Pack<T, VEC> p[N];
+                int first[N];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const int w = w0 + n * threads, v = group_vec<T>(s.groups[min(w / V, many - 1)], w % V);
-                at[n] = w < many * V ? v * VEC : row.end;
-                p[n] = row.raw(min(v, row.vecs() - 1));
-            }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const int e = at[n];
-                if (e >= row.end) continue;
-                uint32_t key[VEC], hits = 0;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    key[i] = key_of(p[n].v[i]);
-                    hits |= key[i] >= least && row.holds(e + i) ? 1u << i : 0;
+                for (int n = 0; n < N; ++n) {
+                    const int w = w0 + n * threads, v = group_vec<T>(s.groups[min(w / V, many - 1)], w % V);
+                    first[n] = w < many * V ? v * VEC : row.end;
+                    p[n] = row.raw(min(v, row.vecs() - 1));
                 }
-                if (hits) {
-                    uint32_t at = atomicAdd(&s.count, (uint32_t)__builtin_popcount(hits));
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i)
-                        if (hits >> i & 1) {
-                            if (at < CAP) s.list[at] = place_of(key[i], e + i - row.lead);
-                            ++at;
-                        }
+                for (int n = 0; n < N; ++n) {
+                    const int e = first[n];
+                    if (e >= row.end) continue;
+                    uint32_t key[VEC], hits = 0;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        key[i] = key_of(p[n].v[i]);
+                        hits |= key[i] >= least && row.holds(e + i) ? 1u << i : 0;
+                    }
+                    if (hits) {
+                        uint32_t at = atomicAdd(&s.count, (uint32_t)__builtin_popcount(hits));
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i)
+                            if (hits >> i & 1) {
+                                if (at < CAP) s.list[at] = place_of(key[i], e + i - row.lead);
+                                ++at;
+                            }
+                    }
                 }
             }
-        }
+        };
+        if (many * V <= threads) look(std::integral_constant<int, 1>{});
+        else look(std::integral_constant<int, 4>{});
         __syncthreads();
         if (s.count <= CAP) return (int)s.count;
     }
