@@ -695,7 +695,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
 template <class T, int MODE, int THREADS>
 __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == PLAIN ? 1 : 3) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ PickShared<MODE, THREADS == 1024 ? 8192 : 2048> s;
+    __shared__ PickShared<MODE, THREADS == 1024 ? 8192 : 4096> s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     make_table(s.table);
     for (int64_t at = blockIdx.x; at < rows; at += gridDim.x) {
@@ -1027,7 +1027,7 @@ void launch_sample(int dtype, const SampleArgs& a, hipStream_t st) {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
             const unsigned blocks = (unsigned)rows;
-            const bool many = rows > 512;
+            const bool many = rows > 256;
             auto both = [&](auto mode) {
                 constexpr int MODE = decltype(mode)::value;
                 sample_tiles_kernel<T, MODE><<<dim3((unsigned)a.tiles, blocks), kTileGroups, 0, st>>>(a, set, row0);

@@ -253,8 +253,8 @@ void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
             auto both = [&](auto lse) {
                 constexpr bool LSE = decltype(lse)::value;
                 topk_groups_kernel<T, LSE><<<tiles, kTileGroups, 0, st>>>(a, row0);
-                if (rows > 512 && for_a_wave<T>(a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
-                else topk_pick_kernel<T, LSE><<<blocks, rows <= 512 ? 1024 : 256, 0, st>>>(a, row0, rows);  // (few rows: more threads for each)
+                if (rows > 256 && for_a_wave<T>(a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
+                else topk_pick_kernel<T, LSE><<<blocks, rows <= 256 ? 1024 : 256, 0, st>>>(a, row0, rows);
             };
             if (a.lse) both(std::true_type{});
             else both(std::false_type{});
