@@ -6,12 +6,16 @@
 //
 // Which token that is hangs on sums over the row: an error of 1e-7 of the sum, f32's, moves one of 10^5 borders across u in a row out of fifty. Weights and sums have 52
 // bits here: with t = x log2 e 128 / temperature and n the whole number next to it, w is 2^(n / 128), from a table of 128, times a polynomial in t - n (degree 3, 3e-13). f64
-// multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s; it is bound by its instructions, some 17 for each logit.
+// multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s; it is bound by its instructions, 16 for each logit.
 //
 // Two launches. The first takes tiles of 8192 logits and leaves, by what the row's filters need: the largest keys of its groups (top_k of at most 1024: only the first places
 // matter); the sum of the weights (no filter); or the weights' sums by size, in buckets of an eighth of a power of two, as integers, whose sum has no order (with their
 // numbers where top_k is larger). The second has a workgroup for each row: it finds the bucket in which a border lies, collects that bucket's logits, narrows the border to one
-// place, and then looks through the one tile in which u's token lies. (Rows of which at most 128 places matter take a wavefront each.)
+// place, and then looks through the one tile in which u's token lies. (Many rows of which at most 128 places matter take a wavefront each.)
+//
+// us of the two launches, bf16 [2048, 50257] (206 MB): without a filter 85 + 14 (2.4 TB/s in the first), top_k 50 39 + 24 (5.3), 600 39 + 50, top_p 0.9 133 + 95 (1.5: two LDS additions' worth of
+// instructions more). bf16 [1, 152000] with top_k 20 and top_p 0.8 2.5 + 11.5, f32 [33, 50257] with top_p 0.95 8 + 29, [64, 152000] with settings for each row 14 + 45: the steps of one workgroup, most of
+// them the collection of a bucket, at a compute unit's own rate.
 #include <algorithm>
 
 #include "top_rows.hpp"
@@ -693,7 +697,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
 
 // THREADS: at most. Few rows have larger workgroups, and room for more of a bucket.
 template <class T, int MODE, int THREADS>
-__global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == PLAIN ? 1 : 3) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == SORTED ? 3 : 1) void sample_pick_kernel(const SampleArgs a, const Settings all_rows, int64_t row0, int64_t rows) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ PickShared<MODE, THREADS == 1024 ? 8192 : 4096> s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -1027,6 +1031,7 @@ void launch_sample(int dtype, const SampleArgs& a, hipStream_t st) {
         for (int64_t row0 = 0; row0 < a.rows; row0 += a.run) {
             const int64_t rows = std::min(a.run, a.rows - row0);
             const unsigned blocks = (unsigned)rows;
+            // (beyond a workgroup for each compute unit, smaller ones, several to a unit. bf16 [200, 50257] and [500, 50257], top_p 0.9, us: 48.8 and 91.9 with 1024 threads, 49.8 and 72.8 with 256)
             const bool many = rows > 256;
             auto both = [&](auto mode) {
                 constexpr int MODE = decltype(mode)::value;

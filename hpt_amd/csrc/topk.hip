@@ -4,8 +4,8 @@
 // adds the exponentials of its 2048 below their largest). The second has a workgroup for each row, which finds the first k places from those keys (top_rows.hpp).
 // The second is bound by the latency of its steps.
 //
-// The first reads bf16 [4096, 50257] in 68 us (6.0 TB/s) without the sum; with it the launch is bound by its instructions, five for each logit, 88 to 92 us (4.6 TB/s). The second takes 35 of k = 64
-// there (by wavefronts), 9.7 of one row of 152000 and of 37 of 50257, 19.5 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
+// The first reads bf16 [4096, 50257] in 71 to 73 us (5.7 TB/s) without the sum; with it the launch is bound by its instructions, five for each logit: 88 to 92 us (4.6 TB/s). The second takes 32 to 35
+// of k = 64 there (by wavefronts), 9.7 of one row of 152000 and of 37 of 50257, 19.5 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
 #include <algorithm>
 #include <cmath>
 
@@ -253,6 +253,8 @@ void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
             auto both = [&](auto lse) {
                 constexpr bool LSE = decltype(lse)::value;
                 topk_groups_kernel<T, LSE><<<tiles, kTileGroups, 0, st>>>(a, row0);
+                // A wavefront for each of many rows, a workgroup for each of few (k = 20, us: bf16 [1, 152000] 13.2 / 9.7 of the second launch, all of [300, 50257] 20.1 / 28.5), of 1024 threads while
+                // they do not fill the compute units (k = 200: [300, 50257] 24.8, and 29.8 with 1024; [200, 50257] 17.5 with them).
                 if (rows > 256 && for_a_wave<T>(a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
                 else topk_pick_kernel<T, LSE><<<blocks, rows <= 256 ? 1024 : 256, 0, st>>>(a, row0, rows);
             };

@@ -93,11 +93,6 @@ template <class T> struct LogitRow {
         for (int i = 0; i < VEC; ++i)
             if (!holds(v * VEC + i)) p.v[i] = Elem<T>::narrow(-__builtin_huge_valf());
     }
-    __device__ __forceinline__ Pack<T, VEC> vec(int v) const {
-        Pack<T, VEC> p = raw(v);
-        clean(p, v);
-        return p;
-    }
 };
 // Vector b of the 32 logits that a thread has of a tile: a wavefront has 2048 neighbours, and its vectors lie lane beside lane.
 template <class T> constexpr int kTileVecs = kTile * sizeof(T) / 16 / kTileGroups;  // of a thread

@@ -276,8 +276,8 @@ int32_t hpt_hip_add_layernorm(int32_t dev, void* stream, const hpt_view* in, con
 
 /* ---- operators around a transformer's blocks ---------------------------------
  * No trait of the reference has these; they stand beside layernorm, softmax_causal and log_softmax for models that
- * norm by the root mean square, bias attention by relative positions, or are trained on a policy loss, and give
- * their gradients. Dtypes f16, bf16 and f32; statistics, sums and the results called f32 below are f32 for all
+ * norm by the root mean square, bias attention by relative positions, are trained on a policy loss or by a teacher, or answer
+ * with the largest or with sampled logits, and give their gradients. Dtypes f16, bf16 and f32; statistics, sums and the results called f32 below are f32 for all
  * of them (a scaled score, or a row's sum of squares, beyond its range is an infinity), and every result is rounded
  * once. A row's elements must be neighbours in memory, its rows may lie anywhere; every other operand and every
  * result is contiguous. Results share no memory with each other or with operands, except that one may take the very
