@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kTileGroups) void sample_tiles_kernel(const SampleA
         uint32_t key = 0;
 #pragma unroll
         for (int b = 0; b < V; ++b) key = max(key, most_key<T>(p[b]));
-        key = group_reduce<MaxU>(key, 64);
+        key = wave_max(key);
         double sum = 0.0;
         if (!BUCKETS || mode == PLAIN) {
             // a wavefront's part, in the octave of its own largest: nobody waits for anybody
@@ -630,7 +630,7 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
         const bool reached = lane < left && (by_count ? q.count_before + number >= k : q.before + (double)upto * unit >= target);
         // the first that reaches it, or the last there is
         const uint32_t score = reached ? 1024 - number : lane < left ? number : 0;
-        const uint64_t best = __ballot(score == group_reduce<MaxU>(score, 64));
+        const uint64_t best = __ballot(score == wave_max(score));
         wave_fence();
         if (lane == __builtin_ctzll(best)) {
             q.border = mine;
@@ -691,7 +691,7 @@ template <class T> __device__ __forceinline__ void pick_of_few(const SampleArgs&
     uint32_t token = 0;
     if (lane * 2 < kept && v[0] > 0.0 && s0 <= part) token = index[0] + 1;
     if (lane * 2 + 1 < kept && v[1] > 0.0 && s1 <= part) token = max(token, index[1] + 1);
-    const uint32_t best = group_reduce<MaxU>(token, 64);
+    const uint32_t best = wave_max(token);
     if (token == best && best) answer(a, row, best - 1, log((index[0] + 1 == best ? v[0] : v[1]) / whole));
 }
 
@@ -813,7 +813,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == SORTED ? 3 :
             auto head = [&](int t) -> const SampleHead& { return tiles[t / per].heads[t % per]; };
             uint32_t most = 0;
             for (int t = lane; t < parts; t += 64) most = max(most, head(t).most);
-            most = group_reduce<MaxU>(most, 64);
+            most = wave_max(most);
             if (no_number<T>(most)) {
                 if (threadIdx.x == 0) answer(a, row, -1, __builtin_nan(""));
                 continue;

@@ -134,7 +134,10 @@ template <class T, int CAP> __device__ __forceinline__ int collect_top(TopShared
     }
     s.digits.clear();
     if (threadIdx.x == 0) s.count = s.many = 0;
-    most = block_reduce<MaxU>(most, s.waves);
+    most = wave_max(most);
+    if ((threadIdx.x & 63) == 0) s.waves[threadIdx.x >> 6] = most;
+    __syncthreads();
+    most = wave_max((threadIdx.x & 63) < blockDim.x / 64 ? s.waves[threadIdx.x & 63] : 0);  // (every wavefront for itself)
     for (int r = 0; r < rounds; ++r) {
         const Keys p = keys_of_round(r);
 #pragma unroll
@@ -258,7 +261,7 @@ template <class T> __device__ __forceinline__ int wave_top(WaveShared& s, const 
         }
     }
     static_assert(kWaveRounds % 4 == 0, "the last round of four stays within");
-    most = group_reduce<MaxU>(most, 64);
+    most = wave_max(most);
     // the smallest distance below the largest, in sixteenths of a power of two, that k of them are within
     auto from = [&](int d) {
         const uint32_t far = (uint32_t)(d + 1) << SHIFT;
@@ -381,7 +384,7 @@ template <int CAP, class Out> __device__ __forceinline__ void rank_top(TopShared
             sum += c[i];
             largest = max(largest, c[i]);
         }
-        largest = group_reduce<MaxU>(largest, 64);
+        largest = wave_max(largest);
         uint32_t at = wave_scan(sum) - sum;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

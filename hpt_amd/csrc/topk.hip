@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs
             // a wavefront's part of the sum, below its own largest (log2 e / temperature as one f32: 2^-25 of a distance D, which costs the log D / 2^25; two pieces are a sixth more
             // instructions of a kernel that is bound by them)
             const float steps = a.steps.hi + a.steps.lo;
-            const uint32_t top = group_reduce<MaxU>(key, 64);
+            const uint32_t top = wave_max(key);
             float part = 0.0f;
             // (NaN, +inf and nothing but -inf are told from the largest alone)
             const bool number = top < kInfKey<T> && top > kNegInfKey<T>;
@@ -159,15 +159,6 @@ __global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a
 }
 
 // Rows of at most 64 N elements, a wavefront each, one launch: the row stays in registers (element i of lane l is at 64 i + l), and the largest is taken out k times.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    v = max(v, dpp_or_zero<0x111, 0xF>(v));
-    v = max(v, dpp_or_zero<0x112, 0xF>(v));
-    v = max(v, dpp_or_zero<0x114, 0xF>(v));
-    v = max(v, dpp_or_zero<0x118, 0xF>(v));
-    v = max(v, dpp_or_zero<0x142, 0xA>(v));
-    v = max(v, dpp_or_zero<0x143, 0xC>(v));
-    return lane_of(v, 63);
-}
 template <class T, int N, bool LSE>
 __global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -115,9 +115,6 @@ template <class T> __device__ __forceinline__ void load_tile(const LogitRow<T>& 
     }
 }
 
-struct MaxU {
-    __device__ static __forceinline__ uint32_t comb(uint32_t a, uint32_t b) { return a > b ? a : b; }
-};
 // A tile's logits are dealt to groups of 32 neighbours, whose largest keys its threads get one each: lane l that of the kTileVecs vectors of its wavefront from
 // (l % kTileVecs) * 64 + l / kTileVecs * kTileVecs on (vectors that neighbouring lanes have loaded together; 64 or 128 bytes side by side, so that a group that is read again is one or two lines).
 // Each of 4 (8) lanes gives away half of its vectors' largest for the other half of its partner's, then half of those, until one is left.
@@ -219,6 +216,16 @@ template <class A> __device__ __forceinline__ A wave_scan(A v) {
     v += dpp_or_zero<0x142, 0xA>(v);  // row_bcast:15
     v += dpp_or_zero<0x143, 0xC>(v);  // row_bcast:31
     return v;
+}
+// The largest of a wavefront's, in the same way.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, dpp_or_zero<0x111, 0xF>(v));
+    v = max(v, dpp_or_zero<0x112, 0xF>(v));
+    v = max(v, dpp_or_zero<0x114, 0xF>(v));
+    v = max(v, dpp_or_zero<0x118, 0xF>(v));
+    v = max(v, dpp_or_zero<0x142, 0xA>(v));
+    v = max(v, dpp_or_zero<0x143, 0xC>(v));
+    return lane_of(v, 63);
 }
 // The sum of v over the threads before this one; `total`: over all of them. Every order is fixed. `place`: one number for each wavefront.
 __device__ __forceinline__ double scan_before(double v, double* place, double& total) {
