@@ -11,7 +11,7 @@
 // bf16 [8192, 50257], k = 64, with the rest: 142 us forward (5.8 TB/s), 22 of the launch that joins the rows' parts with their entries, 5 of the mean over the rows, 285 backward (5.8 TB/s).
 #include <algorithm>
 
-#include "block_rows.hpp"
+#include "vocab_rows.hpp"
 
 namespace hpt {
 
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(64 * kRowsAtOnce, 8) void distill_rows_kernel(const
 
 // The sums over the rows, in one workgroup and a fixed order, and each row's weight. Without a row that counts all are 0.
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const DistillArgs a) {
-    __shared__ double place[16];
+    __shared__ double place[2 * 16];
     double loss = 0.0, count = 0.0;
 #pragma unroll 4
     for (int64_t row = threadIdx.x; row < a.rows; row += 1024) {
@@ -349,8 +349,18 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const DistillArgs a) 
             count += mask;
         }
     }
-    loss = block_reduce<SumD>(loss, place);
-    count = block_reduce<SumD>(count, place);
+    loss = group_reduce<SumD>(loss, 64);
+    count = group_reduce<SumD>(count, 64);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane == 0) {
+        place[wave] = loss;
+        place[16 + wave] = count;
+    }
+    __syncthreads();
+    // (every wavefront for itself, both sums side by side: one read of LDS)
+    const double both = group_reduce<SumD>(place[lane & 31], 16);
+    loss = lane_of(both, 0);
+    count = lane_of(both, 16);
     const double inv = count == 0.0 ? 0.0 : 1.0 / count;
     if (threadIdx.x == 0) a.loss[0] = (float)(loss * inv * a.temperature * a.temperature);
 #pragma unroll 4
