@@ -8,7 +8,7 @@
 //
 // Bound by memory, as the policy loss is: one read forward, one read and one write backward. The entries (some hundred a row) come through LDS: as a bit for each token
 // forward, where s is summed without the named tokens (1 - sum p would lose what is small), as a number for each token of a piece backward.
-// bf16 [8192, 50257], k = 64, with the rest: 142 us forward (5.8 TB/s), 22 of the launch that joins the rows' parts with their entries, 5 of the mean over the rows, 285 backward (5.8 TB/s).
+// bf16 [8192, 50257], k = 64, with the rest: 142 us forward (5.8 TB/s), 22 of the launch that joins the rows' parts with their entries, 4 of the mean over the rows, 285 backward (5.8 TB/s).
 #include <algorithm>
 
 #include "vocab_rows.hpp"

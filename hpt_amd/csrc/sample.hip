@@ -14,7 +14,7 @@
 // place, and then looks through the one tile in which u's token lies. (Many rows of which at most 128 places matter take a wavefront each.)
 //
 // us of the two launches, bf16 [2048, 50257] (206 MB): without a filter 85 + 14 (2.4 TB/s in the first), top_k 50 39 + 24 (5.3), 600 39 + 50, top_p 0.9 133 + 95 (1.5: two LDS additions' worth of
-// instructions more). bf16 [1, 152000] with top_k 20 and top_p 0.8 2.5 + 11.5, f32 [33, 50257] with top_p 0.95 8 + 29, [64, 152000] with settings for each row 14 + 45: the steps of one workgroup, most of
+// instructions more). bf16 [1, 152000] with top_k 20 and top_p 0.8 2.5 + 10.5, f32 [33, 50257] with top_p 0.95 8 + 29, [64, 152000] with settings for each row 14 + 44: the steps of one workgroup, most of
 // them the collection of a bucket, at a compute unit's own rate.
 #include <algorithm>
 

@@ -5,7 +5,7 @@
 // The second is bound by the latency of its steps.
 //
 // The first reads bf16 [4096, 50257] in 71 to 73 us (5.7 TB/s) without the sum; with it the launch is bound by its instructions, five for each logit: 88 to 92 us (4.6 TB/s). The second takes 32 to 35
-// of k = 64 there (by wavefronts), 9.7 of one row of 152000 and of 37 of 50257, 19.5 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
+// of k = 64 there (by wavefronts), 9 of one row of 152000 and of 37 of 50257, 19 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
 #include <algorithm>
 #include <cmath>
 
