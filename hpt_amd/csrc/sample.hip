@@ -11,7 +11,7 @@
 // Two launches. The first takes tiles of 8192 logits and leaves, by what the row's filters need: the largest keys of its groups (top_k of at most 1024: only the first places
 // matter); the sum of the weights (no filter); or the weights' sums by size, in buckets of an eighth of a power of two, as integers, whose sum has no order (with their
 // numbers where top_k is larger). The second has a workgroup for each row: it finds the bucket in which a border lies, collects that bucket's logits, narrows the border to one
-// place, and then looks through the one tile in which u's token lies. (Many rows of which at most 128 places matter take a wavefront each.)
+// place, and then looks through the one tile in which u's token lies. (Very many rows of which at most 64 places matter take a wavefront each.)
 //
 // us of the two launches, bf16 [2048, 50257] (206 MB): without a filter 85 + 14 (2.4 TB/s in the first), top_k 50 39 + 24 (5.3), 600 39 + 50, top_p 0.9 133 + 95 (1.5: two LDS additions' worth of
 // instructions more). bf16 [1, 152000] with top_k 20 and top_p 0.8 2.5 + 10.5, f32 [33, 50257] with top_p 0.95 8 + 29, [64, 152000] with settings for each row 14 + 44: the steps of one workgroup, most of
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == SORTED ? 3 :
     }
 }
 
-// A wavefront for each row, of which at most 128 places matter. One of which it would collect too much is left to the workgroup.
+// A wavefront for each row, of which at most kWaveTop places matter. One of which it would collect too much is left to the workgroup.
 template <class T>
 __global__ __launch_bounds__(kTileGroups) void sample_wave_kernel(const SampleArgs a, const Settings set, int64_t row0, int64_t rows) {
     constexpr int N = kTileGroups / 64;
@@ -1040,7 +1040,7 @@ void launch_sample(int dtype, const SampleArgs& a, hipStream_t st) {
                     sample_pick_kernel<T, MODE, 256><<<blocks, 256, 0, st>>>(a, set, row0, rows);
                 } else {
                     if constexpr (MODE == FEW)
-                        if (many && for_a_wave<T>(a.tiles, set.k)) return sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, set, row0, rows);
+                        if (for_a_wave<T>(rows, a.tiles, set.k)) return sample_wave_kernel<T><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, set, row0, rows);
                     if constexpr (MODE != FEW)
                         if (many) return sample_pick_kernel<T, MODE, 256><<<blocks, 256, 0, st>>>(a, set, row0, rows);
                     sample_pick_kernel<T, MODE, 1024><<<blocks, many ? 256 : 1024, 0, st>>>(a, set, row0, rows);

@@ -6,7 +6,7 @@
 // some more. What they hold at or above that key is collected, and its first k places are the row's. Where that is too much (a row of few different
 // values), the k-th place itself is found by sweeps over the row, eight bits of its key at a time, and the row is collected in its order.
 //
-// Up to 128 places are a wavefront's work, which waits for nobody (wave_top): its histogram is a search by halves over the largest of each vector of keys.
+// Up to 64 places of very many rows are a wavefront's work, which waits for nobody (wave_top): its histogram is a search by halves over the largest of each vector of keys.
 #pragma once
 
 #include "vocab_rows.hpp"
@@ -218,7 +218,7 @@ template <class T, int CAP> __device__ __forceinline__ int collect_top(TopShared
 
 // ---- a wavefront's form ---------------------------------------------------------------------------
 
-constexpr int kWaveTop = 128;    // places at most
+constexpr int kWaveTop = 64;     // places at most
 constexpr int kWaveList = 256;   // places, groups and vectors of keys that are collected
 constexpr int kWaveRounds = 20;  // vectors of keys of a lane
 struct WaveShared {
@@ -228,10 +228,11 @@ struct WaveShared {
     };
     uint32_t vectors[kWaveList], groups[kWaveList];
 };
-// Whether a row is for it: fewer vectors of keys than places would find no bound.
-template <class T> __host__ __device__ constexpr bool for_a_wave(int tiles, int k) {
+// Whether rows are for it: fewer vectors of keys than places would find no bound, and it takes more rows than a workgroup each fills the compute units with. (us, a wavefront and a workgroup of 256, top-k:
+// bf16 [300, 50257] k = 20 16.3 / 15.1, 64 24.3 / 18.0; [700, 50257] 23.5 / 23.0, 32.9 / 25.8; [2000, 50257] 42.5 / 49.0, 54.9 / 54.9, of 100 68 / 58; [4096, 50257] 84.7 / 105, 95.7 / 113.)
+template <class T> __host__ __device__ constexpr bool for_a_wave(int64_t rows, int tiles, int k) {
     constexpr int per = kTileGroups * (int)sizeof(T) / 16;
-    return k <= kWaveTop && tiles * per >= 2 * k && tiles * per <= kWaveRounds * 64;
+    return rows > 1024 && k <= kWaveTop && tiles * per >= 2 * k && tiles * per <= kWaveRounds * 64;
 }
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }  // (a wavefront's accesses to LDS are in order)
 __device__ __forceinline__ int lanes_before(uint64_t who) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0)); }

@@ -244,9 +244,8 @@ void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
             auto both = [&](auto lse) {
                 constexpr bool LSE = decltype(lse)::value;
                 topk_groups_kernel<T, LSE><<<tiles, kTileGroups, 0, st>>>(a, row0);
-                // A wavefront for each of many rows, a workgroup for each of few (k = 20, us: bf16 [1, 152000] 13.2 / 9.7 of the second launch, all of [300, 50257] 20.1 / 28.5), of 1024 threads while
-                // they do not fill the compute units (k = 200: [300, 50257] 24.8, and 29.8 with 1024; [200, 50257] 17.5 with them).
-                if (rows > 256 && for_a_wave<T>(a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
+                // (a workgroup of 1024 threads while they do not fill the compute units: bf16 [300, 50257], k = 200, 24.8 us with 256 and 29.8 with 1024, [200, 50257] 17.5 with them)
+                if (for_a_wave<T>(rows, a.tiles, a.k)) topk_wave_kernel<T, LSE><<<(blocks + 3) / 4, kTileGroups, 0, st>>>(a, row0, rows);
                 else topk_pick_kernel<T, LSE><<<blocks, rows <= 256 ? 1024 : 256, 0, st>>>(a, row0, rows);
             };
             if (a.lse) both(std::true_type{});

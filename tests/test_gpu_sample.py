@@ -222,3 +222,28 @@ def test_a_bucket_of_many(hpt, dev):
     t, x = Kind(hpt, "f32").up(np.stack([rng.permutation(r) for r in x]))
     for settings in (dict(top_p=0.5), dict(top_k=20000), dict(top_k=20000, top_p=0.3), dict(min_p=0.97)):
         check(hpt, t, x, np.array([0.4, 0.9], np.float32), settings)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("settings", [dict(top_k=20, top_p=0.8), dict(top_k=64, min_p=0.01, temperature=1.5), dict(top_k=1), dict(top_p=0.9), dict()], ids=str)
+def test_very_many_rows(hpt, dev, name, settings):
+    """More rows than a workgroup each is for, of few values and masks among others."""
+    kind, rng, cols, rep, n = Kind(hpt, name), np.random.default_rng(10), 20001, 100, 12
+    x = rng.standard_normal((n, cols)) * 3
+    x[2] = rng.integers(-2, 3, cols)
+    x[4] = 1.5
+    x[6, cols // 9:] = -np.inf
+    x[8, cols // 2] = np.nan
+    x[10] = -np.inf
+    t, x = kind.up(x)
+    u = rng.uniform(size=n).astype(np.float32)
+    want = [sampled(x[r], u[r], **settings) for r in range(n)]
+    clear = np.array([w[2] > NEAR for w in want])
+    assert clear.sum() >= n - 2 and rep * n > 1024
+    v = hpt.Tensor.from_raw(t.ptr, [rep, n, cols], kind.dtype, 0, [0, cols, 1])
+    token, logp = v.sample(up(hpt, np.tile(u, rep)), **settings)
+    token, logp = token.numpy().reshape(rep, n), logp.numpy().reshape(rep, n).astype(np.float64)
+    assert (token == token[:1]).all() and np.array_equal(logp, np.broadcast_to(logp[:1], logp.shape), equal_nan=True)
+    assert np.array_equal(token[0][clear], np.array([w[0] for w in want])[clear])
+    logs = np.array([w[1] for w in want])
+    near(logp[0][clear], logs[clear], F32_STEP * np.abs(logs[clear]) + 1e-11)

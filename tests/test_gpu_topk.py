@@ -179,3 +179,23 @@ def test_small_rows(hpt, dev, name, cols, k):
     assert np.array_equal(kind.load(many[0].numpy()), np.broadcast_to(np.take_along_axis(x, at, -1), (50, n, k)), equal_nan=True)
     apart = v[:, ::2]
     assert np.array_equal(apart.topk(k)[1].numpy(), np.broadcast_to(at[::2], (50, len(at[::2]), k)))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("cols,k", [(20001, 1), (20001, 20), (20001, 64), (40003, 50)])
+def test_very_many_rows(hpt, dev, name, cols, k):
+    """More rows than a workgroup each is for, of few values and masks among others."""
+    kind, rng, rep = Kind(hpt, name), np.random.default_rng(cols + k), 50
+    x = np.concatenate([rows_that_tie(rng, cols), rng.standard_normal((11, cols)) * 3, np.sort(rng.standard_normal((3, cols)))])
+    t, x = kind.up(x)
+    n = len(x)
+    v = hpt.Tensor.from_raw(t.ptr, [rep, n, cols], kind.dtype, 0, [0, cols, 1])
+    assert rep * n > 1024
+    values, index, lse = v.topk(k, lse=True)
+    want = order(x)[:, :k]
+    assert np.array_equal(index.numpy(), np.broadcast_to(want, (rep, n, k)))
+    assert np.array_equal(kind.load(values.numpy()), np.broadcast_to(np.take_along_axis(x, want, -1), (rep, n, k)), equal_nan=True)
+    got, nan = lse.numpy().astype(np.float64), np.isnan(x).any(-1)
+    exact = np.where(nan, np.nan, logsumexp(np.where(np.isnan(x), 0, x)))
+    near(got[-1], exact, LSE + F32_STEP * np.abs(np.where(np.isfinite(exact), exact, 0)))
+    assert np.array_equal(got, np.broadcast_to(got[:1], got.shape), equal_nan=True)
