@@ -1688,7 +1688,9 @@ int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* 
 int32_t hpt_hip_topk_workspace(const hpt_view* in, int64_t k, size_t* bytes) {
     return guarded([&] {
         if (!bytes) fail(HPT_ERR_PARAM, "topk_workspace: null output");
-        *bytes = topk_bytes(in, top_rows_of(in, k), true);
+        // (a row without lse takes less, but then a run has more of them)
+        const RowsOf r = top_rows_of(in, k);
+        *bytes = std::max(topk_bytes(in, r, true), topk_bytes(in, r, false));
     });
 }
 
