@@ -1733,9 +1733,10 @@ int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, d
         a.run = rows_of_run(r.rows, row);
         use_device(dev);
         hipStream_t st = (hipStream_t)stream;
-        with_workspace(dev, st, workspace, (size_t)a.run * row, false, "topk", [&](void* p) {
+        const size_t need = topk_in_registers(a.rows, a.cols, a.k) ? 0 : (size_t)a.run * row;
+        with_workspace(dev, st, workspace, need, false, "topk", [&](void* p) {
             a.keys = p;
-            a.sums = (double*)((char*)p + (size_t)a.run * a.tiles * kTileGroups * dtype_size(in->dtype));
+            a.sums = p ? (double*)((char*)p + (size_t)a.run * a.tiles * kTileGroups * dtype_size(in->dtype)) : nullptr;
             launch_topk(in->dtype, a, st);
             check_launch("topk");
         });

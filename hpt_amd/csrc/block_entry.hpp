@@ -225,6 +225,8 @@ int64_t tiles_of(int dtype, int64_t cols, bool shifted);
 bool rows_shifted(int dtype, const void* x, const Dims& kept);
 size_t topk_row_bytes(int dtype, int64_t cols, bool lse);
 int64_t rows_of_run(int64_t rows, size_t row_bytes);
+// Rows that a wavefront takes in one launch, without scratch.
+bool topk_in_registers(int64_t rows, int64_t cols, int64_t k);
 void launch_topk(int dtype, const TopkArgs& a, hipStream_t st);
 
 // A setting of each row's sampling: one number for all, or a tensor of f32, i32 or i64.

@@ -215,15 +215,15 @@ __global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a) {
     }
 }
 
-// Which rows it takes (us, f32, against the two launches). Few rows, where a wavefront's steps stand one behind the other: [1, 2000] of k 8 10.0 / 10.4, of 20 18.6 / 11.1, [1, 256] of 64 12.9 / 14.2.
-// Many: [500, 2000] of 20 19.9 / 20.2, of 64 52 / 70; a router's [16384, 64] of 8 7.2 / 132, [16384, 1000] of 64 161 / 717.
-bool for_registers(const TopkArgs& a) { return a.cols <= 64 * 32 && a.k <= 64 && (a.rows > 256 || a.k * ((a.cols + 63) / 64) <= 256); }
-
 }  // namespace
+
+// Which rows topk_small_kernel takes (us, f32, against the two launches). Few rows, where a wavefront's steps stand one behind the other: [1, 2000] of k 8 10.0 / 10.4, of 20 18.6 / 11.1, [1, 256] of 64 12.9 / 14.2.
+// Many: [500, 2000] of 20 19.9 / 20.2, of 64 52 / 70; a router's [16384, 64] of 8 7.2 / 132, [16384, 1000] of 64 161 / 717.
+bool topk_in_registers(int64_t rows, int64_t cols, int64_t k) { return cols <= 64 * 32 && k <= 64 && (rows > 256 || k * ((cols + 63) / 64) <= 256); }
 
 void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
-        if (for_registers(a)) {
+        if (topk_in_registers(a.rows, a.cols, a.k)) {
             auto small = [&](auto n, auto lse) {
                 topk_small_kernel<T, decltype(n)::value, decltype(lse)::value><<<(unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20), 256, 0, st>>>(a);
             };

@@ -371,7 +371,8 @@ int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* 
 
 /* The k largest elements of each row of `in` [..., cols], 1 <= k <= 1024 (and cols), in order: a NaN before everything, then the larger value, equal
  * values (and -0 and +0) by their index. `values` [..., k] of in's dtype, `index` [..., k] i32 or i64. `lse` (may be NULL; f32, one for each
- * row): log sum exp(in / temperature), NaN where the row has one, otherwise +inf where it has one. The workspace is enough for calls with lse and without. */
+ * row): log sum exp(in / temperature), NaN where the row has one, otherwise +inf where it has one. The workspace is enough for calls with lse and without; rows of at
+ * most 2048 elements of which at most 64 are wanted need none where they are more than 256, or where k * ceil(cols / 64) is at most 256. */
 int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, double temperature, const hpt_view* workspace,
                      hpt_view* values, hpt_view* index, hpt_view* lse);
 int32_t hpt_hip_topk_workspace(const hpt_view* in, int64_t k, size_t* bytes);

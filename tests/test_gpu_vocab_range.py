@@ -2,10 +2,13 @@
 logits that lie anywhere, rows by many millions.
 
 Tolerances count half steps of f32, as beside each test."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 from block_util import Guarded, Kind, up
+from test_gpu_block_calls import P, hip, stream  # noqa: F401
 from vocab_util import order
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +30,30 @@ def test_a_workspace_of_the_size_that_is_asked_for(hpt, dev, name, rows, cols):
         got = v.topk(k, lse=lse, workspace=ws.t)
         ws.numpy()
         assert np.array_equal(got[1].numpy(), want)
+
+
+def test_rows_that_registers_hold_take_no_scratch(hpt, dev, hip, stream):  # noqa: F811
+    """They are captured without a workspace."""
+    kind, rng, k = Kind(hpt, "f32"), np.random.default_rng(1), 8
+    t, x = kind.up(rng.standard_normal((600, 64)))
+    v, i, lse = hpt.Tensor.empty([600, k], hpt.f32), hpt.Tensor.empty([600, k], hpt.i64), hpt.Tensor.empty([600], hpt.f32)
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    try:
+        t.topk(k, lse=True, stream=stream, values_out=v, index_out=i, lse_out=lse)
+    finally:
+        g = P()
+        rc = hip.hipStreamEndCapture(stream, C.byref(g))
+    assert rc == 0 and g.value
+    e = P()
+    assert hip.hipGraphInstantiate(C.byref(e), g, None, None, 0) == 0
+    try:
+        for scale in (1.0, 0.5, -2.0):
+            a = (x * scale).astype(np.float32)
+            assert hpt.lib().hpt_hip_memcpy_h2d_sync(0, P(t.ptr), a.ctypes.data_as(P), a.nbytes) == 0
+            assert hip.hipGraphLaunch(e, stream) == 0 and hip.hipStreamSynchronize(stream) == 0
+            assert np.array_equal(i.numpy(), order(a)[:, :k])
+            want = [r.numpy() for r in t.topk(k, lse=True)]
+            assert all(np.array_equal(r.numpy(), w) for r, w in zip((v, i, lse), want))
+    finally:
+        hip.hipGraphExecDestroy(e)
+        hip.hipGraphDestroy(g)
