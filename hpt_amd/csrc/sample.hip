@@ -941,7 +941,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == SORTED ? 3 :
                 }
             }
             part = lane_of(part, owner);
-            double rest = fmax(target - lane_of(before, owner), 0.0);
+            const double rest = fmax(target - lane_of(before, owner), 0.0);
             // and its token there: a thread has `run` neighbours of the part
             const int size = kTile / per, run = max(size / (int)blockDim.x, VEC), e0 = part * size + (int)threadIdx.x * run;
             mine = 0.0;
@@ -956,13 +956,13 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : MODE == SORTED ? 3 :
                     mine += on ? r.w.of(Elem<T>::widen(p.v[i]), most_value) : 0.0;
                 }
             }
-            double part_sum;
-            const double here = scan_before(mine, s.place, part_sum);
-            // (the sum over the part may be a rounding off what it was chosen by)
-            if (rest >= part_sum) rest = part_sum * (1.0 - 0x1p-50);
-            // the wavefront in which the sum crosses it, the first thread there that does, or the last that has something
-            const double wave_before = lane_of(here, 0), wave_upto = lane_of(wave_scan(lane < waves ? s.place[lane] : 0.0), wave);
-            if ((wave == 0 || wave_before <= rest) && wave_upto > rest) {
+            double whole_part;
+            const double here = scan_before(mine, s.place, whole_part);
+            // The wavefront in which the sum crosses it and the first thread there that does, or the last that has something (the sum over the part may be a rounding off what it was chosen by).
+            // Every wavefront looks at the same numbers, so one answers. (Sums up to a wavefront are a tree's, which behind the last weight may still rise by a rounding.)
+            const double wave_sum = lane < waves ? s.place[lane] : 0.0, wave_upto = wave_scan(wave_sum);
+            const uint64_t beyond = __ballot(wave_sum > 0.0 && wave_upto > rest), weighty = __ballot(wave_sum > 0.0);
+            if (wave == (beyond ? __builtin_ctzll(beyond) : weighty ? 63 - __builtin_clzll(weighty) : 0)) {
                 const uint64_t crosses = __ballot(mine > 0.0 && here + mine > rest), some = __ballot(mine > 0.0);
                 const int l = crosses ? __builtin_ctzll(crosses) : some ? 63 - __builtin_clzll(some) : 0;
                 const int e = lane_of(e0, l) + lane;

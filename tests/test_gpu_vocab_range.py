@@ -7,7 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from block_util import Guarded, Kind, up
+from block_util import F32_STEP, Guarded, Kind, near, up
 from test_gpu_block_calls import P, hip, stream  # noqa: F401
 from vocab_util import order
 
@@ -57,3 +57,31 @@ def test_rows_that_registers_hold_take_no_scratch(hpt, dev, hip, stream):  # noq
     finally:
         hip.hipGraphExecDestroy(e)
         hip.hipGraphDestroy(g)
+
+
+# ---- sampling: borders within a rounding of what decides ---------------------------------------------------
+
+OCTAVE = 1.4426950408889634  # the temperature at which logits are octaves
+
+
+def test_halves_of_the_same_sum(hpt, dev):
+    """Twice the same weights, each time with a stretch of nothing behind them, and u in the middle of the row's sum: where the sums in 64 bits put the border between the halves depends on their
+    order, but the token is the last of the first half or the first of the second, and its probability is its own."""
+    rows, n = 1200, 2048
+    x = np.full((rows, 2 * n), -np.inf)
+    for r in range(rows):
+        rng = np.random.default_rng(r)
+        a = -rng.integers(0, 24, 1536).astype(float)
+        a[0] = 0
+        x[r, :1536], x[r, n:n + 1536] = a, rng.permutation(a)
+    t, x = Kind(hpt, "f32").up(x)
+    for part in (slice(0, 200), slice(0, rows)):  # (forms for few rows and for many)
+        count = part.stop
+        u = up(hpt, np.full(count, 0.5, np.float32))
+        v = hpt.Tensor.from_raw(t.ptr, [count, 2 * n], hpt.f32, 0)
+        each = dict(temperature=up(hpt, np.full(count, OCTAVE, np.float32)))
+        for settings in (dict(temperature=OCTAVE), each, dict(temperature=OCTAVE, min_p=1e-30)):
+            token, logp = (a.numpy() for a in v.sample(u, **settings))
+            assert np.isin(token, [1535, n]).all(), (settings, token[~np.isin(token, [1535, n])][:4])
+            w = np.exp2(x[:count])
+            near(logp, np.log(w[np.arange(count), token] / w.sum(-1)), 30 * F32_STEP)
