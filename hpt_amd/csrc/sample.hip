@@ -516,15 +516,17 @@ template <class T, class Shared> __device__ __forceinline__ uint64_t find_border
     const int bucket = q.bucket;
     const double up = pow2(bucket >> 3), unit = pow2(-(bucket >> 3)) * r.fixed.unit;  // of the bucket's octave
     auto weight = [&](float x) { return r.fixed(r.w.of(x, r.most_value) * up); };
-    if (listed != bucket) {
+    // Sums that differ by a rounding may show something in an empty bucket (one without any key has its range upside down): what is before it reaches the target then.
+    const bool none = q.lo > q.hi;
+    if (!none && listed != bucket) {
         find_active(r, s, bucket);
         r.collect(q, r.key_at(q.lo), r.key_at(q.hi));
         listed = q.n <= kMostList ? bucket : -1;
-        // (sums that differ by a rounding may show something in an empty bucket: what is before it reaches the target then)
-        if (q.n == 0) {
-            if (threadIdx.x == 0) q.reach = q.before;
-            return q.hi + 1;
-        }
+    }
+    if (none || q.n == 0) {
+        if (threadIdx.x == 0) q.reach = q.before;
+        __syncthreads();
+        return q.hi + 1;
     }
     uint32_t n = q.n;
     bool have = n <= kMostList;

@@ -85,3 +85,34 @@ def test_halves_of_the_same_sum(hpt, dev):
             assert np.isin(token, [1535, n]).all(), (settings, token[~np.isin(token, [1535, n])][:4])
             w = np.exp2(x[:count])
             near(logp, np.log(w[np.arange(count), token] / w.sum(-1)), 30 * F32_STEP)
+
+
+# (temperature, numbers of logits 200, 199, ..., how far below 200 1500 and 2500 more lie, top_p): with the sums of the kernels top_p's border lies in a bucket of which rounding
+# makes something though it is empty, and in which no bf16 number lies
+BETWEEN = [
+    (6.53, [67, 221, 131, 264, 243, 34, 81, 59, 53, 20, 252, 248], 17, 0.7570882010828001),
+    (6.45, [135, 298, 217, 230, 88, 29, 108], 10, 0.5078388538921861),
+    (6.26, [23, 172, 268, 218, 16, 186, 153, 42, 194, 252, 292, 246], 16, 0.7572712300091017),
+    (6.31, [190, 133, 209, 67, 272, 32, 114], 14, 0.6392513511158395),
+    (6.74, [165, 115, 192, 84, 102, 141, 212], 10, 0.4474014156237754),
+    (6.86, [99, 293, 289, 102, 77, 50, 10, 256, 173, 230], 13, 0.6240515076129396),
+]
+
+
+@pytest.mark.parametrize("case", range(len(BETWEEN)))
+def test_a_border_in_an_empty_bucket(hpt, dev, case):
+    temperature, counts, low, top_p = BETWEEN[case]
+    x = np.full((1, 8192), -np.inf)
+    many = sum(counts)
+    x[0, :many] = 200.0 - np.repeat(np.arange(len(counts)), counts)
+    x[0, many:many + 4000] = 200.0 - low - np.repeat([0, 1], [1500, 2500])
+    t = Kind(hpt, "bf16").up(x)[0]
+    w = np.exp((x[0] - 200) / temperature)
+    assert abs(w[:many].sum() / w.sum() - top_p) < 2.0 ** -40
+    for u in (0.0, 0.3, 0.9, 0.9999):
+        token, logp = (a.numpy()[0] for a in t.sample(up(hpt, np.array([u], np.float32)), temperature=temperature, top_p=top_p))
+        # (the first of those below may or may not be needed to reach top_p)
+        upto = w[:many + 1].cumsum()
+        wants = {int((upto[:n] <= np.float32(u) * upto[n - 1]).sum()) for n in (many, many + 1)}
+        assert token in wants, (token, wants, many)
+        near(logp, np.log(w[token] / upto[many - 1]), 20 * F32_STEP + w[many] / upto[many])
