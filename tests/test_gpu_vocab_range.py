@@ -9,9 +9,10 @@ import pytest
 
 from block_util import F32_STEP, Guarded, Kind, near, up
 from test_gpu_block_calls import P, hip, stream  # noqa: F401
-from vocab_util import order
+from vocab_util import order, sampled
 
 pytestmark = pytest.mark.gpu
+TYPES = ["f32", "f16", "bf16"]
 
 
 # ---- scratch ------------------------------------------------------------------------------------
@@ -116,3 +117,31 @@ def test_a_border_in_an_empty_bucket(hpt, dev, case):
         wants = {int((upto[:n] <= np.float32(u) * upto[n - 1]).sum()) for n in (many, many + 1)}
         assert token in wants, (token, wants, many)
         near(logp, np.log(w[token] / upto[many - 1]), 20 * F32_STEP + w[many] / upto[many])
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("settings", [dict(top_k=1500, top_p=0.9003), dict(top_k=4000, top_p=0.3001), dict(top_p=0.65037), dict(temperature=1e12, top_p=0.30003), dict(top_k=777, top_p=0.5003)], ids=str)
+def test_tied_rows_that_decide_clearly(hpt, dev, name, settings):
+    """Rows of equal logits, of few values, and of masks, with a border and a u that no part of them equals."""
+    kind, rng, cols = Kind(hpt, name), np.random.default_rng(11), 20001
+    low = {"f32": -3.4028235e38, "f16": -65504.0, "bf16": -3.3895314e38}[name]
+    x = np.zeros((8, cols))
+    x[1] = -7.25
+    x[2] = low
+    x[3, cols // 2:] = -np.inf
+    x[4, :cols // 3] = low
+    x[5] = np.where(np.arange(cols) % 2, 3.0, 3.5)
+    x[6] = rng.integers(0, 3, cols) / 8
+    x[7] = np.where(np.arange(cols) % 5, low, 1.0)
+    t, x = kind.up(x)
+    u = np.array([0.30103, 0.61803, 0.14159, 0.71828, 0.57721, 0.41421, 0.73205, 0.23606], np.float32)
+    with np.errstate(over="ignore"):
+        want = [sampled(x[r], u[r], **settings) for r in range(8)]
+    clear = np.array([w[2] > 2.0 ** -36 for w in want])
+    assert clear.all(), [w[2] for w in want]
+    for rep in (1, 40, 200):
+        v = hpt.Tensor.from_raw(t.ptr, [rep, 8, cols], kind.dtype, 0, [0, cols, 1])
+        token, logp = v.sample(up(hpt, np.tile(u, rep)), **settings)
+        assert np.array_equal(token.numpy(), np.broadcast_to([w[0] for w in want], (rep, 8)))
+        logs = np.array([w[1] for w in want])
+        near(logp.numpy(), np.broadcast_to(logs, (rep, 8)), F32_STEP * np.abs(logs) + 1e-11)
