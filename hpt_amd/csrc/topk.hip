@@ -50,23 +50,26 @@ __global__ __launch_bounds__(kTileGroups) void topk_groups_kernel(const TopkArgs
         const uint32_t key = group_key<T>(p);
         ((KeyOf<T>*)a.keys)[at * kTileGroups + threadIdx.x] = (KeyOf<T>)key;
         if constexpr (LSE) {
-            // a wavefront's part of the sum, below its own largest (log2 e / temperature as one f32: 2^-25 of a distance D, which costs the log D / 2^25; two pieces are a sixth more
-            // instructions of a kernel that is bound by them)
-            const float steps = a.steps.hi + a.steps.lo;
+            // a wavefront's part of the sum, below its own largest: in 32 bits within a vector, by twos, in 64 beyond. (Exponents from log2 e / temperature in two pieces: as one f32
+            // it would be 2^-25 of a distance D off itself, and all terms at D with it.)
             const uint32_t top = wave_max(key);
-            float part = 0.0f;
+            double part = 0.0;
             // (NaN, +inf and nothing but -inf are told from the largest alone)
             const bool number = top < kInfKey<T> && top > kNegInfKey<T>;
             const float most = number ? value_of<T>(top) : top == kInfKey<T> ? __builtin_huge_valf() : top <= kNegInfKey<T> ? -__builtin_huge_valf() : __builtin_nanf("");
             if (number) {
 #pragma unroll
-                for (int b = 0; b < V; ++b)
+                for (int b = 0; b < V; ++b) {
+                    float e[VEC];
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        part += __builtin_amdgcn_exp2f((Elem<T>::widen(p[b].v[i]) - most) * steps);
+                        const float d = Elem<T>::widen(p[b].v[i]) - most;
+                        e[i] = __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo));
                     }
+                    part += (double)sum_by_twos(e);
+                }
             }
-            const double sum = group_reduce<SumD>((double)part, 64);
+            const double sum = group_reduce<SumD>(part, 64);
             if ((threadIdx.x & 63) == 0) {
                 double* to = a.sums + (at * kTileWaves + (threadIdx.x >> 6)) * 2;
                 to[0] = most;
@@ -89,26 +92,38 @@ template <class T> struct Answer {
         else ((int32_t*)a.index)[row * a.k + rank] = (int32_t)i;
     }
 };
-// The log of the sum from its parts, by a wavefront. They are weighted by the hardware's exponential: one of -D is off by D / 2^24 of itself or so, which is D e^-D / 2^24
-// of the sum at most, less than a rounding. The sum is at least 1; its logarithm in 32 bits is off by one part of 2^24 of lse at most.
-__device__ __forceinline__ void store_lse(const TopkArgs& a, const double* p, int64_t row) {
-    const int lane = threadIdx.x & 63;
-    const float steps = a.steps.hi + a.steps.lo;
-    auto scale = [&](double from, double to) { return (double)(from == to ? 1.0f : __builtin_amdgcn_exp2f((float)(from - to) * steps)); };
-    double top = -__builtin_huge_val(), sum = 0.0;
-    bool nan = false;
-    for (int t = lane; t < a.tiles * kTileWaves; t += 64) {
-        const double most = p[2 * t], part = p[2 * t + 1], n = fmax(top, most);
+// The largest logit of a row and its sum of exponentials below that, from the row's parts, for a wavefront. Parts are weighted by the hardware's exponential of a fraction (two half steps), and by whole octaves.
+struct RowSum {
+    double most, sum;
+};
+__device__ __forceinline__ RowSum sum_of_parts(const TopkArgs& a, const double* p) {
+    const int lane = threadIdx.x & 63, parts = a.tiles * kTileWaves;
+    const double inf = __builtin_huge_val(), steps = 1.4426950408889634 * a.inv_temperature;
+    // (a lane's first part stays; those of longer rows are fetched again)
+    const bool any = lane < parts;
+    const double most0 = any ? p[2 * lane] : -inf, part0 = any ? p[2 * lane + 1] : 0.0;
+    double all = most0;
+    bool nan = most0 != most0;
+    for (int t = lane + 64; t < parts; t += 64) {
+        const double most = p[2 * t];
         nan |= most != most;
-        sum = sum * scale(top, n) + (part > 0.0 ? part * scale(most, n) : 0.0);
-        top = n;
+        all = fmax(all, most);
     }
-    double all = top;
 #pragma unroll
     for (int w = 1; w < 64; w <<= 1) all = fmax(all, shfl_xor_any(all, w));
-    sum = group_reduce<SumD>(sum * scale(top, all), 64);
-    if (__any(nan)) all = __builtin_nan("");
-    if (lane == 0) a.lse[row] = (float)(all * a.inv_temperature + (fabs(all) < __builtin_huge_val() ? (double)__builtin_amdgcn_logf((float)sum) * 0.6931471805599453 : 0.0));
+    auto share = [&](double most, double part) {
+        const double d = fmax((most - all) * steps, -1000.0), whole = rint(d);
+        return part > 0.0 ? part * ldexp((double)__builtin_amdgcn_exp2f((float)(d - whole)), (int)whole) : 0.0;
+    };
+    double sum = share(most0, part0);
+    for (int t = lane + 64; t < parts; t += 64) sum += share(p[2 * t], p[2 * t + 1]);
+    sum = group_reduce<SumD>(sum, 64);
+    return {__any(nan) ? __builtin_nan("") : all, sum};
+}
+// The logarithm is one of 64 bits: what is off in lse are the parts' roundings, some 2^-24 of the sum whatever lse's own size, and its own one. (32 bits of it would be 2^-24 of the logarithm, of which
+// little may be left in lse: of log-probabilities, nothing.)
+__device__ __forceinline__ void store_lse(const TopkArgs& a, const RowSum& s, int64_t row) {
+    a.lse[row] = (float)(s.most * a.inv_temperature + (fabs(s.most) < __builtin_huge_val() ? log(s.sum) : 0.0));
 }
 
 // A workgroup for each row.
@@ -120,14 +135,17 @@ __global__ __launch_bounds__(1024) void topk_pick_kernel(const TopkArgs a, int64
         const int n = collect_top(s, LogitRow<T>(x, a.cols), (const KeyOf<T>*)a.keys + r * a.tiles * kTileGroups, a.tiles, a.k, kTileGroups * sizeof(T));
         rank_top(s, n, a.k, Answer<T>{a, x, row0 + r});
         // (the last wavefront has fewest places to rank)
-        if (LSE && threadIdx.x >= blockDim.x - 64) store_lse(a, a.sums + 2 * r * a.tiles * kTileWaves, row0 + r);
+        if (LSE && threadIdx.x >= blockDim.x - 64) {
+            const RowSum sum = sum_of_parts(a, a.sums + 2 * r * a.tiles * kTileWaves);
+            if (threadIdx.x == blockDim.x - 64) store_lse(a, sum, row0 + r);
+        }
         __syncthreads();
     }
 }
 
-// A wavefront for each row, few places. A row of which it would collect too much is left to the workgroup.
+// A wavefront for each row, few places. A row of which it would collect too much is left to the workgroup. (As many wavefronts of a SIMD as LDS has room for.)
 template <class T, bool LSE>
-__global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a, int64_t row0, int64_t rows) {
+__global__ __launch_bounds__(kTileGroups, 5) void topk_wave_kernel(const TopkArgs a, int64_t row0, int64_t rows) {
     constexpr int N = kTileGroups / 64;
     __shared__ union {
         WaveShared wave[N];
@@ -135,6 +153,7 @@ __global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a
     } s;
     static_assert(kWaveTop <= 512, "the first k fit the list");
     __shared__ int left[N];
+    __shared__ RowSum sums[LSE ? N : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int64_t r0 = (int64_t)blockIdx.x * N; r0 < rows; r0 += (int64_t)gridDim.x * N) {
         const int64_t r = r0 + wave;
@@ -143,10 +162,15 @@ __global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a
             const T* x = (const T*)a.x + offset_of(a.kept, row0 + r);
             n = wave_top(s.wave[wave], LogitRow<T>(x, a.cols), (const KeyOf<T>*)a.keys + r * a.tiles * kTileGroups, a.tiles, a.k, kTileGroups * sizeof(T));
             if (n >= 0) wave_rank(s.wave[wave], n, a.k, Answer<T>{a, x, row0 + r});
-            if (LSE) store_lse(a, a.sums + 2 * r * a.tiles * kTileWaves, row0 + r);
+            if constexpr (LSE) {
+                const RowSum sum = sum_of_parts(a, a.sums + 2 * r * a.tiles * kTileWaves);
+                if ((threadIdx.x & 63) == 0) sums[wave] = sum;
+            }
         }
         if ((threadIdx.x & 63) == 0) left[wave] = n < 0;
         __syncthreads();
+        // (logarithms of the workgroup's rows side by side, a lane each)
+        if (LSE && threadIdx.x < N && r0 + threadIdx.x < rows) store_lse(a, sums[LSE ? threadIdx.x : 0], row0 + r0 + threadIdx.x);
         for (int w = 0; w < N; ++w) {
             if (!left[w]) continue;
             const T* x = (const T*)a.x + offset_of(a.kept, row0 + r0 + w);
@@ -158,60 +182,80 @@ __global__ __launch_bounds__(kTileGroups) void topk_wave_kernel(const TopkArgs a
     }
 }
 
+constexpr int kMostEach = 4;  // rows of a wavefront
 // Rows of at most 64 N elements, a wavefront each, one launch: the row stays in registers (element i of lane l is at 64 i + l), and the largest is taken out k times.
 template <class T, int N, bool LSE>
-__global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a) {
+__global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a, int each) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows; row += (int64_t)gridDim.x * 4) {
-        const T* x = (const T*)a.x + offset_of(a.kept, row);
-        T v[N];
-        uint32_t key[N];
+    __shared__ RowSum sums[LSE ? 4 * kMostEach : 1];
+    for (int64_t row0 = (int64_t)blockIdx.x * 4 * each; row0 < a.rows; row0 += (int64_t)gridDim.x * 4 * each) {
+        for (int n = 0; n < each; ++n) {
+            const int64_t row = row0 + n * 4 + wave;
+            if (row >= a.rows) break;
+            const T* x = (const T*)a.x + offset_of(a.kept, row);
+            T v[N];
+            uint32_t key[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = x[min(i * 64 + lane, a.cols - 1)];
+            for (int i = 0; i < N; ++i) v[i] = x[min(i * 64 + lane, a.cols - 1)];
 #pragma unroll
-        for (int i = 0; i < N; ++i) key[i] = i * 64 + lane < a.cols ? key_of(v[i]) : 0;
-        uint32_t best = 0;
-        int which = 0;
-        auto find = [&] {
-            best = 0;
+            for (int i = 0; i < N; ++i) key[i] = i * 64 + lane < a.cols ? key_of(v[i]) : 0;
+            uint32_t best = 0;
+            int which = 0;
+            auto find = [&] {
+                best = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (key[i] > best) {
-                    best = key[i];
-                    which = i;
-                }
-        };
-        find();
-        if constexpr (LSE) {
-            // (as the groups' launch and store_lse have it)
-            const float steps = a.steps.hi + a.steps.lo;
-            const uint32_t top = wave_max(best);
-            const bool number = top < kInfKey<T> && top > kNegInfKey<T>;
-            const float most = number ? value_of<T>(top) : top == kInfKey<T> ? __builtin_huge_valf() : top <= kNegInfKey<T> ? -__builtin_huge_valf() : __builtin_nanf("");
-            float part = 0.0f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) part += i * 64 + lane < a.cols ? __builtin_amdgcn_exp2f((Elem<T>::widen(v[i]) - most) * steps) : 0.0f;
-            const double sum = group_reduce<SumD>((double)part, 64);
-            if (lane == 0) a.lse[row] = (float)((double)most * a.inv_temperature + (number ? (double)__builtin_amdgcn_logf((float)sum) * 0.6931471805599453 : 0.0));
-        }
-        uint32_t mine = 0, at = 0;
-#pragma clang loop unroll(disable)
-        for (int r = 0; r < a.k; ++r) {
-            const uint32_t most = wave_max(best);
-            const uint64_t who = __ballot(best == most);
-            int l = __builtin_ctzll(who);
-            if (who & (who - 1)) l = (int)(~wave_max(best == most ? ~(uint32_t)(which * 64 + lane) : 0u) & 63);  // (equal ones: the first)
-            const uint32_t index = (uint32_t)lane_of(which, l) * 64 + l;
-            if (lane == r) {
-                mine = most;
-                at = index;
-            }
-            const int gone = lane == l ? which : -1;
-#pragma unroll
-            for (int i = 0; i < N; ++i) key[i] = i == gone ? 0 : key[i];
+                for (int i = 0; i < N; ++i)
+                    if (key[i] > best) {
+                        best = key[i];
+                        which = i;
+                    }
+            };
             find();
+            if constexpr (LSE) {
+                // (as the groups' launch has it)
+                constexpr int M = N < 4 ? N : 4;
+                const uint32_t top = wave_max(best);
+                const bool number = top < kInfKey<T> && top > kNegInfKey<T>;
+                const float most = number ? value_of<T>(top) : top == kInfKey<T> ? __builtin_huge_valf() : top <= kNegInfKey<T> ? -__builtin_huge_valf() : __builtin_nanf("");
+                double part = 0.0;
+#pragma unroll
+                for (int i = 0; i < N; i += M) {
+                    float e[M];
+#pragma unroll
+                    for (int j = 0; j < M; ++j) {
+                        const float d = Elem<T>::widen(v[i + j]) - most;
+                        e[j] = (i + j) * 64 + lane < a.cols ? __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo)) : 0.0f;
+                    }
+                    part += (double)sum_by_twos(e);
+                }
+                const double sum = group_reduce<SumD>(part, 64);
+                if (lane == 0) sums[n * 4 + wave] = {most, sum};
+            }
+            uint32_t mine = 0, at = 0;
+#pragma clang loop unroll(disable)
+            for (int r = 0; r < a.k; ++r) {
+                const uint32_t first = wave_max(best);
+                const uint64_t who = __ballot(best == first);
+                int l = __builtin_ctzll(who);
+                if (who & (who - 1)) l = (int)(~wave_max(best == first ? ~(uint32_t)(which * 64 + lane) : 0u) & 63);  // (equal ones: the first)
+                const uint32_t index = (uint32_t)lane_of(which, l) * 64 + l;
+                if (lane == r) {
+                    mine = first;
+                    at = index;
+                }
+                const int gone = lane == l ? which : -1;
+#pragma unroll
+                for (int i = 0; i < N; ++i) key[i] = i == gone ? 0 : key[i];
+                find();
+            }
+            if (lane < a.k) Answer<T>{a, x, row}(lane, place_of(mine, at));
         }
-        if (lane < a.k) Answer<T>{a, x, row}(lane, place_of(mine, at));
+        if constexpr (LSE) {
+            // (logarithms of the workgroup's rows side by side)
+            __syncthreads();
+            if (threadIdx.x < 4 * each && row0 + threadIdx.x < a.rows) store_lse(a, sums[threadIdx.x], row0 + threadIdx.x);
+            __syncthreads();
+        }
     }
 }
 
@@ -225,7 +269,9 @@ void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {
     HPT_WITH_TYPE(dtype, {
         if (topk_in_registers(a.rows, a.cols, a.k)) {
             auto small = [&](auto n, auto lse) {
-                topk_small_kernel<T, decltype(n)::value, decltype(lse)::value><<<(unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20), 256, 0, st>>>(a);
+                // (rows' logarithms side by side, with lse: f32 [100000, 64], k = 8, 42.5 us of four rows a wavefront and 46.5 of one, [16384, 64] 10.5 and 10.2)
+                const int each = decltype(lse)::value && a.rows > 32768 ? kMostEach : 1;
+                topk_small_kernel<T, decltype(n)::value, decltype(lse)::value><<<(unsigned)std::min<int64_t>((a.rows + 4 * each - 1) / (4 * each), 1 << 20), 256, 0, st>>>(a, each);
             };
             auto sized = [&](auto lse) {
                 if (a.cols <= 64) small(std::integral_constant<int, 1>{}, lse);

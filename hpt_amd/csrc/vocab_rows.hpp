@@ -227,6 +227,14 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     v = max(v, dpp_or_zero<0x143, 0xC>(v));
     return lane_of(v, 63);
 }
+// The sum of N numbers (a power of two) of this lane, two by two: log2 N roundings deep.
+template <int N> __device__ __forceinline__ float sum_by_twos(float (&v)[N]) {
+#pragma unroll
+    for (int w = N / 2; w > 0; w /= 2)
+#pragma unroll
+        for (int i = 0; i < w; ++i) v[i] += v[i + w];
+    return v[0];
+}
 // The sum of v over the threads before this one; `total`: over all of them. Every order is fixed. `place`: one number for each wavefront.
 __device__ __forceinline__ double scan_before(double v, double* place, double& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;

@@ -9,7 +9,7 @@ import pytest
 
 from block_util import F32_STEP, Guarded, Kind, near, up
 from test_gpu_block_calls import P, hip, stream  # noqa: F401
-from vocab_util import order, sampled
+from vocab_util import logsumexp, order, sampled
 
 pytestmark = pytest.mark.gpu
 TYPES = ["f32", "f16", "bf16"]
@@ -145,3 +145,48 @@ def test_tied_rows_that_decide_clearly(hpt, dev, name, settings):
         assert np.array_equal(token.numpy(), np.broadcast_to([w[0] for w in want], (rep, 8)))
         logs = np.array([w[1] for w in want])
         near(logp.numpy(), np.broadcast_to(logs, (rep, 8)), F32_STEP * np.abs(logs) + 1e-11)
+
+
+# ---- top-k: the log of the sum -----------------------------------------------------------------------------
+
+
+def lse_tolerance(z):
+    """A term at distance D below the largest is off by 2 D (its distance and its exponent are rounded) + 2 (the exponential) half steps, and by 3 of the sum of eight of them; the join of
+    wavefronts' parts is another exponential's 2 of what is not next to the largest, and the result is rounded once. Terms at distance 0 are 1."""
+    d = z.max(-1, keepdims=True) - z
+    p = np.exp(z - logsumexp(z)[:, None])
+    return F32_STEP * ((p * np.where(d > 0, 2 * d + 4, 0)).sum(-1) + np.where((d > 0).any(-1), 3, 0) + np.abs(logsumexp(z))) + 1e-13
+
+
+LENGTHS = [(3, 6), (3, 64), (700, 256), (5, 1000), (700, 2000), (3, 5000), (300, 20001), (1100, 20001), (2, 152000), (40003, 70)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,cols", LENGTHS)
+def test_the_sum_of_equal_logits(hpt, dev, name, rows, cols):
+    """Every term is 1: only the result is rounded, also where the logits are about the negative log of their number and the result is next to 0."""
+    kind = Kind(hpt, name)
+    x = np.array([0.0, -np.log(cols), 1.25, -100.0, 300.0, -3e4, -np.log(cols) + 1e-3])
+    for tau in (1.0, 2.0, 0.7):
+        for value in x:
+            t, v = kind.up(np.full((1, cols), value * tau))
+            b = hpt.Tensor.from_raw(t.ptr, [rows, cols], kind.dtype, 0, [0, 1])
+            want = logsumexp(v / tau)
+            near(b.topk(3, lse=True, temperature=tau)[2].numpy(), np.broadcast_to(want, rows), F32_STEP * np.abs(want) + 1e-12 * (1 + np.abs(v[0, 0] / tau)), f"{value} at {tau}")
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,cols", LENGTHS)
+@pytest.mark.parametrize("sd", [0.3, 3.0, 8.0])
+def test_the_sum_to_a_few_roundings(hpt, dev, name, rows, cols, sd):
+    """Logits, and log-probabilities, whose sum is 1."""
+    kind, rng = Kind(hpt, name), np.random.default_rng(cols)
+    x = rng.standard_normal((3, cols)) * sd
+    x[1] -= logsumexp(x[1:2])
+    x[2, 0] = x[2].max() + 6 * sd + 5
+    x[2] -= logsumexp(x[2:3])
+    for tau in (1.0, 1.7):
+        t, v = kind.up(x * tau)
+        n = max(1, rows // 3)
+        b = hpt.Tensor.from_raw(t.ptr, [n, 3, cols], kind.dtype, 0, [0, cols, 1])
+        near(b.topk(5, lse=True, temperature=tau)[2].numpy(), np.broadcast_to(logsumexp(v / tau), (n, 3)), lse_tolerance(v / tau))
