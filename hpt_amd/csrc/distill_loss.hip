@@ -51,53 +51,48 @@ constexpr int kGradVecs = 4;  // vectors of a lane
 struct RowSums {
     double most, sum;          // of the logits (of those that no entry names, where the rest counts)
     double named_most, named;  // of the others
-    double teacher_most, a, b; // of the entries: sum e, sum e (t - x) / temperature with e = exp((t - teacher_most) / temperature)
+    // of the entries: sum e, sum e ((t - teacher_most) - (x - the larger of most and named_most)) / temperature with e = exp((t - teacher_most) / temperature)
+    double teacher_most, a, b;
 };
 
-// A row's divergence, and what its gradient needs: log2 of the sums that probabilities are over, in two pieces each (f32 alone would cost a gradient |lse| / 2^24 of itself).
+// A row's divergence, and what its gradient needs. Logits count by their distances below the largest alone, the teacher's too (but for its own log of the sum): they may lie anywhere, as in a
+// row of which a mask has left nothing but -1e9 or the type's lowest value. Terms: 0 the largest logit, 1 what a named token's exponential below it is multiplied by; 2 and 3 the same of an
+// unnamed one; 4 and 5 the same of an entry's; 7 the weight.
 __device__ __forceinline__ double finish_row(const DistillArgs& a, int64_t row, const RowSums& s) {
-    const double inv = 1.0 / a.temperature, inf = __builtin_huge_val();
-    double lse, rest, kl, base, coef = 1.0, teacher;
-    bool counts = true;
+    const double inv = 1.0 / a.temperature;
+    float* t = a.terms + row * kTerms;
+    double kl;
     if (!a.teacher_lse) {
-        lse = rest = s.most * inv + log(s.sum);
-        base = lse * kLog2eD;
-        teacher = s.teacher_most * inv + log(s.a);
-        kl = s.b / s.a - teacher + lse;
-        counts = s.a != 0.0;
-        if (!counts) kl = 0.0;
+        kl = s.a == 0.0 ? 0.0 : s.b / s.a - log(s.a) + log(s.sum);
+        t[0] = t[2] = (float)s.most;
+        t[1] = t[3] = (float)(1.0 / s.sum);
+        t[4] = (float)s.teacher_most;
+        t[5] = (float)(1.0 / s.a);
     } else {
         // (one exponential for both sums' distance; equal infinities are no distance apart)
         const bool below = s.most < s.named_most;
         const double far = s.most == s.named_most ? 1.0 : exp(-fabs(s.most - s.named_most) * inv);
-        const double left = s.sum * (below ? far : 1.0), all = left + s.named * (below ? 1.0 : far);
-        lse = fmax(s.most, s.named_most) * inv + log(all);
-        teacher = a.teacher_lse[row];
-        const double part = s.a == 0.0 ? 0.0 : exp(s.teacher_most * inv - teacher), q = s.a * part;
+        const double left = s.sum * (below ? far : 1.0), all = left + s.named * (below ? 1.0 : far), log_all = log(all);
+        const double largest = fmax(s.most, s.named_most), beyond = s.teacher_most * inv - a.teacher_lse[row];
+        const double part = s.a == 0.0 ? 0.0 : exp(beyond), q = s.a * part;
         const bool others = s.sum != 0.0;
         double r = 1.0 - q, mass = 1.0;
         if (!others || r < 0.0) {
             r = 0.0;
             mass = q;
         }
-        rest = others ? s.most * inv + log(s.sum) : lse;
-        kl = r == 0.0 ? 0.0 : r * (log(r) - (rest - lse));
-        if (q != 0.0) kl += part * s.b + q * (lse - teacher);
-        base = lse * kLog2eD - (mass == 1.0 ? 0.0 : log2(mass));
-        coef = others ? mass * (left / all) - r : 0.0;
+        kl = r == 0.0 ? 0.0 : r * (log(r) - ((s.most - largest) * inv + log(s.sum) - log_all));
+        if (q != 0.0) kl += part * s.b + q * (beyond + log_all);
+        t[0] = (float)largest;
+        t[1] = (float)(mass / all);
+        t[2] = (float)(others ? s.most : largest);
+        t[3] = others ? (float)((mass * (left / all) - r) / s.sum) : 0.0f;
+        t[4] = s.a == 0.0 ? 0.0f : (float)s.teacher_most;
+        t[5] = (float)part;
     }
     a.kl[row] = (float)kl;
-    float* t = a.terms + row * kTerms;
-    auto pieces = [&](float* to, double v) {
-        const float hi = (float)v;
-        to[0] = hi;
-        to[1] = fabsf(hi) < (float)inf ? (float)(v - (double)hi) : 0.0f;
-    };
-    pieces(t, base);
-    pieces(t + 2, rest * kLog2eD);
-    pieces(t + 4, teacher * kLog2eD);
-    t[6] = (float)coef;
-    t[7] = counts ? 1.0f : 0.0f;  // (becomes the weight in the last launch)
+    t[6] = 0.0f;
+    t[7] = a.teacher_lse || s.a != 0.0 ? 1.0f : 0.0f;  // (becomes the weight in the last launch)
     return kl;
 }
 __device__ __forceinline__ void skip_row(const DistillArgs& a, int64_t row) {
@@ -231,7 +226,6 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
     const double inf = __builtin_huge_val(), inv = 1.0 / a.temperature;
     const T* x = (const T*)a.x + offset_of(a.kept, row);
     RowSums r{-inf, 0.0, -inf, 0.0, -inf, 0.0, 0.0};
-    const float steps = a.steps.hi + a.steps.lo;
     double twice = 0.0;
     if (lane < a.split) {
         const double* p = a.partial + (row * a.split + lane) * kDistillPart;
@@ -269,6 +263,19 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
     }
     teacher_most = group_reduce<MaxF>(teacher_most, 64);
     named_most = group_reduce<MaxF>(named_most, 64);
+    // the parts together
+    if (a.split > 1) {
+        double most = r.most;
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) most = fmax(most, shfl_xor_any(most, w));
+        if (r.sum != 0.0) r.sum *= exp((r.most - most) * inv);
+        r.sum = group_reduce<SumD>(r.sum, 64);
+        r.most = most;
+    } else {
+        r.sum = lane_of(r.sum, 0);
+        r.most = lane_of(r.most, 0);
+    }
+    const double largest = fmax(r.most, (double)named_most);
     for (int j0 = 0; j0 < a.k; j0 += 256) {
         if (a.k > 256)
 #pragma unroll
@@ -279,7 +286,7 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
             if (e.token < 0 || e.token == a.cols) continue;
             const double p = e.t == -(float)inf ? 0.0 : exp(((double)e.t - (double)teacher_most) * inv);
             r.a += p;
-            if (p != 0.0) r.b += p * (((double)e.t - (double)e.x) * inv);
+            if (p != 0.0) r.b += p * ((((double)e.t - (double)teacher_most) - ((double)e.x - largest)) * inv);
         }
         if (rest) {
             // the student's, each token once: where one is named twice, an entry whose token one before it names is passed over
@@ -301,16 +308,6 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
     r.named = group_reduce<SumD>(r.named, 64);
     r.teacher_most = teacher_most;
     r.named_most = named_most;
-    // (lane 0 has them all)
-    if (a.split > 1) {
-        for (int w = 1; w < a.split; w <<= 1) {
-            const double m2 = shfl_xor_any(r.most, w), s2 = shfl_xor_any(r.sum, w), n = fmax(r.most, m2);
-            // (the hardware's exponential: one of -D is off by D / 2^24 of itself or so, which is D e^-D / 2^24 of the row's sum at most, less than a rounding)
-            const float f1 = r.most == n ? 1.0f : __builtin_amdgcn_exp2f((float)(r.most - n) * steps), f2 = m2 == n ? 1.0f : __builtin_amdgcn_exp2f((float)(m2 - n) * steps);
-            r.sum = r.sum * (double)f1 + s2 * (double)f2;
-            r.most = n;
-        }
-    }
     return r;
 }
 
@@ -402,7 +399,8 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
             if (lane < head) first = x[lane];
             if (lane < n - tail) last = x[tail + lane];
         }
-        const float rest_hi = terms[2], rest_lo = terms[3], coef = w * terms[6];
+        const float rest_most = terms[2], coef = w * terms[3];
+        auto below = [&](float d) { return __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo)); };
         // a token's bit stands so that those of a vector stand together
         const int shift = VEC - head;
         if (on) {
@@ -425,11 +423,11 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
             while (mine) {
                 const int j = __builtin_ctz(mine) * 64 + lane, e = token(j);
                 mine &= mine - 1;
-                const double teacher = (double)terms[4] + (double)terms[5], per = kLog2eD / a.temperature;
+                const double teacher_most = terms[4], per = kLog2eD / a.temperature;
                 // (the exponent in 64 bits, its fraction's power by the hardware: the library's 64-bit routine costs a wavefront a SIMD in registers)
                 auto prob = [&](int j) {
-                    const double d = (double)logit_of(a.teacher, a.teacher_dtype, row * a.k + j) * per - teacher, whole = rint(d);
-                    return d < -160.0 ? 0.0f : ldexpf(__builtin_amdgcn_exp2f((float)(d - whole)), (int)fmin(whole, 1000.0));
+                    const double d = ((double)logit_of(a.teacher, a.teacher_dtype, row * a.k + j) - teacher_most) * per, whole = rint(d);
+                    return d < -160.0 ? 0.0f : terms[5] * ldexpf(__builtin_amdgcn_exp2f((float)(d - whole)), (int)whole);
                 };
                 const float f = Elem<T>::widen(x[e - e0]);
                 float q = prob(j);
@@ -439,13 +437,13 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
                     for (int l = j + 1; l < a.k && is_first; ++l)
                         if (token(l) == e) q += prob(l);
                 }
-                const float y = __builtin_amdgcn_exp2f(fmaf(f, a.steps.hi, -terms[0]) + fmaf(f, a.steps.lo, -terms[1]));
+                const float y = terms[1] * below(f - terms[0]);
                 if (is_first) out[e - e0] = Elem<T>::narrow(w * (y - q));
             }
         }
         auto grad = [&](T v) {
             const float f = Elem<T>::widen(v);
-            return Elem<T>::narrow(coef * __builtin_amdgcn_exp2f(fmaf(f, a.steps.hi, -rest_hi) + fmaf(f, a.steps.lo, -rest_lo)));
+            return Elem<T>::narrow(coef * below(f - rest_most));
         };
         auto is_named = [&](int e) { return on && bits[(e + shift) >> 5] >> ((e + shift) & 31) & 1; };
         if (lane < head && !is_named(lane)) out[lane] = on ? grad(first) : first;

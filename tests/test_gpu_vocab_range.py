@@ -190,3 +190,110 @@ def test_the_sum_to_a_few_roundings(hpt, dev, name, rows, cols, sd):
         n = max(1, rows // 3)
         b = hpt.Tensor.from_raw(t.ptr, [n, 3, cols], kind.dtype, 0, [0, cols, 1])
         near(b.topk(5, lse=True, temperature=tau)[2].numpy(), np.broadcast_to(logsumexp(v / tau), (n, 3)), lse_tolerance(v / tau))
+
+
+# ---- distillation: logits anywhere -------------------------------------------------------------------------
+
+
+def diverged(x, t, index, tau, teacher_lse=None):
+    """(kl, its gradient by x / tau) of each row, every entry a token of its own, from distances alone: what lies so far below that its probability is no number of 64 bits still has a logarithm."""
+    rows = len(x)
+    kl, grad = np.zeros(rows), np.zeros(x.shape)
+    for r in range(rows):
+        z = (x[r] - x[r].max()) / tau
+        e = (t[r] - t[r].max()) / tau
+        lse = logsumexp(z)
+        logq = e - logsumexp(e) if teacher_lse is None else t[r] / tau - teacher_lse[r]
+        q = np.exp(logq)
+        rest = 0.0 if teacher_lse is None else max(0.0, 1 - q.sum())
+        on = q > 0
+        kl[r] = (q[on] * (logq[on] - (z[index[r]][on] - lse))).sum()
+        grad[r] = (q.sum() + rest) * np.exp(z - lse)
+        grad[r, index[r]] -= q
+        if rest:
+            out = np.ones(len(z), bool)
+            out[index[r]] = False
+            logs = logsumexp(z[out])
+            kl[r] += rest * (np.log(rest) - (logs - lse))
+            grad[r][out] -= rest * np.exp(z[out] - logs)
+    return kl, grad
+
+
+def kl_tolerance(x, tau, kl):
+    """The student's log of the sum, as above (a rescaled sum in 64 bits), and the result's own rounding; of the rest the sum over the unnamed counts too, at most as much."""
+    z = (x - x.max(-1, keepdims=True)) / tau
+    return 2 * (lse_tolerance(z) - F32_STEP * np.abs(logsumexp(z))) + F32_STEP * np.abs(kl) + 1e-12
+
+
+def gradient_tolerance(k, x, t, tau, grad, w, lse_part):
+    """A probability p at distance D is off by 2 D + 2 half steps as above, by its sum's, and by one each of the reciprocal of the sum, its weight, two products and the difference; q by 8, or as p where it is r / s times p; the result by half a step of its
+    type. An exponential below f32's normal numbers may be 0, which loses 2^-126 of p at most."""
+    z = (x - x.max(-1, keepdims=True)) / tau
+    lse = logsumexp(z)[:, None]
+    p = np.exp(z - lse)
+    q = np.abs(p - grad)
+    w = np.abs(w)[:, None]
+    return w * (p + q) * (F32_STEP * (2 * -z + 8) + 2 * lse_part[:, None]) + k.step * np.abs(grad) * w + k.least + 2.0 ** -126 * (1 + w)
+
+
+OFFSETS = [0.0, -1e4, 6e4, -9e4, 1e6, -1e9, 1e12, -1e20, 1e30, -1e37, 1.6e38, "low"]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("rows,cols,n", [(6, 50, 5), (6, 5000, 60), (6, 40001, 300), (2100, 70, 8)])
+def test_students_that_lie_anywhere(hpt, dev, name, rest, rows, cols, n):
+    """The divergence does not change with a number added to all logits of a row, whatever is left of their differences; rows that a mask has left nothing but the type's lowest value."""
+    k, rng = Kind(hpt, name), np.random.default_rng(cols)
+    low = {"f32": -3.4028235e38, "f16": -65504.0, "bf16": -3.3895314e38}[name]
+    for offset in OFFSETS if rows < 100 else OFFSETS[::3] + OFFSETS[-1:]:
+        value = low if offset == "low" else offset
+        if abs(value) > 65504 and name == "f16":
+            continue
+        for tau in (1.0, 2.0, 0.6):
+            teacher = k.round(rng.standard_normal((rows, cols)) * 3)
+            index = order(teacher)[:, :n]
+            tt = np.take_along_axis(teacher, index, -1)
+            lse_t = logsumexp(teacher / tau).astype(np.float32)
+            x = np.full((rows, cols), value)
+            if offset != "low":
+                with np.errstate(over="ignore"):
+                    x = k.round(x + rng.standard_normal((rows, cols)) * max(3.0, abs(value) * 2.0 ** -9))
+                x = np.clip(x, low, -low)
+            x[-1] = value
+            tx, x = k.up(x)
+            args = (k.up(tt)[0], up(hpt, index))
+            kw = dict(teacher_lse=up(hpt, lse_t)) if rest else {}
+            got = tx.distill_loss(*args, temperature=tau, **kw)
+            shifted = x - x.max(-1, keepdims=True)
+            with np.errstate(all="ignore"):
+                want, grad = diverged(x, tt, index, tau, lse_t.astype(np.float64) if rest else None)
+            # (a divergence beyond f32 is an infinity)
+            fits = np.abs(want) < 3.4e38
+            part = lse_tolerance(shifted / tau)
+            near(got.kl.numpy()[fits], want[fits], kl_tolerance(x, tau, want)[fits] + np.abs(want[fits]) * 1e-12, f"kl at {value}, {tau}")
+            scale = float(rows)
+            d = tx.distill_loss_backward(*args, got.terms, temperature=tau, grad=scale)
+            w = np.full(rows, tau)
+            near(k.down(d), grad * tau, gradient_tolerance(k, x, tt, tau, grad, w, part), f"gradient at {value}, {tau}")
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_teachers_that_lie_anywhere(hpt, dev, name):
+    """Without the rest, a number added to all of a teacher's entries changes nothing."""
+    k, rng = Kind(hpt, name), np.random.default_rng(3)
+    low = {"f32": -3.4028235e38, "f16": -65504.0, "bf16": -3.3895314e38}[name]
+    rows, cols, n = 5, 3000, 40
+    x = rng.standard_normal((rows, cols)) * 2
+    index = order(rng.standard_normal((rows, cols)))[:, :n]
+    tx, x = k.up(x)
+    for value in (-1e4, 6e4, -1e9, 1e20, -1e37, low):
+        if abs(value) > 65504 and name == "f16":
+            continue
+        t = k.round(value + (rng.standard_normal((rows, n)) * max(2.0, abs(value) * 2.0 ** -9) if value != low else 0.0 * index))
+        for tau in (1.0, 0.6):
+            got = tx.distill_loss(k.up(t)[0], up(hpt, index), temperature=tau)
+            want, grad = diverged(x, t, index, tau)
+            near(got.kl.numpy(), want, kl_tolerance(x, tau, want))
+            d = tx.distill_loss_backward(k.up(t)[0], up(hpt, index), got.terms, temperature=tau, grad=float(rows))
+            near(k.down(d), grad * tau, gradient_tolerance(k, x, t, tau, grad, np.full(rows, tau), lse_tolerance((x - x.max(-1, keepdims=True)) / tau)))
