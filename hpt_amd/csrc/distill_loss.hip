@@ -315,10 +315,10 @@ template <class T> __device__ __forceinline__ RowSums sums_of_row(const DistillA
 // instructions, for one lane as for all).
 constexpr int kRowsAtOnce = 16;
 template <class T>
-__global__ __launch_bounds__(64 * kRowsAtOnce, 8) void distill_rows_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(64 * kRowsAtOnce, 8) void distill_rows_kernel(const DistillArgs a, int64_t from) {
     __shared__ RowSums sums[kRowsAtOnce];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row0 = (int64_t)blockIdx.x * kRowsAtOnce;
+    const int64_t row0 = from + (int64_t)blockIdx.x * kRowsAtOnce;
     if (row0 + wave < a.rows && mask_of(a.mask, a.mask_bool, row0 + wave) != 0.0f) {
         const RowSums r = sums_of_row<T>(a, row0 + wave);
         if ((threadIdx.x & 63) == 0) sums[wave] = r;
@@ -484,7 +484,10 @@ void launch_distill_loss(int dtype, const DistillArgs& a, hipStream_t st) {
             const unsigned blocks = (unsigned)std::min<int64_t>(a.rows * a.split, 1 << 20);
             if (a.teacher_lse) distill_stats_kernel<T, true><<<blocks, kThreads, 0, st>>>(a);
             else distill_stats_kernel<T, false><<<blocks, kThreads, 0, st>>>(a);
-            distill_rows_kernel<T><<<(unsigned)((a.rows + kRowsAtOnce - 1) / kRowsAtOnce), 64 * kRowsAtOnce, 0, st>>>(a);
+            // (a launch has fewer than 2^32 work items. Walked by the kernel, 49 registers would spill: f32 [100000, 64] 384 -> 631 us)
+            constexpr int64_t most = (int64_t)kRowsAtOnce << 20;
+            for (int64_t from = 0; from < a.rows; from += most)
+                distill_rows_kernel<T><<<(unsigned)((std::min(most, a.rows - from) + kRowsAtOnce - 1) / kRowsAtOnce), 64 * kRowsAtOnce, 0, st>>>(a, from);
         });
     distill_sum_kernel<<<1, 1024, 0, st>>>(a);
 }

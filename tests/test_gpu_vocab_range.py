@@ -297,3 +297,19 @@ def test_teachers_that_lie_anywhere(hpt, dev, name):
             near(got.kl.numpy(), want, kl_tolerance(x, tau, want))
             d = tx.distill_loss_backward(k.up(t)[0], up(hpt, index), got.terms, temperature=tau, grad=float(rows))
             near(k.down(d), grad * tau, gradient_tolerance(k, x, t, tau, grad, np.full(rows, tau), lse_tolerance((x - x.max(-1, keepdims=True)) / tau)))
+
+
+def test_more_than_2_26_rows(hpt, dev):
+    """One row of logits and its entries, so often that a workgroup of 1024 threads for each 16 rows would be more work items than a launch has."""
+    rows = (1 << 26) + 21
+    base = Kind(hpt, "f32").up(np.array([0.25, -1.5, 0.75]))[0]
+    v = hpt.Tensor.from_raw(base.ptr, [rows, 3], hpt.f32, 0, [0, 1])
+    teacher, index = hpt.Tensor.empty([rows, 1], hpt.f32), hpt.Tensor.empty([rows, 1], hpt.i32)
+    for t, a in ((teacher, np.ones(rows, np.float32)), (index, (np.arange(rows) % 3).astype(np.int32))):
+        assert hpt.lib().hpt_hip_memcpy_h2d_sync(0, P(t.ptr), a.ctypes.data_as(P), a.nbytes) == 0
+    got = v.distill_loss(teacher, index)
+    want = (logsumexp(np.array([[0.25, -1.5, 0.75]])) - np.array([0.25, -1.5, 0.75])).astype(np.float32)
+    kl = got.kl.numpy()
+    assert np.abs(kl.reshape(-1)[:rows // 3 * 3].reshape(-1, 3) - want).max() < 16 * F32_STEP
+    assert np.abs(kl[-3:] - want[np.arange(rows - 3, rows) % 3]).max() < 16 * F32_STEP
+    near(got.loss.numpy()[0], want.astype(np.float64).mean(), 16 * F32_STEP)
