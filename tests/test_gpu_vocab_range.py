@@ -219,10 +219,10 @@ def diverged(x, t, index, tau, teacher_lse=None):
     return kl, grad
 
 
-def kl_tolerance(x, tau, kl):
+def kl_tolerance(x, tau, kl, rest=True):
     """The student's log of the sum, as above (a rescaled sum in 64 bits), and the result's own rounding; of the rest the sum over the unnamed counts too, at most as much."""
     z = (x - x.max(-1, keepdims=True)) / tau
-    return 2 * (lse_tolerance(z) - F32_STEP * np.abs(logsumexp(z))) + F32_STEP * np.abs(kl) + 1e-12
+    return (1 + rest) * (lse_tolerance(z) - F32_STEP * np.abs(logsumexp(z))) + F32_STEP * np.abs(kl) + 1e-12
 
 
 def gradient_tolerance(k, x, t, tau, grad, w, lse_part):
@@ -297,6 +297,42 @@ def test_teachers_that_lie_anywhere(hpt, dev, name):
             near(got.kl.numpy(), want, kl_tolerance(x, tau, want))
             d = tx.distill_loss_backward(k.up(t)[0], up(hpt, index), got.terms, temperature=tau, grad=float(rows))
             near(k.down(d), grad * tau, gradient_tolerance(k, x, t, tau, grad, np.full(rows, tau), lse_tolerance((x - x.max(-1, keepdims=True)) / tau)))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("cols", [300, 5000, 50257])
+def test_sums_of_equal_terms(hpt, dev, name, rest, cols):
+    """One largest logit and all others at one distance below it: as many equal terms, whose sum would be off by a rounding for each were they added in f32 one after the other. Without the largest, terms of 1, which
+    are not off at all."""
+    k = Kind(hpt, name)
+    rows = 400
+    x = np.repeat(-np.linspace(0.003, 1.7, rows)[:, None], cols, 1)
+    x[:, cols // 3] = 0
+    tx, x = k.up(x)
+    index = np.broadcast_to(np.array([[cols // 3, 1]]), (rows, 2))
+    tt = np.broadcast_to(k.round(np.array([[0.5, 0.25]])), (rows, 2))
+    lse_t = np.full(rows, 1.7, np.float32)
+    got = tx.distill_loss(k.up(tt)[0], up(hpt, index), **(dict(teacher_lse=up(hpt, lse_t)) if rest else {}))
+    want, _ = diverged(x, tt, index, 1.0, lse_t.astype(np.float64) if rest else None)
+    near(got.kl.numpy(), want, kl_tolerance(x, 1.0, want, rest))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("rows,cols", [(2100, 1 << 20), (2100, 50257), (300, 50257), (1, 300000), (2100, 300)])
+def test_rising_rows(hpt, dev, name, rest, rows, cols):
+    """Every vector of a thread has a new largest logit: the sum is rescaled each time. One row again and again."""
+    k, rng = Kind(hpt, name), np.random.default_rng(4)
+    for span in (4.0, 30.0):
+        t, x = k.up(np.linspace(-span, 0, cols)[None])
+        v = hpt.Tensor.from_raw(t.ptr, [rows, cols], k.dtype, 0, [0, 1])
+        index = np.broadcast_to(np.array([[1, cols // 2, cols - 2]]), (rows, 3))
+        tt = np.broadcast_to(k.round(rng.standard_normal((1, 3))), (rows, 3))
+        lse_t = np.full(rows, logsumexp(tt[:1])[0] + 0.7, np.float32)
+        got = v.distill_loss(k.up(tt)[0], up(hpt, index), **(dict(teacher_lse=up(hpt, lse_t)) if rest else {}))
+        want, _ = diverged(x, tt[:1], index[:1], 1.0, lse_t[:1].astype(np.float64) if rest else None)
+        near(got.kl.numpy(), np.broadcast_to(want, rows), kl_tolerance(x, 1.0, want)[0], f"span {span}")
 
 
 def test_more_than_2_26_rows(hpt, dev):
