@@ -35,11 +35,14 @@ __device__ __forceinline__ float logit_of(const void* t, int dtype, int64_t at) 
     return dtype == HPT_F16 ? Elem<f16_t>::widen(((const f16_t*)t)[at]) : Elem<bf16_t>::widen(((const bf16_t*)t)[at]);
 }
 
-// (largest logit, sum of exponentials below it) of two lanes or wavefronts; `steps` = log2 e / temperature.
-__device__ __forceinline__ void meet(float& m, double& s, float m2, double s2, float steps) {
+// The exponential of a distance over the temperature.
+__device__ __forceinline__ float exp_of(float d, const Steps& steps) { return __builtin_amdgcn_exp2f(fmaf(d, steps.hi, d * steps.lo)); }
+
+// (largest logit, sum of exponentials below it) of two lanes or wavefronts.
+__device__ __forceinline__ void meet(float& m, double& s, float m2, double s2, const Steps& steps) {
     const float n = fmaxf(m, m2);
     // (nothing seen is (-inf, 0); equal infinities are no distance apart; a NaN is in its sum)
-    s = s * (double)(m == n ? 1.0f : __builtin_amdgcn_exp2f((m - n) * steps)) + s2 * (double)(m2 == n ? 1.0f : __builtin_amdgcn_exp2f((m2 - n) * steps));
+    s = s * (double)(m == n ? 1.0f : exp_of(m - n, steps)) + s2 * (double)(m2 == n ? 1.0f : exp_of(m2 - n, steps));
     m = n;
 }
 
@@ -109,7 +112,6 @@ __global__ __launch_bounds__(kThreads, kStatsWaves<T>) void distill_stats_kernel
     __shared__ float most[4];
     __shared__ double sums[4];
     __shared__ int again;  // a token is named twice
-    const float steps = a.steps.hi + a.steps.lo;
     for (int64_t at = blockIdx.x; at < a.rows * a.split; at += gridDim.x) {
         const int64_t row = quotient(at, a.split);
         const int part = (int)(at - row * a.split);
@@ -127,13 +129,9 @@ __global__ __launch_bounds__(kThreads, kStatsWaves<T>) void distill_stats_kernel
             for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
             top = fmaxf(m, top);
             const float from = top == -inf ? 0.0f : top;
-            float add = 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float d = v[i] - from;
-                add += __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo));
-            }
-            s = s * (double)__builtin_amdgcn_exp2f((m - from) * steps) + (double)add;
+            for (int i = 0; i < N; ++i) v[i] = exp_of(v[i] - from, a.steps);
+            s = s * (double)exp_of(m - from, a.steps) + (double)sum_by_twos(v);
             m = top;
         };
         for (int b0 = e0; b0 < e1; b0 += REST ? kBlock : e1 - e0) {
@@ -201,7 +199,7 @@ __global__ __launch_bounds__(kThreads, kStatsWaves<T>) void distill_stats_kernel
             }
         }
 #pragma unroll
-        for (int w = 1; w < 64; w <<= 1) meet(m, s, __shfl_xor(m, w, 64), shfl_xor_any(s, w), steps);
+        for (int w = 1; w < 64; w <<= 1) meet(m, s, __shfl_xor(m, w, 64), shfl_xor_any(s, w), a.steps);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) {
             most[threadIdx.x >> 6] = m;
@@ -211,7 +209,7 @@ __global__ __launch_bounds__(kThreads, kStatsWaves<T>) void distill_stats_kernel
         if (threadIdx.x == 0) {
             m = most[0];
             s = sums[0];
-            for (int w = 1; w < 4; ++w) meet(m, s, most[w], sums[w], steps);
+            for (int w = 1; w < 4; ++w) meet(m, s, most[w], sums[w], a.steps);
             double* p = a.partial + at * kDistillPart;
             p[0] = m;
             p[1] = s;
@@ -400,7 +398,6 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
             if (lane < n - tail) last = x[tail + lane];
         }
         const float rest_most = terms[2], coef = w * terms[3];
-        auto below = [&](float d) { return __builtin_amdgcn_exp2f(fmaf(d, a.steps.hi, d * a.steps.lo)); };
         // a token's bit stands so that those of a vector stand together
         const int shift = VEC - head;
         if (on) {
@@ -437,13 +434,13 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(const DistillGra
                     for (int l = j + 1; l < a.k && is_first; ++l)
                         if (token(l) == e) q += prob(l);
                 }
-                const float y = terms[1] * below(f - terms[0]);
+                const float y = terms[1] * exp_of(f - terms[0], a.steps);
                 if (is_first) out[e - e0] = Elem<T>::narrow(w * (y - q));
             }
         }
         auto grad = [&](T v) {
             const float f = Elem<T>::widen(v);
-            return Elem<T>::narrow(coef * below(f - rest_most));
+            return Elem<T>::narrow(coef * exp_of(f - rest_most, a.steps));
         };
         auto is_named = [&](int e) { return on && bits[(e + shift) >> 5] >> ((e + shift) & 31) & 1; };
         if (lane < head && !is_named(lane)) out[lane] = on ? grad(first) : first;
