@@ -147,6 +147,35 @@ def test_tied_rows_that_decide_clearly(hpt, dev, name, settings):
         near(logp.numpy(), np.broadcast_to(logs, (rep, 8)), F32_STEP * np.abs(logs) + 1e-11)
 
 
+# ---- top-k and sampling: logits anywhere -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("reps,cols,k", [(1, 5000, 50), (1, 50257, 600), (20, 5000, 64), (60, 20001, 33), (260, 9000, 20), (260, 9000, 300)])
+def test_first_places_anywhere(hpt, dev, name, reps, cols, k):
+    """A number added to all logits: the first places of either sign, on both sides of zero, and far from it. Five rows again and again."""
+    kind, rng = Kind(hpt, name), np.random.default_rng(cols + k)
+    base = rng.standard_normal((5, cols)) * np.array([[0.5], [1], [2], [4], [8]])
+    u = rng.uniform(size=5).astype(np.float32)
+    for offset in (-4.0, -8.0, -30.0, 100.0, -100.0, 6e4, -1e9, 1e20, -1e34):
+        if abs(offset) > 6e4 and name == "f16":
+            continue
+        t, x = kind.up(base * max(1.0, abs(offset) / 2e4) + offset)
+        v = hpt.Tensor.from_raw(t.ptr, [reps, 5, cols], kind.dtype, 0, [0, cols, 1])
+        want = order(x)[:, :k]
+        values, index = v.topk(k)
+        assert np.array_equal(index.numpy(), np.broadcast_to(want, (reps, 5, k))), offset
+        assert np.array_equal(kind.load(values.numpy()), np.broadcast_to(np.take_along_axis(x, want, -1), (reps, 5, k)))
+        for settings in (dict(top_k=k), dict(top_k=k, top_p=0.7), dict(top_p=0.9), dict(min_p=0.02), dict()):
+            settings["temperature"] = max(1.0, abs(offset) / 2e4)
+            chosen = [sampled(x[r], u[r], **settings) for r in range(5)]
+            clear = np.array([c[2] > 2.0 ** -36 for c in chosen])
+            token, logp = v.sample(up(hpt, np.tile(u, reps)), **settings)
+            tokens, logs = np.array([c[0] for c in chosen]), np.array([c[1] for c in chosen])
+            assert np.array_equal(token.numpy()[:, clear], np.broadcast_to(tokens, (reps, 5))[:, clear]), (offset, settings)
+            near(logp.numpy()[:, clear], np.broadcast_to(logs, (reps, 5))[:, clear], (F32_STEP * np.abs(logs) + 1e-11)[clear], f"{offset} {settings}")
+
+
 # ---- top-k: the log of the sum -----------------------------------------------------------------------------
 
 
