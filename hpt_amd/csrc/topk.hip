@@ -4,7 +4,7 @@
 // adds the exponentials of its 2048 below their largest). The second has a workgroup for each row, which finds the first k places from those keys (top_rows.hpp).
 // The second is bound by the latency of its steps.
 //
-// The first reads bf16 [4096, 50257] in 71 to 73 us (5.7 TB/s) without the sum; with it the launch is bound by its instructions, five for each logit: 88 to 92 us (4.6 TB/s). The second takes 32 to 35
+// The first reads bf16 [4096, 50257] in 71 to 73 us (5.7 TB/s) without the sum; with it the launch is bound by its instructions, six for each logit: 94 to 102 us (4.2 TB/s; f32 148 to 153, 5.5 TB/s). The second takes 32 to 36
 // of k = 64 there (by wavefronts), 9 of one row of 152000 and of 37 of 50257, 19 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
 #include <algorithm>
 #include <cmath>
@@ -185,7 +185,8 @@ __global__ __launch_bounds__(kTileGroups, 5) void topk_wave_kernel(const TopkArg
 constexpr int kMostEach = 4;  // rows of a wavefront
 // Rows of at most 64 N elements, a wavefront each, one launch: the row stays in registers (element i of lane l is at 64 i + l), and the largest is taken out k times.
 template <class T, int N, bool LSE>
-__global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a, int each) {
+__global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a, int rows_each) {
+    const int each = LSE ? rows_each : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __shared__ RowSum sums[LSE ? 4 * kMostEach : 1];
     for (int64_t row0 = (int64_t)blockIdx.x * 4 * each; row0 < a.rows; row0 += (int64_t)gridDim.x * 4 * each) {
