@@ -255,7 +255,7 @@ void launch_sample(int dtype, const SampleArgs& a, hipStream_t st);
 
 // ---- distillation -----------------------------------------------------------------------------------
 
-constexpr int kTerms = 8;  // numbers that a row keeps for its gradient
+constexpr int kTerms = 8;  // numbers that a row keeps for its gradient (distill_loss.hip's finish_row says which)
 
 struct DistillArgs {
     const void* x;            // rows of `cols` neighbouring logits

@@ -5,10 +5,11 @@
 // teacher_lse) where the teacher's own log of the sum is given, in which case all other tokens count as one with r = max(0, 1 - sum q) against the student's s = 1 - sum p:
 //   kl = sum q (log q - log p) + r (log r - log s),   loss = temperature^2 * the mean of kl over the rows, with the mask as weights.
 // By x / temperature, a token's derivative is mass p - q (mass = sum q + r; q summed over entries that name it), and that of one which no entry names (mass - r / s) p.
+// All of it from distances below the largest logit and the largest entry, so rows may lie anywhere.
 //
 // Bound by memory, as the policy loss is: one read forward, one read and one write backward. The entries (some hundred a row) come through LDS: as a bit for each token
 // forward, where s is summed without the named tokens (1 - sum p would lose what is small), as a number for each token of a piece backward.
-// bf16 [8192, 50257], k = 64, with the rest: 142 us forward (5.8 TB/s), 22 of the launch that joins the rows' parts with their entries, 4 of the mean over the rows, 285 backward (5.8 TB/s).
+// bf16 [8192, 50257], k = 64, with the rest: 142 us forward (5.8 TB/s), 22 of the launch that joins the rows' parts with their entries, 4 of the mean over the rows, 289 backward (5.7 TB/s).
 #include <algorithm>
 
 #include "vocab_rows.hpp"

@@ -4,17 +4,17 @@
 // order: the first top_k; of these the fewest whose weights reach top_p of theirs together; of these the ones with w >= min_p. So what is kept is
 // a place of the order (key and index), and the token is the first, by index, at which the kept weights' sum is above u of their whole.
 //
-// Which token that is hangs on sums over the row: an error of 1e-7 of the sum, f32's, moves one of 10^5 borders across u in a row out of fifty. Weights and sums have 52
-// bits here: with t = x log2 e 128 / temperature and n the whole number next to it, w is 2^(n / 128), from a table of 128, times a polynomial in t - n (degree 3, 3e-13). f64
-// multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s; it is bound by its instructions, 16 for each logit.
+// Which token that is hangs on sums over the row: an error of 1e-7 of the sum, f32's, moves one of 10^5 borders across u in a row out of fifty. Weights and sums are of 64
+// bits here: with t = x log2 e 128 / temperature and n the whole number next to it, w is 2^(n / 128), from a table of 128, times a polynomial in t - n (degree 3, 3e-13), and whole
+// numbers of a bucket are of 2^-44 or 2^-40 of an octave: what is decided is the definition's wherever no border lies within 2^-36 of the row's sum of it. f64 multiply-adds run at the rate of f32 ones, so the first launch still reads at some TB/s; it is bound by its instructions, 16 for each logit.
 //
 // Two launches. The first takes tiles of 8192 logits and leaves, by what the row's filters need: the largest keys of its groups (top_k of at most 1024: only the first places
 // matter); the sum of the weights (no filter); or the weights' sums by size, in buckets of an eighth of a power of two, as integers, whose sum has no order (with their
 // numbers where top_k is larger). The second has a workgroup for each row: it finds the bucket in which a border lies, collects that bucket's logits, narrows the border to one
 // place, and then looks through the one tile in which u's token lies. (Very many rows of which at most 64 places matter take a wavefront each.)
 //
-// us of the two launches, bf16 [2048, 50257] (206 MB): without a filter 85 + 14 (2.4 TB/s in the first), top_k 50 39 + 24 (5.3), 600 39 + 50, top_p 0.9 133 + 95 (1.5: two LDS additions' worth of
-// instructions more). bf16 [1, 152000] with top_k 20 and top_p 0.8 2.5 + 10.5, f32 [33, 50257] with top_p 0.95 8 + 29, [64, 152000] with settings for each row 14 + 44: the steps of one workgroup, most of
+// us of the two launches, bf16 [2048, 50257] (206 MB): without a filter 85 + 14 (2.4 TB/s in the first), top_k 50 39 + 24 (5.3), 600 39 + 99, top_p 0.9 137 + 108 (1.5: two LDS additions' worth of
+// instructions more). bf16 [1, 152000] with top_k 20 and top_p 0.8 2.5 + 10.5, f32 [33, 50257] with top_p 0.95 8 + 27, [64, 152000] with settings for each row 14 + 43: the steps of one workgroup, most of
 // them the collection of a bucket, at a compute unit's own rate.
 #include <algorithm>
 

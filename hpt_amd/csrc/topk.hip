@@ -5,7 +5,7 @@
 // The second is bound by the latency of its steps.
 //
 // The first reads bf16 [4096, 50257] in 71 to 73 us (5.7 TB/s) without the sum; with it the launch is bound by its instructions, six for each logit: 94 to 102 us (4.2 TB/s; f32 148 to 153, 5.5 TB/s). The second takes 32 to 36
-// of k = 64 there (by wavefronts), 9 of one row of 152000 and of 37 of 50257, 19 of f16 [256, 152000] with k = 512. Small rows have a launch of their own.
+// of k = 64 there (by wavefronts), 9 of one row of 152000 and of 37 of 50257, 19 of f16 [256, 152000] with k = 512, where the first places lie in an octave or two (top_rows.hpp has the others). Small rows have a launch of their own.
 #include <algorithm>
 #include <cmath>
 
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void topk_small_kernel(const TopkArgs a, int r
 }  // namespace
 
 // Which rows topk_small_kernel takes (us, f32, against the two launches). Few rows, where a wavefront's steps stand one behind the other: [1, 2000] of k 8 10.0 / 10.4, of 20 18.6 / 11.1, [1, 256] of 64 12.9 / 14.2.
-// Many: [500, 2000] of 20 19.9 / 20.2, of 64 52 / 70; a router's [16384, 64] of 8 7.2 / 132, [16384, 1000] of 64 161 / 717.
+// Many: [500, 2000] of 20 19.9 / 20.2, of 64 52 / 70; a router's [16384, 64] of 8 7.8 / 132, [16384, 1000] of 64 161 / 717.
 bool topk_in_registers(int64_t rows, int64_t cols, int64_t k) { return cols <= 64 * 32 && k <= 64 && (rows > 256 || k * ((cols + 63) / 64) <= 256); }
 
 void launch_topk(int dtype, const TopkArgs& a, hipStream_t st) {

@@ -371,7 +371,7 @@ int32_t hpt_hip_policy_loss_backward(int32_t dev, void* stream, const hpt_view* 
 
 /* The k largest elements of each row of `in` [..., cols], 1 <= k <= 1024 (and cols), in order: a NaN before everything, then the larger value, equal
  * values (and -0 and +0) by their index. `values` [..., k] of in's dtype, `index` [..., k] i32 or i64. `lse` (may be NULL; f32, one for each
- * row): log sum exp(in / temperature), NaN where the row has one, otherwise +inf where it has one. The workspace is enough for calls with lse and without; rows of at
+ * row): log sum exp(in / temperature), off by some 1e-7 to 1e-6 of the sum whatever its own size, and by its rounding, NaN where the row has one, otherwise +inf where it has one. The workspace is enough for calls with lse and without; rows of at
  * most 2048 elements of which at most 64 are wanted need none where they are more than 256, or where k * ceil(cols / 64) is at most 256. */
 int32_t hpt_hip_topk(int32_t dev, void* stream, const hpt_view* in, int64_t k, double temperature, const hpt_view* workspace,
                      hpt_view* values, hpt_view* index, hpt_view* lse);
@@ -381,7 +381,8 @@ int32_t hpt_hip_topk_workspace(const hpt_view* in, int64_t k, size_t* bytes);
  * the nearer end, a NaN as 0). With weights w = exp((logit - largest) / temperature), what is kept of the row are the `top_k` first of the order of hpt_hip_topk (k <= 0: all),
  * of these the fewest first ones whose weights reach top_p of theirs together (top_p >= 1: all; the first in any case), and of these the ones with w >= min_p
  * (<= 0: all; above 1 counts as 1). `token` (i32 or i64) is the first, by index, at which the sum of the kept weights exceeds u times the sum of all
- * kept ones, and `logp` (f32) the logarithm of its weight over that sum. Sums and weights have 64 bits. A temperature of 0 takes the first of the
+ * kept ones, and `logp` (f32) the logarithm of its weight over that sum. Sums and weights are held in 64 bits and good to 2^-38 of the row's sum, so
+ * the token is that of real numbers wherever no border (of top_p, of min_p, between two tokens) lies within 2^-36 of what decides. The same call gives the same bits. A temperature of 0 takes the first of the
  * order. Settings are for all rows, or for each (a view that is not NULL: temperatures, top_ps and min_ps f32, top_ks i32 or i64; the number beside it
  * is then not looked at). A row without a distribution (largest logit NaN or infinite, a temperature that is neither 0 nor 1e-30 ... 1e30, another setting that
  * is NaN; as a number for all rows such settings are refused) has token -1 and logp NaN. */
@@ -395,8 +396,8 @@ int32_t hpt_hip_sample_workspace(const hpt_view* logits, size_t* bytes);
  * temperature) over the row's entries, kl = sum q (log q - log p). With `teacher_lse` (f32, one for each row, of all of the teacher's logits over the
  * temperature: hpt_hip_topk's) q = exp(teacher / temperature - teacher_lse), and all tokens without an entry count as one: kl gets r (log r -
  * log s) with r = max(0, 1 - sum q) and s what p gives them (r is 0 where nothing is left to s). `loss` (one element) is temperature^2 times the mean of `kl` (one for each row) with `mask` (f32 weights
- * or bool; NULL: all ones) as weights, 0 where the mask sums to 0. Rows whose mask is 0 are not read, and their kl is 0, as is that of a row whose entries
- * are missing or -inf altogether. An entry outside the vocabulary makes the row's kl NaN; entries that name one token twice both count. `terms`: 8 numbers for each row, for the gradient. All f32. */
+ * or bool; NULL: all ones) as weights, 0 where the mask sums to 0. Rows whose mask is 0 are not read, and their kl is 0, as is, without teacher_lse, that of a row whose
+ * entries are missing or -inf altogether. What is added to all logits of a row, or without teacher_lse to all of its entries, changes nothing. An entry outside the vocabulary makes the row's kl NaN; entries that name one token twice both count. `terms`: 8 numbers for each row, for the gradient. All f32. */
 int32_t hpt_hip_distill_loss(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* teacher, const hpt_view* index,
                              const hpt_view* teacher_lse, const hpt_view* mask, double temperature, const hpt_view* workspace,
                              hpt_view* loss, hpt_view* kl, hpt_view* terms);
