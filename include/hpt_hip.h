@@ -395,7 +395,7 @@ int32_t hpt_hip_sample_workspace(const hpt_view* logits, size_t* bytes);
  * student's are) at the tokens `index` [..., k] (i32 or i64; negative: no entry). With p = softmax(logits / temperature) and q = softmax(teacher /
  * temperature) over the row's entries, kl = sum q (log q - log p). With `teacher_lse` (f32, one for each row, of all of the teacher's logits over the
  * temperature: hpt_hip_topk's) q = exp(teacher / temperature - teacher_lse), and all tokens without an entry count as one: kl gets r (log r -
- * log s) with r = max(0, 1 - sum q) and s what p gives them (r is 0 where nothing is left to s). `loss` (one element) is temperature^2 times the mean of `kl` (one for each row) with `mask` (f32 weights
+ * log s) with r = max(0, 1 - sum q) and s what p gives them (r is 0 where nothing is left to s: no other token, or -inf alone; a finite mask is a logit). `loss` (one element) is temperature^2 times the mean of `kl` (one for each row) with `mask` (f32 weights
  * or bool; NULL: all ones) as weights, 0 where the mask sums to 0. Rows whose mask is 0 are not read, and their kl is 0, as is, without teacher_lse, that of a row whose
  * entries are missing or -inf altogether. What is added to all logits of a row, or without teacher_lse to all of its entries, changes nothing. An entry outside the vocabulary makes the row's kl NaN; entries that name one token twice both count. `terms`: 8 numbers for each row, for the gradient. All f32. */
 int32_t hpt_hip_distill_loss(int32_t dev, void* stream, const hpt_view* logits, const hpt_view* teacher, const hpt_view* index,
